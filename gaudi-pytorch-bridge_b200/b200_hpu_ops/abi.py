@@ -22,6 +22,7 @@ EXPORTS = [
     "b200q_amax", "b200q_scale_from_amax", "b200q_amax_history_update",
     "b200q_softmax_fp8", "b200q_sum_fp8_workspace_bytes", "b200q_sum_fp8", "b200q_in_place_interleave", "b200q_im2col_fp8",
     "b200q_nchw_to_nhwc_u8", "b200q_im2col_nhwc_fp8",
+    "b200q_paged_plan", "b200q_qk_norm_rope_append", "b200q_paged_attention_workspace_bytes", "b200q_paged_attention",
 ]
 
 DTYPE = {torch.float32: F32, torch.bfloat16: BF16, torch.float8_e4m3fn: E4M3, torch.float8_e5m2: E5M2}
@@ -63,6 +64,38 @@ class SdpaArgs(C.Structure):
         ("m_out", C.c_void_p), ("linv_out", C.c_void_p), ("amax_s", C.c_void_p), ("amax_o", C.c_void_p),
         ("force_plain", C.c_int), ("stream", C.c_void_p),
         ("zero_ptr", C.c_void_p * 5), ("zero_bytes", C.c_int * 5),
+    ]
+
+
+class AppendArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("src_dtype", C.c_int), ("tokens", C.c_int64),
+        ("heads", C.c_int), ("kv_heads", C.c_int), ("dim", C.c_int),
+        ("q_token_stride", C.c_int64), ("q_head_stride", C.c_int64), ("k_token_stride", C.c_int64), ("k_head_stride", C.c_int64),
+        ("v_token_stride", C.c_int64), ("v_head_stride", C.c_int64),
+        ("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("weight_dtype", C.c_int), ("eps", C.c_float),
+        ("cos_sin", C.c_void_p), ("max_positions", C.c_int64), ("rotary_dim", C.c_int), ("interleaved", C.c_int),
+        ("positions", C.c_void_p), ("slot_map", C.c_void_p),
+        ("k_cache", C.c_void_p), ("v_cache", C.c_void_p), ("cache_dtype", C.c_int), ("num_pages", C.c_int64), ("page_size", C.c_int64),
+        ("k_page_stride", C.c_int64), ("k_slot_stride", C.c_int64), ("k_cache_head_stride", C.c_int64),
+        ("v_page_stride", C.c_int64), ("v_slot_stride", C.c_int64), ("v_cache_head_stride", C.c_int64),
+        ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("q_scale", C.c_void_p),
+        ("q_out", C.c_void_p), ("q_out_dtype", C.c_int), ("stream", C.c_void_p),
+    ]
+
+
+class PagedAttentionArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("q_token_stride", C.c_int64), ("q_head_stride", C.c_int64), ("requests", C.c_int64),
+        ("heads", C.c_int), ("kv_heads", C.c_int), ("dim", C.c_int),
+        ("k_cache", C.c_void_p), ("v_cache", C.c_void_p), ("cache_dtype", C.c_int), ("num_pages", C.c_int64), ("page_size", C.c_int64),
+        ("k_page_stride", C.c_int64), ("k_slot_stride", C.c_int64), ("k_head_stride", C.c_int64),
+        ("v_page_stride", C.c_int64), ("v_slot_stride", C.c_int64), ("v_head_stride", C.c_int64),
+        ("block_table", C.c_void_p), ("table_width", C.c_int64), ("table_stride", C.c_int64), ("kv_lens", C.c_void_p),
+        ("window", C.c_int64), ("softmax_scale", C.c_float),
+        ("k_scale_inv", C.c_void_p), ("v_scale_inv", C.c_void_p), ("out_scale", C.c_void_p),
+        ("out", C.c_void_p), ("out_dtype", C.c_int), ("lse", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("force_plain", C.c_int), ("stream", C.c_void_p),
     ]
 
 
@@ -113,6 +146,12 @@ def _bind():
     lib.b200q_w4a16_workspace_bytes.argtypes = [C.c_int64, C.c_int64, C.c_int64]
     lib.b200q_swiglu_cast_fp8.argtypes = [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_float,
                                           C.c_int64, C.c_int64, C.c_void_p, C.c_void_p]
+    lib.b200q_paged_plan.argtypes = [C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p,
+                                     C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]
+    lib.b200q_qk_norm_rope_append.argtypes = [C.POINTER(AppendArgs)]
+    lib.b200q_paged_attention_workspace_bytes.restype = C.c_size_t
+    lib.b200q_paged_attention_workspace_bytes.argtypes = [C.c_int64, C.c_int, C.c_int, C.c_int, C.c_int]
+    lib.b200q_paged_attention.argtypes = [C.POINTER(PagedAttentionArgs)]
     return lib
 
 

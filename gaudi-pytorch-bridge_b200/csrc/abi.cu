@@ -5,6 +5,7 @@
 #include "common.cuh"
 #include "fp8_misc.cuh"
 #include "gemm_common.cuh"
+#include "paged.cuh"
 #include "tcgen05_ptx.cuh"
 
 namespace b200q {
@@ -115,6 +116,11 @@ int gptq_repack_impl(const int32_t*, int32_t*, int64_t, int64_t, const int32_t*,
 int w4a16_gemm_noalloc_impl(const void*, int64_t, const int32_t*, const void*, const int32_t*, int, int, int64_t, int64_t,
                             int64_t, int64_t, void*, int, int64_t, cudaStream_t);
 
+int paged_plan_impl(const PagedPlanParams&, cudaStream_t);
+int qk_norm_rope_append_impl(const b200q_append_args&, cudaStream_t);
+int paged_attention_impl(const b200q_paged_attention_args&, cudaStream_t);
+size_t paged_attention_workspace_bytes_impl(int64_t, int, int, int, int);
+
 static bool is_fp8(int d) { return d == B200Q_E4M3 || d == B200Q_E5M2; }
 static bool is_wide(int d) { return d == B200Q_F32 || d == B200Q_BF16; }
 static bool scale_args_ok(const float* dev, int mode) {
@@ -146,7 +152,13 @@ const char* b200q_last_cuda_error(void) { return t_cuda_error; }
 uint64_t b200q_launch_count(void) { return g_launches.load(std::memory_order_relaxed); }
 
 size_t b200q_sizeof_args(int which) {
-  return which == 0 ? sizeof(b200q_gemm_args) : which == 1 ? sizeof(b200q_sdpa_args) : 0;
+  switch (which) {
+    case 0: return sizeof(b200q_gemm_args);
+    case 1: return sizeof(b200q_sdpa_args);
+    case 2: return sizeof(b200q_append_args);
+    case 3: return sizeof(b200q_paged_attention_args);
+    default: return 0;
+  }
 }
 
 int b200q_device_status(int* code_out) {
@@ -416,6 +428,82 @@ int b200q_fp8_sdpa_fwd(const b200q_sdpa_args* a) {
   if (a->out_dtype != B200Q_BF16 && a->out_dtype != B200Q_E4M3) return B200Q_ERR_BAD_ARGUMENT;
   if (a->mask && (a->mask_kind < 1 || a->mask_kind > 3)) return B200Q_ERR_BAD_ARGUMENT;
   return sdpa_fp8_fwd_impl(*a, static_cast<cudaStream_t>(a->stream));
+}
+
+int b200q_paged_plan(const int32_t* context_lens, const int32_t* new_lens, int64_t requests, int32_t* block_table,
+                     int64_t table_width, int64_t table_stride, const int32_t* free_pages, int64_t free_count,
+                     const int32_t* free_head, int64_t page_size, int64_t num_tokens, int64_t* slot_map, int64_t* positions,
+                     int32_t* query_start, int32_t* kv_lens, int32_t* free_head_out, void* stream) {
+  if (requests < 0 || table_width < 0 || table_stride < table_width || free_count < 0 || page_size < 1 || num_tokens < 0)
+    return B200Q_ERR_BAD_ARGUMENT;
+  if (requests > kPagedMaxRequests || table_width > INT32_MAX || requests * table_width > INT32_MAX || num_tokens > INT32_MAX ||
+      page_size > INT32_MAX)
+    return B200Q_ERR_TOO_LARGE;
+  if (!query_start || !free_head_out || (num_tokens > 0 && (!slot_map || !positions))) return B200Q_ERR_BAD_ARGUMENT;
+  if (requests > 0 && (!context_lens || !new_lens || !kv_lens || (table_width > 0 && !block_table))) return B200Q_ERR_BAD_ARGUMENT;
+  if (free_count > 0 && !free_pages) return B200Q_ERR_BAD_ARGUMENT;
+  PagedPlanParams p;
+  p.context_lens = context_lens; p.new_lens = new_lens; p.requests = (int)requests;
+  p.table = block_table; p.table_width = (int)table_width; p.table_stride = table_stride;
+  p.free_pages = free_pages; p.free_count = free_count; p.free_head = free_head;
+  p.page_size = (int)page_size; p.num_tokens = (int)num_tokens;
+  p.slot_map = slot_map; p.positions = positions; p.query_start = query_start; p.kv_lens = kv_lens; p.free_head_out = free_head_out;
+  return paged_plan_impl(p, static_cast<cudaStream_t>(stream));
+}
+
+// whether the address is a multiple of n elements of the type
+static bool on_elements(const void* p, int dtype, int n) {
+  const int size = dtype == B200Q_F32 ? 4 : dtype == B200Q_BF16 ? 2 : 1;
+  return reinterpret_cast<uintptr_t>(p) % (size_t)(size * n) == 0;
+}
+
+int b200q_qk_norm_rope_append(const b200q_append_args* a) {
+  if (!a) return B200Q_ERR_BAD_ARGUMENT;
+  if (a->tokens < 0 || a->heads < 0 || a->kv_heads < 0 || a->dim < 0 || a->num_pages < 0 || a->page_size < 1) return B200Q_ERR_BAD_ARGUMENT;
+  if (!is_wide(a->src_dtype) || !(a->q_out_dtype == B200Q_BF16 || is_fp8(a->q_out_dtype)) ||
+      !(a->cache_dtype == B200Q_BF16 || is_fp8(a->cache_dtype)))
+    return B200Q_ERR_BAD_ARGUMENT;
+  if ((a->q_weight || a->k_weight) && !is_wide(a->weight_dtype)) return B200Q_ERR_BAD_ARGUMENT;
+  if (a->dim < 8 || a->dim > 256 || a->dim % 8) return B200Q_ERR_UNSUPPORTED;
+  if (a->cos_sin && (a->rotary_dim < 8 || a->rotary_dim > a->dim || a->rotary_dim % 8)) return B200Q_ERR_UNSUPPORTED;
+  if (a->tokens > INT32_MAX || a->num_pages > INT32_MAX || a->page_size > INT32_MAX || a->num_pages * a->page_size > INT32_MAX)
+    return B200Q_ERR_TOO_LARGE;
+  if ((int64_t)a->heads + 2 * (int64_t)a->kv_heads > 65536) return B200Q_ERR_TOO_LARGE;
+  if (a->tokens == 0 || (a->heads == 0 && a->kv_heads == 0)) return B200Q_OK;
+  if (!a->slot_map || (a->cos_sin && (!a->positions || a->max_positions < 0))) return B200Q_ERR_BAD_ARGUMENT;
+  if (a->heads > 0 && (!a->q || !a->q_out)) return B200Q_ERR_BAD_ARGUMENT;
+  if (a->kv_heads > 0 && (!a->k || !a->v || (a->num_pages > 0 && (!a->k_cache || !a->v_cache)))) return B200Q_ERR_BAD_ARGUMENT;
+  for (const void* p : {a->q, a->k, a->v})
+    if (!on_elements(p, a->src_dtype, 4)) return B200Q_ERR_UNSUPPORTED;
+  for (const void* p : {a->q_weight, a->k_weight})
+    if (!on_elements(p, a->weight_dtype, 4)) return B200Q_ERR_UNSUPPORTED;
+  for (const void* p : {a->k_cache, a->v_cache})
+    if (!on_elements(p, a->cache_dtype, 4)) return B200Q_ERR_UNSUPPORTED;
+  if (!on_elements(a->q_out, a->q_out_dtype, 4) || !on_elements(a->cos_sin, B200Q_F32, 4)) return B200Q_ERR_UNSUPPORTED;
+  for (int64_t s : {a->q_token_stride, a->q_head_stride, a->k_token_stride, a->k_head_stride, a->v_token_stride, a->v_head_stride,
+                    a->k_page_stride, a->k_slot_stride, a->k_cache_head_stride, a->v_page_stride, a->v_slot_stride, a->v_cache_head_stride})
+    if (s % 4) return B200Q_ERR_UNSUPPORTED;
+  return qk_norm_rope_append_impl(*a, static_cast<cudaStream_t>(a->stream));
+}
+
+size_t b200q_paged_attention_workspace_bytes(int64_t requests, int heads, int kv_heads, int dim, int cache_dtype) {
+  if (requests <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || dim <= 0) return 0;
+  return paged_attention_workspace_bytes_impl(requests, heads, kv_heads, dim, cache_dtype);
+}
+
+int b200q_paged_attention(const b200q_paged_attention_args* a) {
+  if (!a) return B200Q_ERR_BAD_ARGUMENT;
+  if (a->requests < 0 || a->heads < 0 || a->kv_heads < 1 || a->heads % a->kv_heads || a->dim < 1 || a->num_pages < 0 || a->page_size < 1 ||
+      a->table_width < 0 || a->window < 0)
+    return B200Q_ERR_BAD_ARGUMENT;
+  if (!(a->cache_dtype == B200Q_BF16 || is_fp8(a->cache_dtype)) || !(is_wide(a->out_dtype) || a->out_dtype == B200Q_E4M3))
+    return B200Q_ERR_BAD_ARGUMENT;
+  if (a->dim > 256) return B200Q_ERR_UNSUPPORTED;
+  if (a->num_pages > INT32_MAX || a->page_size > INT32_MAX || a->table_width > INT32_MAX) return B200Q_ERR_TOO_LARGE;
+  if (a->requests == 0 || a->heads == 0) return B200Q_OK;
+  if (!a->q || !a->out || !a->kv_lens || (a->table_width > 0 && !a->block_table)) return B200Q_ERR_BAD_ARGUMENT;
+  if (a->num_pages > 0 && (!a->k_cache || !a->v_cache)) return B200Q_ERR_BAD_ARGUMENT;
+  return paged_attention_impl(*a, static_cast<cudaStream_t>(a->stream));
 }
 
 int b200q_tp_reduce_bcast(const void* stage, void* const* out_ptrs_host, int tp, int me, int64_t rows, int64_t d,

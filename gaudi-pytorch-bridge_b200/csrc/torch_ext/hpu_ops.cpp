@@ -1331,6 +1331,242 @@ at::Tensor cast_moment_to_fp8(const at::Tensor& moment, at::Tensor& scale, at::S
   return std::get<0>(r);
 }
 
+// ------------------------------------------------------------------ paged key/value cache
+// (no counterpart in the reference; the contract is in b200q.h)
+void paged_same_device(const at::Device& dev, std::initializer_list<const at::Tensor*> tensors, const char* op) {
+  for (const at::Tensor* t : tensors)
+    TORCH_CHECK(!t->defined() || t->device() == dev, op, ": all tensors must be on ", dev, ", got one on ", t->device());
+}
+at::Tensor paged_optional(const OptTensor& t) { return t.has_value() ? *t : at::Tensor(); }
+const float* paged_scale(const at::Tensor& t, const char* op, const char* name) {
+  if (!t.defined()) return nullptr;
+  TORCH_CHECK(t.scalar_type() == at::kFloat && t.numel() == 1, op, ": ", name, " must be a float tensor of one element");
+  return t.const_data_ptr<float>();
+}
+// [n0, n1, values]: values contiguous, and everything on boundaries of `bytes` (a view that is not is copied)
+at::Tensor paged_rows(const at::Tensor& t, int64_t bytes) {
+  const int64_t size = (int64_t)t.element_size();
+  auto off = [&](int64_t stride) { return stride * size % bytes != 0; };
+  const bool plain = (t.size(2) <= 1 || t.stride(2) == 1) && (t.size(0) <= 1 || !off(t.stride(0))) && (t.size(1) <= 1 || !off(t.stride(1))) &&
+                     reinterpret_cast<uintptr_t>(t.const_data_ptr()) % bytes == 0;
+  if (plain) return t;
+  at::Tensor c = t.contiguous();
+  return c.is_same(t) ? t.clone() : c;
+}
+// A stride that no index uses (one entry) is whatever the view says; the kernels want it aligned.
+int64_t paged_stride(const at::Tensor& t, int64_t dim) { return t.size(dim) > 1 ? t.stride(dim) : 0; }
+
+struct PagedCache {
+  int64_t pages, page_size, kv_heads, dim;
+};
+PagedCache paged_check_caches(const at::Tensor& k, const at::Tensor& v, const char* op) {
+  TORCH_CHECK(k.dim() == 4 && v.dim() == 4 && k.sizes() == v.sizes(), op,
+              ": k_cache and v_cache must both be [pages, page_size, kv_heads, dim], got ", k.sizes(), " and ", v.sizes());
+  TORCH_CHECK(k.scalar_type() == v.scalar_type() && (k.scalar_type() == at::kBFloat16 || is_fp8(k.scalar_type())), op,
+              ": the caches must both be bfloat16, float8_e4m3fn or float8_e5m2, got ", k.scalar_type(), " and ", v.scalar_type());
+  TORCH_CHECK(k.size(1) > 0, op, ": a page must hold at least one token");
+  for (const at::Tensor* c : {&k, &v})
+    TORCH_CHECK(c->size(3) <= 1 || c->stride(3) == 1, op, ": the values of a head must be contiguous in the caches");
+  return {k.size(0), k.size(1), k.size(2), k.size(3)};
+}
+at::Tensor paged_int32(const at::Tensor& t, int64_t dim, const char* op, const char* name) {
+  TORCH_CHECK(t.scalar_type() == at::kInt && t.dim() == dim, op, ": ", name, " must be a ", dim, "-dimensional int32 tensor");
+  return dim == 1 ? t.contiguous() : t;
+}
+int64_t paged_table_stride(const at::Tensor& table, const char* op) {
+  TORCH_CHECK(table.size(1) <= 1 || table.stride(1) == 1, op, ": the entries of a block_table row must be contiguous");
+  return table.size(0) > 1 ? table.stride(0) : table.size(1);
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> paged_plan(const at::Tensor& context_lens, const at::Tensor& new_lens,
+                                                                                  at::Tensor& block_table, const at::Tensor& free_pages,
+                                                                                  const OptTensor& free_head_opt, int64_t page_size,
+                                                                                  int64_t num_tokens) {
+  const char* op = "paged_plan";
+  const at::Device dev = block_table.device();
+  at::Tensor head = paged_optional(free_head_opt);
+  paged_same_device(dev, {&context_lens, &new_lens, &free_pages, &head}, op);
+  c10::cuda::CUDAGuard guard(dev);
+  at::Tensor ctx = paged_int32(context_lens, 1, op, "context_lens"), add = paged_int32(new_lens, 1, op, "new_lens");
+  at::Tensor pages = paged_int32(free_pages, 1, op, "free_pages");
+  paged_int32(block_table, 2, op, "block_table");
+  const int64_t n = ctx.numel();
+  TORCH_CHECK(add.numel() == n && block_table.size(0) == n, op, ": context_lens, new_lens and block_table must be of the same number of requests, got ",
+              n, ", ", add.numel(), " and ", block_table.size(0));
+  TORCH_CHECK(!head.defined() || (head.scalar_type() == at::kInt && head.numel() == 1), op, ": free_head must be an int32 tensor of one element");
+  TORCH_CHECK(page_size > 0 && num_tokens >= 0, op, ": page_size must be positive and num_tokens not negative, got ", page_size, " and ", num_tokens);
+  const int64_t stride = paged_table_stride(block_table, op);
+  TORCH_CHECK(stride >= block_table.size(1), op, ": the rows of block_table must not overlap");
+  at::Tensor slots = new_tensor({num_tokens}, at::kLong, dev), positions = new_tensor({num_tokens}, at::kLong, dev);
+  at::Tensor start = new_tensor({n + 1}, at::kInt, dev), lens = new_tensor({n}, at::kInt, dev), next = new_tensor({1}, at::kInt, dev);
+  check_status(b200q_paged_plan(ctx.const_data_ptr<int32_t>(), add.const_data_ptr<int32_t>(), n, block_table.data_ptr<int32_t>(),
+                                block_table.size(1), stride, pages.const_data_ptr<int32_t>(), pages.numel(),
+                                head.defined() ? head.const_data_ptr<int32_t>() : nullptr, page_size, num_tokens, slots.data_ptr<int64_t>(),
+                                positions.data_ptr<int64_t>(), start.data_ptr<int32_t>(), lens.data_ptr<int32_t>(), next.data_ptr<int32_t>(),
+                                current_stream()),
+               op);
+  return {slots, positions, start, lens, next};
+}
+
+at::Tensor qk_norm_rope_append(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const OptTensor& q_weight_opt,
+                               const OptTensor& k_weight_opt, double eps, const OptTensor& cos_sin_opt, const OptTensor& positions_opt,
+                               bool interleaved, const at::Tensor& slot_map, at::Tensor& k_cache, at::Tensor& v_cache,
+                               const OptTensor& k_scale_opt, const OptTensor& v_scale_opt, const OptTensor& q_scale_opt,
+                               c10::optional<at::ScalarType> q_dtype) {
+  const char* op = "qk_norm_rope_append";
+  const at::Device dev = q.device();
+  at::Tensor q_weight = paged_optional(q_weight_opt), k_weight = paged_optional(k_weight_opt), cos_sin = paged_optional(cos_sin_opt),
+             positions = paged_optional(positions_opt), k_scale = paged_optional(k_scale_opt), v_scale = paged_optional(v_scale_opt),
+             q_scale = paged_optional(q_scale_opt);
+  paged_same_device(dev, {&k, &v, &q_weight, &k_weight, &cos_sin, &positions, &slot_map, &k_cache, &v_cache, &k_scale, &v_scale, &q_scale}, op);
+  c10::cuda::CUDAGuard guard(dev);
+  const auto src = q.scalar_type();
+  TORCH_CHECK(src == at::kFloat || src == at::kBFloat16, op, ": q must be float or bfloat16, got ", src);
+  TORCH_CHECK(k.scalar_type() == src && v.scalar_type() == src, op, ": q, k and v must have the same dtype");
+  TORCH_CHECK(q.dim() == 3 && k.dim() == 3 && v.dim() == 3 && k.sizes() == v.sizes() && k.size(0) == q.size(0) && k.size(2) == q.size(2), op,
+              ": q must be [tokens, heads, dim] and k and v [tokens, kv_heads, dim], got ", q.sizes(), ", ", k.sizes(), " and ", v.sizes());
+  const int64_t tokens = q.size(0), dim = q.size(2);
+  TORCH_CHECK(dim >= 8 && dim <= 256 && dim % 8 == 0, op, ": the head dimension must be a multiple of 8 and at most 256, got ", dim);
+  const PagedCache cache = paged_check_caches(k_cache, v_cache, op);
+  TORCH_CHECK(cache.kv_heads == k.size(1) && cache.dim == dim, op, ": caches of ", k_cache.sizes(), " do not take keys of ", k.sizes());
+  const auto out_dtype = q_dtype.value_or(at::kBFloat16);
+  TORCH_CHECK(out_dtype == at::kBFloat16 || is_fp8(out_dtype), op, ": q_dtype must be bfloat16, float8_e4m3fn or float8_e5m2, got ", out_dtype);
+  TORCH_CHECK(slot_map.scalar_type() == at::kLong && slot_map.dim() == 1 && slot_map.numel() == tokens, op,
+              ": slot_map must be an int64 tensor of one slot per token");
+  int64_t rotary = 0;
+  if (cos_sin.defined()) {
+    TORCH_CHECK(cos_sin.scalar_type() == at::kFloat && cos_sin.dim() == 2, op, ": cos_sin must be a float tensor [positions, rotary_dim]");
+    rotary = cos_sin.size(1);
+    TORCH_CHECK(rotary >= 8 && rotary <= dim && rotary % 8 == 0, op, ": rotary_dim must be a multiple of 8 and at most the head dimension, got ", rotary);
+    TORCH_CHECK(positions.defined() && positions.scalar_type() == at::kLong && positions.dim() == 1 && positions.numel() == tokens, op,
+                ": a rotation needs positions, an int64 tensor of one position per token");
+    cos_sin = cos_sin.contiguous();
+    if (reinterpret_cast<uintptr_t>(cos_sin.const_data_ptr()) % 16) cos_sin = cos_sin.clone();
+    positions = positions.contiguous();
+  }
+  at::Tensor weights[2] = {q_weight, k_weight};
+  auto weight_dtype = at::kBFloat16;
+  for (at::Tensor& w : weights) {
+    if (!w.defined()) continue;
+    TORCH_CHECK((w.scalar_type() == at::kFloat || w.scalar_type() == at::kBFloat16) && w.dim() == 1 && w.numel() == dim, op,
+                ": norm weights must be float or bfloat16 tensors of the head dimension");
+    weight_dtype = w.scalar_type();
+    w = w.contiguous();
+    if (reinterpret_cast<uintptr_t>(w.const_data_ptr()) % 16) w = w.clone();
+  }
+  TORCH_CHECK(!weights[0].defined() || !weights[1].defined() || weights[0].scalar_type() == weights[1].scalar_type(), op,
+              ": both norm weights must have the same dtype");
+  for (const at::Tensor* c : {&k_cache, &v_cache}) {
+    bool aligned = reinterpret_cast<uintptr_t>(c->const_data_ptr()) % (4 * c->element_size()) == 0;
+    for (int d = 0; d < 3; ++d) aligned = aligned && paged_stride(*c, d) % 4 == 0;
+    TORCH_CHECK(aligned, op, ": the caches must lie on boundaries of four values");
+  }
+  const int64_t row = 4 * (int64_t)q.element_size();
+  at::Tensor qr = paged_rows(q, row), kr = paged_rows(k, row), vr = paged_rows(v, row), slots = slot_map.contiguous();
+  at::Tensor out = new_tensor(q.sizes(), out_dtype, dev);
+  b200q_append_args a{};
+  a.q = qr.const_data_ptr(); a.k = kr.const_data_ptr(); a.v = vr.const_data_ptr();
+  a.src_dtype = to_b200q_dtype(src);
+  a.tokens = tokens; a.heads = (int)q.size(1); a.kv_heads = (int)k.size(1); a.dim = (int)dim;
+  a.q_token_stride = paged_stride(qr, 0); a.q_head_stride = paged_stride(qr, 1);
+  a.k_token_stride = paged_stride(kr, 0); a.k_head_stride = paged_stride(kr, 1);
+  a.v_token_stride = paged_stride(vr, 0); a.v_head_stride = paged_stride(vr, 1);
+  a.q_weight = weights[0].defined() ? weights[0].const_data_ptr() : nullptr;
+  a.k_weight = weights[1].defined() ? weights[1].const_data_ptr() : nullptr;
+  a.weight_dtype = to_b200q_dtype(weight_dtype);
+  a.eps = (float)eps;
+  if (cos_sin.defined()) {
+    a.cos_sin = cos_sin.const_data_ptr<float>();
+    a.max_positions = cos_sin.size(0);
+    a.rotary_dim = (int)rotary;
+    a.interleaved = interleaved;
+    a.positions = positions.const_data_ptr<int64_t>();
+  }
+  a.slot_map = slots.const_data_ptr<int64_t>();
+  a.k_cache = k_cache.data_ptr(); a.v_cache = v_cache.data_ptr(); a.cache_dtype = to_b200q_dtype(k_cache.scalar_type());
+  a.num_pages = cache.pages; a.page_size = cache.page_size;
+  a.k_page_stride = paged_stride(k_cache, 0); a.k_slot_stride = paged_stride(k_cache, 1); a.k_cache_head_stride = paged_stride(k_cache, 2);
+  a.v_page_stride = paged_stride(v_cache, 0); a.v_slot_stride = paged_stride(v_cache, 1); a.v_cache_head_stride = paged_stride(v_cache, 2);
+  a.k_scale = paged_scale(k_scale, op, "k_scale"); a.v_scale = paged_scale(v_scale, op, "v_scale"); a.q_scale = paged_scale(q_scale, op, "q_scale");
+  a.q_out = out.data_ptr(); a.q_out_dtype = to_b200q_dtype(out_dtype);
+  a.stream = current_stream();
+  check_status(b200q_qk_norm_rope_append(&a), op);
+  return out;
+}
+
+std::tuple<at::Tensor, at::Tensor> paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                                   const at::Tensor& block_table, const at::Tensor& kv_lens, double softmax_scale,
+                                                   const OptTensor& k_scale_inv_opt, const OptTensor& v_scale_inv_opt, int64_t window,
+                                                   const OptTensor& out_scale_opt, c10::optional<at::ScalarType> out_dtype_opt) {
+  const char* op = "paged_attention";
+  const at::Device dev = q.device();
+  at::Tensor k_scale_inv = paged_optional(k_scale_inv_opt), v_scale_inv = paged_optional(v_scale_inv_opt), out_scale = paged_optional(out_scale_opt);
+  paged_same_device(dev, {&k_cache, &v_cache, &block_table, &kv_lens, &k_scale_inv, &v_scale_inv, &out_scale}, op);
+  c10::cuda::CUDAGuard guard(dev);
+  TORCH_CHECK(q.scalar_type() == at::kBFloat16 && q.dim() == 3, op, ": q must be a bfloat16 tensor [requests, heads, dim]");
+  const PagedCache cache = paged_check_caches(k_cache, v_cache, op);
+  const int64_t requests = q.size(0), heads = q.size(1), dim = q.size(2);
+  TORCH_CHECK(cache.dim == dim && dim >= 1 && dim <= 256, op, ": q of ", q.sizes(), " does not read caches of ", k_cache.sizes(),
+              " (head dimensions must agree, at most 256)");
+  TORCH_CHECK(cache.kv_heads > 0 && heads % cache.kv_heads == 0, op, ": ", heads, " query heads cannot share ", cache.kv_heads, " key/value heads");
+  at::Tensor lens = paged_int32(kv_lens, 1, op, "kv_lens");
+  paged_int32(block_table, 2, op, "block_table");
+  TORCH_CHECK(lens.numel() == requests && block_table.size(0) == requests, op, ": block_table and kv_lens must have a row per request, got ",
+              block_table.size(0), " and ", lens.numel(), " for ", requests);
+  TORCH_CHECK(window >= 0, op, ": window must not be negative");
+  const auto out_dtype = out_dtype_opt.value_or(at::kBFloat16);
+  TORCH_CHECK(out_dtype == at::kBFloat16 || out_dtype == at::kFloat || out_dtype == at::kFloat8_e4m3fn, op,
+              ": out_dtype must be bfloat16, float or float8_e4m3fn, got ", out_dtype);
+  at::Tensor qr = paged_rows(q, 16);
+  at::Tensor out = new_tensor(q.sizes(), out_dtype, dev), lse = new_tensor({requests, heads}, at::kFloat, dev);
+  b200q_paged_attention_args a{};
+  a.q = qr.const_data_ptr();
+  a.q_token_stride = paged_stride(qr, 0); a.q_head_stride = paged_stride(qr, 1);
+  a.requests = requests; a.heads = (int)heads; a.kv_heads = (int)cache.kv_heads; a.dim = (int)dim;
+  a.k_cache = k_cache.const_data_ptr(); a.v_cache = v_cache.const_data_ptr(); a.cache_dtype = to_b200q_dtype(k_cache.scalar_type());
+  a.num_pages = cache.pages; a.page_size = cache.page_size;
+  a.k_page_stride = paged_stride(k_cache, 0); a.k_slot_stride = paged_stride(k_cache, 1); a.k_head_stride = paged_stride(k_cache, 2);
+  a.v_page_stride = paged_stride(v_cache, 0); a.v_slot_stride = paged_stride(v_cache, 1); a.v_head_stride = paged_stride(v_cache, 2);
+  a.block_table = block_table.const_data_ptr<int32_t>();
+  a.table_width = block_table.size(1); a.table_stride = paged_table_stride(block_table, op);
+  a.kv_lens = lens.const_data_ptr<int32_t>();
+  a.window = window;
+  a.softmax_scale = (float)softmax_scale;
+  a.k_scale_inv = paged_scale(k_scale_inv, op, "k_scale_inv"); a.v_scale_inv = paged_scale(v_scale_inv, op, "v_scale_inv");
+  a.out_scale = paged_scale(out_scale, op, "out_scale");
+  a.out = out.data_ptr(); a.out_dtype = to_b200q_dtype(out_dtype);
+  a.lse = lse.data_ptr<float>();
+  const size_t bytes = b200q_paged_attention_workspace_bytes(requests, a.heads, a.kv_heads, a.dim, a.cache_dtype);
+  at::Tensor workspace;
+  if (bytes) {
+    workspace = new_tensor({(int64_t)bytes}, at::kByte, dev);
+    a.workspace = workspace.data_ptr();
+    a.workspace_bytes = bytes;
+  }
+  a.stream = current_stream();
+  check_status(b200q_paged_attention(&a), op);
+  return {out, lse};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> meta_paged_plan(const at::Tensor& context_lens, const at::Tensor&,
+                                                                                       at::Tensor&, const at::Tensor&, const OptTensor&,
+                                                                                       int64_t, int64_t num_tokens) {
+  const auto i32 = context_lens.options().dtype(at::kInt), i64 = context_lens.options().dtype(at::kLong);
+  const int64_t n = context_lens.size(0);
+  return {at::empty({num_tokens}, i64), at::empty({num_tokens}, i64), at::empty({n + 1}, i32), at::empty({n}, i32), at::empty({1}, i32)};
+}
+at::Tensor meta_qk_norm_rope_append(const at::Tensor& q, const at::Tensor&, const at::Tensor&, const OptTensor&, const OptTensor&, double,
+                                    const OptTensor&, const OptTensor&, bool, const at::Tensor&, at::Tensor&, at::Tensor&, const OptTensor&,
+                                    const OptTensor&, const OptTensor&, c10::optional<at::ScalarType> q_dtype) {
+  return at::empty(q.sizes(), q.options().dtype(q_dtype.value_or(at::kBFloat16)));
+}
+std::tuple<at::Tensor, at::Tensor> meta_paged_attention(const at::Tensor& q, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                                                        const at::Tensor&, double, const OptTensor&, const OptTensor&, int64_t,
+                                                        const OptTensor&, c10::optional<at::ScalarType> out_dtype) {
+  return {at::empty(q.sizes(), q.options().dtype(out_dtype.value_or(at::kBFloat16))),
+          at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat))};
+}
+
 void set_sr_seed(int64_t seed) {
   g_sr_seed.store(seed);
   g_sr_offset.store(0);
@@ -1519,6 +1755,9 @@ TORCH_LIBRARY(b200q, m) {
   m.def("scale_from_amax_(Tensor(a!) scale, Tensor amax, float fp8_max, bool pow2=True, int margin=0) -> Tensor(a!)");
   m.def("amax_history_update_(Tensor(a!) scale, Tensor(b!) history, int pos, Tensor new_amax, bool use_max, float fp8_max, bool pow2=True, int margin=0) -> Tensor(a!)");
   m.def("cast_moment_to_fp8(Tensor moment, Tensor(a!) scale, ScalarType dtype) -> Tensor");
+  m.def("paged_plan(Tensor context_lens, Tensor new_lens, Tensor(a!) block_table, Tensor free_pages, Tensor? free_head, int page_size, int num_tokens) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("qk_norm_rope_append(Tensor q, Tensor k, Tensor v, Tensor? q_weight, Tensor? k_weight, float eps, Tensor? cos_sin, Tensor? positions, bool interleaved, Tensor slot_map, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor? k_scale=None, Tensor? v_scale=None, Tensor? q_scale=None, ScalarType? q_dtype=None) -> Tensor");
+  m.def("paged_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor kv_lens, float softmax_scale, Tensor? k_scale_inv=None, Tensor? v_scale_inv=None, int window=0, Tensor? out_scale=None, ScalarType? out_dtype=None) -> (Tensor, Tensor)");
   m.def("set_sr_seed(int seed) -> ()", set_sr_seed);
   m.def("set_cast_mul_in_fp32(bool on) -> ()", set_cast_mul_in_fp32);
   m.def("launch_count() -> int", launch_count);
@@ -1537,4 +1776,13 @@ TORCH_LIBRARY_IMPL(b200q, CUDA, m) {
   m.impl("scale_from_amax_", scale_from_amax_);
   m.impl("amax_history_update_", amax_history_update_);
   m.impl("cast_moment_to_fp8", cast_moment_to_fp8);
+  m.impl("paged_plan", paged_plan);
+  m.impl("qk_norm_rope_append", qk_norm_rope_append);
+  m.impl("paged_attention", paged_attention);
+}
+
+TORCH_LIBRARY_IMPL(b200q, Meta, m) {
+  m.impl("paged_plan", meta_paged_plan);
+  m.impl("qk_norm_rope_append", meta_qk_norm_rope_append);
+  m.impl("paged_attention", meta_paged_attention);
 }

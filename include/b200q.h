@@ -75,8 +75,8 @@ int b200q_device_status(int* code_out);
 int b200q_selftest_wait_timeout(int code, void* stream);
 /* Number of kernels this library has launched in this process (all threads). */
 uint64_t b200q_launch_count(void);
-/* sizeof of an argument struct as this library was built: which = 0 b200q_gemm_args, 1 b200q_sdpa_args; 0 for
- * any other value.  A binding that mirrors the structs (ctypes, cgo, JNI) checks its own layout against it. */
+/* sizeof of an argument struct as this library was built: which = 0 b200q_gemm_args, 1 b200q_sdpa_args,
+ * 2 b200q_append_args, 3 b200q_paged_attention_args; 0 for any other value.  A binding that mirrors the structs (ctypes, cgo, JNI) checks its own layout against it. */
 size_t b200q_sizeof_args(int which);
 
 /*
@@ -473,6 +473,122 @@ int b200q_nchw_to_nhwc_u8(const void* in, void* out, int64_t N, int64_t C, int64
 int b200q_im2col_nhwc_fp8(const void* in, void* out, int64_t N, int64_t C, int64_t H, int64_t W, int kh,
                           int kw, int sh, int sw, int ph, int pw, int dh, int dw, int64_t c0,
                           int64_t cg, int64_t ld_out, void* stream);
+
+/*
+ * A key/value cache in pages and one decode step over it.  The reference has no counterpart: its callers keep one
+ * contiguous cache per request and run sdpa_recomp_fwd (hpu_ops/backend/sdpa_gen.cpp:820-1000) over the whole of it.
+ *
+ * paged_plan: where the new tokens of a step go, from the requests' lengths, on the device.  Request b holds
+ * context_lens[b] tokens and gets new_lens[b] (negative counts as 0); a page holds page_size tokens.  Pages that its new
+ * tokens begin are taken from free_pages, in request order, from index *free_head on (NULL: 0):
+ *   block_table[b][j] = the next free page for ceil(context / page_size) <= j < ceil((context + new) / page_size)
+ * (other entries stay).  Then, with query_start the running sum of new_lens, new token i of request b is token
+ * t = query_start[b] + i:
+ *   positions[t] = context + i,   slot_map[t] = page * page_size + positions[t] % page_size.
+ * Tokens t behind the last request's get position 0 and slot -1; so does the slot of a token whose table entry is negative,
+ * lies beyond table_width, or would need more free pages than there are (the table gets -1 there).
+ *
+ * context_lens, new_lens  int32 [requests]; requests <= 8192
+ * block_table   int32 [requests][table_width], row stride table_stride >= table_width; requests * table_width < 2^31
+ * free_pages    int32 [free_count]
+ * slot_map, positions  int64 [num_tokens];  query_start int32 [requests + 1];  kv_lens int32 [requests]: context + new
+ * free_head_out one int32: *free_head + the pages that the step needs (above free_count: there were too few)
+ * Outputs must not overlap inputs.  A call writes the same values again when it is repeated with the same inputs.
+ */
+int b200q_paged_plan(const int32_t* context_lens, const int32_t* new_lens, int64_t requests,
+                     int32_t* block_table, int64_t table_width, int64_t table_stride,
+                     const int32_t* free_pages, int64_t free_count, const int32_t* free_head,
+                     int64_t page_size, int64_t num_tokens, int64_t* slot_map, int64_t* positions,
+                     int32_t* query_start, int32_t* kv_lens, int32_t* free_head_out, void* stream);
+
+/*
+ * qk_norm_rope_append: the step between a projection and the attention over a paged cache, in one pass.
+ *   y = x * rsqrt(mean(x^2) + eps) * weight           per head of q / k (only with a weight)
+ *   pairs (y[i], y[i + r/2]) (interleaved: (y[2i], y[2i + 1])) of the first r = rotary_dim values are turned:
+ *     (a, b) -> (a c - b s, b c + a s),   c = cos_sin[position][i], s = cos_sin[position][r/2 + i]
+ *   q_out = T(y * q_scale);  k_cache[slot] = T(y * k_scale);  v_cache[slot] = T(v * v_scale)
+ * computed in fp32 and rounded once (fp8: to nearest even, saturating; NaN -> 0x7F).  Tokens with a slot outside
+ * [0, num_pages * page_size) write nothing to the caches.  A position outside [0, max_positions) turns q and k into NaN.
+ * Slots that are not negative must differ from one another.
+ *
+ * q / k / v     src_dtype (F32 / BF16) [tokens][heads or kv_heads][dim], token and head strides in elements, values
+ *               contiguous; strides multiples of 4, bases aligned to four elements
+ * dim           a multiple of 8, at most 256;  rotary_dim a multiple of 8, at most dim
+ * q_weight, k_weight   [dim] of weight_dtype (F32 / BF16), aligned like q; NULL = no norm
+ * cos_sin       fp32 [max_positions][rotary_dim], 16-byte aligned, or NULL (no rotation; positions is not read)
+ * caches        cache_dtype (BF16 / E4M3 / E5M2), element (page, slot of the page, head) at page * page_stride +
+ *               slot * slot_stride + head * head_stride (elements, multiples of 4), values contiguous, bases aligned to
+ *               four elements; num_pages * page_size < 2^31
+ * q_out         q_out_dtype (BF16 / E4M3 / E5M2) [tokens][heads][dim] contiguous, aligned to four elements
+ * scales        one fp32 each on the device, or NULL (1)
+ */
+typedef struct b200q_append_args {
+  const void *q, *k, *v;
+  int src_dtype;
+  int64_t tokens;
+  int heads, kv_heads, dim;
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  const void *q_weight, *k_weight;
+  int weight_dtype;
+  float eps;
+  const float* cos_sin;
+  int64_t max_positions;
+  int rotary_dim, interleaved;
+  const int64_t *positions, *slot_map;
+  void *k_cache, *v_cache;
+  int cache_dtype;
+  int64_t num_pages, page_size;
+  int64_t k_page_stride, k_slot_stride, k_cache_head_stride, v_page_stride, v_slot_stride, v_cache_head_stride;
+  const float *k_scale, *v_scale, *q_scale;
+  void* q_out;
+  int q_out_dtype;
+  void* stream;
+} b200q_append_args;
+
+int b200q_qk_norm_rope_append(const b200q_append_args* args);
+
+/*
+ * paged_attention: attention of one new token per request over the paged cache,
+ *   s_j = softmax_scale * k_scale_inv * <q, k_j>,  p = softmax(s) over j in [max(0, len - window), len) (window 0: all),
+ *   out = T(v_scale_inv * sum_j p_j v_j * out_scale),  lse = log sum_j exp(s_j)
+ * with scores, softmax and sums in fp32 and one rounding to T.  A request of length 0 gets zeros and lse = -inf.
+ * Query head h reads key/value head h / (heads / kv_heads).  Lengths are cut to table_width * page_size; keys whose table
+ * entry is outside [0, num_pages) do not exist.  The cache behind a request's length is not looked at.
+ *
+ * q             bf16 [requests][heads][dim], strides in elements, values contiguous
+ * caches        as above, any strides;  block_table int32 [requests][table_width];  kv_lens int32 [requests]
+ * out           out_dtype (BF16 / F32 / E4M3) [requests][heads][dim] contiguous; lse: NULL or fp32 [requests][heads]
+ * workspace     b200q_paged_attention_workspace_bytes(...) bytes, 16-byte aligned, not shared by calls that may overlap
+ * dim = 64, 128 or 256 with pages of a multiple of 16 tokens, and caches and q whose bases and strides are multiples of 16
+ * bytes run the tensor-core kernel; other head dimensions (<= 256) and layouts, or force_plain = 1, a plain CUDA kernel.
+ * The former wants requests <= 8192 and requests * table_width * page_size / 16 < 2^31 (B200Q_ERR_TOO_LARGE).
+ */
+typedef struct b200q_paged_attention_args {
+  const void* q;
+  int64_t q_token_stride, q_head_stride;
+  int64_t requests;
+  int heads, kv_heads, dim;
+  const void *k_cache, *v_cache;
+  int cache_dtype;
+  int64_t num_pages, page_size;
+  int64_t k_page_stride, k_slot_stride, k_head_stride, v_page_stride, v_slot_stride, v_head_stride;
+  const int32_t* block_table;
+  int64_t table_width, table_stride;
+  const int32_t* kv_lens;
+  int64_t window;
+  float softmax_scale;
+  const float *k_scale_inv, *v_scale_inv, *out_scale;
+  void* out;
+  int out_dtype;
+  float* lse;
+  void* workspace;
+  size_t workspace_bytes;
+  int force_plain;
+  void* stream;
+} b200q_paged_attention_args;
+
+size_t b200q_paged_attention_workspace_bytes(int64_t requests, int heads, int kv_heads, int dim, int cache_dtype);
+int b200q_paged_attention(const b200q_paged_attention_args* args);
 
 #ifdef __cplusplus
 }

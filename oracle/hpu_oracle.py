@@ -616,3 +616,76 @@ def fp8_sdpa_recomp_fwd(q, k, v, attention_mask=None, p=0.0, scale=None, is_caus
     else:
         m_out, linv = torch.zeros(1, dtype=torch.bfloat16), torch.zeros(1, dtype=torch.bfloat16)
     return out, m_out, linv, torch.zeros(1, dtype=torch.int32), amax_s, amax_o
+
+
+# ---------------------------------------------------------------------------- paged key/value cache
+# (no counterpart in the reference; the definitions are those of include/b200q.h, computed in 64 bits)
+def paged_plan(context_lens, new_lens, block_table, free_pages, free_head, page_size, num_tokens):
+    """(slot_map, positions, query_start, kv_lens, free_head_out, block_table after the step), request by request."""
+    table = block_table.clone()
+    width, free = table.shape[1], free_pages.tolist()
+    head = 0 if free_head is None else max(0, int(free_head))
+    slots, positions, start, lens = [], [], [0], []
+    for b, (c, n) in enumerate(zip(context_lens.tolist(), new_lens.tolist())):
+        c, n = max(c, 0), max(n, 0)
+        have, need = min(-(-c // page_size), width), min(-(-(c + n) // page_size), width)
+        for j in range(have, need):
+            table[b, j] = free[head] if head < len(free) else -1
+            head += 1
+        for pos in range(c, c + n):
+            page = int(table[b, pos // page_size]) if pos // page_size < width else -1
+            positions.append(pos)
+            slots.append(page * page_size + pos % page_size if page >= 0 else -1)
+        start.append(start[-1] + n)
+        lens.append(c + n)
+    pad = max(0, num_tokens - len(slots))
+    i32 = dict(dtype=torch.int32)
+    return (torch.tensor((slots + [-1] * pad)[:num_tokens], dtype=torch.int64), torch.tensor((positions + [0] * pad)[:num_tokens], dtype=torch.int64),
+            torch.tensor(start, **i32), torch.tensor(lens, **i32), torch.tensor([head], **i32), table)
+
+
+def norm_rope(x, weight, eps, cos_sin, positions, interleaved):
+    """RMS norm of each head (with a weight) and rotation of its first values by the position, in fp64: [tokens, heads, dim]."""
+    x = x.double()
+    if weight is not None:
+        x = x / (x.square().mean(-1, keepdim=True) + eps).sqrt() * weight.double()
+    if cos_sin is None:
+        return x
+    rot = cos_sin.shape[1]
+    half = rot // 2
+    rows = torch.full((x.shape[0], rot), math.nan, dtype=torch.float64)
+    known = (positions >= 0) & (positions < cos_sin.shape[0])
+    rows[known] = cos_sin.double()[positions[known]]
+    angle = torch.complex(rows[:, :half], rows[:, half:])[:, None]
+    r = x[..., :rot]
+    z = torch.complex(r[..., 0::2], r[..., 1::2]) if interleaved else torch.complex(r[..., :half], r[..., half:])
+    z = z * angle
+    r = torch.stack([z.real, z.imag], -1).flatten(-2) if interleaved else torch.cat([z.real, z.imag], -1)
+    return torch.cat([r, x[..., rot:]], -1)
+
+
+def paged_attention(q, k_cache, v_cache, block_table, kv_lens, softmax_scale, k_scale_inv=1.0, v_scale_inv=1.0, window=0):
+    """(out, lse, sum_j p_j |v_j|) in fp64; rows that see nothing are 0 and -inf.  The third bounds what a relative error of the
+    probabilities can do to the output."""
+    requests, heads, dim = q.shape
+    pages, page_size, kv_heads, _ = k_cache.shape
+    group = heads // kv_heads
+    out, size = (torch.zeros(requests, heads, dim, dtype=torch.float64) for _ in range(2))
+    lse = torch.full((requests, heads), -math.inf, dtype=torch.float64)
+    for b, n in enumerate(kv_lens.tolist()):
+        n = min(max(n, 0), block_table.shape[1] * page_size)
+        at = torch.arange(max(0, n - window) if window else 0, n)
+        page = block_table[b].long()[at // page_size]
+        there = (page >= 0) & (page < pages)
+        page, at = page[there], at[there]
+        if not len(at):
+            continue
+        k = k_cache[page, at % page_size].double() * k_scale_inv
+        v = v_cache[page, at % page_size].double() * v_scale_inv
+        for g in range(kv_heads):
+            rows = slice(g * group, (g + 1) * group)
+            s = q[b, rows].double() @ k[:, g].T * softmax_scale
+            p = torch.softmax(s, -1)
+            out[b, rows], size[b, rows] = p @ v[:, g], p @ v[:, g].abs()
+            lse[b, rows] = torch.logsumexp(s, -1)
+    return out, lse, size
