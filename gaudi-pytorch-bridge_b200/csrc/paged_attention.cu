@@ -96,9 +96,824 @@ __global__ void __launch_bounds__(kPlainThreads) paged_attention_plain_kernel(co
   if (tid == 0 && a.lse) a.lse[b * a.heads + head] = empty ? -INFINITY : m + logf(l);
 }
 
-size_t paged_attention_workspace_bytes_impl(int64_t requests, int heads, int kv_heads, int dim, int cache_dtype) { return 0; }
+// ---------------------------------------------------------------------------- tensor cores
+// Memory bound: every cached key and value is used once for the 8 or 16 query heads that share it.  What the kernel does
+// beside reading must stay under the reads: 16 flops a byte and head group are beyond the CUDA cores' rate in fp32, so both
+// products are m16n8k16 matrix instructions with the CACHE as the operand of 16 rows (keys of K, dimensions of V) and the heads as
+// the 8 columns, which fills the instruction when eight heads share a key/value head.
+//
+// A warp works on steps of 16 keys.  Its lanes copy the operands' fragments, 16 bytes at a time, straight from the pages
+// into a ring of its own in shared memory (cp.async) and each lane reads back only what it copied itself: no barrier, no
+// bank conflict, no transposition.  Lane (g = lane / 4, t = lane % 4) owns
+//   of K: keys g and g + 8, bytes 64 c + 16 t ... + 15 of their rows   (the dimensions of a dot product may come in any order:
+//         the queries are laid out to match)
+//   of V: keys 2t, 2t + 1, 2t + 8, 2t + 9, bytes (8 c + g) * 16 ... + 15  (the dimensions are the rows of the second product, which
+//         may come in any order too)
+// fp8 values become f16 exactly; the probabilities are rounded to f16 (11 bits, scaled by 2^7 so that the small ones stay normal).
+// For a bf16 cache they are split into two bf16 terms (16 bits) that take a product each.  Queries meet fp8 keys as f16, scaled
+// by a power of two per head, which is exact over 2^22 of a head's largest value.
+//
+// Work is the list of all steps (request-major, then key/value head, then the length), cut into equal runs for the CTAs and
+// then for their warps, so that ragged lengths and few requests load every SM alike.  A run may begin or end inside a row of
+// steps: such partial results (maximum, sum, output) are joined in the CTA, and, where a row goes on in another CTA, by a second
+// kernel.
+constexpr int kPagedGrid = kNumSMs;
+constexpr int kPagedRingBytes = 192 * 1024;
+constexpr int kPagedMinSteps = 2;     // a warp gets at least this many steps while there are enough for the others
+constexpr float kPagedShift = 7.f;    // probabilities are held relative to 2^(maximum - 7) ...
+constexpr float kPagedRescale = 15.f; // ... and the maximum is raised when one would pass 2^15 (f16 ends at 2^16)
+constexpr float kPagedNoMax = -3.0e38f;
+
+template <int DIM, int FMT, int NT>
+struct PagedTile {
+  static constexpr int kElt = FMT == B200Q_BF16 ? 2 : 1;
+  static constexpr int kRow = DIM * kElt;           // bytes of a key
+  static constexpr int kStage = 2 * 16 * kRow;      // keys and values of a step
+  static constexpr int kWarps = DIM == 256 ? 4 : 8;
+  static constexpr int kStages = kPagedRingBytes / kWarps / kStage < 8 ? kPagedRingBytes / kWarps / kStage : 8;
+  static constexpr int kKChunks = kRow / 64;        // 16-byte pieces of a key per lane
+  static constexpr int kVPiece = kRow / 8 < 16 ? 8 : 16;
+  static constexpr int kVChunks = kRow / 8 / kVPiece;
+  static constexpr int kVPer = kVPiece / kElt;      // values of a piece
+  static constexpr int kTiles = DIM / 16;           // k-steps of the first product, row tiles of the second
+  static constexpr int kRows = 8 * NT;              // query heads
+  static constexpr int kPart = kRows * (DIM + 2);   // floats of a partial result: output, maxima, sums
+  static constexpr int kRing = kStages * kStage;    // bytes per warp
+  static_assert(kPart * 4 <= kRing && kStages >= 2, "a partial result takes the place of the ring");
+};
+
+// Where a row that is cut by the first step of a CTA comes together: {row begins in the CTA before, request, head index, CTAs from here}
+struct alignas(16) PagedJoin {
+  int valid, request, sub, count;
+};
+
+struct PagedWork {
+  int heads_per_request;  // key/value heads x row tiles
+  int row_tiles;
+  int group;              // query heads per key/value head
+  PagedJoin* joins;       // [grid]
+  float* cta_part;        // [grid][2][kPart]: rows from the CTA before, rows into the CTA behind
+  float* warp_part;       // [grid][warps][kPart]: rows from the warp before that end inside a warp's run
+};
+
+__device__ __forceinline__ uint32_t paged_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+template <int BYTES>
+__device__ __forceinline__ void paged_copy(uint32_t dst, const void* src, bool there) {
+  const int n = there ? BYTES : 0;  // (nothing is read, and zeros are written, where there is no key)
+  if (BYTES == 16) asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+  else asm volatile("cp.async.ca.shared.global.L2::128B [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void paged_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void paged_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint4 paged_lds16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 paged_lds8(uint32_t at) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ float paged_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <int FMT>
+__device__ __forceinline__ void paged_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if (FMT == B200Q_BF16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// rows of 8 x 8 16-bit values held as fragments become columns
+__device__ __forceinline__ uint32_t paged_transpose(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+// four fp8 values -> (0, 1) and (2, 3) as f16 pairs, exactly
+template <int FMT>
+__device__ __forceinline__ void paged_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if (FMT == B200Q_E4M3) {
+    asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.f16x2.e4m3x2 %0, a;\ncvt.rn.f16x2.e4m3x2 %1, b;\n}" : "=r"(lo), "=r"(hi) : "r"(w));
+  } else {  // (an e5m2 value is the upper byte of the f16 one)
+    lo = __byte_perm(w, 0u, 0x1404);
+    hi = __byte_perm(w, 0u, 0x3424);
+  }
+}
+__device__ __forceinline__ uint32_t paged_pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ void paged_store4(void* out, int dtype, int64_t at, const float (&v)[4]) {
+  if (dtype == B200Q_BF16)
+    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(out) + at) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+  else if (dtype == B200Q_F32) *reinterpret_cast<float4*>(static_cast<float*>(out) + at) = make_float4(v[0], v[1], v[2], v[3]);
+  else *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(out) + at) = cvt_fp8x2<B200Q_E4M3>(v[0], v[1]) | (cvt_fp8x2<B200Q_E4M3>(v[2], v[3]) << 16);
+}
+__device__ __forceinline__ float paged_lse(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147180559945309f; }
+__device__ __forceinline__ float paged_out_scale(const b200q_paged_attention_args& a) {
+  return (a.v_scale_inv ? *a.v_scale_inv : 1.f) * (a.out_scale ? *a.out_scale : 1.f);
+}
+
+// the keys that a request's token sees: [first, len); its steps begin at a multiple of 16
+struct PagedSpan {
+  int64_t len, first;
+  __device__ __forceinline__ PagedSpan(const b200q_paged_attention_args& a, int b) {
+    len = paged_length(a, b);
+    first = a.window > 0 && len > a.window ? len - a.window : 0;
+  }
+  __device__ __forceinline__ int steps() const { return (int)((len + 15) / 16 - first / 16); }
+};
+
+// A place in the list of steps.
+struct PagedCursor {
+  int b, sub, step, steps;
+  // the place of global step g < total; prefix: inclusive sums of the requests' steps
+  __device__ __forceinline__ void locate(const int* prefix, int requests, int heads, int64_t g) {
+    int lo = 0, hi = requests - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if ((int64_t)prefix[mid] * heads > g) hi = mid;
+      else lo = mid + 1;
+    }
+    b = lo;
+    const int before = b ? prefix[b - 1] : 0;
+    steps = prefix[b] - before;
+    const int64_t r = g - (int64_t)before * heads;
+    sub = (int)(r / steps);
+    step = (int)(r - (int64_t)sub * steps);
+  }
+  // to the first step of the next row; there is one
+  __device__ __forceinline__ bool next_row(const int* prefix, int requests, int heads) {
+    step = 0;
+    if (++sub < heads) return true;
+    sub = 0;
+    do {
+      if (++b >= requests) return false;
+      steps = prefix[b] - prefix[b - 1];
+    } while (steps == 0);
+    return true;
+  }
+};
+
+// One of a warp's partial results, in the order in which rows are written out: [kRows][DIM], then maxima, then sums.
+template <int DIM, int FMT, int NT>
+struct PagedAcc {
+  using Tile = PagedTile<DIM, FMT, NT>;
+  float o[Tile::kTiles][NT][4];  // dimensions x heads: fragment j holds the lane's values 2j (0, 1) and 2j + 1 (2, 3) for heads 2t, 2t + 1
+  float m[NT][2], l[NT][2];
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int j = 0; j < Tile::kTiles; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[j][n][i] = 0.f;
+      m[n][0] = m[n][1] = kPagedNoMax;
+      l[n][0] = l[n][1] = 0.f;
+    }
+  }
+  // every lane has the whole sums
+  __device__ __forceinline__ void sum_lanes() {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int s = 4; s < 32; s <<= 1) l[n][i] += __shfl_xor_sync(0xFFFFFFFFu, l[n][i], s);
+  }
+  // calls f(head row, first dimension, four values) for all that the lane holds
+  template <typename F>
+  __device__ __forceinline__ void each4(int g, int t, F f) const {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < Tile::kVChunks * Tile::kVPer; e += 4) {
+          const float v[4] = {o[e / 2][n][i], o[e / 2][n][i + 2], o[e / 2 + 1][n][i], o[e / 2 + 1][n][i + 2]};
+          f(8 * n + 2 * t + i, (e / Tile::kVPer * 8 + g) * Tile::kVPer + e % Tile::kVPer, v, n, i);
+        }
+  }
+  __device__ __forceinline__ void save(float* to, int g, int t) const {
+    each4(g, t, [&](int row, int d, const float (&v)[4], int, int) {
+      *reinterpret_cast<float4*>(to + row * DIM + d) = make_float4(v[0], v[1], v[2], v[3]);
+    });
+    if (g == 0) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int row = 8 * n + 2 * t + i;
+          to[Tile::kRows * DIM + row] = m[n][i];
+          to[Tile::kRows * DIM + Tile::kRows + row] = l[n][i];
+        }
+    }
+  }
+};
+
+// Joins one head's results from `count` places (at(i): a partial result): the values of dimensions lane, lane + 32, ...
+template <int DIM, int ROWS, typename At>
+__device__ __forceinline__ void paged_merge(At at, int count, int row, int lane, float (&o)[DIM / 32], float& m, float& l) {
+  m = kPagedNoMax;
+  for (int i = 0; i < count; ++i) m = fmaxf(m, __ldcg(at(i) + ROWS * DIM + row));  // (written by other CTAs: read past L1)
+  l = 0.f;
+#pragma unroll
+  for (int d = 0; d < DIM / 32; ++d) o[d] = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < count; ++i) {
+    const float* p = at(i);
+    const float w = exp2f(__ldcg(p + ROWS * DIM + row) - m);  // (inf - inf: a NaN row, as its parts are)
+    l += w * __ldcg(p + ROWS * DIM + ROWS + row);
+#pragma unroll
+    for (int d = 0; d < DIM / 32; ++d) o[d] += w * __ldcg(p + row * DIM + d * 32 + lane);
+  }
+}
+template <int DIM>
+__device__ __forceinline__ void paged_finish(const b200q_paged_attention_args& a, int b, int head, int lane, const float (&o)[DIM / 32], float m, float l,
+                                             float scale) {
+  const int64_t at = ((int64_t)b * a.heads + head) * DIM;
+  const float inv = l == 0.f ? 0.f : scale / l;
+#pragma unroll
+  for (int d = 0; d < DIM / 32; ++d) paged_store(a.out, a.out_dtype, at + d * 32 + lane, o[d] * inv);
+  if (lane == 0 && a.lse) a.lse[(int64_t)b * a.heads + head] = paged_lse(m, l);
+}
+
+template <int DIM, int FMT, int NT>
+__global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
+    paged_attention_kernel(const b200q_paged_attention_args a, const PagedWork w) {
+  using Tile = PagedTile<DIM, FMT, NT>;
+  constexpr int kWarps = Tile::kWarps, kStages = Tile::kStages, kTiles = Tile::kTiles, kElt = Tile::kElt;
+  extern __shared__ __align__(16) uint8_t s_ring[];  // [warps][kRing], then the prefix sums
+  __shared__ int s_sum[kWarps];
+  __shared__ int s_final[kWarps], s_from[kWarps], s_done[kWarps], s_b[kWarps], s_sub[kWarps];
+  int* prefix = reinterpret_cast<int*>(s_ring + kWarps * Tile::kRing);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int requests = (int)a.requests, heads = w.heads_per_request;
+  pdl_enter();
+
+  // ---- the list of steps
+  {
+    const int per = (requests + 32 * kWarps - 1) / (32 * kWarps);
+    const int b0 = min(tid * per, requests), b1 = min(b0 + per, requests);
+    int sum = 0;
+    for (int b = b0; b < b1; ++b) {
+      sum += PagedSpan(a, b).steps();
+      prefix[b] = sum;
+    }
+    int scan = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xFFFFFFFFu, scan, o);
+      if (lane >= o) scan += v;
+    }
+    if (lane == 31) s_sum[warp] = scan;
+    __syncthreads();
+    int before = scan - sum;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i)
+      if (i < warp) before += s_sum[i];
+    for (int b = b0; b < b1; ++b) prefix[b] += before;
+    __syncthreads();
+  }
+  const int64_t total = (int64_t)prefix[requests - 1] * heads;
+  const float out_scale = paged_out_scale(a);
+
+  // requests that see nothing
+  for (int b = blockIdx.x; b < requests; b += gridDim.x) {
+    if (prefix[b] != (b ? prefix[b - 1] : 0)) continue;
+    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int i = tid; i < a.heads * (DIM / 4); i += 32 * kWarps) paged_store4(a.out, a.out_dtype, (int64_t)b * a.heads * DIM + 4 * i, zero);
+    if (a.lse)
+      for (int i = tid; i < a.heads; i += 32 * kWarps) a.lse[(int64_t)b * a.heads + i] = -INFINITY;
+  }
+
+  // ---- this CTA's run, and this warp's
+  const int64_t wanted = (total + kWarps * kPagedMinSteps - 1) / (kWarps * kPagedMinSteps);
+  const int64_t ctas = wanted < (int64_t)gridDim.x ? wanted : (int64_t)gridDim.x;
+  const int c = blockIdx.x;
+  if (c >= ctas) {
+    if (tid == 0) w.joins[c].valid = 0;
+    return;
+  }
+  const int64_t run0 = total * c / ctas, run1 = total * (c + 1) / ctas;
+  auto warp_begin = [&](int i) { return run0 + ((run1 - run0) * i + kWarps - 1) / kWarps; };
+  const int64_t first_step = warp_begin(warp);
+  const int todo = (int)(warp_begin(warp + 1) - first_step);
+  if (tid == 0) {
+    PagedCursor cut;
+    cut.locate(prefix, requests, heads, run0);
+    PagedJoin join = {0, cut.b, cut.sub, 0};
+    const int64_t row0 = run0 - cut.step, row1 = row0 + cut.steps;
+    if (cut.step > 0 && row0 >= total * (c - 1) / ctas) {  // the row is cut here for the first time
+      join.valid = 1;
+      join.count = (int)((row1 * ctas + total - 1) / total - 1) - c + 1;  // CTAs that hold steps [run0, row1)
+    }
+    w.joins[c] = join;
+  }
+
+  const uint32_t ring = paged_smem(s_ring + warp * Tile::kRing);
+  float* const part_smem = reinterpret_cast<float*>(s_ring + warp * Tile::kRing);
+  int final_part = 0, from_here = 0, row_done = 0;  // of the row that the warp's run ends in
+  PagedCursor cc = {0, 0, 0, 0};
+
+  if (todo > 0) {
+    // ---- copies, kStages - 1 steps ahead
+    PagedCursor pc;
+    pc.locate(prefix, requests, heads, first_step);
+    cc = pc;
+    const int ps = (int)a.page_size;
+    const uint8_t* const k_base = static_cast<const uint8_t*>(a.k_cache);
+    const uint8_t* const v_base = static_cast<const uint8_t*>(a.v_cache);
+    const int64_t k_lane = (int64_t)g * a.k_slot_stride * kElt + 16 * t, k_eight = 8 * a.k_slot_stride * kElt;
+    const int64_t v_slot = a.v_slot_stride * kElt, v_lane = 2 * t * v_slot + g * Tile::kVPiece;
+    int64_t p_pos, p_len, p_first;  // of the step that is copied next
+    int p_off, p_page;              // its place in its page, and the page
+    int64_t p_index;                // of the page in the table
+    uint32_t bad = 0;               // bit s: the step in stage s has no page
+    auto page_at = [&](int b, int64_t index) {  // steps lie within a request's length, which its table covers
+      const int p = a.block_table[(int64_t)b * a.table_stride + index];
+      return p >= 0 && p < a.num_pages ? p : -1;
+    };
+    auto enter_row = [&] {
+      const PagedSpan span(a, pc.b);
+      p_len = span.len;
+      p_first = span.first;
+      p_pos = span.first / 16 * 16 + (int64_t)pc.step * 16;
+      p_index = p_pos / ps;
+      p_off = (int)(p_pos - p_index * ps);
+      p_page = page_at(pc.b, p_index);
+    };
+    int copied = 0;
+    auto copy_step = [&](int stage) {
+      if (copied < todo) {
+        const uint32_t dst = ring + stage * Tile::kStage + lane * 16;
+        const uint32_t dst_v = ring + stage * Tile::kStage + 16 * Tile::kRow + lane * Tile::kVPiece;
+        const bool page_there = p_page >= 0;
+        bad = (bad & ~(1u << stage)) | (page_there ? 0u : 1u << stage);
+        const int kv = pc.sub / w.row_tiles;
+        const int64_t page = page_there ? p_page : 0;
+        const uint8_t* k = k_base + ((page * a.k_page_stride + p_off * a.k_slot_stride + kv * a.k_head_stride) * kElt + k_lane);
+        const uint8_t* v = v_base + ((page * a.v_page_stride + p_off * a.v_slot_stride + kv * a.v_head_stride) * kElt + v_lane);
+        auto there = [&](int key) { return page_there && p_pos + key < p_len && p_pos + key >= p_first; };
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const bool ok = there(8 * h + g);
+          const uint8_t* src = ok ? k + h * k_eight : k_base;
+#pragma unroll
+          for (int i = 0; i < Tile::kKChunks; ++i) paged_copy<16>(dst + (h * Tile::kKChunks + i) * 512, src + 64 * i, ok);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int key = (q >> 1) * 8 + (q & 1);
+          const bool ok = there(key + 2 * t);
+          const uint8_t* src = ok ? v + key * v_slot : v_base;
+#pragma unroll
+          for (int i = 0; i < Tile::kVChunks; ++i)
+            paged_copy<Tile::kVPiece>(dst_v + (q * Tile::kVChunks + i) * 32 * Tile::kVPiece, src + 8 * Tile::kVPiece * i, ok);
+        }
+        if (++copied < todo) {
+          if (++pc.step < pc.steps) {
+            p_pos += 16;
+            p_off += 16;
+            if (p_off >= ps) {
+              p_off = 0;
+              p_page = page_at(pc.b, ++p_index);
+            }
+          } else if (pc.next_row(prefix, requests, heads)) {
+            enter_row();
+          }
+        }
+      }
+      paged_commit();
+    };
+    enter_row();
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) copy_step(s);
+
+    // ---- the products
+    PagedAcc<DIM, FMT, NT> acc;
+    uint32_t qf[kTiles][NT][2];
+    float coef[NT][2];  // scores in powers of two for heads 2t, 2t + 1
+    int64_t c_len = 0, c_first = 0, c_pos = 0;
+    const float score_scale = a.softmax_scale * (a.k_scale_inv ? *a.k_scale_inv : 1.f) * 1.44269504088896341f;
+    const __nv_bfloat16* const q = static_cast<const __nv_bfloat16*>(a.q);
+    auto begin_row = [&] {
+      const PagedSpan span(a, cc.b);
+      c_len = span.len;
+      c_first = span.first;
+      c_pos = span.first / 16 * 16 + (int64_t)cc.step * 16;
+      from_here = cc.step == 0;
+      acc.clear();
+      const int kv = cc.sub / w.row_tiles, row0 = (cc.sub - kv * w.row_tiles) * Tile::kRows;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int row = row0 + 8 * n + g;
+        const bool live = row < w.group;
+        const __nv_bfloat16* src = q + (int64_t)cc.b * a.q_token_stride + (int64_t)(kv * w.group + (live ? row : 0)) * a.q_head_stride;
+        if (FMT == B200Q_BF16) {
+#pragma unroll
+          for (int i = 0; i < Tile::kKChunks; ++i) {
+            uint4 v = *reinterpret_cast<const uint4*>(src + (4 * i + t) * 8);
+            if (!live) v = make_uint4(0, 0, 0, 0);
+            qf[2 * i][n][0] = v.x; qf[2 * i][n][1] = v.y; qf[2 * i + 1][n][0] = v.z; qf[2 * i + 1][n][1] = v.w;
+          }
+          coef[n][0] = coef[n][1] = score_scale;
+        } else {
+          uint32_t raw[Tile::kKChunks][8];
+          uint32_t top = 0;
+#pragma unroll
+          for (int i = 0; i < Tile::kKChunks; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint4 v = *reinterpret_cast<const uint4*>(src + (4 * i + t) * 16 + 8 * h);
+              if (!live) v = make_uint4(0, 0, 0, 0);
+              raw[i][4 * h] = v.x; raw[i][4 * h + 1] = v.y; raw[i][4 * h + 2] = v.z; raw[i][4 * h + 3] = v.w;
+              top = __vmaxu2(top, __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu)));
+            }
+          top = max(top & 0xFFFFu, top >> 16);
+          top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+          top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+          // largest exponent of the head -> 2^8 (nothing to do for zeros; infinities and NaN stay what they are)
+          const int e = (int)(top >> 7) - 127;
+          const int up = top == 0 || e == 128 ? 0 : min(8 - e, 120);
+          const float mul = __uint_as_float((uint32_t)(127 + up) << 23), back = __uint_as_float((uint32_t)(127 - up) << 23);
+#pragma unroll
+          for (int i = 0; i < Tile::kKChunks; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              qf[4 * i + j / 2][n][j % 2] = paged_pack_f16(bf16_bits_to_float(raw[i][j] & 0xFFFFu) * mul, bf16_bits_to_float(raw[i][j] >> 16) * mul);
+          coef[n][0] = score_scale * __shfl_sync(0xFFFFFFFFu, back, 8 * t);
+          coef[n][1] = score_scale * __shfl_sync(0xFFFFFFFFu, back, 8 * t + 4);
+        }
+      }
+    };
+    begin_row();
+
+    int stage = 0;
+    for (int done = 0; done < todo; ++done) {
+      paged_wait<kStages - 2>();
+      const uint32_t src = ring + stage * Tile::kStage + lane * 16;
+      const uint32_t src_v = ring + stage * Tile::kStage + 16 * Tile::kRow + lane * Tile::kVPiece;
+      // scores: keys x heads
+      float s[NT][4], s2[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[n][i] = s2[n][i] = 0.f;
+#pragma unroll
+      for (int i = 0; i < Tile::kKChunks; ++i) {
+        const uint4 lo4 = paged_lds16(src + i * 512), hi4 = paged_lds16(src + (Tile::kKChunks + i) * 512);
+        const uint32_t lo[4] = {lo4.x, lo4.y, lo4.z, lo4.w}, hi[4] = {hi4.x, hi4.y, hi4.z, hi4.w};
+        if (FMT == B200Q_BF16) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            paged_mma<FMT>(s[n], lo[0], hi[0], lo[1], hi[1], qf[2 * i][n][0], qf[2 * i][n][1]);
+            paged_mma<FMT>(s2[n], lo[2], hi[2], lo[3], hi[3], qf[2 * i + 1][n][0], qf[2 * i + 1][n][1]);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t a0, a1, a2, a3;
+            paged_f16<FMT>(lo[j], a0, a2);
+            paged_f16<FMT>(hi[j], a1, a3);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) paged_mma<FMT>(j & 1 ? s2[n] : s[n], a0, a1, a2, a3, qf[4 * i + j][n][0], qf[4 * i + j][n][1]);
+          }
+        }
+      }
+      const bool nowhere = bad >> stage & 1u;
+      bool ok0 = true, ok1 = true;  // keys g, g + 8
+      if (nowhere || c_pos + 16 > c_len || c_pos < c_first) {
+        ok0 = !nowhere && c_pos + g < c_len && c_pos + g >= c_first;
+        ok1 = !nowhere && c_pos + 8 + g < c_len && c_pos + 8 + g >= c_first;
+      }
+      uint32_t p_hi[NT][2], p_lo[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[n][i] += s2[n][i];
+        auto exponents = [&] {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = (i < 2 ? ok0 : ok1) ? fmaf(s[n][i], coef[n][i & 1], -acc.m[n][i & 1]) : -INFINITY;
+        };
+        exponents();
+        if (__any_sync(0xFFFFFFFFu, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) > kPagedRescale)) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float top = fmaxf(ok0 ? s[n][i] * coef[n][i] : -INFINITY, ok1 ? s[n][i + 2] * coef[n][i] : -INFINITY);
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+            const float raised = top > acc.m[n][i] + kPagedRescale ? top - kPagedShift : acc.m[n][i];
+            const float keep = paged_exp2(acc.m[n][i] - raised);
+            acc.m[n][i] = raised;
+            acc.l[n][i] *= keep;
+#pragma unroll
+            for (int j = 0; j < kTiles; ++j) {
+              acc.o[j][n][i] *= keep;
+              acc.o[j][n][i + 2] *= keep;
+            }
+          }
+          exponents();
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = paged_exp2(x[i]);
+        acc.l[n][0] += x[0] + x[2];
+        acc.l[n][1] += x[1] + x[3];
+        if (FMT == B200Q_BF16) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t hi = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+            const uint32_t lo = pack_bf16x2(x[2 * i] - bf16_bits_to_float(hi & 0xFFFFu), x[2 * i + 1] - bf16_bits_to_float(hi >> 16));
+            p_hi[n][i] = paged_transpose(hi);
+            p_lo[n][i] = paged_transpose(lo);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) p_hi[n][i] = paged_transpose(paged_pack_f16(x[2 * i], x[2 * i + 1]));
+        }
+      }
+      // output: dimensions x heads
+#pragma unroll
+      for (int i = 0; i < Tile::kVChunks; ++i) {
+        uint32_t v[4][Tile::kVPiece / 4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t at = src_v + (k * Tile::kVChunks + i) * 32 * Tile::kVPiece;
+          if (Tile::kVPiece == 16) {
+            const uint4 x = paged_lds16(at);
+            v[k][0] = x.x; v[k][1] = x.y; v[k][Tile::kVPiece / 4 - 2] = x.z; v[k][Tile::kVPiece / 4 - 1] = x.w;
+          } else {
+            const uint2 x = paged_lds8(at);
+            v[k][0] = x.x; v[k][1] = x.y;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < Tile::kVPiece / 4; ++j) {
+          if (FMT == B200Q_BF16) {
+            const uint32_t a0 = __byte_perm(v[0][j], v[1][j], 0x5410), a1 = __byte_perm(v[0][j], v[1][j], 0x7632);
+            const uint32_t a2 = __byte_perm(v[2][j], v[3][j], 0x5410), a3 = __byte_perm(v[2][j], v[3][j], 0x7632);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              paged_mma<FMT>(acc.o[i * 4 + j][n], a0, a1, a2, a3, p_hi[n][0], p_hi[n][1]);
+              paged_mma<FMT>(acc.o[i * 4 + j][n], a0, a1, a2, a3, p_lo[n][0], p_lo[n][1]);
+            }
+          } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t sel = h ? 0x7362 : 0x5140;  // (key, next key) of two dimensions
+              uint32_t a0, a1, a2, a3;
+              paged_f16<FMT>(__byte_perm(v[0][j], v[1][j], sel), a0, a1);
+              paged_f16<FMT>(__byte_perm(v[2][j], v[3][j], sel), a2, a3);
+#pragma unroll
+              for (int n = 0; n < NT; ++n)
+                paged_mma<FMT>(acc.o[(i * Tile::kVPiece + j * 4) / 2 + h][n], a0, a1, a2, a3, p_hi[n][0], p_hi[n][1]);
+            }
+          }
+        }
+      }
+      // the stage of the step before this one is free
+      copy_step(stage == 0 ? kStages - 1 : stage - 1);
+      if (++stage == kStages) stage = 0;
+      c_pos += 16;
+
+      const bool row_end = ++cc.step == cc.steps, last = done + 1 == todo;
+      if (row_end || last) {
+        acc.sum_lanes();
+        if (row_end && from_here) {
+          const int kv = cc.sub / w.row_tiles, row0 = (cc.sub - kv * w.row_tiles) * Tile::kRows;
+          acc.each4(g, t, [&](int row, int d, const float (&v)[4], int n, int i) {
+            if (row0 + row >= w.group) return;
+            const float inv = acc.l[n][i] == 0.f ? 0.f : out_scale / acc.l[n][i];
+            const float r[4] = {v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
+            paged_store4(a.out, a.out_dtype, ((int64_t)cc.b * a.heads + kv * w.group + row0 + row) * DIM + d, r);
+          });
+          if (a.lse && g == 0) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const int row = row0 + 8 * n + 2 * t + i;
+                if (row < w.group) a.lse[(int64_t)cc.b * a.heads + kv * w.group + row] = paged_lse(acc.m[n][i], acc.l[n][i]);
+              }
+          }
+        } else if (last) {
+          paged_wait<0>();
+          __syncwarp();
+          acc.save(part_smem, g, t);
+          final_part = 1;
+          row_done = row_end;
+        } else {
+          acc.save(w.warp_part + ((int64_t)c * kWarps + warp) * Tile::kPart, g, t);
+        }
+        if (!last && cc.next_row(prefix, requests, heads)) begin_row();
+      }
+    }
+  }
+  if (lane == 0) {
+    s_final[warp] = todo > 0 ? final_part : -1;  // -1: no steps
+    s_from[warp] = from_here;
+    s_done[warp] = row_done;
+    s_b[warp] = cc.b;
+    s_sub[warp] = cc.sub;
+  }
+  __syncthreads();
+
+  // ---- rows that several warps have a part of: the heads are dealt to the warps
+  bool cut = false;  // whether the first row began in an earlier CTA
+  PagedCursor at0;
+  at0.locate(prefix, requests, heads, run0);
+  cut = at0.step > 0;
+  for (int i = 0; i < 2 * kWarps; ++i) {
+    const int first = i >> 1;
+    const bool from_cut = !(i & 1);  // the row from the CTA before; the row that begins in warp `first` and goes on
+    if (from_cut ? !(first == 0 && cut) : !(s_final[first] == 1 && s_from[first])) continue;
+    // its parts: the first warp's, then those of the following ones until the row ends
+    const float* parts[kWarps];
+    int count = 0;
+    bool ended = false;
+#pragma unroll
+    for (int v = 0; v < kWarps; ++v) {
+      parts[v] = nullptr;
+      if (v < first || ended || s_final[v] < 0) continue;
+      const bool whole = s_final[v] == 1 && (!s_from[v] || (v == first && !from_cut));
+      parts[v] = whole ? reinterpret_cast<const float*>(s_ring + v * Tile::kRing) : w.warp_part + ((int64_t)c * kWarps + v) * Tile::kPart;
+      ended = whole ? s_done[v] : true;
+      ++count;
+    }
+    const int b = from_cut ? at0.b : s_b[first], sub = from_cut ? at0.sub : s_sub[first];
+    const int kv = sub / w.row_tiles, row0 = (sub - kv * w.row_tiles) * Tile::kRows;
+    for (int row = warp; row < Tile::kRows; row += kWarps) {
+      if (row0 + row >= w.group) continue;
+      float m = kPagedNoMax, l = 0.f, o[DIM / 32];
+#pragma unroll
+      for (int v = 0; v < kWarps; ++v)
+        if (parts[v]) m = fmaxf(m, parts[v][Tile::kRows * DIM + row]);
+#pragma unroll
+      for (int d = 0; d < DIM / 32; ++d) o[d] = 0.f;
+#pragma unroll
+      for (int v = 0; v < kWarps; ++v) {
+        if (!parts[v]) continue;
+        const float x = exp2f(parts[v][Tile::kRows * DIM + row] - m);  // (inf - inf: a NaN row, as its parts are)
+        l += x * parts[v][Tile::kRows * DIM + Tile::kRows + row];
+#pragma unroll
+        for (int d = 0; d < DIM / 32; ++d) o[d] += x * parts[v][row * DIM + d * 32 + lane];
+      }
+      if (!from_cut && ended) {
+        paged_finish<DIM>(a, b, kv * w.group + row0 + row, lane, o, m, l, out_scale);
+      } else {
+        float* to = w.cta_part + ((int64_t)c * 2 + (from_cut ? 0 : 1)) * Tile::kPart;
+#pragma unroll
+        for (int d = 0; d < DIM / 32; ++d) to[row * DIM + d * 32 + lane] = o[d];
+        if (lane == 0) {
+          to[Tile::kRows * DIM + row] = m;
+          to[Tile::kRows * DIM + Tile::kRows + row] = l;
+        }
+      }
+    }
+  }
+}
+
+// Rows that several CTAs have a part of.  Block (c, row): the row of steps that is first cut where CTA c begins.
+template <int DIM, int ROWS>
+__global__ void __launch_bounds__(128) paged_join_kernel(const b200q_paged_attention_args a, const PagedWork w) {
+  constexpr int kPart = ROWS * (DIM + 2);
+  __shared__ float s_o[4][DIM], s_m[4], s_l[4];
+  pdl_enter();
+  const int c = blockIdx.x, row = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int4 v = __ldcg(reinterpret_cast<const int4*>(w.joins + c));
+  const PagedJoin join = {v.x, v.y, v.z, v.w};
+  if (!join.valid) return;
+  if (c < 1 || join.count < 1 || join.count > (int)gridDim.x - c || join.request < 0 || join.request >= a.requests || join.sub < 0 ||
+      join.sub >= w.heads_per_request)
+    return;
+  const int kv = join.sub / w.row_tiles, row0 = (join.sub - kv * w.row_tiles) * ROWS;
+  if (row0 + row >= w.group) return;
+  // part 0: the CTA before's last row; part i: the first row of CTA c + i - 1.  A warp takes a quarter of them.
+  const int count = join.count + 1, per = (count + 3) / 4, i0 = min(warp * per, count), n = min(per, count - i0);
+  float m, l, o[DIM / 32];
+  paged_merge<DIM, ROWS>([&](int i) { return w.cta_part + (i0 + i == 0 ? (int64_t)(c - 1) * 2 + 1 : (int64_t)(c + i0 + i - 1) * 2) * kPart; }, n, row, lane, o, m, l);
+#pragma unroll
+  for (int d = 0; d < DIM / 32; ++d) s_o[warp][d * 32 + lane] = o[d];
+  if (lane == 0) {
+    s_m[warp] = m;
+    s_l[warp] = l;
+  }
+  __syncthreads();
+  if (warp != 0) return;
+  m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+  l = 0.f;
+#pragma unroll
+  for (int d = 0; d < DIM / 32; ++d) o[d] = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (i * per >= count) break;
+    const float x = exp2f(s_m[i] - m);
+    l += x * s_l[i];
+#pragma unroll
+    for (int d = 0; d < DIM / 32; ++d) o[d] += x * s_o[i][d * 32 + lane];
+  }
+  paged_finish<DIM>(a, join.request, kv * w.group + row0 + row, lane, o, m, l, paged_out_scale(a));
+}
+
+// ---------------------------------------------------------------------------- host
+static bool paged_tensor_dim(int dim) { return dim == 64 || dim == 128 || dim == 256; }
+// query heads of a row tile: 16 where more than 8 share a key/value head, which then is read once for them; heads of 256
+// values in two tiles do not fit the registers
+static int paged_rows_of(int group, int dim) { return group <= 8 || dim == 256 ? 8 : 16; }
+static size_t paged_align(size_t n) { return (n + 255) / 256 * 256; }
+
+size_t paged_attention_workspace_bytes_impl(int64_t requests, int heads, int kv_heads, int dim, int cache_dtype) {
+  (void)requests;  // (rows are joined per CTA, whatever the number of requests)
+  (void)cache_dtype;
+  if (!paged_tensor_dim(dim)) return 0;
+  const size_t part = sizeof(float) * paged_rows_of(heads / kv_heads, dim) * (dim + 2);
+  const size_t warps = dim == 256 ? 4 : 8;
+  return paged_align(sizeof(PagedJoin) * kPagedGrid) + paged_align(part * 2 * kPagedGrid) + paged_align(part * warps * kPagedGrid);
+}
+
+template <int DIM, int FMT, int NT>
+static int paged_launch(const b200q_paged_attention_args& a, cudaStream_t st) {
+  using Tile = PagedTile<DIM, FMT, NT>;
+  auto kernel = paged_attention_kernel<DIM, FMT, NT>;
+  static std::atomic<int> ready[kMaxDevices];
+  const int dev = current_device_index();
+  if (dev < 0) return B200Q_ERR_CUDA;
+  if (!ready[dev].load(std::memory_order_acquire)) {
+    B200Q_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(Tile::kWarps * Tile::kRing + 4 * kPagedMaxRequests)));
+    ready[dev].store(1, std::memory_order_release);
+  }
+  PagedWork w;
+  w.group = a.heads / a.kv_heads;
+  w.row_tiles = (w.group + Tile::kRows - 1) / Tile::kRows;
+  w.heads_per_request = a.kv_heads * w.row_tiles;
+  uint8_t* p = static_cast<uint8_t*>(a.workspace);
+  w.joins = reinterpret_cast<PagedJoin*>(p);
+  p += paged_align(sizeof(PagedJoin) * kPagedGrid);
+  w.cta_part = reinterpret_cast<float*>(p);
+  p += paged_align(sizeof(float) * Tile::kPart * 2 * kPagedGrid);
+  w.warp_part = reinterpret_cast<float*>(p);
+  // no more CTAs than the longest rows that the tables can hold would fill
+  const int64_t most = a.requests * ((a.table_width * a.page_size + 15) / 16) * w.heads_per_request;
+  int64_t grid = (most + Tile::kWarps * kPagedMinSteps - 1) / (Tile::kWarps * kPagedMinSteps);
+  if (grid < 1) grid = 1;
+  if (grid > kPagedGrid) grid = kPagedGrid;
+  launch_dependent(kernel, dim3((unsigned)grid), dim3(32 * Tile::kWarps), Tile::kWarps * Tile::kRing + 4 * (size_t)a.requests, st, a, w);
+  B200Q_LAUNCH_CHECK();
+  if (grid > 1) {
+    launch_dependent(paged_join_kernel<DIM, 8 * NT>, dim3((unsigned)grid, 8 * NT), dim3(128), 0, st, a, w);
+    B200Q_LAUNCH_CHECK();
+  }
+  return B200Q_OK;
+}
+
+template <int DIM, int FMT>
+static int paged_launch_rows(const b200q_paged_attention_args& a, cudaStream_t st) {
+  if constexpr (DIM < 256) {
+    if (paged_rows_of(a.heads / a.kv_heads, DIM) == 16) return paged_launch<DIM, FMT, 2>(a, st);
+  }
+  return paged_launch<DIM, FMT, 1>(a, st);
+}
+template <int DIM>
+static int paged_launch_dtype(const b200q_paged_attention_args& a, cudaStream_t st) {
+  switch (a.cache_dtype) {
+    case B200Q_BF16: return paged_launch_rows<DIM, B200Q_BF16>(a, st);
+    case B200Q_E4M3: return paged_launch_rows<DIM, B200Q_E4M3>(a, st);
+    default: return paged_launch_rows<DIM, B200Q_E5M2>(a, st);
+  }
+}
+
+static bool paged_fits_tensor_cores(const b200q_paged_attention_args& a) {
+  if (a.force_plain || !paged_tensor_dim(a.dim) || a.page_size % 16 || a.num_pages == 0) return false;
+  const int64_t size = a.cache_dtype == B200Q_BF16 ? 2 : 1;
+  for (const void* p : {a.q, a.k_cache, a.v_cache, static_cast<const void*>(a.out)})
+    if (reinterpret_cast<uintptr_t>(p) % 16) return false;
+  for (int64_t s : {a.k_page_stride, a.k_slot_stride, a.k_head_stride, a.v_page_stride, a.v_slot_stride, a.v_head_stride})
+    if (s * size % 16) return false;
+  return a.q_token_stride % 8 == 0 && a.q_head_stride % 8 == 0;
+}
 
 int paged_attention_impl(const b200q_paged_attention_args& a, cudaStream_t st) {
+  if (paged_fits_tensor_cores(a)) {
+    if (a.requests > kPagedMaxRequests) return B200Q_ERR_TOO_LARGE;
+    // (table_width and page_size are below 2^31)
+    if (a.table_width > 0 && a.page_size / 16 > ((int64_t)INT32_MAX / a.requests) / a.table_width) return B200Q_ERR_TOO_LARGE;
+    if (a.workspace_bytes < paged_attention_workspace_bytes_impl(a.requests, a.heads, a.kv_heads, a.dim, a.cache_dtype) || !a.workspace ||
+        reinterpret_cast<uintptr_t>(a.workspace) % 16)
+      return B200Q_ERR_BAD_ARGUMENT;
+    if (a.dim == 64) return paged_launch_dtype<64>(a, st);
+    if (a.dim == 128) return paged_launch_dtype<128>(a, st);
+    return paged_launch_dtype<256>(a, st);
+  }
   const int64_t blocks = a.requests * a.heads;
   if (blocks > 0x7FFFFFFF) return B200Q_ERR_TOO_LARGE;
   launch_dependent(paged_attention_plain_kernel, dim3((unsigned)blocks), dim3(kPlainThreads), 0, st, a);
