@@ -2,6 +2,8 @@
 //   s_j = softmax_scale * k_scale_inv * <q, k_j>,  j in [max(0, len - window), len);   p = softmax(s)
 //   out = v_scale_inv * sum_j p_j v_j,   lse = log sum_j exp(s_j);   nothing to see: out = 0, lse = -inf.
 #include "paged.cuh"
+#include "tcgen05_ptx.cuh"
+#include "tma_host.cuh"
 
 namespace b200q {
 
@@ -16,9 +18,9 @@ __device__ __forceinline__ void paged_store(void* out, int dtype, int64_t at, fl
   else static_cast<uint8_t*>(out)[at] = (uint8_t)(cvt_fp8x2<B200Q_E4M3>(v, 0.f) & 0xFFu);
 }
 // tokens of the request that its table can hold
-__device__ __forceinline__ int64_t paged_length(const b200q_paged_attention_args& a, int64_t b) {
+__device__ __forceinline__ int paged_length(const b200q_paged_attention_args& a, int64_t b) {
   const int64_t most = a.table_width * a.page_size;
-  return min((int64_t)max(a.kv_lens[b], 0), most);
+  return (int)min((int64_t)max(a.kv_lens[b], 0), most);
 }
 
 // ---------------------------------------------------------------------------- plain
@@ -102,13 +104,15 @@ __global__ void __launch_bounds__(kPlainThreads) paged_attention_plain_kernel(co
 // products are m16n8k16 matrix instructions with the CACHE as the operand of 16 rows (keys of K, dimensions of V) and the heads as
 // the 8 columns, which fills the instruction when eight heads share a key/value head.
 //
-// A warp works on steps of 16 keys.  Its lanes copy the operands' fragments, 16 bytes at a time, straight from the pages
-// into a ring of its own in shared memory (cp.async) and each lane reads back only what it copied itself: no barrier, no
-// bank conflict, no transposition.  Lane (g = lane / 4, t = lane % 4) owns
-//   of K: keys g and g + 8, bytes 64 c + 16 t ... + 15 of their rows   (the dimensions of a dot product may come in any order:
-//         the queries are laid out to match)
-//   of V: keys 2t, 2t + 1, 2t + 8, 2t + 9, bytes (8 c + g) * 16 ... + 15  (the dimensions are the rows of the second product, which
-//         may come in any order too)
+// A warp works on steps of 16 keys.  It has a ring of its own in shared memory that TMA fills, a box of 16 keys and 128 bytes
+// at a time (cp.async of the same bytes, 16 at a time, ends at 4.4 TB/s), and nothing to wait for but its own copies.
+// Lane (g = lane / 4, t = lane % 4) reads the operands' fragments as they lie:
+//   of K: keys R(g) and R(g) + 8, bytes 64 c + 16 t ... + 15 of their rows   (the dimensions of a dot product may come in any
+//         order: the queries are laid out to match; so may the keys, as long as V follows)
+//   of V: the keys of rows 2t, 2t + 1, 2t + 8, 2t + 9, that is t, t + 4, t + 8, t + 12, bytes (8 c + R(g)) * 16 ... + 15  (the
+//         dimensions are the rows of the second product, which may come in any order too)
+// R exchanges bits (0, 4, 1, 5, 2, 6, 3, 7): with it the eight lanes of a 16-byte access lie in different banks of the
+// swizzled tile.
 // fp8 values become f16 exactly; the probabilities are rounded to f16 (11 bits, scaled by 2^7 so that the small ones stay normal).
 // For a bf16 cache they are split into two bf16 terms (16 bits) that take a product each.  Queries meet fp8 keys as f16, scaled
 // by a power of two per head, which is exact over 2^22 of a head's largest value.
@@ -123,18 +127,24 @@ constexpr int kPagedMinSteps = 2;     // a warp gets at least this many steps wh
 constexpr float kPagedShift = 7.f;    // probabilities are held relative to 2^(maximum - 7) ...
 constexpr float kPagedRescale = 15.f; // ... and the maximum is raised when one would pass 2^15 (f16 ends at 2^16)
 constexpr float kPagedNoMax = -3.0e38f;
+constexpr int kPagedErrCopy = 801;  // status code: a copy of keys and values did not arrive
 
 template <int DIM, int FMT, int NT>
 struct PagedTile {
   static constexpr int kElt = FMT == B200Q_BF16 ? 2 : 1;
   static constexpr int kRow = DIM * kElt;           // bytes of a key
   static constexpr int kStage = 2 * 16 * kRow;      // keys and values of a step
-  static constexpr int kWarps = DIM == 256 ? 4 : 8;
+  #ifndef PW
+#define PW 8
+#endif
+  static constexpr int kWarps = DIM == 256 ? 4 : NT == 1 && kStage <= 4096 ? PW : 8;
   static constexpr int kStages = kPagedRingBytes / kWarps / kStage < 8 ? kPagedRingBytes / kWarps / kStage : 8;
   static constexpr int kKChunks = kRow / 64;        // 16-byte pieces of a key per lane
   static constexpr int kVPiece = kRow / 8 < 16 ? 8 : 16;
   static constexpr int kVChunks = kRow / 8 / kVPiece;
   static constexpr int kVPer = kVPiece / kElt;      // values of a piece
+  static constexpr int kBox = kRow < 128 ? kRow : 128;  // bytes of a key in one copy
+  static constexpr int kBoxes = kRow / kBox;
   static constexpr int kTiles = DIM / 16;           // k-steps of the first product, row tiles of the second
   static constexpr int kRows = 8 * NT;              // query heads
   static constexpr int kPart = kRows * (DIM + 2);   // floats of a partial result: output, maxima, sums
@@ -154,18 +164,17 @@ struct PagedWork {
   PagedJoin* joins;       // [grid]
   float* cta_part;        // [grid][2][kPart]: rows from the CTA before, rows into the CTA behind
   float* warp_part;       // [grid][warps][kPart]: rows from the warp before that end inside a warp's run
+  int* status;
 };
 
 __device__ __forceinline__ uint32_t paged_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-template <int BYTES>
-__device__ __forceinline__ void paged_copy(uint32_t dst, const void* src, bool there) {
-  const int n = there ? BYTES : 0;  // (nothing is read, and zeros are written, where there is no key)
-  if (BYTES == 16) asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-  else asm volatile("cp.async.ca.shared.global.L2::128B [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+// a box of a cache: `kBox` bytes from x on of 16 tokens' head
+__device__ __forceinline__ void paged_copy(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int head, int slot, int page) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(head), "r"(slot), "r"(page)
+      : "memory");
 }
-__device__ __forceinline__ void paged_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void paged_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ uint4 paged_lds16(uint32_t at) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
@@ -224,12 +233,12 @@ __device__ __forceinline__ float paged_out_scale(const b200q_paged_attention_arg
 
 // the keys that a request's token sees: [first, len); its steps begin at a multiple of 16
 struct PagedSpan {
-  int64_t len, first;
+  int len, first;
   __device__ __forceinline__ PagedSpan(const b200q_paged_attention_args& a, int b) {
     len = paged_length(a, b);
-    first = a.window > 0 && len > a.window ? len - a.window : 0;
+    first = a.window > 0 && len > a.window ? len - (int)a.window : 0;
   }
-  __device__ __forceinline__ int steps() const { return (int)((len + 15) / 16 - first / 16); }
+  __device__ __forceinline__ int steps() const { return (int)(((uint32_t)len + 15u) / 16u) - first / 16; }
 };
 
 // A place in the list of steps.
@@ -292,7 +301,7 @@ struct PagedAcc {
   }
   // calls f(head row, first dimension, four values) for all that the lane holds
   template <typename F>
-  __device__ __forceinline__ void each4(int g, int t, F f) const {
+  __device__ __forceinline__ void each4(int piece, int t, F f) const {
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -300,11 +309,11 @@ struct PagedAcc {
 #pragma unroll
         for (int e = 0; e < Tile::kVChunks * Tile::kVPer; e += 4) {
           const float v[4] = {o[e / 2][n][i], o[e / 2][n][i + 2], o[e / 2 + 1][n][i], o[e / 2 + 1][n][i + 2]};
-          f(8 * n + 2 * t + i, (e / Tile::kVPer * 8 + g) * Tile::kVPer + e % Tile::kVPer, v, n, i);
+          f(8 * n + 2 * t + i, (e / Tile::kVPer * 8 + piece) * Tile::kVPer + e % Tile::kVPer, v, n, i);
         }
   }
-  __device__ __forceinline__ void save(float* to, int g, int t) const {
-    each4(g, t, [&](int row, int d, const float (&v)[4], int, int) {
+  __device__ __forceinline__ void save(float* to, int g, int piece, int t) const {
+    each4(piece, t, [&](int row, int d, const float (&v)[4], int, int) {
       *reinterpret_cast<float4*>(to + row * DIM + d) = make_float4(v[0], v[1], v[2], v[3]);
     });
     if (g == 0) {
@@ -349,15 +358,29 @@ __device__ __forceinline__ void paged_finish(const b200q_paged_attention_args& a
 
 template <int DIM, int FMT, int NT>
 __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
-    paged_attention_kernel(const b200q_paged_attention_args a, const PagedWork w) {
+    paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                           const b200q_paged_attention_args a, const PagedWork w) {
   using Tile = PagedTile<DIM, FMT, NT>;
   constexpr int kWarps = Tile::kWarps, kStages = Tile::kStages, kTiles = Tile::kTiles, kElt = Tile::kElt;
-  extern __shared__ __align__(16) uint8_t s_ring[];  // [warps][kRing], then the prefix sums
+  extern __shared__ __align__(1024) uint8_t s_raw[];
+  uint8_t* const s_ring = s_raw + (0u - paged_smem(s_raw) & 1023u);  // [warps][kRing] (swizzled tiles repeat every 1024 bytes), then the prefix sums
+  __shared__ __align__(8) uint64_t s_bars[kWarps * kStages];
+  __shared__ int s_abort;
   __shared__ int s_sum[kWarps];
   __shared__ int s_final[kWarps], s_from[kWarps], s_done[kWarps], s_b[kWarps], s_sub[kWarps];
   int* prefix = reinterpret_cast<int*>(s_ring + kWarps * Tile::kRing);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int requests = (int)a.requests, heads = w.heads_per_request;
+  const uint32_t bars = paged_smem(s_bars + warp * kStages);
+  if (lane == 0) {
+    for (int s = 0; s < kStages; ++s) ptx::mbar_init(bars + 8 * s, 1);
+    ptx::fence_barrier_init();
+  }
+  if (tid == 0) {
+    s_abort = 0;
+    ptx::tma_prefetch_desc(&map_k);
+    ptx::tma_prefetch_desc(&map_v);
+  }
   pdl_enter();
 
   // ---- the list of steps
@@ -430,87 +453,62 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
     PagedCursor pc;
     pc.locate(prefix, requests, heads, first_step);
     cc = pc;
-    const int ps = (int)a.page_size;
-    const uint8_t* const k_base = static_cast<const uint8_t*>(a.k_cache);
-    const uint8_t* const v_base = static_cast<const uint8_t*>(a.v_cache);
-    const int64_t k_lane = (int64_t)g * a.k_slot_stride * kElt + 16 * t, k_eight = 8 * a.k_slot_stride * kElt;
-    const int64_t v_slot = a.v_slot_stride * kElt, v_lane = 2 * t * v_slot + g * Tile::kVPiece;
-    int64_t p_pos, p_len, p_first;  // of the step that is copied next
-    int p_off, p_page;              // its place in its page, and the page
-    int64_t p_index;                // of the page in the table
-    uint32_t bad = 0;               // bit s: the step in stage s has no page
-    auto page_at = [&](int b, int64_t index) {  // steps lie within a request's length, which its table covers
-      const int p = a.block_table[(int64_t)b * a.table_stride + index];
-      return p >= 0 && p < a.num_pages ? p : -1;
+    const int steps_per_page = (int)a.page_size / 16;
+    const int32_t* p_table;
+    int p_todo = todo, p_left, p_page_left, p_page, p_slot, p_kv;  // steps: to copy, of the row, of the page; where the next one is
+    uint32_t bad = 0;  // bit s: the step in stage s has no page
+    auto enter_page = [&](int step_of_page) {  // (steps lie within a request's length, which its table covers)
+      const int p = *p_table;
+      p_page = (uint32_t)p < (uint32_t)a.num_pages ? p : (int)a.num_pages;  // (behind the last page a copy brings zeros)
+      p_slot = 16 * step_of_page;
+      p_page_left = steps_per_page - step_of_page;
     };
     auto enter_row = [&] {
       const PagedSpan span(a, pc.b);
-      p_len = span.len;
-      p_first = span.first;
-      p_pos = span.first / 16 * 16 + (int64_t)pc.step * 16;
-      p_index = p_pos / ps;
-      p_off = (int)(p_pos - p_index * ps);
-      p_page = page_at(pc.b, p_index);
+      const int at = span.first / 16 + pc.step, index = at / steps_per_page;  // in steps
+      p_kv = pc.sub / w.row_tiles;
+      p_left = pc.steps - pc.step;
+      p_table = a.block_table + (int64_t)pc.b * a.table_stride + index;
+      enter_page(at - index * steps_per_page);
     };
-    int copied = 0;
     auto copy_step = [&](int stage) {
-      if (copied < todo) {
-        const uint32_t dst = ring + stage * Tile::kStage + lane * 16;
-        const uint32_t dst_v = ring + stage * Tile::kStage + 16 * Tile::kRow + lane * Tile::kVPiece;
-        const bool page_there = p_page >= 0;
-        bad = (bad & ~(1u << stage)) | (page_there ? 0u : 1u << stage);
-        const int kv = pc.sub / w.row_tiles;
-        const int64_t page = page_there ? p_page : 0;
-        const uint8_t* k = k_base + ((page * a.k_page_stride + p_off * a.k_slot_stride + kv * a.k_head_stride) * kElt + k_lane);
-        const uint8_t* v = v_base + ((page * a.v_page_stride + p_off * a.v_slot_stride + kv * a.v_head_stride) * kElt + v_lane);
-        auto there = [&](int key) { return page_there && p_pos + key < p_len && p_pos + key >= p_first; };
+      if (p_todo == 0) return;
+      const uint32_t bar = bars + 8 * stage, dst = ring + stage * Tile::kStage;
+      bad = (bad & ~(1u << stage)) | ((uint32_t)(p_page == (int)a.num_pages) << stage);
+      if (ptx::elect_one()) {
+        ptx::mbar_arrive_expect_tx(bar, Tile::kStage);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const bool ok = there(8 * h + g);
-          const uint8_t* src = ok ? k + h * k_eight : k_base;
+        for (int i = 0; i < Tile::kBoxes; ++i) paged_copy(dst + i * 16 * Tile::kBox, &map_k, bar, i * Tile::kBox, p_kv, p_slot, p_page);
 #pragma unroll
-          for (int i = 0; i < Tile::kKChunks; ++i) paged_copy<16>(dst + (h * Tile::kKChunks + i) * 512, src + 64 * i, ok);
-        }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int key = (q >> 1) * 8 + (q & 1);
-          const bool ok = there(key + 2 * t);
-          const uint8_t* src = ok ? v + key * v_slot : v_base;
-#pragma unroll
-          for (int i = 0; i < Tile::kVChunks; ++i)
-            paged_copy<Tile::kVPiece>(dst_v + (q * Tile::kVChunks + i) * 32 * Tile::kVPiece, src + 8 * Tile::kVPiece * i, ok);
-        }
-        if (++copied < todo) {
-          if (++pc.step < pc.steps) {
-            p_pos += 16;
-            p_off += 16;
-            if (p_off >= ps) {
-              p_off = 0;
-              p_page = page_at(pc.b, ++p_index);
-            }
-          } else if (pc.next_row(prefix, requests, heads)) {
-            enter_row();
-          }
-        }
+        for (int i = 0; i < Tile::kBoxes; ++i)
+          paged_copy(dst + 16 * Tile::kRow + i * 16 * Tile::kBox, &map_v, bar, i * Tile::kBox, p_kv, p_slot, p_page);
       }
-      paged_commit();
+      --p_todo;
+      if (--p_left > 0) {
+        p_slot += 16;
+        if (--p_page_left == 0 && p_todo > 0) {
+          ++p_table;
+          enter_page(0);
+        }
+      } else if (p_todo > 0 && pc.next_row(prefix, requests, heads)) {
+        enter_row();
+      }
     };
     enter_row();
-#pragma unroll
     for (int s = 0; s < kStages - 1; ++s) copy_step(s);
 
     // ---- the products
     PagedAcc<DIM, FMT, NT> acc;
     uint32_t qf[kTiles][NT][2];
     float coef[NT][2];  // scores in powers of two for heads 2t, 2t + 1
-    int64_t c_len = 0, c_first = 0, c_pos = 0;
+    int c_lo = 0, c_end = 0, c_left = 0;  // keys of this step before c_lo are not seen, nor those of the row's last step from c_end on
     const float score_scale = a.softmax_scale * (a.k_scale_inv ? *a.k_scale_inv : 1.f) * 1.44269504088896341f;
     const __nv_bfloat16* const q = static_cast<const __nv_bfloat16*>(a.q);
     auto begin_row = [&] {
       const PagedSpan span(a, cc.b);
-      c_len = span.len;
-      c_first = span.first;
-      c_pos = span.first / 16 * 16 + (int64_t)cc.step * 16;
+      c_lo = cc.step == 0 ? span.first % 16 : 0;
+      c_end = (span.len - 1) % 16 + 1;
+      c_left = cc.steps - cc.step;
       from_here = cc.step == 0;
       acc.clear();
       const int kv = cc.sub / w.row_tiles, row0 = (cc.sub - kv * w.row_tiles) * Tile::kRows;
@@ -558,11 +556,23 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
     };
     begin_row();
 
+    // where the lane's pieces are in a stage: of keys R(g) + 8 h in box c / 2 at k_at ^ 64 (c % 2); of values key t + 4 i + 8 h
+    const int rg = (g >> 1) | ((g & 1) << 2);
+    const uint32_t k_at = Tile::kBox == 128 ? rg * 128 + ((t ^ rg) << 4) : rg * 64 + ((t ^ (rg >> 1)) << 4);
+    const uint32_t v_at = Tile::kBox == 128 ? t * 128 + ((rg ^ t) << 4) : t * 64 + (((g >> 1) ^ (t >> 1)) << 4) + (g & 1) * 8;
     int stage = 0;
+    uint32_t phase = 0;
     for (int done = 0; done < todo; ++done) {
-      paged_wait<kStages - 2>();
-      const uint32_t src = ring + stage * Tile::kStage + lane * 16;
-      const uint32_t src_v = ring + stage * Tile::kStage + 16 * Tile::kRow + lane * Tile::kVPiece;
+      if (!ptx::mbar_wait_uniform(bars + 8 * stage, phase, &s_abort, w.status, kPagedErrCopy)) {
+        // gives up: waits for the other copies in flight, as far as they come, and leaves
+        for (int s = 1; s < kStages && done + s < todo - p_todo; ++s) {
+          const int next = (stage + s) % kStages;
+          for (int i = 0; i < 4096 && !ptx::mbar_try_wait(bars + 8 * next, phase ^ (stage + s >= kStages)); ++i) __nanosleep(64);
+        }
+        final_part = from_here = 0;
+        break;
+      }
+      const uint32_t src = ring + stage * Tile::kStage, src_v = src + 16 * Tile::kRow + v_at;
       // scores: keys x heads
       float s[NT][4], s2[NT][4];
 #pragma unroll
@@ -571,7 +581,8 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
         for (int i = 0; i < 4; ++i) s[n][i] = s2[n][i] = 0.f;
 #pragma unroll
       for (int i = 0; i < Tile::kKChunks; ++i) {
-        const uint4 lo4 = paged_lds16(src + i * 512), hi4 = paged_lds16(src + (Tile::kKChunks + i) * 512);
+        const uint32_t at = src + (i >> 1) * 16 * Tile::kBox + (k_at ^ (64 * (i & 1)));
+        const uint4 lo4 = paged_lds16(at), hi4 = paged_lds16(at + 8 * Tile::kBox);
         const uint32_t lo[4] = {lo4.x, lo4.y, lo4.z, lo4.w}, hi[4] = {hi4.x, hi4.y, hi4.z, hi4.w};
         if (FMT == B200Q_BF16) {
 #pragma unroll
@@ -591,10 +602,12 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
         }
       }
       const bool nowhere = bad >> stage & 1u;
-      bool ok0 = true, ok1 = true;  // keys g, g + 8
-      if (nowhere || c_pos + 16 > c_len || c_pos < c_first) {
-        ok0 = !nowhere && c_pos + g < c_len && c_pos + g >= c_first;
-        ok1 = !nowhere && c_pos + 8 + g < c_len && c_pos + 8 + g >= c_first;
+      const bool edge = nowhere || c_lo > 0 || c_left == 1;  // some of its keys are not to be seen
+      const int lo = nowhere ? 16 : c_lo, end = c_left == 1 ? c_end : 16;
+      bool ok0 = true, ok1 = true;  // keys R(g), R(g) + 8
+      if (edge) {
+        ok0 = rg >= lo && rg < end;
+        ok1 = 8 + rg >= lo && 8 + rg < end;
       }
       uint32_t p_hi[NT][2], p_lo[NT][2];
 #pragma unroll
@@ -643,18 +656,28 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
         }
       }
       // output: dimensions x heads
+      // the piece of the key four rows on: the swizzle turns its place by 64 (rows of 128 bytes) or 32 bytes (of 64)
+      auto v_four = [&](uint32_t at) { return (at + 4 * Tile::kBox) ^ (Tile::kBox == 128 ? 64 : 32); };
 #pragma unroll
       for (int i = 0; i < Tile::kVChunks; ++i) {
         uint32_t v[4][Tile::kVPiece / 4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const uint32_t at = src_v + (k * Tile::kVChunks + i) * 32 * Tile::kVPiece;
+          // key t + 4 (k % 2) + 8 (k / 2): four rows on, the swizzled piece is the one across
+          const uint32_t at = src_v + i * 16 * Tile::kBox + (k >> 1) * 8 * Tile::kBox;
           if (Tile::kVPiece == 16) {
-            const uint4 x = paged_lds16(at);
+            const uint4 x = paged_lds16(k & 1 ? v_four(at) : at);
             v[k][0] = x.x; v[k][1] = x.y; v[k][Tile::kVPiece / 4 - 2] = x.z; v[k][Tile::kVPiece / 4 - 1] = x.w;
           } else {
-            const uint2 x = paged_lds8(at);
+            const uint2 x = paged_lds8(k & 1 ? v_four(at) : at);
             v[k][0] = x.x; v[k][1] = x.y;
+          }
+          if (edge) {  // whatever lies there, 0 times it must be 0
+            const int key = t + 4 * (k & 1) + 8 * (k >> 1);
+            if (key < lo || key >= end) {
+#pragma unroll
+              for (int j = 0; j < Tile::kVPiece / 4; ++j) v[k][j] = 0;
+            }
           }
         }
 #pragma unroll
@@ -682,16 +705,20 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
         }
       }
       // the stage of the step before this one is free
+      __syncwarp();
       copy_step(stage == 0 ? kStages - 1 : stage - 1);
-      if (++stage == kStages) stage = 0;
-      c_pos += 16;
+      if (++stage == kStages) {
+        stage = 0;
+        phase ^= 1;
+      }
+      c_lo = 0;
 
-      const bool row_end = ++cc.step == cc.steps, last = done + 1 == todo;
+      const bool row_end = --c_left == 0, last = done + 1 == todo;
       if (row_end || last) {
         acc.sum_lanes();
         if (row_end && from_here) {
           const int kv = cc.sub / w.row_tiles, row0 = (cc.sub - kv * w.row_tiles) * Tile::kRows;
-          acc.each4(g, t, [&](int row, int d, const float (&v)[4], int n, int i) {
+          acc.each4((Tile::kVPiece == 16 ? rg : g), t, [&](int row, int d, const float (&v)[4], int n, int i) {
             if (row0 + row >= w.group) return;
             const float inv = acc.l[n][i] == 0.f ? 0.f : out_scale / acc.l[n][i];
             const float r[4] = {v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
@@ -707,13 +734,12 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
               }
           }
         } else if (last) {
-          paged_wait<0>();
           __syncwarp();
-          acc.save(part_smem, g, t);
+          acc.save(part_smem, g, (Tile::kVPiece == 16 ? rg : g), t);
           final_part = 1;
           row_done = row_end;
         } else {
-          acc.save(w.warp_part + ((int64_t)c * kWarps + warp) * Tile::kPart, g, t);
+          acc.save(w.warp_part + ((int64_t)c * kWarps + warp) * Tile::kPart, g, (Tile::kVPiece == 16 ? rg : g), t);
         }
         if (!last && cc.next_row(prefix, requests, heads)) begin_row();
       }
@@ -837,8 +863,26 @@ size_t paged_attention_workspace_bytes_impl(int64_t requests, int heads, int kv_
   (void)cache_dtype;
   if (!paged_tensor_dim(dim)) return 0;
   const size_t part = sizeof(float) * paged_rows_of(heads / kv_heads, dim) * (dim + 2);
-  const size_t warps = dim == 256 ? 4 : 8;
+  const size_t warps = 16;
   return paged_align(sizeof(PagedJoin) * kPagedGrid) + paged_align(part * 2 * kPagedGrid) + paged_align(part * warps * kPagedGrid);
+}
+
+// A cache as [pages][slots][heads][bytes of a head], whatever the order of its strides, in boxes of 16 slots
+static int paged_map(CUtensorMap* map, const void* base, const b200q_paged_attention_args& a, int64_t size, int64_t page_stride, int64_t slot_stride,
+                     int64_t head_stride) {
+  EncodeTiledFn enc = get_encode_fn();
+  if (!enc) return B200Q_ERR_CUDA;
+  const cuuint64_t row = (cuuint64_t)(a.dim * size);
+  const cuuint32_t inner = row < 128 ? (cuuint32_t)row : 128;
+  // (the stride of a dimension of one entry is never used, and may be anything in the caller's view)
+  const cuuint64_t dims[4] = {row, (cuuint64_t)a.kv_heads, (cuuint64_t)a.page_size, (cuuint64_t)a.num_pages};
+  const cuuint64_t strides[3] = {a.kv_heads > 1 ? (cuuint64_t)(head_stride * size) : row, (cuuint64_t)(slot_stride * size),
+                                 a.num_pages > 1 ? (cuuint64_t)(page_stride * size) : row};
+  const cuuint32_t box[4] = {inner, 1, 16, 1}, step[4] = {1, 1, 1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         inner == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? B200Q_OK : B200Q_ERR_UNSUPPORTED;
 }
 
 template <int DIM, int FMT, int NT>
@@ -849,10 +893,15 @@ static int paged_launch(const b200q_paged_attention_args& a, cudaStream_t st) {
   const int dev = current_device_index();
   if (dev < 0) return B200Q_ERR_CUDA;
   if (!ready[dev].load(std::memory_order_acquire)) {
-    B200Q_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(Tile::kWarps * Tile::kRing + 4 * kPagedMaxRequests)));
+    B200Q_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(Tile::kWarps * Tile::kRing + 1024 + 4 * kPagedMaxRequests)));
     ready[dev].store(1, std::memory_order_release);
   }
+  CUtensorMap map_k, map_v;
+  if (int rc = paged_map(&map_k, a.k_cache, a, Tile::kElt, a.k_page_stride, a.k_slot_stride, a.k_head_stride)) return rc;
+  if (int rc = paged_map(&map_v, a.v_cache, a, Tile::kElt, a.v_page_stride, a.v_slot_stride, a.v_head_stride)) return rc;
   PagedWork w;
+  w.status = device_status_ptr();
+  if (!w.status) return B200Q_ERR_CUDA;
   w.group = a.heads / a.kv_heads;
   w.row_tiles = (w.group + Tile::kRows - 1) / Tile::kRows;
   w.heads_per_request = a.kv_heads * w.row_tiles;
@@ -867,7 +916,7 @@ static int paged_launch(const b200q_paged_attention_args& a, cudaStream_t st) {
   int64_t grid = (most + Tile::kWarps * kPagedMinSteps - 1) / (Tile::kWarps * kPagedMinSteps);
   if (grid < 1) grid = 1;
   if (grid > kPagedGrid) grid = kPagedGrid;
-  launch_dependent(kernel, dim3((unsigned)grid), dim3(32 * Tile::kWarps), Tile::kWarps * Tile::kRing + 4 * (size_t)a.requests, st, a, w);
+  launch_dependent(kernel, dim3((unsigned)grid), dim3(32 * Tile::kWarps), Tile::kWarps * Tile::kRing + 1024 + 4 * (size_t)a.requests, st, map_k, map_v, a, w);
   B200Q_LAUNCH_CHECK();
   if (grid > 1) {
     launch_dependent(paged_join_kernel<DIM, 8 * NT>, dim3((unsigned)grid, 8 * NT), dim3(128), 0, st, a, w);
@@ -898,7 +947,7 @@ static bool paged_fits_tensor_cores(const b200q_paged_attention_args& a) {
   for (const void* p : {a.q, a.k_cache, a.v_cache, static_cast<const void*>(a.out)})
     if (reinterpret_cast<uintptr_t>(p) % 16) return false;
   for (int64_t s : {a.k_page_stride, a.k_slot_stride, a.k_head_stride, a.v_page_stride, a.v_slot_stride, a.v_head_stride})
-    if (s * size % 16) return false;
+    if (s < 0 || s * size % 16) return false;
   return a.q_token_stride % 8 == 0 && a.q_head_stride % 8 == 0;
 }
 
@@ -910,9 +959,8 @@ int paged_attention_impl(const b200q_paged_attention_args& a, cudaStream_t st) {
     if (a.workspace_bytes < paged_attention_workspace_bytes_impl(a.requests, a.heads, a.kv_heads, a.dim, a.cache_dtype) || !a.workspace ||
         reinterpret_cast<uintptr_t>(a.workspace) % 16)
       return B200Q_ERR_BAD_ARGUMENT;
-    if (a.dim == 64) return paged_launch_dtype<64>(a, st);
-    if (a.dim == 128) return paged_launch_dtype<128>(a, st);
-    return paged_launch_dtype<256>(a, st);
+    const int rc = a.dim == 64 ? paged_launch_dtype<64>(a, st) : a.dim == 128 ? paged_launch_dtype<128>(a, st) : paged_launch_dtype<256>(a, st);
+    if (rc != B200Q_ERR_UNSUPPORTED) return rc;  // (a layout that has no tensor map takes the plain kernel)
   }
   const int64_t blocks = a.requests * a.heads;
   if (blocks > 0x7FFFFFFF) return B200Q_ERR_TOO_LARGE;
