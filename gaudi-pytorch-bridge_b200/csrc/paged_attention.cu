@@ -117,16 +117,19 @@ __global__ void __launch_bounds__(kPlainThreads) paged_attention_plain_kernel(co
 // For a bf16 cache they are split into two bf16 terms (16 bits) that take a product each.  Queries meet fp8 keys as f16, scaled
 // by a power of two per head, which is exact over 2^22 of a head's largest value.
 //
-// Work is the list of all steps (request-major, then key/value head, then the length), cut into equal runs for the CTAs and
-// then for their warps, so that ragged lengths and few requests load every SM alike.  A run may begin or end inside a row of
-// steps: such partial results (maximum, sum, output) are joined in the CTA, and, where a row goes on in another CTA, by a second
-// kernel.
+// Work is the list of all steps (request-major, then key/value head, then the length), cut into equal runs for the CTAs, so that
+// ragged lengths and few requests load every SM alike.  In a CTA `lanes` warps take neighbouring heads of the same keys -- the
+// whole row of a token is read at one time, which is worth 5.0 -> 6.4 TB/s where the heads of a token lie together -- and the
+// kWarps / lanes groups of such warps cut the run again.  A run may begin or end inside a row of steps: such partial results
+// (maximum, sum, output) are joined in the CTA, and, where a row goes on in another CTA, by a second kernel.
 constexpr int kPagedGrid = kNumSMs;
 constexpr int kPagedRingBytes = 192 * 1024;
+constexpr int kPagedLaneSteps = 24;   // a warp's steps from which on heads go side by side
 constexpr int kPagedMinSteps = 2;     // a warp gets at least this many steps while there are enough for the others
 constexpr float kPagedShift = 7.f;    // probabilities are held relative to 2^(maximum - 7) ...
 constexpr float kPagedRescale = 15.f; // ... and the maximum is raised when one would pass 2^15 (f16 ends at 2^16)
 constexpr float kPagedNoMax = -3.0e38f;
+constexpr int kPagedLengthsHere = (int)kPagedMaxRequests / 2;  // up to so many requests' lengths lie in shared memory beside the sums
 constexpr int kPagedErrCopy = 801;  // status code: a copy of keys and values did not arrive
 
 template <int DIM, int FMT, int NT>
@@ -134,10 +137,7 @@ struct PagedTile {
   static constexpr int kElt = FMT == B200Q_BF16 ? 2 : 1;
   static constexpr int kRow = DIM * kElt;           // bytes of a key
   static constexpr int kStage = 2 * 16 * kRow;      // keys and values of a step
-  #ifndef PW
-#define PW 8
-#endif
-  static constexpr int kWarps = DIM == 256 ? 4 : NT == 1 && kStage <= 4096 ? PW : 8;
+    static constexpr int kWarps = DIM == 256 ? 4 : 8;
   static constexpr int kStages = kPagedRingBytes / kWarps / kStage < 8 ? kPagedRingBytes / kWarps / kStage : 8;
   static constexpr int kKChunks = kRow / 64;        // 16-byte pieces of a key per lane
   static constexpr int kVPiece = kRow / 8 < 16 ? 8 : 16;
@@ -152,17 +152,19 @@ struct PagedTile {
   static_assert(kPart * 4 <= kRing && kStages >= 2, "a partial result takes the place of the ring");
 };
 
-// Where a row that is cut by the first step of a CTA comes together: {row begins in the CTA before, request, head index, CTAs from here}
+// The row (of `lanes` neighbouring heads, `sub` the index of their group) that is first cut by the first step of a CTA: it begins in the CTA
+// before and goes on in `count` CTAs from here.
 struct alignas(16) PagedJoin {
-  int valid, request, sub, count;
+  int lanes, request, sub, count;  // lanes: 0 where no row is first cut here
 };
 
 struct PagedWork {
   int heads_per_request;  // key/value heads x row tiles
   int row_tiles;
   int group;              // query heads per key/value head
+  int lane_bits;          // log2 of the largest power of two, at most the warps of a CTA, that divides heads_per_request
   PagedJoin* joins;       // [grid]
-  float* cta_part;        // [grid][2][kPart]: rows from the CTA before, rows into the CTA behind
+  float* cta_part;        // [grid][2][warps][kPart]: rows from the CTA before, rows into the CTA behind, of each lane
   float* warp_part;       // [grid][warps][kPart]: rows from the warp before that end inside a warp's run
   int* status;
 };
@@ -234,30 +236,30 @@ __device__ __forceinline__ float paged_out_scale(const b200q_paged_attention_arg
 // the keys that a request's token sees: [first, len); its steps begin at a multiple of 16
 struct PagedSpan {
   int len, first;
-  __device__ __forceinline__ PagedSpan(const b200q_paged_attention_args& a, int b) {
-    len = paged_length(a, b);
+  __device__ __forceinline__ PagedSpan(const b200q_paged_attention_args& a, int length) {
+    len = length;
     first = a.window > 0 && len > a.window ? len - (int)a.window : 0;
   }
   __device__ __forceinline__ int steps() const { return (int)(((uint32_t)len + 15u) / 16u) - first / 16; }
 };
 
-// A place in the list of steps.
+// A place in the list of steps (of fewer than 2^31).
 struct PagedCursor {
   int b, sub, step, steps;
-  // the place of global step g < total; prefix: inclusive sums of the requests' steps
-  __device__ __forceinline__ void locate(const int* prefix, int requests, int heads, int64_t g) {
+  // the place of step `at`; prefix: inclusive sums of the requests' steps
+  __device__ __forceinline__ void locate(const int* prefix, int requests, int heads, int at) {
     int lo = 0, hi = requests - 1;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
-      if ((int64_t)prefix[mid] * heads > g) hi = mid;
+      if (prefix[mid] * heads > at) hi = mid;
       else lo = mid + 1;
     }
     b = lo;
     const int before = b ? prefix[b - 1] : 0;
     steps = prefix[b] - before;
-    const int64_t r = g - (int64_t)before * heads;
-    sub = (int)(r / steps);
-    step = (int)(r - (int64_t)sub * steps);
+    const uint32_t r = (uint32_t)(at - before * heads);
+    sub = (int)(r / (uint32_t)steps);
+    step = (int)r - sub * steps;
   }
   // to the first step of the next row; there is one
   __device__ __forceinline__ bool next_row(const int* prefix, int requests, int heads) {
@@ -269,6 +271,21 @@ struct PagedCursor {
       steps = prefix[b] - prefix[b - 1];
     } while (steps == 0);
     return true;
+  }
+};
+
+// The list in equal runs: the first `more` of `ctas` have a step more than the others.
+struct PagedRuns {
+  int ctas, each, more;
+  __device__ __forceinline__ PagedRuns(int total, int ctas_) {
+    ctas = ctas_;
+    each = (int)((uint32_t)total / (uint32_t)ctas);
+    more = total - each * ctas;
+  }
+  __device__ __forceinline__ int begin(int c) const { return c * each + min(c, more); }
+  __device__ __forceinline__ int cta_of(int at) const {  // (each > 0)
+    const int longer = more * (each + 1);
+    return at < longer ? (int)((uint32_t)at / (uint32_t)(each + 1)) : more + (int)((uint32_t)(at - longer) / (uint32_t)each);
   }
 };
 
@@ -329,21 +346,41 @@ struct PagedAcc {
   }
 };
 
-// Joins one head's results from `count` places (at(i): a partial result): the values of dimensions lane, lane + 32, ...
+// Joins one head's results from `count` places (at(i): a partial result): the values of dimensions lane, lane + 32, ...  Eight places at a
+// time, all their loads in flight together (a trip to L2 is what a join costs).
 template <int DIM, int ROWS, typename At>
 __device__ __forceinline__ void paged_merge(At at, int count, int row, int lane, float (&o)[DIM / 32], float& m, float& l) {
+  constexpr int kBatch = 8;
   m = kPagedNoMax;
-  for (int i = 0; i < count; ++i) m = fmaxf(m, __ldcg(at(i) + ROWS * DIM + row));  // (written by other CTAs: read past L1)
   l = 0.f;
 #pragma unroll
   for (int d = 0; d < DIM / 32; ++d) o[d] = 0.f;
-#pragma unroll 4
-  for (int i = 0; i < count; ++i) {
-    const float* p = at(i);
-    const float w = exp2f(__ldcg(p + ROWS * DIM + row) - m);  // (inf - inf: a NaN row, as its parts are)
-    l += w * __ldcg(p + ROWS * DIM + ROWS + row);
+  for (int base = 0; base < count; base += kBatch) {
+    float pm[kBatch], pl[kBatch], x[kBatch][DIM / 32];
 #pragma unroll
-    for (int d = 0; d < DIM / 32; ++d) o[d] += w * __ldcg(p + row * DIM + d * 32 + lane);
+    for (int i = 0; i < kBatch; ++i) {
+      const float* p = at(min(base + i, count - 1));  // (written by other CTAs: read past L1)
+      pm[i] = __ldcg(p + ROWS * DIM + row);
+      pl[i] = __ldcg(p + ROWS * DIM + ROWS + row);
+#pragma unroll
+      for (int d = 0; d < DIM / 32; ++d) x[i][d] = __ldcg(p + row * DIM + d * 32 + lane);
+    }
+    float top = m;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) top = fmaxf(top, pm[i]);
+    const float keep = exp2f(m - top);  // (inf - inf: a NaN row, as its parts are)
+    m = top;
+    l *= keep;
+#pragma unroll
+    for (int d = 0; d < DIM / 32; ++d) o[d] *= keep;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (base + i >= count) break;
+      const float weight = exp2f(pm[i] - top);
+      l += weight * pl[i];
+#pragma unroll
+      for (int d = 0; d < DIM / 32; ++d) o[d] += weight * x[i][d];
+    }
   }
 }
 template <int DIM>
@@ -361,19 +398,20 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
     paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                            const b200q_paged_attention_args a, const PagedWork w) {
   using Tile = PagedTile<DIM, FMT, NT>;
-  constexpr int kWarps = Tile::kWarps, kStages = Tile::kStages, kTiles = Tile::kTiles, kElt = Tile::kElt;
+  constexpr int kWarps = Tile::kWarps, kWarpBits = kWarps == 8 ? 3 : 2, kStages = Tile::kStages, kTiles = Tile::kTiles;
+  static_assert(1 << kWarpBits == kWarps, "a power of two");
   extern __shared__ __align__(1024) uint8_t s_raw[];
   uint8_t* const s_ring = s_raw + (0u - paged_smem(s_raw) & 1023u);  // [warps][kRing] (swizzled tiles repeat every 1024 bytes), then the prefix sums
   __shared__ __align__(8) uint64_t s_bars[kWarps * kStages];
   __shared__ int s_abort;
   __shared__ int s_sum[kWarps];
-  __shared__ int s_final[kWarps], s_from[kWarps], s_done[kWarps], s_b[kWarps], s_sub[kWarps];
+  __shared__ int s_state[kWarps], s_b[kWarps], s_sub[kWarps], s_cut_b, s_cut_sub;
   int* prefix = reinterpret_cast<int*>(s_ring + kWarps * Tile::kRing);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const int requests = (int)a.requests, heads = w.heads_per_request;
+  const int requests = (int)a.requests;
   const uint32_t bars = paged_smem(s_bars + warp * kStages);
-  if (lane == 0) {
-    for (int s = 0; s < kStages; ++s) ptx::mbar_init(bars + 8 * s, 1);
+  if (lane < kStages) {
+    ptx::mbar_init(bars + 8 * lane, 1);
     ptx::fence_barrier_init();
   }
   if (tid == 0) {
@@ -384,13 +422,17 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
   pdl_enter();
 
   // ---- the list of steps
+  int* const lengths = prefix + requests;  // (where there is room: the rows of the loop then need no loads that wait behind the copies)
+  const bool lengths_here = requests <= kPagedLengthsHere;
   {
     const int per = (requests + 32 * kWarps - 1) / (32 * kWarps);
     const int b0 = min(tid * per, requests), b1 = min(b0 + per, requests);
     int sum = 0;
     for (int b = b0; b < b1; ++b) {
-      sum += PagedSpan(a, b).steps();
+      const int len = paged_length(a, b);
+      sum += PagedSpan(a, len).steps();
       prefix[b] = sum;
+      if (lengths_here) lengths[b] = len;
     }
     int scan = sum;
 #pragma unroll
@@ -407,7 +449,16 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
     for (int b = b0; b < b1; ++b) prefix[b] += before;
     __syncthreads();
   }
-  const int64_t total = (int64_t)prefix[requests - 1] * heads;
+  auto span_of = [&](int b) { return PagedSpan(a, lengths_here ? lengths[b] : paged_length(a, b)); };
+  // Heads side by side where a warp's share is long enough to pay for a partial result of its own, or where rows are so many that
+  // few of them are cut, and only where a token's head is short of 512 bytes.  us, side by side / one head per CTA (8 key/value heads of 128
+  // in e4m3): 64 x 8192 175 / 212, 64 x 1000 37.7 / 42.0, 16 x 2600 29.2 / 27.6, 1 x 8192 18.1 / 14.6; 128 x 200 26.9 / 29.6,
+  // 256 x 200 39.7 / 43.8, 32 x 400 18.1 / 18.3; 2 heads of 256 in bf16, 40 x 4000: 66.8 / 63.7.  (Two or four of the heads: no better than either.)
+  const int key_steps = prefix[requests - 1], warps = kWarps * (int)gridDim.x;
+  const bool beside = Tile::kRow < 512 && (key_steps * w.heads_per_request >= kPagedLaneSteps * warps || requests * w.heads_per_request >= warps / 4);
+  const int shift = beside ? w.lane_bits : 0;
+  const int lanes = 1 << shift, groups = kWarps >> shift, my_lane = warp & (lanes - 1), my_group = warp >> shift;
+  const int heads = w.heads_per_request >> shift, total = key_steps * heads;
   const float out_scale = paged_out_scale(a);
 
   // requests that see nothing
@@ -420,32 +471,24 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
   }
 
   // ---- this CTA's run, and this warp's
-  const int64_t wanted = (total + kWarps * kPagedMinSteps - 1) / (kWarps * kPagedMinSteps);
-  const int64_t ctas = wanted < (int64_t)gridDim.x ? wanted : (int64_t)gridDim.x;
   const int c = blockIdx.x;
+  const int wanted = (int)(((uint32_t)total + (uint32_t)(groups * kPagedMinSteps - 1)) / (uint32_t)(groups * kPagedMinSteps));
+  const int ctas = min(wanted, (int)gridDim.x);
   if (c >= ctas) {
-    if (tid == 0) w.joins[c].valid = 0;
+    if (tid == 0) w.joins[c].lanes = 0;
     return;
   }
-  const int64_t run0 = total * c / ctas, run1 = total * (c + 1) / ctas;
-  auto warp_begin = [&](int i) { return run0 + ((run1 - run0) * i + kWarps - 1) / kWarps; };
-  const int64_t first_step = warp_begin(warp);
-  const int todo = (int)(warp_begin(warp + 1) - first_step);
-  if (tid == 0) {
-    PagedCursor cut;
-    cut.locate(prefix, requests, heads, run0);
-    PagedJoin join = {0, cut.b, cut.sub, 0};
-    const int64_t row0 = run0 - cut.step, row1 = row0 + cut.steps;
-    if (cut.step > 0 && row0 >= total * (c - 1) / ctas) {  // the row is cut here for the first time
-      join.valid = 1;
-      join.count = (int)((row1 * ctas + total - 1) / total - 1) - c + 1;  // CTAs that hold steps [run0, row1)
-    }
-    w.joins[c] = join;
-  }
+  const PagedRuns runs(total, ctas);
+  const int run0 = runs.begin(c), run1 = runs.begin(c + 1);
+  const int group_bits = kWarpBits - shift;
+  auto group_begin = [&](int i) { return run0 + (int)(((int64_t)(run1 - run0) * i + groups - 1) >> group_bits); };
+  const int first_step = group_begin(my_group);
+  const int todo = group_begin(my_group + 1) - first_step;
 
   const uint32_t ring = paged_smem(s_ring + warp * Tile::kRing);
   float* const part_smem = reinterpret_cast<float*>(s_ring + warp * Tile::kRing);
   int final_part = 0, from_here = 0, row_done = 0;  // of the row that the warp's run ends in
+  int cut = 0;                                      // the run begins inside a row
   PagedCursor cc = {0, 0, 0, 0};
 
   if (todo > 0) {
@@ -453,6 +496,11 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
     PagedCursor pc;
     pc.locate(prefix, requests, heads, first_step);
     cc = pc;
+    cut = pc.step > 0;
+    if (warp == 0 && lane == 0) {
+      s_cut_b = pc.b;
+      s_cut_sub = pc.sub;
+    }
     const int steps_per_page = (int)a.page_size / 16;
     const int32_t* p_table;
     int p_todo = todo, p_left, p_page_left, p_page, p_slot, p_kv;  // steps: to copy, of the row, of the page; where the next one is
@@ -463,13 +511,25 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
       p_slot = 16 * step_of_page;
       p_page_left = steps_per_page - step_of_page;
     };
+    const __nv_bfloat16* const q = static_cast<const __nv_bfloat16*>(a.q);
     auto enter_row = [&] {
-      const PagedSpan span(a, pc.b);
+      const PagedSpan span = span_of(pc.b);
       const int at = span.first / 16 + pc.step, index = at / steps_per_page;  // in steps
-      p_kv = pc.sub / w.row_tiles;
+      p_kv = (pc.sub * lanes + my_lane) / w.row_tiles;
       p_left = pc.steps - pc.step;
       p_table = a.block_table + (int64_t)pc.b * a.table_stride + index;
       enter_page(at - index * steps_per_page);
+    };
+    // the queries of a row that the copies have reached, into L1 by the time that the products reach it
+    auto fetch_queries = [&] {
+      constexpr int kLines = DIM * 2 / 128;
+      const int sub = pc.sub * lanes + my_lane, kv = sub / w.row_tiles, row = (sub - kv * w.row_tiles) * Tile::kRows + lane / kLines;
+      if (lane < Tile::kRows * kLines && row < w.group) {
+        uint32_t unused;
+        asm volatile("ld.global.ca.u32 %0, [%1];"
+                     : "=r"(unused)
+                     : "l"(q + (int64_t)pc.b * a.q_token_stride + (int64_t)(kv * w.group + row) * a.q_head_stride + lane % kLines * 64));
+      }
     };
     auto copy_step = [&](int stage) {
       if (p_todo == 0) return;
@@ -492,10 +552,9 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
         }
       } else if (p_todo > 0 && pc.next_row(prefix, requests, heads)) {
         enter_row();
+        fetch_queries();
       }
     };
-    enter_row();
-    for (int s = 0; s < kStages - 1; ++s) copy_step(s);
 
     // ---- the products
     PagedAcc<DIM, FMT, NT> acc;
@@ -503,40 +562,39 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
     float coef[NT][2];  // scores in powers of two for heads 2t, 2t + 1
     int c_lo = 0, c_end = 0, c_left = 0;  // keys of this step before c_lo are not seen, nor those of the row's last step from c_end on
     const float score_scale = a.softmax_scale * (a.k_scale_inv ? *a.k_scale_inv : 1.f) * 1.44269504088896341f;
-    const __nv_bfloat16* const q = static_cast<const __nv_bfloat16*>(a.q);
-    auto begin_row = [&] {
-      const PagedSpan span(a, cc.b);
-      c_lo = cc.step == 0 ? span.first % 16 : 0;
-      c_end = (span.len - 1) % 16 + 1;
-      c_left = cc.steps - cc.step;
-      from_here = cc.step == 0;
-      acc.clear();
-      const int kv = cc.sub / w.row_tiles, row0 = (cc.sub - kv * w.row_tiles) * Tile::kRows;
+    constexpr int kQ = Tile::kKChunks * (FMT == B200Q_BF16 ? 4 : 8);  // words of a head per lane
+    auto load_queries = [&](uint32_t (&raw)[NT][kQ]) {
+      const int sub = cc.sub * lanes + my_lane, kv = sub / w.row_tiles, row0 = (sub - kv * w.row_tiles) * Tile::kRows;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const int row = row0 + 8 * n + g;
         const bool live = row < w.group;
         const __nv_bfloat16* src = q + (int64_t)cc.b * a.q_token_stride + (int64_t)(kv * w.group + (live ? row : 0)) * a.q_head_stride;
+#pragma unroll
+        for (int i = 0; i < kQ / 4; ++i) {  // values as they meet the keys' bytes 64 c + 16 t ... + 15
+          uint4 v = *reinterpret_cast<const uint4*>(src + (FMT == B200Q_BF16 ? (4 * i + t) * 8 : (4 * (i / 2) + t) * 16 + 8 * (i % 2)));
+          if (!live) v = make_uint4(0, 0, 0, 0);
+          raw[n][4 * i] = v.x; raw[n][4 * i + 1] = v.y; raw[n][4 * i + 2] = v.z; raw[n][4 * i + 3] = v.w;
+        }
+      }
+    };
+    auto begin_row = [&](const uint32_t (&raw)[NT][kQ]) {
+      const PagedSpan span = span_of(cc.b);
+      c_lo = cc.step == 0 ? span.first % 16 : 0;
+      c_end = (span.len - 1) % 16 + 1;
+      c_left = cc.steps - cc.step;
+      from_here = cc.step == 0;
+      acc.clear();
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
         if (FMT == B200Q_BF16) {
 #pragma unroll
-          for (int i = 0; i < Tile::kKChunks; ++i) {
-            uint4 v = *reinterpret_cast<const uint4*>(src + (4 * i + t) * 8);
-            if (!live) v = make_uint4(0, 0, 0, 0);
-            qf[2 * i][n][0] = v.x; qf[2 * i][n][1] = v.y; qf[2 * i + 1][n][0] = v.z; qf[2 * i + 1][n][1] = v.w;
-          }
+          for (int i = 0; i < kQ; ++i) qf[i / 2][n][i % 2] = raw[n][i];
           coef[n][0] = coef[n][1] = score_scale;
         } else {
-          uint32_t raw[Tile::kKChunks][8];
           uint32_t top = 0;
 #pragma unroll
-          for (int i = 0; i < Tile::kKChunks; ++i)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint4 v = *reinterpret_cast<const uint4*>(src + (4 * i + t) * 16 + 8 * h);
-              if (!live) v = make_uint4(0, 0, 0, 0);
-              raw[i][4 * h] = v.x; raw[i][4 * h + 1] = v.y; raw[i][4 * h + 2] = v.z; raw[i][4 * h + 3] = v.w;
-              top = __vmaxu2(top, __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu)));
-            }
+          for (int i = 0; i < kQ; ++i) top = __vmaxu2(top, raw[n][i] & 0x7FFF7FFFu);
           top = max(top & 0xFFFFu, top >> 16);
           top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
           top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
@@ -545,16 +603,30 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
           const int up = top == 0 || e == 128 ? 0 : min(8 - e, 120);
           const float mul = __uint_as_float((uint32_t)(127 + up) << 23), back = __uint_as_float((uint32_t)(127 - up) << 23);
 #pragma unroll
-          for (int i = 0; i < Tile::kKChunks; ++i)
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              qf[4 * i + j / 2][n][j % 2] = paged_pack_f16(bf16_bits_to_float(raw[i][j] & 0xFFFFu) * mul, bf16_bits_to_float(raw[i][j] >> 16) * mul);
+          for (int i = 0; i < kQ; ++i)
+            qf[i / 2][n][i % 2] = paged_pack_f16(bf16_bits_to_float(raw[n][i] & 0xFFFFu) * mul, bf16_bits_to_float(raw[n][i] >> 16) * mul);
           coef[n][0] = score_scale * __shfl_sync(0xFFFFFFFFu, back, 8 * t);
           coef[n][1] = score_scale * __shfl_sync(0xFFFFFFFFu, back, 8 * t + 4);
         }
       }
     };
-    begin_row();
+    {
+      // the first queries are asked for before the copies: behind them a load takes 3 us
+      uint32_t raw[NT][kQ];
+      load_queries(raw);
+      enter_row();
+      for (int s = 0; s < kStages - 1; ++s) copy_step(s);
+      begin_row(raw);
+    }
+    if (tid == 0) {  // (while the first copies are on their way)
+      PagedJoin join = {0, cc.b, cc.sub, 0};
+      const int row0 = run0 - cc.step, row1 = row0 + cc.steps;
+      if (cc.step > 0 && row0 >= runs.begin(c - 1)) {  // the row is cut here for the first time
+        join.lanes = lanes;
+        join.count = runs.cta_of(row1 - 1) - c + 1;
+      }
+      w.joins[c] = join;
+    }
 
     // where the lane's pieces are in a stage: of keys R(g) + 8 h in box c / 2 at k_at ^ 64 (c % 2); of values key t + 4 i + 8 h
     const int rg = (g >> 1) | ((g & 1) << 2);
@@ -717,7 +789,7 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
       if (row_end || last) {
         acc.sum_lanes();
         if (row_end && from_here) {
-          const int kv = cc.sub / w.row_tiles, row0 = (cc.sub - kv * w.row_tiles) * Tile::kRows;
+          const int sub = cc.sub * lanes + my_lane, kv = sub / w.row_tiles, row0 = (sub - kv * w.row_tiles) * Tile::kRows;
           acc.each4((Tile::kVPiece == 16 ? rg : g), t, [&](int row, int d, const float (&v)[4], int n, int i) {
             if (row0 + row >= w.group) return;
             const float inv = acc.l[n][i] == 0.f ? 0.f : out_scale / acc.l[n][i];
@@ -733,6 +805,8 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
                 if (row < w.group) a.lse[(int64_t)cc.b * a.heads + kv * w.group + row] = paged_lse(acc.m[n][i], acc.l[n][i]);
               }
           }
+        } else if (groups == 1) {  // nobody else in the CTA has a part of it
+          acc.save(w.cta_part + (((int64_t)c * 2 + from_here) * kWarps + my_lane) * Tile::kPart, g, (Tile::kVPiece == 16 ? rg : g), t);
         } else if (last) {
           __syncwarp();
           acc.save(part_smem, g, (Tile::kVPiece == 16 ? rg : g), t);
@@ -741,63 +815,86 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
         } else {
           acc.save(w.warp_part + ((int64_t)c * kWarps + warp) * Tile::kPart, g, (Tile::kVPiece == 16 ? rg : g), t);
         }
-        if (!last && cc.next_row(prefix, requests, heads)) begin_row();
+        if (!last && cc.next_row(prefix, requests, heads)) {
+          uint32_t raw[NT][kQ];
+          load_queries(raw);
+          begin_row(raw);
+        }
       }
     }
   }
+  if (groups == 1) return;
+  // what each warp leaves: 1 it had steps, 2 a part of its last row, 4 which it began, 8 which is done, 16 its run began inside a row
   if (lane == 0) {
-    s_final[warp] = todo > 0 ? final_part : -1;  // -1: no steps
-    s_from[warp] = from_here;
-    s_done[warp] = row_done;
+    s_state[warp] = todo > 0 ? 1 | final_part << 1 | from_here << 2 | row_done << 3 | cut << 4 : 0;
     s_b[warp] = cc.b;
     s_sub[warp] = cc.sub;
   }
   __syncthreads();
 
-  // ---- rows that several warps have a part of: the heads are dealt to the warps
-  bool cut = false;  // whether the first row began in an earlier CTA
-  PagedCursor at0;
-  at0.locate(prefix, requests, heads, run0);
-  cut = at0.step > 0;
-  for (int i = 0; i < 2 * kWarps; ++i) {
-    const int first = i >> 1;
-    const bool from_cut = !(i & 1);  // the row from the CTA before; the row that begins in warp `first` and goes on
-    if (from_cut ? !(first == 0 && cut) : !(s_final[first] == 1 && s_from[first])) continue;
-    // its parts: the first warp's, then those of the following ones until the row ends
-    const float* parts[kWarps];
-    int count = 0;
-    bool ended = false;
-#pragma unroll
-    for (int v = 0; v < kWarps; ++v) {
-      parts[v] = nullptr;
-      if (v < first || ended || s_final[v] < 0) continue;
-      const bool whole = s_final[v] == 1 && (!s_from[v] || (v == first && !from_cut));
-      parts[v] = whole ? reinterpret_cast<const float*>(s_ring + v * Tile::kRing) : w.warp_part + ((int64_t)c * kWarps + v) * Tile::kPart;
-      ended = whole ? s_done[v] : true;
-      ++count;
+  // ---- rows that several groups of warps have a part of; a task is one head of one lane
+  const int state = lane < groups ? s_state[lane << shift] : 0;  // (the lanes of a group are alike in all but the head)
+  const uint32_t has = __ballot_sync(0xFFFFFFFFu, state & 1), last_part = __ballot_sync(0xFFFFFFFFu, state & 2);
+  const uint32_t began = __ballot_sync(0xFFFFFFFFu, state & 4), done_bits = __ballot_sync(0xFFFFFFFFu, state & 8);
+  const uint32_t through = last_part & ~began;            // the group's last row came from the one before: its part is in shared memory
+  const uint32_t on = through & ~done_bits;               // ... and goes on
+  uint32_t starts = last_part & began;                    // rows that begin in a group and go on
+  bool from_cut = __shfl_sync(0xFFFFFFFFu, state, 0) & 16;  // the row from the CTA before comes first
+  while (from_cut || starts) {
+    const int first = from_cut ? 0 : __ffs(starts) - 1;
+    if (!from_cut) starts &= starts - 1;
+    uint32_t parts = 1u << first;
+    bool ended = from_cut && !(on & 1u);
+    if (!ended) {  // the groups behind, up to the first one in which the row does not go on
+      const uint32_t behind = has & ~((2u << first) - 1u), stops = behind & ~on;
+      ended = stops != 0;
+      parts |= ended ? behind & ((stops & (0u - stops)) * 2u - 1u) : behind;
     }
-    const int b = from_cut ? at0.b : s_b[first], sub = from_cut ? at0.sub : s_sub[first];
-    const int kv = sub / w.row_tiles, row0 = (sub - kv * w.row_tiles) * Tile::kRows;
-    for (int row = warp; row < Tile::kRows; row += kWarps) {
+    const uint32_t here = (from_cut ? through : through | 1u << first) & parts;  // the others ended in the middle of a run
+    const int b = from_cut ? s_cut_b : s_b[first << shift], group = from_cut ? s_cut_sub : s_sub[first << shift];
+    for (int task = warp; task < lanes * Tile::kRows; task += kWarps) {
+      const int l_head = task & (lanes - 1), row = task >> shift;
+      const int sub = (group << shift) + l_head, kv = sub / w.row_tiles, row0 = (sub - kv * w.row_tiles) * Tile::kRows;
       if (row0 + row >= w.group) continue;
-      float m = kPagedNoMax, l = 0.f, o[DIM / 32];
+      auto part_of = [&](int v) -> const float* {
+        const int who = (v << shift) + l_head;
+        return here >> v & 1u ? reinterpret_cast<const float*>(s_ring + who * Tile::kRing) : w.warp_part + ((int64_t)c * kWarps + who) * Tile::kPart;
+      };
+      const bool mine = lane < kWarps && (parts >> lane & 1u);
+      float pm = kPagedNoMax, pl = 0.f, x[kWarps][DIM / 32];
+      if (mine) {
+        const float* p = part_of(lane);
+        pm = p[Tile::kRows * DIM + row];
+        pl = p[Tile::kRows * DIM + Tile::kRows + row];
+      }
 #pragma unroll
-      for (int v = 0; v < kWarps; ++v)
-        if (parts[v]) m = fmaxf(m, parts[v][Tile::kRows * DIM + row]);
+      for (int v = 0; v < kWarps; ++v) {
+        const bool part = parts >> v & 1u;
+        const float* p = part_of(part ? v : first) + row * DIM + lane;
+#pragma unroll
+        for (int d = 0; d < DIM / 32; ++d) x[v][d] = part ? p[d * 32] : 0.f;
+      }
+      float m = pm;
+#pragma unroll
+      for (int s = kWarps / 2; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, s));
+      m = __shfl_sync(0xFFFFFFFFu, m, 0);
+      const float weight = mine ? exp2f(pm - m) : 0.f;  // (inf - inf: a NaN row, as its parts are)
+      float l = weight * pl, o[DIM / 32];
+#pragma unroll
+      for (int s = kWarps / 2; s > 0; s >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, s);
+      l = __shfl_sync(0xFFFFFFFFu, l, 0);
 #pragma unroll
       for (int d = 0; d < DIM / 32; ++d) o[d] = 0.f;
 #pragma unroll
       for (int v = 0; v < kWarps; ++v) {
-        if (!parts[v]) continue;
-        const float x = exp2f(parts[v][Tile::kRows * DIM + row] - m);  // (inf - inf: a NaN row, as its parts are)
-        l += x * parts[v][Tile::kRows * DIM + Tile::kRows + row];
+        const float y = __shfl_sync(0xFFFFFFFFu, weight, v);
 #pragma unroll
-        for (int d = 0; d < DIM / 32; ++d) o[d] += x * parts[v][row * DIM + d * 32 + lane];
+        for (int d = 0; d < DIM / 32; ++d) o[d] += y * x[v][d];
       }
       if (!from_cut && ended) {
         paged_finish<DIM>(a, b, kv * w.group + row0 + row, lane, o, m, l, out_scale);
       } else {
-        float* to = w.cta_part + ((int64_t)c * 2 + (from_cut ? 0 : 1)) * Tile::kPart;
+        float* to = w.cta_part + (((int64_t)c * 2 + (from_cut ? 0 : 1)) * kWarps + l_head) * Tile::kPart;
 #pragma unroll
         for (int d = 0; d < DIM / 32; ++d) to[row * DIM + d * 32 + lane] = o[d];
         if (lane == 0) {
@@ -806,49 +903,86 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
         }
       }
     }
+    from_cut = false;
   }
 }
 
-// Rows that several CTAs have a part of.  Block (c, row): the row of steps that is first cut where CTA c begins.
-template <int DIM, int ROWS>
-__global__ void __launch_bounds__(128) paged_join_kernel(const b200q_paged_attention_args a, const PagedWork w) {
+// Rows that several CTAs have a part of.  Every block makes the list of them; one (row of heads, lane, head) is a task, of a warp where
+// there are many, and of a whole block where there are fewer than blocks (long rows of few requests, with up to a part per CTA).
+constexpr int kPagedJoinBlocks = 4 * kNumSMs;
+constexpr int kPagedJoinWarps = 8;
+
+template <int DIM, int ROWS, int WARPS>
+__global__ void __launch_bounds__(32 * kPagedJoinWarps) paged_join_kernel(const b200q_paged_attention_args a, const PagedWork w, int ctas) {
   constexpr int kPart = ROWS * (DIM + 2);
-  __shared__ float s_o[4][DIM], s_m[4], s_l[4];
+  __shared__ float s_o[kPagedJoinWarps][DIM], s_m[kPagedJoinWarps], s_l[kPagedJoinWarps];
+  __shared__ PagedJoin s_join[kPagedGrid];
+  __shared__ int s_cta[kPagedGrid], s_count[kPagedJoinWarps];
+  static_assert(kPagedGrid <= 32 * kPagedJoinWarps, "a thread per CTA");
   pdl_enter();
-  const int c = blockIdx.x, row = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int4 v = __ldcg(reinterpret_cast<const int4*>(w.joins + c));
-  const PagedJoin join = {v.x, v.y, v.z, v.w};
-  if (!join.valid) return;
-  if (c < 1 || join.count < 1 || join.count > (int)gridDim.x - c || join.request < 0 || join.request >= a.requests || join.sub < 0 ||
-      join.sub >= w.heads_per_request)
-    return;
-  const int kv = join.sub / w.row_tiles, row0 = (join.sub - kv * w.row_tiles) * ROWS;
-  if (row0 + row >= w.group) return;
-  // part 0: the CTA before's last row; part i: the first row of CTA c + i - 1.  A warp takes a quarter of them.
-  const int count = join.count + 1, per = (count + 3) / 4, i0 = min(warp * per, count), n = min(per, count - i0);
-  float m, l, o[DIM / 32];
-  paged_merge<DIM, ROWS>([&](int i) { return w.cta_part + (i0 + i == 0 ? (int64_t)(c - 1) * 2 + 1 : (int64_t)(c + i0 + i - 1) * 2) * kPart; }, n, row, lane, o, m, l);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int4 v = make_int4(0, 0, 0, 0);
+  if (tid < ctas) v = __ldcg(reinterpret_cast<const int4*>(w.joins) + tid);
+  const uint32_t vote = __ballot_sync(0xFFFFFFFFu, v.x != 0);
+  if (lane == 0) s_count[warp] = __popc(vote);
+  __syncthreads();
+  int rows = 0, before = __popc(vote & ((1u << lane) - 1u));
 #pragma unroll
-  for (int d = 0; d < DIM / 32; ++d) s_o[warp][d * 32 + lane] = o[d];
-  if (lane == 0) {
-    s_m[warp] = m;
-    s_l[warp] = l;
+  for (int i = 0; i < kPagedJoinWarps; ++i) {
+    if (i < warp) before += s_count[i];
+    rows += s_count[i];
+  }
+  if (v.x != 0) {
+    s_join[before] = {v.x, v.y, v.z, v.w};
+    s_cta[before] = tid;
   }
   __syncthreads();
-  if (warp != 0) return;
-  m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-  l = 0.f;
+  if (rows == 0) return;
+  const int lanes = s_join[0].lanes, per_row = lanes * ROWS, tasks = rows * per_row;
+  const bool by_block = tasks <= (int)gridDim.x;
+  const float scale = paged_out_scale(a);
+  for (int task = by_block ? blockIdx.x : blockIdx.x * kPagedJoinWarps + warp; task < tasks; task += by_block ? gridDim.x : gridDim.x * kPagedJoinWarps) {
+    const PagedJoin join = s_join[task / per_row];
+    const int c = s_cta[task / per_row], l_head = task % per_row / ROWS, row = task % ROWS;
+    const int sub = join.sub * lanes + l_head, kv = sub / w.row_tiles, row0 = (sub - kv * w.row_tiles) * ROWS;
+    if (row0 + row >= w.group) continue;
+    const int head = kv * w.group + row0 + row;
+    // part 0: the CTA before's last row; part i: the first row of CTA c + i - 1
+    const int count = join.count + 1, per = by_block ? (count + kPagedJoinWarps - 1) / kPagedJoinWarps : count;
+    const int i0 = by_block ? min(warp * per, count) : 0, n = min(per, count - i0);
+    float m, l, o[DIM / 32];
+    paged_merge<DIM, ROWS>(
+        [&](int i) { return w.cta_part + ((i0 + i == 0 ? (int64_t)(c - 1) * 2 + 1 : (int64_t)(c + i0 + i - 1) * 2) * WARPS + l_head) * kPart; }, n, row, lane, o, m,
+        l);
+    if (by_block) {
 #pragma unroll
-  for (int d = 0; d < DIM / 32; ++d) o[d] = 0.f;
+      for (int d = 0; d < DIM / 32; ++d) s_o[warp][d * 32 + lane] = o[d];
+      if (lane == 0) {
+        s_m[warp] = m;
+        s_l[warp] = l;
+      }
+      __syncthreads();
+      if (warp == 0) {
+        m = kPagedNoMax;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (i * per >= count) break;
-    const float x = exp2f(s_m[i] - m);
-    l += x * s_l[i];
+        for (int i = 0; i < kPagedJoinWarps; ++i) m = fmaxf(m, s_m[i]);
+        l = 0.f;
 #pragma unroll
-    for (int d = 0; d < DIM / 32; ++d) o[d] += x * s_o[i][d * 32 + lane];
+        for (int d = 0; d < DIM / 32; ++d) o[d] = 0.f;
+#pragma unroll
+        for (int i = 0; i < kPagedJoinWarps; ++i) {
+          if (i * per >= count) break;
+          const float x = exp2f(s_m[i] - m);
+          l += x * s_l[i];
+#pragma unroll
+          for (int d = 0; d < DIM / 32; ++d) o[d] += x * s_o[i][d * 32 + lane];
+        }
+      }
+      __syncthreads();
+      if (warp != 0) continue;
+    }
+    paged_finish<DIM>(a, join.request, head, lane, o, m, l, scale);
   }
-  paged_finish<DIM>(a, join.request, kv * w.group + row0 + row, lane, o, m, l, paged_out_scale(a));
 }
 
 // ---------------------------------------------------------------------------- host
@@ -863,8 +997,8 @@ size_t paged_attention_workspace_bytes_impl(int64_t requests, int heads, int kv_
   (void)cache_dtype;
   if (!paged_tensor_dim(dim)) return 0;
   const size_t part = sizeof(float) * paged_rows_of(heads / kv_heads, dim) * (dim + 2);
-  const size_t warps = 16;
-  return paged_align(sizeof(PagedJoin) * kPagedGrid) + paged_align(part * 2 * kPagedGrid) + paged_align(part * warps * kPagedGrid);
+  const size_t warps = dim == 256 ? 4 : 8;
+  return paged_align(sizeof(PagedJoin) * kPagedGrid) + paged_align(part * 2 * warps * kPagedGrid) + paged_align(part * warps * kPagedGrid);
 }
 
 // A cache as [pages][slots][heads][bytes of a head], whatever the order of its strides, in boxes of 16 slots
@@ -905,21 +1039,25 @@ static int paged_launch(const b200q_paged_attention_args& a, cudaStream_t st) {
   w.group = a.heads / a.kv_heads;
   w.row_tiles = (w.group + Tile::kRows - 1) / Tile::kRows;
   w.heads_per_request = a.kv_heads * w.row_tiles;
+  w.lane_bits = 0;
+  while ((2 << w.lane_bits) <= Tile::kWarps && w.heads_per_request % (2 << w.lane_bits) == 0) ++w.lane_bits;
   uint8_t* p = static_cast<uint8_t*>(a.workspace);
   w.joins = reinterpret_cast<PagedJoin*>(p);
   p += paged_align(sizeof(PagedJoin) * kPagedGrid);
   w.cta_part = reinterpret_cast<float*>(p);
-  p += paged_align(sizeof(float) * Tile::kPart * 2 * kPagedGrid);
+  p += paged_align(sizeof(float) * Tile::kPart * 2 * Tile::kWarps * kPagedGrid);
   w.warp_part = reinterpret_cast<float*>(p);
-  // no more CTAs than the longest rows that the tables can hold would fill
-  const int64_t most = a.requests * ((a.table_width * a.page_size + 15) / 16) * w.heads_per_request;
+  // the longest list that the tables can hold: no more CTAs than it would fill
+  const int64_t row_steps = (a.table_width * a.page_size + 15) / 16;
+  if (row_steps > 0 && (row_steps > INT32_MAX || a.requests > INT32_MAX / row_steps / w.heads_per_request)) return B200Q_ERR_TOO_LARGE;
+  const int64_t most = a.requests * row_steps * w.heads_per_request;
   int64_t grid = (most + Tile::kWarps * kPagedMinSteps - 1) / (Tile::kWarps * kPagedMinSteps);
   if (grid < 1) grid = 1;
   if (grid > kPagedGrid) grid = kPagedGrid;
-  launch_dependent(kernel, dim3((unsigned)grid), dim3(32 * Tile::kWarps), Tile::kWarps * Tile::kRing + 1024 + 4 * (size_t)a.requests, st, map_k, map_v, a, w);
+  launch_dependent(kernel, dim3((unsigned)grid), dim3(32 * Tile::kWarps), Tile::kWarps * Tile::kRing + 1024 + (a.requests <= kPagedLengthsHere ? 8 : 4) * (size_t)a.requests, st, map_k, map_v, a, w);
   B200Q_LAUNCH_CHECK();
   if (grid > 1) {
-    launch_dependent(paged_join_kernel<DIM, 8 * NT>, dim3((unsigned)grid, 8 * NT), dim3(128), 0, st, a, w);
+    launch_dependent(paged_join_kernel<DIM, 8 * NT, Tile::kWarps>, dim3(kPagedJoinBlocks), dim3(32 * kPagedJoinWarps), 0, st, a, w, (int)grid);
     B200Q_LAUNCH_CHECK();
   }
   return B200Q_OK;
@@ -954,8 +1092,6 @@ static bool paged_fits_tensor_cores(const b200q_paged_attention_args& a) {
 int paged_attention_impl(const b200q_paged_attention_args& a, cudaStream_t st) {
   if (paged_fits_tensor_cores(a)) {
     if (a.requests > kPagedMaxRequests) return B200Q_ERR_TOO_LARGE;
-    // (table_width and page_size are below 2^31)
-    if (a.table_width > 0 && a.page_size / 16 > ((int64_t)INT32_MAX / a.requests) / a.table_width) return B200Q_ERR_TOO_LARGE;
     if (a.workspace_bytes < paged_attention_workspace_bytes_impl(a.requests, a.heads, a.kv_heads, a.dim, a.cache_dtype) || !a.workspace ||
         reinterpret_cast<uintptr_t>(a.workspace) % 16)
       return B200Q_ERR_BAD_ARGUMENT;
