@@ -149,7 +149,7 @@ struct PagedTile {
   static constexpr int kRows = 8 * NT;              // query heads
   static constexpr int kPart = kRows * (DIM + 2);   // floats of a partial result: output, maxima, sums
   static constexpr int kRing = kStages * kStage;    // bytes per warp
-  static_assert(kPart * 4 <= kRing && kStages >= 2, "a partial result takes the place of the ring");
+  static_assert(2 * kPart * 4 <= kRing && kStages >= 2, "both partial results of a warp take the place of the ring");
 };
 
 // The row (of `lanes` neighbouring heads, `sub` the index of their group) that is first cut by the first step of a CTA: it begins in the CTA
@@ -459,6 +459,9 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
   const int shift = beside ? w.lane_bits : 0;
   const int lanes = 1 << shift, groups = kWarps >> shift, my_lane = warp & (lanes - 1), my_group = warp >> shift;
   const int heads = w.heads_per_request >> shift, total = key_steps * heads;
+  // of the `sub`-th row tile of a request: its key/value head, and its first query head in that head's group
+  auto kv_of = [&](int sub) { return w.row_tiles == 1 ? sub : sub / w.row_tiles; };
+  auto row_of = [&](int sub) { return w.row_tiles == 1 ? 0 : sub % w.row_tiles * Tile::kRows; };
   const float out_scale = paged_out_scale(a);
 
   // requests that see nothing
@@ -486,73 +489,68 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
   const int todo = group_begin(my_group + 1) - first_step;
 
   const uint32_t ring = paged_smem(s_ring + warp * Tile::kRing);
-  float* const part_smem = reinterpret_cast<float*>(s_ring + warp * Tile::kRing);
   int final_part = 0, from_here = 0, row_done = 0;  // of the row that the warp's run ends in
-  int cut = 0;                                      // the run begins inside a row
+  int cut = 0, early = 0;                           // the run begins inside a row; which ends inside the run
   PagedCursor cc = {0, 0, 0, 0};
 
   if (todo > 0) {
-    // ---- copies, kStages - 1 steps ahead
-    PagedCursor pc;
-    pc.locate(prefix, requests, heads, first_step);
-    cc = pc;
-    cut = pc.step > 0;
+    // ---- copies, kStages - 1 steps ahead.  Where steps lie is found out for 32 of them at a time, one per lane, a whole such batch before
+    // it is needed: behind the copies of all SMs a load (of a page's number, above all) takes 2 to 3 us.
+    cc.locate(prefix, requests, heads, first_step);
+    cut = cc.step > 0;
     if (warp == 0 && lane == 0) {
-      s_cut_b = pc.b;
-      s_cut_sub = pc.sub;
+      s_cut_b = cc.b;
+      s_cut_sub = cc.sub;
     }
     const int steps_per_page = (int)a.page_size / 16;
-    const int32_t* p_table;
-    int p_todo = todo, p_left, p_page_left, p_page, p_slot, p_kv;  // steps: to copy, of the row, of the page; where the next one is
-    uint32_t bad = 0;  // bit s: the step in stage s has no page
-    auto enter_page = [&](int step_of_page) {  // (steps lie within a request's length, which its table covers)
-      const int p = *p_table;
-      p_page = (uint32_t)p < (uint32_t)a.num_pages ? p : (int)a.num_pages;  // (behind the last page a copy brings zeros)
-      p_slot = 16 * step_of_page;
-      p_page_left = steps_per_page - step_of_page;
-    };
     const __nv_bfloat16* const q = static_cast<const __nv_bfloat16*>(a.q);
-    auto enter_row = [&] {
-      const PagedSpan span = span_of(pc.b);
-      const int at = span.first / 16 + pc.step, index = at / steps_per_page;  // in steps
-      p_kv = (pc.sub * lanes + my_lane) / w.row_tiles;
-      p_left = pc.steps - pc.step;
-      p_table = a.block_table + (int64_t)pc.b * a.table_stride + index;
-      enter_page(at - index * steps_per_page);
+    struct Place {
+      int page, slot, kv;
     };
-    // the queries of a row that the copies have reached, into L1 by the time that the products reach it
-    auto fetch_queries = [&] {
-      constexpr int kLines = DIM * 2 / 128;
-      const int sub = pc.sub * lanes + my_lane, kv = sub / w.row_tiles, row = (sub - kv * w.row_tiles) * Tile::kRows + lane / kLines;
-      if (lane < Tile::kRows * kLines && row < w.group) {
-        uint32_t unused;
-        asm volatile("ld.global.ca.u32 %0, [%1];"
-                     : "=r"(unused)
-                     : "l"(q + (int64_t)pc.b * a.q_token_stride + (int64_t)(kv * w.group + row) * a.q_head_stride + lane % kLines * 64));
+    auto plan = [&](int base) {
+      Place at = {-1, 0, 0};
+      if (base + lane < todo) {
+        PagedCursor pc = cc;
+        pc.step += lane;
+        if (base > 0 || pc.step >= pc.steps) pc.locate(prefix, requests, heads, first_step + base + lane);  // (cc: where the run begins, while base is 0)
+        const int step = span_of(pc.b).first / 16 + pc.step, index = step / steps_per_page, sub = pc.sub * lanes + my_lane;
+        at.page = a.block_table[(int64_t)pc.b * a.table_stride + index];  // (a step lies within a request's length, which its table covers)
+        at.slot = 16 * (step - index * steps_per_page);
+        at.kv = kv_of(sub);
+        if (pc.step == 0 && base + lane > 0) {  // the queries of a row that begins here, into L1
+          const int row0 = row_of(sub);
+          const __nv_bfloat16* src = q + (int64_t)pc.b * a.q_token_stride + (int64_t)(at.kv * w.group + row0) * a.q_head_stride;
+          for (int i = 0; i < min(Tile::kRows, w.group - row0); ++i)
+#pragma unroll
+            for (int d = 0; d < DIM; d += 64) {
+              uint32_t unused;
+              asm volatile("ld.global.ca.u32 %0, [%1];" : "=r"(unused) : "l"(src + i * a.q_head_stride + d));
+            }
+        }
       }
+      return at;
     };
+    Place now, soon;  // of steps [copied / 32 * 32, ...), and of the 32 behind them
+    int copied = 0;
+    uint32_t bad = 0;  // bit s: the step in stage s has no page
     auto copy_step = [&](int stage) {
-      if (p_todo == 0) return;
+      if (copied == todo) return;
+      const int p = __shfl_sync(0xFFFFFFFFu, now.page, copied & 31);
+      const int page = (uint32_t)p < (uint32_t)a.num_pages ? p : (int)a.num_pages;  // (behind the last page a copy brings zeros)
+      const int slot = __shfl_sync(0xFFFFFFFFu, now.slot, copied & 31), kv = __shfl_sync(0xFFFFFFFFu, now.kv, copied & 31);
       const uint32_t bar = bars + 8 * stage, dst = ring + stage * Tile::kStage;
-      bad = (bad & ~(1u << stage)) | ((uint32_t)(p_page == (int)a.num_pages) << stage);
+      bad = (bad & ~(1u << stage)) | ((uint32_t)(page == (int)a.num_pages) << stage);
       if (ptx::elect_one()) {
         ptx::mbar_arrive_expect_tx(bar, Tile::kStage);
 #pragma unroll
-        for (int i = 0; i < Tile::kBoxes; ++i) paged_copy(dst + i * 16 * Tile::kBox, &map_k, bar, i * Tile::kBox, p_kv, p_slot, p_page);
+        for (int i = 0; i < Tile::kBoxes; ++i) paged_copy(dst + i * 16 * Tile::kBox, &map_k, bar, i * Tile::kBox, kv, slot, page);
 #pragma unroll
         for (int i = 0; i < Tile::kBoxes; ++i)
-          paged_copy(dst + 16 * Tile::kRow + i * 16 * Tile::kBox, &map_v, bar, i * Tile::kBox, p_kv, p_slot, p_page);
+          paged_copy(dst + 16 * Tile::kRow + i * 16 * Tile::kBox, &map_v, bar, i * Tile::kBox, kv, slot, page);
       }
-      --p_todo;
-      if (--p_left > 0) {
-        p_slot += 16;
-        if (--p_page_left == 0 && p_todo > 0) {
-          ++p_table;
-          enter_page(0);
-        }
-      } else if (p_todo > 0 && pc.next_row(prefix, requests, heads)) {
-        enter_row();
-        fetch_queries();
+      if ((++copied & 31) == 0) {
+        now = soon;
+        soon = plan(copied + 32);
       }
     };
 
@@ -563,30 +561,34 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
     int c_lo = 0, c_end = 0, c_left = 0;  // keys of this step before c_lo are not seen, nor those of the row's last step from c_end on
     const float score_scale = a.softmax_scale * (a.k_scale_inv ? *a.k_scale_inv : 1.f) * 1.44269504088896341f;
     constexpr int kQ = Tile::kKChunks * (FMT == B200Q_BF16 ? 4 : 8);  // words of a head per lane
-    auto load_queries = [&](uint32_t (&raw)[NT][kQ]) {
-      const int sub = cc.sub * lanes + my_lane, kv = sub / w.row_tiles, row0 = (sub - kv * w.row_tiles) * Tile::kRows;
+    auto load_queries = [&](const PagedCursor& at, uint32_t (&raw)[NT][kQ]) {
+      const int sub = at.sub * lanes + my_lane, kv = kv_of(sub), row0 = row_of(sub);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const int row = row0 + 8 * n + g;
         const bool live = row < w.group;
-        const __nv_bfloat16* src = q + (int64_t)cc.b * a.q_token_stride + (int64_t)(kv * w.group + (live ? row : 0)) * a.q_head_stride;
+        const __nv_bfloat16* src = q + (int64_t)at.b * a.q_token_stride + (int64_t)(kv * w.group + (live ? row : 0)) * a.q_head_stride;
 #pragma unroll
         for (int i = 0; i < kQ / 4; ++i) {  // values as they meet the keys' bytes 64 c + 16 t ... + 15
-          uint4 v = *reinterpret_cast<const uint4*>(src + (FMT == B200Q_BF16 ? (4 * i + t) * 8 : (4 * (i / 2) + t) * 16 + 8 * (i % 2)));
-          if (!live) v = make_uint4(0, 0, 0, 0);
+          const uint4 v = *reinterpret_cast<const uint4*>(src + (FMT == B200Q_BF16 ? (4 * i + t) * 8 : (4 * (i / 2) + t) * 16 + 8 * (i % 2)));
           raw[n][4 * i] = v.x; raw[n][4 * i + 1] = v.y; raw[n][4 * i + 2] = v.z; raw[n][4 * i + 3] = v.w;
         }
       }
     };
-    auto begin_row = [&](const uint32_t (&raw)[NT][kQ]) {
+    auto begin_row = [&](uint32_t (&raw)[NT][kQ]) {
       const PagedSpan span = span_of(cc.b);
       c_lo = cc.step == 0 ? span.first % 16 : 0;
       c_end = (span.len - 1) % 16 + 1;
       c_left = cc.steps - cc.step;
       from_here = cc.step == 0;
       acc.clear();
+      const int rows = w.group - row_of(cc.sub * lanes + my_lane);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
+        if (8 * n + g >= rows) {  // (a head that the group does not have: the loads brought another's)
+#pragma unroll
+          for (int i = 0; i < kQ; ++i) raw[n][i] = 0;
+        }
         if (FMT == B200Q_BF16) {
 #pragma unroll
           for (int i = 0; i < kQ; ++i) qf[i / 2][n][i % 2] = raw[n][i];
@@ -613,9 +615,10 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
     {
       // the first queries are asked for before the copies: behind them a load takes 3 us
       uint32_t raw[NT][kQ];
-      load_queries(raw);
-      enter_row();
+      load_queries(cc, raw);
+      now = plan(0);
       for (int s = 0; s < kStages - 1; ++s) copy_step(s);
+      soon = plan(32);
       begin_row(raw);
     }
     if (tid == 0) {  // (while the first copies are on their way)
@@ -637,7 +640,7 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
     for (int done = 0; done < todo; ++done) {
       if (!ptx::mbar_wait_uniform(bars + 8 * stage, phase, &s_abort, w.status, kPagedErrCopy)) {
         // gives up: waits for the other copies in flight, as far as they come, and leaves
-        for (int s = 1; s < kStages && done + s < todo - p_todo; ++s) {
+        for (int s = 1; s < kStages && done + s < copied; ++s) {
           const int next = (stage + s) % kStages;
           for (int i = 0; i < 4096 && !ptx::mbar_try_wait(bars + 8 * next, phase ^ (stage + s >= kStages)); ++i) __nanosleep(64);
         }
@@ -787,43 +790,68 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
 
       const bool row_end = --c_left == 0, last = done + 1 == todo;
       if (row_end || last) {
+        // the next row's queries are on their way while this one is finished, where there are registers for them
+        constexpr bool kAhead = NT == 1 && DIM < 256;
+        PagedCursor next = cc;
+        uint32_t raw[NT][kQ];
+        const bool more = !last && next.next_row(prefix, requests, heads);
+        if (kAhead && more) load_queries(next, raw);
         acc.sum_lanes();
         if (row_end && from_here) {
-          const int sub = cc.sub * lanes + my_lane, kv = sub / w.row_tiles, row0 = (sub - kv * w.row_tiles) * Tile::kRows;
-          acc.each4((Tile::kVPiece == 16 ? rg : g), t, [&](int row, int d, const float (&v)[4], int n, int i) {
-            if (row0 + row >= w.group) return;
-            const float inv = acc.l[n][i] == 0.f ? 0.f : out_scale / acc.l[n][i];
-            const float r[4] = {v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
-            paged_store4(a.out, a.out_dtype, ((int64_t)cc.b * a.heads + kv * w.group + row0 + row) * DIM + d, r);
-          });
+          const int sub = cc.sub * lanes + my_lane, rows = w.group - row_of(sub);
+          const int64_t head = (int64_t)cc.b * a.heads + kv_of(sub) * w.group + row_of(sub);
+          float inv[NT][2];
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) inv[n][i] = acc.l[n][i] == 0.f ? 0.f : __fdividef(out_scale, acc.l[n][i]);
+          auto write = [&](int dtype) {
+            acc.each4(Tile::kVPiece == 16 ? rg : g, t, [&](int row, int d, const float (&v)[4], int n, int i) {
+              const float r[4] = {v[0] * inv[n][i], v[1] * inv[n][i], v[2] * inv[n][i], v[3] * inv[n][i]};
+              if (row < rows) paged_store4(a.out, dtype, head * DIM + (row * DIM + d), r);
+            });
+          };
+          if (a.out_dtype == B200Q_BF16) write(B200Q_BF16);
+          else write(a.out_dtype);
           if (a.lse && g == 0) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
               for (int i = 0; i < 2; ++i) {
-                const int row = row0 + 8 * n + 2 * t + i;
-                if (row < w.group) a.lse[(int64_t)cc.b * a.heads + kv * w.group + row] = paged_lse(acc.m[n][i], acc.l[n][i]);
+                const int row = 8 * n + 2 * t + i;
+                if (row < rows) a.lse[head + row] = paged_lse(acc.m[n][i], acc.l[n][i]);
               }
           }
-        } else if (groups == 1) {  // nobody else in the CTA has a part of it
-          acc.save(w.cta_part + (((int64_t)c * 2 + from_here) * kWarps + my_lane) * Tile::kPart, g, (Tile::kVPiece == 16 ? rg : g), t);
-        } else if (last) {
-          __syncwarp();
-          acc.save(part_smem, g, (Tile::kVPiece == 16 ? rg : g), t);
-          final_part = 1;
-          row_done = row_end;
         } else {
-          acc.save(w.warp_part + ((int64_t)c * kWarps + warp) * Tile::kPart, g, (Tile::kVPiece == 16 ? rg : g), t);
+          // to the joining kernel, where no other warp of the CTA has a part of the row; else to where the CTA joins it
+          float* to = groups == 1 ? w.cta_part + (((int64_t)c * 2 + from_here) * kWarps + my_lane) * Tile::kPart
+                      : last      ? reinterpret_cast<float*>(s_ring + warp * Tile::kRing)
+                                  : w.warp_part + ((int64_t)c * kWarps + warp) * Tile::kPart;
+          __syncwarp();
+          acc.save(to, g, Tile::kVPiece == 16 ? rg : g, t);
+          if (last) {
+            final_part = 1;
+            row_done = row_end;
+          } else {
+            early = groups > 1;
+          }
         }
-        if (!last && cc.next_row(prefix, requests, heads)) {
-          uint32_t raw[NT][kQ];
-          load_queries(raw);
+        if (more) {
+          cc = next;
+          if (!kAhead) load_queries(cc, raw);
           begin_row(raw);
         }
       }
     }
   }
   if (groups == 1) return;
+  if (early) {  // into shared memory too, behind the part of the last row
+    const float4* from = reinterpret_cast<const float4*>(w.warp_part + ((int64_t)c * kWarps + warp) * Tile::kPart);
+    float4* to = reinterpret_cast<float4*>(s_ring + warp * Tile::kRing + 4 * Tile::kPart);
+    __syncwarp();
+#pragma unroll 9
+    for (int i = lane; i < Tile::kPart / 4; i += 32) to[i] = from[i];
+  }
   // what each warp leaves: 1 it had steps, 2 a part of its last row, 4 which it began, 8 which is done, 16 its run began inside a row
   if (lane == 0) {
     s_state[warp] = todo > 0 ? 1 | final_part << 1 | from_here << 2 | row_done << 3 | cut << 4 : 0;
@@ -854,18 +882,17 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
     const int b = from_cut ? s_cut_b : s_b[first << shift], group = from_cut ? s_cut_sub : s_sub[first << shift];
     for (int task = warp; task < lanes * Tile::kRows; task += kWarps) {
       const int l_head = task & (lanes - 1), row = task >> shift;
-      const int sub = (group << shift) + l_head, kv = sub / w.row_tiles, row0 = (sub - kv * w.row_tiles) * Tile::kRows;
+      const int sub = (group << shift) + l_head, kv = kv_of(sub), row0 = row_of(sub);
       if (row0 + row >= w.group) continue;
-      auto part_of = [&](int v) -> const float* {
-        const int who = (v << shift) + l_head;
-        return here >> v & 1u ? reinterpret_cast<const float*>(s_ring + who * Tile::kRing) : w.warp_part + ((int64_t)c * kWarps + who) * Tile::kPart;
+      auto part_of = [&](int v) {
+        return reinterpret_cast<const float*>(s_ring + ((v << shift) + l_head) * Tile::kRing + (here >> v & 1u ? 0 : 4 * Tile::kPart));
       };
       const bool mine = lane < kWarps && (parts >> lane & 1u);
       float pm = kPagedNoMax, pl = 0.f, x[kWarps][DIM / 32];
       if (mine) {
-        const float* p = part_of(lane);
-        pm = p[Tile::kRows * DIM + row];
-        pl = p[Tile::kRows * DIM + Tile::kRows + row];
+        const float* p = part_of(lane) + Tile::kRows * DIM + row;
+        pm = p[0];
+        pl = p[Tile::kRows];
       }
 #pragma unroll
       for (int v = 0; v < kWarps; ++v) {
