@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(kPlainThreads) paged_attention_plain_kernel(co
 // (maximum, sum, output) are joined in the CTA, and, where a row goes on in another CTA, by a second kernel.
 constexpr int kPagedGrid = kNumSMs;
 constexpr int kPagedRingBytes = 192 * 1024;
-constexpr int kPagedLaneSteps = 24;   // a warp's steps from which on heads go side by side
+constexpr int kPagedLaneSteps = 14;   // a warp's steps from which on heads go side by side
 constexpr int kPagedMinSteps = 2;     // a warp gets at least this many steps while there are enough for the others
 constexpr float kPagedShift = 7.f;    // probabilities are held relative to 2^(maximum - 7) ...
 constexpr float kPagedRescale = 15.f; // ... and the maximum is raised when one would pass 2^15 (f16 ends at 2^16)
@@ -450,12 +450,14 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
     __syncthreads();
   }
   auto span_of = [&](int b) { return PagedSpan(a, lengths_here ? lengths[b] : paged_length(a, b)); };
-  // Heads side by side where a warp's share is long enough to pay for a partial result of its own, or where rows are so many that
-  // few of them are cut, and only where a token's head is short of 512 bytes.  us, side by side / one head per CTA (8 key/value heads of 128
-  // in e4m3): 64 x 8192 175 / 212, 64 x 1000 37.7 / 42.0, 16 x 2600 29.2 / 27.6, 1 x 8192 18.1 / 14.6; 128 x 200 26.9 / 29.6,
-  // 256 x 200 39.7 / 43.8, 32 x 400 18.1 / 18.3; 2 heads of 256 in bf16, 40 x 4000: 66.8 / 63.7.  (Two or four of the heads: no better than either.)
+  // Heads side by side where a warp's share is long enough to pay for a partial result of its own, or where rows are so many that few of
+  // them are cut (and no warps of a CTA have parts of the same one), and only where a token's head is short of 512 bytes.  us, side by
+  // side / one head per CTA, 8 key/value heads of 128 in e4m3: 64 x 8192 tokens 176 / 218, 64 x 1000 36.8 / 41.3, 16 of 1024 to 4096 29.5 / 34.6,
+  // 4 x 10000 25.4 / 26.5, 1 x 32768 25.9 / 22.6, 1 x 8192 18.4 / 15.4; 256 x 200 38.2 / 43.9, 32 x 400 17.8 / 18.9; 4 heads, 100 of 75 to 300
+  // 25.1 / 20.0; 2 heads of 256 in bf16, 40 x 4000 66.0 / 63.7.
   const int key_steps = prefix[requests - 1], warps = kWarps * (int)gridDim.x;
-  const bool beside = Tile::kRow < 512 && (key_steps * w.heads_per_request >= kPagedLaneSteps * warps || requests * w.heads_per_request >= warps / 4);
+  const bool beside = Tile::kRow < 512 && (key_steps * w.heads_per_request >= kPagedLaneSteps * warps ||
+                                           (w.lane_bits == kWarpBits && requests * w.heads_per_request >= warps / 4));
   const int shift = beside ? w.lane_bits : 0;
   const int lanes = 1 << shift, groups = kWarps >> shift, my_lane = warp & (lanes - 1), my_group = warp >> shift;
   const int heads = w.heads_per_request >> shift, total = key_steps * heads;
