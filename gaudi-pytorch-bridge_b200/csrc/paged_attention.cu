@@ -1076,10 +1076,8 @@ static int paged_launch(const b200q_paged_attention_args& a, cudaStream_t st) {
   w.cta_part = reinterpret_cast<float*>(p);
   p += paged_align(sizeof(float) * Tile::kPart * 2 * Tile::kWarps * kPagedGrid);
   w.warp_part = reinterpret_cast<float*>(p);
-  // the longest list that the tables can hold: no more CTAs than it would fill
-  const int64_t row_steps = (a.table_width * a.page_size + 15) / 16;
-  if (row_steps > 0 && (row_steps > INT32_MAX || a.requests > INT32_MAX / row_steps / w.heads_per_request)) return B200Q_ERR_TOO_LARGE;
-  const int64_t most = a.requests * row_steps * w.heads_per_request;
+  // no more CTAs than the longest list that the tables can hold would fill
+  const int64_t most = a.requests * ((a.table_width * a.page_size + 15) / 16) * w.heads_per_request;
   int64_t grid = (most + Tile::kWarps * kPagedMinSteps - 1) / (Tile::kWarps * kPagedMinSteps);
   if (grid < 1) grid = 1;
   if (grid > kPagedGrid) grid = kPagedGrid;
@@ -1121,6 +1119,10 @@ static bool paged_fits_tensor_cores(const b200q_paged_attention_args& a) {
 int paged_attention_impl(const b200q_paged_attention_args& a, cudaStream_t st) {
   if (paged_fits_tensor_cores(a)) {
     if (a.requests > kPagedMaxRequests) return B200Q_ERR_TOO_LARGE;
+    // the steps that the tables can hold, of all heads' row tiles, are counted in 31 bits
+    const int rows = paged_rows_of(a.heads / a.kv_heads, a.dim);
+    const int64_t tiles = (int64_t)a.kv_heads * ((a.heads / a.kv_heads + rows - 1) / rows), row_steps = (a.table_width * a.page_size + 15) / 16;
+    if (row_steps > INT32_MAX || tiles > INT32_MAX || (row_steps > 0 && a.requests > INT32_MAX / row_steps / tiles)) return B200Q_ERR_TOO_LARGE;
     if (a.workspace_bytes < paged_attention_workspace_bytes_impl(a.requests, a.heads, a.kv_heads, a.dim, a.cache_dtype) || !a.workspace ||
         reinterpret_cast<uintptr_t>(a.workspace) % 16)
       return B200Q_ERR_BAD_ARGUMENT;

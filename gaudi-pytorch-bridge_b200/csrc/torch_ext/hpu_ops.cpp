@@ -1343,9 +1343,10 @@ const float* paged_scale(const at::Tensor& t, const char* op, const char* name) 
   TORCH_CHECK(t.scalar_type() == at::kFloat && t.numel() == 1, op, ": ", name, " must be a float tensor of one element");
   return t.const_data_ptr<float>();
 }
-// [n0, n1, values]: values contiguous, and everything on boundaries of `bytes` (a view that is not is copied)
+// [n0, n1, values]: values contiguous, and everything on boundaries of `bytes` (a view that is not is copied), where rows can be
 at::Tensor paged_rows(const at::Tensor& t, int64_t bytes) {
   const int64_t size = (int64_t)t.element_size();
+  if (t.size(2) * size % bytes != 0) return t.size(2) <= 1 || t.stride(2) == 1 ? t : t.contiguous();
   auto off = [&](int64_t stride) { return stride * size % bytes != 0; };
   const bool plain = (t.size(2) <= 1 || t.stride(2) == 1) && (t.size(0) <= 1 || !off(t.stride(0))) && (t.size(1) <= 1 || !off(t.stride(1))) &&
                      reinterpret_cast<uintptr_t>(t.const_data_ptr()) % bytes == 0;

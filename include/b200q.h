@@ -561,7 +561,10 @@ int b200q_qk_norm_rope_append(const b200q_append_args* args);
  * workspace     b200q_paged_attention_workspace_bytes(...) bytes, 16-byte aligned, not shared by calls that may overlap
  * dim = 64, 128 or 256 with pages of a multiple of 16 tokens, and caches and q whose bases and strides are multiples of 16
  * bytes run the tensor-core kernel; other head dimensions (<= 256) and layouts, or force_plain = 1, a plain CUDA kernel.
- * The former wants requests <= 8192 and requests * table_width * page_size / 16 < 2^31 (B200Q_ERR_TOO_LARGE).
+ * The former wants requests <= 8192 and requests * (table_width * page_size / 16) * kv_heads * t < 2^31 (B200Q_ERR_TOO_LARGE), where a
+ * tile is 8 query heads of a key/value head, 16 where more than 8 share it (and dim < 256), and t the tiles of a group.  Results do
+ * not depend on timing: the same call gives the same bytes.  A row whose scores are all -inf counts as empty.
+ * As with the other entry points, make the first call on a device before a stream capture.
  */
 typedef struct b200q_paged_attention_args {
   const void* q;

@@ -83,6 +83,9 @@ def _attend(**kw):
     (dict(requests=-1), BAD), (dict(heads=-4), BAD), (dict(kv_heads=0), BAD), (dict(heads=5), BAD), (dict(dim=0), BAD), (dict(num_pages=-1), BAD),
     (dict(page_size=0), BAD), (dict(table_width=-1), BAD), (dict(window=-1), BAD), (dict(cache_dtype=abi.F32), BAD), (dict(out_dtype=abi.E5M2), BAD),
     (dict(q=None), BAD), (dict(out=None), BAD), (dict(kv_lens=None), BAD), (dict(block_table=None), BAD), (dict(k_cache=None), BAD), (dict(v_cache=None), BAD),
+    (dict(requests=8193), TOO_LARGE), (dict(requests=8192, table_width=1 << 18, page_size=16), TOO_LARGE), (dict(table_width=1 << 30, page_size=1 << 30), TOO_LARGE),
+    (dict(kv_heads=128, heads=128 * 20, requests=1024, table_width=8192), TOO_LARGE), (dict(workspace=None), BAD), (dict(workspace=AT, workspace_bytes=1000), BAD),
+    (dict(workspace=AT + 8, workspace_bytes=1 << 30), BAD),
     (dict(dim=257), UNSUPPORTED), (dict(num_pages=1 << 31), TOO_LARGE), (dict(page_size=1 << 31), TOO_LARGE), (dict(table_width=1 << 31), TOO_LARGE),
 ])
 def test_attention_refuses(kw, rc):
@@ -152,3 +155,17 @@ def test_oracle_attention_against_dense():
         assert torch.allclose(lse[b], s.logsumexp(-1))
         assert torch.allclose(out[b], torch.einsum("hn,nhd->hd", s.softmax(-1), vv) * 2.0)
     assert math.isinf(O.paged_attention(q, k, v, table, torch.tensor([0, -3]), 0.3)[1].max())
+
+
+def test_paged_attention_kernels_do_not_spill():
+    """Nothing of the attention kernels lives in local memory (a step of theirs is some 200 instructions)."""
+    import os
+    import re
+    from conftest import ROOT
+    path = os.path.join(ROOT, "gaudi-pytorch-bridge_b200", "build", "paged_attention.ptxas")
+    if not os.path.exists(path):
+        pytest.skip("the kernels were not built in this tree")
+    with open(path) as f:
+        kernels = re.findall(r"Compiling entry function '(\S*paged\S*)'.*?\n.*?\n\s*(\d+) bytes stack frame, (\d+) bytes spill stores", f.read())
+    assert len(kernels) > 15
+    assert [k for k in kernels if k[1:] != ("0", "0")] == []

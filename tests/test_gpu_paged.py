@@ -338,6 +338,42 @@ def test_attention_lengths(lens, cache, dim):
     _attend_check(lens, 8, 1, dim, cache, 16, seed=len(lens))
 
 
+@pytest.mark.parametrize("heads,kv,dim,cache,window", [(8, 8, 128, E4M3, 0), (64, 8, 64, BF16, 0), (80, 4, 128, E4M3, 0), (4, 4, 256, E4M3, 0), (16, 16, 64, E5M2, 33),
+                                                       (24, 8, 128, BF16, 20)])
+def test_attention_heads_side_by_side(heads, kv, dim, cache, window):
+    """Rows enough for all warps: neighbouring heads go side by side, and rows are cut between CTAs in all places."""
+    lens = [0, 1, 200, 15, 16, 17] + [(37 * i) % 150 for i in range(90)] + [0, 0, 333]
+    _attend_check(lens, heads, kv, dim, cache, 16, window=window, seed=dim)
+
+
+@pytest.mark.parametrize("heads,kv,dim,cache,lens", [(8, 8, 64, E4M3, [23000, 9000]), (8, 4, 128, BF16, [1, 0, 70000]), (3, 1, 64, BF16, [300000])])
+def test_attention_long_rows(heads, kv, dim, cache, lens):
+    """Rows that every CTA has a part of, with a warp's share above and below what puts heads side by side."""
+    _attend_check(lens, heads, kv, dim, cache, 64)
+
+
+@pytest.mark.parametrize("requests", [4096, 4097, 8192])
+def test_attention_many_requests(requests):
+    """Up to 4096 requests' lengths are kept on chip; 8192 is the most."""
+    _attend_check([(i * 7) % 19 for i in range(requests)], 1, 1, 64, BF16, 16)
+
+
+def test_attention_too_many_requests():
+    q, kc = torch.zeros(8193, 1, 64, dtype=BF16).cuda(), torch.zeros(1, 16, 1, 64, dtype=BF16).cuda()
+    with pytest.raises(RuntimeError, match="maximum"):
+        torch.ops.b200q.paged_attention(q, kc, kc, torch.zeros(8193, 1, dtype=torch.int32).cuda(), torch.zeros(8193, dtype=torch.int32).cuda(), 1.0)
+
+
+def test_attention_repeats_its_bytes():
+    p = _Paged([5000, 1, 777, 2048, 64, 3000], 4, 128, E4M3, 16)
+    q = torch.randn(6, 16, 128, generator=p.g).to(BF16).cuda()
+    args = (q, p.kd, p.vd, p.table.cuda(), p.lens.cuda(), 0.1)
+    first, first_lse = torch.ops.b200q.paged_attention(*args)
+    for _ in range(20):
+        out, lse = torch.ops.b200q.paged_attention(*args)
+        assert torch.equal(out, first) and torch.equal(lse, first_lse)
+
+
 @pytest.mark.parametrize("heads,kv", [(64, 8), (32, 32), (128, 1), (7, 7), (14, 2)])
 @pytest.mark.parametrize("cache", [E4M3, BF16])
 def test_attention_heads(heads, kv, cache):
