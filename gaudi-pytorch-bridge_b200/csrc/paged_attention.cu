@@ -421,6 +421,9 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
   }
   pdl_enter();
 
+  // (asked for before anything else, used much later)
+  const float k_scale = a.k_scale_inv ? *a.k_scale_inv : 1.f, v_scale = a.v_scale_inv ? *a.v_scale_inv : 1.f, o_scale = a.out_scale ? *a.out_scale : 1.f;
+
   // ---- the list of steps
   int* const lengths = prefix + requests;  // (where there is room: the rows of the loop then need no loads that wait behind the copies)
   const bool lengths_here = requests <= kPagedLengthsHere;
@@ -464,16 +467,17 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
   // of the `sub`-th row tile of a request: its key/value head, and its first query head in that head's group
   auto kv_of = [&](int sub) { return w.row_tiles == 1 ? sub : sub / w.row_tiles; };
   auto row_of = [&](int sub) { return w.row_tiles == 1 ? 0 : sub % w.row_tiles * Tile::kRows; };
-  const float out_scale = paged_out_scale(a);
+  const float out_scale = v_scale * o_scale;
 
-  // requests that see nothing
-  for (int b = blockIdx.x; b < requests; b += gridDim.x) {
-    if (prefix[b] != (b ? prefix[b - 1] : 0)) continue;
-    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int i = tid; i < a.heads * (DIM / 4); i += 32 * kWarps) paged_store4(a.out, a.out_dtype, (int64_t)b * a.heads * DIM + 4 * i, zero);
-    if (a.lse)
-      for (int i = tid; i < a.heads; i += 32 * kWarps) a.lse[(int64_t)b * a.heads + i] = -INFINITY;
-  }
+  auto write_empty = [&] {  // requests that see nothing
+    for (int b = blockIdx.x; b < requests; b += gridDim.x) {
+      if (prefix[b] != (b ? prefix[b - 1] : 0)) continue;
+      const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int i = tid; i < a.heads * (DIM / 4); i += 32 * kWarps) paged_store4(a.out, a.out_dtype, (int64_t)b * a.heads * DIM + 4 * (int64_t)i, zero);
+      if (a.lse)
+        for (int i = tid; i < a.heads; i += 32 * kWarps) a.lse[(int64_t)b * a.heads + i] = -INFINITY;
+    }
+  };
 
   // ---- this CTA's run, and this warp's
   const int c = blockIdx.x;
@@ -481,6 +485,7 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
   const int ctas = min(wanted, (int)gridDim.x);
   if (c >= ctas) {
     if (tid == 0) w.joins[c].lanes = 0;
+    write_empty();
     return;
   }
   const PagedRuns runs(total, ctas);
@@ -561,7 +566,7 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
     uint32_t qf[kTiles][NT][2];
     float coef[NT][2];  // scores in powers of two for heads 2t, 2t + 1
     int c_lo = 0, c_end = 0, c_left = 0;  // keys of this step before c_lo are not seen, nor those of the row's last step from c_end on
-    const float score_scale = a.softmax_scale * (a.k_scale_inv ? *a.k_scale_inv : 1.f) * 1.44269504088896341f;
+    const float score_scale = a.softmax_scale * k_scale * 1.44269504088896341f;
     constexpr int kQ = Tile::kKChunks * (FMT == B200Q_BF16 ? 4 : 8);  // words of a head per lane
     auto load_queries = [&](const PagedCursor& at, uint32_t (&raw)[NT][kQ]) {
       const int sub = at.sub * lanes + my_lane, kv = kv_of(sub), row0 = row_of(sub);
@@ -846,6 +851,7 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
       }
     }
   }
+  write_empty();
   if (groups == 1) return;
   if (early) {  // into shared memory too, behind the part of the last row
     const float4* from = reinterpret_cast<const float4*>(w.warp_part + ((int64_t)c * kWarps + warp) * Tile::kPart);
@@ -938,7 +944,7 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
 
 // Rows that several CTAs have a part of.  Every block makes the list of them; one (row of heads, lane, head) is a task, of a warp where
 // there are many, and of a whole block where there are fewer than blocks (long rows of few requests, with up to a part per CTA).
-constexpr int kPagedJoinBlocks = 4 * kNumSMs;
+constexpr int kPagedJoinBlocks = 2 * kNumSMs;  // (all resident at once; one per SM leaves 128 x 200 tokens at 31.4 instead of 26.5 us)
 constexpr int kPagedJoinWarps = 8;
 
 template <int DIM, int ROWS, int WARPS>
@@ -968,9 +974,10 @@ __global__ void __launch_bounds__(32 * kPagedJoinWarps) paged_join_kernel(const 
   __syncthreads();
   if (rows == 0) return;
   const int lanes = s_join[0].lanes, per_row = lanes * ROWS, tasks = rows * per_row;
-  const bool by_block = tasks <= (int)gridDim.x;
+  // a warp's task takes a trip to L2 per 8 parts, of which a row has 1 + (ctas - 1) / rows on average; a block's takes one or two
+  const bool by_block = (tasks - 1) / (int)gridDim.x <= (ctas - 1) / (8 * rows);
   const float scale = paged_out_scale(a);
-  for (int task = by_block ? blockIdx.x : blockIdx.x * kPagedJoinWarps + warp; task < tasks; task += by_block ? gridDim.x : gridDim.x * kPagedJoinWarps) {
+  for (int task = blockIdx.x + (by_block ? 0 : gridDim.x * warp); task < tasks; task += by_block ? gridDim.x : gridDim.x * kPagedJoinWarps) {
     const PagedJoin join = s_join[task / per_row];
     const int c = s_cta[task / per_row], l_head = task % per_row / ROWS, row = task % ROWS;
     const int sub = join.sub * lanes + l_head, kv = sub / w.row_tiles, row0 = (sub - kv * w.row_tiles) * ROWS;
