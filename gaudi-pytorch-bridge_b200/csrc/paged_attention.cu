@@ -122,6 +122,10 @@ __global__ void __launch_bounds__(kPlainThreads) paged_attention_plain_kernel(co
 // whole row of a token is read at one time, which is worth 5.0 -> 6.4 TB/s where the heads of a token lie together -- and the
 // kWarps / lanes groups of such warps cut the run again.  A run may begin or end inside a row of steps: such partial results
 // (maximum, sum, output) are joined in the CTA, and, where a row goes on in another CTA, by a second kernel.
+//
+// Measured (from a CUDA graph, shuffled pages): 64 requests of 8192 tokens, 8 key/value heads of 128 in e4m3, 173 us = 6.2 TB/s; the same in bf16, 32
+// requests, 163 us = 6.6 TB/s.  About 9 us of a call do not depend on the length: 3 of dependent loads (lengths, page numbers, first keys), 5 of
+// joining, and the launches.
 constexpr int kPagedGrid = kNumSMs;
 constexpr int kPagedRingBytes = 192 * 1024;
 constexpr int kPagedLaneSteps = 14;   // a warp's steps from which on heads go side by side
@@ -404,7 +408,7 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
   uint8_t* const s_ring = s_raw + (0u - paged_smem(s_raw) & 1023u);  // [warps][kRing] (swizzled tiles repeat every 1024 bytes), then the prefix sums
   __shared__ __align__(8) uint64_t s_bars[kWarps * kStages];
   __shared__ int s_abort;
-  __shared__ int s_sum[kWarps];
+  __shared__ int s_sum[2][kWarps];
   __shared__ int s_state[kWarps], s_b[kWarps], s_sub[kWarps], s_cut_b, s_cut_sub;
   int* prefix = reinterpret_cast<int*>(s_ring + kWarps * Tile::kRing);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -428,28 +432,30 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
   int* const lengths = prefix + requests;  // (where there is room: the rows of the loop then need no loads that wait behind the copies)
   const bool lengths_here = requests <= kPagedLengthsHere;
   {
-    const int per = (requests + 32 * kWarps - 1) / (32 * kWarps);
-    const int b0 = min(tid * per, requests), b1 = min(b0 + per, requests);
-    int sum = 0;
-    for (int b = b0; b < b1; ++b) {
-      const int len = paged_length(a, b);
-      sum += PagedSpan(a, len).steps();
-      prefix[b] = sum;
-      if (lengths_here) lengths[b] = len;
-    }
-    int scan = sum;
+    int sums = 0;
+    for (int base = 0, turn = 0; base < requests; base += 32 * kWarps, turn ^= 1) {
+      const int b = base + tid;
+      int scan = 0;
+      if (b < requests) {
+        const int len = paged_length(a, b);
+        scan = PagedSpan(a, len).steps();
+        if (lengths_here) lengths[b] = len;
+      }
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xFFFFFFFFu, scan, o);
-      if (lane >= o) scan += v;
-    }
-    if (lane == 31) s_sum[warp] = scan;
-    __syncthreads();
-    int before = scan - sum;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xFFFFFFFFu, scan, o);
+        if (lane >= o) scan += v;
+      }
+      if (lane == 31) s_sum[turn][warp] = scan;
+      __syncthreads();  // (the other half of s_sum is written next, and this one only behind the next barrier)
+      int before = sums;
 #pragma unroll
-    for (int i = 0; i < kWarps; ++i)
-      if (i < warp) before += s_sum[i];
-    for (int b = b0; b < b1; ++b) prefix[b] += before;
+      for (int i = 0; i < kWarps; ++i) {
+        if (i < warp) before += s_sum[turn][i];
+        sums += s_sum[turn][i];
+      }
+      if (b < requests) prefix[b] = before + scan;
+    }
     __syncthreads();
   }
   auto span_of = [&](int b) { return PagedSpan(a, lengths_here ? lengths[b] : paged_length(a, b)); };
