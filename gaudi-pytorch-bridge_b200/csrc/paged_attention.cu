@@ -111,15 +111,15 @@ __global__ void __launch_bounds__(kPlainThreads) paged_attention_plain_kernel(co
 //         order: the queries are laid out to match; so may the keys, as long as V follows)
 //   of V: the keys of rows 2t, 2t + 1, 2t + 8, 2t + 9, that is t, t + 4, t + 8, t + 12, bytes (8 c + R(g)) * 16 ... + 15  (the
 //         dimensions are the rows of the second product, which may come in any order too)
-// R exchanges bits (0, 4, 1, 5, 2, 6, 3, 7): with it the eight lanes of a 16-byte access lie in different banks of the
-// swizzled tile.
+// R(0 ... 7) = 0, 4, 1, 5, 2, 6, 3, 7: with it the eight lanes of a 16-byte access lie in different banks of the swizzled tile.  (Where a row
+// is 64 bytes the pieces of V are 8 bytes, and a lane's the g-th.)
 // fp8 values become f16 exactly; the probabilities are rounded to f16 (11 bits, scaled by 2^7 so that the small ones stay normal).
 // For a bf16 cache they are split into two bf16 terms (16 bits) that take a product each.  Queries meet fp8 keys as f16, scaled
 // by a power of two per head, which is exact over 2^22 of a head's largest value.
 //
 // Work is the list of all steps (request-major, then key/value head, then the length), cut into equal runs for the CTAs, so that
 // ragged lengths and few requests load every SM alike.  In a CTA `lanes` warps take neighbouring heads of the same keys -- the
-// whole row of a token is read at one time, which is worth 5.0 -> 6.4 TB/s where the heads of a token lie together -- and the
+// whole row of a token is read at one time, which is worth 5.0 -> 6.2 TB/s where the heads of a token lie together -- and the
 // kWarps / lanes groups of such warps cut the run again.  A run may begin or end inside a row of steps: such partial results
 // (maximum, sum, output) are joined in the CTA, and, where a row goes on in another CTA, by a second kernel.
 //
@@ -141,7 +141,7 @@ struct PagedTile {
   static constexpr int kElt = FMT == B200Q_BF16 ? 2 : 1;
   static constexpr int kRow = DIM * kElt;           // bytes of a key
   static constexpr int kStage = 2 * 16 * kRow;      // keys and values of a step
-    static constexpr int kWarps = DIM == 256 ? 4 : 8;
+  static constexpr int kWarps = DIM == 256 ? 4 : 8;
   static constexpr int kStages = kPagedRingBytes / kWarps / kStage < 8 ? kPagedRingBytes / kWarps / kStage : 8;
   static constexpr int kKChunks = kRow / 64;        // 16-byte pieces of a key per lane
   static constexpr int kVPiece = kRow / 8 < 16 ? 8 : 16;
