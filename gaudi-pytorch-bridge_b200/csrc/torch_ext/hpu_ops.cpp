@@ -1459,7 +1459,10 @@ at::Tensor qk_norm_rope_append(const at::Tensor& q, const at::Tensor& k, const a
               ": both norm weights must have the same dtype");
   for (const at::Tensor* c : {&k_cache, &v_cache}) {
     bool aligned = reinterpret_cast<uintptr_t>(c->const_data_ptr()) % (4 * c->element_size()) == 0;
-    for (int d = 0; d < 3; ++d) aligned = aligned && paged_stride(*c, d) % 4 == 0;
+    for (int d = 0; d < 3; ++d) {
+      aligned = aligned && paged_stride(*c, d) % 4 == 0;
+      TORCH_CHECK(c->size(d) <= 1 || c->stride(d) > 0, op, ": the slots of a cache must not overlap");
+    }
     TORCH_CHECK(aligned, op, ": the caches must lie on boundaries of four values");
   }
   const int64_t row = 4 * (int64_t)q.element_size();

@@ -258,7 +258,7 @@ def test_append_refusals():
                 dict(q_weight=w.float()), dict(k_weight=w.half()), dict(cos_sin=t.bfloat16()), dict(cos_sin=_table(12).cuda()), dict(cos_sin=_table(128).cuda()),
                 dict(positions=None), dict(positions=slots.int()), dict(positions=slots[:2]), dict(slot_map=slots.int()), dict(slot_map=slots[:2]),
                 dict(k_cache=kc.float(), v_cache=vc.float()), dict(k_cache=kc.to(E4M3)), dict(k_cache=kc[:, :, :1], v_cache=vc[:, :, :1]),
-                dict(k_cache=odd, v_cache=odd), dict(k_cache=kc.transpose(2, 3), v_cache=vc.transpose(2, 3)), dict(k_scale=torch.ones(2).cuda()),
+                dict(k_cache=odd, v_cache=odd), dict(k_cache=kc[:1].expand(2, 16, 2, 64)), dict(v_cache=vc[:, :, :1].expand(2, 16, 2, 64)), dict(k_cache=kc.transpose(2, 3), v_cache=vc.transpose(2, 3)), dict(k_scale=torch.ones(2).cuda()),
                 dict(k_scale=torch.ones(1)), dict(q_dtype=F32), dict(slot_map=slots.cpu())):
         with pytest.raises(RuntimeError):
             torch.ops.b200q.qk_norm_rope_append(**{**ok, **bad})
