@@ -113,8 +113,11 @@ __global__ void __launch_bounds__(kPlainThreads) paged_attention_plain_kernel(co
 //         dimensions are the rows of the second product, which may come in any order too)
 // R(0 ... 7) = 0, 4, 1, 5, 2, 6, 3, 7: with it the eight lanes of a 16-byte access lie in different banks of the swizzled tile.  (Where a row
 // is 64 bytes the pieces of V are 8 bytes, and a lane's the g-th.)
-// fp8 values become f16 exactly; the probabilities are rounded to f16 (11 bits, scaled by 2^7 so that the small ones stay normal).
-// For a bf16 cache they are split into two bf16 terms (16 bits) that take a product each.  Queries meet fp8 keys as f16, scaled
+// fp8 values become f16 exactly.  The probabilities of an fp8 cache are f16 too, scaled by 2^7 so that the small ones stay normal: one term
+// (11 bits) where the output is bf16 or e4m3, whose own rounding is 8 bits or fewer, and two terms (22 bits) that take a product each
+// where it is fp32.  Two terms everywhere would be 120.8 -> 130.5 us for 64 requests of 2048 to 8192 tokens (8 key/value heads of 128), a
+// branch in the loop 127; the error of that case's bf16 output is 1.66e-3 with one term and 1.65e-3 with 24 bits.  For a bf16 cache
+// they are two bf16 terms (16 bits), twice as fine as any bf16 output.  Queries meet fp8 keys as f16, scaled
 // by a power of two per head, which is exact over 2^22 of a head's largest value.
 //
 // Work is the list of all steps (request-major, then key/value head, then the length), cut into equal runs for the CTAs, so that
@@ -224,6 +227,11 @@ __device__ __forceinline__ void paged_f16(uint32_t w, uint32_t& lo, uint32_t& hi
 __device__ __forceinline__ uint32_t paged_pack_f16(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float2 paged_unpack_f16(uint32_t v) {
+  float2 r;
+  asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.f32.f16 %0, a;\ncvt.f32.f16 %1, b;\n}" : "=f"(r.x), "=f"(r.y) : "r"(v));
   return r;
 }
 __device__ __forceinline__ void paged_store4(void* out, int dtype, int64_t at, const float (&v)[4]) {
@@ -397,11 +405,12 @@ __device__ __forceinline__ void paged_finish(const b200q_paged_attention_args& a
   if (lane == 0 && a.lse) a.lse[(int64_t)b * a.heads + head] = paged_lse(m, l);
 }
 
-template <int DIM, int FMT, int NT>
+template <int DIM, int FMT, int NT, int TERMS>
 __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
     paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                            const b200q_paged_attention_args a, const PagedWork w) {
   using Tile = PagedTile<DIM, FMT, NT>;
+  static_assert(TERMS == 2 || FMT != B200Q_BF16, "a bf16 term alone would be 8 bits");
   constexpr int kWarps = Tile::kWarps, kWarpBits = kWarps == 8 ? 3 : 2, kStages = Tile::kStages, kTiles = Tile::kTiles;
   static_assert(1 << kWarpBits == kWarps, "a power of two");
   extern __shared__ __align__(1024) uint8_t s_raw[];
@@ -740,7 +749,14 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < 2; ++i) p_hi[n][i] = paged_transpose(paged_pack_f16(x[2 * i], x[2 * i + 1]));
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t hi = paged_pack_f16(x[2 * i], x[2 * i + 1]);
+            p_hi[n][i] = paged_transpose(hi);
+            if (TERMS == 2) {
+              const float2 back = paged_unpack_f16(hi);
+              p_lo[n][i] = paged_transpose(paged_pack_f16(x[2 * i] - back.x, x[2 * i + 1] - back.y));
+            }
+          }
         }
       }
       // output: dimensions x heads
@@ -786,8 +802,11 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
               paged_f16<FMT>(__byte_perm(v[0][j], v[1][j], sel), a0, a1);
               paged_f16<FMT>(__byte_perm(v[2][j], v[3][j], sel), a2, a3);
 #pragma unroll
-              for (int n = 0; n < NT; ++n)
-                paged_mma<FMT>(acc.o[(i * Tile::kVPiece + j * 4) / 2 + h][n], a0, a1, a2, a3, p_hi[n][0], p_hi[n][1]);
+              for (int n = 0; n < NT; ++n) {
+                auto& o = acc.o[(i * Tile::kVPiece + j * 4) / 2 + h][n];
+                paged_mma<FMT>(o, a0, a1, a2, a3, p_hi[n][0], p_hi[n][1]);
+                if (TERMS == 2) paged_mma<FMT>(o, a0, a1, a2, a3, p_lo[n][0], p_lo[n][1]);
+              }
             }
           }
         }
@@ -1061,10 +1080,10 @@ static int paged_map(CUtensorMap* map, const void* base, const b200q_paged_atten
   return r == CUDA_SUCCESS ? B200Q_OK : B200Q_ERR_UNSUPPORTED;
 }
 
-template <int DIM, int FMT, int NT>
+template <int DIM, int FMT, int NT, int TERMS>
 static int paged_launch(const b200q_paged_attention_args& a, cudaStream_t st) {
   using Tile = PagedTile<DIM, FMT, NT>;
-  auto kernel = paged_attention_kernel<DIM, FMT, NT>;
+  auto kernel = paged_attention_kernel<DIM, FMT, NT, TERMS>;
   static std::atomic<int> ready[kMaxDevices];
   const int dev = current_device_index();
   if (dev < 0) return B200Q_ERR_CUDA;
@@ -1103,19 +1122,24 @@ static int paged_launch(const b200q_paged_attention_args& a, cudaStream_t st) {
   return B200Q_OK;
 }
 
-template <int DIM, int FMT>
+template <int DIM, int FMT, int TERMS>
 static int paged_launch_rows(const b200q_paged_attention_args& a, cudaStream_t st) {
   if constexpr (DIM < 256) {
-    if (paged_rows_of(a.heads / a.kv_heads, DIM) == 16) return paged_launch<DIM, FMT, 2>(a, st);
+    if (paged_rows_of(a.heads / a.kv_heads, DIM) == 16) return paged_launch<DIM, FMT, 2, TERMS>(a, st);
   }
-  return paged_launch<DIM, FMT, 1>(a, st);
+  return paged_launch<DIM, FMT, 1, TERMS>(a, st);
+}
+// One term for an fp8 cache where the output is rounded to 8 bits or fewer, two where it is fp32 (see above).
+template <int DIM, int FMT>
+static int paged_launch_terms(const b200q_paged_attention_args& a, cudaStream_t st) {
+  return a.out_dtype == B200Q_F32 ? paged_launch_rows<DIM, FMT, 2>(a, st) : paged_launch_rows<DIM, FMT, 1>(a, st);
 }
 template <int DIM>
 static int paged_launch_dtype(const b200q_paged_attention_args& a, cudaStream_t st) {
   switch (a.cache_dtype) {
-    case B200Q_BF16: return paged_launch_rows<DIM, B200Q_BF16>(a, st);
-    case B200Q_E4M3: return paged_launch_rows<DIM, B200Q_E4M3>(a, st);
-    default: return paged_launch_rows<DIM, B200Q_E5M2>(a, st);
+    case B200Q_BF16: return paged_launch_rows<DIM, B200Q_BF16, 2>(a, st);
+    case B200Q_E4M3: return paged_launch_terms<DIM, B200Q_E4M3>(a, st);
+    default: return paged_launch_terms<DIM, B200Q_E5M2>(a, st);
   }
 }
 
