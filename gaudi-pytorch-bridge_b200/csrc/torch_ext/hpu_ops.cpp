@@ -1434,14 +1434,16 @@ at::Tensor qk_norm_rope_append(const at::Tensor& q, const at::Tensor& k, const a
   TORCH_CHECK(out_dtype == at::kBFloat16 || is_fp8(out_dtype), op, ": q_dtype must be bfloat16, float8_e4m3fn or float8_e5m2, got ", out_dtype);
   TORCH_CHECK(slot_map.scalar_type() == at::kLong && slot_map.dim() == 1 && slot_map.numel() == tokens, op,
               ": slot_map must be an int64 tensor of one slot per token");
-  int64_t rotary = 0;
+  int64_t rotary = 0, max_positions = 0;
   if (cos_sin.defined()) {
     TORCH_CHECK(cos_sin.scalar_type() == at::kFloat && cos_sin.dim() == 2, op, ": cos_sin must be a float tensor [positions, rotary_dim]");
     rotary = cos_sin.size(1);
     TORCH_CHECK(rotary >= 8 && rotary <= dim && rotary % 8 == 0, op, ": rotary_dim must be a multiple of 8 and at most the head dimension, got ", rotary);
     TORCH_CHECK(positions.defined() && positions.scalar_type() == at::kLong && positions.dim() == 1 && positions.numel() == tokens, op,
                 ": a rotation needs positions, an int64 tensor of one position per token");
-    cos_sin = cos_sin.contiguous();
+    max_positions = cos_sin.size(0);
+    // (a table of no positions has no address, which would mean no rotation; nothing reads the one it gets here)
+    cos_sin = max_positions ? cos_sin.contiguous() : new_tensor({1, rotary}, at::kFloat, dev);
     if (reinterpret_cast<uintptr_t>(cos_sin.const_data_ptr()) % 16) cos_sin = cos_sin.clone();
     positions = positions.contiguous();
   }
@@ -1481,7 +1483,7 @@ at::Tensor qk_norm_rope_append(const at::Tensor& q, const at::Tensor& k, const a
   a.eps = (float)eps;
   if (cos_sin.defined()) {
     a.cos_sin = cos_sin.const_data_ptr<float>();
-    a.max_positions = cos_sin.size(0);
+    a.max_positions = max_positions;
     a.rotary_dim = (int)rotary;
     a.interleaved = interleaved;
     a.positions = positions.const_data_ptr<int64_t>();

@@ -515,7 +515,8 @@ int b200q_paged_plan(const int32_t* context_lens, const int32_t* new_lens, int64
  *               contiguous; strides multiples of 4, bases aligned to four elements
  * dim           a multiple of 8, at most 256;  rotary_dim a multiple of 8, at most dim
  * q_weight, k_weight   [dim] of weight_dtype (F32 / BF16), aligned like q; NULL = no norm
- * cos_sin       fp32 [max_positions][rotary_dim], 16-byte aligned, or NULL (no rotation; positions is not read)
+ * cos_sin       fp32 [max_positions][rotary_dim], 16-byte aligned, or NULL (no rotation; positions is not read).  A table of no positions
+ *               is max_positions = 0 with any other address: every position is then outside it
  * caches        cache_dtype (BF16 / E4M3 / E5M2), element (page, slot of the page, head) at page * page_stride +
  *               slot * slot_stride + head * head_stride (elements, multiples of 4), values contiguous, bases aligned to
  *               four elements; num_pages * page_size < 2^31

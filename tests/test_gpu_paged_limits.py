@@ -29,3 +29,16 @@ def test_fp32_output_has_more_bits_than_a_half(cache, heads, kv, dim):
     got, got_lse = torch.ops.b200q.paged_attention(q.cuda(), p.k.cuda(), p.vd, p.table.cuda(), p.lens.cuda(), scale, out_dtype=F32)
     _close(got, want, 2.0 ** -23 * want.abs() + 2.0 ** (-14 if cache == BF16 else -15) * size)
     _close(got_lse, lse, 2.0 ** -16 + 2.0 ** -22 * torch.where(lse.isfinite(), lse.abs(), 0.0))
+
+
+# ----------------------------------------------------------------------------- append
+@pytest.mark.parametrize("rot", [8, 64])
+def test_append_with_a_table_of_no_positions(rot):
+    """Every position is outside such a table: what turns becomes NaN, values are stored as ever."""
+    x = torch.randn(4, 3, 64).to(BF16).cuda()
+    kc, vc = torch.zeros(2, 1, 16, 1, 64, dtype=BF16).cuda()
+    at = torch.arange(4).cuda()
+    q = torch.ops.b200q.qk_norm_rope_append(x[:, :1], x[:, 1:2], x[:, 2:], None, None, 1e-6, torch.empty(0, rot).cuda(), at, False, at, kc, vc)
+    for t in (q, kc[0, :4]):
+        assert bool(t[..., :rot].isnan().all()) and bool(t[..., rot:].isfinite().all())
+    assert torch.equal(vc[0, :4], x[:, 2:])
