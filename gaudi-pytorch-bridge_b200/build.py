@@ -38,7 +38,7 @@ def _run(cmd, quiet=True):
 def build_kernels(force=False, ptxas_verbose=False):
     os.makedirs(LIB, exist_ok=True)
     os.makedirs(OBJ, exist_ok=True)
-    headers = glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(ROOT, "include", "*.h"))
+    headers = glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(CSRC, "*.h")) + glob.glob(os.path.join(ROOT, "include", "*.h"))
     objs = []
     log = ""
     for src in sorted(glob.glob(os.path.join(CSRC, "*.cu"))):
@@ -65,7 +65,7 @@ def build_torch_ext(force=False):
 
     src = os.path.join(CSRC, "torch_ext", "hpu_ops.cpp")
     so = os.path.join(LIB, "b200_hpu_ops_ext.so")
-    deps = [src, os.path.join(ROOT, "include", "b200q.h"), os.path.join(LIB, "libb200q.so")]
+    deps = [src, os.path.join(CSRC, "paged_layout.h"), os.path.join(ROOT, "include", "b200q.h"), os.path.join(LIB, "libb200q.so")]
     if not (force or _newer(so, deps)):
         return so
     tlib = os.path.join(os.path.dirname(torch.__file__), "lib")
@@ -74,7 +74,7 @@ def build_torch_ext(force=False):
         inc += ["-isystem", p]
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),
            "-DTORCH_API_INCLUDE_EXTENSION_H", *inc, "-isystem", "/usr/local/cuda/include",
-           "-I", os.path.join(ROOT, "include"), src, "-o", so,
+           "-I", os.path.join(ROOT, "include"), "-I", CSRC, src, "-o", so,
            "-L", LIB, "-lb200q", "-Wl,-rpath,$ORIGIN", "-L", tlib, "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda",
            "-ltorch_cuda", "-Wl,-rpath," + tlib]
     _run(cmd)

@@ -6,6 +6,7 @@
 #include "fp8_misc.cuh"
 #include "gemm_common.cuh"
 #include "paged.cuh"
+#include "paged_layout.h"
 #include "tcgen05_ptx.cuh"
 
 namespace b200q {
@@ -483,6 +484,12 @@ int b200q_qk_norm_rope_append(const b200q_append_args* a) {
   for (int64_t s : {a->q_token_stride, a->q_head_stride, a->k_token_stride, a->k_head_stride, a->v_token_stride, a->v_head_stride,
                     a->k_page_stride, a->k_slot_stride, a->k_cache_head_stride, a->v_page_stride, a->v_slot_stride, a->v_cache_head_stride})
     if (s % 4) return B200Q_ERR_UNSUPPORTED;
+  if (a->kv_heads > 0) {
+    const int64_t sizes[3] = {a->num_pages, a->page_size, a->kv_heads}, elt = a->cache_dtype == B200Q_BF16 ? 2 : 1;
+    const CacheLayout k(a->k_cache, elt, a->dim, sizes, {a->k_page_stride, a->k_slot_stride, a->k_cache_head_stride});
+    const CacheLayout v(a->v_cache, elt, a->dim, sizes, {a->v_page_stride, a->v_slot_stride, a->v_cache_head_stride});
+    if (!k.apart() || !v.apart() || !k.apart_from(v)) return B200Q_ERR_BAD_ARGUMENT;
+  }
   return qk_norm_rope_append_impl(*a, static_cast<cudaStream_t>(a->stream));
 }
 

@@ -17,6 +17,7 @@
 #include <variant>
 
 #include "b200q.h"
+#include "paged_layout.h"
 
 namespace {
 
@@ -1357,6 +1358,11 @@ at::Tensor paged_rows(const at::Tensor& t, int64_t bytes) {
 // A stride that no index uses (one entry) is whatever the view says; the kernels want it aligned.
 int64_t paged_stride(const at::Tensor& t, int64_t dim) { return t.size(dim) > 1 ? t.stride(dim) : 0; }
 
+b200q::CacheLayout paged_layout(const at::Tensor& c) {
+  return b200q::CacheLayout(c.const_data_ptr(), (int64_t)c.element_size(), c.size(3), {c.size(0), c.size(1), c.size(2)},
+                            {paged_stride(c, 0), paged_stride(c, 1), paged_stride(c, 2)});
+}
+
 struct PagedCache {
   int64_t pages, page_size, kv_heads, dim;
 };
@@ -1461,12 +1467,11 @@ at::Tensor qk_norm_rope_append(const at::Tensor& q, const at::Tensor& k, const a
               ": both norm weights must have the same dtype");
   for (const at::Tensor* c : {&k_cache, &v_cache}) {
     bool aligned = reinterpret_cast<uintptr_t>(c->const_data_ptr()) % (4 * c->element_size()) == 0;
-    for (int d = 0; d < 3; ++d) {
-      aligned = aligned && paged_stride(*c, d) % 4 == 0;
-      TORCH_CHECK(c->size(d) <= 1 || c->stride(d) > 0, op, ": the slots of a cache must not overlap");
-    }
+    for (int d = 0; d < 3; ++d) aligned = aligned && paged_stride(*c, d) % 4 == 0;
     TORCH_CHECK(aligned, op, ": the caches must lie on boundaries of four values");
+    TORCH_CHECK(paged_layout(*c).apart(), op, ": the slots of a cache must not overlap");
   }
+  TORCH_CHECK(paged_layout(k_cache).apart_from(paged_layout(v_cache)), op, ": k_cache and v_cache must not overlap");
   const int64_t row = 4 * (int64_t)q.element_size();
   at::Tensor qr = paged_rows(q, row), kr = paged_rows(k, row), vr = paged_rows(v, row), slots = slot_map.contiguous();
   at::Tensor out = new_tensor(q.sizes(), out_dtype, dev);

@@ -509,7 +509,9 @@ int b200q_paged_plan(const int32_t* context_lens, const int32_t* new_lens, int64
  *   q_out = T(y * q_scale);  k_cache[slot] = T(y * k_scale);  v_cache[slot] = T(v * v_scale)
  * computed in fp32 and rounded once (fp8: to nearest even, saturating; NaN -> 0x7F).  Tokens with a slot outside
  * [0, num_pages * page_size) write nothing to the caches.  A position outside [0, max_positions) turns q and k into NaN.
- * Slots that are not negative must differ from one another.
+ * Slots that are not negative must differ from one another.  The slots and heads of a cache must lie apart, each stride at least as
+ * long as all that lies inside it, and no byte may belong to both caches (they may alternate within one allocation): B200Q_ERR_BAD_ARGUMENT.
+ * q, k, v and the other inputs must not overlap the outputs.
  *
  * q / k / v     src_dtype (F32 / BF16) [tokens][heads or kv_heads][dim], token and head strides in elements, values
  *               contiguous; strides multiples of 4, bases aligned to four elements

@@ -42,3 +42,48 @@ def test_append_with_a_table_of_no_positions(rot):
     for t in (q, kc[0, :4]):
         assert bool(t[..., :rot].isnan().all()) and bool(t[..., rot:].isfinite().all())
     assert torch.equal(vc[0, :4], x[:, 2:])
+
+
+def _append_to(kc, vc, tokens=7):
+    kv, dim = kc.shape[2:]
+    x = torch.randn(tokens, 3 * kv, dim).to(BF16).cuda()
+    slots = torch.randperm(kc.shape[0] * kc.shape[1])[:tokens].cuda()
+    torch.ops.b200q.qk_norm_rope_append(x[:, :kv], x[:, kv:2 * kv], x[:, 2 * kv:], None, None, 1e-6, None, None, False, slots, kc, vc)
+    return x[:, kv:2 * kv], x[:, 2 * kv:], slots
+
+
+def test_append_refuses_caches_that_overlap():
+    """Strides too short for what lies inside them, one tensor as both caches, two that share part of an allocation."""
+    flat = torch.zeros(1 << 14, dtype=BF16).cuda()
+    view = lambda s, at=0, n=(4, 16, 2, 64): flat.as_strided(n, (*s, 1), at)  # noqa: E731
+    good, far = view((2048, 128, 64)), torch.zeros(4, 16, 2, 64, dtype=BF16).cuda()
+    _append_to(good, far)
+    for bad in ((2048, 128, 4), (2048, 64, 64), (1024, 128, 64), (0, 128, 64), (2048, 0, 64), (2048, 128, 60)):
+        for kc, vc in ((view(bad), far), (far, view(bad))):
+            with pytest.raises(RuntimeError, match="must not overlap"):
+                _append_to(kc, vc)
+    for other in (good, view((2048, 128, 64), 64), view((2048, 128, 64), 6144), view((2048, 64, 1024), 2048)):
+        with pytest.raises(RuntimeError, match="must not overlap"):
+            _append_to(good, other)
+
+
+@pytest.mark.parametrize("form", ["halves", "pages", "slots", "heads", "values", "orders"])
+def test_append_to_caches_in_one_allocation(form):
+    n, page, kv, dim = 5, 16, 3, 64
+    if form == "orders":  # a page of keys slot by slot, then one of values head by head
+        pool = torch.zeros(n, 2, page * kv * dim, dtype=BF16).cuda()
+        kc, vc = pool[:, 0].view(n, page, kv, dim), pool[:, 1].view(n, kv, page, dim).transpose(1, 2)
+    else:
+        at = ("halves", "pages", "slots", "heads", "values").index(form)
+        sizes = [n, page, kv]
+        if form == "values":
+            pool = torch.zeros(n, page, kv, 2 * dim, dtype=BF16).cuda()
+            kc, vc = pool[..., :dim], pool[..., dim:]
+        else:
+            pool = torch.zeros(*sizes[:at], 2, *sizes[at:], dim, dtype=BF16).cuda()
+            kc, vc = pool.select(at, 0), pool.select(at, 1)
+    k, v, slots = _append_to(kc, vc)
+    for cache, x in ((kc, k), (vc, v)):
+        want = torch.zeros(n, page, kv, dim, dtype=BF16).cuda()
+        want.view(-1, kv, dim)[slots] = x
+        assert torch.equal(cache, want)
