@@ -119,8 +119,8 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PagedPla
     }
   }
   const int stride = gridDim.x * kPlanThreads;
-  for (int i = blockIdx.x * kPlanThreads + tid; i < total_pages; i += stride) {
-    const int b = first_above(page_end, p.requests, i);
+  for (int64_t i64 = blockIdx.x * kPlanThreads + tid; i64 < total_pages; i64 += stride) {  // (up to 2^31 - 1 of them)
+    const int i = (int)i64, b = first_above(page_end, p.requests, i);
     const PlanRequest r = plan_request(p, b);
     p.table[b * p.table_stride + r.need - (page_end[b] - i)] = free_page(i);
   }

@@ -87,3 +87,18 @@ def test_append_to_caches_in_one_allocation(form):
         want = torch.zeros(n, page, kv, dim, dtype=BF16).cuda()
         want.view(-1, kv, dim)[slots] = x
         assert torch.equal(cache, want)
+
+
+# ----------------------------------------------------------------------------- plan
+def test_plan_of_almost_2_to_the_31_pages():
+    """The largest table that is taken, all of it new: the pages are counted to within 2^14 of the type's end."""
+    requests, width = 8192, 262143
+    whole = torch.full((requests * width + 2048,), 7, dtype=torch.int32, device="cuda")
+    table = whole[1024:-1024].view(requests, width)
+    ctx, new = torch.zeros(requests, dtype=torch.int32).cuda(), torch.full((requests,), width, dtype=torch.int32).cuda()
+    slots, pos, start, lens, head = torch.ops.b200q.paged_plan(ctx, new, table, _i32([5, 6]).cuda(), None, 1, 200000)
+    assert head.tolist() == [requests * width] and lens.tolist() == [width] * requests
+    assert table[0, :3].tolist() == [5, 6, -1] and int((table == -1).sum()) == requests * width - 2
+    assert bool((whole[:1024] == 7).all()) and bool((whole[-1024:] == 7).all())
+    assert slots[:3].tolist() == [5, 6, -1] and bool((slots[2:] == -1).all()) and torch.equal(pos.cpu(), torch.arange(200000))
+    assert torch.equal(start.cpu(), (torch.arange(requests + 1) * width).int())
