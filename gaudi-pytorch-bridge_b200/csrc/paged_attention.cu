@@ -488,9 +488,9 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
     for (int b = blockIdx.x; b < requests; b += gridDim.x) {
       if (prefix[b] != (b ? prefix[b - 1] : 0)) continue;
       const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-      for (int i = tid; i < a.heads * (DIM / 4); i += 32 * kWarps) paged_store4(a.out, a.out_dtype, (int64_t)b * a.heads * DIM + 4 * (int64_t)i, zero);
+      for (int64_t i = tid; i < (int64_t)a.heads * (DIM / 4); i += 32 * kWarps) paged_store4(a.out, a.out_dtype, (int64_t)b * a.heads * DIM + 4 * i, zero);
       if (a.lse)
-        for (int i = tid; i < a.heads; i += 32 * kWarps) a.lse[(int64_t)b * a.heads + i] = -INFINITY;
+        for (int64_t i = tid; i < a.heads; i += 32 * kWarps) a.lse[(int64_t)b * a.heads + i] = -INFINITY;
     }
   };
 

@@ -102,3 +102,14 @@ def test_plan_of_almost_2_to_the_31_pages():
     assert bool((whole[:1024] == 7).all()) and bool((whole[-1024:] == 7).all())
     assert slots[:3].tolist() == [5, 6, -1] and bool((slots[2:] == -1).all()) and torch.equal(pos.cpu(), torch.arange(200000))
     assert torch.equal(start.cpu(), (torch.arange(requests + 1) * width).int())
+
+
+# ----------------------------------------------------------------------------- attention: sizes
+def test_attention_empty_rows_of_very_many_heads():
+    """2^31 values of four in one request's output, which are all to be cleared."""
+    heads, dim = 1 << 25, 256
+    dirty = torch.ones(1, heads, dim, dtype=BF16, device="cuda")
+    del dirty  # (the output takes its place)
+    q, kc = torch.ones(1, heads, 1, dtype=BF16, device="cuda").expand(1, heads, dim).contiguous(), torch.ones(1, 16, 1, dim, dtype=BF16).cuda()
+    out, lse = torch.ops.b200q.paged_attention(q, kc, kc, _i32([[0]]).cuda(), _i32([0]).cuda(), 1.0)
+    assert not bool(out.any()) and bool((lse == -math.inf).all())
