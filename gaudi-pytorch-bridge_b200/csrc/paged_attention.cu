@@ -712,15 +712,19 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
         float x[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) s[n][i] += s2[n][i];
+        // The product is rounded before the maximum is taken away, as it is where the maximum is found: the difference of a fused and a rounded
+        // product of scores of 2^27 and more is a large number itself, and the largest probability then infinite, or none at all.
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[n][i] = (i < 2 ? ok0 : ok1) ? __fmul_rn(s[n][i], coef[n][i & 1]) : -INFINITY;
         auto exponents = [&] {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = (i < 2 ? ok0 : ok1) ? fmaf(s[n][i], coef[n][i & 1], -acc.m[n][i & 1]) : -INFINITY;
+          for (int i = 0; i < 4; ++i) x[i] = __fsub_rn(s[n][i], acc.m[n][i & 1]);
         };
         exponents();
         if (__any_sync(0xFFFFFFFFu, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) > kPagedRescale)) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            float top = fmaxf(ok0 ? s[n][i] * coef[n][i] : -INFINITY, ok1 ? s[n][i + 2] * coef[n][i] : -INFINITY);
+            float top = fmaxf(s[n][i], s[n][i + 2]);
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
             const float raised = top > acc.m[n][i] + kPagedRescale ? top - kPagedShift : acc.m[n][i];

@@ -113,3 +113,21 @@ def test_attention_empty_rows_of_very_many_heads():
     q, kc = torch.ones(1, heads, 1, dtype=BF16, device="cuda").expand(1, heads, dim).contiguous(), torch.ones(1, 16, 1, dim, dtype=BF16).cuda()
     out, lse = torch.ops.b200q.paged_attention(q, kc, kc, _i32([[0]]).cuda(), _i32([0]).cuda(), 1.0)
     assert not bool(out.any()) and bool((lse == -math.inf).all())
+
+
+@pytest.mark.parametrize("cache,heads,kv,dim", [(E4M3, 8, 1, 128), (BF16, 4, 2, 64), (E5M2, 12, 1, 64), (BF16, 2, 1, 256), (E4M3, 2, 1, 72)])
+@pytest.mark.parametrize("size", [-3e8, 1e9, -1e12, 3e20, -1e38, 2.2e38])
+def test_attention_large_scores(cache, heads, kv, dim, size):
+    """All keys of a row score the same, up to 3.2e38 away from 0 in powers of two, where neighbouring numbers are far apart.  The roundings of
+    a score (its factor's three, its own, two of the way back to powers of e) are 6 * 2^-24 of lse."""
+    p = _Paged([0, 1, 5, 40, 300, 5000], kv, dim, cache, 16, seed=3)
+    k = torch.where(p.k.float().isnan(), math.nan, 0.0)
+    k[..., 0] += 1.0
+    p.k = k.to(cache)
+    q = torch.zeros(6, heads, dim)
+    q[..., 0] = size
+    q = q.to(BF16)
+    want, lse, size = O.paged_attention(q, p.k, p.v, p.table, p.lens, 1.0)
+    got, got_lse = torch.ops.b200q.paged_attention(q.cuda(), p.k.cuda(), p.vd, p.table.cuda(), p.lens.cuda(), 1.0)
+    _close(got.float(), want, 2.0 ** -8 * want.abs() + (2.0 ** -11 + 2.0 ** -13) * size)
+    _close(got_lse, lse, 2.0 ** -21 * torch.where(lse.isfinite(), lse.abs(), 0.0))
