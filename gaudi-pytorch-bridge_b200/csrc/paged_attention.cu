@@ -135,7 +135,7 @@ constexpr int kPagedLaneSteps = 14;   // a warp's steps from which on heads go s
 constexpr int kPagedMinSteps = 2;     // a warp gets at least this many steps while there are enough for the others
 constexpr float kPagedShift = 7.f;    // probabilities are held relative to 2^(maximum - 7) ...
 constexpr float kPagedRescale = 15.f; // ... and the maximum is raised when one would pass 2^15 (f16 ends at 2^16)
-constexpr float kPagedNoMax = -3.0e38f;
+constexpr float kPagedNoMax = -3.402823466e38f;  // the lowest finite number: no finite score is below it
 constexpr int kPagedLengthsHere = (int)kPagedMaxRequests / 2;  // up to so many requests' lengths lie in shared memory beside the sums
 constexpr int kPagedErrCopy = 801;  // status code: a copy of keys and values did not arrive
 

@@ -116,9 +116,10 @@ def test_attention_empty_rows_of_very_many_heads():
 
 
 @pytest.mark.parametrize("cache,heads,kv,dim", [(E4M3, 8, 1, 128), (BF16, 4, 2, 64), (E5M2, 12, 1, 64), (BF16, 2, 1, 256), (E4M3, 2, 1, 72)])
-@pytest.mark.parametrize("size", [-3e8, 1e9, -1e12, 3e20, -1e38, 2.2e38])
+@pytest.mark.parametrize("size", [-3e8, 1e9, -1e12, 3e20, -1e38, 2.2e38, -2.2e38, -2.35e38])
 def test_attention_large_scores(cache, heads, kv, dim, size):
-    """All keys of a row score the same, up to 3.2e38 away from 0 in powers of two, where neighbouring numbers are far apart.  The roundings of
+    """All keys of a row score the same, up to 3.39e38 away from 0 in powers of two, where neighbouring numbers are far apart, and a row
+    of the lowest ones is not an empty one.  The roundings of
     a score (its factor's three, its own, two of the way back to powers of e) are 6 * 2^-24 of lse."""
     p = _Paged([0, 1, 5, 40, 300, 5000], kv, dim, cache, 16, seed=3)
     k = torch.where(p.k.float().isnan(), math.nan, 0.0)
