@@ -23,6 +23,7 @@ EXPORTS = [
     "b200q_softmax_fp8", "b200q_sum_fp8_workspace_bytes", "b200q_sum_fp8", "b200q_in_place_interleave", "b200q_im2col_fp8",
     "b200q_nchw_to_nhwc_u8", "b200q_im2col_nhwc_fp8",
     "b200q_paged_plan", "b200q_qk_norm_rope_append", "b200q_paged_attention_workspace_bytes", "b200q_paged_attention",
+    "b200q_selftest_paged_wait_timeout",
 ]
 
 DTYPE = {torch.float32: F32, torch.bfloat16: BF16, torch.float8_e4m3fn: E4M3, torch.float8_e5m2: E5M2}
@@ -152,6 +153,7 @@ def _bind():
     lib.b200q_paged_attention_workspace_bytes.restype = C.c_size_t
     lib.b200q_paged_attention_workspace_bytes.argtypes = [C.c_int64, C.c_int, C.c_int, C.c_int, C.c_int]
     lib.b200q_paged_attention.argtypes = [C.POINTER(PagedAttentionArgs)]
+    lib.b200q_selftest_paged_wait_timeout.argtypes = [C.POINTER(PagedAttentionArgs), C.c_int, C.c_int, C.c_int]
     return lib
 
 

@@ -120,6 +120,7 @@ int w4a16_gemm_noalloc_impl(const void*, int64_t, const int32_t*, const void*, c
 int paged_plan_impl(const PagedPlanParams&, cudaStream_t);
 int qk_norm_rope_append_impl(const b200q_append_args&, cudaStream_t);
 int paged_attention_impl(const b200q_paged_attention_args&, cudaStream_t);
+int paged_selftest_impl(const b200q_paged_attention_args&, int, int, int, cudaStream_t);
 size_t paged_attention_workspace_bytes_impl(int64_t, int, int, int, int);
 
 static bool is_fp8(int d) { return d == B200Q_E4M3 || d == B200Q_E5M2; }
@@ -498,7 +499,9 @@ size_t b200q_paged_attention_workspace_bytes(int64_t requests, int heads, int kv
   return paged_attention_workspace_bytes_impl(requests, heads, kv_heads, dim, cache_dtype);
 }
 
-int b200q_paged_attention(const b200q_paged_attention_args* a) {
+// What b200q_paged_attention refuses; `nothing`: there is nothing to do.
+static int check_paged_attention(const b200q_paged_attention_args* a, bool* nothing) {
+  *nothing = false;
   if (!a) return B200Q_ERR_BAD_ARGUMENT;
   if (a->requests < 0 || a->heads < 0 || a->kv_heads < 1 || a->heads % a->kv_heads || a->dim < 1 || a->num_pages < 0 || a->page_size < 1 ||
       a->table_width < 0 || a->window < 0)
@@ -507,10 +510,28 @@ int b200q_paged_attention(const b200q_paged_attention_args* a) {
     return B200Q_ERR_BAD_ARGUMENT;
   if (a->dim > 256) return B200Q_ERR_UNSUPPORTED;
   if (a->num_pages > INT32_MAX || a->page_size > INT32_MAX || a->table_width > INT32_MAX) return B200Q_ERR_TOO_LARGE;
-  if (a->requests == 0 || a->heads == 0) return B200Q_OK;
+  if (a->requests == 0 || a->heads == 0) {
+    *nothing = true;
+    return B200Q_OK;
+  }
   if (!a->q || !a->out || !a->kv_lens || (a->table_width > 0 && !a->block_table)) return B200Q_ERR_BAD_ARGUMENT;
   if (a->num_pages > 0 && (!a->k_cache || !a->v_cache)) return B200Q_ERR_BAD_ARGUMENT;
+  return B200Q_OK;
+}
+
+int b200q_paged_attention(const b200q_paged_attention_args* a) {
+  bool nothing;
+  const int rc = check_paged_attention(a, &nothing);
+  if (rc || nothing) return rc;
   return paged_attention_impl(*a, static_cast<cudaStream_t>(a->stream));
+}
+
+int b200q_selftest_paged_wait_timeout(const b200q_paged_attention_args* a, int cta, int warp, int step) {
+  bool nothing;
+  const int rc = check_paged_attention(a, &nothing);
+  if (rc) return rc;
+  if (nothing || cta < 0 || warp < 0 || step < 0) return B200Q_ERR_BAD_ARGUMENT;
+  return paged_selftest_impl(*a, cta, warp, step, static_cast<cudaStream_t>(a->stream));
 }
 
 int b200q_tp_reduce_bcast(const void* stage, void* const* out_ptrs_host, int tp, int me, int64_t rows, int64_t d,

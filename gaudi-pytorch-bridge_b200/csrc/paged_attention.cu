@@ -174,6 +174,7 @@ struct PagedWork {
   float* cta_part;        // [grid][2][warps][kPart]: rows from the CTA before, rows into the CTA behind, of each lane
   float* warp_part;       // [grid][warps][kPart]: rows from the warp before that end inside a warp's run
   int* status;
+  int drop_cta, drop_warp, drop_step;  // self-test: the step of the warp's run whose copies are never made
 };
 
 __device__ __forceinline__ uint32_t paged_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -405,7 +406,8 @@ __device__ __forceinline__ void paged_finish(const b200q_paged_attention_args& a
   if (lane == 0 && a.lse) a.lse[(int64_t)b * a.heads + head] = paged_lse(m, l);
 }
 
-template <int DIM, int FMT, int NT, int TERMS>
+// DROP: the instance of the self-test, in which one step's copies are never made and waits are short.
+template <int DIM, int FMT, int NT, int TERMS, bool DROP = false>
 __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
     paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                            const b200q_paged_attention_args a, const PagedWork w) {
@@ -562,7 +564,8 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
       const int slot = __shfl_sync(0xFFFFFFFFu, now.slot, copied & 31), kv = __shfl_sync(0xFFFFFFFFu, now.kv, copied & 31);
       const uint32_t bar = bars + 8 * stage, dst = ring + stage * Tile::kStage;
       bad = (bad & ~(1u << stage)) | ((uint32_t)(page == (int)a.num_pages) << stage);
-      if (ptx::elect_one()) {
+      const bool made = !DROP || c != w.drop_cta || warp != w.drop_warp || copied != w.drop_step;
+      if (made && ptx::elect_one()) {
         ptx::mbar_arrive_expect_tx(bar, Tile::kStage);
 #pragma unroll
         for (int i = 0; i < Tile::kBoxes; ++i) paged_copy(dst + i * 16 * Tile::kBox, &map_k, bar, i * Tile::kBox, kv, slot, page);
@@ -659,16 +662,7 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
     const uint32_t v_at = Tile::kBox == 128 ? t * 128 + ((rg ^ t) << 4) : t * 64 + (((g >> 1) ^ (t >> 1)) << 4) + (g & 1) * 8;
     int stage = 0;
     uint32_t phase = 0;
-    for (int done = 0; done < todo; ++done) {
-      if (!ptx::mbar_wait_uniform(bars + 8 * stage, phase, &s_abort, w.status, kPagedErrCopy)) {
-        // gives up: waits for the other copies in flight, as far as they come, and leaves
-        for (int s = 1; s < kStages && done + s < copied; ++s) {
-          const int next = (stage + s) % kStages;
-          for (int i = 0; i < 4096 && !ptx::mbar_try_wait(bars + 8 * next, phase ^ (stage + s >= kStages)); ++i) __nanosleep(64);
-        }
-        final_part = from_here = 0;
-        break;
-      }
+    auto step_products = [&] {
       const uint32_t src = ring + stage * Tile::kStage, src_v = src + 16 * Tile::kRow + v_at;
       // scores: keys x heads
       float s[NT][4], s2[NT][4];
@@ -815,9 +809,27 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
           }
         }
       }
-      // the stage of the step before this one is free
-      __syncwarp();
-      copy_step(stage == 0 ? kStages - 1 : stage - 1);
+    };
+    bool failed = false;  // a wait ran out: the rows of what is left of the run become NaN
+    for (int done = 0; done < todo; ++done) {
+      if (!failed && !ptx::mbar_wait_uniform(bars + 8 * stage, phase, &s_abort, w.status, kPagedErrCopy, DROP ? 1u << 12 : ptx::kWaitLimit)) {
+        // gives up: makes no more copies, and waits for the others in flight, as far as they come
+        failed = true;
+        for (int s = 1; s < kStages && done + s < copied; ++s) {
+          const int next = (stage + s) % kStages;
+          for (int i = 0; i < 4096 && !ptx::mbar_try_wait(bars + 8 * next, phase ^ (stage + s >= kStages)); ++i) __nanosleep(64);
+        }
+        copied = todo;
+      }
+      if (failed) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc.l[n][0] = acc.l[n][1] = __int_as_float(0x7FC00000);
+      } else {
+        step_products();
+        // the stage of the step before this one is free
+        __syncwarp();
+        copy_step(stage == 0 ? kStages - 1 : stage - 1);
+      }
       if (++stage == kStages) {
         stage = 0;
         phase ^= 1;
@@ -929,7 +941,7 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
       if (mine) {
         const float* p = part_of(lane) + Tile::kRows * DIM + row;
         pm = p[0];
-        pl = p[Tile::kRows];
+        pl = s_abort ? __int_as_float(0x7FC00000) : p[Tile::kRows];  // (where a wait ran out, a late copy may yet land on a part)
       }
 #pragma unroll
       for (int v = 0; v < kWarps; ++v) {
@@ -1084,10 +1096,13 @@ static int paged_map(CUtensorMap* map, const void* base, const b200q_paged_atten
   return r == CUDA_SUCCESS ? B200Q_OK : B200Q_ERR_UNSUPPORTED;
 }
 
-template <int DIM, int FMT, int NT, int TERMS>
-static int paged_launch(const b200q_paged_attention_args& a, cudaStream_t st) {
+struct PagedDrop {
+  int cta, warp, step;
+};
+template <int DIM, int FMT, int NT, int TERMS, bool DROP = false>
+static int paged_launch(const b200q_paged_attention_args& a, cudaStream_t st, PagedDrop drop = {}) {
   using Tile = PagedTile<DIM, FMT, NT>;
-  auto kernel = paged_attention_kernel<DIM, FMT, NT, TERMS>;
+  auto kernel = paged_attention_kernel<DIM, FMT, NT, TERMS, DROP>;
   static std::atomic<int> ready[kMaxDevices];
   const int dev = current_device_index();
   if (dev < 0) return B200Q_ERR_CUDA;
@@ -1099,6 +1114,9 @@ static int paged_launch(const b200q_paged_attention_args& a, cudaStream_t st) {
   if (int rc = paged_map(&map_k, a.k_cache, a, Tile::kElt, a.k_page_stride, a.k_slot_stride, a.k_head_stride)) return rc;
   if (int rc = paged_map(&map_v, a.v_cache, a, Tile::kElt, a.v_page_stride, a.v_slot_stride, a.v_head_stride)) return rc;
   PagedWork w;
+  w.drop_cta = drop.cta;
+  w.drop_warp = drop.warp;
+  w.drop_step = drop.step;
   w.status = device_status_ptr();
   if (!w.status) return B200Q_ERR_CUDA;
   w.group = a.heads / a.kv_heads;
@@ -1157,16 +1175,21 @@ static bool paged_fits_tensor_cores(const b200q_paged_attention_args& a) {
   return a.q_token_stride % 8 == 0 && a.q_head_stride % 8 == 0;
 }
 
+static int paged_check_tensor_cores(const b200q_paged_attention_args& a) {
+  if (a.requests > kPagedMaxRequests) return B200Q_ERR_TOO_LARGE;
+  // the steps that the tables can hold, of all heads' row tiles, are counted in 31 bits
+  const int rows = paged_rows_of(a.heads / a.kv_heads, a.dim);
+  const int64_t tiles = (int64_t)a.kv_heads * ((a.heads / a.kv_heads + rows - 1) / rows), row_steps = (a.table_width * a.page_size + 15) / 16;
+  if (row_steps > INT32_MAX || tiles > INT32_MAX || (row_steps > 0 && a.requests > INT32_MAX / row_steps / tiles)) return B200Q_ERR_TOO_LARGE;
+  if (a.workspace_bytes < paged_attention_workspace_bytes_impl(a.requests, a.heads, a.kv_heads, a.dim, a.cache_dtype) || !a.workspace ||
+      reinterpret_cast<uintptr_t>(a.workspace) % 16)
+    return B200Q_ERR_BAD_ARGUMENT;
+  return B200Q_OK;
+}
+
 int paged_attention_impl(const b200q_paged_attention_args& a, cudaStream_t st) {
   if (paged_fits_tensor_cores(a)) {
-    if (a.requests > kPagedMaxRequests) return B200Q_ERR_TOO_LARGE;
-    // the steps that the tables can hold, of all heads' row tiles, are counted in 31 bits
-    const int rows = paged_rows_of(a.heads / a.kv_heads, a.dim);
-    const int64_t tiles = (int64_t)a.kv_heads * ((a.heads / a.kv_heads + rows - 1) / rows), row_steps = (a.table_width * a.page_size + 15) / 16;
-    if (row_steps > INT32_MAX || tiles > INT32_MAX || (row_steps > 0 && a.requests > INT32_MAX / row_steps / tiles)) return B200Q_ERR_TOO_LARGE;
-    if (a.workspace_bytes < paged_attention_workspace_bytes_impl(a.requests, a.heads, a.kv_heads, a.dim, a.cache_dtype) || !a.workspace ||
-        reinterpret_cast<uintptr_t>(a.workspace) % 16)
-      return B200Q_ERR_BAD_ARGUMENT;
+    if (int rc = paged_check_tensor_cores(a)) return rc;
     const int rc = a.dim == 64 ? paged_launch_dtype<64>(a, st) : a.dim == 128 ? paged_launch_dtype<128>(a, st) : paged_launch_dtype<256>(a, st);
     if (rc != B200Q_ERR_UNSUPPORTED) return rc;  // (a layout that has no tensor map takes the plain kernel)
   }
@@ -1175,6 +1198,14 @@ int paged_attention_impl(const b200q_paged_attention_args& a, cudaStream_t st) {
   launch_dependent(paged_attention_plain_kernel, dim3((unsigned)blocks), dim3(kPlainThreads), 0, st, a);
   B200Q_LAUNCH_CHECK();
   return B200Q_OK;
+}
+
+// The kernel for heads of 128 in e4m3 with a step whose keys and values never arrive.
+int paged_selftest_impl(const b200q_paged_attention_args& a, int cta, int warp, int step, cudaStream_t st) {
+  if (!paged_fits_tensor_cores(a) || a.dim != 128 || a.cache_dtype != B200Q_E4M3 || a.out_dtype != B200Q_BF16 || paged_rows_of(a.heads / a.kv_heads, 128) != 8)
+    return B200Q_ERR_UNSUPPORTED;
+  if (int rc = paged_check_tensor_cores(a)) return rc;
+  return paged_launch<128, B200Q_E4M3, 1, 1, true>(a, st, {cta, warp, step});
 }
 
 }  // namespace b200q

@@ -569,6 +569,8 @@ int b200q_qk_norm_rope_append(const b200q_append_args* args);
  * tile is 8 query heads of a key/value head, 16 where more than 8 share it (and dim < 256), and t the tiles of a group.  Results do
  * not depend on timing: the same call gives the same bytes.  A row whose scores are all -inf counts as empty.
  * As with the other entry points, make the first call on a device before a stream capture.
+ * Should a copy of keys and values not arrive within the wait's limit (b200q_device_status: 801), the rows that it was for, and others that the
+ * same CTA had a part of, are NaN in out and lse.
  */
 typedef struct b200q_paged_attention_args {
   const void* q;
@@ -596,6 +598,10 @@ typedef struct b200q_paged_attention_args {
 
 size_t b200q_paged_attention_workspace_bytes(int64_t requests, int heads, int kv_heads, int dim, int cache_dtype);
 int b200q_paged_attention(const b200q_paged_attention_args* args);
+/* Self-test of that: the same call (heads of 128, e4m3 caches, bf16 output, at most 8 query heads to a key/value head, else
+ * B200Q_ERR_UNSUPPORTED) in which the copies for step `step` of warp `warp`'s run in CTA `cta` are never made and waits are short.  The GPU
+ * does not fault.  A run that is not so long: nothing is left out. */
+int b200q_selftest_paged_wait_timeout(const b200q_paged_attention_args* args, int cta, int warp, int step);
 
 #ifdef __cplusplus
 }

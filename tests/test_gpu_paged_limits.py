@@ -1,5 +1,6 @@
 """The paged key/value cache where it is easily wrong: precision of fp32 outputs, sizes near the ends of their types, tables and
 caches of unusual form.  The oracle and the helpers are those of test_gpu_paged.py."""
+import ctypes as C
 import math
 
 import pytest
@@ -132,3 +133,68 @@ def test_attention_large_scores(cache, heads, kv, dim, size):
     got, got_lse = torch.ops.b200q.paged_attention(q.cuda(), p.k.cuda(), p.vd, p.table.cuda(), p.lens.cuda(), 1.0)
     _close(got.float(), want, 2.0 ** -8 * want.abs() + (2.0 ** -11 + 2.0 ** -13) * size)
     _close(got_lse, lse, 2.0 ** -21 * torch.where(lse.isfinite(), lse.abs(), 0.0))
+
+
+# ----------------------------------------------------------------------------- attention: a copy that does not arrive
+@pytest.mark.parametrize("lens,kv,drops", [
+    ([200], 1, [(0, 0, 0), (0, 3, 1), (0, 6, 0)]),                                       # one CTA, no joining kernel
+    ([700, 40, 0, 1500, 16, 900], 8, [(0, 0, 0), (0, 7, 1), (1, 0, 0), (50, 3, 0), (99, 7, 0)]),  # rows cut between warps and CTAs; the last CTA has 15 steps
+    ([3000 + 7 * i for i in range(16)], 8, [(0, 0, 0), (10, 3, 5), (73, 0, 15), (147, 7, 12)]),   # heads side by side
+    ([131072], 8, [(0, 0, 0), (80, 4, 7)]),                                               # rows that every CTA has a part of
+])
+def test_attention_rows_whose_copies_do_not_arrive_are_nan(lens, kv, drops):
+    """The wait runs out (no GPU fault), the status says so, the rows that missed their keys are NaN as a whole, all others have the bytes
+    of an undisturbed call."""
+    import b200_hpu_ops
+    from b200_hpu_ops import abi
+    heads, dim, page = 8 * kv, 128, 16
+    g = torch.Generator(device="cuda").manual_seed(1)
+    need = [-(-n // page) for n in lens]
+    kc, vc = (torch.randint(0, 256, (sum(need), page, kv, dim), generator=g, device="cuda", dtype=torch.uint8).bitwise_and(0xBF).view(E4M3) for _ in range(2))
+    table, at = torch.full((len(lens), max(need)), -1, dtype=torch.int32), 0
+    for b, n in enumerate(need):
+        table[b, :n] = torch.arange(at, at + n)
+        at += n
+    table, kv_lens = table.cuda(), _i32(lens).cuda()
+    q = torch.randn(len(lens), heads, dim, generator=g, device="cuda").to(BF16)
+    run = lambda: torch.ops.b200q.paged_attention(q, kc, vc, table, kv_lens, 0.05)  # noqa: E731
+    want, want_lse = run()
+    assert bool(want.isfinite().all())
+    for cta, warp, step in drops:
+        out, lse = torch.zeros_like(want), torch.zeros_like(want_lse)
+        space = torch.full((abi.lib.b200q_paged_attention_workspace_bytes(len(lens), heads, kv, dim, abi.E4M3),), 0x11, dtype=torch.uint8, device="cuda")
+        a = abi.PagedAttentionArgs()
+        a.q, a.q_token_stride, a.q_head_stride, a.requests, a.heads, a.kv_heads, a.dim = q.data_ptr(), heads * dim, dim, len(lens), heads, kv, dim
+        a.k_cache, a.v_cache, a.cache_dtype, a.num_pages, a.page_size = kc.data_ptr(), vc.data_ptr(), abi.E4M3, kc.shape[0], page
+        a.k_page_stride, a.k_slot_stride, a.k_head_stride = a.v_page_stride, a.v_slot_stride, a.v_head_stride = kc.stride()[:3]
+        a.block_table, a.table_width, a.table_stride, a.kv_lens = table.data_ptr(), table.shape[1], table.shape[1], kv_lens.data_ptr()
+        a.softmax_scale, a.out, a.out_dtype, a.lse = 0.05, out.data_ptr(), abi.BF16, lse.data_ptr()
+        a.workspace, a.workspace_bytes, a.stream = space.data_ptr(), space.numel(), torch.cuda.current_stream().cuda_stream
+        assert abi.lib.b200q_selftest_paged_wait_timeout(C.byref(a), cta, warp, step) == 0
+        assert b200_hpu_ops.device_status() == 801
+        lost = lse.isnan()
+        assert torch.equal(out.isnan().all(-1), lost) and torch.equal(out.isnan().any(-1), lost)
+        assert torch.equal(out[~lost], want[~lost]) and torch.equal(lse[~lost], want_lse[~lost])
+        if (cta, warp, step) == (0, 0, 0):
+            assert bool(lost[0, :8].all())  # (the first step of the list: request 0, key/value head 0)
+        assert 8 <= int(lost.sum()) <= 128 and (len(lens) == 1 or not bool(lost.all()))  # (no CTA has a part of more than 16 rows of 8 heads)
+        for x, y in zip(run(), (want, want_lse)):
+            assert torch.equal(x, y)
+    assert b200_hpu_ops.device_status() == 0
+
+
+def test_attention_selftest_refusals():
+    from b200_hpu_ops import abi
+    test = abi.lib.b200q_selftest_paged_wait_timeout
+    assert test(None, 0, 0, 0) == -1
+    a = abi.PagedAttentionArgs()
+    x = torch.zeros(1 << 16, dtype=torch.uint8).cuda()
+    a.q = a.k_cache = a.v_cache = a.out = a.block_table = a.kv_lens = x.data_ptr()
+    a.requests, a.heads, a.kv_heads, a.dim, a.num_pages, a.page_size, a.table_width, a.cache_dtype, a.out_dtype = 1, 8, 1, 128, 1, 16, 1, abi.E4M3, abi.BF16
+    assert test(C.byref(a), -1, 0, 0) == -1 and test(C.byref(a), 0, 0, -1) == -1
+    assert test(C.byref(a), 0, 0, 0) == -1  # no workspace
+    for name, value in (("dim", 64), ("cache_dtype", abi.BF16), ("out_dtype", abi.F32), ("heads", 9)):
+        old = getattr(a, name)
+        setattr(a, name, value)
+        assert test(C.byref(a), 0, 0, 0) == -2
+        setattr(a, name, old)
