@@ -2,6 +2,8 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <initializer_list>
+
 #include "common.cuh"
 #include "fp8_misc.cuh"
 #include "gemm_common.cuh"
@@ -125,6 +127,17 @@ size_t paged_attention_workspace_bytes_impl(int64_t, int, int, int, int);
 
 static bool is_fp8(int d) { return d == B200Q_E4M3 || d == B200Q_E5M2; }
 static bool is_wide(int d) { return d == B200Q_F32 || d == B200Q_BF16; }
+// whether the address is a multiple of n elements of the type
+static bool on_elements(const void* p, int dtype, int n) {
+  const int size = dtype == B200Q_F32 ? 4 : dtype == B200Q_BF16 ? 2 : 1;
+  return reinterpret_cast<uintptr_t>(p) % (size_t)(size * n) == 0;
+}
+// whether each is a multiple of `bytes`
+static bool on_bytes(size_t bytes, std::initializer_list<const void*> pointers) {
+  for (const void* p : pointers)
+    if (reinterpret_cast<uintptr_t>(p) % bytes) return false;
+  return true;
+}
 static bool scale_args_ok(const float* dev, int mode) {
   if (mode < B200Q_BCAST_NONE || mode > B200Q_BCAST_FULL) return false;
   if (mode >= B200Q_BCAST_SCALAR_DEV && !dev) return false;
@@ -444,6 +457,8 @@ int b200q_paged_plan(const int32_t* context_lens, const int32_t* new_lens, int64
   if (!query_start || !free_head_out || (num_tokens > 0 && (!slot_map || !positions))) return B200Q_ERR_BAD_ARGUMENT;
   if (requests > 0 && (!context_lens || !new_lens || !kv_lens || (table_width > 0 && !block_table))) return B200Q_ERR_BAD_ARGUMENT;
   if (free_count > 0 && !free_pages) return B200Q_ERR_BAD_ARGUMENT;
+  if (!on_bytes(4, {context_lens, new_lens, block_table, free_pages, free_head, query_start, kv_lens, free_head_out}) || !on_bytes(8, {slot_map, positions}))
+    return B200Q_ERR_UNSUPPORTED;
   PagedPlanParams p;
   p.context_lens = context_lens; p.new_lens = new_lens; p.requests = (int)requests;
   p.table = block_table; p.table_width = (int)table_width; p.table_stride = table_stride;
@@ -451,12 +466,6 @@ int b200q_paged_plan(const int32_t* context_lens, const int32_t* new_lens, int64
   p.page_size = (int)page_size; p.num_tokens = (int)num_tokens;
   p.slot_map = slot_map; p.positions = positions; p.query_start = query_start; p.kv_lens = kv_lens; p.free_head_out = free_head_out;
   return paged_plan_impl(p, static_cast<cudaStream_t>(stream));
-}
-
-// whether the address is a multiple of n elements of the type
-static bool on_elements(const void* p, int dtype, int n) {
-  const int size = dtype == B200Q_F32 ? 4 : dtype == B200Q_BF16 ? 2 : 1;
-  return reinterpret_cast<uintptr_t>(p) % (size_t)(size * n) == 0;
 }
 
 int b200q_qk_norm_rope_append(const b200q_append_args* a) {
@@ -482,6 +491,7 @@ int b200q_qk_norm_rope_append(const b200q_append_args* a) {
   for (const void* p : {a->k_cache, a->v_cache})
     if (!on_elements(p, a->cache_dtype, 4)) return B200Q_ERR_UNSUPPORTED;
   if (!on_elements(a->q_out, a->q_out_dtype, 4) || !on_elements(a->cos_sin, B200Q_F32, 4)) return B200Q_ERR_UNSUPPORTED;
+  if (!on_bytes(8, {a->positions, a->slot_map}) || !on_bytes(4, {a->k_scale, a->v_scale, a->q_scale})) return B200Q_ERR_UNSUPPORTED;
   for (int64_t s : {a->q_token_stride, a->q_head_stride, a->k_token_stride, a->k_head_stride, a->v_token_stride, a->v_head_stride,
                     a->k_page_stride, a->k_slot_stride, a->k_cache_head_stride, a->v_page_stride, a->v_slot_stride, a->v_cache_head_stride})
     if (s % 4) return B200Q_ERR_UNSUPPORTED;
@@ -516,6 +526,9 @@ static int check_paged_attention(const b200q_paged_attention_args* a, bool* noth
   }
   if (!a->q || !a->out || !a->kv_lens || (a->table_width > 0 && !a->block_table)) return B200Q_ERR_BAD_ARGUMENT;
   if (a->num_pages > 0 && (!a->k_cache || !a->v_cache)) return B200Q_ERR_BAD_ARGUMENT;
+  if (!on_elements(a->q, B200Q_BF16, 1) || !on_elements(a->k_cache, a->cache_dtype, 1) || !on_elements(a->v_cache, a->cache_dtype, 1) ||
+      !on_elements(a->out, a->out_dtype, 1) || !on_bytes(4, {a->block_table, a->kv_lens, a->lse, a->k_scale_inv, a->v_scale_inv, a->out_scale}))
+    return B200Q_ERR_UNSUPPORTED;
   return B200Q_OK;
 }
 

@@ -475,7 +475,8 @@ int b200q_im2col_nhwc_fp8(const void* in, void* out, int64_t N, int64_t C, int64
                           int64_t cg, int64_t ld_out, void* stream);
 
 /*
- * A key/value cache in pages and one decode step over it.  The reference has no counterpart: its callers keep one
+ * A key/value cache in pages and one decode step over it.  An address that is not a multiple of its elements' size is
+ * B200Q_ERR_UNSUPPORTED.  The reference has no counterpart: its callers keep one
  * contiguous cache per request and run sdpa_recomp_fwd (hpu_ops/backend/sdpa_gen.cpp:820-1000) over the whole of it.
  *
  * paged_plan: where the new tokens of a step go, from the requests' lengths, on the device.  Request b holds

@@ -8,7 +8,8 @@ import subprocess
 import pytest
 
 from conftest import ROOT
-from test_cpu_paged import AT, BAD, _append
+from b200_hpu_ops import abi
+from test_cpu_paged import AT, BAD, UNSUPPORTED, _append, _attend, _plan
 
 CSRC = os.path.join(ROOT, "gaudi-pytorch-bridge_b200", "csrc")
 
@@ -107,3 +108,25 @@ def test_layouts_that_are_taken(layouts):
     page = 2 * 16 * 3 * dim
     assert two(2, dim, (4096, n, [page, 3 * dim, dim]), (4096 + page, n, [page, dim, 16 * dim]))
     assert two(2, dim, (4096, [0, 16, 3], [page, 24, 8]), (4096, [0, 16, 3], [page, 24, 8]))  # no pages
+
+
+# ----------------------------------------------------------------------------- addresses between elements
+@pytest.mark.parametrize("name", ["context", "new", "table", "free", "head", "start", "lens", "next", "slots", "positions"])
+def test_plan_refuses_addresses_between_elements(name):
+    assert _plan(**{name: AT + 2}) == UNSUPPORTED
+    if name in ("slots", "positions"):
+        assert _plan(**{name: AT + 4}) == UNSUPPORTED
+
+
+@pytest.mark.parametrize("kw", [dict(slot_map=AT + 4), dict(cos_sin=AT, rotary_dim=64, positions=AT + 4), dict(k_scale=AT + 2), dict(v_scale=AT + 1),
+                                dict(q_scale=AT + 2)])
+def test_append_refuses_addresses_between_elements(kw):
+    assert _append(**{**dict(v_cache=AT << 4), **kw}) == UNSUPPORTED
+
+
+@pytest.mark.parametrize("kw", [dict(q=AT + 1), dict(out=AT + 1), dict(out=AT + 2, out_dtype=abi.F32), dict(k_cache=AT + 1, cache_dtype=abi.BF16),
+                                dict(v_cache=AT + 1, cache_dtype=abi.BF16), dict(block_table=AT + 2), dict(kv_lens=AT + 1), dict(lse=AT + 2),
+                                dict(k_scale_inv=AT + 2), dict(v_scale_inv=AT + 1), dict(out_scale=AT + 3)])
+@pytest.mark.parametrize("plain", [0, 1])
+def test_attention_refuses_addresses_between_elements(kw, plain):
+    assert _attend(force_plain=plain, **kw) == UNSUPPORTED
