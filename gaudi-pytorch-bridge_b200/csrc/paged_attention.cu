@@ -139,12 +139,14 @@ constexpr float kPagedNoMax = -3.402823466e38f;  // the lowest finite number: no
 constexpr int kPagedLengthsHere = (int)kPagedMaxRequests / 2;  // up to so many requests' lengths lie in shared memory beside the sums
 constexpr int kPagedErrCopy = 801;  // status code: a copy of keys and values did not arrive
 
+constexpr int paged_warps_of(int dim) { return dim == 256 ? 4 : 8; }  // of a CTA
+
 template <int DIM, int FMT, int NT>
 struct PagedTile {
   static constexpr int kElt = FMT == B200Q_BF16 ? 2 : 1;
   static constexpr int kRow = DIM * kElt;           // bytes of a key
   static constexpr int kStage = 2 * 16 * kRow;      // keys and values of a step
-  static constexpr int kWarps = DIM == 256 ? 4 : 8;
+  static constexpr int kWarps = paged_warps_of(DIM);
   static constexpr int kStages = kPagedRingBytes / kWarps / kStage < 8 ? kPagedRingBytes / kWarps / kStage : 8;
   static constexpr int kKChunks = kRow / 64;        // 16-byte pieces of a key per lane
   static constexpr int kVPiece = kRow / 8 < 16 ? 8 : 16;
@@ -1067,15 +1069,22 @@ static bool paged_tensor_dim(int dim) { return dim == 64 || dim == 128 || dim ==
 // query heads of a row tile: 16 where more than 8 share a key/value head, which then is read once for them; heads of 256
 // values in two tiles do not fit the registers
 static int paged_rows_of(int group, int dim) { return group <= 8 || dim == 256 ? 8 : 16; }
-static size_t paged_align(size_t n) { return (n + 255) / 256 * 256; }
+
+// Where the three parts of the workspace lie, for the size that a caller is told and for the kernels alike.
+struct PagedSpace {
+  size_t cta_part, warp_part, bytes;
+  static constexpr size_t align(size_t n) { return (n + 255) / 256 * 256; }
+  constexpr PagedSpace(int rows, int dim, int warps)
+      : cta_part(align(sizeof(PagedJoin) * kPagedGrid)),
+        warp_part(cta_part + align(sizeof(float) * rows * (dim + 2) * 2 * warps * kPagedGrid)),
+        bytes(warp_part + align(sizeof(float) * rows * (dim + 2) * warps * kPagedGrid)) {}
+};
 
 size_t paged_attention_workspace_bytes_impl(int64_t requests, int heads, int kv_heads, int dim, int cache_dtype) {
   (void)requests;  // (rows are joined per CTA, whatever the number of requests)
   (void)cache_dtype;
   if (!paged_tensor_dim(dim)) return 0;
-  const size_t part = sizeof(float) * paged_rows_of(heads / kv_heads, dim) * (dim + 2);
-  const size_t warps = dim == 256 ? 4 : 8;
-  return paged_align(sizeof(PagedJoin) * kPagedGrid) + paged_align(part * 2 * warps * kPagedGrid) + paged_align(part * warps * kPagedGrid);
+  return PagedSpace(paged_rows_of(heads / kv_heads, dim), dim, paged_warps_of(dim)).bytes;
 }
 
 // A cache as [pages][slots][heads][bytes of a head], whatever the order of its strides, in boxes of 16 slots
@@ -1124,12 +1133,13 @@ static int paged_launch(const b200q_paged_attention_args& a, cudaStream_t st, Pa
   w.heads_per_request = a.kv_heads * w.row_tiles;
   w.lane_bits = 0;
   while ((2 << w.lane_bits) <= Tile::kWarps && w.heads_per_request % (2 << w.lane_bits) == 0) ++w.lane_bits;
+  constexpr PagedSpace space(Tile::kRows, DIM, Tile::kWarps);
+  static_assert(Tile::kPart == Tile::kRows * (DIM + 2), "the size of a part in PagedSpace");
+  if (a.workspace_bytes < space.bytes) return B200Q_ERR_BAD_ARGUMENT;  // (this instance's own need, whatever the caller was told)
   uint8_t* p = static_cast<uint8_t*>(a.workspace);
   w.joins = reinterpret_cast<PagedJoin*>(p);
-  p += paged_align(sizeof(PagedJoin) * kPagedGrid);
-  w.cta_part = reinterpret_cast<float*>(p);
-  p += paged_align(sizeof(float) * Tile::kPart * 2 * Tile::kWarps * kPagedGrid);
-  w.warp_part = reinterpret_cast<float*>(p);
+  w.cta_part = reinterpret_cast<float*>(p + space.cta_part);
+  w.warp_part = reinterpret_cast<float*>(p + space.warp_part);
   // no more CTAs than the longest list that the tables can hold would fill
   const int64_t most = a.requests * ((a.table_width * a.page_size + 15) / 16) * w.heads_per_request;
   int64_t grid = (most + Tile::kWarps * kPagedMinSteps - 1) / (Tile::kWarps * kPagedMinSteps);

@@ -198,3 +198,32 @@ def test_attention_selftest_refusals():
         setattr(a, name, value)
         assert test(C.byref(a), 0, 0, 0) == -2
         setattr(a, name, old)
+
+
+# ----------------------------------------------------------------------------- attention: workspace
+@pytest.mark.parametrize("cache,heads,kv,dim", [(E4M3, 8, 1, 64), (BF16, 16, 1, 64), (E4M3, 64, 8, 128), (E5M2, 20, 1, 128), (E4M3, 16, 1, 256), (BF16, 8, 4, 256)])
+def test_attention_stays_within_its_workspace(cache, heads, kv, dim):
+    """A workspace of just the size that is asked for, filled with NaN, between guards: rows cut between warps and between all CTAs, empty
+    ones and whole ones.  A workspace that is smaller by one byte is refused."""
+    from b200_hpu_ops import abi
+    lens = [40000, 0, 17, 3000, 1]
+    p = _Paged(lens, kv, dim, cache, 16, seed=4)
+    q = torch.randn(5, heads, dim, generator=p.g).to(BF16).cuda()
+    table, kv_lens = p.table.cuda(), p.lens.cuda()
+    want, want_lse = torch.ops.b200q.paged_attention(q, p.kd, p.vd, table, kv_lens, 0.1)
+    out, lse = torch.empty_like(want), torch.empty_like(want_lse)
+    size = abi.lib.b200q_paged_attention_workspace_bytes(5, heads, kv, dim, abi.DTYPE[cache])
+    space = torch.full((size + 2 * 65536,), 0xFF, dtype=torch.uint8, device="cuda")
+    a = abi.PagedAttentionArgs()
+    a.q, a.q_token_stride, a.q_head_stride, a.requests, a.heads, a.kv_heads, a.dim = q.data_ptr(), heads * dim, dim, 5, heads, kv, dim
+    a.k_cache, a.v_cache, a.cache_dtype, a.num_pages, a.page_size = p.kd.data_ptr(), p.vd.data_ptr(), abi.DTYPE[cache], p.kd.shape[0], 16
+    a.k_page_stride, a.k_slot_stride, a.k_head_stride = a.v_page_stride, a.v_slot_stride, a.v_head_stride = p.kd.stride()[:3]
+    a.block_table, a.table_width, a.table_stride, a.kv_lens = table.data_ptr(), p.width, p.width, kv_lens.data_ptr()
+    a.softmax_scale, a.out, a.out_dtype, a.lse = 0.1, out.data_ptr(), abi.BF16, lse.data_ptr()
+    a.workspace, a.workspace_bytes, a.stream = space.data_ptr() + 65536, size, torch.cuda.current_stream().cuda_stream
+    for _ in range(2):
+        assert abi.lib.b200q_paged_attention(C.byref(a)) == 0
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    assert bool((space[:65536] == 0xFF).all()) and bool((space[65536 + size:] == 0xFF).all())
+    a.workspace_bytes = size - 1
+    assert abi.lib.b200q_paged_attention(C.byref(a)) == -1
