@@ -560,7 +560,8 @@ int b200q_qk_norm_rope_append(const b200q_append_args* args);
  * Query head h reads key/value head h / (heads / kv_heads).  Lengths are cut to table_width * page_size; keys whose table
  * entry is outside [0, num_pages) do not exist.  The cache behind a request's length is not looked at.
  *
- * q             bf16 [requests][heads][dim], strides in elements, values contiguous
+ * q             bf16 [requests][heads][dim], strides in elements, values contiguous: row b is request b's newest token, which is row
+ *               query_start[b + 1] - 1 of the step's tokens
  * caches        as above, any strides;  block_table int32 [requests][table_width];  kv_lens int32 [requests]
  * out           out_dtype (BF16 / F32 / E4M3) [requests][heads][dim] contiguous; lse: NULL or fp32 [requests][heads]
  * workspace     b200q_paged_attention_workspace_bytes(...) bytes, 16-byte aligned, not shared by calls that may overlap

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from oracle import hpu_oracle as O
-from test_gpu_paged import BF16, E4M3, E5M2, F32, _close, _i32, _one, _Paged, _status  # noqa: F401 (_status: device status after each test)
+from test_gpu_paged import BF16, E4M3, E5M2, F32, _close, _dense_check, _i32, _Model, _one, _Paged, _status  # noqa: F401 (_status: device status after each test)
 
 pytestmark = pytest.mark.gpu
 
@@ -227,3 +227,52 @@ def test_attention_stays_within_its_workspace(cache, heads, kv, dim):
     assert bool((space[:65536] == 0xFF).all()) and bool((space[65536 + size:] == 0xFF).all())
     a.workspace_bytes = size - 1
     assert abi.lib.b200q_paged_attention(C.byref(a)) == -1
+
+
+# ----------------------------------------------------------------------------- a server's steps
+def _captured(m, tokens, requests):
+    """A step of plan, append and the attention of each request's newest token, captured: (new lengths, projections, answers, replay)."""
+    new, qkv = torch.zeros(requests, dtype=torch.int32).cuda(), torch.zeros(tokens, m.heads + 2 * m.kv, m.dim, dtype=BF16).cuda()
+
+    def step():
+        h, g = m.heads, m.kv
+        slots, pos, start, lens, head = torch.ops.b200q.paged_plan(m.lens, new, m.table, m.free, m.head, m.page, tokens)
+        q = torch.ops.b200q.qk_norm_rope_append(qkv[:, :h], qkv[:, h:h + g], qkv[:, h + g:], m.qw, m.kw, 1e-6, m.cos_sin, pos, False, slots, m.kc, m.vc, m.scale,
+                                                m.scale)
+        last = (start[1:] - 1).clamp(min=0)
+        out = torch.ops.b200q.paged_attention(q.index_select(0, last), m.kc, m.vc, m.table, lens, 1 / math.sqrt(m.dim), m.inv, m.inv)[0]
+        return slots, lens, head, out
+
+    lens, head, table = m.lens.clone(), m.head.clone(), m.table.clone()
+    step()  # (each operator runs once before the capture; with no new tokens nothing is written)
+    torch.cuda.synchronize()
+    assert torch.equal(m.table, table) and torch.equal(m.lens, lens) and torch.equal(m.head, head)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    return new, qkv, outs, graph
+
+
+@pytest.mark.parametrize("cache", [E4M3, BF16])
+def test_captured_steps_with_idle_requests_and_prompts(cache):
+    """From 0 to 9 new tokens for each request, other ones in every replay; a request's answer is that of its newest token."""
+    m, gen = _Model(cache, requests=5), torch.Generator().manual_seed(11)
+    new, qkv, (slots, lens, head, out), graph = _captured(m, 24, 5)
+    seen = [[] for _ in range(5)]
+    for step in range(24):
+        counts = [[1, 1, 1, 1, 1], [1, 0, 1, 0, 1], [0, 0, 1, 1, 0], [9, 0, 1, 7, 1], [0, 0, 0, 0, 0], [0, 1, 0, 0, 5]][step % 6]
+        x = torch.randn(24, 12, 128, generator=gen).to(BF16)
+        new.copy_(_i32(counts))
+        qkv.copy_(x)
+        graph.replay()
+        t = 0
+        for b, n in enumerate(counts):
+            seen[b] += list(x[t:t + n])
+            t += n
+        assert bool((slots[t:] == -1).all()) and lens.tolist() == [len(s) for s in seen]
+        if step % 4 == 3 or step == 4:
+            busy = [b for b, n in enumerate(counts) if n]
+            answers = out.cpu()
+            _dense_check(m, [seen[b] for b in busy], answers[busy])
+        m.lens.copy_(lens)
+        m.head.copy_(head)
