@@ -491,9 +491,11 @@ int b200q_im2col_nhwc_fp8(const void* in, void* out, int64_t N, int64_t C, int64
  *
  * context_lens, new_lens  int32 [requests]; requests <= 8192
  * block_table   int32 [requests][table_width], row stride table_stride >= table_width; requests * table_width < 2^31
- * free_pages    int32 [free_count]
+ * free_pages    int32 [free_count]; a negative entry is no page.  The index into it does not wrap around.
  * slot_map, positions  int64 [num_tokens];  query_start int32 [requests + 1];  kv_lens int32 [requests]: context + new
- * free_head_out one int32: *free_head + the pages that the step needs (above free_count: there were too few)
+ * free_head_out one int32: *free_head + the pages that the step needs.  Above free_count (or the number of entries that are pages): there were too few.
+ *               The step is then to be run again with the same context_lens and *free_head over a list that has more from that index on (or with
+ *               *free_head 0 over a list that begins with what was not taken); to go on from this value would skip as many pages as were missing.
  * Outputs must not overlap inputs.  A call writes the same values again when it is repeated with the same inputs.
  */
 int b200q_paged_plan(const int32_t* context_lens, const int32_t* new_lens, int64_t requests,

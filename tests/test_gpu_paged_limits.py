@@ -276,3 +276,45 @@ def test_captured_steps_with_idle_requests_and_prompts(cache):
             _dense_check(m, [seen[b] for b in busy], answers[busy])
         m.lens.copy_(lens)
         m.head.copy_(head)
+
+
+@pytest.mark.parametrize("cache", [E4M3, BF16])
+def test_captured_steps_while_requests_come_and_go(cache):
+    """The pool is gone through several times.  Its list has one length and one address for the graph: a host that finds `free_head` above the
+    number of free pages keeps the lengths and the head of before, puts what was not taken and what has come back to the front of
+    the list with the head at 0, and runs the step again."""
+    m, gen = _Model(cache, requests=4, pages=24, width=8), torch.Generator().manual_seed(12)
+    new, qkv, (slots, lens, head, out), graph = _captured(m, 4, 4)
+    seen, life = [[] for _ in range(4)], [40, 70, 55, 100]
+    count, retired, short, taken = 24, [], 0, 0
+    new.fill_(1)
+    for step in range(400):
+        x = torch.randn(4, 12, 128, generator=gen).to(BF16)
+        qkv.copy_(x)
+        graph.replay()
+        if int(head) > count:
+            short += 1
+            begin = int(m.head)
+            assert bool((slots < 0).any())  # a token without a page
+            pool = m.free[begin:count].tolist() + retired
+            taken, count, retired = taken + begin, len(pool), []
+            m.free.copy_(_i32(pool + [-1] * (24 - count)))
+            m.head.zero_()
+            graph.replay()
+            assert int(head) <= count
+        assert bool((slots >= 0).all()) and slots.unique().numel() == 4
+        for b in range(4):
+            seen[b].append(x[b])
+        if step % 40 == 39 or step in (0, 97, 98):
+            _dense_check(m, seen, out.cpu())
+        m.lens.copy_(lens)
+        m.head.copy_(head)
+        held = [m.table[b, :-(-len(seen[b]) // m.page)].tolist() for b in range(4)]
+        left = m.free[int(m.head):count].tolist()
+        assert sorted(sum(held, []) + left + retired) == list(range(24))  # every page once: held, free or retired
+        for b in range(4):
+            if len(seen[b]) == life[b]:  # its pages go back, and another request takes its row
+                retired += held[b]
+                seen[b] = []
+                m.lens[b] = 0
+    assert short >= 4 and taken > 48
