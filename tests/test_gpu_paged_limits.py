@@ -318,3 +318,31 @@ def test_captured_steps_while_requests_come_and_go(cache):
                 seen[b] = []
                 m.lens[b] = 0
     assert short >= 4 and taken > 48
+
+
+def test_prompts_through_the_fp8_attention():
+    """Prompts without a cached prefix: their keys and values gathered from the pages, one request at a time, for fp8_sdpa_recomp_fwd."""
+    m, gen = _Model(E4M3, requests=4), torch.Generator().manual_seed(13)
+    prompts, h, g, rep = [37, 0, 130, 5], m.heads, m.kv, m.heads // m.kv
+    x = torch.randn(sum(prompts) + 4, h + 2 * g, 128, generator=gen).to(BF16)
+    qkv, q_scale = x.cuda(), _one(32.0).cuda()
+    slots, pos, start, lens, head = torch.ops.b200q.paged_plan(m.lens, _i32(prompts).cuda(), m.table, m.free, m.head, m.page, len(x))
+    q = torch.ops.b200q.qk_norm_rope_append(qkv[:, :h], qkv[:, h:h + g], qkv[:, h + g:], m.qw, m.kw, 1e-6, m.cos_sin, pos, False, slots, m.kc, m.vc, m.scale,
+                                            m.scale, q_scale, E4M3)
+    at = 0
+    for b, n in enumerate(prompts):
+        if not n:
+            continue
+        pages = m.table[b, :-(-n // m.page)].long()
+        k, v = (c.view(torch.uint8)[pages].view(E4M3).flatten(0, 1)[:n].transpose(0, 1).unsqueeze(1) for c in (m.kc, m.vc))  # [kv_heads, 1, n, dim]
+        rows = q[at:at + n].view(n, g, rep, 128).permute(1, 2, 0, 3)                                                       # [kv_heads, heads of each, n, dim]
+        got = torch.ops.hpu.fp8_sdpa_recomp_fwd(rows, k, v, None, 0.0, 128 ** -0.5, True, False, "None", 1 / q_scale, m.inv, m.inv, None, None, None,
+                                                False, False, None, "None")[0]
+        # keys and values as the oracle makes them from the projections; what is left is the output's rounding (2^-8 at most, of each value) and the
+        # few e4m3 values that round the other way from fp32
+        kk = (O.norm_rope(x[at:at + n, h:h + g], m.kw.cpu(), 1e-6, m.cos_sin.cpu(), torch.arange(n), False) * 16).clamp(-448, 448).float().to(E4M3)
+        vv = (x[at:at + n, h + g:].float() * 16).clamp(-448, 448).to(E4M3)
+        want = O.fp8_sdpa_recomp_fwd(rows.cpu(), kk.transpose(0, 1).unsqueeze(1), vv.transpose(0, 1).unsqueeze(1), None, 0.0, 128 ** -0.5, True,
+                                     d_scale_q=_one(1 / 32.0), d_scale_k=_one(1 / 16.0), d_scale_v=_one(1 / 16.0))[0]
+        assert O.rel_frobenius(got.float().cpu(), want.float()) < 2.0 ** -7
+        at += n
