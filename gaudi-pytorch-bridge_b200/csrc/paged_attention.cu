@@ -133,8 +133,6 @@ constexpr int kPagedGrid = kNumSMs;
 constexpr int kPagedRingBytes = 192 * 1024;
 constexpr int kPagedLaneSteps = 14;   // a warp's steps from which on heads go side by side
 constexpr int kPagedMinSteps = 2;     // a warp gets at least this many steps while there are enough for the others
-constexpr float kPagedShift = 7.f;    // probabilities are held relative to 2^(maximum - 7) ...
-constexpr float kPagedRescale = 15.f; // ... and the maximum is raised when one would pass 2^15 (f16 ends at 2^16)
 constexpr float kPagedNoMax = -3.402823466e38f;  // the lowest finite number: no finite score is below it
 constexpr int kPagedLengthsHere = (int)kPagedMaxRequests / 2;  // up to so many requests' lengths lie in shared memory beside the sums
 constexpr int kPagedErrCopy = 801;  // status code: a copy of keys and values did not arrive
@@ -156,6 +154,10 @@ struct PagedTile {
   static constexpr int kBoxes = kRow / kBox;
   static constexpr int kTiles = DIM / 16;           // k-steps of the first product, row tiles of the second
   static constexpr int kRows = 8 * NT;              // query heads
+  // Probabilities are held relative to 2^(maximum - kShift), and the maximum is raised when one would pass 2^kRescale.  f16 ends at 2^16, and
+  // below 2^-14 it loses bits: 2^7 and 2^15.  bf16 has the range of fp32, and so have the values that it meets, whose products with
+  // probabilities of at most 1 do not overflow: 2^-8 and 1.
+  static constexpr float kShift = FMT == B200Q_BF16 ? -8.f : 7.f, kRescale = FMT == B200Q_BF16 ? 0.f : 15.f;
   static constexpr int kPart = kRows * (DIM + 2);   // floats of a partial result: output, maxima, sums
   static constexpr int kRing = kStages * kStage;    // bytes per warp
   static_assert(2 * kPart * 4 <= kRing && kStages >= 2, "both partial results of a warp take the place of the ring");
@@ -717,13 +719,13 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
           for (int i = 0; i < 4; ++i) x[i] = __fsub_rn(s[n][i], acc.m[n][i & 1]);
         };
         exponents();
-        if (__any_sync(0xFFFFFFFFu, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) > kPagedRescale)) {
+        if (__any_sync(0xFFFFFFFFu, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) > Tile::kRescale)) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             float top = fmaxf(s[n][i], s[n][i + 2]);
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-            const float raised = top > acc.m[n][i] + kPagedRescale ? top - kPagedShift : acc.m[n][i];
+            const float raised = top > acc.m[n][i] + Tile::kRescale ? top - Tile::kShift : acc.m[n][i];
             const float keep = paged_exp2(acc.m[n][i] - raised);
             acc.m[n][i] = raised;
             acc.l[n][i] *= keep;

@@ -346,3 +346,29 @@ def test_prompts_through_the_fp8_attention():
                                      d_scale_q=_one(1 / 32.0), d_scale_k=_one(1 / 16.0), d_scale_v=_one(1 / 16.0))[0]
         assert O.rel_frobenius(got.float().cpu(), want.float()) < 2.0 ** -7
         at += n
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(8, 1, 128), (4, 2, 64), (2, 1, 256), (12, 1, 64), (2, 1, 72)])
+@pytest.mark.parametrize("rising", [False, True])
+def test_attention_large_values_of_a_bf16_cache(heads, kv, dim, rising):
+    """Values of 3e36: an average of them is nowhere near the end of fp32, 2^7 times one of them is beyond it.  With scores that rise by 7
+    from one step of 16 keys to the next the running maximum trails behind the scores as far as it may."""
+    p = _Paged([0, 1, 5, 40, 300], kv, dim, BF16, 16, seed=6)
+    p.v = (p.v.float() * 3e36).to(BF16)
+    scale = 0.1
+    if rising:
+        k = torch.zeros(p.k.shape)
+        for b, n in enumerate(p.lens.tolist()):
+            for i in range(-(-n // 16)):
+                k[int(p.table[b, i]), :, :, 0] = 7 * math.log(2) * i
+        p.k = torch.where(p.k.float().isnan(), math.nan, k).to(BF16)
+        scale = 1.0
+    q = torch.randn(5, heads, dim, generator=p.g)
+    if rising:
+        q = torch.zeros(5, heads, dim)
+        q[..., 0] = 1.0
+    q = q.to(BF16)
+    want, lse, size = O.paged_attention(q, p.k, p.v, p.table, p.lens, scale)
+    got, got_lse = torch.ops.b200q.paged_attention(q.cuda(), p.k.cuda(), p.v.cuda(), p.table.cuda(), p.lens.cuda(), scale)
+    _close(got.float(), want, 2.0 ** -8 * want.abs() + (2.0 ** -11 + 2.0 ** -13) * size)
+    _close(got_lse, lse, 2.0 ** -13 + 2.0 ** -22 * torch.where(lse.isfinite(), lse.abs(), 0.0))
