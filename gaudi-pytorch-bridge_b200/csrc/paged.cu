@@ -165,8 +165,8 @@ int paged_plan_impl(const PagedPlanParams& p, cudaStream_t st) {
 // the token's position in pairs (i, i + r/2) or (2i, 2i + 1); one rounding from fp32 to the output's type.
 // Memory bound, if the instructions are few: 16 lanes own a head of 128, 8 values each, and a first version of 221 instructions per
 // lane and head was bound by them (82 % of the issue slots, 4.0 TB/s).  So a lane holds four values and the four that they are paired
-// with: the rotation needs no exchange between lanes.  Weight, scale, cosine and sine are multiplied once per token into four factors
-// per pair, which serve every head that the lane walks through; the norm is one factor at the end.
+// with: the rotation needs no exchange between lanes.  Weight, cosine and sine are multiplied once per token into four factors
+// per pair, which serve every head that the lane walks through; norm and scale are one factor at the end.
 constexpr int kAppendThreads = 128;
 constexpr int kAppendBatch = 2;  // rounds of heads in flight: what more would bring costs as many registers, and with them blocks per SM
 
@@ -231,7 +231,8 @@ __device__ __forceinline__ void store8(void* p, int dtype, int64_t at, int lo, i
 template <typename Src, int LANES, bool INTERLEAVED>
 __global__ void __launch_bounds__(kAppendThreads) qk_norm_rope_append_kernel(const b200q_append_args a, float inv_dim, int rounds_per_block) {
   constexpr int kGroups = kAppendThreads / LANES;
-  __shared__ __align__(16) float s_weight[2][8 * LANES];  // scale times weight, of query and key heads
+  __shared__ __align__(16) float s_weight[2][8 * LANES];  // of query and key heads
+  __shared__ float s_scale[2];
   pdl_enter();
   const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
   const bool on = lane < a.dim / 8;
@@ -244,10 +245,12 @@ __global__ void __launch_bounds__(kAppendThreads) qk_norm_rope_append_kernel(con
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const void* weight = i ? a.k_weight : a.q_weight;
-    const float* scale = i ? a.k_scale : a.q_scale;
     for (int d = threadIdx.x; d < a.dim; d += kAppendThreads)
-      s_weight[i][d] = (scale ? *scale : 1.f) * (!weight ? 1.f : a.weight_dtype == B200Q_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(weight)[d])
-                                                                                             : static_cast<const float*>(weight)[d]);
+      s_weight[i][d] = !weight ? 1.f : a.weight_dtype == B200Q_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(weight)[d]) : static_cast<const float*>(weight)[d];
+  }
+  if (threadIdx.x == 0) {
+    s_scale[0] = a.q_scale ? *a.q_scale : 1.f;
+    s_scale[1] = a.k_scale ? *a.k_scale : 1.f;
   }
   const float v_scale = a.v_scale ? *a.v_scale : 1.f;
   const int k_begin = (a.heads + kGroups - 1) / kGroups, v_begin = k_begin + (a.kv_heads + kGroups - 1) / kGroups;
@@ -322,14 +325,15 @@ __global__ void __launch_bounds__(kAppendThreads) qk_norm_rope_append_kernel(con
         gb[i] = wb * sn[i];
       }
       heads(r0, r1, n_heads, src, src_stride, out, dtype, out_at, out_stride, [&](float (&x)[4], float (&y)[4]) {
-        float norm = 1.f;
+        // (the scale comes last: a rotation of values that it has made infinite would be NaN)
+        float norm = s_scale[which];
         if (normed) {
           float sum = 0.f;
 #pragma unroll
           for (int i = 0; i < 4; ++i) sum += x[i] * x[i] + y[i] * y[i];
 #pragma unroll
           for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o, LANES);
-          norm = rsqrtf(sum * inv_dim + a.eps);
+          norm *= rsqrtf(sum * inv_dim + a.eps);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from oracle import hpu_oracle as O
-from test_gpu_paged import BF16, E4M3, E5M2, F32, _close, _dense_check, _i32, _Model, _one, _Paged, _status  # noqa: F401 (_status: device status after each test)
+from test_gpu_paged import BF16, E4M3, E5M2, F32, _close, _dense_check, _i32, _Model, _one, _Paged, _status, _table  # noqa: F401 (_status: device status after each test)
 
 pytestmark = pytest.mark.gpu
 
@@ -43,6 +43,42 @@ def test_append_with_a_table_of_no_positions(rot):
     for t in (q, kc[0, :4]):
         assert bool(t[..., :rot].isnan().all()) and bool(t[..., rot:].isfinite().all())
     assert torch.equal(vc[0, :4], x[:, 2:])
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("src,cache", [(F32, E4M3), (BF16, E4M3), (F32, E5M2), (F32, BF16)])
+def test_append_large_values_times_a_scale(interleaved, src, cache):
+    """Values whose product with the scale passes the end of fp32: they turn first, and then saturate (or become infinite in bf16) with the sign
+    that the turned value has."""
+    g = torch.Generator().manual_seed(2)
+    x = ((torch.rand(5, 4, 64, generator=g) + 0.1) * torch.where(torch.rand(5, 4, 64, generator=g) < 0.5, -1e37, 1e37)).to(src)
+    kc, vc = (torch.zeros(1, 16, 1, 64).to(cache).cuda() for _ in range(2))
+    at, table, scale = torch.arange(5), _table(64), _one(1000.0).cuda()
+    q_dtype = E4M3 if cache == BF16 else cache
+    q = torch.ops.b200q.qk_norm_rope_append(x[:, :2].cuda(), x[:, 2:3].cuda(), x[:, 3:].cuda(), None, None, 1e-6, table.cuda(), at.cuda(), interleaved, at.cuda(), kc, vc,
+                                            scale, scale, scale, q_dtype)
+    limit = {E4M3: 448.0, E5M2: 57344.0, BF16: math.inf}
+    for got, dtype, rows in ((q, q_dtype, x[:, :2]), (kc[0, :5], cache, x[:, 2:3])):
+        want = O.norm_rope(rows, None, 0.0, table, at, interleaved)
+        far = want.abs() > 1e36  # (of the others a few may end below fp32's end)
+        assert float(far.double().mean()) > 0.8
+        assert torch.equal(got.float().cpu().double()[far], (want.sign() * limit[dtype])[far])
+    assert torch.equal(vc[0, :5].float().cpu(), x[:, 3:].float().sign() * limit[cache])
+
+
+@pytest.mark.parametrize("heads,kv", [(0, 2), (3, 0), (0, 0)])
+def test_append_without_queries_or_without_keys(heads, kv):
+    x = torch.randn(9, heads + 2 * kv, 64).to(BF16).cuda()
+    kc, vc = (torch.zeros(2, 16, kv, 64, dtype=BF16).cuda() for _ in range(2))
+    slots, pos = torch.randperm(32)[:9], torch.arange(9)
+    q = torch.ops.b200q.qk_norm_rope_append(x[:, :heads], x[:, heads:heads + kv], x[:, heads + kv:], None, None, 1e-6, _table(64).cuda(), pos.cuda(), False, slots.cuda(),
+                                            kc, vc)
+    assert q.shape == (9, heads, 64)
+    y = O.norm_rope(x.cpu(), None, 0.0, _table(64), pos, False)
+    tol = 2.0 ** -8 * y.abs() + 2.0 ** -20 * y.abs().amax(-1, keepdim=True) if heads + kv else y
+    _close(q.float(), y[:, :heads], tol[:, :heads])
+    _close(kc.view(32, kv, 64)[slots.cuda()].float(), y[:, heads:heads + kv], tol[:, heads:heads + kv])
+    assert torch.equal(vc.view(32, kv, 64)[slots.cuda()], x[:, heads + kv:])
 
 
 def _append_to(kc, vc, tokens=7):
