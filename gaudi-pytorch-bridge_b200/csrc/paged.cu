@@ -12,8 +12,10 @@ namespace b200q {
 // to ceil((c_b + n_b) / ps) come from the free list, in request order.  So everything follows from two prefix sums over
 // the requests (new tokens, new pages); a block forms both in shared memory for itself, and then no block waits for
 // another: a token reads its page either from an old table entry, which nobody writes, or from the free list.
-// All of it is latency (a few KB to 1 MB of output): 3.1 us for 64 requests, 5.2 for 32 prompts of 80 000 tokens together, 7.7 for 1024 requests and
-// 24 for 8192, whose sums are taken 256 requests at a time.
+// All of it is latency (a few KB to 1 MB of output): 3.1 us for 64 requests, 5.1 for 32 prompts of 80 000 tokens together, 7.7 for 1024 requests and
+// 24 for 8192, whose sums are taken 256 requests at a time.  Every block forms the sums again, so that more blocks cost SMs, not time: in blocks of 256 /
+// 1024 / 4096 tokens the 32 prompts take 4.6 / 5.1 / 12.8 us, 64 requests of 256 tokens each 3.1 / 6.2 / 16.4, 1024 of 16 4.8 / 8.2 / 21.5, one of 16384
+// 2.6 / 3.6 / 8.2, and steps of a token each up to 64 requests the same.
 constexpr int kPlanThreads = 256;
 constexpr int kPlanTokensPerBlock = 1024;
 
@@ -381,7 +383,10 @@ static int append_launch(const b200q_append_args& a, cudaStream_t st) {
   constexpr int kGroups = kAppendThreads / LANES;
   const int rounds = (a.heads + kGroups - 1) / kGroups + 2 * ((a.kv_heads + kGroups - 1) / kGroups);
   // Few tokens: a block per round or per batch of rounds, so that the whole device takes part.  Many: one resident set of blocks walks through
-  // them (8192 tokens of 64 + 2 x 8 heads of 128 in bf16, caches in e4m3: 65 us = 5.0 TB/s, against 71 with a block per token).
+  // them (8192 tokens of 64 + 2 x 8 heads of 128 in bf16, caches in e4m3: 65.8 us = 4.9 TB/s, against 71 with a block per token).
+  // us with a block per round / per batch / for all rounds of a token, of that shape (10 rounds): 16 tokens 2.57 / 2.70 / 4.87, 32 2.70 / 2.82 / 5.00,
+  // 64 2.95 / 2.95 / 5.00, 96 3.98 / 3.21 / 5.01, 256 7.70 / 5.65 / 8.36, 384 10.5 / 8.21 / 8.87, 512 13.0 / 9.34 / 9.22, 1024 23.0 / 15.3 / 11.8: the limits
+  // below are at 59 and 473 tokens.  3 rounds (8 + 2 x 1 heads): 64 2.57 / 2.95 / 3.33, 256 3.84 / 3.21 / 3.46, 1024 7.18 / 6.15 / 5.77 (limits 197 and 1184).
   const int64_t batches = (rounds + kAppendBatch - 1) / kAppendBatch;
   const int per = a.tokens * rounds <= 4 * kNumSMs ? 1 : a.tokens * batches <= 16 * kNumSMs ? kAppendBatch : rounds;
   const int64_t most = (int64_t)per_sm * kNumSMs;

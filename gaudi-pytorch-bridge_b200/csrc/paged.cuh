@@ -5,8 +5,6 @@
 
 namespace b200q {
 
-// Smallest number of 128-byte-or-less pieces etc. are the kernels' own business; these are the limits that the
-// C ABI documents.
 constexpr int64_t kPagedMaxRequests = 8192;  // the prefix sums over the requests live in shared memory
 
 struct PagedPlanParams {

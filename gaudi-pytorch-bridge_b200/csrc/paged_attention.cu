@@ -115,8 +115,8 @@ __global__ void __launch_bounds__(kPlainThreads) paged_attention_plain_kernel(co
 // is 64 bytes the pieces of V are 8 bytes, and a lane's the g-th.)
 // fp8 values become f16 exactly.  The probabilities of an fp8 cache are f16 too, scaled by 2^7 so that the small ones stay normal: one term
 // (11 bits) where the output is bf16 or e4m3, whose own rounding is 8 bits or fewer, and two terms (22 bits) that take a product each
-// where it is fp32.  Two terms everywhere would be 120.8 -> 130.5 us for 64 requests of 2048 to 8192 tokens (8 key/value heads of 128), a
-// branch in the loop 127; the error of that case's bf16 output is 1.66e-3 with one term and 1.65e-3 with 24 bits.  For a bf16 cache
+// where it is fp32.  Two terms everywhere would be 124 -> 131 us for 64 requests of 2048 to 8192 tokens (8 key/value heads of 128), and a branch
+// in the loop would cost all outputs 5 %; that case's bf16 output is 1.5e-3 from 64-bit arithmetic with one term, with two and with 24 bits.  For a bf16 cache
 // they are two bf16 terms (16 bits), twice as fine as any bf16 output.  Queries meet fp8 keys as f16, scaled
 // by a power of two per head, which is exact over 2^22 of a head's largest value.
 //
@@ -126,9 +126,9 @@ __global__ void __launch_bounds__(kPlainThreads) paged_attention_plain_kernel(co
 // kWarps / lanes groups of such warps cut the run again.  A run may begin or end inside a row of steps: such partial results
 // (maximum, sum, output) are joined in the CTA, and, where a row goes on in another CTA, by a second kernel.
 //
-// Measured (from a CUDA graph, shuffled pages): 64 requests of 8192 tokens, 8 key/value heads of 128 in e4m3, 173 us = 6.2 TB/s; the same in bf16, 32
-// requests, 163 us = 6.6 TB/s.  About 9 us of a call do not depend on the length: 3 of dependent loads (lengths, page numbers, first keys), 5 of
-// joining, and the launches.
+// Measured (from a CUDA graph, shuffled pages): 64 requests of 8192 tokens, 8 key/value heads of 128 in e4m3, 175 us = 6.1 TB/s (fp32 output 180); the same in
+// bf16, 32 requests, 165 us = 6.5 TB/s.  About 9 us of a call do not depend on the length: 3 of dependent loads (lengths, page numbers, first keys),
+// joining (a kernel of 5 to 11 us by itself, in part behind this one's end), and the launches.
 constexpr int kPagedGrid = kNumSMs;
 constexpr int kPagedRingBytes = 192 * 1024;
 constexpr int kPagedLaneSteps = 14;   // a warp's steps from which on heads go side by side
@@ -476,9 +476,10 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
   auto span_of = [&](int b) { return PagedSpan(a, lengths_here ? lengths[b] : paged_length(a, b)); };
   // Heads side by side where a warp's share is long enough to pay for a partial result of its own, or where rows are so many that few of
   // them are cut (and no warps of a CTA have parts of the same one), and only where a token's head is short of 512 bytes.  us, side by
-  // side / one head per CTA, 8 key/value heads of 128 in e4m3: 64 x 8192 tokens 176 / 218, 64 x 1000 36.8 / 41.3, 16 of 1024 to 4096 29.5 / 34.6,
-  // 4 x 10000 25.4 / 26.5, 1 x 32768 25.9 / 22.6, 1 x 8192 18.4 / 15.4; 256 x 200 38.2 / 43.9, 32 x 400 17.8 / 18.9; 4 heads, 100 of 75 to 300
-  // 25.1 / 20.0; 2 heads of 256 in bf16, 40 x 4000 66.0 / 63.7.
+  // side / one head per CTA, 8 key/value heads of 128 in e4m3: 64 x 8192 tokens 175 / 221, 8 x 16000 56 / 62, 64 x 1000 36.1 / 40.6, 256 x 200 37.4 / 43.3,
+  // 2 x 34000 36.0 / 37.9, 1 x 131072 58.1 / 62.8, 4 x 10000 25.3 / 25.6; below the limit 8 x 4000 24.8 / 23.4, 1 x 16384 20.8 / 16.9, 1 x 8192 18.3 / 15.2.
+  // 4 heads, 100 of 75 to 300 26.7 / 20.3; 2 heads of 256 in bf16, 40 x 4000 64.4 / 61.8.  The total of steps does not tell all of it: 16 requests of 1024 to
+  // 4096 30.0 / 26.2, 16 x 2600 28.0 / 27.1, 1 x 34000 26.5 / 23.2 and 1 x 65536 37.3 / 36.1 lie above the limit, 32 x 400 17.3 / 18.4 below.
   const int key_steps = prefix[requests - 1], warps = kWarps * (int)gridDim.x;
   const bool beside = Tile::kRow < 512 && (key_steps * w.heads_per_request >= kPagedLaneSteps * warps ||
                                            (w.lane_bits == kWarpBits && requests * w.heads_per_request >= warps / 4));

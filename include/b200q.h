@@ -558,7 +558,8 @@ int b200q_qk_norm_rope_append(const b200q_append_args* args);
  *   s_j = softmax_scale * k_scale_inv * <q, k_j>,  p = softmax(s) over j in [max(0, len - window), len) (window 0: all),
  *   out = T(v_scale_inv * sum_j p_j v_j * out_scale),  lse = log sum_j exp(s_j)
  * with scores, softmax and sums in fp32 and one rounding to T.  Before their product with the values the tensor-core kernel rounds the
- * probabilities: to 22 bits for an fp8 cache and T = F32, 11 bits for an fp8 cache and a narrower T, 16 bits for a bf16 cache.  A request of length 0 gets zeros and lse = -inf.
+ * probabilities: to 22 bits for an fp8 cache and T = F32, 11 bits for an fp8 cache and a narrower T, 16 bits for a bf16 cache.  Queries meet
+ * an fp8 cache as f16 after scaling by a power of two per head: exactly, down to 2^-22 of a head's largest value.  A request of length 0 gets zeros and lse = -inf.
  * Query head h reads key/value head h / (heads / kv_heads).  Lengths are cut to table_width * page_size; keys whose table
  * entry is outside [0, num_pages) do not exist.  The cache behind a request's length is not looked at.
  *
