@@ -726,7 +726,7 @@ __global__ void __launch_bounds__(32 * PagedTile<DIM, FMT, NT>::kWarps, 1)
             float top = fmaxf(s[n][i], s[n][i + 2]);
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-            const float raised = top > acc.m[n][i] + Tile::kRescale ? top - Tile::kShift : acc.m[n][i];
+            const float raised = __fsub_rn(top, acc.m[n][i]) > Tile::kRescale ? top - Tile::kShift : acc.m[n][i];  // (by the exponent itself: m + 15 may be rounded up)
             const float keep = paged_exp2(acc.m[n][i] - raised);
             acc.m[n][i] = raised;
             acc.l[n][i] *= keep;

@@ -408,3 +408,28 @@ def test_attention_large_values_of_a_bf16_cache(heads, kv, dim, rising):
     got, got_lse = torch.ops.b200q.paged_attention(q.cuda(), p.k.cuda(), p.v.cuda(), p.table.cuda(), p.lens.cuda(), scale)
     _close(got.float(), want, 2.0 ** -8 * want.abs() + (2.0 ** -11 + 2.0 ** -13) * size)
     _close(got_lse, lse, 2.0 ** -13 + 2.0 ** -22 * torch.where(lse.isfinite(), lse.abs(), 0.0))
+
+
+@pytest.mark.parametrize("cache", [E4M3, E5M2, BF16])
+@pytest.mark.parametrize("dim,heads", [(64, 8), (128, 1), (128, 12), (256, 4)])
+@pytest.mark.parametrize("base,rise", [(base * 2.0 ** i, rise) for base in (1.5, -1.5) for i, rise in ((24, 8), (25, 8), (26, 8), (27, 16), (28, 32))])
+def test_attention_scores_that_rise_far_from_0(cache, dim, heads, base, rise):
+    """Scores of 1.5 times 2^24 to 2^28 (in powers of two, exactly), where the neighbours of a number are 2 to 32 away, and a little more for
+    every 16 keys: probabilities of up to 2^16 against the maximum so far, less the 7 that it is held below, which f16 does not hold.  (Not for the plain kernel, whose
+    scores are in powers of e and not exact here: spacing 8 against a difference of 8 ln 2 and 16 ln 2.)"""
+    p = _Paged([0, 16, 17, 40, 128, 128, 128], 1, dim, cache, 16, seed=8)
+    k = torch.zeros(p.k.shape)
+    k[..., 0] = 256.0
+    for b, n in enumerate(p.lens.tolist()):
+        for i in range(-(-n // 16)):
+            k[int(p.table[b, i]), :, :, 1] = i
+    p.k = torch.where(p.k.float().isnan(), math.nan, k).to(cache)
+    q = torch.zeros(7, heads, dim)
+    q[..., 0], q[..., 1] = base / 256, rise
+    q, scale = q.to(BF16), float.fromhex("0x1.62e42fefa39efp-1")
+    as_held = float(torch.tensor(scale, dtype=F32))
+    assert float(torch.tensor(as_held, dtype=F32) * torch.tensor(1.44269504088896341, dtype=F32)) == 1.0
+    want, lse, size = O.paged_attention(q, p.k, p.v, p.table, p.lens, scale)
+    got, got_lse = torch.ops.b200q.paged_attention(q.cuda(), p.k.cuda(), p.vd, p.table.cuda(), p.lens.cuda(), scale)
+    _close(got.float(), want, 2.0 ** -8 * want.abs() + (2.0 ** -11 + 2.0 ** -13) * size)
+    _close(got_lse, lse, 2.0 ** -21 * torch.where(lse.isfinite(), lse.abs(), 0.0))
