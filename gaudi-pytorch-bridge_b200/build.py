@@ -5,6 +5,7 @@ Usage: python build.py [--force] [--verbose-ptxas]
 Objects are rebuilt only when a source or header is newer.  What ptxas says of each kernel (registers, spills, shared memory) is
 kept beside the object as build/<source>.ptxas.
 """
+import concurrent.futures
 import glob
 import os
 import subprocess
@@ -39,20 +40,24 @@ def build_kernels(force=False, ptxas_verbose=False):
     os.makedirs(LIB, exist_ok=True)
     os.makedirs(OBJ, exist_ok=True)
     headers = glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(CSRC, "*.h")) + glob.glob(os.path.join(ROOT, "include", "*.h"))
-    objs = []
-    log = ""
+    objs, stale = [], []
     for src in sorted(glob.glob(os.path.join(CSRC, "*.cu"))):
         obj = os.path.join(OBJ, os.path.basename(src)[:-3] + ".o")
         objs.append(obj)
-        report = obj[:-2] + ".ptxas"
-        if force or _newer(obj, [src] + headers) or not os.path.exists(report):
-            cmd = [NVCC, *ARCH, "-O3", "-lineinfo", "-std=c++17", "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC", "-Xptxas", "-v",
-                   "-I", os.path.join(ROOT, "include"), "-I", CSRC, "-c", src, "-o", obj]
-            text = _run(cmd)
-            with open(report, "w") as f:
-                f.write(text)
-            if ptxas_verbose:
-                log += text
+        if force or _newer(obj, [src] + headers) or not os.path.exists(obj[:-2] + ".ptxas"):
+            stale.append((src, obj))
+
+    def compile_one(job):
+        src, obj = job
+        text = _run([NVCC, *ARCH, "-O3", "-lineinfo", "-std=c++17", "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC", "-Xptxas", "-v",
+                     "-I", os.path.join(ROOT, "include"), "-I", CSRC, "-c", src, "-o", obj])
+        with open(obj[:-2] + ".ptxas", "w") as f:
+            f.write(text)
+        return text
+
+    with concurrent.futures.ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
+        logs = list(pool.map(compile_one, stale))
+    log = "".join(logs) if ptxas_verbose else ""
     so = os.path.join(LIB, "libb200q.so")
     if force or _newer(so, objs):
         _run([NVCC, *ARCH, "-shared", "-o", so, *objs])
