@@ -24,6 +24,7 @@ EXPORTS = [
     "b200q_nchw_to_nhwc_u8", "b200q_im2col_nhwc_fp8",
     "b200q_paged_plan", "b200q_qk_norm_rope_append", "b200q_paged_attention_workspace_bytes", "b200q_paged_attention",
     "b200q_selftest_paged_wait_timeout",
+    "b200q_add_rms_norm_cast", "b200q_lora_workspace_bytes", "b200q_lora_add", "b200q_moe_workspace_bytes", "b200q_moe_layer",
 ]
 
 DTYPE = {torch.float32: F32, torch.bfloat16: BF16, torch.float8_e4m3fn: E4M3, torch.float8_e5m2: E5M2}
@@ -100,6 +101,34 @@ class PagedAttentionArgs(C.Structure):
     ]
 
 
+class NormArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("x_dtype", C.c_int), ("tokens", C.c_int64), ("dim", C.c_int64), ("x_stride", C.c_int64),
+        ("residual", C.c_void_p), ("residual_stride", C.c_int64), ("weight", C.c_void_p), ("weight_dtype", C.c_int), ("eps", C.c_float),
+        ("out", C.c_void_p), ("out_dtype", C.c_int), ("scale", C.c_void_p), ("scale_inv", C.c_void_p), ("kept", C.c_void_p), ("stream", C.c_void_p),
+    ]
+
+
+class LoraArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("x_stride", C.c_int64), ("y", C.c_void_p), ("y_dtype", C.c_int), ("y_stride", C.c_int64),
+        ("a", C.c_void_p), ("b", C.c_void_p), ("a_stride", C.c_int64), ("a_row_stride", C.c_int64), ("b_stride", C.c_int64), ("b_row_stride", C.c_int64),
+        ("adapter", C.c_void_p), ("scales", C.c_void_p),
+        ("tokens", C.c_int64), ("k", C.c_int64), ("n", C.c_int64), ("rank", C.c_int64), ("adapters", C.c_int64),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("force_plain", C.c_int), ("stream", C.c_void_p),
+    ]
+
+
+class MoeArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("x_stride", C.c_int64), ("tokens", C.c_int64), ("hidden", C.c_int64), ("inner", C.c_int64),
+        ("experts", C.c_int), ("top_k", C.c_int), ("renormalize", C.c_int), ("router", C.c_void_p), ("router_dtype", C.c_int),
+        ("gate_up", C.c_void_p), ("down", C.c_void_p), ("weight_dtype", C.c_int), ("gate_up_scale", C.c_void_p), ("down_scale", C.c_void_p),
+        ("num_tokens", C.c_void_p), ("out", C.c_void_p), ("out_dtype", C.c_int), ("weights", C.c_void_p), ("ids", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("force_plain", C.c_int), ("stream", C.c_void_p),
+    ]
+
+
 def _bind():
     lib = C.CDLL(_LIB_PATH, mode=C.RTLD_GLOBAL)
     lib.b200q_strerror.restype = C.c_char_p
@@ -154,6 +183,13 @@ def _bind():
     lib.b200q_paged_attention_workspace_bytes.argtypes = [C.c_int64, C.c_int, C.c_int, C.c_int, C.c_int]
     lib.b200q_paged_attention.argtypes = [C.POINTER(PagedAttentionArgs)]
     lib.b200q_selftest_paged_wait_timeout.argtypes = [C.POINTER(PagedAttentionArgs), C.c_int, C.c_int, C.c_int]
+    lib.b200q_add_rms_norm_cast.argtypes = [C.POINTER(NormArgs)]
+    lib.b200q_lora_workspace_bytes.restype = C.c_size_t
+    lib.b200q_lora_workspace_bytes.argtypes = [C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_int64]
+    lib.b200q_lora_add.argtypes = [C.POINTER(LoraArgs)]
+    lib.b200q_moe_workspace_bytes.restype = C.c_size_t
+    lib.b200q_moe_workspace_bytes.argtypes = [C.c_int64, C.c_int64, C.c_int64, C.c_int, C.c_int]
+    lib.b200q_moe_layer.argtypes = [C.POINTER(MoeArgs)]
     return lib
 
 

@@ -7,6 +7,7 @@
 #include "common.cuh"
 #include "fp8_misc.cuh"
 #include "gemm_common.cuh"
+#include "layer.cuh"
 #include "paged.cuh"
 #include "paged_layout.h"
 #include "tcgen05_ptx.cuh"
@@ -138,6 +139,12 @@ static bool on_bytes(size_t bytes, std::initializer_list<const void*> pointers) 
     if (reinterpret_cast<uintptr_t>(p) % bytes) return false;
   return true;
 }
+// whether no byte belongs to both of two matrices of one type and shape (the first one's rows lie apart)
+static bool rows_apart(const void* p, int64_t p_stride, const void* q, int64_t q_stride, int dtype, int64_t rows, int64_t cols) {
+  const int64_t sizes[3] = {rows, 1, 1}, elt = dtype == B200Q_F32 ? 4 : 2;
+  const CacheLayout first(p, elt, cols, sizes, {p_stride, 0, 0}), second(q, elt, cols, sizes, {q_stride, 0, 0});
+  return first.apart() && first.apart_from(second);
+}
 static bool scale_args_ok(const float* dev, int mode) {
   if (mode < B200Q_BCAST_NONE || mode > B200Q_BCAST_FULL) return false;
   if (mode >= B200Q_BCAST_SCALAR_DEV && !dev) return false;
@@ -172,6 +179,9 @@ size_t b200q_sizeof_args(int which) {
     case 1: return sizeof(b200q_sdpa_args);
     case 2: return sizeof(b200q_append_args);
     case 3: return sizeof(b200q_paged_attention_args);
+    case 4: return sizeof(b200q_norm_args);
+    case 5: return sizeof(b200q_lora_args);
+    case 6: return sizeof(b200q_moe_args);
     default: return 0;
   }
 }
@@ -580,6 +590,60 @@ int b200q_w4a16_gemm_noalloc(const void* x, int64_t ldx, const int32_t* qweight,
   if (zp_kind == B200Q_ZP_PACKED && !zp) return B200Q_ERR_BAD_ARGUMENT;
   return w4a16_gemm_noalloc_impl(x, ldx, qweight, scale, zp, zp_kind, k_packed, M, N, K, group, out, out_dtype, ldo,
                                  static_cast<cudaStream_t>(stream));
+}
+
+int b200q_add_rms_norm_cast(const b200q_norm_args* a) {
+  if (!a) return B200Q_ERR_BAD_ARGUMENT;
+  if (a->tokens < 0 || a->dim < 0 || !is_wide(a->x_dtype) || !(a->out_dtype == B200Q_BF16 || is_fp8(a->out_dtype))) return B200Q_ERR_BAD_ARGUMENT;
+  if (a->weight && !is_wide(a->weight_dtype)) return B200Q_ERR_BAD_ARGUMENT;
+  if (a->scale_inv && (a->scale || !is_fp8(a->out_dtype))) return B200Q_ERR_BAD_ARGUMENT;
+  if (a->residual && a->tokens > 1 && a->residual_stride < a->dim) return B200Q_ERR_BAD_ARGUMENT;
+  if (a->tokens > INT32_MAX || a->dim > INT32_MAX) return B200Q_ERR_TOO_LARGE;
+  if (a->tokens == 0) return B200Q_OK;
+  if (a->dim > 0 && (!a->x || !a->out)) return B200Q_ERR_BAD_ARGUMENT;
+  if (!on_elements(a->x, a->x_dtype, 1) || !on_elements(a->residual, a->x_dtype, 1) || !on_elements(a->weight, a->weight_dtype, 1) ||
+      !on_elements(a->out, a->out_dtype, 1) || !on_bytes(2, {a->kept}) || !on_bytes(4, {a->scale, a->scale_inv}))
+    return B200Q_ERR_UNSUPPORTED;
+  if (a->dim == 0 && !a->scale_inv) return B200Q_OK;
+  if (a->residual && !rows_apart(a->residual, a->residual_stride, a->x, a->x_stride, a->x_dtype, a->tokens, a->dim)) return B200Q_ERR_BAD_ARGUMENT;
+  return add_rms_norm_cast_impl(*a, static_cast<cudaStream_t>(a->stream));
+}
+
+size_t b200q_lora_workspace_bytes(int64_t tokens, int64_t k, int64_t n, int64_t rank, int64_t adapters) {
+  if (tokens <= 0 || k <= 0 || n <= 0 || rank <= 0 || adapters <= 0 || rank > kLoraMaxRank || adapters > kLoraMaxAdapters) return 0;
+  return lora_workspace_bytes_impl(tokens, k, n, rank, adapters);
+}
+
+int b200q_lora_add(const b200q_lora_args* a) {
+  if (!a) return B200Q_ERR_BAD_ARGUMENT;
+  if (a->tokens < 0 || a->k < 0 || a->n < 0 || a->rank < 0 || a->adapters < 0 || !is_wide(a->y_dtype)) return B200Q_ERR_BAD_ARGUMENT;
+  if (a->tokens > 1 && a->y_stride < a->n) return B200Q_ERR_BAD_ARGUMENT;
+  if (a->rank > kLoraMaxRank || a->adapters > kLoraMaxAdapters || a->tokens > INT32_MAX || a->k > INT32_MAX || a->n > INT32_MAX) return B200Q_ERR_TOO_LARGE;
+  if (a->tokens == 0 || a->n == 0 || a->rank == 0 || a->adapters == 0 || a->k == 0) return B200Q_OK;  // (nothing is added)
+  if (!a->x || !a->y || !a->a || !a->b || !a->adapter) return B200Q_ERR_BAD_ARGUMENT;
+  if (!on_bytes(2, {a->x, a->a, a->b}) || !on_elements(a->y, a->y_dtype, 1) || !on_bytes(4, {a->adapter, a->scales})) return B200Q_ERR_UNSUPPORTED;
+  return lora_add_impl(*a, static_cast<cudaStream_t>(a->stream));
+}
+
+size_t b200q_moe_workspace_bytes(int64_t tokens, int64_t hidden, int64_t inner, int experts, int top_k) {
+  if (tokens <= 0 || hidden < 0 || inner < 0 || experts <= 0 || top_k <= 0 || experts > kMoeMaxExperts || top_k > kMoeMaxTopK) return 0;
+  return moe_workspace_bytes_impl(tokens, hidden, inner, experts, top_k);
+}
+
+int b200q_moe_layer(const b200q_moe_args* a) {
+  if (!a) return B200Q_ERR_BAD_ARGUMENT;
+  if (a->tokens < 0 || a->hidden < 0 || a->inner < 0 || a->experts < 1 || a->top_k < 1 || a->top_k > a->experts) return B200Q_ERR_BAD_ARGUMENT;
+  if (!is_wide(a->router_dtype) || !is_wide(a->out_dtype) || !(a->weight_dtype == B200Q_BF16 || a->weight_dtype == B200Q_E4M3)) return B200Q_ERR_BAD_ARGUMENT;
+  if (a->experts > kMoeMaxExperts || a->top_k > kMoeMaxTopK || a->tokens > INT32_MAX || a->hidden > INT32_MAX || a->inner > INT32_MAX / 2)
+    return B200Q_ERR_TOO_LARGE;
+  if (a->tokens == 0) return B200Q_OK;
+  if (!a->weights || !a->ids) return B200Q_ERR_BAD_ARGUMENT;
+  if (a->hidden > 0 && (!a->x || !a->router || !a->out || (a->inner > 0 && (!a->gate_up || !a->down)))) return B200Q_ERR_BAD_ARGUMENT;
+  if (!on_bytes(2, {a->x}) || !on_elements(a->router, a->router_dtype, 1) || !on_elements(a->gate_up, a->weight_dtype, 1) ||
+      !on_elements(a->down, a->weight_dtype, 1) || !on_elements(a->out, a->out_dtype, 1) ||
+      !on_bytes(4, {a->gate_up_scale, a->down_scale, a->num_tokens, a->weights, a->ids}))
+    return B200Q_ERR_UNSUPPORTED;
+  return moe_layer_impl(*a, static_cast<cudaStream_t>(a->stream));
 }
 
 }  // extern "C"

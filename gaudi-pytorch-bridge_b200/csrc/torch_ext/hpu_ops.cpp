@@ -1578,6 +1578,190 @@ std::tuple<at::Tensor, at::Tensor> meta_paged_attention(const at::Tensor& q, con
           at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat))};
 }
 
+// ---- what stands around the FP8 products of a decoder layer (no counterpart in the reference; the contract is in b200q.h) ----
+// rows of contiguous values; a view whose values are not contiguous is copied
+at::Tensor layer_rows(const at::Tensor& t) { return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+int64_t layer_row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(-1); }
+// Whether a written matrix [rows][values] lies apart in itself, and from one that is read.
+b200q::CacheLayout layer_layout(const at::Tensor& t) {
+  return b200q::CacheLayout(t.const_data_ptr(), (int64_t)t.element_size(), t.size(1), {t.size(0), 1, 1}, {t.size(0) > 1 ? t.stride(0) : 0, 0, 0});
+}
+void layer_check_written(const at::Tensor& out, const char* op, const char* name) {
+  TORCH_CHECK(out.size(1) <= 1 || out.stride(1) == 1, op, ": the values of a row of ", name, " must be contiguous");
+  TORCH_CHECK(out.size(0) <= 1 || out.stride(0) >= out.size(1), op, ": the rows of ", name, " must not overlap");
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rms_norm_cast(const at::Tensor& x, const OptTensor& residual_opt, const OptTensor& weight_opt, double eps,
+                                                                 at::ScalarType dtype, const OptTensor& scale_opt, bool keep) {
+  const char* op = "add_rms_norm_cast";
+  const at::Device dev = x.device();
+  at::Tensor residual = paged_optional(residual_opt), weight = paged_optional(weight_opt), scale = paged_optional(scale_opt);
+  paged_same_device(dev, {&residual, &weight, &scale}, op);
+  c10::cuda::CUDAGuard guard(dev);
+  const auto src = x.scalar_type();
+  TORCH_CHECK(src == at::kFloat || src == at::kBFloat16, op, ": x must be float or bfloat16, got ", src);
+  TORCH_CHECK(x.dim() == 2, op, ": x must be [tokens, dim], got ", x.sizes());
+  TORCH_CHECK(dtype == at::kBFloat16 || is_fp8(dtype), op, ": dtype must be bfloat16, float8_e4m3fn or float8_e5m2, got ", dtype);
+  const int64_t tokens = x.size(0), dim = x.size(1);
+  at::Tensor xr = layer_rows(x);
+  if (residual.defined()) {
+    TORCH_CHECK(residual.scalar_type() == src && residual.sizes() == x.sizes(), op, ": residual must have x's dtype and shape, got ", residual.scalar_type(), " ",
+                residual.sizes());
+    layer_check_written(residual, op, "residual");
+    TORCH_CHECK(layer_layout(residual).apart_from(layer_layout(xr)), op, ": residual must not overlap x");
+  }
+  if (weight.defined()) {
+    TORCH_CHECK((weight.scalar_type() == at::kFloat || weight.scalar_type() == at::kBFloat16) && weight.dim() == 1 && weight.numel() == dim, op,
+                ": weight must be a float or bfloat16 tensor of ", dim, " values");
+    weight = weight.contiguous();
+  }
+  const bool dynamic = is_fp8(dtype) && !scale.defined();
+  at::Tensor out = new_tensor({tokens, dim}, dtype, dev);
+  at::Tensor scale_inv = dynamic ? new_tensor({tokens, 1}, at::kFloat, dev) : new_tensor({0}, at::kFloat, dev);
+  at::Tensor kept = keep ? new_tensor({tokens, dim}, at::kBFloat16, dev) : new_tensor({0}, at::kBFloat16, dev);
+  b200q_norm_args a{};
+  a.x = xr.const_data_ptr(); a.x_dtype = to_b200q_dtype(src);
+  a.tokens = tokens; a.dim = dim; a.x_stride = layer_row_stride(xr);
+  if (residual.defined()) {
+    a.residual = residual.data_ptr();
+    a.residual_stride = layer_row_stride(residual);
+  }
+  if (weight.defined()) {
+    a.weight = weight.const_data_ptr();
+    a.weight_dtype = to_b200q_dtype(weight.scalar_type());
+  }
+  a.eps = (float)eps;
+  a.out = out.data_ptr(); a.out_dtype = to_b200q_dtype(dtype);
+  a.scale = paged_scale(scale, op, "scale");
+  a.scale_inv = dynamic ? scale_inv.data_ptr<float>() : nullptr;
+  a.kept = keep ? kept.data_ptr() : nullptr;
+  a.stream = current_stream();
+  check_status(b200q_add_rms_norm_cast(&a), op);
+  return {out, scale_inv, kept};
+}
+
+at::Tensor& lora_add_(at::Tensor& y, const at::Tensor& x, const at::Tensor& a_w, const at::Tensor& b_w, const at::Tensor& adapter, const OptTensor& scales_opt) {
+  const char* op = "lora_add_";
+  const at::Device dev = y.device();
+  at::Tensor scales = paged_optional(scales_opt);
+  paged_same_device(dev, {&x, &a_w, &b_w, &adapter, &scales}, op);
+  c10::cuda::CUDAGuard guard(dev);
+  TORCH_CHECK(y.scalar_type() == at::kFloat || y.scalar_type() == at::kBFloat16, op, ": y must be float or bfloat16, got ", y.scalar_type());
+  for (const at::Tensor* t : {&x, &a_w, &b_w}) TORCH_CHECK(t->scalar_type() == at::kBFloat16, op, ": x, a and b must be bfloat16, got ", t->scalar_type());
+  TORCH_CHECK(y.dim() == 2 && x.dim() == 2 && a_w.dim() == 3 && b_w.dim() == 3, op,
+              ": y [tokens, n], x [tokens, k], a [adapters, rank, k] and b [adapters, n, rank] wanted, got ", y.sizes(), ", ", x.sizes(), ", ", a_w.sizes(), " and ",
+              b_w.sizes());
+  const int64_t tokens = y.size(0), n = y.size(1), k = x.size(1), adapters = a_w.size(0), rank = a_w.size(1);
+  TORCH_CHECK(x.size(0) == tokens && a_w.size(2) == k && b_w.size(0) == adapters && b_w.size(1) == n && b_w.size(2) == rank, op,
+              ": y [tokens, n], x [tokens, k], a [adapters, rank, k] and b [adapters, n, rank] wanted, got ", y.sizes(), ", ", x.sizes(), ", ", a_w.sizes(), " and ",
+              b_w.sizes());
+  TORCH_CHECK(adapter.scalar_type() == at::kInt && adapter.dim() == 1 && adapter.numel() == tokens, op, ": adapter must be an int32 tensor of one entry per token");
+  TORCH_CHECK(!scales.defined() || (scales.scalar_type() == at::kFloat && scales.dim() == 1 && scales.numel() == adapters), op,
+              ": scales must be a float tensor of one entry per adapter");
+  layer_check_written(y, op, "y");
+  at::Tensor xr = layer_rows(x), ar = layer_rows(a_w), br = layer_rows(b_w), which = adapter.contiguous();
+  if (scales.defined()) scales = scales.contiguous();
+  for (const at::Tensor* t : {&xr, &ar, &br}) {
+    if (t->numel() == 0 || y.numel() == 0 || !t->is_alias_of(y)) continue;
+    TORCH_CHECK(t == &xr && y.scalar_type() == at::kBFloat16 && layer_layout(y).apart_from(layer_layout(xr)), op, ": y must not overlap x, a or b");
+  }
+  b200q_lora_args a{};
+  a.x = xr.const_data_ptr(); a.x_stride = layer_row_stride(xr);
+  a.y = y.data_ptr(); a.y_dtype = to_b200q_dtype(y.scalar_type()); a.y_stride = layer_row_stride(y);
+  a.a = ar.const_data_ptr(); a.b = br.const_data_ptr();
+  a.a_stride = ar.stride(0); a.a_row_stride = rank > 1 ? ar.stride(1) : k;
+  a.b_stride = br.stride(0); a.b_row_stride = n > 1 ? br.stride(1) : rank;
+  if (adapters <= 1) {  // (a stride that no index uses)
+    a.a_stride = a.a_row_stride * rank;
+    a.b_stride = a.b_row_stride * n;
+  }
+  a.adapter = which.const_data_ptr<int32_t>();
+  a.scales = scales.defined() ? scales.const_data_ptr<float>() : nullptr;
+  a.tokens = tokens; a.k = k; a.n = n; a.rank = rank; a.adapters = adapters;
+  const size_t bytes = b200q_lora_workspace_bytes(tokens, k, n, rank, adapters);
+  at::Tensor workspace;
+  if (bytes) {
+    workspace = new_tensor({(int64_t)bytes}, at::kByte, dev);
+    a.workspace = workspace.data_ptr();
+    a.workspace_bytes = bytes;
+  }
+  a.stream = current_stream();
+  check_status(b200q_lora_add(&a), op);
+  return y;
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> moe_layer(const at::Tensor& x, const at::Tensor& router, const at::Tensor& gate_up, const at::Tensor& down,
+                                                         const OptTensor& gate_up_scale_opt, const OptTensor& down_scale_opt, int64_t top_k, bool renormalize,
+                                                         const OptTensor& num_tokens_opt, c10::optional<at::ScalarType> out_dtype_opt) {
+  const char* op = "moe_layer";
+  const at::Device dev = x.device();
+  at::Tensor scales[2] = {paged_optional(gate_up_scale_opt), paged_optional(down_scale_opt)}, num_tokens = paged_optional(num_tokens_opt);
+  paged_same_device(dev, {&router, &gate_up, &down, &scales[0], &scales[1], &num_tokens}, op);
+  c10::cuda::CUDAGuard guard(dev);
+  TORCH_CHECK(x.scalar_type() == at::kBFloat16 && x.dim() == 2, op, ": x must be a bfloat16 tensor [tokens, hidden]");
+  TORCH_CHECK((router.scalar_type() == at::kBFloat16 || router.scalar_type() == at::kFloat) && router.dim() == 2, op,
+              ": router must be a float or bfloat16 tensor [experts, hidden]");
+  const auto wt = gate_up.scalar_type();
+  TORCH_CHECK((wt == at::kBFloat16 || wt == at::kFloat8_e4m3fn) && down.scalar_type() == wt, op,
+              ": gate_up and down must both be bfloat16 or float8_e4m3fn, got ", wt, " and ", down.scalar_type());
+  const int64_t tokens = x.size(0), hidden = x.size(1), experts = router.size(0);
+  TORCH_CHECK(gate_up.dim() == 3 && down.dim() == 3 && router.size(1) == hidden && gate_up.size(0) == experts && down.size(0) == experts &&
+                  gate_up.size(1) == 2 * down.size(2) && gate_up.size(2) == hidden && down.size(1) == hidden,
+              op, ": x [tokens, hidden], router [experts, hidden], gate_up [experts, 2 inner, hidden] and down [experts, hidden, inner] wanted, got ", x.sizes(), ", ",
+              router.sizes(), ", ", gate_up.sizes(), " and ", down.sizes());
+  const int64_t inner = down.size(2);
+  TORCH_CHECK(gate_up.is_contiguous() && down.is_contiguous(), op, ": gate_up and down must be contiguous");
+  TORCH_CHECK(experts >= 1 && experts <= 512, op, ": 1 to 512 experts wanted, got ", experts);
+  TORCH_CHECK(top_k >= 1 && top_k <= std::min<int64_t>(16, experts), op, ": top_k must be from 1 to 16, and at most the number of experts, got ", top_k);
+  const int64_t channels[2] = {2 * inner, hidden};
+  for (int i = 0; i < 2; ++i) {
+    if (!scales[i].defined()) continue;
+    TORCH_CHECK(scales[i].scalar_type() == at::kFloat && scales[i].dim() == 2 && scales[i].size(0) == experts && scales[i].size(1) == channels[i], op, ": ",
+                i ? "down_scale_inv" : "gate_up_scale_inv", " must be a float tensor [", experts, ", ", channels[i], "], got ", scales[i].sizes());
+    scales[i] = scales[i].contiguous();
+  }
+  TORCH_CHECK(!num_tokens.defined() || (num_tokens.scalar_type() == at::kInt && num_tokens.numel() == 1), op, ": num_tokens must be an int32 tensor of one element");
+  const auto out_dtype = out_dtype_opt.value_or(at::kBFloat16);
+  TORCH_CHECK(out_dtype == at::kBFloat16 || out_dtype == at::kFloat, op, ": out_dtype must be bfloat16 or float, got ", out_dtype);
+  at::Tensor xr = layer_rows(x), rr = router.contiguous();
+  at::Tensor out = new_tensor({tokens, hidden}, out_dtype, dev), weights = new_tensor({tokens, top_k}, at::kFloat, dev), ids = new_tensor({tokens, top_k}, at::kInt, dev);
+  b200q_moe_args a{};
+  a.x = xr.const_data_ptr(); a.x_stride = layer_row_stride(xr);
+  a.tokens = tokens; a.hidden = hidden; a.inner = inner;
+  a.experts = (int)experts; a.top_k = (int)top_k; a.renormalize = renormalize;
+  a.router = rr.const_data_ptr(); a.router_dtype = to_b200q_dtype(rr.scalar_type());
+  a.gate_up = gate_up.const_data_ptr(); a.down = down.const_data_ptr(); a.weight_dtype = to_b200q_dtype(wt);
+  a.gate_up_scale = scales[0].defined() ? scales[0].const_data_ptr<float>() : nullptr;
+  a.down_scale = scales[1].defined() ? scales[1].const_data_ptr<float>() : nullptr;
+  a.num_tokens = num_tokens.defined() ? num_tokens.const_data_ptr<int32_t>() : nullptr;
+  a.out = out.data_ptr(); a.out_dtype = to_b200q_dtype(out_dtype);
+  a.weights = weights.data_ptr<float>(); a.ids = ids.data_ptr<int32_t>();
+  const size_t bytes = b200q_moe_workspace_bytes(tokens, hidden, inner, a.experts, a.top_k);
+  at::Tensor workspace;
+  if (bytes) {
+    workspace = new_tensor({(int64_t)bytes}, at::kByte, dev);
+    a.workspace = workspace.data_ptr();
+    a.workspace_bytes = bytes;
+  }
+  a.stream = current_stream();
+  check_status(b200q_moe_layer(&a), op);
+  return {out, weights, ids};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> meta_add_rms_norm_cast(const at::Tensor& x, const OptTensor&, const OptTensor&, double, at::ScalarType dtype,
+                                                                      const OptTensor& scale, bool keep) {
+  const bool dynamic = is_fp8(dtype) && !(scale.has_value() && scale->defined());
+  const auto f32 = x.options().dtype(at::kFloat), bf16 = x.options().dtype(at::kBFloat16);
+  return {at::empty(x.sizes(), x.options().dtype(dtype)), dynamic ? at::empty({x.size(0), 1}, f32) : at::empty({0}, f32),
+          keep ? at::empty(x.sizes(), bf16) : at::empty({0}, bf16)};
+}
+at::Tensor& meta_lora_add_(at::Tensor& y, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const OptTensor&) { return y; }
+std::tuple<at::Tensor, at::Tensor, at::Tensor> meta_moe_layer(const at::Tensor& x, const at::Tensor&, const at::Tensor&, const at::Tensor&, const OptTensor&,
+                                                              const OptTensor&, int64_t top_k, bool, const OptTensor&, c10::optional<at::ScalarType> out_dtype) {
+  return {at::empty(x.sizes(), x.options().dtype(out_dtype.value_or(at::kBFloat16))), at::empty({x.size(0), top_k}, x.options().dtype(at::kFloat)),
+          at::empty({x.size(0), top_k}, x.options().dtype(at::kInt))};
+}
+
 void set_sr_seed(int64_t seed) {
   g_sr_seed.store(seed);
   g_sr_offset.store(0);
@@ -1769,6 +1953,9 @@ TORCH_LIBRARY(b200q, m) {
   m.def("paged_plan(Tensor context_lens, Tensor new_lens, Tensor(a!) block_table, Tensor free_pages, Tensor? free_head, int page_size, int num_tokens) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
   m.def("qk_norm_rope_append(Tensor q, Tensor k, Tensor v, Tensor? q_weight, Tensor? k_weight, float eps, Tensor? cos_sin, Tensor? positions, bool interleaved, Tensor slot_map, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor? k_scale=None, Tensor? v_scale=None, Tensor? q_scale=None, ScalarType? q_dtype=None) -> Tensor");
   m.def("paged_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor kv_lens, float softmax_scale, Tensor? k_scale_inv=None, Tensor? v_scale_inv=None, int window=0, Tensor? out_scale=None, ScalarType? out_dtype=None) -> (Tensor, Tensor)");
+  m.def("add_rms_norm_cast(Tensor x, Tensor(a!)? residual, Tensor? weight, float eps, ScalarType dtype, Tensor? scale=None, bool keep=False) -> (Tensor, Tensor, Tensor)");
+  m.def("lora_add_(Tensor(a!) y, Tensor x, Tensor a, Tensor b, Tensor adapter, Tensor? scales=None) -> Tensor(a!)");
+  m.def("moe_layer(Tensor x, Tensor router, Tensor gate_up, Tensor down, Tensor? gate_up_scale_inv, Tensor? down_scale_inv, int top_k, bool renormalize=True, Tensor? num_tokens=None, ScalarType? out_dtype=None) -> (Tensor, Tensor, Tensor)");
   m.def("set_sr_seed(int seed) -> ()", set_sr_seed);
   m.def("set_cast_mul_in_fp32(bool on) -> ()", set_cast_mul_in_fp32);
   m.def("launch_count() -> int", launch_count);
@@ -1790,10 +1977,16 @@ TORCH_LIBRARY_IMPL(b200q, CUDA, m) {
   m.impl("paged_plan", paged_plan);
   m.impl("qk_norm_rope_append", qk_norm_rope_append);
   m.impl("paged_attention", paged_attention);
+  m.impl("add_rms_norm_cast", add_rms_norm_cast);
+  m.impl("lora_add_", lora_add_);
+  m.impl("moe_layer", moe_layer);
 }
 
 TORCH_LIBRARY_IMPL(b200q, Meta, m) {
   m.impl("paged_plan", meta_paged_plan);
   m.impl("qk_norm_rope_append", meta_qk_norm_rope_append);
   m.impl("paged_attention", meta_paged_attention);
+  m.impl("add_rms_norm_cast", meta_add_rms_norm_cast);
+  m.impl("lora_add_", meta_lora_add_);
+  m.impl("moe_layer", meta_moe_layer);
 }

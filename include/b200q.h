@@ -608,6 +608,123 @@ int b200q_paged_attention(const b200q_paged_attention_args* args);
  * does not fault.  A run that is not so long: nothing is left out. */
 int b200q_selftest_paged_wait_timeout(const b200q_paged_attention_args* args, int cta, int warp, int step);
 
+/*
+ * What stands around the FP8 products of a decoder layer: the norm in front of them, adapters beside them, experts in their
+ * place.  The reference has no counterpart: its callers compose each from separate nodes.  Addresses that are no multiple of their elements' size
+ * are B200Q_ERR_UNSUPPORTED.
+ *
+ * add_rms_norm_cast: the step between two products, in one pass.  Per token
+ *   z = T(residual + x) (stored to residual; the sum is formed in fp32 and rounded once), or x where residual is NULL
+ *   y = z * rsqrt(mean(z^2) + eps) * weight                           in fp32
+ *   kept = bf16(y)                                                    where kept is not NULL
+ *   out  = U(y * scale)                                               scale one fp32 on the device, or NULL: 1
+ *   or, where scale_inv is not NULL (fp8 outputs; scale must be NULL):
+ *   scale_inv = max|y| / max(U),  out = U(y * (max(U) / max|y|));     a token of zeros gets scale_inv 1 and zeros
+ * fp8: to nearest even, saturating; NaN -> 0x7F.  A NaN anywhere in y makes the token's scale_inv NaN, and its fp8 values with it.
+ * A quotient max(U) / max|y| that passes the end of fp32 (all of y below 1e-36) is cut to it.
+ *
+ * x             F32 / BF16 [tokens][dim], row stride in elements, values contiguous
+ * residual      type and shape of x, row stride >= dim, or NULL.  No byte may belong to an input as well
+ * weight        F32 / BF16 [dim], or NULL: 1
+ * out           BF16 / E4M3 / E5M2 [tokens][dim] contiguous;  kept: bf16 alike, or NULL;  scale_inv: fp32 [tokens], or NULL
+ * Rows on boundaries of eight values run in 16-byte accesses; others element by element.
+ */
+typedef struct b200q_norm_args {
+  const void* x;
+  int x_dtype;
+  int64_t tokens, dim, x_stride;
+  void* residual;
+  int64_t residual_stride;
+  const void* weight;
+  int weight_dtype;
+  float eps;
+  void* out;
+  int out_dtype;
+  const float* scale;
+  float* scale_inv;
+  void* kept;
+  void* stream;
+} b200q_norm_args;
+
+int b200q_add_rms_norm_cast(const b200q_norm_args* args);
+
+/*
+ * lora_add: low-rank adapters of many requests beside a product that they share.  Per token t with i = adapter[t] in [0, adapters)
+ *   y[t] = T(y[t] + scales[i] * b[i] (a[i] x[t]))
+ * and nothing for the others, whose rows of y are neither read nor written.  a x is summed in fp32 and meets b as three bf16 terms (24 bits) where y
+ * is fp32 and as two (16 bits) where it is bf16; that product is summed in fp32, and rounded once with y.
+ *
+ * x             bf16 [tokens][k];  y: F32 / BF16 [tokens][n], row stride >= n; row strides in elements, values contiguous
+ * a             bf16 [adapters][rank][k];  b: bf16 [adapters][n][rank]; strides of adapter and row in elements, values contiguous
+ * adapter       int32 [tokens];  scales: fp32 [adapters], or NULL: 1
+ * rank <= 256, adapters <= 2048
+ * workspace     b200q_lora_workspace_bytes(...) bytes, 16-byte aligned, not shared by calls that may overlap
+ * A rank of a multiple of 8, k and n of multiples of 8 and rows on 16-byte boundaries run tensor-core kernels, anything else (or
+ * force_plain = 1) a plain one.  y must not overlap the inputs.  The same call gives the same bytes.
+ */
+typedef struct b200q_lora_args {
+  const void* x;
+  int64_t x_stride;
+  void* y;
+  int y_dtype;
+  int64_t y_stride;
+  const void *a, *b;
+  int64_t a_stride, a_row_stride, b_stride, b_row_stride;
+  const int32_t* adapter;
+  const float* scales;
+  int64_t tokens, k, n, rank, adapters;
+  void* workspace;
+  size_t workspace_bytes;
+  int force_plain;
+  void* stream;
+} b200q_lora_args;
+
+size_t b200q_lora_workspace_bytes(int64_t tokens, int64_t k, int64_t n, int64_t rank, int64_t adapters);
+int b200q_lora_add(const b200q_lora_args* args);
+
+/*
+ * moe_layer: a whole mixture-of-experts layer (router, choice, gated experts, sum) for a few tokens.  Per token x
+ *   logits = router x, summed in fp64;  ids = the top_k largest in descending order, the lower index first among equals (NaN above all)
+ *   weights = softmax(logits)[ids], over all experts, or over the chosen ones (renormalize != 0)
+ *   h_j = silu(g) * u with [g; u] = gate_up_scale * (gate_up[ids_j] x),   out = T(sum_j weights_j * down_scale * (down[ids_j] h_j))
+ * in fp32 with one rounding to T.  Before its product an 8-bit weight meets x as two e4m3 terms (exact down to 2^-22 of the token's largest value)
+ * and h as three (12 bits, down to 2^-26 of the largest of the token and expert); a bf16 weight meets x as it is and h as two bf16 terms (16 bits).
+ * Tokens from *num_tokens on (NULL: none) are not routed: out and weights 0, ids -1, and no expert is read for them.
+ *
+ * x             bf16 [tokens][hidden], row stride in elements;  router: F32 / BF16 [experts][hidden]
+ * gate_up       E4M3 / BF16 [experts][2 inner][hidden], the gate's rows first;  down: the same type, [experts][hidden][inner]
+ * gate_up_scale fp32 [experts][2 inner], down_scale fp32 [experts][hidden], or NULL: 1
+ * out           BF16 / F32 [tokens][hidden];  weights fp32, ids int32 [tokens][top_k];  all but x contiguous
+ * experts <= 512, top_k <= min(16, experts)
+ * workspace     b200q_moe_workspace_bytes(...) bytes, 16-byte aligned, not shared by calls that may overlap
+ * hidden and inner of multiples of 16 bytes with 16-byte aligned weights run the tensor-core kernel, anything else (or force_plain = 1) plain ones.
+ * Weights of the chosen experts are read once for up to 32 tokens each, and batches of more than 256 tokens are taken 256 at a time: for a few tokens.
+ * The same call gives the same bytes.
+ */
+typedef struct b200q_moe_args {
+  const void* x;
+  int64_t x_stride;
+  int64_t tokens, hidden, inner;
+  int experts, top_k, renormalize;
+  const void* router;
+  int router_dtype;
+  const void *gate_up, *down;
+  int weight_dtype;
+  const float *gate_up_scale, *down_scale;
+  const int32_t* num_tokens;
+  void* out;
+  int out_dtype;
+  float* weights;
+  int32_t* ids;
+  void* workspace;
+  size_t workspace_bytes;
+  int force_plain;
+  void* stream;
+} b200q_moe_args;
+
+size_t b200q_moe_workspace_bytes(int64_t tokens, int64_t hidden, int64_t inner, int experts, int top_k);
+int b200q_moe_layer(const b200q_moe_args* args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -689,3 +689,65 @@ def paged_attention(q, k_cache, v_cache, block_table, kv_lens, softmax_scale, k_
             out[b, rows], size[b, rows] = p @ v[:, g], p @ v[:, g].abs()
             lse[b, rows] = torch.logsumexp(s, -1)
     return out, lse, size
+
+
+# ----------------------------------------------------------------------------- around the FP8 products of a decoder layer
+def add_rms_norm(x, residual, weight, eps):
+    """(z as it is stored, y) of the norm of x, or of the residual stream with x added to it: y in fp64, not yet scaled or rounded."""
+    z = x if residual is None else (residual.float() + x.float()).to(x.dtype)
+    d = z.double()
+    y = d / (d.square().mean(-1, keepdim=True) + eps).sqrt()
+    return z, y if weight is None else y * weight.double()
+
+
+def lora_add(y, x, a, b, adapter, scales):
+    """(y + scale b (a x), scale |b| (|a| |x|), rows with an adapter) in fp64.  The second bounds what relative errors of the products and of their
+    sums can do."""
+    want, size = y.double().clone(), torch.zeros(y.shape, dtype=torch.float64)
+    live = (adapter >= 0) & (adapter < a.shape[0])
+    for t in live.nonzero()[:, 0].tolist():
+        i = int(adapter[t])
+        s = 1.0 if scales is None else float(scales[i])
+        u, v, row = a[i].double(), b[i].double(), x[t].double()
+        want[t] += s * (v @ (u @ row))
+        size[t] = abs(s) * (v.abs() @ (u.abs() @ row.abs()))
+    return want, size, live
+
+
+def moe_route(x, router, top_k, renormalize, count=None):
+    """(weights in fp64, ids); tokens from `count` on have weights 0 and ids -1.  A NaN comes before everything, the lower index before its equals."""
+    logits = x.double() @ router.double().T
+    key = torch.where(logits.isnan(), math.inf, logits)
+    order = torch.sort(logits.isnan().double(), dim=-1, descending=True, stable=True).indices
+    order = order.gather(-1, torch.sort(key.gather(-1, order), dim=-1, descending=True, stable=True).indices)
+    ids = order[:, :top_k]
+    top = logits.gather(-1, ids)
+    weights = torch.softmax(top, -1) if renormalize else torch.softmax(logits, -1).gather(-1, ids)
+    live = torch.arange(x.shape[0]) < (x.shape[0] if count is None else count)
+    return torch.where(live[:, None], weights, 0.0), torch.where(live[:, None], ids, -1).to(torch.int32)
+
+
+def moe_experts(x, weights, ids, gate_up, down, gate_up_scale=None, down_scale=None, rel_sum=0.0, rel_hidden=0.0, abs_hidden=0.0):
+    """(out, bound) in fp64.  bound: how far out may be off when sums are off by rel_sum of the sum of their terms' absolute values, and h by rel_hidden
+    of itself and abs_hidden of its token's and expert's largest value, before the last rounding."""
+    inner = down.shape[2]
+    out, bound = (torch.zeros(x.shape[0], down.shape[1], dtype=torch.float64) for _ in range(2))
+    for t in range(x.shape[0]):
+        row = x[t].double()
+        for w, e in zip(weights[t].tolist(), ids[t].tolist()):
+            if e < 0:
+                continue
+            first, second = gate_up[e].double(), down[e].double()
+            if gate_up_scale is not None:
+                first = first * gate_up_scale[e].double()[:, None]
+            if down_scale is not None:
+                second = second * down_scale[e].double()[:, None]
+            gu, off = first @ row, rel_sum * (first.abs() @ row.abs())
+            g, u, dg, du = gu[:inner], gu[inner:], off[:inner], off[inner:]
+            s = g * torch.sigmoid(g)
+            h = s * u
+            dh = 1.1 * dg * (u.abs() + du) + (s.abs() + 2.0 ** -21 * s.abs()) * du + (2.0 ** -21 + rel_hidden) * h.abs()  # (|silu'| <= 1.1)
+            dh = dh + abs_hidden * (h.abs().max() if inner else 0.0)
+            out[t] += w * (second @ h)
+            bound[t] += abs(w) * (second.abs() @ dh + (rel_sum + 2.0 ** -20) * (second.abs() @ h.abs()))
+    return out, bound
