@@ -3,6 +3,7 @@
 #include <float.h>
 
 #include "layer.cuh"
+#include "tcgen05_ptx.cuh"
 
 namespace b200q {
 
@@ -90,6 +91,50 @@ __device__ __forceinline__ float norm_weight(const b200q_norm_args& a, int64_t a
   return a.weight_dtype == B200Q_BF16 ? norm_get(static_cast<const __nv_bfloat16*>(a.weight) + at) : static_cast<const float*>(a.weight)[at];
 }
 
+// How a row lies: on boundaries of eight values (16-byte accesses); on any boundary, but the same in x, residual and the outputs (rows of an
+// odd length one behind the other: 16-byte accesses between the row's ends); or in any other way (value by value).
+enum NormForm { kNormEven, kNormShifted, kNormLoose };
+
+// the weights of the eight values from `at` on, of a row that begins `shift` values behind such a boundary; 0 outside the row
+template <int FORM, int THREADS>
+__device__ __forceinline__ void norm_weights(const b200q_norm_args& a, int at, int v, int tid, int dim, float (&w)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = a.weight ? 0.f : 1.f;
+  if (!a.weight) return;
+  if (FORM == kNormEven) {
+    if (at >= dim) return;
+    if (a.weight_dtype == B200Q_BF16) norm_load8(static_cast<const __nv_bfloat16*>(a.weight) + at, w);
+    else norm_load8(static_cast<const float*>(a.weight) + at, w);
+  } else {
+    if (FORM == kNormShifted && at >= dim) return;
+    const int off = -at & 7;  // of the eight, so many lie before the next boundary; the same for all vectors of a row
+    if (FORM == kNormShifted && a.weight_dtype == B200Q_BF16 && off != 0 && at >= 0 && at + off + 8 <= dim) {
+      // sixteen values on boundaries, moved by 8 - off places: value by value the weights would be half of a row's instructions
+      const uint4* p = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.weight) + (at + off - 8));
+      const uint4 lo = p[0], hi = p[1];
+      uint32_t u[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+      const int by = 8 - off;
+#pragma unroll
+      for (int i = 0; i < 6; ++i) u[i] = by & 4 ? u[i + 2] : u[i];
+#pragma unroll
+      for (int i = 0; i < 5; ++i) u[i] = by & 2 ? u[i + 1] : u[i];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) u[i] = by & 1 ? __funnelshift_r(u[i], u[i + 1], 16) : u[i];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        w[2 * i] = __uint_as_float(u[i] << 16);
+        w[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int k = FORM == kNormShifted ? at + i : (v * 8 + i) * THREADS + tid;
+      if (k >= 0 && k < dim) w[i] = norm_weight(a, k);
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------- rows of any length
 // Three passes by one block; the second and third find the row in L2 (z lies in residual where there is one).
 constexpr int kNormLongThreads = 1024;
@@ -129,13 +174,421 @@ __global__ void __launch_bounds__(kNormLongThreads) norm_long_kernel(const b200q
   }
 }
 
-int add_rms_norm_cast_impl(const b200q_norm_args& a, cudaStream_t st) {
-  const float inv_dim = a.dim ? 1.f / (float)a.dim : 0.f;
-  const unsigned grid = (unsigned)(a.tokens < 2 * kNumSMs ? a.tokens : 2 * kNumSMs);
-  if (a.x_dtype == B200Q_BF16) launch_dependent(norm_long_kernel<__nv_bfloat16>, dim3(grid), dim3(kNormLongThreads), 0, st, a, inv_dim);
-  else launch_dependent(norm_long_kernel<float>, dim3(grid), dim3(kNormLongThreads), 0, st, a, inv_dim);
+// ---------------------------------------------------------------------------- rows that fit the registers
+// A row belongs to THREADS threads (a warp, or a whole block), which hold it in registers: VECS times eight values each, in 16-byte accesses
+// (WIDE), or 8 VECS times one value where rows do not lie on such boundaries.  Everything is loaded before anything is used.
+template <typename T>
+struct NormRaw8;
+template <>
+struct NormRaw8<__nv_bfloat16> {
+  uint4 w;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { w = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(u[i] << 16);
+      v[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+    }
+  }
+};
+template <>
+struct NormRaw8<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p) {
+    a = reinterpret_cast<const float4*>(p)[0];
+    b = reinterpret_cast<const float4*>(p)[1];
+  }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  }
+};
+
+template <typename T, int FORM, int THREADS, int VECS>
+__global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS) norm_row_kernel(const b200q_norm_args a, float inv_dim) {
+  constexpr int kBlock = THREADS < 128 ? 128 : THREADS, kRows = kBlock / THREADS, kWarps = THREADS / 32;
+  __shared__ NormSums s_warp[2][kWarps];  // (the other half is written for the next row, and this one only behind its barrier)
+  pdl_enter();
+  const int tid = threadIdx.x % THREADS, dim = (int)a.dim;
+  const float given = a.scale ? *a.scale : 1.f;
+  const int64_t step = (int64_t)gridDim.x * kRows;
+  // a thread's vector v of row t: values at .. at + 7, of which (kNormShifted) some may lie outside the row
+  auto shift_of = [&](int64_t t) { return FORM == kNormShifted ? (int)((t * dim) & 7) : 0; };
+  auto begin = [&](int v, int shift) { return (v * THREADS + tid) * 8 - shift; };
+  auto inside = [&](int at) { return at >= 0 && at + 8 <= dim; };
+  NormRaw8<T> rx[VECS], rr[VECS];  // of the row that is next: on its way while the one before is reduced
+  auto load = [&](int64_t t) {
+    const T* x = static_cast<const T*>(a.x) + t * a.x_stride;
+    const T* residual = static_cast<const T*>(a.residual) + t * a.residual_stride;
+    const int shift = shift_of(t);
+#pragma unroll
+    for (int v = 0; v < VECS; ++v) {
+      const int at = begin(v, shift);
+      if (inside(at)) {
+        rx[v].load(x + at);
+        if (a.residual) rr[v].load(residual + at);
+      }
+    }
+  };
+  int64_t t = (int64_t)blockIdx.x * kRows + threadIdx.x / THREADS;
+  if (FORM != kNormLoose && t < a.tokens) load(t);
+  for (int turn = 0; t < a.tokens; t += step, turn ^= 1) {
+    const T* x = static_cast<const T*>(a.x) + t * a.x_stride;
+    T* residual = a.residual ? static_cast<T*>(a.residual) + t * a.residual_stride : nullptr;
+    const int shift = shift_of(t);
+    float z[VECS][8];
+    NormSums s = {0.f, 0u};
+    if (FORM != kNormLoose) {
+#pragma unroll
+      for (int v = 0; v < VECS; ++v) {
+        const int at = begin(v, shift);
+        if (inside(at)) {
+          rx[v].get(z[v]);
+          if (residual) {
+            float r[8];
+            rr[v].get(r);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) z[v][i] = norm_rounded(r[i] + z[v][i], x);
+            norm_store8(residual + at, z[v]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            z[v][i] = 0.f;
+            if (FORM == kNormShifted && at + i >= 0 && at + i < dim) {  // (an end of the row)
+              z[v][i] = norm_get(x + at + i);
+              if (residual) {
+                z[v][i] = norm_rounded(norm_get(residual + at + i) + z[v][i], x);
+                residual[at + i] = T(z[v][i]);
+              }
+            }
+          }
+        }
+      }
+      if (t + step < a.tokens) load(t + step);
+    } else {
+#pragma unroll
+      for (int v = 0; v < VECS; ++v)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int at = (v * 8 + i) * THREADS + tid;
+          z[v][i] = at < dim ? norm_get(x + at) : 0.f;
+        }
+      if (residual) {
+#pragma unroll
+        for (int v = 0; v < VECS; ++v) {
+          float r[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int at = (v * 8 + i) * THREADS + tid;
+            r[i] = at < dim ? norm_get(residual + at) : 0.f;
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int at = (v * 8 + i) * THREADS + tid;
+            z[v][i] = norm_rounded(r[i] + z[v][i], x);
+            if (at < dim) residual[at] = T(z[v][i]);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < VECS; ++v) {
+      float w[8];
+      norm_weights<FORM, THREADS>(a, begin(v, shift), v, tid, dim, w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        s.squares += z[v][i] * z[v][i];
+        z[v][i] *= w[i];
+        s.top = max(s.top, __float_as_uint(z[v][i]) & 0x7FFFFFFFu);
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s = norm_join(s, {__shfl_xor_sync(0xFFFFFFFFu, s.squares, o), __shfl_xor_sync(0xFFFFFFFFu, s.top, o)});
+    if (kWarps > 1) {
+      if ((tid & 31) == 0) s_warp[turn][tid >> 5] = s;
+      __syncthreads();
+      s = s_warp[turn][tid & (kWarps - 1)];
+#pragma unroll
+      for (int o = kWarps / 2; o > 0; o >>= 1) s = norm_join(s, {__shfl_xor_sync(0xFFFFFFFFu, s.squares, o), __shfl_xor_sync(0xFFFFFFFFu, s.top, o)});
+    }
+    const NormFactors f = norm_factors(a, s, inv_dim, given);
+    if (a.scale_inv && tid == 0) a.scale_inv[t] = f.inverse;
+#pragma unroll
+    for (int v = 0; v < VECS; ++v) {
+      const int at = begin(v, shift);
+      if (FORM != kNormLoose && inside(at)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[v][i] *= f.norm;
+        if (a.kept) norm_store8(static_cast<__nv_bfloat16*>(a.kept) + t * dim + at, z[v]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[v][i] *= f.scale;
+        norm_out8(a, t * dim + at, z[v]);
+      } else if (FORM != kNormEven) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int k = FORM == kNormShifted ? at + i : (v * 8 + i) * THREADS + tid;
+          if (k < 0 || k >= dim) continue;
+          const float y = z[v][i] * f.norm;
+          if (a.kept) static_cast<__nv_bfloat16*>(a.kept)[t * dim + k] = __float2bfloat16_rn(y);
+          norm_out1(a, t * dim + k, y * f.scale);
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int FORM, int THREADS, int VECS>
+static int norm_launch(const b200q_norm_args& a, float inv_dim, cudaStream_t st) {
+  auto kernel = norm_row_kernel<T, FORM, THREADS, VECS>;
+  constexpr int kBlock = THREADS < 128 ? 128 : THREADS, kRows = kBlock / THREADS;
+  static std::atomic<int> resident[kMaxDevices];  // blocks per SM
+  const int dev = current_device_index();
+  if (dev < 0) return B200Q_ERR_CUDA;
+  int per_sm = resident[dev].load(std::memory_order_acquire);
+  if (!per_sm) {
+    B200Q_CUDA_OK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kBlock, 0));
+    if (per_sm < 1) per_sm = 1;
+    resident[dev].store(per_sm, std::memory_order_release);
+  }
+  const int64_t blocks = (a.tokens + kRows - 1) / kRows, most = (int64_t)per_sm * kNumSMs;
+  launch_dependent(kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(kBlock), 0, st, a, inv_dim);
   B200Q_LAUNCH_CHECK();
   return B200Q_OK;
+}
+
+// ---------------------------------------------------------------------------- many long rows
+// The same with the rows on their way to shared memory, as bulk copies: what is in flight then costs no registers, and a block that
+// waits for its sums has its next rows coming.  A row that begins between boundaries (kNormShifted) is fetched from the boundary before it to the one
+// behind it; what that brings of its neighbours is masked out, and behind the last row nothing is fetched: its end is read value by value.
+constexpr int kNormErrCopy = 811;  // status code: a copy of a row did not arrive
+constexpr int kNormRingBytes = 216 * 1024;  // of an SM
+
+__device__ __forceinline__ void norm_bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+template <typename T>
+__host__ __device__ constexpr int64_t norm_slot_row(int64_t dim, int form) {  // bytes of a row's place
+  return (dim + (form == kNormShifted ? 7 : 0) + 7) / 8 * 8 * (int64_t)sizeof(T);  // (all vectors that begin in the row end in its place)
+}
+
+template <typename T, int FORM, int THREADS, int VECS, int BLOCKS>
+__global__ void __launch_bounds__(THREADS, BLOCKS) norm_ring_kernel(const b200q_norm_args a, float inv_dim, int depth, int* status) {
+  constexpr int kWarps = THREADS / 32, kMostDepth = 8;
+  extern __shared__ __align__(128) uint8_t s_ring[];  // [depth] rows of x, with that of residual behind it
+  __shared__ __align__(8) uint64_t s_bars[kMostDepth];
+  __shared__ NormSums s_warp[2][kWarps];
+  __shared__ int s_abort;
+  const int tid = threadIdx.x, dim = (int)a.dim;
+  constexpr bool kShifted = FORM == kNormShifted;
+  const uint32_t bars = ptx::smem_u32(s_bars), ring = ptx::smem_u32(s_ring);
+  const uint32_t row = (uint32_t)norm_slot_row<T>(dim, FORM), slot_bytes = a.residual ? 2 * row : row;
+  auto shift_of = [&](int64_t t) { return kShifted ? (int)((t * dim) & 7) : 0; };
+  auto bytes_of = [&](int64_t t) {  // of a row that are fetched
+    const uint32_t n = (uint32_t)((shift_of(t) + dim) * sizeof(T));
+    return !kShifted || t + 1 < a.tokens ? (n + 15u) & ~15u : n & ~15u;
+  };
+  if (tid == 0) {
+    for (int i = 0; i < depth; ++i) ptx::mbar_init(bars + 8 * i, 1);
+    s_abort = 0;
+    ptx::fence_barrier_init();
+  }
+  __syncthreads();
+  pdl_enter();
+  const float given = a.scale ? *a.scale : 1.f;
+  auto copy = [&](int64_t t, int slot) {  // (one thread)
+    const uint32_t bytes = bytes_of(t);
+    const int64_t back = shift_of(t);
+    ptx::mbar_arrive_expect_tx(bars + 8 * slot, a.residual ? 2 * bytes : bytes);
+    norm_bulk_copy(ring + slot * slot_bytes, static_cast<const T*>(a.x) + (t * a.x_stride - back), bytes, bars + 8 * slot);
+    if (a.residual)
+      norm_bulk_copy(ring + slot * slot_bytes + row, static_cast<const T*>(a.residual) + (t * a.residual_stride - back), bytes, bars + 8 * slot);
+  };
+  if (tid == 0)
+    for (int i = 0; i < depth && (int64_t)blockIdx.x + (int64_t)i * gridDim.x < a.tokens; ++i) copy((int64_t)blockIdx.x + (int64_t)i * gridDim.x, i);
+  int slot = 0, turn = 0;
+  uint32_t phase = 0;
+  for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x, turn ^= 1) {
+    const bool here = ptx::mbar_wait(bars + 8 * slot, phase, &s_abort, status, kNormErrCopy);
+    const T* x = reinterpret_cast<const T*>(s_ring + slot * slot_bytes);
+    T* residual = static_cast<T*>(a.residual) + t * a.residual_stride;
+    const int shift = shift_of(t);
+    auto begin = [&](int v) { return (v * THREADS + tid) * 8 - shift; };
+    auto inside = [&](int at) { return at >= 0 && at + 8 <= dim; };
+    // values at .. at + 7 of the row in shared memory at p, which lies at `from` in global memory
+    auto get = [&](const T* p, const T* from, int at, float (&v)[8]) {
+      norm_load8(p + at + shift, v);
+      if (kShifted && !inside(at)) {
+        const int there = (int)(bytes_of(t) / sizeof(T)) - shift;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = at + i < 0 || at + i >= dim ? 0.f : at + i < there ? v[i] : norm_get(from + at + i);
+      }
+    };
+    float z[VECS][8];
+    NormSums s = {0.f, 0u};
+#pragma unroll
+    for (int v = 0; v < VECS; ++v) {
+      const int at = begin(v);
+      if (here && at < dim) {
+        get(x, static_cast<const T*>(a.x) + t * a.x_stride, at, z[v]);
+        if (a.residual) {
+          float r[8];
+          get(x + row / sizeof(T), residual, at, r);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) z[v][i] = norm_rounded(r[i] + z[v][i], x);
+          if (inside(at)) {
+            norm_store8(residual + at, z[v]);
+          } else if (kShifted) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (at + i >= 0 && at + i < dim) residual[at + i] = T(z[v][i]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[v][i] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < VECS; ++v) {
+      float w[8];
+      norm_weights<FORM, THREADS>(a, begin(v), v, tid, dim, w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        s.squares += z[v][i] * z[v][i];
+        z[v][i] *= w[i];
+        s.top = max(s.top, __float_as_uint(z[v][i]) & 0x7FFFFFFFu);
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s = norm_join(s, {__shfl_xor_sync(0xFFFFFFFFu, s.squares, o), __shfl_xor_sync(0xFFFFFFFFu, s.top, o)});
+    if ((tid & 31) == 0) s_warp[turn][tid >> 5] = s;
+    __syncthreads();  // (and the slot has been read by all)
+    if (s_abort) {  // a copy is missing: nothing more is written, and the copies in flight are waited for, as far as they come
+      if (tid == 0)
+        for (int i = 0; i < depth && t + (int64_t)i * gridDim.x < a.tokens; ++i) {
+          const int at = slot + i < depth ? slot + i : slot + i - depth;
+          for (int k = 0; k < 4096 && !ptx::mbar_try_wait(bars + 8 * at, slot + i < depth ? phase : phase ^ 1); ++k) __nanosleep(64);
+        }
+      break;
+    }
+    if (tid == 0 && t + (int64_t)depth * gridDim.x < a.tokens) copy(t + (int64_t)depth * gridDim.x, slot);
+    s = s_warp[turn][tid & (kWarps - 1)];
+#pragma unroll
+    for (int o = kWarps / 2; o > 0; o >>= 1) s = norm_join(s, {__shfl_xor_sync(0xFFFFFFFFu, s.squares, o), __shfl_xor_sync(0xFFFFFFFFu, s.top, o)});
+    const NormFactors f = norm_factors(a, s, inv_dim, given);
+    if (a.scale_inv && tid == 0) a.scale_inv[t] = f.inverse;
+#pragma unroll
+    for (int v = 0; v < VECS; ++v) {
+      const int at = begin(v);
+      if (at >= dim) continue;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) z[v][i] *= f.norm;
+      if (inside(at)) {
+        if (a.kept) norm_store8(static_cast<__nv_bfloat16*>(a.kept) + t * dim + at, z[v]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[v][i] *= f.scale;
+        norm_out8(a, t * dim + at, z[v]);
+      } else if (kShifted) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (at + i < 0 || at + i >= dim) continue;
+          if (a.kept) static_cast<__nv_bfloat16*>(a.kept)[t * dim + at + i] = __float2bfloat16_rn(z[v][i]);
+          norm_out1(a, t * dim + at + i, z[v][i] * f.scale);
+        }
+      }
+    }
+    if (++slot == depth) {
+      slot = 0;
+      phase ^= 1;
+    }
+  }
+}
+
+template <typename T, int FORM, int THREADS, int VECS, int BLOCKS>
+static int norm_launch_ring(const b200q_norm_args& a, float inv_dim, cudaStream_t st) {
+  auto kernel = norm_ring_kernel<T, FORM, THREADS, VECS, BLOCKS>;
+  constexpr int kMost = kNormRingBytes / BLOCKS / 1024 * 1024;
+  static std::atomic<int> ready[kMaxDevices];
+  const int dev = current_device_index();
+  if (dev < 0) return B200Q_ERR_CUDA;
+  if (!ready[dev].load(std::memory_order_acquire)) {
+    B200Q_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost));
+    ready[dev].store(1, std::memory_order_release);
+  }
+  int* status = device_status_ptr();
+  if (!status) return B200Q_ERR_CUDA;
+  const int64_t bytes = norm_slot_row<T>(a.dim, FORM) * (a.residual ? 2 : 1);
+  const int64_t fits = kMost / bytes;
+  const int depth = fits < 1 ? 0 : fits < 8 ? (int)fits : 8;
+  if (!depth) return B200Q_ERR_UNSUPPORTED;
+  const int64_t most = (int64_t)BLOCKS * kNumSMs;
+  launch_dependent(kernel, dim3((unsigned)(a.tokens < most ? a.tokens : most)), dim3(THREADS), (size_t)(depth * bytes), st, a, inv_dim, depth, status);
+  B200Q_LAUNCH_CHECK();
+  return B200Q_OK;
+}
+
+// Few tokens: as many threads to a row as it has use for.  us for 1 x 8192, 64 x 4096: 3.2, 2.4.
+template <typename T, int FORM>
+static int norm_launch_few(const b200q_norm_args& a, float inv_dim, cudaStream_t st) {
+  const int64_t dim = a.dim + (FORM == kNormShifted ? 7 : 0);
+  if (dim <= 256) return norm_launch<T, FORM, 32, 1>(a, inv_dim, st);
+  if (dim <= 1024) return norm_launch<T, FORM, 128, 1>(a, inv_dim, st);
+  if (dim <= 4096) return norm_launch<T, FORM, 512, 1>(a, inv_dim, st);
+  if (dim <= 8192) return norm_launch<T, FORM, 1024, 1>(a, inv_dim, st);
+  if (dim <= 16384) return norm_launch<T, FORM, 1024, 2>(a, inv_dim, st);
+  return norm_launch<T, FORM, 1024, 4>(a, inv_dim, st);
+}
+template <typename T, int FORM>
+static int norm_launch_many(const b200q_norm_args& a, float inv_dim, cudaStream_t st) {
+  const int64_t dim = a.dim + (FORM == kNormShifted ? 7 : 0);
+  if (dim <= 256) return norm_launch<T, FORM, 32, 1>(a, inv_dim, st);
+  if (dim <= 512) return norm_launch<T, FORM, 32, 2>(a, inv_dim, st);
+  if constexpr (FORM != kNormLoose) {
+    int rc = B200Q_ERR_UNSUPPORTED;
+    if (dim <= 1024) rc = norm_launch_ring<T, FORM, 64, 2, 12>(a, inv_dim, st);
+    else if (dim <= 2048) rc = norm_launch_ring<T, FORM, 128, 2, 6>(a, inv_dim, st);
+    else if (dim <= 2560) rc = norm_launch_ring<T, FORM, 128, 4, 6>(a, inv_dim, st);
+    else if (dim <= 4096) rc = norm_launch_ring<T, FORM, 256, 2, 4>(a, inv_dim, st);
+    else if (dim <= 8192) rc = norm_launch_ring<T, FORM, 512, 2, 2>(a, inv_dim, st);
+    else if (dim <= 16384) rc = norm_launch_ring<T, FORM, 512, 4, 2>(a, inv_dim, st);
+    else rc = norm_launch_ring<T, FORM, 1024, 4, 1>(a, inv_dim, st);
+    if (rc != B200Q_ERR_UNSUPPORTED) return rc;  // (rows too long for shared memory)
+    return norm_launch<T, FORM, 1024, 4>(a, inv_dim, st);
+  }
+  if (dim <= 1024) return norm_launch<T, FORM, 128, 1>(a, inv_dim, st);
+  if (dim <= 4096) return norm_launch<T, FORM, 256, 2>(a, inv_dim, st);
+  if (dim <= 16384) return norm_launch<T, FORM, 512, 4>(a, inv_dim, st);
+  return norm_launch<T, FORM, 1024, 4>(a, inv_dim, st);
+}
+template <typename T, int FORM>
+static int norm_launch_form(const b200q_norm_args& a, float inv_dim, cudaStream_t st) {
+  return a.tokens <= kNumSMs ? norm_launch_few<T, FORM>(a, inv_dim, st) : norm_launch_many<T, FORM>(a, inv_dim, st);
+}
+
+template <typename T>
+static int norm_launch_type(const b200q_norm_args& a, float inv_dim, cudaStream_t st) {
+  if (a.dim > 32768 || (a.dim > 32760 && a.dim % 8)) {
+    const unsigned grid = (unsigned)(a.tokens < 2 * kNumSMs ? a.tokens : 2 * kNumSMs);
+    launch_dependent(norm_long_kernel<T>, dim3(grid), dim3(kNormLongThreads), 0, st, a, inv_dim);
+    B200Q_LAUNCH_CHECK();
+    return B200Q_OK;
+  }
+  bool aligned = true;
+  for (const void* p : {a.x, static_cast<const void*>(a.residual), a.weight, static_cast<const void*>(a.out), static_cast<const void*>(a.kept)})
+    aligned = aligned && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+  const int64_t strides[2] = {a.x_stride, a.residual ? a.residual_stride : a.x_stride};
+  const bool one = a.tokens == 1;  // (no stride is used)
+  if (aligned && a.dim % 8 == 0 && (one || (strides[0] % 8 == 0 && strides[1] % 8 == 0))) return norm_launch_form<T, kNormEven>(a, inv_dim, st);
+  if (aligned && (one || ((strides[0] - a.dim) % 8 == 0 && (strides[1] - a.dim) % 8 == 0))) return norm_launch_form<T, kNormShifted>(a, inv_dim, st);
+  return norm_launch_form<T, kNormLoose>(a, inv_dim, st);
+}
+
+int add_rms_norm_cast_impl(const b200q_norm_args& a, cudaStream_t st) {
+  const float inv_dim = a.dim ? 1.f / (float)a.dim : 0.f;
+  return a.x_dtype == B200Q_BF16 ? norm_launch_type<__nv_bfloat16>(a, inv_dim, st) : norm_launch_type<float>(a, inv_dim, st);
 }
 
 }  // namespace b200q
