@@ -12,7 +12,7 @@ constexpr size_t moe_align(size_t n) { return (n + 255) / 256 * 256; }
 
 // Where the parts of the workspace lie.
 struct MoeSpace {
-  size_t logits, x_top, control, h_top, hidden, outputs, parts, bytes;
+  size_t logits, x_top, control, h_top, hidden, outputs, x_terms, h_terms, parts, bytes;
   int clear_words;  // from control on
   MoeSpace(int64_t tokens, int64_t h, int64_t f, int experts, int top_k);
 };
@@ -32,6 +32,37 @@ __device__ __forceinline__ float moe_silu(float g) { return g / (1.f + expf(-g))
 // ---------------------------------------------------------------------------- router
 // Sums in fp64: neighbours in the order of the experts may be closer than the rounding of a sum in fp32, and another expert is another answer.
 constexpr int kMoeThreads = 256;
+
+// The power of two that brings a largest value (its bits) to [128, 256), and its inverse.
+__device__ __forceinline__ float moe_up_factor(uint32_t top) {
+  const int e = (int)(top >> 23) - 127;
+  const int up = e == 128 ? 0 : max(-126, min(7 - e, 126));
+  return __uint_as_float((uint32_t)(127 + up) << 23);
+}
+__device__ __forceinline__ float moe_down_factor(uint32_t top) {
+  const int e = (int)(top >> 23) - 127;
+  const int up = e == 128 ? 0 : max(-126, min(7 - e, 126));
+  return __uint_as_float((uint32_t)(127 - up) << 23);
+}
+
+// Eight values in TERMS terms of e4m3, each the rounded rest of the one before times 32 (a rest is at most 8 where the largest value is below 256).
+template <int TERMS>
+__device__ __forceinline__ void moe_terms_fp8(float (&v)[8], uint2 (&out)[TERMS]) {
+#pragma unroll
+  for (int t = 0; t < TERMS; ++t) {
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t pair = cvt_fp8x2<B200Q_E4M3>(v[2 * i], v[2 * i + 1]);
+      w[i / 2] |= pair << (16 * (i & 1));
+      if (t + 1 < TERMS) {
+        v[2 * i] = (v[2 * i] - fp8_to_float<B200Q_E4M3>(pair & 0xFFu)) * 32.f;
+        v[2 * i + 1] = (v[2 * i + 1] - fp8_to_float<B200Q_E4M3>(pair >> 8)) * 32.f;
+      }
+    }
+    out[t] = make_uint2(w[0], w[1]);
+  }
+}
 
 template <typename W>
 __device__ __forceinline__ void moe_load8(const W* p, bool wide, int64_t i, int64_t n, float (&v)[8]) {
@@ -55,14 +86,18 @@ __device__ __forceinline__ void moe_load8(const W* p, bool wide, int64_t i, int6
   }
 }
 
-// A warp has EB experts' rows and TB tokens'.  What the fused kernel wants cleared, and the tokens' largest values, come from here too.
+// A block has EB experts' rows and TB tokens', its warps an eighth of the row each: all of a warp's loads of a row of 4096 are then in flight at once.  What the
+// fused kernel wants cleared, and the tokens' largest values, come from here too.
 template <typename W, int EB, int TB>
-__global__ void __launch_bounds__(kMoeThreads) moe_logits_kernel(const b200q_moe_args a, int64_t first, double* logits, uint32_t* x_top, uint32_t* clear, int clear_words, bool wide) {
+__global__ void __launch_bounds__(kMoeThreads) moe_logits_kernel(const b200q_moe_args a, int64_t first, double* logits, uint32_t* x_top, uint8_t* x_terms, uint32_t* clear, int clear_words, bool wide) {
+  constexpr int kWarps = kMoeThreads / 32;
+  __shared__ double s_sum[kWarps][EB * TB];
+  __shared__ uint32_t s_top[kWarps][TB];
   pdl_enter();
   for (int i = blockIdx.x * kMoeThreads + threadIdx.x; i < clear_words; i += gridDim.x * kMoeThreads) clear[i] = 0;
-  const int lane = threadIdx.x & 31, tokens = moe_tokens(a, first);
-  const int64_t at = (int64_t)blockIdx.x * (kMoeThreads / 32) + (threadIdx.x >> 5), expert_blocks = (a.experts + EB - 1) / EB;
-  const int64_t t0 = at / expert_blocks * TB, e0 = (at % expert_blocks) * EB;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tokens = moe_tokens(a, first);
+  const int64_t expert_blocks = (a.experts + EB - 1) / EB;
+  const int64_t t0 = blockIdx.x / expert_blocks * TB, e0 = (blockIdx.x % expert_blocks) * EB;
   if (t0 >= tokens) return;
   const W* router[EB];
   const __nv_bfloat16* x[TB];
@@ -70,9 +105,10 @@ __global__ void __launch_bounds__(kMoeThreads) moe_logits_kernel(const b200q_moe
   for (int e = 0; e < EB; ++e) router[e] = static_cast<const W*>(a.router) + min(e0 + e, (int64_t)a.experts - 1) * a.hidden;
 #pragma unroll
   for (int t = 0; t < TB; ++t) x[t] = static_cast<const __nv_bfloat16*>(a.x) + min(t0 + t, (int64_t)tokens - 1) * a.x_stride;
-  double sum[EB][TB] = {};
+  double sum[EB * TB] = {};
   uint32_t top[TB] = {};
-  for (int64_t i = 8 * lane; i < a.hidden; i += 256) {
+#pragma unroll 2
+  for (int64_t i = 8 * threadIdx.x; i < a.hidden; i += 8 * kMoeThreads) {
     float xv[TB][8], wv[EB][8];
 #pragma unroll
     for (int t = 0; t < TB; ++t) moe_load8(x[t], wide, i, a.hidden, xv[t]);
@@ -90,88 +126,130 @@ __global__ void __launch_bounds__(kMoeThreads) moe_logits_kernel(const b200q_moe
       for (int e = 0; e < EB; ++e) {
         const double wd = (double)wv[e][c];
 #pragma unroll
-        for (int t = 0; t < TB; ++t) sum[e][t] += wd * xd[t];
+        for (int t = 0; t < TB; ++t) sum[e * TB + t] += wd * xd[t];
       }
     }
   }
 #pragma unroll
+  for (int i = 0; i < EB * TB; ++i) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum[i] += __shfl_xor_sync(0xFFFFFFFFu, sum[i], o);
+    if (lane == 0) s_sum[warp][i] = sum[i];
+  }
+#pragma unroll
   for (int t = 0; t < TB; ++t) {
+    top[t] = __reduce_max_sync(0xFFFFFFFFu, top[t]);
+    if (lane == 0) s_top[warp][t] = top[t];
+  }
+  __syncthreads();
+  if (threadIdx.x < EB * TB) {
+    const int e = threadIdx.x / TB, t = threadIdx.x % TB;
+    double all = 0.0;
 #pragma unroll
-    for (int e = 0; e < EB; ++e) {
+    for (int i = 0; i < kWarps; ++i) all += s_sum[i][threadIdx.x];
+    if (t0 + t < tokens && e0 + e < a.experts) logits[(t0 + t) * a.experts + e0 + e] = all;
+    if (e0 == 0 && e == 0 && t0 + t < tokens) {
+      uint32_t most = 0;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum[e][t] += __shfl_xor_sync(0xFFFFFFFFu, sum[e][t], o);
-      if (lane == 0 && t0 + t < tokens && e0 + e < a.experts) logits[(t0 + t) * a.experts + e0 + e] = sum[e][t];
+      for (int i = 0; i < kWarps; ++i) most = max(most, s_top[i][t]);
+      x_top[t0 + t] = most;
     }
-    if (e0 == 0 && t0 + t < tokens) {
-      top[t] = __reduce_max_sync(0xFFFFFFFFu, top[t]);
-      if (lane == 0) x_top[t0 + t] = top[t];
+  }
+  if (!x_terms || e0 != 0) return;
+  // the tokens' two terms for 8-bit weights
+#pragma unroll 1
+  for (int t = 0; t < TB && t0 + t < tokens; ++t) {
+    uint32_t most = 0;
+    for (int i = 0; i < kWarps; ++i) most = max(most, s_top[i][t]);
+    const float factor = moe_up_factor(most);
+    const __nv_bfloat16* row = static_cast<const __nv_bfloat16*>(a.x) + (t0 + t) * a.x_stride;
+    for (int64_t i = 8 * threadIdx.x; i < a.hidden; i += 8 * kMoeThreads) {
+      float v[8];
+      moe_load8(row, true, i, a.hidden, v);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) v[c] *= factor;
+      uint2 term[2];
+      moe_terms_fp8<2>(v, term);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) *reinterpret_cast<uint2*>(x_terms + (c * a.tokens + t0 + t) * a.hidden + i) = term[c];
     }
   }
 }
 
-// whether (v, i) comes before (w, j) in the order of choice
-__device__ __forceinline__ bool moe_before(double v, int i, double w, int j) {
-  const bool vn = v != v, wn = w != w;
-  if (vn || wn) return vn && wn ? i < j : vn;
-  return v > w || (v == w && i < j);
+// A logit as an integer that is ordered as the choice is: a NaN above all; the two zeros are one.  0 is below every logit.
+__device__ __forceinline__ unsigned long long moe_key(double v) {
+  if (v != v) return ~0ull;
+  const long long b = __double_as_longlong(v + 0.0);  // (-0 + 0 = 0)
+  return (unsigned long long)b ^ (b < 0 ? ~0ull : 1ull << 63);
+}
+__device__ __forceinline__ double moe_value(unsigned long long key) {
+  return key == ~0ull ? __longlong_as_double(~0ll) : __longlong_as_double((long long)(key ^ (key >> 63 ? 1ull << 63 : ~0ull)));
 }
 
-// The choice for one token by one warp: lane j has the j-th expert.  top_k rounds of a maximum over the logits, of which a lane has each 32nd.
+// The choice for one token by one warp: lane j has the j-th expert.  A lane has each 32nd logit and knows the best of those it has left, so that a
+// round is a maximum over the lanes in three steps of 32 bits: upper half of the key, lower half, lowest index.
 struct MoeChoice {
   int id;
   float weight;
 };
-__device__ __forceinline__ MoeChoice moe_choose(const b200q_moe_args& a, const double* logits, bool live, int lane) {
+template <int MINE>
+__device__ __forceinline__ MoeChoice moe_choose_of(const b200q_moe_args& a, const double* logits, int lane) {
   MoeChoice c = {-1, 0.f};
-  if (!live) return c;
-  constexpr int kMine = kMoeMaxExperts / 32;
-  double mine[kMine];
+  double mine[MINE];
 #pragma unroll
-  for (int i = 0; i < kMine; ++i) mine[i] = lane + 32 * i < a.experts ? __ldcg(logits + lane + 32 * i) : 0.0;
-  uint32_t taken = 0;  // bit i: expert lane + 32 i
-  double first = 0.0, value = 0.0;
-  for (int j = 0; j < a.top_k; ++j) {
-    double best = 0.0;
-    int at = -1;
+  for (int i = 0; i < MINE; ++i) mine[i] = lane + 32 * i < a.experts ? __ldcg(logits + lane + 32 * i) : 0.0;
+  unsigned long long key[MINE];  // 0: taken, or behind the last expert
 #pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-      if (32 * i >= a.experts) break;
-      if (lane + 32 * i >= a.experts || (taken >> i & 1u)) continue;
-      if (at < 0 || moe_before(mine[i], lane + 32 * i, best, at)) {
-        best = mine[i];
+  for (int i = 0; i < MINE; ++i) key[i] = lane + 32 * i < a.experts ? moe_key(mine[i]) : 0;
+  unsigned long long best, first = 0, value = 0;
+  int at;
+  auto look = [&] {
+    best = key[0];
+    at = lane;
+#pragma unroll
+    for (int i = 1; i < MINE; ++i)
+      if (key[i] > best) {
+        best = key[i];
         at = lane + 32 * i;
       }
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const double v = __shfl_xor_sync(0xFFFFFFFFu, best, o);
-      const int k = __shfl_xor_sync(0xFFFFFFFFu, at, o);
-      if (k >= 0 && (at < 0 || moe_before(v, k, best, at))) {
-        best = v;
-        at = k;
-      }
-    }
-    if (lane == (at & 31)) taken |= 1u << (at >> 5);
-    if (j == 0) first = best;
+  };
+  look();
+  for (int j = 0; j < a.top_k; ++j) {
+    const uint32_t hi = (uint32_t)(best >> 32), hi_most = __reduce_max_sync(0xFFFFFFFFu, hi);
+    const uint32_t lo = hi == hi_most ? (uint32_t)best : 0u, lo_most = __reduce_max_sync(0xFFFFFFFFu, lo);
+    const int id = (int)__reduce_min_sync(0xFFFFFFFFu, hi == hi_most && (uint32_t)best == lo_most ? (uint32_t)at : 0x7FFFu);
+    const unsigned long long most = (unsigned long long)hi_most << 32 | lo_most;
+    if (j == 0) first = most;
     if (lane == j) {
-      c.id = at;
-      value = best;
+      c.id = id;
+      value = most;
+    }
+    if (id == at) {
+#pragma unroll
+      for (int i = 0; i < MINE; ++i)
+        if (id >> 5 == i) key[i] = 0;
+      look();
     }
   }
   // exponents are differences taken in fp64, and small ones exact enough in fp32
-  const float p = lane < a.top_k ? expf((float)(value - first)) : 0.f;
+  const double top = moe_value(first);
+  const float p = lane < a.top_k ? expf((float)(moe_value(value) - top)) : 0.f;
   float sum = 0.f;
   if (a.renormalize) {
     sum = p;
   } else {
 #pragma unroll
-    for (int i = 0; i < kMine; ++i)
-      if (lane + 32 * i < a.experts) sum += expf((float)(mine[i] - first));
+    for (int i = 0; i < MINE; ++i)
+      if (lane + 32 * i < a.experts) sum += expf((float)(mine[i] - top));
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
   c.weight = p / sum;
   return c;
+}
+__device__ __forceinline__ MoeChoice moe_choose(const b200q_moe_args& a, const double* logits, bool live, int lane) {
+  if (!live) return {-1, 0.f};
+  return a.experts <= 128 ? moe_choose_of<4>(a, logits, lane) : moe_choose_of<kMoeMaxExperts / 32>(a, logits, lane);
 }
 __device__ __forceinline__ void moe_store_choice(const b200q_moe_args& a, int64_t t, int lane, const MoeChoice& c) {
   a.ids[t * a.top_k + lane] = c.id;
@@ -247,21 +325,29 @@ __global__ void __launch_bounds__(kMoeThreads) moe_sum_kernel(const b200q_moe_ar
 // weights then go from global memory to the tensor core as they are, by TMA alone; f16 operands would want every weight converted in
 // registers first.
 //
-// One persistent CTA per SM; the list of (expert, 32 tokens of it at most), weight rows and steps of 128 bytes of a row is cut into equal runs for the
-// CTAs, so that few experts and ragged sizes load every SM alike.  A row tile that several CTAs have a part of is summed by the one that finishes
-// last, in the CTAs' order.  Both products are one stream of weights: while the last tiles of the first product are finished, and all CTAs wait for them, the
-// second one's weights fill the ring.
-//   warp 0: weights, by TMA     warp 1: MMAs     warps 2-5: tokens' terms into shared memory     warps 6-9: results
-constexpr int kMoeWarps = 10;
+// One persistent CTA per SM; the units of the work are (group of an expert's tokens, tile of weight rows), which the CTAs take from a counter: in equal
+// runs of one list the SMs that get at the memory fastest were done after 203 us and the last ones after 272 (29 tokens, 108 experts of 4096 x 1792).  The last
+// tile and a quarter per CTA are cut into parts of a few steps of 128 bytes of a row, so that all end together, and few experts load every SM; a cut
+// tile is summed, in the parts' order, by a CTA that its number gives.  (By the one whose part comes last, a CTA that falls behind gets the sums too.)
+// Both products are one stream of units without a barrier between: the second one of a group waits for the group's first.
+//
+// The terms of x are made by the router's kernel, those of a slot's h when its last tile is finished (its largest value gives their scale), and come by
+// TMA as the weights do, an expert's tokens by gathered rows.  (Made by each CTA for itself, step by step from registers, they paced the kernel.)
+//   warp 0: weights     warp 1: MMAs     warp 2: terms     warp 3: tells of the parts of cut tiles     warps 4-7: sums, terms of h     warps 8-11: results
+constexpr int kMoeWarps = 12;
 constexpr int kMoeErrWeights = 821, kMoeErrTokens = 822, kMoeErrMma = 823, kMoeErrResults = 824, kMoeErrGrid = 825;  // status codes: a wait ran out
 constexpr int kMoeGroupTokens = 32;     // of an expert, at a time
 constexpr int kMoeSubBytes = 128 * 128;  // a weight tile: 128 rows of 128 bytes; a step has two (gate and up, or 256 outputs)
 constexpr int kMoeMostDim = 65536;
 constexpr uint32_t kMoeGridPolls = 1u << 23;
 
+constexpr int kMoeCutTiles = kNumSMs * 5 / 4, kMoeMostParts = 8;
+constexpr int kMoeMostGroups = kMoeMaxExperts + (int)kMoeChunk * kMoeMaxTopK / kMoeGroupTokens;
 struct MoeControl {  // cleared by the router's kernel
-  uint32_t chosen, up_done, down_done, unused;
-  uint32_t joins[2][kNumSMs];  // parts that have arrived, by the CTA that has the first one
+  uint32_t chosen, done, next[2];
+  uint32_t parts[2][kMoeCutTiles];  // of a cut tile that are there
+  uint32_t up[kMoeMostGroups];      // tiles of a group's first product that are finished, four warps each
+  uint32_t terms[kMoeMostGroups];   // slots of a group whose terms are there, four warps each
 };
 
 template <bool FP8, int MAXN>
@@ -281,43 +367,14 @@ struct MoeFused {
   const double* logits;
   const uint32_t* x_top;   // bits of max |x| per token
   uint32_t* h_top;         // bits of max |h| per slot
-  float *hidden, *outputs;  // [slots][inner], [slots][hidden]: slots in the order of experts
-  float* parts;            // [grid][2][kPart]
+  float *hidden, *outputs;  // [slots][inner] (8-bit weights), [slots][hidden]: slots in the order of experts
+  uint8_t* h_terms;        // [terms][slots][inner]
+  int slots;               // of that
+  float* parts;            // [products][cut tiles][parts][kPart]
   MoeControl* control;
   int* status;
   int up_tiles, up_steps, down_tiles, down_steps;
 };
-
-// The power of two that brings a largest value (its bits) to [128, 256), and its inverse.
-__device__ __forceinline__ float moe_up_factor(uint32_t top) {
-  const int e = (int)(top >> 23) - 127;
-  const int up = e == 128 ? 0 : max(-126, min(7 - e, 126));
-  return __uint_as_float((uint32_t)(127 + up) << 23);
-}
-__device__ __forceinline__ float moe_down_factor(uint32_t top) {
-  const int e = (int)(top >> 23) - 127;
-  const int up = e == 128 ? 0 : max(-126, min(7 - e, 126));
-  return __uint_as_float((uint32_t)(127 - up) << 23);
-}
-
-// Eight values in TERMS terms of e4m3, each the rounded rest of the one before times 32 (a rest is at most 8 where the largest value is below 256).
-template <int TERMS>
-__device__ __forceinline__ void moe_terms_fp8(float (&v)[8], uint2 (&out)[TERMS]) {
-#pragma unroll
-  for (int t = 0; t < TERMS; ++t) {
-    uint32_t w[2] = {0, 0};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t pair = cvt_fp8x2<B200Q_E4M3>(v[2 * i], v[2 * i + 1]);
-      w[i / 2] |= pair << (16 * (i & 1));
-      if (t + 1 < TERMS) {
-        v[2 * i] = (v[2 * i] - fp8_to_float<B200Q_E4M3>(pair & 0xFFu)) * 32.f;
-        v[2 * i + 1] = (v[2 * i + 1] - fp8_to_float<B200Q_E4M3>(pair >> 8)) * 32.f;
-      }
-    }
-    out[t] = make_uint2(w[0], w[1]);
-  }
-}
 
 __device__ __forceinline__ uint32_t moe_ld_acquire(const uint32_t* p) {
   uint32_t v;
@@ -336,6 +393,30 @@ __device__ __forceinline__ bool moe_grid_wait(const uint32_t* p, uint32_t want, 
   atomicCAS(status, 0, kMoeErrGrid);
   return false;
 }
+// four rows of a matrix, 128 bytes of each from column x on
+__device__ __forceinline__ void moe_gather4(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, const int (&rows)[4]) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(rows[0]), "r"(rows[1]), "r"(rows[2]), "r"(rows[3])
+      : "memory");
+}
+// between ordinary accesses to memory and those of copies
+__device__ __forceinline__ void moe_fence_async() { asm volatile("fence.proxy.async;" ::: "memory"); }
+// A named barrier that tells whether all its threads say yes.  Warps that share a barrier must all come to it, also where the waits of some have run out.
+__device__ __forceinline__ bool moe_bar_and(int id, int threads, bool yes) {
+  uint32_t all;
+  asm volatile(
+      "{\n"
+      ".reg .pred p, q;\n"
+      "setp.ne.u32 p, %3, 0;\n"
+      "barrier.cta.red.and.aligned.pred q, %1, %2, p;\n"
+      "selp.u32 %0, 1, 0, q;\n"
+      "}\n"
+      : "=r"(all)
+      : "r"(id), "r"(threads), "r"((uint32_t)yes)
+      : "memory");
+  return all != 0;
+}
 __device__ __forceinline__ void moe_tmem_ld8(uint32_t taddr, float (&v)[8]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
@@ -343,29 +424,43 @@ __device__ __forceinline__ void moe_tmem_ld8(uint32_t taddr, float (&v)[8]) {
                : "memory");
 }
 
-// A CTA's run of the list of steps of a product, and the pieces of tiles in it.
-struct MoeRun {
-  int steps, begin, end;  // steps of a tile; of the run
-  int each, more;
-  __device__ __forceinline__ MoeRun(int groups, int tiles, int steps_, int cta, int ctas) {
+// The units of a product: `whole` tiles, then the parts of the others.
+struct MoeUnits {
+  int tiles, steps, whole, parts, units;  // tiles of a group, steps of a tile
+  __device__ __forceinline__ MoeUnits(int groups, int tiles_, int steps_, int ctas) {
+    tiles = tiles_;
     steps = steps_;
-    const int total = groups * tiles * steps;
-    each = total / ctas;
-    more = total - each * ctas;
-    begin = at(cta);
-    end = at(cta + 1);
+    const int total = groups * tiles, cut = min(total, ctas + ctas / 4);
+    const int length = max(4, min((int)((int64_t)total * steps / (4 * ctas)), 8));
+    parts = min((steps + length - 1) / length, kMoeMostParts);
+    whole = parts > 1 ? total - cut : total;
+    units = whole + (parts > 1 ? cut * parts : 0);
   }
-  __device__ __forceinline__ int at(int cta) const { return cta * each + min(cta, more); }
-  __device__ __forceinline__ int cta_of(int step) const {
-    const int longer = more * (each + 1);
-    return step < longer ? step / (each + 1) : more + (step - longer) / each;
+};
+struct MoeUnit {
+  int group, row, part, cut, k0, k1;  // part: -1 for a whole tile; cut: index among the cut tiles
+  __device__ __forceinline__ MoeUnit(const MoeUnits& u, int i) {
+    int tile = i;
+    part = -1;
+    cut = 0;
+    k0 = 0;
+    k1 = u.steps;
+    if (i >= u.whole) {
+      cut = (i - u.whole) / u.parts;
+      part = (i - u.whole) - cut * u.parts;
+      tile = u.whole + cut;
+      k0 = part * u.steps / u.parts;
+      k1 = (part + 1) * u.steps / u.parts;
+    }
+    group = tile / u.tiles;
+    row = tile - group * u.tiles;
   }
 };
 
 template <bool FP8, int MAXN>
 __global__ void __launch_bounds__(32 * kMoeWarps, 1)
-    moe_fused_kernel(const __grid_constant__ CUtensorMap map_up, const __grid_constant__ CUtensorMap map_down, const b200q_moe_args a, int64_t first,
-                     const MoeFused w) {
+    moe_fused_kernel(const __grid_constant__ CUtensorMap map_up, const __grid_constant__ CUtensorMap map_down, const __grid_constant__ CUtensorMap map_x,
+                     const __grid_constant__ CUtensorMap map_h, const b200q_moe_args a, int64_t first, const MoeFused w) {
   using Tile = MoeTile<FP8, MAXN>;
   constexpr int kStages = Tile::kStages, kSteps = Tile::kStep;
   constexpr int kMostSlots = MAXN == 8 ? 8 * kMoeMaxTopK : (int)kMoeChunk * kMoeMaxTopK;
@@ -376,9 +471,12 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
   __shared__ uint16_t s_slot_of[kMostSlots], s_token_of[kMostSlots];  // slot of (token, j); token of a slot
   __shared__ uint16_t s_group_expert[kMostGroups], s_group_slot[kMostGroups];
   __shared__ uint8_t s_group_tokens[kMostGroups];
-  __shared__ __align__(8) uint64_t s_bars[3 * kStages + 4];
+  constexpr int kQueue = 4;  // units that the producer is ahead of the others at most
+  constexpr int kCuts = 4;   // cut units whose parts are not told of yet
+  __shared__ __align__(8) uint64_t s_bars[3 * kStages + 4 + 2 * kQueue + 2 * kCuts];
   __shared__ uint32_t s_tmem;
-  __shared__ int s_abort, s_groups, s_last, s_scan[2][kMoeWarps];
+  __shared__ int s_abort, s_groups, s_slots, s_scan[2][kMoeWarps], s_unit[kQueue];
+  __shared__ uint16_t s_expert_slot[kMoeMaxExperts];  // an expert's first slot
   // before the ring is in use: a bit per token of each expert
   uint32_t* const s_mask = reinterpret_cast<uint32_t*>(s_ring);
   int16_t* const s_ids = reinterpret_cast<int16_t*>(s_ring + sizeof(uint32_t) * kMoeMaxExperts * kMaskWords);  // [tokens][top_k]
@@ -387,21 +485,33 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
   const int cta = blockIdx.x, ctas = gridDim.x;
   const uint32_t bar_weights = ptx::smem_u32(s_bars), bar_tokens = bar_weights + 8 * kStages, bar_empty = bar_tokens + 8 * kStages;
   const uint32_t bar_full = bar_empty + 8 * kStages, bar_free = bar_full + 16;  // of the two accumulators
+  const uint32_t bar_unit = bar_free + 16, bar_taken = bar_unit + 8 * kQueue;
+  const uint32_t bar_parts = bar_taken + 8 * kQueue, bar_told = bar_parts + 8 * kCuts;
   const uint32_t ring = ptx::smem_u32(s_ring);
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
       ptx::mbar_init(bar_weights + 8 * i, 1);
-      ptx::mbar_init(bar_tokens + 8 * i, 4);
+      ptx::mbar_init(bar_tokens + 8 * i, 1);
       ptx::mbar_init(bar_empty + 8 * i, 1);
     }
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(bar_full + 8 * i, 1);
       ptx::mbar_init(bar_free + 8 * i, 4);
     }
+    for (int i = 0; i < kCuts; ++i) {
+      ptx::mbar_init(bar_parts + 8 * i, 4);
+      ptx::mbar_init(bar_told + 8 * i, 1);
+    }
+    for (int i = 0; i < kQueue; ++i) {
+      ptx::mbar_init(bar_unit + 8 * i, 1);
+      ptx::mbar_init(bar_taken + 8 * i, 7);  // (MMAs, terms, sums, four of the results)
+    }
     s_abort = 0;
     ptx::fence_barrier_init();
     ptx::tma_prefetch_desc(&map_up);
     ptx::tma_prefetch_desc(&map_down);
+    ptx::tma_prefetch_desc(&map_x);
+    ptx::tma_prefetch_desc(&map_h);
   }
   if (warp == 1) {
     ptx::tmem_alloc(ptx::smem_u32(&s_tmem), Tile::kTmem);
@@ -409,10 +519,12 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
   }
   pdl_enter();
 
-  // ---- the choice: by every CTA for itself where a warp has two tokens at most, else a token per warp of the grid
+  // ---- the choice: by every CTA for itself where a warp has few tokens (29 tokens of 128 experts: a barrier between the CTAs takes longer than three more
+  // rounds), else a token per warp of the grid
   const int tokens = (int)a.tokens, live = moe_tokens(a, first), top_k = a.top_k, slots = live * top_k;
   bool ok = true;
-  if (MAXN == 8) {
+  for (int i = tid; i < a.experts * kMaskWords; i += 32 * kMoeWarps) s_mask[i] = 0;
+  if (MAXN == 8 || tokens <= 4 * kMoeWarps) {
     for (int t = warp; t < tokens; t += kMoeWarps) {
       const MoeChoice c = moe_choose(a, w.logits + (int64_t)t * a.experts, t < live, lane);
       if (lane < top_k) {
@@ -420,20 +532,18 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
         if (cta == 0) moe_store_choice(a, t, lane, c);
       }
     }
-    for (int i = tid; i < a.experts * kMaskWords; i += 32 * kMoeWarps) s_mask[i] = 0;
     __syncthreads();
   } else {
     for (int t = warp * ctas + cta; t < tokens; t += kMoeWarps * ctas) {
       const MoeChoice c = moe_choose(a, w.logits + (int64_t)t * a.experts, t < live, lane);
       if (lane < top_k) moe_store_choice(a, t, lane, c);
     }
-    for (int i = tid; i < a.experts * kMaskWords; i += 32 * kMoeWarps) s_mask[i] = 0;
     __threadfence();
     __syncthreads();
     if (tid == 0) moe_add_release(&w.control->chosen);
     ok = moe_grid_wait(&w.control->chosen, (uint32_t)ctas, &s_abort, w.status);
     for (int i = tid; i < slots; i += 32 * kMoeWarps) s_ids[i] = (int16_t)__ldcg(a.ids + i);
-    __syncthreads();
+    ok = __syncthreads_and(ok);
   }
 
   // ---- the list: slots in the order of experts, and tokens, and groups of at most MAXN tokens of an expert
@@ -467,27 +577,30 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
       slots_before = all & 0xFFFF;
       groups_before = all >> 16;
       if (n) {
-        int slot = before & 0xFFFF, group = before >> 16;
+        const int slot = before & 0xFFFF;
+        int group = before >> 16;
+        s_expert_slot[e] = (uint16_t)slot;
         for (int i = 0; i < n; i += MAXN, ++group) {
           s_group_expert[group] = (uint16_t)e;
           s_group_slot[group] = (uint16_t)(slot + i);
           s_group_tokens[group] = (uint8_t)min(n - i, MAXN);
         }
-        for (int i = 0; i < kMaskWords; ++i)
-          for (uint32_t m = s_mask[e * kMaskWords + i]; m; m &= m - 1, ++slot) s_token_of[slot] = (uint16_t)(32 * i + __ffs(m) - 1);
       }
     }
-    if (tid == 0) s_groups = groups_before;
+    if (tid == 0) {
+      s_groups = groups_before;
+      s_slots = slots_before;
+    }
   }
   __syncthreads();
-  // slot of (t, j): the expert's first slot and the tokens before t.  (The slots' order is in s_token_of; found by the expert's group.)
-  for (int g = tid; g < s_groups; g += 32 * kMoeWarps) {
-    const int e = s_group_expert[g], s0 = s_group_slot[g];
-    for (int i = 0; i < s_group_tokens[g]; ++i) {
-      const int t = s_token_of[s0 + i];
-      for (int j = 0; j < top_k; ++j)
-        if (s_ids[t * top_k + j] == e) s_slot_of[t * top_k + j] = (uint16_t)(s0 + i);
-    }
+  for (int i = tid; i < slots; i += 32 * kMoeWarps) {  // an expert's slots are in the order of its tokens
+    const int t = i / top_k, e = s_ids[i];
+    if (e < 0 || e >= a.experts) continue;
+    int slot = s_expert_slot[e];
+    for (int k = 0; k < t / 32; ++k) slot += __popc(s_mask[e * kMaskWords + k]);
+    slot += __popc(s_mask[e * kMaskWords + t / 32] & ((1u << (t & 31)) - 1u));
+    s_slot_of[i] = (uint16_t)slot;
+    s_token_of[slot] = (uint16_t)t;
   }
   ptx::tc_fence_before();
   __syncthreads();
@@ -496,69 +609,196 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
   ptx::fence_proxy_async_smem();
   __syncthreads();
   const uint32_t tmem = s_tmem;
-  const int groups = s_groups;
-  const MoeRun runs[2] = {MoeRun(groups, w.up_tiles, w.up_steps, cta, ctas), MoeRun(groups, w.down_tiles, w.down_steps, cta, ctas)};
+  const int groups = s_groups, slots_here = s_slots;
+  const MoeUnits lists[2] = {MoeUnits(groups, w.up_tiles, w.up_steps, ctas), MoeUnits(groups, w.down_tiles, w.down_steps, ctas)};
 
-  if (!ok) {
+  // The next unit as the producer has passed it on, or -1 at the end of a product; the same for all warps but the producer.
+  uint32_t turn = 0, turn_phase = 0;
+  auto next_unit = [&](int code) {
+    int unit = -1;
+    ok = ptx::mbar_wait_uniform(bar_unit + 8 * turn, turn_phase, &s_abort, w.status, code);
+    if (!ok) return unit;
+    unit = *(volatile int*)&s_unit[turn];
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(bar_taken + 8 * turn);
+    if (++turn == kQueue) {
+      turn = 0;
+      turn_phase ^= 1;
+    }
+    return unit;
+  };
+
+  // where a wait has run out: the copies in flight are waited for, as far as they come
+  int made = 0;
+  auto drain = [&](uint32_t bars, uint32_t stage, uint32_t phase) {
+    for (int i = 0; i < min(made, kStages); ++i) {
+      phase ^= stage == 0;
+      stage = stage == 0 ? kStages - 1 : stage - 1;
+      for (int k = 0; k < 4096 && !ptx::mbar_try_wait(bars + 8 * stage, phase); ++k) __nanosleep(64);
+    }
+  };
+  // the terms of a slot's h, by the four warps of the sums
+  auto terms_of_h = [&](int slot) {
+    int group = 0;
+    for (int hi = groups - 1; group < hi;) {  // the last group that does not begin behind the slot
+      const int mid = (group + hi + 1) >> 1;
+      if (s_group_slot[mid] <= slot) group = mid;
+      else hi = mid - 1;
+    }
+    ok = moe_grid_wait(&w.control->up[group], 4 * (uint32_t)w.up_tiles, &s_abort, w.status);
+    if (!ok) return;
+    const float factor = moe_up_factor(__ldcg(w.h_top + slot));
+    for (int64_t i = 8 * (tid - 128); i < a.inner; i += 8 * 128) {
+      const float4* p = reinterpret_cast<const float4*>(w.hidden + slot * a.inner + i);
+      const float4 x = __ldcg(p), y = __ldcg(p + 1);
+      float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        v[c] *= factor;
+        if (!(fabsf(v[c]) <= 3.4e38f)) v[c] = __int_as_float(0x7FC00000);  // (e4m3 has no infinity, and would make it 448)
+      }
+      uint2 term[3];
+      moe_terms_fp8<3>(v, term);
+#pragma unroll
+      for (int c = 0; c < 3; ++c) *reinterpret_cast<uint2*>(w.h_terms + ((int64_t)c * w.slots + slot) * a.inner + i) = term[c];
+    }
+    moe_fence_async();
+    __syncwarp();
+    if (lane == 0) moe_add_release(&w.control->terms[group]);
+  };
+  // what a group's values are to be multiplied by: lane j has token j's
+  auto backs_of = [&](auto which, const MoeUnit& unit) {
+    constexpr int product = decltype(which)::value;
+    const int slot = s_group_slot[unit.group] + lane;
+    if (!FP8 || lane >= s_group_tokens[unit.group]) return 1.f;
+    return moe_down_factor(product ? __ldcg(w.h_top + slot) : __ldcg(w.x_top + s_token_of[slot]));
+  };
+  // a result: token j of a group's values in row `row` of the two tiles of a unit
+  auto finish = [&](auto which, const MoeUnit& unit, int row, int j, float v0, float v1, const float (&scale)[2], float backs) {
+    constexpr int product = decltype(which)::value;
+    const int slot = s_group_slot[unit.group] + j;
+    const float back = __shfl_sync(0xFFFFFFFFu, backs, j);
+    if (product == 0) {
+      const int64_t r = unit.row * 128 + row;
+      const float h = r < a.inner ? moe_silu(v0 * back * scale[0]) * (v1 * back * scale[1]) : 0.f;
+      if constexpr (FP8) {
+        if (r < a.inner) __stcg(w.hidden + (int64_t)slot * a.inner + r, h);
+        const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(h) & 0x7FFFFFFFu);
+        if (lane == 0) atomicMax(w.h_top + slot, top);
+      } else if (r < a.inner) {
+        __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(w.h_terms) + (int64_t)slot * a.inner + r;
+        const __nv_bfloat16 hi = __float2bfloat16_rn(h);
+        to[0] = hi;
+        to[(int64_t)w.slots * a.inner] = __float2bfloat16_rn(h - __bfloat162float(hi));
+      }
+    } else {
+      const int64_t r = unit.row * 256 + row;
+      if (r < a.hidden) __stcg(w.outputs + (int64_t)slot * a.hidden + r, v0 * back * scale[0]);
+      if (r + 128 < a.hidden) __stcg(w.outputs + (int64_t)slot * a.hidden + r + 128, v1 * back * scale[1]);
+    }
+  };
+  // the scales of a row of the two tiles
+  auto scales_of = [&](auto which, const MoeUnit& unit, int row, float (&scale)[2]) {
+    constexpr int product = decltype(which)::value;
+    const int64_t e = s_group_expert[unit.group], r = (product ? unit.row * 256 : unit.row * 128) + row;
+    const float* scales = product ? a.down_scale : a.gate_up_scale;
+    scale[0] = scale[1] = 1.f;
+    if (!scales) return;
+    if (product == 0 && r < a.inner) {
+      scale[0] = scales[e * 2 * a.inner + r];
+      scale[1] = scales[e * 2 * a.inner + a.inner + r];
+    } else if (product == 1) {
+      if (r < a.hidden) scale[0] = scales[e * a.hidden + r];
+      if (r + 128 < a.hidden) scale[1] = scales[e * a.hidden + r + 128];
+    }
+  };
+  // behind the last unit: the warps of the sums and of the results together, whatever became of their waits
+  auto finished_all = [&] {
+    __threadfence();
+    ok = moe_bar_and(3, 256, ok);
+    if (ok && tid == 128) moe_add_release(&w.control->done);
+  };
+  // a tile of a group's first product is finished (one of four warps)
+  auto finished_up = [&](int group) {
+    if (!FP8) moe_fence_async();
+    __syncwarp();
+    if (lane == 0) moe_add_release(&w.control->up[group]);
+  };
+
+  if (!ok && warp < 4) {
     // (a CTA did not come: nothing is in flight, and nobody goes on)
   } else if (warp == 0) {
     // ------------------------------------------------------------ weights
     uint32_t stage = 0, phase = 0;
-    int made = 0;
-    for (int product = 0; product < 2 && ok; ++product) {
-      const MoeRun& run = runs[product];
-      const int tiles = product ? w.down_tiles : w.up_tiles;
-      int tile = run.begin / run.steps, k = run.begin - tile * run.steps;
-      for (int at = run.begin; at < run.end; ++at) {
-        ok = ptx::mbar_wait_uniform(bar_empty + 8 * stage, phase ^ 1, &s_abort, w.status, kMoeErrWeights);
-        if (!ok) break;
-        const int group = tile / tiles, row = tile - group * tiles, e = s_group_expert[group];
-        if (ptx::elect_one()) {
-          const uint32_t bar = bar_weights + 8 * stage, dst = ring + stage * Tile::kStage;
-          ptx::mbar_arrive_expect_tx(bar, 2 * kMoeSubBytes);
-          if (product == 0) {
-            ptx::tma_load_3d(dst, &map_up, bar, k * kSteps, row * 128, 2 * e);
-            ptx::tma_load_3d(dst + kMoeSubBytes, &map_up, bar, k * kSteps, row * 128, 2 * e + 1);
-          } else {
-            ptx::tma_load_3d(dst, &map_down, bar, k * kSteps, row * 256, e);
-            ptx::tma_load_3d(dst + kMoeSubBytes, &map_down, bar, k * kSteps, row * 256 + 128, e);
+    auto publish = [&](int u) {
+      ok = ok && ptx::mbar_wait_uniform(bar_taken + 8 * turn, turn_phase ^ 1, &s_abort, w.status, kMoeErrWeights);
+      if (!ok) return;
+      if (lane == 0) {
+        *(volatile int*)&s_unit[turn] = u;
+        ptx::mbar_arrive(bar_unit + 8 * turn);
+      }
+      if (++turn == kQueue) {
+        turn = 0;
+        turn_phase ^= 1;
+      }
+    };
+    auto stream = [&](auto which) {
+      constexpr int product = decltype(which)::value;
+      const MoeUnits& list = lists[product];
+      // The first units, `dealt` each, are the CTA's by its index.  The others come from the counter, whose answer takes a microsecond or two behind the copies
+      // and is asked for before a unit's copies are.
+      const int dealt = max(1, list.units / ctas * 5 / 8);
+      for (int i = 0, u = cta; ok; ++i) {
+        publish(u < list.units ? u : -1);
+        if (!ok || u >= list.units) break;
+        int next = u + ctas;
+        if (i + 1 >= dealt && lane == 0) next = dealt * ctas + (int)atomicAdd(&w.control->next[product], 1u);
+        const MoeUnit unit(list, u);
+        const int e = s_group_expert[unit.group];
+        for (int k = unit.k0; k < unit.k1; ++k) {
+          ok = ptx::mbar_wait_uniform(bar_empty + 8 * stage, phase ^ 1, &s_abort, w.status, kMoeErrWeights);
+          if (!ok) break;
+          if (ptx::elect_one()) {
+            const uint32_t bar = bar_weights + 8 * stage, dst = ring + stage * Tile::kStage;
+            ptx::mbar_arrive_expect_tx(bar, 2 * kMoeSubBytes);
+            if (product == 0) {
+              ptx::tma_load_3d(dst, &map_up, bar, k * kSteps, unit.row * 128, 2 * e);
+              ptx::tma_load_3d(dst + kMoeSubBytes, &map_up, bar, k * kSteps, unit.row * 128, 2 * e + 1);
+            } else {
+              ptx::tma_load_3d(dst, &map_down, bar, k * kSteps, unit.row * 256, e);
+              ptx::tma_load_3d(dst + kMoeSubBytes, &map_down, bar, k * kSteps, unit.row * 256 + 128, e);
+            }
+          }
+          ++made;
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1;
           }
         }
-        ++made;
-        if (++k == run.steps) {
-          k = 0;
-          ++tile;
-        }
-        if (++stage == kStages) {
-          stage = 0;
-          phase ^= 1;
-        }
+        u = __shfl_sync(0xFFFFFFFFu, next, 0);
       }
-    }
-    if (!ok) {  // the copies in flight are waited for, as far as they come
-      for (int i = 0; i < min(made, kStages); ++i) {
-        phase ^= stage == 0;
-        stage = stage == 0 ? kStages - 1 : stage - 1;
-        for (int k = 0; k < 4096 && !ptx::mbar_try_wait(bar_weights + 8 * stage, phase); ++k) __nanosleep(64);
-      }
-    }
+    };
+    stream(std::integral_constant<int, 0>());
+    if (ok) stream(std::integral_constant<int, 1>());
+    if (!ok) drain(bar_weights, stage, phase);
   } else if (warp == 1) {
     // ------------------------------------------------------------ products
     uint32_t stage = 0, phase = 0;
     int pieces = 0;
     const uint64_t a0 = ptx::smem_desc_k_sw128(ring), b0 = ptx::smem_desc_k_sw128(ring + 2 * kMoeSubBytes);
     for (int product = 0; product < 2 && ok; ++product) {
-      const MoeRun& run = runs[product];
-      const int tiles = product ? w.down_tiles : w.up_tiles, terms = product ? Tile::kDownTerms : Tile::kUpTerms;
-      for (int at = run.begin; at < run.end && ok; ++pieces) {
-        const int tile = run.begin < run.end ? at / run.steps : 0, end = min(run.end, (tile + 1) * run.steps);
-        const int cols = (terms * ((s_group_tokens[tile / tiles] + 7) / 8 * 8) + 15) / 16 * 16;
+      const int terms = product ? Tile::kDownTerms : Tile::kUpTerms;
+      for (; ok; ++pieces) {
+        const int u = next_unit(kMoeErrMma);
+        if (u < 0) break;
+        const MoeUnit unit(lists[product], u);
+        const int cols = ((s_group_tokens[unit.group] + 7) / 8 * 8 * terms + 15) / 16 * 16;
         const uint32_t idesc = FP8 ? ptx::umma_idesc(0, 0, 128, cols) : ptx::umma_idesc(1, 1, 128, cols);
         const uint32_t acc = pieces & 1, d = tmem + acc * 2 * Tile::kCols;
         ok = ptx::mbar_wait_uniform(bar_free + 8 * acc, ((pieces >> 1) & 1) ^ 1, &s_abort, w.status, kMoeErrMma);
         if (!ok) break;
         ptx::tc_fence_after();
-        for (int k = 0; at < end; ++at, ++k) {
+        for (int k = unit.k0; k < unit.k1; ++k) {
           ok = ptx::mbar_wait2_uniform(bar_weights + 8 * stage, phase, bar_tokens + 8 * stage, phase, &s_abort, w.status, kMoeErrMma);
           if (!ok) break;
           ptx::tc_fence_after();
@@ -566,11 +806,11 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
           if (ptx::elect_one()) {
 #pragma unroll
             for (int sub = 0; sub < 2; ++sub) {
-              if (FP8) ptx::umma_f8_x4(d + sub * Tile::kCols, a0 + off + sub * (kMoeSubBytes >> 4), b0 + off, idesc, k != 0, 2, 2);
-              else ptx::umma_f16_x4(d + sub * Tile::kCols, a0 + off + sub * (kMoeSubBytes >> 4), b0 + off, idesc, k != 0, 2, 2);
+              if (FP8) ptx::umma_f8_x4(d + sub * Tile::kCols, a0 + off + sub * (kMoeSubBytes >> 4), b0 + off, idesc, k != unit.k0, 2, 2);
+              else ptx::umma_f16_x4(d + sub * Tile::kCols, a0 + off + sub * (kMoeSubBytes >> 4), b0 + off, idesc, k != unit.k0, 2, 2);
             }
             ptx::umma_commit(bar_empty + 8 * stage);
-            if (at + 1 == end) ptx::umma_commit(bar_full + 8 * acc);
+            if (k + 1 == unit.k1) ptx::umma_commit(bar_full + 8 * acc);
           }
           __syncwarp();
           if (++stage == kStages) {
@@ -580,203 +820,160 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
         }
       }
     }
-  } else if (warp < 6) {
-    // ------------------------------------------------------------ tokens
-    constexpr int kPieces = MAXN * (kSteps / 8) / 128 > 0 ? MAXN * (kSteps / 8) / 128 : 1;  // of eight values, per thread
-    const int lt = tid - 64;
+  } else if (warp == 2) {
+    // ------------------------------------------------------------ terms
     uint32_t stage = 0, phase = 0;
+    auto stream = [&](auto which) {
+      constexpr int product = decltype(which)::value, terms = product ? Tile::kDownTerms : Tile::kUpTerms;
+      int there = -1;  // the group whose h is known to be there
+      while (ok) {
+        const int u = next_unit(kMoeErrTokens);
+        if (u < 0) break;
+        const MoeUnit unit(lists[product], u);
+        const int slot = s_group_slot[unit.group], n = s_group_tokens[unit.group], blocks = (n + 7) / 8;
+        if (product == 1 && unit.group != there) {
+          ok = FP8 ? moe_grid_wait(&w.control->terms[unit.group], 4 * (uint32_t)n, &s_abort, w.status)
+                   : moe_grid_wait(&w.control->up[unit.group], 4 * (uint32_t)w.up_tiles, &s_abort, w.status);
+          if (!ok) break;
+          moe_fence_async();
+          there = unit.group;
+        }
+        // x: lane i fetches four tokens' rows of a term (columns behind the last token are that token's again, and not looked at)
+        const int four = lane & 1, term = (lane >> 1) % terms, block = (lane >> 1) / terms;
+        int rows[4] = {};
+        if (product == 0 && block < blocks) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) rows[i] = term * tokens + s_token_of[slot + min(8 * block + 4 * four + i, n - 1)];
+        }
+        for (int k = unit.k0; k < unit.k1; ++k) {
+          ok = ptx::mbar_wait_uniform(bar_empty + 8 * stage, phase ^ 1, &s_abort, w.status, kMoeErrTokens);
+          if (!ok) break;
+          if (ptx::elect_one()) {
+            const uint32_t bar = bar_tokens + 8 * stage, dst = ring + stage * Tile::kStage + 2 * kMoeSubBytes;
+            ptx::mbar_arrive_expect_tx(bar, blocks * terms * 1024);
+            if (product == 1)
+              for (int g = 0; g < blocks; ++g) ptx::tma_load_3d(dst + g * terms * 1024, &map_h, bar, k * kSteps, slot + 8 * g, 0);
+          }
+          __syncwarp();
+          if (product == 0 && block < blocks)
+            moe_gather4(ring + stage * Tile::kStage + 2 * kMoeSubBytes + (lane >> 1) * 1024 + four * 512, &map_x, bar_tokens + 8 * stage, k * kSteps, rows);
+          __syncwarp();
+          ++made;
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+    };
+    stream(std::integral_constant<int, 0>());
+    if (ok) stream(std::integral_constant<int, 1>());
+    if (!ok) drain(bar_tokens, stage, phase);
+  } else if (warp == 3) {
+    // ------------------------------------------------------------ parts of cut tiles
+    uint32_t cut = 0, cut_phase = 0;
     for (int product = 0; product < 2 && ok; ++product) {
-      const MoeRun& run = runs[product];
-      if (product == 1) {
-        ok = moe_grid_wait(&w.control->up_done, (uint32_t)ctas, &s_abort, w.status);
+      while (ok) {
+        const int u = next_unit(kMoeErrResults);
+        if (u < 0) break;
+        const MoeUnit unit(lists[product], u);
+        if (unit.part < 0) continue;
+        ok = ptx::mbar_wait_uniform(bar_parts + 8 * cut, cut_phase, &s_abort, w.status, kMoeErrResults);
         if (!ok) break;
-      }
-      const int tiles = product ? w.down_tiles : w.up_tiles;
-      const int64_t depth = product ? a.inner : a.hidden;
-      int tile = run.begin / run.steps, k = run.begin - tile * run.steps, group = tile / tiles;
-      uint4 raw[kPieces][2];
-      float factor[kPieces];
-      const uint4 zero = make_uint4(0, 0, 0, 0);
-      // piece i of a thread: token j's values 8 c ... of a step
-      auto token_of = [&](int i) { return (lt + 128 * i) / (kSteps / 8); };
-      auto fetch = [&](int group, int k) {
-        const int n = s_group_tokens[group], slot = s_group_slot[group];
-#pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-          const int j = token_of(i);
-          const int64_t at = (int64_t)k * kSteps + (lt + 128 * i) % (kSteps / 8) * 8;
-          raw[i][0] = raw[i][1] = zero;
-          if (j >= n || at >= depth) continue;
-          if (product == 0) {
-            raw[i][0] = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.x) + s_token_of[slot + j] * a.x_stride + at));
-          } else {
-            const uint4* p = reinterpret_cast<const uint4*>(w.hidden + (int64_t)(slot + j) * a.inner + at);
-            raw[i][0] = __ldcg(p);
-            raw[i][1] = __ldcg(p + 1);
-          }
+        if (lane == 0) {
+          ptx::mbar_arrive(bar_told + 8 * cut);
+          moe_add_release(&w.control->parts[product][unit.cut]);  // (of what the results' warps have written, whose arrivals this one has seen)
         }
-      };
-      auto factors = [&](int group) {
-        const int n = s_group_tokens[group], slot = s_group_slot[group];
-#pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-          const int j = token_of(i);
-          factor[i] = 1.f;
-          if (FP8 && j < n) factor[i] = moe_up_factor(product ? __ldcg(w.h_top + slot + j) : __ldcg(w.x_top + s_token_of[slot + j]));
-        }
-      };
-      if (run.begin < run.end) {
-        factors(group);
-        fetch(group, k);
-      }
-      for (int at = run.begin; at < run.end; ++at) {
-        const int n8 = (s_group_tokens[group] + 7) / 8 * 8;
-        // the terms, while the stage is still in use
-        uint2 low[kPieces][FP8 ? 3 : 1];
-        uint4 wide[kPieces][FP8 ? 1 : 2];
-#pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-          float v[8];
-          if (product == 0) {
-            if (!FP8) {
-              wide[i][0] = raw[i][0];
-              continue;
-            }
-            const uint32_t u[4] = {raw[i][0].x, raw[i][0].y, raw[i][0].z, raw[i][0].w};
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              v[2 * c] = __uint_as_float(u[c] << 16) * factor[i];
-              v[2 * c + 1] = __uint_as_float(u[c] & 0xFFFF0000u) * factor[i];
-            }
-          } else {
-            const uint32_t u[8] = {raw[i][0].x, raw[i][0].y, raw[i][0].z, raw[i][0].w, raw[i][1].x, raw[i][1].y, raw[i][1].z, raw[i][1].w};
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              v[c] = __uint_as_float(u[c]) * factor[i];
-              if (FP8 && !(fabsf(v[c]) <= 3.4e38f)) v[c] = __int_as_float(0x7FC00000);  // (e4m3 has no infinity, and would make it 448)
-            }
-          }
-          if (FP8) {
-            if (product == 0) {
-              uint2 two[2];
-              moe_terms_fp8<2>(v, two);
-              low[i][0] = two[0];
-              low[i][FP8 ? 1 : 0] = two[1];
-            } else {
-              uint2 three[3];
-              moe_terms_fp8<3>(v, three);
-#pragma unroll
-              for (int c = 0; c < 3; ++c) low[i][FP8 ? c : 0] = three[c];
-            }
-          } else {
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              hi[c] = pack_bf16x2(v[2 * c], v[2 * c + 1]);
-              lo[c] = pack_bf16x2(v[2 * c] - __uint_as_float(hi[c] << 16), v[2 * c + 1] - __uint_as_float(hi[c] & 0xFFFF0000u));
-            }
-            wide[i][0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            wide[i][FP8 ? 0 : 1] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-          }
-        }
-        const int here = s_group_tokens[group];
-        // the next step's values are asked for
-        int next_k = k + 1, next_tile = tile;
-        if (next_k == run.steps) {
-          next_k = 0;
-          ++next_tile;
-        }
-        const int next_group = next_tile / tiles;
-        if (at + 1 < run.end) {
-          if (next_group != group) factors(next_group);
-          fetch(next_group, next_k);
-        }
-        ok = ptx::mbar_wait_uniform(bar_empty + 8 * stage, phase ^ 1, &s_abort, w.status, kMoeErrTokens);
-        if (!ok) break;
-        const uint32_t dst = ring + stage * Tile::kStage + 2 * kMoeSubBytes;
-#pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-          const int j = token_of(i), c = (lt + 128 * i) % (kSteps / 8);
-          if (j >= here) continue;
-          const int terms = product ? Tile::kDownTerms : Tile::kUpTerms;
-#pragma unroll
-          for (int t = 0; t < Tile::kDownTerms; ++t) {
-            if (t >= terms) break;
-            const uint32_t row = (uint32_t)(t * n8 + j);
-            if (FP8) {
-              const uint32_t to = dst + row * 128 + ((((uint32_t)c >> 1) ^ (row & 7)) << 4) + (c & 1) * 8;
-              asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to), "r"(low[i][FP8 ? t : 0].x), "r"(low[i][FP8 ? t : 0].y) : "memory");
-            } else {
-              const uint32_t to = dst + row * 128 + (((uint32_t)c ^ (row & 7)) << 4);
-              const uint4 x = wide[i][FP8 ? 0 : t];
-              asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
-            }
-          }
-        }
-        ptx::fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(bar_tokens + 8 * stage);
-        k = next_k;
-        tile = next_tile;
-        group = next_group;
-        if (++stage == kStages) {
-          stage = 0;
-          phase ^= 1;
+        if (++cut == kCuts) {
+          cut = 0;
+          cut_phase ^= 1;
         }
       }
     }
+  } else if (warp < 8) {
+    // ------------------------------------------------------------ sums of cut tiles, terms of h
+    const int row = tid - 128;
+    auto sums_of = [&](auto which) {
+      constexpr int product = decltype(which)::value;
+      const MoeUnits& list = lists[product];
+      const int cut_tiles = list.parts > 1 ? (list.units - list.whole) / list.parts : 0;
+      for (int c = cta; c < cut_tiles; c += ctas) {
+        ok = ok && moe_grid_wait(&w.control->parts[product][c], (uint32_t)list.parts, &s_abort, w.status);
+        if (!ok) break;
+        const MoeUnit unit(list, list.whole + c * list.parts);
+        float scale[2];
+        scales_of(which, unit, row, scale);
+        const float backs = backs_of(which, unit);
+        const int n = s_group_tokens[unit.group];
+        const float* p = w.parts + ((int64_t)product * kMoeCutTiles + unit.cut) * kMoeMostParts * Tile::kPart + row;
+        constexpr int kBatch = 4;  // tokens whose parts are on their way together
+        for (int j0 = 0; j0 < n; j0 += kBatch) {
+          float v[kBatch][2][kMoeMostParts];
+#pragma unroll
+          for (int b = 0; b < kBatch; ++b)
+#pragma unroll
+            for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+              for (int c = 0; c < kMoeMostParts; ++c) v[b][sub][c] = c < list.parts && j0 + b < n ? __ldcg(p + c * Tile::kPart + (sub * MAXN + j0 + b) * 128) : 0.f;
+#pragma unroll
+          for (int b = 0; b < kBatch; ++b) {
+#pragma unroll
+            for (int c = 1; c < kMoeMostParts; ++c) {
+              v[b][0][0] += v[b][0][c];
+              v[b][1][0] += v[b][1][c];
+            }
+            if (j0 + b < n) finish(which, unit, row, j0 + b, v[b][0][0], v[b][1][0], scale, backs);
+          }
+        }
+        if (product == 0) finished_up(unit.group);
+      }
+    };
+    // the slots of groups without cut tiles are ready before those tiles are, the others behind them
+    const int first_cut = groups > 0 ? lists[0].whole / lists[0].tiles : 0, early = first_cut < groups ? s_group_slot[first_cut] : slots_here;
+    int mine = cta;
+    if (FP8)
+      for (; ok && mine < early; mine += ctas) terms_of_h(mine);
+    sums_of(std::integral_constant<int, 0>());
+    if (FP8)
+      for (; ok && mine < slots_here; mine += ctas) terms_of_h(mine);
+    sums_of(std::integral_constant<int, 1>());
+    finished_all();
   } else {
     // ------------------------------------------------------------ results
     const int row = 32 * (warp & 3) + lane;  // of a tile: the lane of tensor memory that this thread reads
     const uint32_t lane_base = (uint32_t)(32 * (warp & 3)) << 16;
-    auto barrier = [] { ptx::named_bar_sync(1, 128); };
     int pieces = 0;
+    uint32_t cut = 0, cut_phase = 0;
     auto results_of = [&](auto which) {
       constexpr int product = decltype(which)::value, terms = product ? Tile::kDownTerms : Tile::kUpTerms;
-      const MoeRun& run = runs[product];
-      const int tiles = product ? w.down_tiles : w.up_tiles;
-      for (int at = run.begin; at < run.end; ++pieces) {
-        const int tile = at / run.steps, tile0 = tile * run.steps, end = min(run.end, tile0 + run.steps);
-        const int group = tile / tiles, row_tile = tile - group * tiles, e = s_group_expert[group], slot = s_group_slot[group], n = s_group_tokens[group];
-        const int n8 = (n + 7) / 8 * 8;
+      for (;; ++pieces) {
+        const int u = next_unit(kMoeErrResults);
+        if (u < 0) break;
+        const MoeUnit unit(lists[product], u);
+        const bool whole = unit.part < 0;
+        const int n = s_group_tokens[unit.group];
         const uint32_t acc = pieces & 1, d = tmem + acc * 2 * Tile::kCols + lane_base;
-        ok = ptx::mbar_wait_uniform(bar_full + 8 * acc, (pieces >> 1) & 1, &s_abort, w.status, kMoeErrResults);
-        if (!ok) return;
-        ptx::tc_fence_after();
-        const bool whole = at == tile0 && end == tile0 + run.steps;
-        // of the rows that this thread has: the two tiles' scales
-        const int64_t r0 = product ? row_tile * 256 + row : row_tile * 128 + row, r1 = product ? r0 + 128 : r0;
-        const int64_t width = product ? a.hidden : a.inner;
-        float scale[2] = {1.f, 1.f};
-        const float* scales = product ? a.down_scale : a.gate_up_scale;
-        if (scales) {
-          if (r0 < width) scale[0] = scales[product ? e * a.hidden + r0 : e * 2 * a.inner + r0];
-          if (r1 < width) scale[1] = scales[product ? e * a.hidden + r1 : e * 2 * a.inner + a.inner + r1];
+        float scale[2], backs = 1.f;
+        if (whole) {
+          scales_of(which, unit, row, scale);
+          if (product == 0) backs = backs_of(which, unit);
+        } else {
+          ok = ptx::mbar_wait_uniform(bar_told + 8 * cut, cut_phase ^ 1, &s_abort, w.status, kMoeErrResults);
+          if (!ok) break;
         }
-        auto finish = [&](int j, float v0, float v1) {  // token j's values of the two tiles
-          if (product == 0) {
-            const float back = FP8 ? moe_down_factor(__ldcg(w.x_top + s_token_of[slot + j])) : 1.f;
-            const float g = v0 * back * scale[0], u = v1 * back * scale[1];
-            const float h = r0 < width ? moe_silu(g) * u : 0.f;
-            if (r0 < width) __stcg(w.hidden + (int64_t)(slot + j) * a.inner + r0, h);
-            if (FP8) {
-              const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(h) & 0x7FFFFFFFu);
-              if (lane == 0) atomicMax(w.h_top + slot + j, top);
-            }
-          } else {
-            const float back = FP8 ? moe_down_factor(__ldcg(w.h_top + slot + j)) : 1.f;
-            if (r0 < width) __stcg(w.outputs + (int64_t)(slot + j) * a.hidden + r0, v0 * back * scale[0]);
-            if (r1 < width) __stcg(w.outputs + (int64_t)(slot + j) * a.hidden + r1, v1 * back * scale[1]);
-          }
-        };
-        float* part = w.parts + ((int64_t)cta * 2 + (at == tile0 ? 1 : 0)) * Tile::kPart;
-        for (int j0 = 0; j0 < n8; j0 += 8) {
+        float* part = w.parts + (((int64_t)product * kMoeCutTiles + unit.cut) * kMoeMostParts + unit.part) * Tile::kPart + row;
+        ok = ptx::mbar_wait_uniform(bar_full + 8 * acc, (pieces >> 1) & 1, &s_abort, w.status, kMoeErrResults);
+        if (!ok) break;
+        ptx::tc_fence_after();
+        if (whole && product == 1) backs = backs_of(which, unit);  // (h's largest value is known now that it has been multiplied)
+        for (int j0 = 0; j0 < n; j0 += 8) {
           float v[2][8];
 #pragma unroll
           for (int sub = 0; sub < 2; ++sub) {
             float term[terms][8];
 #pragma unroll
-            for (int t = 0; t < terms; ++t) moe_tmem_ld8(d + sub * Tile::kCols + t * n8 + j0, term[t]);
+            for (int t = 0; t < terms; ++t) moe_tmem_ld8(d + sub * Tile::kCols + j0 * terms + 8 * t, term[t]);
             ptx::tmem_ld_wait();
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -785,52 +982,36 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
               for (int t = terms - 2; t >= 0; --t) v[sub][i] = term[t][i] + (FP8 ? 1.f / 32.f : 1.f) * v[sub][i];
             }
           }
-          if (whole) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (j0 + i < n) finish(j0 + i, v[0][i], v[1][i]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (j0 + i < n) {
-                __stcg(part + (j0 + i) * 128 + row, v[0][i]);
-                __stcg(part + (MAXN + j0 + i) * 128 + row, v[1][i]);
-              }
+          for (int i = 0; i < 8; ++i) {
+            if (j0 + i >= n) break;
+            if (whole) {
+              finish(which, unit, row, j0 + i, v[0][i], v[1][i], scale, backs);
+            } else {
+              __stcg(part + (j0 + i) * 128, v[0][i]);
+              __stcg(part + (MAXN + j0 + i) * 128, v[1][i]);
+            }
           }
         }
         ptx::tc_fence_before();
         __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(bar_free + 8 * acc);
-        if (!whole) {
-          const int c0 = run.cta_of(tile0), c1 = run.cta_of(tile0 + run.steps - 1);
-          __threadfence();
-          barrier();
-          if (warp == 6 && lane == 0) s_last = atomicAdd(&w.control->joins[product][c0], 1u) == (uint32_t)(c1 - c0);
-          barrier();
-          if (s_last) {
-            __threadfence();
-            for (int j = 0; j < n; ++j) {
-              float v0 = 0.f, v1 = 0.f;
-              for (int c = c0; c <= c1; ++c) {
-                const float* p = w.parts + ((int64_t)c * 2 + (c == c0 ? 1 : 0)) * Tile::kPart;
-                v0 += __ldcg(p + j * 128 + row);
-                v1 += __ldcg(p + (MAXN + j) * 128 + row);
-              }
-              finish(j, v0, v1);
-            }
-          }
+        if (lane == 0) {
+          ptx::mbar_arrive(bar_free + 8 * acc);
+          if (!whole) ptx::mbar_arrive(bar_parts + 8 * cut);
         }
-        at = end;
+        if (whole && product == 0) finished_up(unit.group);
+        if (!whole && ++cut == kCuts) {
+          cut = 0;
+          cut_phase ^= 1;
+        }
       }
-      __threadfence();
-      barrier();
-      if (warp == 6 && lane == 0) moe_add_release(product ? &w.control->down_done : &w.control->up_done);
     };
-    results_of(std::integral_constant<int, 0>());
+    if (ok) results_of(std::integral_constant<int, 0>());
     if (ok) results_of(std::integral_constant<int, 1>());
+    finished_all();
     // ---- the weighted sums
-    if (ok) ok = moe_grid_wait(&w.control->down_done, (uint32_t)ctas, &s_abort, w.status);
-    const int et = tid - 192;
+    if (ok) ok = moe_grid_wait(&w.control->done, (uint32_t)ctas, &s_abort, w.status);
+    const int et = tid - 256;
     const int64_t quads = (a.hidden + 3) / 4;
     for (int64_t i = (int64_t)cta * 128 + et; i < tokens * quads; i += (int64_t)ctas * 128) {
       const int t = (int)(i / quads);
@@ -863,9 +1044,11 @@ MoeSpace::MoeSpace(int64_t tokens, int64_t h, int64_t f, int experts, int top_k)
   clear_words = (int)((sizeof(MoeControl) + sizeof(uint32_t) * slots) / sizeof(uint32_t));
   hidden = moe_align(h_top + sizeof(uint32_t) * slots);
   outputs = moe_align(hidden + sizeof(float) * slots * (size_t)f);
-  parts = moe_align(outputs + sizeof(float) * slots * (size_t)h);
-  const int group = t <= 8 ? 8 : kMoeGroupTokens;
-  bytes = moe_align(parts + sizeof(float) * 2 * (size_t)kNumSMs * 2 * group * 128);
+  x_terms = moe_align(outputs + sizeof(float) * slots * (size_t)h);  // [2][tokens][h]
+  h_terms = moe_align(x_terms + 2 * t * (size_t)h);                    // three of a byte, or two of two
+  parts = moe_align(h_terms + 4 * slots * (size_t)f);
+  const size_t group = t <= 8 ? 8 : kMoeGroupTokens;
+  bytes = moe_align(parts + sizeof(float) * 2 * kMoeCutTiles * kMoeMostParts * 2 * group * 128);
 }
 
 size_t moe_workspace_bytes_impl(int64_t tokens, int64_t hidden, int64_t inner, int experts, int top_k) {
@@ -877,19 +1060,19 @@ static int64_t moe_blocks(int64_t warps) { return (warps + kMoeThreads / 32 - 1)
 static bool moe_fits_tensor_cores(const b200q_moe_args& a) {
   const int64_t size = a.weight_dtype == B200Q_BF16 ? 2 : 1;
   if (a.force_plain || a.hidden <= 0 || a.inner <= 0 || a.hidden > kMoeMostDim || a.inner > kMoeMostDim || a.hidden * size % 16 || a.inner * size % 16) return false;
-  if (a.tokens > 1 && a.x_stride % 8) return false;
+  if (a.tokens > 1 && (a.x_stride % 8 || a.x_stride < a.hidden)) return false;
   for (const void* p : {a.x, a.gate_up, a.down, static_cast<const void*>(a.out)})
     if (reinterpret_cast<uintptr_t>(p) % 16) return false;
   return true;
 }
 
-// [planes][rows][depth] of weights in boxes of 128 rows of 128 bytes
-static int moe_map(CUtensorMap* map, const void* base, bool fp8, int64_t depth, int64_t rows, int64_t planes) {
+// [planes][rows][depth] of weights, or of terms, in boxes of rows of 128 bytes
+static int moe_map(CUtensorMap* map, const void* base, bool fp8, int64_t depth, int64_t rows, int64_t planes, int box_rows = 128, int box_planes = 1) {
   EncodeTiledFn enc = get_encode_fn();
   if (!enc) return B200Q_ERR_CUDA;
   const cuuint64_t size = fp8 ? 1 : 2;
   const cuuint64_t dims[3] = {(cuuint64_t)depth, (cuuint64_t)rows, (cuuint64_t)planes}, strides[2] = {depth * size, rows * depth * size};
-  const cuuint32_t box[3] = {fp8 ? 128u : 64u, 128, 1}, step[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {fp8 ? 128u : 64u, (cuuint32_t)box_rows, (cuuint32_t)box_planes}, step[3] = {1, 1, 1};
   const CUresult r = enc(map, fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, step,
                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? B200Q_OK : B200Q_ERR_UNSUPPORTED;
@@ -918,6 +1101,20 @@ static int moe_launch_fused(const b200q_moe_args& a, int64_t first, const MoeSpa
   if (int rc = moe_map(&map_down, a.down, FP8, a.inner, a.hidden, a.experts)) return rc;
   uint8_t* p = static_cast<uint8_t*>(a.workspace);
   MoeFused w;
+  w.slots = (int)a.tokens * a.top_k;
+  w.h_terms = p + space.h_terms;
+  CUtensorMap map_x, map_h;
+  {  // rows one by one: the terms of x, or x itself
+    EncodeTiledFn enc = get_encode_fn();
+    if (!enc) return B200Q_ERR_CUDA;
+    const cuuint64_t dims[2] = {(cuuint64_t)a.hidden, (cuuint64_t)a.tokens * Tile::kUpTerms};
+    const cuuint64_t stride[1] = {FP8 ? (cuuint64_t)a.hidden : (cuuint64_t)(a.tokens > 1 ? a.x_stride : a.hidden) * 2};
+    const cuuint32_t box[2] = {FP8 ? 128u : 64u, 1}, step[2] = {1, 1};
+    const CUresult r = enc(&map_x, FP8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, FP8 ? p + space.x_terms : const_cast<void*>(a.x), dims, stride, box,
+                           step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return B200Q_ERR_UNSUPPORTED;
+  }
+  if (int rc = moe_map(&map_h, w.h_terms, FP8, a.inner, w.slots, Tile::kDownTerms, 8, Tile::kDownTerms)) return rc;
   w.logits = reinterpret_cast<const double*>(p + space.logits);
   w.x_top = reinterpret_cast<const uint32_t*>(p + space.x_top);
   w.h_top = reinterpret_cast<uint32_t*>(p + space.h_top);
@@ -942,7 +1139,7 @@ static int moe_launch_fused(const b200q_moe_args& a, int64_t first, const MoeSpa
   attr[0].val.cooperative = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  (void)cudaLaunchKernelEx(&cfg, kernel, map_up, map_down, a, first, w);
+  (void)cudaLaunchKernelEx(&cfg, kernel, map_up, map_down, map_x, map_h, a, first, w);
   B200Q_LAUNCH_CHECK();
   return B200Q_OK;
 }
@@ -950,19 +1147,20 @@ static int moe_launch_fused(const b200q_moe_args& a, int64_t first, const MoeSpa
 template <typename W, int EB, int TB>
 static int moe_launch_logits(const b200q_moe_args& a, int64_t first, const MoeSpace& space, cudaStream_t st) {
   uint8_t* p = static_cast<uint8_t*>(a.workspace);
-  const int64_t warps = ((a.experts + EB - 1) / EB) * ((a.tokens + TB - 1) / TB);
+  const int64_t blocks = ((a.experts + EB - 1) / EB) * ((a.tokens + TB - 1) / TB);
   bool wide = a.hidden % 8 == 0 && (a.tokens == 1 || a.x_stride % 8 == 0);
   for (const void* q : {a.x, a.router}) wide = wide && reinterpret_cast<uintptr_t>(q) % 16 == 0;
-  launch_dependent(moe_logits_kernel<W, EB, TB>, dim3((unsigned)moe_blocks(warps)), dim3(kMoeThreads), 0, st, a, first, reinterpret_cast<double*>(p + space.logits),
-                   reinterpret_cast<uint32_t*>(p + space.x_top), reinterpret_cast<uint32_t*>(p + space.control), space.clear_words, wide);
+  launch_dependent(moe_logits_kernel<W, EB, TB>, dim3((unsigned)blocks), dim3(kMoeThreads), 0, st, a, first, reinterpret_cast<double*>(p + space.logits),
+                   reinterpret_cast<uint32_t*>(p + space.x_top), a.weight_dtype == B200Q_E4M3 && moe_fits_tensor_cores(a) ? p + space.x_terms : nullptr,
+                   reinterpret_cast<uint32_t*>(p + space.control), space.clear_words, wide);
   B200Q_LAUNCH_CHECK();
   return B200Q_OK;
 }
 template <typename W>
 static int moe_launch_router(const b200q_moe_args& a, int64_t first, const MoeSpace& space, cudaStream_t st) {
   const int64_t dots = a.tokens * a.experts;
-  if (dots >= 16 * 4 * kNumSMs) return moe_launch_logits<W, 4, 4>(a, first, space, st);
-  if (dots >= 4 * 4 * kNumSMs) return moe_launch_logits<W, 2, 2>(a, first, space, st);
+  if (dots >= 16 * kNumSMs) return moe_launch_logits<W, 4, 4>(a, first, space, st);
+  if (dots >= 4 * kNumSMs) return moe_launch_logits<W, 2, 2>(a, first, space, st);
   return moe_launch_logits<W, 1, 1>(a, first, space, st);
 }
 
