@@ -333,8 +333,8 @@ __global__ void __launch_bounds__(kMoeThreads) moe_sum_kernel(const b200q_moe_ar
 //
 // The terms of x are made by the router's kernel, those of a slot's h when its last tile is finished (its largest value gives their scale), and come by
 // TMA as the weights do, an expert's tokens by gathered rows.  (Made by each CTA for itself, step by step from registers, they paced the kernel.)
-//   warp 0: weights     warp 1: MMAs     warp 2: terms     warp 3: tells of the parts of cut tiles     warps 4-7: sums, terms of h     warps 8-11: results
-constexpr int kMoeWarps = 12;
+//   warp 0: weights     warp 1: MMAs     warp 2: terms     warps 3-6: sums of cut tiles, terms of h     warps 7-10: results
+constexpr int kMoeWarps = 11;
 constexpr int kMoeErrWeights = 821, kMoeErrTokens = 822, kMoeErrMma = 823, kMoeErrResults = 824, kMoeErrGrid = 825;  // status codes: a wait ran out
 constexpr int kMoeGroupTokens = 32;     // of an expert, at a time
 constexpr int kMoeSubBytes = 128 * 128;  // a weight tile: 128 rows of 128 bytes; a step has two (gate and up, or 256 outputs)
@@ -345,7 +345,7 @@ constexpr int kMoeCutTiles = kNumSMs * 5 / 4, kMoeMostParts = 8;
 constexpr int kMoeMostGroups = kMoeMaxExperts + (int)kMoeChunk * kMoeMaxTopK / kMoeGroupTokens;
 struct MoeControl {  // cleared by the router's kernel
   uint32_t chosen, done, next[2];
-  uint32_t parts[2][kMoeCutTiles];  // of a cut tile that are there
+  uint32_t parts[2][kMoeCutTiles];  // of a cut tile that are there, four warps each
   uint32_t up[kMoeMostGroups];      // tiles of a group's first product that are finished, four warps each
   uint32_t terms[kMoeMostGroups];   // slots of a group whose terms are there, four warps each
 };
@@ -424,17 +424,24 @@ __device__ __forceinline__ void moe_tmem_ld8(uint32_t taddr, float (&v)[8]) {
                : "memory");
 }
 
-// The units of a product: `whole` tiles, then the parts of the others.
+// x / d for 0 <= x < 2^22 from 1 / d: (x + 1/2) / d is at least 1 / 2d from a whole number, and its two roundings are off by less than x / d * 2^-22.  (A division of
+// integers is a hundred cycles, and some ten of them stood before the first copy.)
+__device__ __forceinline__ int moe_divide(int x, float inverse) { return (int)(((float)x + 0.5f) * inverse); }
+
+// The units of a product: `whole` tiles, then the parts of the others.  Fewer than 2^22 of them: at most 640 groups, of 512 tiles each.
 struct MoeUnits {
   int tiles, steps, whole, parts, units;  // tiles of a group, steps of a tile
+  float per_group, per_tile;
   __device__ __forceinline__ MoeUnits(int groups, int tiles_, int steps_, int ctas) {
     tiles = tiles_;
     steps = steps_;
     const int total = groups * tiles, cut = min(total, ctas + ctas / 4);
-    const int length = max(4, min((int)((int64_t)total * steps / (4 * ctas)), 8));
-    parts = min((steps + length - 1) / length, kMoeMostParts);
+    const int length = max(4, min((int)((float)total * (float)steps / (float)(4 * ctas)), 8));
+    parts = min(moe_divide(steps + length - 1, 1.f / (float)length), kMoeMostParts);
     whole = parts > 1 ? total - cut : total;
     units = whole + (parts > 1 ? cut * parts : 0);
+    per_group = 1.f / (float)tiles;
+    per_tile = 1.f / (float)parts;
   }
 };
 struct MoeUnit {
@@ -446,13 +453,13 @@ struct MoeUnit {
     k0 = 0;
     k1 = u.steps;
     if (i >= u.whole) {
-      cut = (i - u.whole) / u.parts;
+      cut = moe_divide(i - u.whole, u.per_tile);
       part = (i - u.whole) - cut * u.parts;
       tile = u.whole + cut;
-      k0 = part * u.steps / u.parts;
-      k1 = (part + 1) * u.steps / u.parts;
+      k0 = moe_divide(part * u.steps, u.per_tile);
+      k1 = moe_divide((part + 1) * u.steps, u.per_tile);
     }
-    group = tile / u.tiles;
+    group = moe_divide(tile, u.per_group);
     row = tile - group * u.tiles;
   }
 };
@@ -472,8 +479,7 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
   __shared__ uint16_t s_group_expert[kMostGroups], s_group_slot[kMostGroups];
   __shared__ uint8_t s_group_tokens[kMostGroups];
   constexpr int kQueue = 4;  // units that the producer is ahead of the others at most
-  constexpr int kCuts = 4;   // cut units whose parts are not told of yet
-  __shared__ __align__(8) uint64_t s_bars[3 * kStages + 4 + 2 * kQueue + 2 * kCuts];
+  __shared__ __align__(8) uint64_t s_bars[3 * kStages + 4 + 2 * kQueue];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort, s_groups, s_slots, s_scan[2][kMoeWarps], s_unit[kQueue];
   __shared__ uint16_t s_expert_slot[kMoeMaxExperts];  // an expert's first slot
@@ -486,7 +492,6 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
   const uint32_t bar_weights = ptx::smem_u32(s_bars), bar_tokens = bar_weights + 8 * kStages, bar_empty = bar_tokens + 8 * kStages;
   const uint32_t bar_full = bar_empty + 8 * kStages, bar_free = bar_full + 16;  // of the two accumulators
   const uint32_t bar_unit = bar_free + 16, bar_taken = bar_unit + 8 * kQueue;
-  const uint32_t bar_parts = bar_taken + 8 * kQueue, bar_told = bar_parts + 8 * kCuts;
   const uint32_t ring = ptx::smem_u32(s_ring);
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
@@ -498,13 +503,9 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
       ptx::mbar_init(bar_full + 8 * i, 1);
       ptx::mbar_init(bar_free + 8 * i, 4);
     }
-    for (int i = 0; i < kCuts; ++i) {
-      ptx::mbar_init(bar_parts + 8 * i, 4);
-      ptx::mbar_init(bar_told + 8 * i, 1);
-    }
     for (int i = 0; i < kQueue; ++i) {
       ptx::mbar_init(bar_unit + 8 * i, 1);
-      ptx::mbar_init(bar_taken + 8 * i, 7);  // (MMAs, terms, sums, four of the results)
+      ptx::mbar_init(bar_taken + 8 * i, 6);  // (MMAs, terms, four of the results)
     }
     s_abort = 0;
     ptx::fence_barrier_init();
@@ -648,7 +649,7 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
     ok = moe_grid_wait(&w.control->up[group], 4 * (uint32_t)w.up_tiles, &s_abort, w.status);
     if (!ok) return;
     const float factor = moe_up_factor(__ldcg(w.h_top + slot));
-    for (int64_t i = 8 * (tid - 128); i < a.inner; i += 8 * 128) {
+    for (int64_t i = 8 * (tid - 96); i < a.inner; i += 8 * 128) {
       const float4* p = reinterpret_cast<const float4*>(w.hidden + slot * a.inner + i);
       const float4 x = __ldcg(p), y = __ldcg(p + 1);
       float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
@@ -716,7 +717,7 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
   auto finished_all = [&] {
     __threadfence();
     ok = moe_bar_and(3, 256, ok);
-    if (ok && tid == 128) moe_add_release(&w.control->done);
+    if (ok && tid == 96) moe_add_release(&w.control->done);
   };
   // a tile of a group's first product is finished (one of four warps)
   auto finished_up = [&](int group) {
@@ -725,7 +726,7 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
     if (lane == 0) moe_add_release(&w.control->up[group]);
   };
 
-  if (!ok && warp < 4) {
+  if (!ok && warp < 3) {
     // (a CTA did not come: nothing is in flight, and nobody goes on)
   } else if (warp == 0) {
     // ------------------------------------------------------------ weights
@@ -747,7 +748,7 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
       const MoeUnits& list = lists[product];
       // The first units, `dealt` each, are the CTA's by its index.  The others come from the counter, whose answer takes a microsecond or two behind the copies
       // and is asked for before a unit's copies are.
-      const int dealt = max(1, list.units / ctas * 5 / 8);
+      const int dealt = max(1, (int)((float)list.units / (float)ctas) * 5 / 8);
       for (int i = 0, u = cta; ok; ++i) {
         publish(u < list.units ? u : -1);
         if (!ok || u >= list.units) break;
@@ -869,37 +870,15 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
     stream(std::integral_constant<int, 0>());
     if (ok) stream(std::integral_constant<int, 1>());
     if (!ok) drain(bar_tokens, stage, phase);
-  } else if (warp == 3) {
-    // ------------------------------------------------------------ parts of cut tiles
-    uint32_t cut = 0, cut_phase = 0;
-    for (int product = 0; product < 2 && ok; ++product) {
-      while (ok) {
-        const int u = next_unit(kMoeErrResults);
-        if (u < 0) break;
-        const MoeUnit unit(lists[product], u);
-        if (unit.part < 0) continue;
-        ok = ptx::mbar_wait_uniform(bar_parts + 8 * cut, cut_phase, &s_abort, w.status, kMoeErrResults);
-        if (!ok) break;
-        if (lane == 0) {
-          ptx::mbar_arrive(bar_told + 8 * cut);
-          moe_add_release(&w.control->parts[product][unit.cut]);  // (of what the results' warps have written, whose arrivals this one has seen)
-        }
-        __syncwarp();
-        if (++cut == kCuts) {
-          cut = 0;
-          cut_phase ^= 1;
-        }
-      }
-    }
-  } else if (warp < 8) {
+  } else if (warp < 7) {
     // ------------------------------------------------------------ sums of cut tiles, terms of h
-    const int row = tid - 128;
+    const int row = tid - 96;
     auto sums_of = [&](auto which) {
       constexpr int product = decltype(which)::value;
       const MoeUnits& list = lists[product];
-      const int cut_tiles = list.parts > 1 ? (list.units - list.whole) / list.parts : 0;
+      const int cut_tiles = list.parts > 1 ? min(groups * list.tiles, ctas + ctas / 4) : 0;
       for (int c = cta; c < cut_tiles; c += ctas) {
-        ok = ok && moe_grid_wait(&w.control->parts[product][c], (uint32_t)list.parts, &s_abort, w.status);
+        ok = ok && moe_grid_wait(&w.control->parts[product][c], 4 * (uint32_t)list.parts, &s_abort, w.status);
         if (!ok) break;
         const MoeUnit unit(list, list.whole + c * list.parts);
         float scale[2];
@@ -930,7 +909,7 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
       }
     };
     // the slots of groups without cut tiles are ready before those tiles are, the others behind them
-    const int first_cut = groups > 0 ? lists[0].whole / lists[0].tiles : 0, early = first_cut < groups ? s_group_slot[first_cut] : slots_here;
+    const int first_cut = moe_divide(lists[0].whole, lists[0].per_group), early = first_cut < groups ? s_group_slot[first_cut] : slots_here;
     int mine = cta;
     if (FP8)
       for (; ok && mine < early; mine += ctas) terms_of_h(mine);
@@ -944,7 +923,6 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
     const int row = 32 * (warp & 3) + lane;  // of a tile: the lane of tensor memory that this thread reads
     const uint32_t lane_base = (uint32_t)(32 * (warp & 3)) << 16;
     int pieces = 0;
-    uint32_t cut = 0, cut_phase = 0;
     auto results_of = [&](auto which) {
       constexpr int product = decltype(which)::value, terms = product ? Tile::kDownTerms : Tile::kUpTerms;
       for (;; ++pieces) {
@@ -958,9 +936,6 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
         if (whole) {
           scales_of(which, unit, row, scale);
           if (product == 0) backs = backs_of(which, unit);
-        } else {
-          ok = ptx::mbar_wait_uniform(bar_told + 8 * cut, cut_phase ^ 1, &s_abort, w.status, kMoeErrResults);
-          if (!ok) break;
         }
         float* part = w.parts + (((int64_t)product * kMoeCutTiles + unit.cut) * kMoeMostParts + unit.part) * Tile::kPart + row;
         ok = ptx::mbar_wait_uniform(bar_full + 8 * acc, (pieces >> 1) & 1, &s_abort, w.status, kMoeErrResults);
@@ -997,13 +972,9 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
         __syncwarp();
         if (lane == 0) {
           ptx::mbar_arrive(bar_free + 8 * acc);
-          if (!whole) ptx::mbar_arrive(bar_parts + 8 * cut);
+          if (!whole) moe_add_release(&w.control->parts[product][unit.cut]);
         }
         if (whole && product == 0) finished_up(unit.group);
-        if (!whole && ++cut == kCuts) {
-          cut = 0;
-          cut_phase ^= 1;
-        }
       }
     };
     if (ok) results_of(std::integral_constant<int, 0>());
@@ -1011,7 +982,7 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
     finished_all();
     // ---- the weighted sums
     if (ok) ok = moe_grid_wait(&w.control->done, (uint32_t)ctas, &s_abort, w.status);
-    const int et = tid - 256;
+    const int et = tid - 224;
     const int64_t quads = (a.hidden + 3) / 4;
     for (int64_t i = (int64_t)cta * 128 + et; i < tokens * quads; i += (int64_t)ctas * 128) {
       const int t = (int)(i / quads);
