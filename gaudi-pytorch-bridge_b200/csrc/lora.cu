@@ -155,6 +155,47 @@ __global__ void __launch_bounds__(kLoraSortThreads) lora_sort_kernel(const b200q
   }
 }
 
+// The plan as a CTA finds it: made by the kernel in front, or, for up to 32 tokens, here, by one warp (a launch takes longer).
+struct LoraHere {
+  int tiles, adapter[kLoraTile];
+  uint32_t tokens[kLoraTile];  // a bit per token
+};
+__device__ __forceinline__ int lora_tiles(const b200q_lora_args& a, const LoraPlan& p, LoraHere& here) {
+  if (p.tiles_used) return *p.tiles_used;
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x, i = lane < a.tokens ? lora_adapter(a, lane) : -1;
+    const uint32_t same = __match_any_sync(0xFFFFFFFFu, i);
+    const bool first = i >= 0 && lane == __ffs(same) - 1;
+    const uint32_t all = __ballot_sync(0xFFFFFFFFu, first);
+    if (first) {
+      const int tile = __popc(all & ((1u << lane) - 1u));
+      here.adapter[tile] = i;
+      here.tokens[tile] = same;
+    }
+    if (lane == 0) here.tiles = __popc(all);
+  }
+  __syncthreads();
+  return here.tiles;
+}
+// the tile's adapter, number of tokens, and tokens (the last one again behind it); the block's threads together, between two barriers
+__device__ __forceinline__ LoraTile lora_tile(const LoraPlan& p, const LoraHere& here, int index, int (&s_token)[kLoraTile]) {
+  LoraTile tile;
+  const int tid = threadIdx.x;
+  if (p.tiles_used) {
+    tile = p.tiles[index];
+    if (tid < kLoraTile) s_token[tid] = p.sorted[tile.first + min(tid, tile.count - 1)];
+  } else {
+    const uint32_t mask = here.tokens[index];
+    tile = {here.adapter[index], 0, __popc(mask), 0};
+    if (tid < kLoraTile) {
+      const int last = 31 - __clz((int)mask);
+      if (mask >> tid & 1u) s_token[__popc(mask & ((1u << tid) - 1u))] = tid;
+      if (tid >= tile.count) s_token[tid] = last;
+    }
+  }
+  return tile;
+}
+
 // a x of a tile's tokens over a part of k: ranks are the rows of the product, tokens its columns.  Each warp has every eighth 64 bytes of the rows of both, so
 // that nothing is loaded twice; the warps' sums are added in shared memory.
 template <int MT>  // tiles of 16 ranks
@@ -163,14 +204,14 @@ __global__ void __launch_bounds__(kLoraThreads) lora_down_kernel(const b200q_lor
   constexpr int kBatch = MT <= 2 ? 4 : MT == 4 ? 2 : 1;  // steps of 32 values of k on their way together
   extern __shared__ float s_sum[];                       // [warps][tokens][kPitch]
   __shared__ int s_token[kLoraTile];
+  __shared__ LoraHere s_here;
   pdl_enter();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const int blocks = ((int)a.rank + kRanks - 1) / kRanks, items = *p.tiles_used * p.splits * blocks;
+  const int blocks = ((int)a.rank + kRanks - 1) / kRanks, items = lora_tiles(a, p, s_here) * p.splits * blocks;
   for (int item = blockIdx.x; item < items; item += gridDim.x) {
     const int block = item % blocks, part = item / blocks % p.splits;
-    const LoraTile tile = p.tiles[item / blocks / p.splits];
     __syncthreads();  // (the item before this one is done with shared memory)
-    if (tid < kLoraTile) s_token[tid] = p.sorted[tile.first + min(tid, tile.count - 1)];
+    const LoraTile tile = lora_tile(p, s_here, item / blocks / p.splits, s_token);
     __syncthreads();
     const __nv_bfloat16* x[NT];
     const __nv_bfloat16* rows = static_cast<const __nv_bfloat16*>(a.a) + tile.adapter * a.a_stride + (int64_t)(block * kRanks + g) * a.a_row_stride + 8 * t;
@@ -231,24 +272,39 @@ __global__ void __launch_bounds__(kLoraThreads) lora_down_kernel(const b200q_lor
   }
 }
 
-// y += b (scale a x): tokens are the rows of the product, 64 values of y of a warp its columns, of which a lane has 16 neighbours in four rows.
+// y += b (scale a x): tokens are the rows of the product, 32 values of y of a warp its columns, of which a lane has 8 neighbours in four rows.  The values of y for
+// the next step are on their way while this one's products are formed.
 template <typename Y, bool WIDE>  // WIDE: ranks 32 at a time, in 16 bytes a lane; else 16 at a time
-__global__ void __launch_bounds__(kLoraThreads) lora_up_kernel(const b200q_lora_args a, const LoraPlan p, int parts, int width) {
+__global__ void __launch_bounds__(kLoraThreads, 2) lora_up_kernel(const b200q_lora_args a, const LoraPlan p, int parts, int width) {
   constexpr int kTerms = sizeof(Y) == 4 ? 3 : 2, kWarps = kLoraThreads / 32, kStep = WIDE ? 32 : 16, kHalves = WIDE ? 2 : 1;
-  constexpr int kY = sizeof(Y) == 4 ? 4 : 2;  // 16-byte pieces of a lane's 16 values
-  extern __shared__ __align__(16) uint8_t s_raw[];  // [terms][tokens][pitch] of bf16
+  constexpr int kY = sizeof(Y) == 4 ? 2 : 1, kPer = 16 / sizeof(Y);  // 16-byte pieces of a lane's 8 values; values of a piece
+  extern __shared__ __align__(16) uint8_t s_raw[];                   // [terms][tokens][pitch] of bf16
   __shared__ int s_token[kLoraTile];
+  __shared__ LoraHere s_here;
   pdl_enter();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const int rank = (int)a.rank, steps = (rank + kStep - 1) / kStep, pitch = steps * kStep + 8, items = *p.tiles_used * parts;
+  const int rank = (int)a.rank, steps = (rank + kStep - 1) / kStep, pitch = steps * kStep + 8, items = lora_tiles(a, p, s_here) * parts;
   __nv_bfloat16* const s_low = reinterpret_cast<__nv_bfloat16*>(s_raw);
   for (int item = blockIdx.x; item < items; item += gridDim.x) {
     const int part = item % parts;
-    const LoraTile tile = p.tiles[item / parts];
+    __syncthreads();
+    const LoraTile tile = lora_tile(p, s_here, item / parts, s_token);
     const float scale = a.scales ? a.scales[tile.adapter] : 1.f;
     __syncthreads();
-    if (tid < kLoraTile) s_token[tid] = p.sorted[tile.first + min(tid, tile.count - 1)];
-    __syncthreads();
+    const int n_end = (int)min((int64_t)(part + 1) * width, a.n);
+    int n0 = part * width + 32 * warp;
+    Y* rows[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) rows[i] = static_cast<Y*>(a.y) + s_token[g + 8 * i] * a.y_stride + 8 * t;
+    uint4 next[4][kY];
+    auto ask = [&](int n) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int c = 0; c < kY; ++c)
+          if (g + 8 * i < tile.count && n < n_end && n + 8 * t + c * kPer < a.n) next[i][c] = *reinterpret_cast<const uint4*>(rows[i] + n + c * kPer);
+    };
+    ask(n0);
     for (int i = tid; i < kLoraTile * steps * kStep; i += kLoraThreads) {
       const int j = i / (steps * kStep), r = i - j * (steps * kStep);
       float v = 0.f;
@@ -264,37 +320,31 @@ __global__ void __launch_bounds__(kLoraThreads) lora_up_kernel(const b200q_lora_
       }
     }
     __syncthreads();
-    const int64_t n_end = min((int64_t)(part + 1) * width, a.n);
     const bool two = tile.count > 16;
-    for (int64_t n0 = (int64_t)part * width + 64 * warp; n0 < n_end; n0 += 64 * kWarps) {
-      // y first: it comes from the farthest
-      const int64_t ny = n0 + 16 * t;
-      uint4 ry[4][kY];
+    // column g of product c is y's n0 + 8 (g / 2) + 2 c + g % 2
+    const int column = 8 * (g >> 1) + (g & 1);
+    const __nv_bfloat16* const b0 = static_cast<const __nv_bfloat16*>(a.b) + tile.adapter * a.b_stride + column * a.b_row_stride + (WIDE ? 8 : 4) * t;
+    for (; n0 < n_end; n0 += 32 * kWarps) {
+      uint4 now[4][kY];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int j = g + 8 * i;
-        if (j >= tile.count) continue;
-        const Y* y = static_cast<const Y*>(a.y) + s_token[j] * a.y_stride + ny;
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int c = 0; c < kY; ++c)
-          if (ny + c * (16 / kY) < a.n) ry[i][c] = *reinterpret_cast<const uint4*>(y + c * (16 / kY));
-      }
-      float acc[2][8][4];
+        for (int c = 0; c < kY; ++c) now[i][c] = next[i][c];
+      ask(n0 + 32 * kWarps);
+      float acc[2][4][4];
 #pragma unroll
       for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int c = 0; c < 8; ++c)
+        for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int i = 0; i < 4; ++i) acc[m][c][i] = 0.f;
-      // column g of product c is y's n0 + 16 (g / 2) + 2 c + g % 2
-      const int64_t nb = n0 + 16 * (g >> 1) + (g & 1);
-      const __nv_bfloat16* b = static_cast<const __nv_bfloat16*>(a.b) + tile.adapter * a.b_stride + nb * a.b_row_stride + (WIDE ? 8 : 4) * t;
+      const __nv_bfloat16* b = b0 + n0 * a.b_row_stride;
       for (int k = 0; k < steps; ++k) {
-        uint32_t rb[8][2 * kHalves];
+        uint32_t rb[4][2 * kHalves];
         const bool in = k * kStep + (WIDE ? 8 : 4) * t < rank;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          const bool there = in && nb + 2 * c < a.n;
+        for (int c = 0; c < 4; ++c) {
+          const bool there = in && n0 + column + 2 * c < a.n;
           if constexpr (WIDE) {
             const uint4 v = there ? __ldg(reinterpret_cast<const uint4*>(b + 2 * c * a.b_row_stride + k * kStep)) : make_uint4(0, 0, 0, 0);
             rb[c][0] = v.x; rb[c][1] = v.y; rb[c][2] = v.z; rb[c][3] = v.w;
@@ -322,33 +372,32 @@ __global__ void __launch_bounds__(kLoraThreads) lora_up_kernel(const b200q_lora_
 #pragma unroll
             for (int h = 0; h < kHalves; ++h)
 #pragma unroll
-              for (int c = 0; c < 8; ++c) lora_mma(acc[m][c], lo[2 * h], hi[2 * h], lo[2 * h + 1], hi[2 * h + 1], rb[c][2 * h], rb[c][2 * h + 1]);
+              for (int c = 0; c < 4; ++c) lora_mma(acc[m][c], lo[2 * h], hi[2 * h], lo[2 * h + 1], hi[2 * h + 1], rb[c][2 * h], rb[c][2 * h + 1]);
           }
         }
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int j = g + 8 * i;
-        if (j >= tile.count) continue;
-        Y* y = static_cast<Y*>(a.y) + s_token[j] * a.y_stride + ny;
+        if (g + 8 * i >= tile.count) continue;
 #pragma unroll
         for (int c = 0; c < kY; ++c) {
-          if (ny + c * (16 / kY) >= a.n) continue;
+          if (n0 + 8 * t + c * kPer >= a.n) continue;
           // the lane's values 2 q and 2 q + 1 are in product q
+          Y* y = rows[i] + n0 + c * kPer;
           if constexpr (sizeof(Y) == 4) {
             const float* v0 = acc[i >> 1][2 * c] + 2 * (i & 1);
             const float* v1 = acc[i >> 1][2 * c + 1] + 2 * (i & 1);
-            *reinterpret_cast<float4*>(y + 4 * c) = make_float4(__uint_as_float(ry[i][c].x) + v0[0], __uint_as_float(ry[i][c].y) + v0[1],
-                                                                __uint_as_float(ry[i][c].z) + v1[0], __uint_as_float(ry[i][c].w) + v1[1]);
+            *reinterpret_cast<float4*>(y) = make_float4(__uint_as_float(now[i][c].x) + v0[0], __uint_as_float(now[i][c].y) + v0[1],
+                                                        __uint_as_float(now[i][c].z) + v1[0], __uint_as_float(now[i][c].w) + v1[1]);
           } else {
-            const uint32_t u[4] = {ry[i][c].x, ry[i][c].y, ry[i][c].z, ry[i][c].w};
+            const uint32_t u[4] = {now[i][c].x, now[i][c].y, now[i][c].z, now[i][c].w};
             uint32_t w[4];
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-              const float* v = acc[i >> 1][4 * c + q] + 2 * (i & 1);
+              const float* v = acc[i >> 1][q] + 2 * (i & 1);
               w[q] = pack_bf16x2(__uint_as_float(u[q] << 16) + v[0], __uint_as_float(u[q] & 0xFFFF0000u) + v[1]);
             }
-            *reinterpret_cast<uint4*>(y + 8 * c) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(y) = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
       }
@@ -399,8 +448,8 @@ static int lora_launch_up(const b200q_lora_args& a, const LoraPlan& p, int64_t t
   constexpr int kMost = 2 * kTerms * kLoraTile * ((int)kLoraMaxRank + 8);
   static std::atomic<int> done[kMaxDevices];
   if (int rc = lora_ready(reinterpret_cast<const void*>(lora_up_kernel<Y, WIDE>), done, kMost)) return rc;
-  const int64_t most_parts = (a.n + 511) / 512, wanted = (2 * kNumSMs + tiles - 1) / tiles, parts = wanted < most_parts ? wanted : most_parts;
-  const int64_t width = ((a.n + parts - 1) / parts + 511) / 512 * 512, used = (a.n + width - 1) / width;
+  const int64_t most_parts = (a.n + 255) / 256, wanted = (4 * kNumSMs + tiles - 1) / tiles, parts = wanted < most_parts ? wanted : most_parts;
+  const int64_t width = ((a.n + parts - 1) / parts + 255) / 256 * 256, used = (a.n + width - 1) / width;
   const int64_t items = tiles * used, most = 4 * kNumSMs;
   const size_t smem = (size_t)(2 * kTerms * kLoraTile) * ((a.rank + kStep - 1) / kStep * kStep + 8);
   launch_dependent(lora_up_kernel<Y, WIDE>, dim3((unsigned)(items < most ? items : most)), dim3(kLoraThreads), smem, st, a, p, (int)used, (int)width);
@@ -422,8 +471,12 @@ static int lora_chunk_fast(const b200q_lora_args& a, cudaStream_t st) {
   static std::atomic<int> done[kMaxDevices];
   constexpr int kMost = (int)sizeof(uint16_t) * (kLoraSortThreads / 32 + 1) * (int)kLoraMaxAdapters;
   if (int rc = lora_ready(reinterpret_cast<const void*>(lora_sort_kernel), done, kMost)) return rc;
-  launch_dependent(lora_sort_kernel, dim3(1), dim3(kLoraSortThreads), sizeof(uint16_t) * (kLoraSortThreads / 32 + 1) * (size_t)a.adapters, st, a, p);
-  B200Q_LAUNCH_CHECK();
+  if (a.tokens <= kLoraTile) {
+    p.tiles_used = nullptr;  // (each CTA makes the plan for itself)
+  } else {
+    launch_dependent(lora_sort_kernel, dim3(1), dim3(kLoraSortThreads), sizeof(uint16_t) * (kLoraSortThreads / 32 + 1) * (size_t)a.adapters, st, a, p);
+    B200Q_LAUNCH_CHECK();
+  }
   int rc;
   if (a.rank <= 16) rc = lora_launch_down<1>(a, p, tiles, st);
   else if (a.rank <= 32) rc = lora_launch_down<2>(a, p, tiles, st);
