@@ -1,5 +1,6 @@
 // Low-rank adapters of many requests beside a product that they share: y[t] += scale * b (a x[t]) with the adapter of each token.
 #include "layer.cuh"
+#include "tma_host.cuh"
 
 namespace b200q {
 
@@ -48,22 +49,24 @@ __global__ void __launch_bounds__(kLoraPlainThreads) lora_plain_up_kernel(const 
 
 // ---------------------------------------------------------------------------- tensor cores
 // Bound by memory: the adapters that are used where tokens are few, y (read and written) where they are many.  Tokens of one adapter have to be
-// taken together, in whatever order they come, or its matrices are read again for each: a first kernel sorts the tokens by adapter into tiles of 32.
-// Then a x and b (a x) are m16n8k16 products on fragments that come straight from global memory, 16 bytes a lane: the values of K may be taken in any
-// order as long as both operands take the same one, and so may the columns of y, whose order is such that a lane has 16 neighbours.
-constexpr int kLoraTile = 32;
+// taken together, in whatever order they come, or its matrices are read again for each: a first kernel sorts the tokens by adapter into tiles.  In both products
+// the adapter's matrix has the 128 rows of tcgen05.mma (ranks, or columns of y) and the tile's tokens are its columns, so that a warp's results are
+// neighbours in memory: a x is bf16 times bf16, both by TMA (tokens by gathered rows); b (a x) has a x in bf16 terms that follow one another along K.
 constexpr int kLoraSortThreads = 1024;
-constexpr int kLoraThreads = 256;
+constexpr int kLoraFew = 32;  // tokens up to which each CTA sorts for itself
+constexpr int kLoraErrCopy = 831, kLoraErrMma = 832, kLoraErrResults = 833;  // status codes: a wait ran out
 
 struct LoraTile {
   int adapter, first, count, unused;  // tokens sorted[first] ...
 };
 struct LoraPlan {
-  int* tiles_used;
+  int* tiles_used;  // or null: the plan is made by each CTA
   LoraTile* tiles;
   int* sorted;
   float* low;  // [splits][tokens][rank]: a x, in parts over k
-  int splits, slice;  // values of k per part
+  int splits, steps, part_steps;  // parts of k; steps of 64 values of k, and of a part
+  int tile;                       // tokens of a tile at most
+  int* status;
 };
 struct LoraSpace {
   size_t tiles, sorted, low, bytes;
@@ -75,20 +78,22 @@ struct LoraSpace {
     bytes = lora_align(low + sizeof(float) * t * (size_t)(rank * splits));
   }
 };
-// tiles that the tokens may need at most; parts of k and of n such that as many CTAs have work as there are SMs, twice over
-static int64_t lora_most_tiles(int64_t tokens, int64_t adapters) {
-  const int64_t t = tokens < kLoraChunk ? tokens : kLoraChunk, shared = adapters + t / kLoraTile;
+
+// Tiles of 128 tokens where an adapter has many on average and their terms leave room for the copies, else of 16: those take less shared memory, and so more copies
+// are on their way.
+static int lora_tile_tokens(int64_t tokens, int64_t rank, int64_t adapters, bool wide) {
+  const int64_t t = tokens < kLoraChunk ? tokens : kLoraChunk, blocks = (wide ? 3 : 2) * ((rank + 63) / 64);
+  return t >= 24 * adapters && t > 64 && blocks <= 6 ? 128 : 16;
+}
+// tiles that the tokens may need at most, and parts of k such that two CTAs of each SM have work
+static int64_t lora_most_tiles(int64_t tokens, int64_t adapters, int tile) {
+  const int64_t t = tokens < kLoraChunk ? tokens : kLoraChunk, shared = adapters + t / tile;
   return t < shared ? t : shared;
 }
-static int64_t lora_splits(int64_t tokens, int64_t k, int64_t adapters) {
-  const int64_t most = (k + 255) / 256, wanted = (2 * kNumSMs + lora_most_tiles(tokens, adapters) - 1) / lora_most_tiles(tokens, adapters);
-  return wanted < 1 ? 1 : wanted < most ? (wanted < 16 ? wanted : 16) : (most < 16 ? most : 16);
-}
-
-__device__ __forceinline__ void lora_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+static int64_t lora_splits(int64_t tokens, int64_t k, int64_t adapters, int tile) {
+  const int64_t most = (k + 255) / 256, tiles = lora_most_tiles(tokens, adapters, tile), wanted = (2 * kNumSMs + tiles - 1) / tiles;
+  const int64_t splits = wanted < most ? wanted : most;
+  return splits < 1 ? 1 : splits < 16 ? splits : 16;
 }
 
 // A stable counting sort by one block: each warp has a run of the tokens and counts of its own.
@@ -100,13 +105,21 @@ __global__ void __launch_bounds__(kLoraSortThreads) lora_sort_kernel(const b200q
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, adapters = (int)a.adapters, tokens = (int)a.tokens;
   uint16_t* const mine = s_count + warp * adapters;
   uint16_t* const s_first = s_count + kWarps * adapters;
+  constexpr int kKept = (int)kLoraChunk / kLoraSortThreads;  // tokens of a thread
+  const int per = (tokens + 32 * kWarps - 1) / (32 * kWarps), begin = warp * per * 32;
+  int adapter[kKept];
+#pragma unroll
+  for (int i = 0; i < kKept; ++i) adapter[i] = i < per && begin + 32 * i + lane < tokens ? lora_adapter(a, begin + 32 * i + lane) : -1;
   for (int i = tid; i < kWarps * adapters; i += kLoraSortThreads) s_count[i] = 0;
   __syncthreads();
-  const int per = (tokens + 32 * kWarps - 1) / (32 * kWarps) * 32, begin = warp * per, end = min(begin + per, tokens);
-  for (int base = begin; base < end; base += 32) {
-    const int t = base + lane, i = t < end ? lora_adapter(a, t) : -1;
-    const uint32_t same = __match_any_sync(0xFFFFFFFFu, i);
-    if (i >= 0 && lane == __ffs(same) - 1) mine[i] += (uint16_t)__popc(same);
+  int place[kKept];  // among the warp's tokens of the adapter
+#pragma unroll
+  for (int i = 0; i < kKept; ++i) {
+    if (i >= per) break;
+    const uint32_t same = __match_any_sync(0xFFFFFFFFu, adapter[i]);
+    place[i] = adapter[i] >= 0 ? mine[adapter[i]] + __popc(same & ((1u << lane) - 1u)) : 0;
+    __syncwarp();
+    if (adapter[i] >= 0 && lane == __ffs(same) - 1) mine[adapter[i]] += (uint16_t)__popc(same);
     __syncwarp();
   }
   __syncthreads();
@@ -114,13 +127,15 @@ __global__ void __launch_bounds__(kLoraSortThreads) lora_sort_kernel(const b200q
   for (int base = 0, turn = 0; base < adapters; base += kLoraSortThreads, turn ^= 1) {
     const int i = base + tid;
     int n = 0;
-    if (i < adapters)
+    if (i < adapters) {
+#pragma unroll 8
       for (int w = 0; w < kWarps; ++w) {
         const int c = s_count[w * adapters + i];
         s_count[w * adapters + i] = (uint16_t)n;
         n += c;
       }
-    const int tiles = (n + kLoraTile - 1) / kLoraTile, both = n | tiles << 16;  // (sums of at most 8192 each)
+    }
+    const int tiles = (n + p.tile - 1) / p.tile, both = n | tiles << 16;  // (sums of at most 8192 each)
     int scan = both;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -138,288 +153,481 @@ __global__ void __launch_bounds__(kLoraSortThreads) lora_sort_kernel(const b200q
     tokens_before = all & 0xFFFF;
     tiles_before = all >> 16;
     if (i < adapters) s_first[i] = (uint16_t)(before & 0xFFFF);
-    for (int j = 0; j < tiles; ++j) p.tiles[(before >> 16) + j] = {i, (before & 0xFFFF) + j * kLoraTile, min(n - j * kLoraTile, kLoraTile), 0};
+    for (int j = 0; j < tiles; ++j) p.tiles[(before >> 16) + j] = {i, (before & 0xFFFF) + j * p.tile, min(n - j * p.tile, p.tile), 0};
   }
   if (tid == 0) *p.tiles_used = tiles_before;
   __syncthreads();
-  for (int base = begin; base < end; base += 32) {
-    const int t = base + lane, i = t < end ? lora_adapter(a, t) : -1;
-    const uint32_t same = __match_any_sync(0xFFFFFFFFu, i);
-    if (i >= 0) {
-      const int at = mine[i];
-      p.sorted[s_first[i] + at + __popc(same & ((1u << lane) - 1u))] = t;
-    }
-    __syncwarp();
-    if (i >= 0 && lane == __ffs(same) - 1) mine[i] += (uint16_t)__popc(same);
-    __syncwarp();
-  }
+#pragma unroll
+  for (int i = 0; i < kKept; ++i)
+    if (i < per && adapter[i] >= 0) p.sorted[s_first[adapter[i]] + mine[adapter[i]] + place[i]] = begin + 32 * i + lane;
 }
 
-// The plan as a CTA finds it: made by the kernel in front, or, for up to 32 tokens, here, by one warp (a launch takes longer).
-struct LoraHere {
-  int tiles, adapter[kLoraTile];
-  uint32_t tokens[kLoraTile];  // a bit per token
+// The plan as a CTA finds it: made by the kernel in front, or, for few tokens, here, by one warp (a launch takes longer).
+struct LoraFew {
+  int tiles_used, sorted[kLoraFew];
+  LoraTile tiles[kLoraFew];
 };
-__device__ __forceinline__ int lora_tiles(const b200q_lora_args& a, const LoraPlan& p, LoraHere& here) {
-  if (p.tiles_used) return *p.tiles_used;
+struct LoraView {
+  int tiles_used;
+  const LoraTile* tiles;
+  const int* sorted;
+};
+__device__ __forceinline__ LoraView lora_view(const b200q_lora_args& a, const LoraPlan& p, LoraFew& few) {
+  if (p.tiles_used) return {*p.tiles_used, p.tiles, p.sorted};
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x, i = lane < a.tokens ? lora_adapter(a, lane) : -1;
     const uint32_t same = __match_any_sync(0xFFFFFFFFu, i);
+    const int n = __popc(same);
     const bool first = i >= 0 && lane == __ffs(same) - 1;
-    const uint32_t all = __ballot_sync(0xFFFFFFFFu, first);
-    if (first) {
-      const int tile = __popc(all & ((1u << lane) - 1u));
-      here.adapter[tile] = i;
-      here.tokens[tile] = same;
+    const int both = first ? n | (n + p.tile - 1) / p.tile << 16 : 0;
+    int scan = both;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xFFFFFFFFu, scan, o);
+      if (lane >= o) scan += v;
     }
-    if (lane == 0) here.tiles = __popc(all);
+    const int before = scan - both, start = __shfl_sync(0xFFFFFFFFu, before & 0xFFFF, __ffs(same) - 1);
+    if (i >= 0) few.sorted[start + __popc(same & ((1u << lane) - 1u))] = lane;
+    if (first)
+      for (int j = 0; j * p.tile < n; ++j) few.tiles[(before >> 16) + j] = {i, start + j * p.tile, min(n - j * p.tile, p.tile), 0};
+    if (lane == 31) few.tiles_used = scan >> 16;
   }
   __syncthreads();
-  return here.tiles;
+  return {few.tiles_used, few.tiles, few.sorted};
 }
-// the tile's adapter, number of tokens, and tokens (the last one again behind it); the block's threads together, between two barriers
-__device__ __forceinline__ LoraTile lora_tile(const LoraPlan& p, const LoraHere& here, int index, int (&s_token)[kLoraTile]) {
-  LoraTile tile;
-  const int tid = threadIdx.x;
-  if (p.tiles_used) {
-    tile = p.tiles[index];
-    if (tid < kLoraTile) s_token[tid] = p.sorted[tile.first + min(tid, tile.count - 1)];
+
+// where a wait has run out: the last copies are waited for, as far as they come
+__device__ __forceinline__ void lora_drain(uint32_t bars, int stages, int made, uint32_t stage, uint32_t phase) {
+  for (int i = 0; i < min(made, stages); ++i) {
+    phase ^= stage == 0;
+    stage = stage == 0 ? stages - 1 : stage - 1;
+    for (int k = 0; k < 4096 && !ptx::mbar_try_wait(bars + 8 * stage, phase); ++k) __nanosleep(64);
+  }
+}
+__host__ __device__ constexpr int lora_columns(int tokens) { return (tokens + 15) / 16 * 16; }
+
+// a x of a tile's tokens over a part of k: ranks are the rows of the product, tokens its columns.  A step is 64 values of k of up to 128 ranks and the tile's tokens.
+constexpr int kLoraMostStages = 8;
+constexpr int kLoraDownWarps = 6;  // copies, MMAs, four of results
+struct LoraDownShape {
+  int rows, row_bytes, stage, stages;  // ranks of a block; bytes of them and of a stage
+  LoraDownShape(int rank, int tile, int smem) {
+    rows = rank < 128 ? rank : 128;
+    row_bytes = rows * 128;
+    stage = row_bytes + tile * 128;
+    stages = (smem - 16384) / stage;
+    if (stages > kLoraMostStages) stages = kLoraMostStages;
+  }
+};
+
+template <int TILE>
+__global__ void __launch_bounds__(32 * kLoraDownWarps, 2)
+    lora_down_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_x, const b200q_lora_args a, const LoraPlan p, const LoraDownShape d) {
+  extern __shared__ uint8_t s_raw[];
+  uint8_t* const s_ring = s_raw + (0u - ptx::smem_u32(s_raw) & 1023u);
+  __shared__ __align__(8) uint64_t s_bars[2 * kLoraMostStages + 4];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_abort;
+  __shared__ LoraFew s_few;
+  constexpr int kTmem = 2 * TILE < 32 ? 32 : 2 * TILE;
+  const int tid = threadIdx.x, lane = tid & 31, warp = ptx::uniform_warp_index();
+  const uint32_t ring = ptx::smem_u32(s_ring), bar_full = ptx::smem_u32(s_bars), bar_empty = bar_full + 8 * kLoraMostStages;
+  const uint32_t bar_done = bar_empty + 8 * kLoraMostStages, bar_free = bar_done + 16;
+  if (tid == 0) {
+    for (int i = 0; i < d.stages; ++i) {
+      ptx::mbar_init(bar_full + 8 * i, 1);
+      ptx::mbar_init(bar_empty + 8 * i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      ptx::mbar_init(bar_done + 8 * i, 1);
+      ptx::mbar_init(bar_free + 8 * i, 4);
+    }
+    s_abort = 0;
+    ptx::fence_barrier_init();
+    ptx::tma_prefetch_desc(&map_a);
+    ptx::tma_prefetch_desc(&map_x);
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc(ptx::smem_u32(&s_tmem), kTmem);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  pdl_enter();
+  const LoraView view = lora_view(a, p, s_few);
+  const int blocks = ((int)a.rank + 127) / 128, items = view.tiles_used * p.splits * blocks;
+  bool ok = true;
+  // item: block of ranks, part of k, tile
+  struct Item {
+    int block, k0, k1, part;
+    LoraTile tile;
+  };
+  auto item_of = [&](int i) {
+    Item it;
+    it.block = blocks == 1 ? 0 : i & 1;  // (at most two)
+    const int rest = blocks == 1 ? i : i >> 1;
+    const int tile = rest / p.splits;
+    it.part = rest - tile * p.splits;
+    it.k0 = it.part * p.part_steps;
+    it.k1 = min(it.k0 + p.part_steps, p.steps);
+    it.tile = view.tiles[tile];
+    return it;
+  };
+  if (warp == 0) {
+    uint32_t stage = 0, phase = 0;
+    int made = 0;
+    for (int i = blockIdx.x; i < items && ok; i += gridDim.x) {
+      const Item it = item_of(i);
+      const int eights = (it.tile.count + 7) / 8;
+      int rows[4] = {};
+      if (lane < 2 * eights) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) rows[r] = view.sorted[it.tile.first + min(4 * lane + r, it.tile.count - 1)];
+      }
+      for (int k = it.k0; k < it.k1; ++k) {
+        ok = ptx::mbar_wait_uniform(bar_empty + 8 * stage, phase ^ 1, &s_abort, p.status, kLoraErrCopy);
+        if (!ok) break;
+        const uint32_t bar = bar_full + 8 * stage, dst = ring + stage * d.stage;
+        if (ptx::elect_one()) {
+          ptx::mbar_arrive_expect_tx(bar, d.row_bytes + eights * 1024);
+          ptx::tma_load_3d(dst, &map_a, bar, 64 * k, 128 * it.block, it.tile.adapter);
+        }
+        __syncwarp();
+        if (lane < 2 * eights) layer_gather4(dst + d.row_bytes + 512 * lane, &map_x, bar, 64 * k, rows);
+        __syncwarp();
+        ++made;
+        if (++stage == (uint32_t)d.stages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+    }
+    if (!ok) lora_drain(bar_full, d.stages, made, stage, phase);
+  } else if (warp == 1) {
+    uint32_t stage = 0, phase = 0;
+    int n = 0;
+    const uint64_t a0 = ptx::smem_desc_k_sw128(ring), b0 = ptx::smem_desc_k_sw128(ring + d.row_bytes);
+    for (int i = blockIdx.x; i < items && ok; i += gridDim.x) {
+      const Item it = item_of(i);
+      if (it.k0 >= it.k1) continue;
+      const uint32_t acc = n & 1, out = tmem + acc * TILE, idesc = ptx::umma_idesc(1, 1, 128, lora_columns(it.tile.count));
+      ok = ptx::mbar_wait_uniform(bar_free + 8 * acc, ((n >> 1) & 1) ^ 1, &s_abort, p.status, kLoraErrMma);
+      if (!ok) break;
+      ++n;
+      ptx::tc_fence_after();
+      for (int k = it.k0; k < it.k1; ++k) {
+        ok = ptx::mbar_wait_uniform(bar_full + 8 * stage, phase, &s_abort, p.status, kLoraErrMma);
+        if (!ok) break;
+        ptx::tc_fence_after();
+        if (ptx::elect_one()) {
+          const uint64_t off = stage * (uint32_t)(d.stage >> 4);
+          ptx::umma_f16_x4(out, a0 + off, b0 + off, idesc, k != it.k0, 2, 2);
+          ptx::umma_commit(bar_empty + 8 * stage);
+          if (k + 1 == it.k1) ptx::umma_commit(bar_done + 8 * acc);
+        }
+        __syncwarp();
+        if (++stage == (uint32_t)d.stages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+    }
   } else {
-    const uint32_t mask = here.tokens[index];
-    tile = {here.adapter[index], 0, __popc(mask), 0};
-    if (tid < kLoraTile) {
-      const int last = 31 - __clz((int)mask);
-      if (mask >> tid & 1u) s_token[__popc(mask & ((1u << tid) - 1u))] = tid;
-      if (tid >= tile.count) s_token[tid] = last;
+    int n = 0;
+    const int quarter = warp & 3;
+    for (int i = blockIdx.x; i < items && ok; i += gridDim.x) {
+      const Item it = item_of(i);
+      const int r = 128 * it.block + 32 * quarter + lane;
+      const bool none = it.k0 >= it.k1;  // (a part behind the end of k)
+      const uint32_t acc = n & 1, in = tmem + acc * TILE + ((uint32_t)(32 * quarter) << 16);
+      if (!none) {
+        ok = ptx::mbar_wait_uniform(bar_done + 8 * acc, (n >> 1) & 1, &s_abort, p.status, kLoraErrResults);
+        if (!ok) break;
+        ++n;
+        ptx::tc_fence_after();
+      }
+      for (int j0 = 0; j0 < it.tile.count; j0 += 8) {
+        float v[8] = {};
+        if (!none) {
+          layer_tmem_ld8(in + j0, v);
+          ptx::tmem_ld_wait();
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (j0 + j < it.tile.count && r < a.rank) p.low[((int64_t)it.part * a.tokens + view.sorted[it.tile.first + j0 + j]) * a.rank + r] = v[j];
+      }
+      if (!none) {
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(bar_free + 8 * acc);
+      }
     }
   }
-  return tile;
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (warp == 1) ptx::tmem_dealloc(tmem, kTmem);
 }
 
-// a x of a tile's tokens over a part of k: ranks are the rows of the product, tokens its columns.  Each warp has every eighth 64 bytes of the rows of both, so
-// that nothing is loaded twice; the warps' sums are added in shared memory.
-template <int MT>  // tiles of 16 ranks
-__global__ void __launch_bounds__(kLoraThreads) lora_down_kernel(const b200q_lora_args a, const LoraPlan p) {
-  constexpr int kWarps = kLoraThreads / 32, kRanks = 16 * MT, kPitch = kRanks + 4, NT = kLoraTile / 8;
-  constexpr int kBatch = MT <= 2 ? 4 : MT == 4 ? 2 : 1;  // steps of 32 values of k on their way together
-  extern __shared__ float s_sum[];                       // [warps][tokens][kPitch]
-  __shared__ int s_token[kLoraTile];
-  __shared__ LoraHere s_here;
-  pdl_enter();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const int blocks = ((int)a.rank + kRanks - 1) / kRanks, items = lora_tiles(a, p, s_here) * p.splits * blocks;
-  for (int item = blockIdx.x; item < items; item += gridDim.x) {
-    const int block = item % blocks, part = item / blocks % p.splits;
-    __syncthreads();  // (the item before this one is done with shared memory)
-    const LoraTile tile = lora_tile(p, s_here, item / blocks / p.splits, s_token);
-    __syncthreads();
-    const __nv_bfloat16* x[NT];
-    const __nv_bfloat16* rows = static_cast<const __nv_bfloat16*>(a.a) + tile.adapter * a.a_stride + (int64_t)(block * kRanks + g) * a.a_row_stride + 8 * t;
+// y += b (scale a x): columns of y are the rows of the product, tokens its columns.  A tile's terms of a x lie in shared memory and meet one block of 128 columns
+// after the other.  A warp has 32 columns and half of the tokens; it turns its results around in shared memory, eight tokens at a time, so that a lane has 16 bytes of
+// a row of y, and has always asked for the next block's.  (A column and two bytes per lane, 16 of them asked for at a time, was 150 us where this is 45: 4096 tokens of
+// 14336 columns.)
+constexpr int kLoraUpWarps = 10;  // copies, MMAs, eight of results
+struct LoraUpShape {
+  int chunks, terms_bytes, stages, parts, blocks;  // chunks of 64 ranks; bytes of the terms; parts of n, and blocks of 128 columns of a part
+};
+
+template <typename Y>
+__device__ __forceinline__ uint4 lora_load16(const Y* p, bool whole) {
+  if (whole) return *reinterpret_cast<const uint4*>(p);
+  Y v[16 / sizeof(Y)];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) x[n] = static_cast<const __nv_bfloat16*>(a.x) + s_token[8 * n + g] * a.x_stride + 8 * t;
-    const int ranks = (int)a.rank - block * kRanks - g, nt = (tile.count + 7) / 8;  // (of this lane's first row on)
-    float acc[MT][NT][4];
+  for (int i = 0; i < (int)(16 / sizeof(Y)); ++i) v[i] = p[i];
+  return *reinterpret_cast<const uint4*>(v);
+}
+template <typename Y>
+__device__ __forceinline__ void lora_store16(Y* p, const uint4& w, bool whole) {
+  if (whole) {
+    *reinterpret_cast<uint4*>(p) = w;
+  } else {
+    const Y* v = reinterpret_cast<const Y*>(&w);
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[m][n][i] = 0.f;
-    const int64_t end = min((int64_t)(part + 1) * p.slice, a.k);
-    const uint4 zero = make_uint4(0, 0, 0, 0);
-    for (int64_t k0 = (int64_t)part * p.slice + 32 * warp; k0 < end; k0 += 32 * kWarps * kBatch) {
-      uint4 ra[kBatch][MT][2], rx[kBatch][NT];
-#pragma unroll
-      for (int b = 0; b < kBatch; ++b) {
-        const int64_t k = k0 + 32 * kWarps * b;
-        const bool in = k + 8 * t < end;
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) ra[b][m][h] = in && 16 * m + 8 * h < ranks ? __ldg(reinterpret_cast<const uint4*>(rows + (16 * m + 8 * h) * a.a_row_stride + k)) : zero;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) rx[b][n] = in && n < nt ? __ldg(reinterpret_cast<const uint4*>(x[n] + k)) : zero;
-      }
-#pragma unroll
-      for (int b = 0; b < kBatch; ++b)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          if (n >= nt) break;
-#pragma unroll
-          for (int m = 0; m < MT; ++m) {
-            lora_mma(acc[m][n], ra[b][m][0].x, ra[b][m][1].x, ra[b][m][0].y, ra[b][m][1].y, rx[b][n].x, rx[b][n].y);
-            lora_mma(acc[m][n], ra[b][m][0].z, ra[b][m][1].z, ra[b][m][0].w, ra[b][m][1].w, rx[b][n].z, rx[b][n].w);
-          }
-        }
-    }
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      if (n >= nt) break;
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s_sum[(warp * kLoraTile + 8 * n + 2 * t + (i & 1)) * kPitch + 16 * m + g + 8 * (i >> 1)] = acc[m][n][i];
-    }
-    __syncthreads();
-    for (int i = tid; i < tile.count * kRanks; i += kLoraThreads) {
-      const int j = i / kRanks, r = i % kRanks;
-      if (block * kRanks + r >= a.rank) continue;
-      float sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) sum += s_sum[(w * kLoraTile + j) * kPitch + r];
-      p.low[((int64_t)part * a.tokens + s_token[j]) * a.rank + block * kRanks + r] = sum;
-    }
+    for (int i = 0; i < (int)(16 / sizeof(Y)); ++i) p[i] = v[i];
   }
 }
 
-// y += b (scale a x): tokens are the rows of the product, 32 values of y of a warp its columns, of which a lane has 8 neighbours in four rows.  The values of y for
-// the next step are on their way while this one's products are formed.
-template <typename Y, bool WIDE>  // WIDE: ranks 32 at a time, in 16 bytes a lane; else 16 at a time
-__global__ void __launch_bounds__(kLoraThreads, 2) lora_up_kernel(const b200q_lora_args a, const LoraPlan p, int parts, int width) {
-  constexpr int kTerms = sizeof(Y) == 4 ? 3 : 2, kWarps = kLoraThreads / 32, kStep = WIDE ? 32 : 16, kHalves = WIDE ? 2 : 1;
-  constexpr int kY = sizeof(Y) == 4 ? 2 : 1, kPer = 16 / sizeof(Y);  // 16-byte pieces of a lane's 8 values; values of a piece
-  extern __shared__ __align__(16) uint8_t s_raw[];                   // [terms][tokens][pitch] of bf16
-  __shared__ int s_token[kLoraTile];
-  __shared__ LoraHere s_here;
-  pdl_enter();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const int rank = (int)a.rank, steps = (rank + kStep - 1) / kStep, pitch = steps * kStep + 8, items = lora_tiles(a, p, s_here) * parts;
-  __nv_bfloat16* const s_low = reinterpret_cast<__nv_bfloat16*>(s_raw);
-  for (int item = blockIdx.x; item < items; item += gridDim.x) {
-    const int part = item % parts;
-    __syncthreads();
-    const LoraTile tile = lora_tile(p, s_here, item / parts, s_token);
-    const float scale = a.scales ? a.scales[tile.adapter] : 1.f;
-    __syncthreads();
-    const int n_end = (int)min((int64_t)(part + 1) * width, a.n);
-    int n0 = part * width + 32 * warp;
-    Y* rows[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) rows[i] = static_cast<Y*>(a.y) + s_token[g + 8 * i] * a.y_stride + 8 * t;
-    uint4 next[4][kY];
-    auto ask = [&](int n) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int c = 0; c < kY; ++c)
-          if (g + 8 * i < tile.count && n < n_end && n + 8 * t + c * kPer < a.n) next[i][c] = *reinterpret_cast<const uint4*>(rows[i] + n + c * kPer);
-    };
-    ask(n0);
-    for (int i = tid; i < kLoraTile * steps * kStep; i += kLoraThreads) {
-      const int j = i / (steps * kStep), r = i - j * (steps * kStep);
-      float v = 0.f;
-      if (j < tile.count && r < rank) {
-        for (int s = 0; s < p.splits; ++s) v += __ldcg(p.low + ((int64_t)s * a.tokens + s_token[j]) * rank + r);
-        v *= scale;
-      }
-#pragma unroll
-      for (int c = 0; c < kTerms; ++c) {
-        const __nv_bfloat16 hi = __float2bfloat16_rn(v);
-        s_low[(c * kLoraTile + j) * pitch + r] = hi;
-        v -= __bfloat162float(hi);
-      }
+template <typename Y, int TILE>
+__global__ void __launch_bounds__(32 * kLoraUpWarps, sizeof(Y) * TILE == 512 ? 1 : 2) lora_up_kernel(const __grid_constant__ CUtensorMap map_b, const b200q_lora_args a, const LoraPlan p, const LoraUpShape d) {
+  constexpr int kTerms = sizeof(Y) == 4 ? 3 : 2, kStage = 128 * 128, kHalf = TILE / 2;
+  constexpr int kPer = 16 / sizeof(Y), kLanes = 32 / kPer, kRows = 32 / kLanes, kPieces = kHalf / kRows;  // values of a lane's piece of a row; lanes of a row
+  constexpr int kPitch = 36;                                                                             // of eight tokens' results, 32 of them each
+  extern __shared__ uint8_t s_raw[];
+  uint8_t* const s_terms = s_raw + (0u - ptx::smem_u32(s_raw) & 1023u);  // [terms][chunks][tokens][128 bytes], then the ring
+  __shared__ __align__(8) uint64_t s_bars[2 * kLoraMostStages + 6];
+  __shared__ uint32_t s_tmem;
+  __shared__ __align__(16) float s_turn[8][8 * kPitch];
+  __shared__ int s_abort;
+  __shared__ LoraFew s_few;
+  constexpr int kTmem = 2 * TILE < 32 ? 32 : 2 * TILE;
+  const int tid = threadIdx.x, lane = tid & 31, warp = ptx::uniform_warp_index();
+  const uint32_t terms = ptx::smem_u32(s_terms), ring = terms + d.terms_bytes;
+  const uint32_t bar_full = ptx::smem_u32(s_bars), bar_empty = bar_full + 8 * kLoraMostStages, bar_done = bar_empty + 8 * kLoraMostStages, bar_free = bar_done + 16;
+  const uint32_t bar_terms = bar_free + 16, bar_used = bar_terms + 8;
+  if (tid == 0) {
+    for (int i = 0; i < d.stages; ++i) {
+      ptx::mbar_init(bar_full + 8 * i, 1);
+      ptx::mbar_init(bar_empty + 8 * i, 1);
     }
-    __syncthreads();
-    const bool two = tile.count > 16;
-    // column g of product c is y's n0 + 8 (g / 2) + 2 c + g % 2
-    const int column = 8 * (g >> 1) + (g & 1);
-    const __nv_bfloat16* const b0 = static_cast<const __nv_bfloat16*>(a.b) + tile.adapter * a.b_stride + column * a.b_row_stride + (WIDE ? 8 : 4) * t;
-    for (; n0 < n_end; n0 += 32 * kWarps) {
-      uint4 now[4][kY];
+    for (int i = 0; i < 2; ++i) {
+      ptx::mbar_init(bar_done + 8 * i, 1);
+      ptx::mbar_init(bar_free + 8 * i, 8);
+    }
+    ptx::mbar_init(bar_terms, 8);
+    ptx::mbar_init(bar_used, 1);
+    s_abort = 0;
+    ptx::fence_barrier_init();
+    ptx::tma_prefetch_desc(&map_b);
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc(ptx::smem_u32(&s_tmem), kTmem);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  pdl_enter();
+  const LoraView view = lora_view(a, p, s_few);
+  const int items = view.tiles_used * d.parts, n_blocks = (int)((a.n + 127) / 128);
+  bool ok = true;
+  if (warp == 0) {
+    uint32_t stage = 0, phase = 0;
+    int made = 0;
+    for (int i = blockIdx.x; i < items && ok; i += gridDim.x) {
+      const int tile = i / d.parts, part = i - tile * d.parts, adapter = view.tiles[tile].adapter;
+      for (int n = part * d.blocks; n < min((part + 1) * d.blocks, n_blocks) && ok; ++n)
+        for (int c = 0; c < d.chunks; ++c) {
+          ok = ptx::mbar_wait_uniform(bar_empty + 8 * stage, phase ^ 1, &s_abort, p.status, kLoraErrCopy);
+          if (!ok) break;
+          if (ptx::elect_one()) {
+            ptx::mbar_arrive_expect_tx(bar_full + 8 * stage, kStage);
+            ptx::tma_load_3d(ring + stage * kStage, &map_b, bar_full + 8 * stage, 64 * c, 128 * n, adapter);
+          }
+          __syncwarp();
+          ++made;
+          if (++stage == (uint32_t)d.stages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+    }
+    if (!ok) lora_drain(bar_full, d.stages, made, stage, phase);
+  } else if (warp == 1) {
+    uint32_t stage = 0, phase = 0;
+    int done = 0, item = 0;
+    const uint64_t a0 = ptx::smem_desc_k_sw128(ring), b0 = ptx::smem_desc_k_sw128(terms);
+    for (int i = blockIdx.x; i < items && ok; i += gridDim.x, ++item) {
+      const int tile = i / d.parts, part = i - tile * d.parts;
+      const uint32_t idesc = ptx::umma_idesc(1, 1, 128, lora_columns(view.tiles[tile].count));
+      ok = ptx::mbar_wait_uniform(bar_terms, item & 1, &s_abort, p.status, kLoraErrMma);
+      for (int n = part * d.blocks; n < min((part + 1) * d.blocks, n_blocks) && ok; ++n, ++done) {
+        const uint32_t acc = done & 1, out = tmem + acc * TILE;
+        ok = ptx::mbar_wait_uniform(bar_free + 8 * acc, ((done >> 1) & 1) ^ 1, &s_abort, p.status, kLoraErrMma);
+        if (!ok) break;
+        ptx::tc_fence_after();
+        for (int c = 0; c < d.chunks; ++c) {
+          ok = ptx::mbar_wait_uniform(bar_full + 8 * stage, phase, &s_abort, p.status, kLoraErrMma);
+          if (!ok) break;
+          ptx::tc_fence_after();
+          if (ptx::elect_one()) {
+            for (int e = 0; e < kTerms; ++e)
+              ptx::umma_f16_x4(out, a0 + stage * (uint32_t)(kStage >> 4), b0 + (e * d.chunks + c) * (TILE * 128 >> 4), idesc, c + e != 0, 2, 2);
+            ptx::umma_commit(bar_empty + 8 * stage);
+            if (c + 1 == d.chunks) ptx::umma_commit(bar_done + 8 * acc);
+          }
+          __syncwarp();
+          if (++stage == (uint32_t)d.stages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      if (ok && ptx::elect_one()) ptx::umma_commit(bar_used);
+      __syncwarp();
+    }
+  } else {
+    int done = 0, item = 0;
+    const int wt = tid - 64, quarter = warp & 3, half = (warp - 2) >> 2, my_row = lane / kLanes, my_column = 32 * quarter + lane % kLanes * kPer;
+    float* const turn = s_turn[warp - 2];
+    const bool whole = reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && (a.tokens == 1 || a.y_stride % kPer == 0);
+    for (int i = blockIdx.x; i < items; i += gridDim.x, ++item) {  // (all eight warps come to each item's barrier, whatever became of their waits)
+      const int index = i / d.parts, part = i - index * d.parts, n_end = min((part + 1) * d.blocks, n_blocks);
+      const LoraTile tile = view.tiles[index];
+      const int first = tile.first + kHalf * half, count = min(tile.count - kHalf * half, kHalf);  // of this half
+      Y* rows[kPieces];
+      uint4 old[kPieces];
+      auto ask = [&](int c, int n) {
+        if (c * kRows + my_row < count && n < n_end && 128 * n + my_column < a.n) old[c] = lora_load16(rows[c] + 128 * n, whole);
+      };
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int c = 0; c < kPieces; ++c) {
+        rows[c] = static_cast<Y*>(a.y) + my_column;
+        if (c * kRows + my_row < count) rows[c] += view.sorted[first + c * kRows + my_row] * a.y_stride;
+      }
 #pragma unroll
-        for (int c = 0; c < kY; ++c) now[i][c] = next[i][c];
-      ask(n0 + 32 * kWarps);
-      float acc[2][4][4];
-#pragma unroll
-      for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[m][c][i] = 0.f;
-      const __nv_bfloat16* b = b0 + n0 * a.b_row_stride;
-      for (int k = 0; k < steps; ++k) {
-        uint32_t rb[4][2 * kHalves];
-        const bool in = k * kStep + (WIDE ? 8 : 4) * t < rank;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const bool there = in && n0 + column + 2 * c < a.n;
-          if constexpr (WIDE) {
-            const uint4 v = there ? __ldg(reinterpret_cast<const uint4*>(b + 2 * c * a.b_row_stride + k * kStep)) : make_uint4(0, 0, 0, 0);
-            rb[c][0] = v.x; rb[c][1] = v.y; rb[c][2] = v.z; rb[c][3] = v.w;
-          } else {
-            const uint2 v = there ? __ldg(reinterpret_cast<const uint2*>(b + 2 * c * a.b_row_stride + k * kStep)) : make_uint2(0, 0);
-            rb[c][0] = v.x; rb[c][1] = v.y;
+      for (int c = 0; c < kPieces; ++c) ask(c, part * d.blocks);
+      ok = ok && ptx::mbar_wait_uniform(bar_used, (item & 1) ^ 1, &s_abort, p.status, kLoraErrResults);  // (the products with the terms before are done)
+      const float scale = a.scales ? a.scales[tile.adapter] : 1.f;
+      const int pieces = 8 * d.chunks;  // of eight ranks
+      for (int q = wt; ok && q < tile.count * pieces; q += 256) {
+        const int j = q / pieces, r = 8 * (q - j * pieces);
+        float v[8] = {};
+        if (r < a.rank) {
+          const float* low = p.low + (int64_t)view.sorted[tile.first + j] * a.rank + r;
+#pragma unroll 4
+          for (int s = 0; s < p.splits; ++s) {
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(low + s * a.tokens * a.rank)), y = __ldcg(reinterpret_cast<const float4*>(low + s * a.tokens * a.rank) + 1);
+            v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+            v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
           }
         }
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          if (m == 1 && !two) break;
+        for (int c = 0; c < 8; ++c) v[c] *= scale;
 #pragma unroll
-          for (int e = 0; e < kTerms; ++e) {
-            const __nv_bfloat16* low = s_low + (e * kLoraTile + 16 * m + g) * pitch + k * kStep + (WIDE ? 8 : 4) * t;
-            uint32_t lo[2 * kHalves], hi[2 * kHalves];
-            if constexpr (WIDE) {
-              const uint4 u = *reinterpret_cast<const uint4*>(low), v = *reinterpret_cast<const uint4*>(low + 8 * pitch);
-              lo[0] = u.x; lo[1] = u.y; lo[2] = u.z; lo[3] = u.w;
-              hi[0] = v.x; hi[1] = v.y; hi[2] = v.z; hi[3] = v.w;
+        for (int e = 0; e < kTerms; ++e) {
+          uint32_t w[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            w[c] = pack_bf16x2(v[2 * c], v[2 * c + 1]);
+            v[2 * c] -= __uint_as_float(w[c] << 16);
+            v[2 * c + 1] -= __uint_as_float(w[c] & 0xFFFF0000u);
+          }
+          *reinterpret_cast<uint4*>(s_terms + ((e * d.chunks + r / 64) * TILE + j) * 128 + (((r / 8 & 7) ^ (j & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+      ptx::fence_proxy_async_smem();
+      ok = layer_bar_and(1, 256, ok);
+      if (!ok) break;
+      if (lane == 0) ptx::mbar_arrive(bar_terms);
+      for (int n = part * d.blocks; n < n_end && ok; ++n, ++done) {
+        const uint32_t acc = done & 1, in = tmem + acc * TILE + kHalf * half + ((uint32_t)(32 * quarter) << 16);
+        ok = ptx::mbar_wait_uniform(bar_done + 8 * acc, (done >> 1) & 1, &s_abort, p.status, kLoraErrResults);
+        if (!ok) break;
+        ptx::tc_fence_after();
+        const bool there = 128 * n + my_column < a.n;
+#pragma unroll
+        for (int j0 = 0; j0 < kHalf; j0 += 8) {
+          if (j0 >= count) break;
+          float v[8];
+          layer_tmem_ld8(in + j0, v);
+          ptx::tmem_ld_wait();
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 8; ++j) turn[j * kPitch + lane] = v[j];
+          __syncwarp();
+#pragma unroll
+          for (int c = j0 / kRows; c < (j0 + 8) / kRows; ++c) {
+            const float4* from = reinterpret_cast<const float4*>(turn + (c * kRows - j0 + my_row) * kPitch + lane % kLanes * kPer);
+            uint4 w;
+            const float4 x = from[0];
+            if constexpr (sizeof(Y) == 4) {
+              w = make_uint4(__float_as_uint(__uint_as_float(old[c].x) + x.x), __float_as_uint(__uint_as_float(old[c].y) + x.y),
+                             __float_as_uint(__uint_as_float(old[c].z) + x.z), __float_as_uint(__uint_as_float(old[c].w) + x.w));
             } else {
-              const uint2 u = *reinterpret_cast<const uint2*>(low), v = *reinterpret_cast<const uint2*>(low + 8 * pitch);
-              lo[0] = u.x; lo[1] = u.y;
-              hi[0] = v.x; hi[1] = v.y;
+              const float4 z = from[1];
+              w.x = pack_bf16x2(__uint_as_float(old[c].x << 16) + x.x, __uint_as_float(old[c].x & 0xFFFF0000u) + x.y);
+              w.y = pack_bf16x2(__uint_as_float(old[c].y << 16) + x.z, __uint_as_float(old[c].y & 0xFFFF0000u) + x.w);
+              w.z = pack_bf16x2(__uint_as_float(old[c].z << 16) + z.x, __uint_as_float(old[c].z & 0xFFFF0000u) + z.y);
+              w.w = pack_bf16x2(__uint_as_float(old[c].w << 16) + z.z, __uint_as_float(old[c].w & 0xFFFF0000u) + z.w);
             }
-#pragma unroll
-            for (int h = 0; h < kHalves; ++h)
-#pragma unroll
-              for (int c = 0; c < 4; ++c) lora_mma(acc[m][c], lo[2 * h], hi[2 * h], lo[2 * h + 1], hi[2 * h + 1], rb[c][2 * h], rb[c][2 * h + 1]);
+            if (there && c * kRows + my_row < count) lora_store16(rows[c] + 128 * n, w, whole);
+            ask(c, n + 1);
           }
         }
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (g + 8 * i >= tile.count) continue;
-#pragma unroll
-        for (int c = 0; c < kY; ++c) {
-          if (n0 + 8 * t + c * kPer >= a.n) continue;
-          // the lane's values 2 q and 2 q + 1 are in product q
-          Y* y = rows[i] + n0 + c * kPer;
-          if constexpr (sizeof(Y) == 4) {
-            const float* v0 = acc[i >> 1][2 * c] + 2 * (i & 1);
-            const float* v1 = acc[i >> 1][2 * c + 1] + 2 * (i & 1);
-            *reinterpret_cast<float4*>(y) = make_float4(__uint_as_float(now[i][c].x) + v0[0], __uint_as_float(now[i][c].y) + v0[1],
-                                                        __uint_as_float(now[i][c].z) + v1[0], __uint_as_float(now[i][c].w) + v1[1]);
-          } else {
-            const uint32_t u[4] = {now[i][c].x, now[i][c].y, now[i][c].z, now[i][c].w};
-            uint32_t w[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const float* v = acc[i >> 1][q] + 2 * (i & 1);
-              w[q] = pack_bf16x2(__uint_as_float(u[q] << 16) + v[0], __uint_as_float(u[q] & 0xFFFF0000u) + v[1]);
-            }
-            *reinterpret_cast<uint4*>(y) = make_uint4(w[0], w[1], w[2], w[3]);
-          }
-        }
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(bar_free + 8 * acc);
       }
     }
   }
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (warp == 1) ptx::tmem_dealloc(tmem, kTmem);
 }
 
 // ---------------------------------------------------------------------------- host
 size_t lora_workspace_bytes_impl(int64_t tokens, int64_t k, int64_t n, int64_t rank, int64_t adapters) {
   (void)n;
-  return LoraSpace(tokens, rank, lora_splits(tokens, k, adapters)).bytes;
+  size_t bytes = 0;
+  for (int tile : {16, 128}) {  // (which one depends on y's type)
+    const size_t b = LoraSpace(tokens, rank, lora_splits(tokens, k, adapters, tile)).bytes;
+    if (b > bytes) bytes = b;
+  }
+  return bytes;
 }
 
 static bool lora_fits_tensor_cores(const b200q_lora_args& a) {
   if (a.force_plain || a.rank % 8 || a.k % 8 || a.n % 8) return false;
-  const bool many = a.tokens > 1;
-  if (many && (a.x_stride % 8 || a.y_stride % 8)) return false;
-  if (a.adapters > 1 && (a.a_stride % 8 || a.b_stride % 8)) return false;
-  if ((a.rank > 1 && a.a_row_stride % 8) || (a.n > 1 && a.b_row_stride % 8)) return false;
-  for (const void* p : {a.x, static_cast<const void*>(a.y), a.a, a.b})
+  if (a.tokens > 1 && (a.x_stride % 8 || a.x_stride < a.k)) return false;
+  if (a.adapters > 1 && (a.a_stride % 8 || a.b_stride % 8 || a.a_stride <= 0 || a.b_stride <= 0)) return false;
+  if ((a.rank > 1 && (a.a_row_stride % 8 || a.a_row_stride < a.k)) || (a.n > 1 && (a.b_row_stride % 8 || a.b_row_stride < a.rank))) return false;
+  for (const void* p : {a.x, a.a, a.b})
     if (reinterpret_cast<uintptr_t>(p) % 16) return false;
   return true;
+}
+
+// bf16 [planes][rows][depth] in boxes of 64 values of `box` rows
+static int lora_map(CUtensorMap* map, const void* base, int64_t depth, int64_t rows, int64_t planes, int64_t row_stride, int64_t plane_stride, int box_rows, int rank) {
+  EncodeTiledFn enc = get_encode_fn();
+  if (!enc) return B200Q_ERR_CUDA;
+  const cuuint64_t dims[3] = {(cuuint64_t)depth, (cuuint64_t)rows, (cuuint64_t)planes};
+  const cuuint64_t strides[2] = {(cuuint64_t)(rows > 1 ? row_stride : (depth + 7) / 8 * 8) * 2, (cuuint64_t)(planes > 1 ? plane_stride : (depth + 7) / 8 * 8) * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1}, step[3] = {1, 1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? B200Q_OK : B200Q_ERR_UNSUPPORTED;
 }
 
 static int lora_ready(const void* kernel, std::atomic<int> (&done)[kMaxDevices], int smem) {
@@ -432,33 +640,48 @@ static int lora_ready(const void* kernel, std::atomic<int> (&done)[kMaxDevices],
   return B200Q_OK;
 }
 
-template <int MT>
+constexpr int kLoraShared = 100 * 1024;  // of a CTA where two share an SM, beside what its kernel has of its own
+
+template <int TILE>
 static int lora_launch_down(const b200q_lora_args& a, const LoraPlan& p, int64_t tiles, cudaStream_t st) {
-  constexpr int kSmem = (int)sizeof(float) * (kLoraThreads / 32) * kLoraTile * (16 * MT + 4);
   static std::atomic<int> done[kMaxDevices];
-  if (int rc = lora_ready(reinterpret_cast<const void*>(lora_down_kernel<MT>), done, kSmem)) return rc;
-  const int64_t items = tiles * p.splits * ((a.rank + 16 * MT - 1) / (16 * MT)), most = 4 * kNumSMs;
-  launch_dependent(lora_down_kernel<MT>, dim3((unsigned)(items < most ? items : most)), dim3(kLoraThreads), kSmem, st, a, p);
+  if (int rc = lora_ready(reinterpret_cast<const void*>(lora_down_kernel<TILE>), done, kLoraShared)) return rc;
+  const LoraDownShape d((int)a.rank, TILE, kLoraShared - 1024);
+  CUtensorMap map_a, map_x;
+  if (int rc = lora_map(&map_a, a.a, a.k, a.rank, a.adapters, a.a_row_stride, a.a_stride, d.rows, 3)) return rc;
+  if (int rc = lora_map(&map_x, a.x, a.k, a.tokens, 1, a.x_stride, 0, 1, 2)) return rc;
+  const int64_t items = tiles * p.splits * ((a.rank + 127) / 128), most = 2 * kNumSMs;
+  // (the rows behind a block's ranks, which the product reads too and whose results nobody looks at, are within the allocation)
+  launch_dependent(lora_down_kernel<TILE>, dim3((unsigned)(items < most ? items : most)), dim3(32 * kLoraDownWarps), (size_t)d.stages * d.stage + 16384 + 1024, st, map_a, map_x, a,
+                   p, d);
   B200Q_LAUNCH_CHECK();
   return B200Q_OK;
 }
-template <typename Y, bool WIDE>
+template <typename Y, int TILE>
 static int lora_launch_up(const b200q_lora_args& a, const LoraPlan& p, int64_t tiles, cudaStream_t st) {
-  constexpr int kTerms = sizeof(Y) == 4 ? 3 : 2, kStep = WIDE ? 32 : 16;
-  constexpr int kMost = 2 * kTerms * kLoraTile * ((int)kLoraMaxRank + 8);
+  constexpr int kTerms = sizeof(Y) == 4 ? 3 : 2, kMost = 214 * 1024;
   static std::atomic<int> done[kMaxDevices];
-  if (int rc = lora_ready(reinterpret_cast<const void*>(lora_up_kernel<Y, WIDE>), done, kMost)) return rc;
-  const int64_t most_parts = (a.n + 255) / 256, wanted = (4 * kNumSMs + tiles - 1) / tiles, parts = wanted < most_parts ? wanted : most_parts;
-  const int64_t width = ((a.n + parts - 1) / parts + 255) / 256 * 256, used = (a.n + width - 1) / width;
-  const int64_t items = tiles * used, most = 4 * kNumSMs;
-  const size_t smem = (size_t)(2 * kTerms * kLoraTile) * ((a.rank + kStep - 1) / kStep * kStep + 8);
-  launch_dependent(lora_up_kernel<Y, WIDE>, dim3((unsigned)(items < most ? items : most)), dim3(kLoraThreads), smem, st, a, p, (int)used, (int)width);
+  if (int rc = lora_ready(reinterpret_cast<const void*>(lora_up_kernel<Y, TILE>), done, kMost)) return rc;
+  CUtensorMap map_b;
+  if (int rc = lora_map(&map_b, a.b, a.rank, a.n, a.adapters, a.b_row_stride, a.b_stride, 128, 3)) return rc;
+  LoraUpShape d;
+  d.chunks = (int)((a.rank + 63) / 64);
+  d.terms_bytes = kTerms * d.chunks * TILE * 128;
+  const int room = (d.terms_bytes + 2 * 16384 + 1024 <= kLoraShared ? kLoraShared : kMost) - 1024 - d.terms_bytes;
+  d.stages = room / 16384 < kLoraMostStages ? room / 16384 : kLoraMostStages;
+  const int64_t blocks = (a.n + 127) / 128, wanted = (4 * kNumSMs + tiles - 1) / tiles, parts = wanted < blocks ? wanted : blocks;
+  d.blocks = (int)((blocks + parts - 1) / parts);
+  d.parts = (int)((blocks + d.blocks - 1) / d.blocks);
+  const int64_t items = tiles * d.parts, most = 2 * kNumSMs;
+  launch_dependent(lora_up_kernel<Y, TILE>, dim3((unsigned)(items < most ? items : most)), dim3(32 * kLoraUpWarps), (size_t)d.terms_bytes + d.stages * 16384 + 1024, st, map_b, a, p,
+                   d);
   B200Q_LAUNCH_CHECK();
   return B200Q_OK;
 }
 
 static int lora_chunk_fast(const b200q_lora_args& a, cudaStream_t st) {
-  const int64_t splits = lora_splits(a.tokens, a.k, a.adapters), tiles = lora_most_tiles(a.tokens, a.adapters);
+  const int tile = lora_tile_tokens(a.tokens, a.rank, a.adapters, a.y_dtype == B200Q_F32);
+  const int64_t splits = lora_splits(a.tokens, a.k, a.adapters, tile), tiles = lora_most_tiles(a.tokens, a.adapters, tile);
   const LoraSpace space(a.tokens, a.rank, splits);
   uint8_t* w = static_cast<uint8_t*>(a.workspace);
   LoraPlan p;
@@ -467,24 +690,23 @@ static int lora_chunk_fast(const b200q_lora_args& a, cudaStream_t st) {
   p.sorted = reinterpret_cast<int*>(w + space.sorted);
   p.low = reinterpret_cast<float*>(w + space.low);
   p.splits = (int)splits;
-  p.slice = (int)(((a.k + splits - 1) / splits + 255) / 256 * 256);
-  static std::atomic<int> done[kMaxDevices];
-  constexpr int kMost = (int)sizeof(uint16_t) * (kLoraSortThreads / 32 + 1) * (int)kLoraMaxAdapters;
-  if (int rc = lora_ready(reinterpret_cast<const void*>(lora_sort_kernel), done, kMost)) return rc;
-  if (a.tokens <= kLoraTile) {
-    p.tiles_used = nullptr;  // (each CTA makes the plan for itself)
+  p.steps = (int)((a.k + 63) / 64);
+  p.part_steps = (int)((p.steps + splits - 1) / splits);
+  p.tile = tile;
+  p.status = device_status_ptr();
+  if (!p.status) return B200Q_ERR_CUDA;
+  if (a.tokens <= kLoraFew) {
+    p.tiles_used = nullptr;
   } else {
+    static std::atomic<int> done[kMaxDevices];
+    constexpr int kMost = (int)sizeof(uint16_t) * (kLoraSortThreads / 32 + 1) * (int)kLoraMaxAdapters;
+    if (int rc = lora_ready(reinterpret_cast<const void*>(lora_sort_kernel), done, kMost)) return rc;
     launch_dependent(lora_sort_kernel, dim3(1), dim3(kLoraSortThreads), sizeof(uint16_t) * (kLoraSortThreads / 32 + 1) * (size_t)a.adapters, st, a, p);
     B200Q_LAUNCH_CHECK();
   }
-  int rc;
-  if (a.rank <= 16) rc = lora_launch_down<1>(a, p, tiles, st);
-  else if (a.rank <= 32) rc = lora_launch_down<2>(a, p, tiles, st);
-  else if (a.rank <= 64) rc = lora_launch_down<4>(a, p, tiles, st);
-  else rc = lora_launch_down<8>(a, p, tiles, st);
-  if (rc) return rc;
-  if (a.y_dtype == B200Q_F32) return a.rank % 32 ? lora_launch_up<float, false>(a, p, tiles, st) : lora_launch_up<float, true>(a, p, tiles, st);
-  return a.rank % 32 ? lora_launch_up<__nv_bfloat16, false>(a, p, tiles, st) : lora_launch_up<__nv_bfloat16, true>(a, p, tiles, st);
+  if (int rc = tile == 16 ? lora_launch_down<16>(a, p, tiles, st) : lora_launch_down<128>(a, p, tiles, st)) return rc;
+  if (a.y_dtype == B200Q_F32) return tile == 16 ? lora_launch_up<float, 16>(a, p, tiles, st) : lora_launch_up<float, 128>(a, p, tiles, st);
+  return tile == 16 ? lora_launch_up<__nv_bfloat16, 16>(a, p, tiles, st) : lora_launch_up<__nv_bfloat16, 128>(a, p, tiles, st);
 }
 
 static int lora_chunk_plain(const b200q_lora_args& a, cudaStream_t st) {
@@ -509,7 +731,9 @@ int lora_add_impl(const b200q_lora_args& a, cudaStream_t st) {
     c.x = static_cast<const uint8_t*>(a.x) + 2 * t * a.x_stride;
     c.y = static_cast<uint8_t*>(a.y) + (a.y_dtype == B200Q_F32 ? 4 : 2) * t * a.y_stride;
     c.adapter = a.adapter + t;
-    if (int rc = lora_fits_tensor_cores(a) ? lora_chunk_fast(c, st) : lora_chunk_plain(c, st)) return rc;
+    int rc = lora_fits_tensor_cores(a) ? lora_chunk_fast(c, st) : B200Q_ERR_UNSUPPORTED;
+    if (rc == B200Q_ERR_UNSUPPORTED) rc = lora_chunk_plain(c, st);  // (or a layout that has no tensor map)
+    if (rc) return rc;
   }
   return B200Q_OK;
 }

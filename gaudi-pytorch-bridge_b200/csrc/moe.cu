@@ -393,37 +393,8 @@ __device__ __forceinline__ bool moe_grid_wait(const uint32_t* p, uint32_t want, 
   atomicCAS(status, 0, kMoeErrGrid);
   return false;
 }
-// four rows of a matrix, 128 bytes of each from column x on
-__device__ __forceinline__ void moe_gather4(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, const int (&rows)[4]) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(rows[0]), "r"(rows[1]), "r"(rows[2]), "r"(rows[3])
-      : "memory");
-}
 // between ordinary accesses to memory and those of copies
 __device__ __forceinline__ void moe_fence_async() { asm volatile("fence.proxy.async;" ::: "memory"); }
-// A named barrier that tells whether all its threads say yes.  Warps that share a barrier must all come to it, also where the waits of some have run out.
-__device__ __forceinline__ bool moe_bar_and(int id, int threads, bool yes) {
-  uint32_t all;
-  asm volatile(
-      "{\n"
-      ".reg .pred p, q;\n"
-      "setp.ne.u32 p, %3, 0;\n"
-      "barrier.cta.red.and.aligned.pred q, %1, %2, p;\n"
-      "selp.u32 %0, 1, 0, q;\n"
-      "}\n"
-      : "=r"(all)
-      : "r"(id), "r"(threads), "r"((uint32_t)yes)
-      : "memory");
-  return all != 0;
-}
-__device__ __forceinline__ void moe_tmem_ld8(uint32_t taddr, float (&v)[8]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
-               : "r"(taddr)
-               : "memory");
-}
-
 // x / d for 0 <= x < 2^22 from 1 / d: (x + 1/2) / d is at least 1 / 2d from a whole number, and its two roundings are off by less than x / d * 2^-22.  (A division of
 // integers is a hundred cycles, and some ten of them stood before the first copy.)
 __device__ __forceinline__ int moe_divide(int x, float inverse) { return (int)(((float)x + 0.5f) * inverse); }
@@ -716,7 +687,7 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
   // behind the last unit: the warps of the sums and of the results together, whatever became of their waits
   auto finished_all = [&] {
     __threadfence();
-    ok = moe_bar_and(3, 256, ok);
+    ok = layer_bar_and(3, 256, ok);
     if (ok && tid == 96) moe_add_release(&w.control->done);
   };
   // a tile of a group's first product is finished (one of four warps)
@@ -857,7 +828,7 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
           }
           __syncwarp();
           if (product == 0 && block < blocks)
-            moe_gather4(ring + stage * Tile::kStage + 2 * kMoeSubBytes + (lane >> 1) * 1024 + four * 512, &map_x, bar_tokens + 8 * stage, k * kSteps, rows);
+            layer_gather4(ring + stage * Tile::kStage + 2 * kMoeSubBytes + (lane >> 1) * 1024 + four * 512, &map_x, bar_tokens + 8 * stage, k * kSteps, rows);
           __syncwarp();
           ++made;
           if (++stage == kStages) {
@@ -948,7 +919,7 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
           for (int sub = 0; sub < 2; ++sub) {
             float term[terms][8];
 #pragma unroll
-            for (int t = 0; t < terms; ++t) moe_tmem_ld8(d + sub * Tile::kCols + j0 * terms + 8 * t, term[t]);
+            for (int t = 0; t < terms; ++t) layer_tmem_ld8(d + sub * Tile::kCols + j0 * terms + 8 * t, term[t]);
             ptx::tmem_ld_wait();
 #pragma unroll
             for (int i = 0; i < 8; ++i) {

@@ -1660,6 +1660,7 @@ at::Tensor& lora_add_(at::Tensor& y, const at::Tensor& x, const at::Tensor& a_w,
               ": scales must be a float tensor of one entry per adapter");
   layer_check_written(y, op, "y");
   at::Tensor xr = layer_rows(x), ar = layer_rows(a_w), br = layer_rows(b_w), which = adapter.contiguous();
+  if (tokens > 1 && xr.stride(0) < k) xr = xr.contiguous();  // (one row for all tokens)
   if (scales.defined()) scales = scales.contiguous();
   for (const at::Tensor* t : {&xr, &ar, &br}) {
     if (t->numel() == 0 || y.numel() == 0 || !t->is_alias_of(y)) continue;
