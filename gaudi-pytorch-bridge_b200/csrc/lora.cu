@@ -85,13 +85,13 @@ static int lora_tile_tokens(int64_t tokens, int64_t rank, int64_t adapters, bool
   const int64_t t = tokens < kLoraChunk ? tokens : kLoraChunk, blocks = (wide ? 3 : 2) * ((rank + 63) / 64);
   return t >= 24 * adapters && t > 64 && blocks <= 6 ? 128 : 16;
 }
-// tiles that the tokens may need at most, and parts of k such that two CTAs of each SM have work
+// tiles that the tokens may need at most, and parts of k such that two CTAs of each SM have one item at most (a second round costs as much as the first)
 static int64_t lora_most_tiles(int64_t tokens, int64_t adapters, int tile) {
   const int64_t t = tokens < kLoraChunk ? tokens : kLoraChunk, shared = adapters + t / tile;
   return t < shared ? t : shared;
 }
 static int64_t lora_splits(int64_t tokens, int64_t k, int64_t adapters, int tile) {
-  const int64_t most = (k + 255) / 256, tiles = lora_most_tiles(tokens, adapters, tile), wanted = (2 * kNumSMs + tiles - 1) / tiles;
+  const int64_t most = (k + 255) / 256, tiles = lora_most_tiles(tokens, adapters, tile), wanted = 2 * kNumSMs / tiles;
   const int64_t splits = wanted < most ? wanted : most;
   return splits < 1 ? 1 : splits < 16 ? splits : 16;
 }
@@ -374,40 +374,53 @@ __global__ void __launch_bounds__(32 * kLoraDownWarps, 2)
 // after the other.  A warp has 32 columns and half of the tokens; it turns its results around in shared memory, eight tokens at a time, so that a lane has 16 bytes of
 // a row of y, and has always asked for the next block's.  (A column and two bytes per lane, 16 of them asked for at a time, was 150 us where this is 45: 4096 tokens of
 // 14336 columns.)
-constexpr int kLoraUpWarps = 10;  // copies, MMAs, eight of results
+constexpr int lora_result_warps(int tile) { return tile == 16 ? 4 : 8; }
+constexpr int lora_up_threads(int tile) { return 64 + 32 * lora_result_warps(tile); }  // copies, MMAs, results
+constexpr int lora_up_ctas(int wide, int tile) { return tile == 16 ? 4 : wide ? 1 : 2; }  // of an SM
 struct LoraUpShape {
-  int chunks, terms_bytes, stages, parts, blocks;  // chunks of 64 ranks; bytes of the terms; parts of n, and blocks of 128 columns of a part
+  int chunks, terms_bytes, stages, parts;  // chunks of 64 ranks; bytes of the terms; parts of n: every `parts`-th block of 128 columns
 };
 
-template <typename Y>
-__device__ __forceinline__ uint4 lora_load16(const Y* p, bool whole) {
-  if (whole) return *reinterpret_cast<const uint4*>(p);
-  Y v[16 / sizeof(Y)];
-#pragma unroll
-  for (int i = 0; i < (int)(16 / sizeof(Y)); ++i) v[i] = p[i];
-  return *reinterpret_cast<const uint4*>(v);
+// 16 bytes of a row, at once or (rows between boundaries) value by value
+template <bool WHOLE, typename Y>
+__device__ __forceinline__ uint4 lora_load16(const Y* p) {
+  if constexpr (WHOLE) {
+    return *reinterpret_cast<const uint4*>(p);
+  } else if constexpr (sizeof(Y) == 4) {
+    return make_uint4(__float_as_uint(p[0]), __float_as_uint(p[1]), __float_as_uint(p[2]), __float_as_uint(p[3]));
+  } else {
+    const uint16_t* u = reinterpret_cast<const uint16_t*>(p);
+    return make_uint4(u[0] | u[1] << 16, u[2] | u[3] << 16, u[4] | u[5] << 16, u[6] | u[7] << 16);
+  }
 }
-template <typename Y>
-__device__ __forceinline__ void lora_store16(Y* p, const uint4& w, bool whole) {
-  if (whole) {
+template <bool WHOLE, typename Y>
+__device__ __forceinline__ void lora_store16(Y* p, const uint4& w) {
+  const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+  if constexpr (WHOLE) {
     *reinterpret_cast<uint4*>(p) = w;
   } else {
-    const Y* v = reinterpret_cast<const Y*>(&w);
 #pragma unroll
-    for (int i = 0; i < (int)(16 / sizeof(Y)); ++i) p[i] = v[i];
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(Y) == 4) {
+        p[i] = __uint_as_float(v[i]);
+      } else {
+        reinterpret_cast<uint16_t*>(p)[2 * i] = (uint16_t)v[i];
+        reinterpret_cast<uint16_t*>(p)[2 * i + 1] = (uint16_t)(v[i] >> 16);
+      }
+    }
   }
 }
 
-template <typename Y, int TILE>
-__global__ void __launch_bounds__(32 * kLoraUpWarps, sizeof(Y) * TILE == 512 ? 1 : 2) lora_up_kernel(const __grid_constant__ CUtensorMap map_b, const b200q_lora_args a, const LoraPlan p, const LoraUpShape d) {
-  constexpr int kTerms = sizeof(Y) == 4 ? 3 : 2, kStage = 128 * 128, kHalf = TILE / 2;
+template <typename Y, int TILE, bool WHOLE>
+__global__ void __launch_bounds__(lora_up_threads(TILE), lora_up_ctas(sizeof(Y) == 4, TILE)) lora_up_kernel(const __grid_constant__ CUtensorMap map_b, const b200q_lora_args a, const LoraPlan p, const LoraUpShape d) {
+  constexpr int kTerms = sizeof(Y) == 4 ? 3 : 2, kStage = 128 * 128, kWarps = lora_result_warps(TILE), kHalf = TILE / (kWarps / 4);
   constexpr int kPer = 16 / sizeof(Y), kLanes = 32 / kPer, kRows = 32 / kLanes, kPieces = kHalf / kRows;  // values of a lane's piece of a row; lanes of a row
-  constexpr int kPitch = 36;                                                                             // of eight tokens' results, 32 of them each
+  constexpr int kBatch = kHalf < 16 ? kHalf : 16, kPitch = 36;  // tokens turned around together; floats of a token's 32 results
   extern __shared__ uint8_t s_raw[];
   uint8_t* const s_terms = s_raw + (0u - ptx::smem_u32(s_raw) & 1023u);  // [terms][chunks][tokens][128 bytes], then the ring
   __shared__ __align__(8) uint64_t s_bars[2 * kLoraMostStages + 6];
   __shared__ uint32_t s_tmem;
-  __shared__ __align__(16) float s_turn[8][8 * kPitch];
+  __shared__ __align__(16) float s_turn[kWarps][kBatch * kPitch];
   __shared__ int s_abort;
   __shared__ LoraFew s_few;
   constexpr int kTmem = 2 * TILE < 32 ? 32 : 2 * TILE;
@@ -422,9 +435,9 @@ __global__ void __launch_bounds__(32 * kLoraUpWarps, sizeof(Y) * TILE == 512 ? 1
     }
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(bar_done + 8 * i, 1);
-      ptx::mbar_init(bar_free + 8 * i, 8);
+      ptx::mbar_init(bar_free + 8 * i, kWarps);
     }
-    ptx::mbar_init(bar_terms, 8);
+    ptx::mbar_init(bar_terms, kWarps);
     ptx::mbar_init(bar_used, 1);
     s_abort = 0;
     ptx::fence_barrier_init();
@@ -447,7 +460,7 @@ __global__ void __launch_bounds__(32 * kLoraUpWarps, sizeof(Y) * TILE == 512 ? 1
     int made = 0;
     for (int i = blockIdx.x; i < items && ok; i += gridDim.x) {
       const int tile = i / d.parts, part = i - tile * d.parts, adapter = view.tiles[tile].adapter;
-      for (int n = part * d.blocks; n < min((part + 1) * d.blocks, n_blocks) && ok; ++n)
+      for (int n = part; n < n_blocks && ok; n += d.parts)
         for (int c = 0; c < d.chunks; ++c) {
           ok = ptx::mbar_wait_uniform(bar_empty + 8 * stage, phase ^ 1, &s_abort, p.status, kLoraErrCopy);
           if (!ok) break;
@@ -472,7 +485,7 @@ __global__ void __launch_bounds__(32 * kLoraUpWarps, sizeof(Y) * TILE == 512 ? 1
       const int tile = i / d.parts, part = i - tile * d.parts;
       const uint32_t idesc = ptx::umma_idesc(1, 1, 128, lora_columns(view.tiles[tile].count));
       ok = ptx::mbar_wait_uniform(bar_terms, item & 1, &s_abort, p.status, kLoraErrMma);
-      for (int n = part * d.blocks; n < min((part + 1) * d.blocks, n_blocks) && ok; ++n, ++done) {
+      for (int n = part; n < n_blocks && ok; n += d.parts, ++done) {
         const uint32_t acc = done & 1, out = tmem + acc * TILE;
         ok = ptx::mbar_wait_uniform(bar_free + 8 * acc, ((done >> 1) & 1) ^ 1, &s_abort, p.status, kLoraErrMma);
         if (!ok) break;
@@ -501,27 +514,24 @@ __global__ void __launch_bounds__(32 * kLoraUpWarps, sizeof(Y) * TILE == 512 ? 1
     int done = 0, item = 0;
     const int wt = tid - 64, quarter = warp & 3, half = (warp - 2) >> 2, my_row = lane / kLanes, my_column = 32 * quarter + lane % kLanes * kPer;
     float* const turn = s_turn[warp - 2];
-    const bool whole = reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && (a.tokens == 1 || a.y_stride % kPer == 0);
-    for (int i = blockIdx.x; i < items; i += gridDim.x, ++item) {  // (all eight warps come to each item's barrier, whatever became of their waits)
-      const int index = i / d.parts, part = i - index * d.parts, n_end = min((part + 1) * d.blocks, n_blocks);
+    for (int i = blockIdx.x; i < items; i += gridDim.x, ++item) {  // (all its warps come to each item's barrier, whatever became of their waits)
+      const int index = i / d.parts, part = i - index * d.parts;
       const LoraTile tile = view.tiles[index];
       const int first = tile.first + kHalf * half, count = min(tile.count - kHalf * half, kHalf);  // of this half
-      Y* rows[kPieces];
+      int token[kPieces];  // of a lane's pieces; -1 behind the last one
       uint4 old[kPieces];
+      Y* const columns = static_cast<Y*>(a.y) + my_column;
       auto ask = [&](int c, int n) {
-        if (c * kRows + my_row < count && n < n_end && 128 * n + my_column < a.n) old[c] = lora_load16(rows[c] + 128 * n, whole);
+        if (token[c] >= 0 && 128 * n + my_column < a.n) old[c] = lora_load16<WHOLE>(columns + token[c] * a.y_stride + 128 * n);
       };
 #pragma unroll
-      for (int c = 0; c < kPieces; ++c) {
-        rows[c] = static_cast<Y*>(a.y) + my_column;
-        if (c * kRows + my_row < count) rows[c] += view.sorted[first + c * kRows + my_row] * a.y_stride;
-      }
+      for (int c = 0; c < kPieces; ++c) token[c] = c * kRows + my_row < count ? view.sorted[first + c * kRows + my_row] : -1;
 #pragma unroll
-      for (int c = 0; c < kPieces; ++c) ask(c, part * d.blocks);
+      for (int c = 0; c < kPieces; ++c) ask(c, part);
       ok = ok && ptx::mbar_wait_uniform(bar_used, (item & 1) ^ 1, &s_abort, p.status, kLoraErrResults);  // (the products with the terms before are done)
       const float scale = a.scales ? a.scales[tile.adapter] : 1.f;
       const int pieces = 8 * d.chunks;  // of eight ranks
-      for (int q = wt; ok && q < tile.count * pieces; q += 256) {
+      for (int q = wt; ok && q < tile.count * pieces; q += 32 * kWarps) {
         const int j = q / pieces, r = 8 * (q - j * pieces);
         float v[8] = {};
         if (r < a.rank) {
@@ -548,27 +558,33 @@ __global__ void __launch_bounds__(32 * kLoraUpWarps, sizeof(Y) * TILE == 512 ? 1
         }
       }
       ptx::fence_proxy_async_smem();
-      ok = layer_bar_and(1, 256, ok);
+      ok = layer_bar_and(1, 32 * kWarps, ok);
       if (!ok) break;
       if (lane == 0) ptx::mbar_arrive(bar_terms);
-      for (int n = part * d.blocks; n < n_end && ok; ++n, ++done) {
+      for (int n = part; n < n_blocks && ok; n += d.parts, ++done) {
         const uint32_t acc = done & 1, in = tmem + acc * TILE + kHalf * half + ((uint32_t)(32 * quarter) << 16);
         ok = ptx::mbar_wait_uniform(bar_done + 8 * acc, (done >> 1) & 1, &s_abort, p.status, kLoraErrResults);
         if (!ok) break;
         ptx::tc_fence_after();
         const bool there = 128 * n + my_column < a.n;
 #pragma unroll
-        for (int j0 = 0; j0 < kHalf; j0 += 8) {
+        for (int j0 = 0; j0 < kHalf; j0 += kBatch) {
           if (j0 >= count) break;
-          float v[8];
-          layer_tmem_ld8(in + j0, v);
+          float v[kBatch / 8][8];
+#pragma unroll
+          for (int h = 0; h < kBatch / 8; ++h)
+            if (j0 + 8 * h < count) layer_tmem_ld8(in + j0 + 8 * h, v[h]);
           ptx::tmem_ld_wait();
           __syncwarp();
 #pragma unroll
-          for (int j = 0; j < 8; ++j) turn[j * kPitch + lane] = v[j];
+          for (int h = 0; h < kBatch / 8; ++h)
+            if (j0 + 8 * h < count) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) turn[(8 * h + j) * kPitch + lane] = v[h][j];
+            }
           __syncwarp();
 #pragma unroll
-          for (int c = j0 / kRows; c < (j0 + 8) / kRows; ++c) {
+          for (int c = j0 / kRows; c < (j0 + kBatch) / kRows; ++c) {
             const float4* from = reinterpret_cast<const float4*>(turn + (c * kRows - j0 + my_row) * kPitch + lane % kLanes * kPer);
             uint4 w;
             const float4 x = from[0];
@@ -582,8 +598,8 @@ __global__ void __launch_bounds__(32 * kLoraUpWarps, sizeof(Y) * TILE == 512 ? 1
               w.z = pack_bf16x2(__uint_as_float(old[c].z << 16) + z.x, __uint_as_float(old[c].z & 0xFFFF0000u) + z.y);
               w.w = pack_bf16x2(__uint_as_float(old[c].w << 16) + z.z, __uint_as_float(old[c].w & 0xFFFF0000u) + z.w);
             }
-            if (there && c * kRows + my_row < count) lora_store16(rows[c] + 128 * n, w, whole);
-            ask(c, n + 1);
+            if (there && token[c] >= 0) lora_store16<WHOLE>(columns + token[c] * a.y_stride + 128 * n, w);
+            ask(c, n + d.parts);
           }
         }
         ptx::tc_fence_before();
@@ -657,26 +673,35 @@ static int lora_launch_down(const b200q_lora_args& a, const LoraPlan& p, int64_t
   B200Q_LAUNCH_CHECK();
   return B200Q_OK;
 }
-template <typename Y, int TILE>
+template <typename Y, int TILE, bool WHOLE>
 static int lora_launch_up(const b200q_lora_args& a, const LoraPlan& p, int64_t tiles, cudaStream_t st) {
-  constexpr int kTerms = sizeof(Y) == 4 ? 3 : 2, kMost = 214 * 1024;
+  constexpr int kTerms = sizeof(Y) == 4 ? 3 : 2, kMost = 184 * 1024;
   static std::atomic<int> done[kMaxDevices];
-  if (int rc = lora_ready(reinterpret_cast<const void*>(lora_up_kernel<Y, TILE>), done, kMost)) return rc;
+  if (int rc = lora_ready(reinterpret_cast<const void*>(lora_up_kernel<Y, TILE, WHOLE>), done, kMost)) return rc;
   CUtensorMap map_b;
   if (int rc = lora_map(&map_b, a.b, a.rank, a.n, a.adapters, a.b_row_stride, a.b_stride, 128, 3)) return rc;
   LoraUpShape d;
   d.chunks = (int)((a.rank + 63) / 64);
   d.terms_bytes = kTerms * d.chunks * TILE * 128;
-  const int room = (d.terms_bytes + 2 * 16384 + 1024 <= kLoraShared ? kLoraShared : kMost) - 1024 - d.terms_bytes;
+  // as many stages as leave room for the SM's other CTAs, if that is two; else as many as there is room for
+  constexpr int kCtas = lora_up_ctas(sizeof(Y) == 4, TILE), kHere = 4 * lora_result_warps(TILE) * 16 * 36 + 1024;  // (static memory)
+  constexpr int kShare = (226 * 1024 / kCtas - 1024 - kHere) / 1024 * 1024;
+  const int room = (d.terms_bytes + 2 * 16384 + 1024 <= kShare ? kShare : kMost) - 1024 - d.terms_bytes;
   d.stages = room / 16384 < kLoraMostStages ? room / 16384 : kLoraMostStages;
-  const int64_t blocks = (a.n + 127) / 128, wanted = (4 * kNumSMs + tiles - 1) / tiles, parts = wanted < blocks ? wanted : blocks;
-  d.blocks = (int)((blocks + parts - 1) / parts);
-  d.parts = (int)((blocks + d.blocks - 1) / d.blocks);
-  const int64_t items = tiles * d.parts, most = 2 * kNumSMs;
-  launch_dependent(lora_up_kernel<Y, TILE>, dim3((unsigned)(items < most ? items : most)), dim3(32 * kLoraUpWarps), (size_t)d.terms_bytes + d.stages * 16384 + 1024, st, map_b, a, p,
+  const int64_t blocks = (a.n + 127) / 128, wanted = kCtas * kNumSMs / tiles;  // (one round, as above)
+  d.parts = (int)(wanted < 1 ? 1 : wanted < blocks ? wanted : blocks);
+  const int64_t items = tiles * d.parts, most = kCtas * kNumSMs;
+  launch_dependent(lora_up_kernel<Y, TILE, WHOLE>, dim3((unsigned)(items < most ? items : most)), dim3(lora_up_threads(TILE)), (size_t)d.terms_bytes + d.stages * 16384 + 1024, st, map_b, a, p,
                    d);
   B200Q_LAUNCH_CHECK();
   return B200Q_OK;
+}
+
+template <typename Y>
+static int lora_launch_up_tile(const b200q_lora_args& a, const LoraPlan& p, int64_t tiles, cudaStream_t st) {
+  const bool whole = reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && (a.tokens == 1 || a.y_stride * sizeof(Y) % 16 == 0);
+  if (p.tile == 16) return whole ? lora_launch_up<Y, 16, true>(a, p, tiles, st) : lora_launch_up<Y, 16, false>(a, p, tiles, st);
+  return whole ? lora_launch_up<Y, 128, true>(a, p, tiles, st) : lora_launch_up<Y, 128, false>(a, p, tiles, st);
 }
 
 static int lora_chunk_fast(const b200q_lora_args& a, cudaStream_t st) {
@@ -705,8 +730,7 @@ static int lora_chunk_fast(const b200q_lora_args& a, cudaStream_t st) {
     B200Q_LAUNCH_CHECK();
   }
   if (int rc = tile == 16 ? lora_launch_down<16>(a, p, tiles, st) : lora_launch_down<128>(a, p, tiles, st)) return rc;
-  if (a.y_dtype == B200Q_F32) return tile == 16 ? lora_launch_up<float, 16>(a, p, tiles, st) : lora_launch_up<float, 128>(a, p, tiles, st);
-  return tile == 16 ? lora_launch_up<__nv_bfloat16, 16>(a, p, tiles, st) : lora_launch_up<__nv_bfloat16, 128>(a, p, tiles, st);
+  return a.y_dtype == B200Q_F32 ? lora_launch_up_tile<float>(a, p, tiles, st) : lora_launch_up_tile<__nv_bfloat16>(a, p, tiles, st);
 }
 
 static int lora_chunk_plain(const b200q_lora_args& a, cudaStream_t st) {
