@@ -85,7 +85,7 @@ static int lora_tile_tokens(int64_t tokens, int64_t rank, int64_t adapters, bool
   const int64_t t = tokens < kLoraChunk ? tokens : kLoraChunk, blocks = (wide ? 3 : 2) * ((rank + 63) / 64);
   return t >= 24 * adapters && t > 64 && blocks <= 6 ? 128 : 16;
 }
-// tiles that the tokens may need at most, and parts of k such that two CTAs of each SM have one item at most (a second round costs as much as the first)
+// tiles that the tokens may need at most, and parts of k such that none of an SM's two CTAs has a second item (a second round costs as much as the first)
 static int64_t lora_most_tiles(int64_t tokens, int64_t adapters, int tile) {
   const int64_t t = tokens < kLoraChunk ? tokens : kLoraChunk, shared = adapters + t / tile;
   return t < shared ? t : shared;
@@ -144,12 +144,15 @@ __global__ void __launch_bounds__(kLoraSortThreads) lora_sort_kernel(const b200q
     }
     if (lane == 31) s_scan[turn][warp] = scan;
     __syncthreads();  // (the other half is written next, and this one only behind the next barrier)
-    int before = tokens_before | tiles_before << 16, all = before;
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) before += s_scan[turn][w];
-      all += s_scan[turn][w];
+    int sums = s_scan[turn][lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xFFFFFFFFu, sums, o);
+      if (lane >= o) sums += v;
     }
-    before += scan - both;
+    const int here = tokens_before | tiles_before << 16, all = here + __shfl_sync(0xFFFFFFFFu, sums, 31);
+    int before = __shfl_sync(0xFFFFFFFFu, sums, warp == 0 ? 0 : warp - 1);
+    before = here + (warp == 0 ? 0 : before) + scan - both;
     tokens_before = all & 0xFFFF;
     tiles_before = all >> 16;
     if (i < adapters) s_first[i] = (uint16_t)(before & 0xFFFF);
@@ -222,7 +225,7 @@ struct LoraDownShape {
 
 template <int TILE>
 __global__ void __launch_bounds__(32 * kLoraDownWarps, 2)
-    lora_down_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_x, const b200q_lora_args a, const LoraPlan p, const LoraDownShape d) {
+    lora_down_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_run, const b200q_lora_args a, const LoraPlan p, const LoraDownShape d) {
   extern __shared__ uint8_t s_raw[];
   uint8_t* const s_ring = s_raw + (0u - ptx::smem_u32(s_raw) & 1023u);
   __shared__ __align__(8) uint64_t s_bars[2 * kLoraMostStages + 4];
@@ -246,6 +249,7 @@ __global__ void __launch_bounds__(32 * kLoraDownWarps, 2)
     ptx::fence_barrier_init();
     ptx::tma_prefetch_desc(&map_a);
     ptx::tma_prefetch_desc(&map_x);
+    if (TILE > 16) ptx::tma_prefetch_desc(&map_run);
   }
   if (warp == 1) {
     ptx::tmem_alloc(ptx::smem_u32(&s_tmem), kTmem);
@@ -286,16 +290,23 @@ __global__ void __launch_bounds__(32 * kLoraDownWarps, 2)
 #pragma unroll
         for (int r = 0; r < 4; ++r) rows[r] = view.sorted[it.tile.first + min(4 * lane + r, it.tile.count - 1)];
       }
+      // Tokens that follow one another, as those of a prompt do, come as one box: 32 gathers of four rows each take a microsecond.
+      bool run = TILE > 16 && it.tile.count > TILE / 2;
+      const int first = __shfl_sync(0xFFFFFFFFu, rows[0], 0);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) run = run && (4 * lane + r >= it.tile.count || rows[r] == first + 4 * lane + r);
+      run = __all_sync(0xFFFFFFFFu, run);
       for (int k = it.k0; k < it.k1; ++k) {
         ok = ptx::mbar_wait_uniform(bar_empty + 8 * stage, phase ^ 1, &s_abort, p.status, kLoraErrCopy);
         if (!ok) break;
         const uint32_t bar = bar_full + 8 * stage, dst = ring + stage * d.stage;
         if (ptx::elect_one()) {
-          ptx::mbar_arrive_expect_tx(bar, d.row_bytes + eights * 1024);
+          ptx::mbar_arrive_expect_tx(bar, d.row_bytes + (run ? TILE * 128 : eights * 1024));
           ptx::tma_load_3d(dst, &map_a, bar, 64 * k, 128 * it.block, it.tile.adapter);
+          if (run) ptx::tma_load_2d(dst + d.row_bytes, &map_run, bar, 64 * k, first);  // (rows behind the tile's are columns that nobody looks at)
         }
         __syncwarp();
-        if (lane < 2 * eights) layer_gather4(dst + d.row_bytes + 512 * lane, &map_x, bar, 64 * k, rows);
+        if (!run && lane < 2 * eights) layer_gather4(dst + d.row_bytes + 512 * lane, &map_x, bar, 64 * k, rows);
         __syncwarp();
         ++made;
         if (++stage == (uint32_t)d.stages) {
@@ -535,12 +546,20 @@ __global__ void __launch_bounds__(lora_up_threads(TILE), lora_up_ctas(sizeof(Y) 
         const int j = q / pieces, r = 8 * (q - j * pieces);
         float v[8] = {};
         if (r < a.rank) {
-          const float* low = p.low + (int64_t)view.sorted[tile.first + j] * a.rank + r;
-#pragma unroll 4
-          for (int s = 0; s < p.splits; ++s) {
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(low + s * a.tokens * a.rank)), y = __ldcg(reinterpret_cast<const float4*>(low + s * a.tokens * a.rank) + 1);
-            v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
-            v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+          const float4* low = reinterpret_cast<const float4*>(p.low + (int64_t)view.sorted[tile.first + j] * a.rank + r);
+          const int64_t step = a.tokens * a.rank / 4;
+          constexpr int kTogether = 4;  // parts of k on their way
+          for (int s0 = 0; s0 < p.splits; s0 += kTogether) {
+            float4 x[kTogether][2];
+#pragma unroll
+            for (int s = 0; s < kTogether; ++s)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) x[s][h] = s0 + s < p.splits ? __ldcg(low + (s0 + s) * step + h) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int s = 0; s < kTogether; ++s) {
+              v[0] += x[s][0].x; v[1] += x[s][0].y; v[2] += x[s][0].z; v[3] += x[s][0].w;
+              v[4] += x[s][1].x; v[5] += x[s][1].y; v[6] += x[s][1].z; v[7] += x[s][1].w;
+            }
           }
         }
 #pragma unroll
@@ -663,13 +682,14 @@ static int lora_launch_down(const b200q_lora_args& a, const LoraPlan& p, int64_t
   static std::atomic<int> done[kMaxDevices];
   if (int rc = lora_ready(reinterpret_cast<const void*>(lora_down_kernel<TILE>), done, kLoraShared)) return rc;
   const LoraDownShape d((int)a.rank, TILE, kLoraShared - 1024);
-  CUtensorMap map_a, map_x;
+  CUtensorMap map_a, map_x, map_run;
   if (int rc = lora_map(&map_a, a.a, a.k, a.rank, a.adapters, a.a_row_stride, a.a_stride, d.rows, 3)) return rc;
   if (int rc = lora_map(&map_x, a.x, a.k, a.tokens, 1, a.x_stride, 0, 1, 2)) return rc;
+  if (int rc = lora_map(&map_run, a.x, a.k, a.tokens, 1, a.x_stride, 0, TILE, 2)) return rc;
   const int64_t items = tiles * p.splits * ((a.rank + 127) / 128), most = 2 * kNumSMs;
   // (the rows behind a block's ranks, which the product reads too and whose results nobody looks at, are within the allocation)
-  launch_dependent(lora_down_kernel<TILE>, dim3((unsigned)(items < most ? items : most)), dim3(32 * kLoraDownWarps), (size_t)d.stages * d.stage + 16384 + 1024, st, map_a, map_x, a,
-                   p, d);
+  launch_dependent(lora_down_kernel<TILE>, dim3((unsigned)(items < most ? items : most)), dim3(32 * kLoraDownWarps), (size_t)d.stages * d.stage + 16384 + 1024, st, map_a, map_x,
+                   map_run, a, p, d);
   B200Q_LAUNCH_CHECK();
   return B200Q_OK;
 }
