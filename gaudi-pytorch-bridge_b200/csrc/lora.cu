@@ -212,6 +212,9 @@ __host__ __device__ constexpr int lora_columns(int tokens) { return (tokens + 15
 // a x of a tile's tokens over a part of k: ranks are the rows of the product, tokens its columns.  A step is 64 values of k of up to 128 ranks and the tile's tokens.
 constexpr int kLoraMostStages = 8;
 constexpr int kLoraDownWarps = 6;  // copies, MMAs, four of results
+// An addition inside the tensor core drops what does not fit 24 bits: behind a row of 2048 products a y in fp32 would be off by 5e-7 where plain fp32 sums are by 1e-7.  So for
+// such a y no more than 256 are added there (2e-7).
+constexpr int kLoraSub = 4;
 struct LoraDownShape {
   int rows, row_bytes, stage, stages;  // ranks of a block; bytes of them and of a stage
   LoraDownShape(int rank, int tile, int smem) {
@@ -223,7 +226,7 @@ struct LoraDownShape {
   }
 };
 
-template <int TILE>
+template <int TILE, bool EXACT>  // EXACT: no more than kLoraSub steps are added inside the tensor core
 __global__ void __launch_bounds__(32 * kLoraDownWarps, 2)
     lora_down_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_run, const b200q_lora_args a, const LoraPlan p, const LoraDownShape d) {
   extern __shared__ uint8_t s_raw[];
@@ -323,22 +326,28 @@ __global__ void __launch_bounds__(32 * kLoraDownWarps, 2)
     for (int i = blockIdx.x; i < items && ok; i += gridDim.x) {
       const Item it = item_of(i);
       if (it.k0 >= it.k1) continue;
-      const uint32_t acc = n & 1, out = tmem + acc * TILE, idesc = ptx::umma_idesc(1, 1, 128, lora_columns(it.tile.count));
-      ok = ptx::mbar_wait_uniform(bar_free + 8 * acc, ((n >> 1) & 1) ^ 1, &s_abort, p.status, kLoraErrMma);
-      if (!ok) break;
-      ++n;
-      ptx::tc_fence_after();
-      for (int k = it.k0; k < it.k1; ++k) {
+      const uint32_t idesc = ptx::umma_idesc(1, 1, 128, lora_columns(it.tile.count));
+      uint32_t acc = 0, out = 0;
+      for (int k = it.k0, sub = 0; k < it.k1; ++k) {
+        if (sub == 0) {
+          acc = n & 1;
+          out = tmem + acc * TILE;
+          ok = ptx::mbar_wait_uniform(bar_free + 8 * acc, ((n >> 1) & 1) ^ 1, &s_abort, p.status, kLoraErrMma);
+          if (!ok) break;
+          ++n;
+          ptx::tc_fence_after();
+        }
         ok = ptx::mbar_wait_uniform(bar_full + 8 * stage, phase, &s_abort, p.status, kLoraErrMma);
         if (!ok) break;
         ptx::tc_fence_after();
         if (ptx::elect_one()) {
           const uint64_t off = stage * (uint32_t)(d.stage >> 4);
-          ptx::umma_f16_x4(out, a0 + off, b0 + off, idesc, k != it.k0, 2, 2);
+          ptx::umma_f16_x4(out, a0 + off, b0 + off, idesc, sub != 0, 2, 2);
           ptx::umma_commit(bar_empty + 8 * stage);
-          if (k + 1 == it.k1) ptx::umma_commit(bar_done + 8 * acc);
+          if (k + 1 == it.k1 || (EXACT && sub + 1 == kLoraSub)) ptx::umma_commit(bar_done + 8 * acc);
         }
         __syncwarp();
+        if (++sub == kLoraSub && EXACT) sub = 0;
         if (++stage == (uint32_t)d.stages) {
           stage = 0;
           phase ^= 1;
@@ -351,28 +360,41 @@ __global__ void __launch_bounds__(32 * kLoraDownWarps, 2)
     for (int i = blockIdx.x; i < items && ok; i += gridDim.x) {
       const Item it = item_of(i);
       const int r = 128 * it.block + 32 * quarter + lane;
-      const bool none = it.k0 >= it.k1;  // (a part behind the end of k)
-      const uint32_t acc = n & 1, in = tmem + acc * TILE + ((uint32_t)(32 * quarter) << 16);
-      if (!none) {
-        ok = ptx::mbar_wait_uniform(bar_done + 8 * acc, (n >> 1) & 1, &s_abort, p.status, kLoraErrResults);
-        if (!ok) break;
-        ++n;
-        ptx::tc_fence_after();
-      }
-      for (int j0 = 0; j0 < it.tile.count; j0 += 8) {
-        float v[8] = {};
+      // (a part behind the end of k: zeros)
+      for (int k = it.k0; k == it.k0 || (EXACT && k < it.k1); k += kLoraSub) {
+        const bool none = it.k0 >= it.k1;
+        const uint32_t acc = n & 1, in = tmem + acc * TILE + ((uint32_t)(32 * quarter) << 16);
         if (!none) {
-          layer_tmem_ld8(in + j0, v);
-          ptx::tmem_ld_wait();
+          ok = ptx::mbar_wait_uniform(bar_done + 8 * acc, (n >> 1) & 1, &s_abort, p.status, kLoraErrResults);
+          if (!ok) break;
+          ++n;
+          ptx::tc_fence_after();
         }
+        for (int j0 = 0; j0 < it.tile.count; j0 += 8) {
+          float v[8] = {};
+          if (!none) {
+            layer_tmem_ld8(in + j0, v);
+            ptx::tmem_ld_wait();
+          }
+          float* to[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (j0 + j < it.tile.count && r < a.rank) p.low[((int64_t)it.part * a.tokens + view.sorted[it.tile.first + j0 + j]) * a.rank + r] = v[j];
-      }
-      if (!none) {
-        ptx::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(bar_free + 8 * acc);
+          for (int j = 0; j < 8; ++j) to[j] = p.low + ((int64_t)it.part * a.tokens + view.sorted[it.tile.first + min(j0 + j, it.tile.count - 1)]) * a.rank + r;
+          if (EXACT && k > it.k0) {  // (a thread's own sums)
+            float before[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) before[j] = r < a.rank ? *to[j] : 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] += before[j];
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (j0 + j < it.tile.count && r < a.rank) *to[j] = v[j];
+        }
+        if (!none) {
+          ptx::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(bar_free + 8 * acc);
+        }
       }
     }
   }
@@ -506,8 +528,8 @@ __global__ void __launch_bounds__(lora_up_threads(TILE), lora_up_ctas(sizeof(Y) 
           if (!ok) break;
           ptx::tc_fence_after();
           if (ptx::elect_one()) {
-            for (int e = 0; e < kTerms; ++e)
-              ptx::umma_f16_x4(out, a0 + stage * (uint32_t)(kStage >> 4), b0 + (e * d.chunks + c) * (TILE * 128 >> 4), idesc, c + e != 0, 2, 2);
+            for (int e = kTerms - 1; e >= 0; --e)  // (the small ones first)
+              ptx::umma_f16_x4(out, a0 + stage * (uint32_t)(kStage >> 4), b0 + (e * d.chunks + c) * (TILE * 128 >> 4), idesc, c > 0 || e < kTerms - 1, 2, 2);
             ptx::umma_commit(bar_empty + 8 * stage);
             if (c + 1 == d.chunks) ptx::umma_commit(bar_done + 8 * acc);
           }
@@ -677,10 +699,10 @@ static int lora_ready(const void* kernel, std::atomic<int> (&done)[kMaxDevices],
 
 constexpr int kLoraShared = 100 * 1024;  // of a CTA where two share an SM, beside what its kernel has of its own
 
-template <int TILE>
+template <int TILE, bool EXACT>
 static int lora_launch_down(const b200q_lora_args& a, const LoraPlan& p, int64_t tiles, cudaStream_t st) {
   static std::atomic<int> done[kMaxDevices];
-  if (int rc = lora_ready(reinterpret_cast<const void*>(lora_down_kernel<TILE>), done, kLoraShared)) return rc;
+  if (int rc = lora_ready(reinterpret_cast<const void*>(lora_down_kernel<TILE, EXACT>), done, kLoraShared)) return rc;
   const LoraDownShape d((int)a.rank, TILE, kLoraShared - 1024);
   CUtensorMap map_a, map_x, map_run;
   if (int rc = lora_map(&map_a, a.a, a.k, a.rank, a.adapters, a.a_row_stride, a.a_stride, d.rows, 3)) return rc;
@@ -688,14 +710,14 @@ static int lora_launch_down(const b200q_lora_args& a, const LoraPlan& p, int64_t
   if (int rc = lora_map(&map_run, a.x, a.k, a.tokens, 1, a.x_stride, 0, TILE, 2)) return rc;
   const int64_t items = tiles * p.splits * ((a.rank + 127) / 128), most = 2 * kNumSMs;
   // (the rows behind a block's ranks, which the product reads too and whose results nobody looks at, are within the allocation)
-  launch_dependent(lora_down_kernel<TILE>, dim3((unsigned)(items < most ? items : most)), dim3(32 * kLoraDownWarps), (size_t)d.stages * d.stage + 16384 + 1024, st, map_a, map_x,
+  launch_dependent(lora_down_kernel<TILE, EXACT>, dim3((unsigned)(items < most ? items : most)), dim3(32 * kLoraDownWarps), (size_t)d.stages * d.stage + 16384 + 1024, st, map_a, map_x,
                    map_run, a, p, d);
   B200Q_LAUNCH_CHECK();
   return B200Q_OK;
 }
 template <typename Y, int TILE, bool WHOLE>
 static int lora_launch_up(const b200q_lora_args& a, const LoraPlan& p, int64_t tiles, cudaStream_t st) {
-  constexpr int kTerms = sizeof(Y) == 4 ? 3 : 2, kMost = 184 * 1024;
+  constexpr int kTerms = sizeof(Y) == 4 ? 3 : 2, kMost = 200 * 1024;
   static std::atomic<int> done[kMaxDevices];
   if (int rc = lora_ready(reinterpret_cast<const void*>(lora_up_kernel<Y, TILE, WHOLE>), done, kMost)) return rc;
   CUtensorMap map_b;
@@ -705,7 +727,7 @@ static int lora_launch_up(const b200q_lora_args& a, const LoraPlan& p, int64_t t
   d.terms_bytes = kTerms * d.chunks * TILE * 128;
   // as many stages as leave room for the SM's other CTAs, if that is two; else as many as there is room for
   constexpr int kCtas = lora_up_ctas(sizeof(Y) == 4, TILE), kHere = 4 * lora_result_warps(TILE) * 16 * 36 + 1024;  // (static memory)
-  constexpr int kShare = (226 * 1024 / kCtas - 1024 - kHere) / 1024 * 1024;
+  constexpr int kOne = (226 * 1024 / kCtas - 1024 - kHere) / 1024 * 1024, kShare = kOne < kMost ? kOne : kMost;
   const int room = (d.terms_bytes + 2 * 16384 + 1024 <= kShare ? kShare : kMost) - 1024 - d.terms_bytes;
   d.stages = room / 16384 < kLoraMostStages ? room / 16384 : kLoraMostStages;
   const int64_t blocks = (a.n + 127) / 128, wanted = kCtas * kNumSMs / tiles;  // (one round, as above)
@@ -749,7 +771,10 @@ static int lora_chunk_fast(const b200q_lora_args& a, cudaStream_t st) {
     launch_dependent(lora_sort_kernel, dim3(1), dim3(kLoraSortThreads), sizeof(uint16_t) * (kLoraSortThreads / 32 + 1) * (size_t)a.adapters, st, a, p);
     B200Q_LAUNCH_CHECK();
   }
-  if (int rc = tile == 16 ? lora_launch_down<16>(a, p, tiles, st) : lora_launch_down<128>(a, p, tiles, st)) return rc;
+  int rc;
+  if (a.y_dtype == B200Q_F32) rc = tile == 16 ? lora_launch_down<16, true>(a, p, tiles, st) : lora_launch_down<128, true>(a, p, tiles, st);
+  else rc = tile == 16 ? lora_launch_down<16, false>(a, p, tiles, st) : lora_launch_down<128, false>(a, p, tiles, st);
+  if (rc) return rc;
   return a.y_dtype == B200Q_F32 ? lora_launch_up_tile<float>(a, p, tiles, st) : lora_launch_up_tile<__nv_bfloat16>(a, p, tiles, st);
 }
 

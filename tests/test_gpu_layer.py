@@ -204,6 +204,7 @@ def _run_lora(y, x, a, b, which, scales):
 
 LORA_SIZES = [(1, 8, 8, 8, 1), (1, 256, 128, 16, 3), (2, 264, 136, 24, 2), (5, 1024, 512, 64, 4), (8, 512, 1416, 128, 3), (9, 520, 264, 8, 70), (17, 2056, 256, 40, 5),
               (33, 128, 1032, 256, 2), (64, 1024, 1024, 32, 64), (65, 256, 512, 16, 1), (130, 640, 392, 48, 7), (300, 384, 520, 32, 40), (1030, 128, 136, 16, 3),
+              (200, 256, 520, 128, 2), (260, 136, 264, 64, 1), (129, 72, 136, 192, 2), (300, 64, 1416, 256, 3), (70, 4104, 128, 128, 1),
               (3, 7, 5, 3, 2), (4, 100, 61, 4, 3), (6, 129, 64, 8, 2), (7, 64, 99, 16, 2), (11, 64, 64, 20, 2), (2, 1, 1, 1, 1)]
 
 
@@ -265,6 +266,36 @@ def test_lora_strided(pad):
     torch.ops.b200q.lora_add_(wide[:, pad:96 + pad], xs[:, pad:], stack_a[:, 1], stack_b[:, 1, :, :16], which.cuda(), scales.cuda())
     _check_lora(wide[:, pad:96 + pad], y, x, a, b, which, scales)
     assert bool((wide[:, :pad] == 0).all()) and bool((wide[:, 96 + pad:] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("tokens,at", [(5, 1), (200, 3), (200, 8)])
+def test_lora_y_between_boundaries(tokens, at, dtype):
+    """y from a column of a wider matrix on whose rows lie on no 16 bytes."""
+    y, x, a, b, which, scales = _lora_case(tokens, 64, 272, 16, 2, dtype)
+    wide = torch.zeros(tokens, 272 + 13, dtype=dtype).cuda()
+    wide[:, at:at + 272] = y.cuda()
+    torch.ops.b200q.lora_add_(wide[:, at:at + 272], x.cuda(), a.cuda(), b.cuda(), which.cuda(), scales.cuda())
+    _check_lora(wide[:, at:at + 272], y, x, a, b, which, scales)
+    assert bool((wide[:, :at] == 0).all()) and bool((wide[:, at + 272:] == 0).all())
+
+
+def test_lora_one_row_for_all_tokens():
+    y, x, a, b, which, scales = _lora_case(40, 64, 72, 16, 3, F32)
+    yd = y.cuda()
+    torch.ops.b200q.lora_add_(yd, x[:1].cuda().expand(40, 64), a.cuda(), b.cuda(), which.cuda(), scales.cuda())
+    _check_lora(yd, y, x[:1].expand(40, 64), a, b, which, scales)
+
+
+def test_lora_fp32_sums():
+    """Sums over 8192 products of one sign, in which an addition that drops bits adds up.  256 products at a time are added inside the tensor core, 16 by 16: each
+    addition may drop up to 2^-23 of the sum so far, half the last sum on average, 8.5 * 2^-23 in all, and 2^-23 for the products of a step; 32 such sums are added
+    in fp32, 31 * 2^-24; b and its three terms add 4 * 2^-23: below 2^-18 of the sum of the absolute values.  A row of 512 such additions inside could be off by
+    2^-15."""
+    y, x, a, b, which, scales = _lora_case(40, 8192, 64, 8, 1, F32, which=torch.zeros(40))
+    x, a, b, y = x.abs(), a.abs(), b.abs(), torch.zeros_like(y)
+    want, size, _ = O.lora_add(y, x, a, b, which, scales)
+    _close(_run_lora(y, x, a, b, which, scales), want, 2.0 ** -18 * size)
 
 
 def test_lora_other_tokens_do_not_matter():
