@@ -155,10 +155,10 @@ __global__ void __launch_bounds__(kMoeThreads) moe_logits_kernel(const b200q_moe
       x_top[t0 + t] = most;
     }
   }
-  if (!x_terms || e0 != 0) return;
-  // the tokens' two terms for 8-bit weights
+  if (!x_terms) return;
+  // the tokens' two terms for 8-bit weights, a token by each of the blocks that have it
 #pragma unroll 1
-  for (int t = 0; t < TB && t0 + t < tokens; ++t) {
+  for (int64_t t = e0 / EB; t < TB && t0 + t < tokens; t += expert_blocks) {
     uint32_t most = 0;
     for (int i = 0; i < kWarps; ++i) most = max(most, s_top[i][t]);
     const float factor = moe_up_factor(most);
@@ -341,12 +341,12 @@ constexpr int kMoeSubBytes = 128 * 128;  // a weight tile: 128 rows of 128 bytes
 constexpr int kMoeMostDim = 65536;
 constexpr uint32_t kMoeGridPolls = 1u << 23;
 
-constexpr int kMoeCutTiles = kNumSMs * 5 / 4, kMoeMostParts = 8;
+constexpr int kMoeCutTiles = kNumSMs * 5 / 4 + 1, kMoeMostParts = 8, kMoeSumTokens = 4;
 constexpr int kMoeMostGroups = kMoeMaxExperts + (int)kMoeChunk * kMoeMaxTopK / kMoeGroupTokens;
 struct MoeControl {  // cleared by the router's kernel
   uint32_t chosen, done, next[2];
   uint32_t parts[2][kMoeCutTiles];  // of a cut tile that are there, four warps each
-  uint32_t up[kMoeMostGroups];      // tiles of a group's first product that are finished, four warps each
+  uint32_t up[kMoeMostGroups];      // of a group's first product: tiles times blocks of four tokens that are finished, four warps each
   uint32_t terms[kMoeMostGroups];   // slots of a group whose terms are there, four warps each
 };
 
@@ -381,7 +381,7 @@ __device__ __forceinline__ uint32_t moe_ld_acquire(const uint32_t* p) {
   asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
   return v;
 }
-__device__ __forceinline__ void moe_add_release(uint32_t* p) { asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(p) : "memory"); }
+__device__ __forceinline__ void moe_add_release(uint32_t* p, int n = 1) { asm volatile("red.release.gpu.global.add.u32 [%0], %1;" ::"l"(p), "r"(n) : "memory"); }
 // until all CTAs have arrived (one warp); false when they do not
 __device__ __forceinline__ bool moe_grid_wait(const uint32_t* p, uint32_t want, volatile int* abort_flag, int* status) {
   for (uint32_t i = 0; i < kMoeGridPolls; ++i) {
@@ -395,24 +395,28 @@ __device__ __forceinline__ bool moe_grid_wait(const uint32_t* p, uint32_t want, 
 }
 // between ordinary accesses to memory and those of copies
 __device__ __forceinline__ void moe_fence_async() { asm volatile("fence.proxy.async;" ::: "memory"); }
-// x / d for 0 <= x < 2^22 from 1 / d: (x + 1/2) / d is at least 1 / 2d from a whole number, and its two roundings are off by less than x / d * 2^-22.  (A division of
+// x / d for -d < x < 2^22 (0 below 0) from 1 / d: (x + 1/2) / d is at least 1 / 2d from a whole number, and its two roundings are off by less than x / d * 2^-22.  (A division of
 // integers is a hundred cycles, and some ten of them stood before the first copy.)
 __device__ __forceinline__ int moe_divide(int x, float inverse) { return (int)(((float)x + 0.5f) * inverse); }
 
 // The units of a product: `whole` tiles, then the parts of the others.  Fewer than 2^22 of them: at most 640 groups, of 512 tiles each.
+// Cut are the tiles that do not come out even, and a quarter of a round of all CTAs at least; but none where a tile is short, because a sum of parts takes as long as
+// some eight steps, and none where so many CTAs have one whole tile that they draw all that the memory gives.
 struct MoeUnits {
-  int tiles, steps, whole, parts, units;  // tiles of a group, steps of a tile
+  int tiles, steps, whole, cut, parts, units;  // tiles of a group, steps of a tile
   float per_group, per_tile;
   __device__ __forceinline__ MoeUnits(int groups, int tiles_, int steps_, int ctas) {
     tiles = tiles_;
     steps = steps_;
-    const int total = groups * tiles, cut = min(total, ctas + ctas / 4);
-    const int length = max(4, min((int)((float)total * (float)steps / (float)(4 * ctas)), 8));
-    parts = min(moe_divide(steps + length - 1, 1.f / (float)length), kMoeMostParts);
-    whole = parts > 1 ? total - cut : total;
-    units = whole + (parts > 1 ? cut * parts : 0);
-    per_group = 1.f / (float)tiles;
-    per_tile = 1.f / (float)parts;
+    const int total = groups * tiles, rounds = max(0, moe_divide(total - ctas / 4, __frcp_rn((float)ctas)));
+    cut = total - rounds * ctas;
+    if (steps <= 8 || (total <= ctas && 10 * total >= 7 * ctas)) cut = 0;
+    const int length = max(3, min((int)((float)(cut * steps) * __frcp_rn((float)(3 * ctas))), 8));
+    parts = min(moe_divide(steps + length - 1, __frcp_rn((float)length)), kMoeMostParts);
+    whole = total - cut;
+    units = whole + cut * parts;
+    per_group = __frcp_rn((float)tiles);
+    per_tile = __frcp_rn((float)parts);
   }
 };
 struct MoeUnit {
@@ -582,7 +586,7 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
   __syncthreads();
   const uint32_t tmem = s_tmem;
   const int groups = s_groups, slots_here = s_slots;
-  const MoeUnits lists[2] = {MoeUnits(groups, w.up_tiles, w.up_steps, ctas), MoeUnits(groups, w.down_tiles, w.down_steps, ctas)};
+  auto units_of = [&](int product) { return MoeUnits(groups, product ? w.down_tiles : w.up_tiles, product ? w.down_steps : w.up_steps, ctas); };
 
   // The next unit as the producer has passed it on, or -1 at the end of a product; the same for all warps but the producer.
   uint32_t turn = 0, turn_phase = 0;
@@ -609,6 +613,8 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
       for (int k = 0; k < 4096 && !ptx::mbar_try_wait(bars + 8 * stage, phase); ++k) __nanosleep(64);
     }
   };
+  // blocks of tokens that a group's results are counted in
+  auto blocks_of = [&](int group) { return (s_group_tokens[group] + kMoeSumTokens - 1) / kMoeSumTokens; };
   // the terms of a slot's h, by the four warps of the sums
   auto terms_of_h = [&](int slot) {
     int group = 0;
@@ -617,7 +623,7 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
       if (s_group_slot[mid] <= slot) group = mid;
       else hi = mid - 1;
     }
-    ok = moe_grid_wait(&w.control->up[group], 4 * (uint32_t)w.up_tiles, &s_abort, w.status);
+    ok = moe_grid_wait(&w.control->up[group], 4 * (uint32_t)(w.up_tiles * blocks_of(group)), &s_abort, w.status);
     if (!ok) return;
     const float factor = moe_up_factor(__ldcg(w.h_top + slot));
     for (int64_t i = 8 * (tid - 96); i < a.inner; i += 8 * 128) {
@@ -690,11 +696,11 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
     ok = layer_bar_and(3, 256, ok);
     if (ok && tid == 96) moe_add_release(&w.control->done);
   };
-  // a tile of a group's first product is finished (one of four warps)
-  auto finished_up = [&](int group) {
+  // some blocks of tokens of a tile of a group's first product are finished (one of four warps)
+  auto finished_up = [&](int group, int blocks) {
     if (!FP8) moe_fence_async();
     __syncwarp();
-    if (lane == 0) moe_add_release(&w.control->up[group]);
+    if (lane == 0) moe_add_release(&w.control->up[group], blocks);
   };
 
   if (!ok && warp < 3) {
@@ -716,7 +722,7 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
     };
     auto stream = [&](auto which) {
       constexpr int product = decltype(which)::value;
-      const MoeUnits& list = lists[product];
+      const MoeUnits list = units_of(product);
       // The first units, `dealt` each, are the CTA's by its index.  The others come from the counter, whose answer takes a microsecond or two behind the copies
       // and is asked for before a unit's copies are.
       const int dealt = max(1, (int)((float)list.units / (float)ctas) * 5 / 8);
@@ -760,10 +766,11 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
     const uint64_t a0 = ptx::smem_desc_k_sw128(ring), b0 = ptx::smem_desc_k_sw128(ring + 2 * kMoeSubBytes);
     for (int product = 0; product < 2 && ok; ++product) {
       const int terms = product ? Tile::kDownTerms : Tile::kUpTerms;
+      const MoeUnits list = units_of(product);
       for (; ok; ++pieces) {
         const int u = next_unit(kMoeErrMma);
         if (u < 0) break;
-        const MoeUnit unit(lists[product], u);
+        const MoeUnit unit(list, u);
         const int cols = ((s_group_tokens[unit.group] + 7) / 8 * 8 * terms + 15) / 16 * 16;
         const uint32_t idesc = FP8 ? ptx::umma_idesc(0, 0, 128, cols) : ptx::umma_idesc(1, 1, 128, cols);
         const uint32_t acc = pieces & 1, d = tmem + acc * 2 * Tile::kCols;
@@ -797,15 +804,16 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
     uint32_t stage = 0, phase = 0;
     auto stream = [&](auto which) {
       constexpr int product = decltype(which)::value, terms = product ? Tile::kDownTerms : Tile::kUpTerms;
+      const MoeUnits list = units_of(product);
       int there = -1;  // the group whose h is known to be there
       while (ok) {
         const int u = next_unit(kMoeErrTokens);
         if (u < 0) break;
-        const MoeUnit unit(lists[product], u);
+        const MoeUnit unit(list, u);
         const int slot = s_group_slot[unit.group], n = s_group_tokens[unit.group], blocks = (n + 7) / 8;
         if (product == 1 && unit.group != there) {
           ok = FP8 ? moe_grid_wait(&w.control->terms[unit.group], 4 * (uint32_t)n, &s_abort, w.status)
-                   : moe_grid_wait(&w.control->up[unit.group], 4 * (uint32_t)w.up_tiles, &s_abort, w.status);
+                   : moe_grid_wait(&w.control->up[unit.group], 4 * (uint32_t)(w.up_tiles * blocks_of(unit.group)), &s_abort, w.status);
           if (!ok) break;
           moe_fence_async();
           there = unit.group;
@@ -846,41 +854,43 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
     const int row = tid - 96;
     auto sums_of = [&](auto which) {
       constexpr int product = decltype(which)::value;
-      const MoeUnits& list = lists[product];
-      const int cut_tiles = list.parts > 1 ? min(groups * list.tiles, ctas + ctas / 4) : 0;
-      for (int c = cta; c < cut_tiles; c += ctas) {
-        ok = ok && moe_grid_wait(&w.control->parts[product][c], 4 * (uint32_t)list.parts, &s_abort, w.status);
-        if (!ok) break;
+      const MoeUnits list = units_of(product);
+      // A task is four tokens of a tile, so that all CTAs have some where tiles are few; those of the tiles' first tokens come first.
+      constexpr int kBlocks = MAXN / kMoeSumTokens;
+      const float per_block = __frcp_rn((float)max(list.cut, 1));
+      for (int i = cta; i < list.cut * kBlocks && ok; i += ctas) {
+        const int block = moe_divide(i, per_block), c = i - block * list.cut, j0 = kMoeSumTokens * block;
         const MoeUnit unit(list, list.whole + c * list.parts);
+        const int n = s_group_tokens[unit.group];
+        if (j0 >= n) continue;
+        ok = moe_grid_wait(&w.control->parts[product][c], 4 * (uint32_t)list.parts, &s_abort, w.status);
+        if (!ok) break;
         float scale[2];
         scales_of(which, unit, row, scale);
         const float backs = backs_of(which, unit);
-        const int n = s_group_tokens[unit.group];
         const float* p = w.parts + ((int64_t)product * kMoeCutTiles + unit.cut) * kMoeMostParts * Tile::kPart + row;
-        constexpr int kBatch = 4;  // tokens whose parts are on their way together
-        for (int j0 = 0; j0 < n; j0 += kBatch) {
-          float v[kBatch][2][kMoeMostParts];
+        float v[kMoeSumTokens][2][kMoeMostParts];
 #pragma unroll
-          for (int b = 0; b < kBatch; ++b)
+        for (int b = 0; b < kMoeSumTokens; ++b)
 #pragma unroll
-            for (int sub = 0; sub < 2; ++sub)
+          for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
-              for (int c = 0; c < kMoeMostParts; ++c) v[b][sub][c] = c < list.parts && j0 + b < n ? __ldcg(p + c * Tile::kPart + (sub * MAXN + j0 + b) * 128) : 0.f;
+            for (int k = 0; k < kMoeMostParts; ++k) v[b][sub][k] = k < list.parts && j0 + b < n ? __ldcg(p + k * Tile::kPart + (sub * MAXN + j0 + b) * 128) : 0.f;
 #pragma unroll
-          for (int b = 0; b < kBatch; ++b) {
+        for (int b = 0; b < kMoeSumTokens; ++b) {
 #pragma unroll
-            for (int c = 1; c < kMoeMostParts; ++c) {
-              v[b][0][0] += v[b][0][c];
-              v[b][1][0] += v[b][1][c];
-            }
-            if (j0 + b < n) finish(which, unit, row, j0 + b, v[b][0][0], v[b][1][0], scale, backs);
+          for (int k = 1; k < kMoeMostParts; ++k) {
+            v[b][0][0] += v[b][0][k];
+            v[b][1][0] += v[b][1][k];
           }
+          if (j0 + b < n) finish(which, unit, row, j0 + b, v[b][0][0], v[b][1][0], scale, backs);
         }
-        if (product == 0) finished_up(unit.group);
+        if (product == 0) finished_up(unit.group, 1);
       }
     };
     // the slots of groups without cut tiles are ready before those tiles are, the others behind them
-    const int first_cut = moe_divide(lists[0].whole, lists[0].per_group), early = first_cut < groups ? s_group_slot[first_cut] : slots_here;
+    const MoeUnits ups = units_of(0);
+    const int first_cut = moe_divide(ups.whole, ups.per_group), early = first_cut < groups ? s_group_slot[first_cut] : slots_here;
     int mine = cta;
     if (FP8)
       for (; ok && mine < early; mine += ctas) terms_of_h(mine);
@@ -896,10 +906,11 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
     int pieces = 0;
     auto results_of = [&](auto which) {
       constexpr int product = decltype(which)::value, terms = product ? Tile::kDownTerms : Tile::kUpTerms;
+      const MoeUnits list = units_of(product);
       for (;; ++pieces) {
         const int u = next_unit(kMoeErrResults);
         if (u < 0) break;
-        const MoeUnit unit(lists[product], u);
+        const MoeUnit unit(list, u);
         const bool whole = unit.part < 0;
         const int n = s_group_tokens[unit.group];
         const uint32_t acc = pieces & 1, d = tmem + acc * 2 * Tile::kCols + lane_base;
@@ -945,7 +956,7 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
           ptx::mbar_arrive(bar_free + 8 * acc);
           if (!whole) moe_add_release(&w.control->parts[product][unit.cut]);
         }
-        if (whole && product == 0) finished_up(unit.group);
+        if (whole && product == 0) finished_up(unit.group, blocks_of(unit.group));
       }
     };
     if (ok) results_of(std::integral_constant<int, 0>());
