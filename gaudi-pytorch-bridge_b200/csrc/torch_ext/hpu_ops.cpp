@@ -1581,6 +1581,16 @@ std::tuple<at::Tensor, at::Tensor> meta_paged_attention(const at::Tensor& q, con
 // ---- what stands around the FP8 products of a decoder layer (no counterpart in the reference; the contract is in b200q.h) ----
 // rows of contiguous values; a view whose values are not contiguous is copied
 at::Tensor layer_rows(const at::Tensor& t) { return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+// the same on boundaries of 16 bytes, where rows are a multiple of that: a view between them is copied, and one row that stands for all is written out
+at::Tensor layer_aligned_rows(const at::Tensor& t) {
+  const int64_t size = (int64_t)t.element_size();
+  at::Tensor r = layer_rows(t);
+  if (t.numel() == 0 || t.size(1) * size % 16) return r;
+  const bool address = reinterpret_cast<uintptr_t>(r.const_data_ptr()) % 16 == 0, strides = r.size(0) <= 1 || (r.stride(0) * size % 16 == 0 && r.stride(0) >= r.size(1));
+  if (address && strides) return r;
+  at::Tensor c = r.contiguous();
+  return c.is_same(r) ? r.clone() : c;
+}
 int64_t layer_row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(-1); }
 // Whether a written matrix [rows][values] lies apart in itself, and from one that is read.
 b200q::CacheLayout layer_layout(const at::Tensor& t) {
@@ -1659,8 +1669,7 @@ at::Tensor& lora_add_(at::Tensor& y, const at::Tensor& x, const at::Tensor& a_w,
   TORCH_CHECK(!scales.defined() || (scales.scalar_type() == at::kFloat && scales.dim() == 1 && scales.numel() == adapters), op,
               ": scales must be a float tensor of one entry per adapter");
   layer_check_written(y, op, "y");
-  at::Tensor xr = layer_rows(x), ar = layer_rows(a_w), br = layer_rows(b_w), which = adapter.contiguous();
-  if (tokens > 1 && xr.stride(0) < k) xr = xr.contiguous();  // (one row for all tokens)
+  at::Tensor xr = layer_aligned_rows(x), ar = layer_rows(a_w), br = layer_rows(b_w), which = adapter.contiguous();
   if (scales.defined()) scales = scales.contiguous();
   for (const at::Tensor* t : {&xr, &ar, &br}) {
     if (t->numel() == 0 || y.numel() == 0 || !t->is_alias_of(y)) continue;
@@ -1724,7 +1733,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> moe_layer(const at::Tensor& x, co
   TORCH_CHECK(!num_tokens.defined() || (num_tokens.scalar_type() == at::kInt && num_tokens.numel() == 1), op, ": num_tokens must be an int32 tensor of one element");
   const auto out_dtype = out_dtype_opt.value_or(at::kBFloat16);
   TORCH_CHECK(out_dtype == at::kBFloat16 || out_dtype == at::kFloat, op, ": out_dtype must be bfloat16 or float, got ", out_dtype);
-  at::Tensor xr = layer_rows(x), rr = router.contiguous();
+  at::Tensor xr = layer_aligned_rows(x), rr = router.contiguous();
   at::Tensor out = new_tensor({tokens, hidden}, out_dtype, dev), weights = new_tensor({tokens, top_k}, at::kFloat, dev), ids = new_tensor({tokens, top_k}, at::kInt, dev);
   b200q_moe_args a{};
   a.x = xr.const_data_ptr(); a.x_stride = layer_row_stride(xr);

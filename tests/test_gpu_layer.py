@@ -253,6 +253,16 @@ def test_lora_without_scales():
     _check_lora(_run_lora(*c), *c)
 
 
+@pytest.mark.parametrize("tokens", [1, 20, 300])
+def test_lora_x_between_boundaries(tokens):
+    y, x, a, b, which, scales = _lora_case(tokens, 64, 72, 16, 3, BF16)
+    wide = torch.full((tokens, 70), math.nan, dtype=BF16)
+    wide[:, 3:67] = x
+    yd = y.cuda()
+    torch.ops.b200q.lora_add_(yd, wide.cuda()[:, 3:67], a.cuda(), b.cuda(), which.cuda(), scales.cuda())
+    _check_lora(yd, y, x, a, b, which, scales)
+
+
 @pytest.mark.parametrize("pad", [8, 3])
 def test_lora_strided(pad):
     """y a column block of a wider product, x rows of another, adapters of one layer in a stack of layers."""
@@ -480,6 +490,40 @@ def test_moe_values_of_uneven_size():
     # (what a term of x is off by, 2^-22 of the token's largest value, against that of the sum of all terms, enters like a sum's error)
     ok = want.abs() < 1e37
     _close(torch.where(ok, out.cpu().double(), 0.0), torch.where(ok, want, 0.0), torch.where(ok, 2.0 ** -18 * want.abs() + 4 * bound + 1e-37, 1.0))
+
+
+@pytest.mark.parametrize("weights", [E4M3, BF16])
+@pytest.mark.parametrize("form", ["columns", "between", "expanded", "reversed"])
+def test_moe_views_of_x(form, weights):
+    case = list(_moe_case(11, 128, 64, 6, weights))
+    x = case[0]
+    if form == "expanded":
+        case[0] = x[:1].expand(11, 128)
+        xd = x[:1].cuda().expand(11, 128)
+    elif form == "reversed":
+        case[0] = x.t().contiguous().t()
+        xd = x.t().contiguous().cuda().t()
+    else:
+        wide = torch.full((11, 160), math.nan, dtype=BF16)
+        at = 16 if form == "columns" else 3
+        wide[:, at:at + 128] = x
+        xd = wide.cuda()[:, at:at + 128]
+    out = torch.ops.b200q.moe_layer(xd, *(_cu(t) for t in case[1:]), 2)
+    _check_moe(out, case, 2)
+
+
+@pytest.mark.parametrize("experts,top_k,tokens", [(512, 16, 3), (512, 16, 40), (300, 7, 64), (129, 16, 256), (16, 16, 256), (1, 1, 256)])
+def test_moe_largest_numbers_of_experts(experts, top_k, tokens):
+    case = _moe_case(tokens, 64, 32, experts, E4M3)
+    _check_moe(_run_moe(case, top_k), case, top_k)
+
+
+@pytest.mark.parametrize("weights", [E4M3, BF16])
+@pytest.mark.parametrize("tokens,hidden,inner,experts,top_k", [(1, 4096, 128, 4, 1), (3, 128, 4096, 3, 2), (20, 2176, 272, 40, 2), (9, 1280, 1280, 8, 1), (12, 1024, 640, 148, 3), (1, 8192, 32, 1, 1), (100, 1536, 1280, 4, 2), (256, 1184, 144, 5, 1)])
+def test_moe_cut_tiles(tokens, hidden, inner, experts, top_k, weights):
+    """Long rows on few tiles, and numbers of tiles around those of the SMs: all tiles cut into parts, some, or none."""
+    case = _moe_case(tokens, hidden, inner, experts, weights)
+    _check_moe(_run_moe(case, top_k), case, top_k)
 
 
 def test_moe_of_nothing():
