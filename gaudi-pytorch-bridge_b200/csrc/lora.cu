@@ -658,15 +658,17 @@ __global__ void __launch_bounds__(lora_up_threads(TILE), lora_up_ctas(sizeof(Y) 
 size_t lora_workspace_bytes_impl(int64_t tokens, int64_t k, int64_t n, int64_t rank, int64_t adapters) {
   (void)n;
   size_t bytes = 0;
-  for (int tile : {16, 128}) {  // (which one depends on y's type)
-    const size_t b = LoraSpace(tokens, rank, lora_splits(tokens, k, adapters, tile)).bytes;
-    if (b > bytes) bytes = b;
-  }
+  for (int tile : {16, 128})  // (which one depends on y's type)
+    for (int64_t t : {tokens, tokens % kLoraChunk}) {  // (the last tokens of a long call may be cut into more parts of k than those before)
+      const size_t b = t ? LoraSpace(t, rank, lora_splits(t, k, adapters, tile)).bytes : 0;
+      if (b > bytes) bytes = b;
+    }
   return bytes;
 }
 
 static bool lora_fits_tensor_cores(const b200q_lora_args& a) {
   if (a.force_plain || a.rank % 8 || a.k % 8 || a.n % 8) return false;
+  if (a.k > 1 << 30 || a.n > 1 << 30) return false;  // (columns are counted in 32 bits, and past the last one)
   if (a.tokens > 1 && (a.x_stride % 8 || a.x_stride < a.k)) return false;
   if (a.adapters > 1 && (a.a_stride % 8 || a.b_stride % 8 || a.a_stride <= 0 || a.b_stride <= 0)) return false;
   if ((a.rank > 1 && (a.a_row_stride % 8 || a.a_row_stride < a.k)) || (a.n > 1 && (a.b_row_stride % 8 || a.b_row_stride < a.rank))) return false;

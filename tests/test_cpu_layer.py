@@ -99,6 +99,14 @@ def test_workspaces():
     assert abi.lib.b200q_moe_workspace_bytes(4, 64, 32, 16, 2) >= 4 * 2 * (64 + 32) * 4
 
 
+@pytest.mark.parametrize("adapters", [1, 40, 85, 300])
+@pytest.mark.parametrize("last", [1, 100, 4000, 7936])
+def test_lora_workspace_holds_the_last_tokens_of_a_long_call(adapters, last):
+    bytes_of = abi.lib.b200q_lora_workspace_bytes
+    for whole in (8192, 3 * 8192):
+        assert bytes_of(whole + last, 4096, 64, 64, adapters) >= max(bytes_of(8192, 4096, 64, 64, adapters), bytes_of(last, 4096, 64, 64, adapters))
+
+
 def test_schemas_and_meta():
     m = dict(device="meta")
     x = torch.empty(5, 64, dtype=BF16, **m)

@@ -242,6 +242,14 @@ def test_lora_more_tokens_than_are_taken_at_once():
     _check_lora(_run_lora(*c), *c)
 
 
+def test_lora_last_tokens_in_more_parts_than_those_before():
+    """85 adapters: 8192 tokens leave no room for parts of k, the 7936 behind them do."""
+    g = _gen(2)
+    which = torch.randint(-1, 85, (8192 + 7936,), generator=g)
+    c = _lora_case(which.numel(), 512, 32, 8, 85, BF16, which=which)
+    _check_lora(_run_lora(*c), *c)
+
+
 @pytest.mark.parametrize("many", [2048, 1500])
 def test_lora_many_adapters(many):
     c = _lora_case(50, 64, 64, 8, many, F32)
