@@ -9,7 +9,7 @@ constexpr size_t lora_align(size_t n) { return (n + 255) / 256 * 256; }
 
 __device__ __forceinline__ float lora_bf16(const void* p, int64_t at) { return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[at]); }
 __device__ __forceinline__ int lora_adapter(const b200q_lora_args& a, int64_t t) {  // or -1
-  const int i = a.adapter[t];
+  const int i = __ldcg(a.adapter + t);
   return i >= 0 && i < a.adapters ? i : -1;
 }
 
@@ -52,11 +52,14 @@ __global__ void __launch_bounds__(kLoraPlainThreads) lora_plain_up_kernel(const 
 // taken together, in whatever order they come, or its matrices are read again for each: a first kernel sorts the tokens by adapter into tiles.  In both products
 // the adapter's matrix has the 128 rows of tcgen05.mma (ranks, or columns of y) and the tile's tokens are its columns, so that a warp's results are
 // neighbours in memory: a x is bf16 times bf16, both by TMA (tokens by gathered rows); b (a x) has a x in bf16 terms that follow one another along K.
+//
+// us: 4096 tokens of 4096 -> 14336, rank 16, 4 adapters 94 (floor, y twice and x once, 38; the down kernel 21, the up kernel 45 to 65 and the sorting 5, by themselves); 64 tokens of
+// 40 adapters of rank 64 29 (9.4: four launches' worth of latency, not bytes); one token 9.8.  With mma.sync and the tokens as rows the first was 162, and one token 6.2.
 constexpr int kLoraSortThreads = 1024;
-constexpr int kLoraFew = 32;  // tokens up to which each CTA sorts for itself
+constexpr int kLoraFew = 128;  // tokens up to which each CTA sorts for itself
 constexpr int kLoraErrCopy = 831, kLoraErrMma = 832, kLoraErrResults = 833;  // status codes: a wait ran out
 
-struct LoraTile {
+struct __align__(16) LoraTile {
   int adapter, first, count, unused;  // tokens sorted[first] ...
 };
 struct LoraPlan {
@@ -165,38 +168,66 @@ __global__ void __launch_bounds__(kLoraSortThreads) lora_sort_kernel(const b200q
     if (i < per && adapter[i] >= 0) p.sorted[s_first[adapter[i]] + mine[adapter[i]] + place[i]] = begin + 32 * i + lane;
 }
 
-// The plan as a CTA finds it: made by the kernel in front, or, for few tokens, here, by one warp (a launch takes longer).
+// The plan as a CTA finds it: made by the kernel in front, or, for few tokens, here (a launch takes longer): a thread per token counts those that come before it in the order.
 struct LoraFew {
-  int tiles_used, sorted[kLoraFew];
+  int adapter[kLoraFew], sorted[kLoraFew];
   LoraTile tiles[kLoraFew];
+  uint32_t first[kLoraFew / 32];  // a bit for each place that a tile begins at
 };
 struct LoraView {
   int tiles_used;
+  bool made;  // by a kernel: in global memory, and before a kernel has waited read past L1, which may be older than it
   const LoraTile* tiles;
   const int* sorted;
+  __device__ __forceinline__ LoraTile tile(int i) const {
+    if (!made) return tiles[i];
+    const int4 v = __ldcg(reinterpret_cast<const int4*>(tiles) + i);
+    return {v.x, v.y, v.z, v.w};
+  }
+  __device__ __forceinline__ int token(int i) const { return made ? __ldcg(sorted + i) : sorted[i]; }
 };
 __device__ __forceinline__ LoraView lora_view(const b200q_lora_args& a, const LoraPlan& p, LoraFew& few) {
-  if (p.tiles_used) return {*p.tiles_used, p.tiles, p.sorted};
-  if (threadIdx.x < 32) {
-    const int lane = threadIdx.x, i = lane < a.tokens ? lora_adapter(a, lane) : -1;
-    const uint32_t same = __match_any_sync(0xFFFFFFFFu, i);
-    const int n = __popc(same);
-    const bool first = i >= 0 && lane == __ffs(same) - 1;
-    const int both = first ? n | (n + p.tile - 1) / p.tile << 16 : 0;
-    int scan = both;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xFFFFFFFFu, scan, o);
-      if (lane >= o) scan += v;
+  if (p.tiles_used) return {__ldcg(p.tiles_used), true, p.tiles, p.sorted};
+  constexpr int kNone = 0x7FFFFFFF;
+  const int t = threadIdx.x, tokens = (int)a.tokens;
+  int mine = kNone;
+  if (t < kLoraFew) {
+    if (t < tokens) {
+      const int i = lora_adapter(a, t);
+      mine = i < 0 ? kNone : i;
     }
-    const int before = scan - both, start = __shfl_sync(0xFFFFFFFFu, before & 0xFFFF, __ffs(same) - 1);
-    if (i >= 0) few.sorted[start + __popc(same & ((1u << lane) - 1u))] = lane;
-    if (first)
-      for (int j = 0; j * p.tile < n; ++j) few.tiles[(before >> 16) + j] = {i, start + j * p.tile, min(n - j * p.tile, p.tile), 0};
-    if (lane == 31) few.tiles_used = scan >> 16;
+    few.adapter[t] = mine;
+    if (t < kLoraFew / 32) few.first[t] = 0;
   }
   __syncthreads();
-  return {few.tiles_used, few.tiles, few.sorted};
+  int lower = 0, same = 0, same_before = 0;
+  if (mine != kNone) {
+#pragma unroll 4
+    for (int j = 0; j < tokens; j += 4) {
+      const int4 other = *reinterpret_cast<const int4*>(few.adapter + j);
+      const int v[4] = {other.x, other.y, other.z, other.w};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        lower += v[c] < mine;
+        same += v[c] == mine;
+        same_before += v[c] == mine && j + c < t;
+      }
+    }
+  }
+  const int place = lower + same_before;
+  const bool first = mine != kNone && same_before % p.tile == 0;
+  if (mine != kNone) few.sorted[place] = t;
+  if (first) atomicOr(&few.first[place / 32], 1u << (place & 31));
+  __syncthreads();
+  int used = 0, tile = 0;
+#pragma unroll
+  for (int i = 0; i < kLoraFew / 32; ++i) {
+    used += __popc(few.first[i]);
+    tile += __popc(few.first[i] & (place >= 32 * i + 32 ? ~0u : place <= 32 * i ? 0u : (1u << (place & 31)) - 1u));
+  }
+  if (first) few.tiles[tile] = {mine, place, min(same - same_before, p.tile), 0};
+  __syncthreads();
+  return {used, false, few.tiles, few.sorted};
 }
 
 // where a wait has run out: the last copies are waited for, as far as they come
@@ -234,7 +265,7 @@ __global__ void __launch_bounds__(32 * kLoraDownWarps, 2)
   __shared__ __align__(8) uint64_t s_bars[2 * kLoraMostStages + 4];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
-  __shared__ LoraFew s_few;
+  __shared__ __align__(16) LoraFew s_few;
   constexpr int kTmem = 2 * TILE < 32 ? 32 : 2 * TILE;
   const int tid = threadIdx.x, lane = tid & 31, warp = ptx::uniform_warp_index();
   const uint32_t ring = ptx::smem_u32(s_ring), bar_full = ptx::smem_u32(s_bars), bar_empty = bar_full + 8 * kLoraMostStages;
@@ -279,7 +310,7 @@ __global__ void __launch_bounds__(32 * kLoraDownWarps, 2)
     it.part = rest - tile * p.splits;
     it.k0 = it.part * p.part_steps;
     it.k1 = min(it.k0 + p.part_steps, p.steps);
-    it.tile = view.tiles[tile];
+    it.tile = view.tile(tile);
     return it;
   };
   if (warp == 0) {
@@ -414,16 +445,22 @@ struct LoraUpShape {
   int chunks, terms_bytes, stages, parts;  // chunks of 64 ranks; bytes of the terms; parts of n: every `parts`-th block of 128 columns
 };
 
-// 16 bytes of a row, at once or (rows between boundaries) value by value
-template <bool WHOLE, typename Y>
+// 16 bytes of a row, at once or (rows between boundaries) value by value; PAST: past L1, which the kernels before may have left older than y
+template <bool WHOLE, bool PAST, typename Y>
 __device__ __forceinline__ uint4 lora_load16(const Y* p) {
+  auto load = [](const auto* q) {
+    if constexpr (PAST) return __ldcg(q);
+    else return *q;
+  };
   if constexpr (WHOLE) {
-    return *reinterpret_cast<const uint4*>(p);
+    return load(reinterpret_cast<const uint4*>(p));
   } else if constexpr (sizeof(Y) == 4) {
-    return make_uint4(__float_as_uint(p[0]), __float_as_uint(p[1]), __float_as_uint(p[2]), __float_as_uint(p[3]));
+    const unsigned* u = reinterpret_cast<const unsigned*>(p);
+    return make_uint4(load(u), load(u + 1), load(u + 2), load(u + 3));
   } else {
-    const uint16_t* u = reinterpret_cast<const uint16_t*>(p);
-    return make_uint4(u[0] | u[1] << 16, u[2] | u[3] << 16, u[4] | u[5] << 16, u[6] | u[7] << 16);
+    const unsigned short* u = reinterpret_cast<const unsigned short*>(p);
+    auto two = [&](int i) { return (uint32_t)load(u + 2 * i) | (uint32_t)load(u + 2 * i + 1) << 16; };
+    return make_uint4(two(0), two(1), two(2), two(3));
   }
 }
 template <bool WHOLE, typename Y>
@@ -455,7 +492,7 @@ __global__ void __launch_bounds__(lora_up_threads(TILE), lora_up_ctas(sizeof(Y) 
   __shared__ uint32_t s_tmem;
   __shared__ __align__(16) float s_turn[kWarps][kBatch * kPitch];
   __shared__ int s_abort;
-  __shared__ LoraFew s_few;
+  __shared__ __align__(16) LoraFew s_few;
   constexpr int kTmem = 2 * TILE < 32 ? 32 : 2 * TILE;
   const int tid = threadIdx.x, lane = tid & 31, warp = ptx::uniform_warp_index();
   const uint32_t terms = ptx::smem_u32(s_terms), ring = terms + d.terms_bytes;
@@ -484,7 +521,10 @@ __global__ void __launch_bounds__(lora_up_threads(TILE), lora_up_ctas(sizeof(Y) 
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem = s_tmem;
-  pdl_enter();
+  // The kernel in front (a x) was waiting for all before it when it let this one begin, so that all but its own results may be read: the plan, b, and y.  Only the
+  // warps of the results wait for it, behind their first loads of y.
+  constexpr bool kEarly = TILE == 16;
+  if (!kEarly) pdl_enter();
   const LoraView view = lora_view(a, p, s_few);
   const int items = view.tiles_used * d.parts, n_blocks = (int)((a.n + 127) / 128);
   bool ok = true;
@@ -492,7 +532,7 @@ __global__ void __launch_bounds__(lora_up_threads(TILE), lora_up_ctas(sizeof(Y) 
     uint32_t stage = 0, phase = 0;
     int made = 0;
     for (int i = blockIdx.x; i < items && ok; i += gridDim.x) {
-      const int tile = i / d.parts, part = i - tile * d.parts, adapter = view.tiles[tile].adapter;
+      const int tile = i / d.parts, part = i - tile * d.parts, adapter = view.tile(tile).adapter;
       for (int n = part; n < n_blocks && ok; n += d.parts)
         for (int c = 0; c < d.chunks; ++c) {
           ok = ptx::mbar_wait_uniform(bar_empty + 8 * stage, phase ^ 1, &s_abort, p.status, kLoraErrCopy);
@@ -516,7 +556,7 @@ __global__ void __launch_bounds__(lora_up_threads(TILE), lora_up_ctas(sizeof(Y) 
     const uint64_t a0 = ptx::smem_desc_k_sw128(ring), b0 = ptx::smem_desc_k_sw128(terms);
     for (int i = blockIdx.x; i < items && ok; i += gridDim.x, ++item) {
       const int tile = i / d.parts, part = i - tile * d.parts;
-      const uint32_t idesc = ptx::umma_idesc(1, 1, 128, lora_columns(view.tiles[tile].count));
+      const uint32_t idesc = ptx::umma_idesc(1, 1, 128, lora_columns(view.tile(tile).count));
       ok = ptx::mbar_wait_uniform(bar_terms, item & 1, &s_abort, p.status, kLoraErrMma);
       for (int n = part; n < n_blocks && ok; n += d.parts, ++done) {
         const uint32_t acc = done & 1, out = tmem + acc * TILE;
@@ -549,18 +589,19 @@ __global__ void __launch_bounds__(lora_up_threads(TILE), lora_up_ctas(sizeof(Y) 
     float* const turn = s_turn[warp - 2];
     for (int i = blockIdx.x; i < items; i += gridDim.x, ++item) {  // (all its warps come to each item's barrier, whatever became of their waits)
       const int index = i / d.parts, part = i - index * d.parts;
-      const LoraTile tile = view.tiles[index];
+      const LoraTile tile = view.tile(index);
       const int first = tile.first + kHalf * half, count = min(tile.count - kHalf * half, kHalf);  // of this half
       int token[kPieces];  // of a lane's pieces; -1 behind the last one
       uint4 old[kPieces];
       Y* const columns = static_cast<Y*>(a.y) + my_column;
       auto ask = [&](int c, int n) {
-        if (token[c] >= 0 && 128 * n + my_column < a.n) old[c] = lora_load16<WHOLE>(columns + token[c] * a.y_stride + 128 * n);
+        if (token[c] >= 0 && 128 * n + my_column < a.n) old[c] = lora_load16<WHOLE, kEarly>(columns + token[c] * a.y_stride + 128 * n);
       };
 #pragma unroll
-      for (int c = 0; c < kPieces; ++c) token[c] = c * kRows + my_row < count ? view.sorted[first + c * kRows + my_row] : -1;
+      for (int c = 0; c < kPieces; ++c) token[c] = c * kRows + my_row < count ? view.token(first + c * kRows + my_row) : -1;
 #pragma unroll
       for (int c = 0; c < kPieces; ++c) ask(c, part);
+      if (kEarly && item == 0) pdl_enter();
       ok = ok && ptx::mbar_wait_uniform(bar_used, (item & 1) ^ 1, &s_abort, p.status, kLoraErrResults);  // (the products with the terms before are done)
       const float scale = a.scales ? a.scales[tile.adapter] : 1.f;
       const int pieces = 8 * d.chunks;  // of eight ranks
@@ -648,6 +689,7 @@ __global__ void __launch_bounds__(lora_up_threads(TILE), lora_up_ctas(sizeof(Y) 
         if (lane == 0) ptx::mbar_arrive(bar_free + 8 * acc);
       }
     }
+    if (kEarly && blockIdx.x >= items) pdl_enter();  // (no kernel is done before those in front of it)
   }
   ptx::tc_fence_before();
   __syncthreads();

@@ -626,8 +626,9 @@ int b200q_selftest_paged_wait_timeout(const b200q_paged_attention_args* args, in
  * x             F32 / BF16 [tokens][dim], row stride in elements, values contiguous
  * residual      type and shape of x, row stride >= dim, or NULL.  No byte may belong to an input as well
  * weight        F32 / BF16 [dim], or NULL: 1
- * out           BF16 / E4M3 / E5M2 [tokens][dim] contiguous;  kept: bf16 alike, or NULL;  scale_inv: fp32 [tokens], or NULL
- * Rows on boundaries of eight values run in 16-byte accesses; others element by element.
+ * out           BF16 / E4M3 / E5M2 [tokens][dim] contiguous;  kept: bf16 alike, or NULL;  scale_inv: fp32 [tokens], or NULL; apart from all inputs
+ * Rows on boundaries of eight values, and rows of any length that lie alike in all of x, residual and the outputs (packed, on addresses of multiples of 16 bytes), run in
+ * 16-byte accesses; others value by value.  Status 811: a row's copy did not arrive (its outputs, and those of the rows behind it that the block has, are not written).
  */
 typedef struct b200q_norm_args {
   const void* x;
@@ -652,15 +653,15 @@ int b200q_add_rms_norm_cast(const b200q_norm_args* args);
  * lora_add: low-rank adapters of many requests beside a product that they share.  Per token t with i = adapter[t] in [0, adapters)
  *   y[t] = T(y[t] + scales[i] * b[i] (a[i] x[t]))
  * and nothing for the others, whose rows of y are neither read nor written.  a x is summed in fp32 and meets b as three bf16 terms (24 bits) where y
- * is fp32 and as two (16 bits) where it is bf16; that product is summed in fp32, and rounded once with y.
+ * is fp32 and as two (16 bits) where it is bf16; that product is summed in fp32, and rounded once with y.  A scaled a x beyond the end of bf16 makes the token's y NaN.
  *
  * x             bf16 [tokens][k];  y: F32 / BF16 [tokens][n], row stride >= n; row strides in elements, values contiguous
  * a             bf16 [adapters][rank][k];  b: bf16 [adapters][n][rank]; strides of adapter and row in elements, values contiguous
  * adapter       int32 [tokens];  scales: fp32 [adapters], or NULL: 1
  * rank <= 256, adapters <= 2048
  * workspace     b200q_lora_workspace_bytes(...) bytes, 16-byte aligned, not shared by calls that may overlap
- * A rank of a multiple of 8, k and n of multiples of 8 and rows on 16-byte boundaries run tensor-core kernels, anything else (or
- * force_plain = 1) a plain one.  y must not overlap the inputs.  The same call gives the same bytes.
+ * rank, k and n of multiples of 8 with rows of x, a and b apart and on 16-byte boundaries run tensor-core kernels (y may lie anywhere), anything else (or
+ * force_plain = 1) plain ones.  y must not overlap the inputs.  The same call gives the same bytes.  Status 831 to 833: a wait ran out (some of y is as it was).
  */
 typedef struct b200q_lora_args {
   const void* x;
@@ -697,9 +698,10 @@ int b200q_lora_add(const b200q_lora_args* args);
  * out           BF16 / F32 [tokens][hidden];  weights fp32, ids int32 [tokens][top_k];  all but x contiguous
  * experts <= 512, top_k <= min(16, experts)
  * workspace     b200q_moe_workspace_bytes(...) bytes, 16-byte aligned, not shared by calls that may overlap
- * hidden and inner of multiples of 16 bytes with 16-byte aligned weights run the tensor-core kernel, anything else (or force_plain = 1) plain ones.
+ * hidden and inner of at most 65536 and multiples of 16 bytes (of weights), with weights, out and the rows of x apart and on 16-byte boundaries, run the tensor-core
+ * kernel, anything else (or force_plain = 1) plain ones.  It is launched cooperatively, one block on each SM.
  * Weights of the chosen experts are read once for up to 32 tokens each, and batches of more than 256 tokens are taken 256 at a time: for a few tokens.
- * The same call gives the same bytes.
+ * An h beyond the end of fp32 makes its token's out NaN.  The same call gives the same bytes.  Status 821 to 825: a wait ran out (out is NaN where a sum is missing).
  */
 typedef struct b200q_moe_args {
   const void* x;
