@@ -53,8 +53,9 @@ __global__ void __launch_bounds__(kLoraPlainThreads) lora_plain_up_kernel(const 
 // the adapter's matrix has the 128 rows of tcgen05.mma (ranks, or columns of y) and the tile's tokens are its columns, so that a warp's results are
 // neighbours in memory: a x is bf16 times bf16, both by TMA (tokens by gathered rows); b (a x) has a x in bf16 terms that follow one another along K.
 //
-// us: 4096 tokens of 4096 -> 14336, rank 16, 4 adapters 94 (floor, y twice and x once, 38; the down kernel 21, the up kernel 45 to 65 and the sorting 5, by themselves); 64 tokens of
-// 40 adapters of rank 64 29 (9.4: four launches' worth of latency, not bytes); one token 9.8.  With mma.sync and the tokens as rows the first was 162, and one token 6.2.
+// us: 4096 tokens of 4096 -> 14336, rank 64, 8 adapters in runs of 512 tokens 92 (floor, y twice and x once, 38: the sorting 5, a x 20, the rest b (a x)); 64 tokens of 8192 -> 8192 with
+// some 40 of 64 adapters of rank 32 23 (floor 9.4: the steps of two kernels one behind the other); one token of 4096 -> 4096, rank 16, 9.3 (8.2 on the device), two kernels' latency.
+// With mma.sync and the tokens as rows these were 162, 32 and 6.2.
 constexpr int kLoraSortThreads = 1024;
 constexpr int kLoraFew = 128;  // tokens up to which each CTA sorts for itself
 constexpr int kLoraErrCopy = 831, kLoraErrMma = 832, kLoraErrResults = 833;  // status codes: a wait ran out
@@ -86,15 +87,18 @@ struct LoraSpace {
 // are on their way.
 static int lora_tile_tokens(int64_t tokens, int64_t rank, int64_t adapters, bool wide) {
   const int64_t t = tokens < kLoraChunk ? tokens : kLoraChunk, blocks = (wide ? 3 : 2) * ((rank + 63) / 64);
-  return t >= 24 * adapters && t > 64 && blocks <= 6 ? 128 : 16;
+  return t >= 24 * adapters && t > kLoraFew && blocks <= 6 ? 128 : 16;
 }
-// tiles that the tokens may need at most, and parts of k such that none of an SM's two CTAs has a second item (a second round costs as much as the first)
+// CTAs of an SM that share a x: more where ranks are few, because an item is a chain of steps
+// (64 tokens of 40 adapters of rank 32, 8192 values each: 24.3 us with two, 22.6 with four)
+static int lora_down_ctas(int64_t rank, int tile) { return tile == 16 && rank <= 64 ? 4 : 2; }
+// tiles that the tokens may need at most, and parts of k such that no CTA has a second item (a second round costs as much as the first)
 static int64_t lora_most_tiles(int64_t tokens, int64_t adapters, int tile) {
   const int64_t t = tokens < kLoraChunk ? tokens : kLoraChunk, shared = adapters + t / tile;
   return t < shared ? t : shared;
 }
-static int64_t lora_splits(int64_t tokens, int64_t k, int64_t adapters, int tile) {
-  const int64_t most = (k + 255) / 256, tiles = lora_most_tiles(tokens, adapters, tile), wanted = 2 * kNumSMs / tiles;
+static int64_t lora_splits(int64_t tokens, int64_t k, int64_t rank, int64_t adapters, int tile) {
+  const int64_t most = (k + 255) / 256, tiles = lora_most_tiles(tokens, adapters, tile), wanted = lora_down_ctas(rank, tile) * kNumSMs / tiles;
   const int64_t splits = wanted < most ? wanted : most;
   return splits < 1 ? 1 : splits < 16 ? splits : 16;
 }
@@ -186,8 +190,9 @@ struct LoraView {
   }
   __device__ __forceinline__ int token(int i) const { return made ? __ldcg(sorted + i) : sorted[i]; }
 };
+template <int TILE>
 __device__ __forceinline__ LoraView lora_view(const b200q_lora_args& a, const LoraPlan& p, LoraFew& few) {
-  if (p.tiles_used) return {__ldcg(p.tiles_used), true, p.tiles, p.sorted};
+  if (TILE > 16 || p.tiles_used) return {__ldcg(p.tiles_used), true, p.tiles, p.sorted};
   constexpr int kNone = 0x7FFFFFFF;
   const int t = threadIdx.x, tokens = (int)a.tokens;
   int mine = kNone;
@@ -258,7 +263,7 @@ struct LoraDownShape {
 };
 
 template <int TILE, bool EXACT>  // EXACT: no more than kLoraSub steps are added inside the tensor core
-__global__ void __launch_bounds__(32 * kLoraDownWarps, 2)
+__global__ void __launch_bounds__(32 * kLoraDownWarps, TILE == 16 ? 4 : 2)
     lora_down_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_run, const b200q_lora_args a, const LoraPlan p, const LoraDownShape d) {
   extern __shared__ uint8_t s_raw[];
   uint8_t* const s_ring = s_raw + (0u - ptx::smem_u32(s_raw) & 1023u);
@@ -294,7 +299,7 @@ __global__ void __launch_bounds__(32 * kLoraDownWarps, 2)
   ptx::tc_fence_after();
   const uint32_t tmem = s_tmem;
   pdl_enter();
-  const LoraView view = lora_view(a, p, s_few);
+  const LoraView view = lora_view<TILE>(a, p, s_few);
   const int blocks = ((int)a.rank + 127) / 128, items = view.tiles_used * p.splits * blocks;
   bool ok = true;
   // item: block of ranks, part of k, tile
@@ -440,7 +445,7 @@ __global__ void __launch_bounds__(32 * kLoraDownWarps, 2)
 // 14336 columns.)
 constexpr int lora_result_warps(int tile) { return tile == 16 ? 4 : 8; }
 constexpr int lora_up_threads(int tile) { return 64 + 32 * lora_result_warps(tile); }  // copies, MMAs, results
-constexpr int lora_up_ctas(int wide, int tile) { return tile == 16 ? 4 : wide ? 1 : 2; }  // of an SM
+constexpr int lora_up_ctas(int wide, int tile) { return tile == 16 ? (wide ? 3 : 4) : wide ? 1 : 2; }  // of an SM, as many as the registers are enough for
 struct LoraUpShape {
   int chunks, terms_bytes, stages, parts;  // chunks of 64 ranks; bytes of the terms; parts of n: every `parts`-th block of 128 columns
 };
@@ -525,7 +530,7 @@ __global__ void __launch_bounds__(lora_up_threads(TILE), lora_up_ctas(sizeof(Y) 
   // warps of the results wait for it, behind their first loads of y.
   constexpr bool kEarly = TILE == 16;
   if (!kEarly) pdl_enter();
-  const LoraView view = lora_view(a, p, s_few);
+  const LoraView view = lora_view<TILE>(a, p, s_few);
   const int items = view.tiles_used * d.parts, n_blocks = (int)((a.n + 127) / 128);
   bool ok = true;
   if (warp == 0) {
@@ -611,7 +616,7 @@ __global__ void __launch_bounds__(lora_up_threads(TILE), lora_up_ctas(sizeof(Y) 
         if (r < a.rank) {
           const float4* low = reinterpret_cast<const float4*>(p.low + (int64_t)view.sorted[tile.first + j] * a.rank + r);
           const int64_t step = a.tokens * a.rank / 4;
-          constexpr int kTogether = 4;  // parts of k on their way
+          constexpr int kTogether = sizeof(Y) == 4 ? 2 : 4;  // parts of k on their way (with more, an fp32 y's kernel spills)
           for (int s0 = 0; s0 < p.splits; s0 += kTogether) {
             float4 x[kTogether][2];
 #pragma unroll
@@ -702,7 +707,7 @@ size_t lora_workspace_bytes_impl(int64_t tokens, int64_t k, int64_t n, int64_t r
   size_t bytes = 0;
   for (int tile : {16, 128})  // (which one depends on y's type)
     for (int64_t t : {tokens, tokens % kLoraChunk}) {  // (the last tokens of a long call may be cut into more parts of k than those before)
-      const size_t b = t ? LoraSpace(t, rank, lora_splits(t, k, adapters, tile)).bytes : 0;
+      const size_t b = t ? LoraSpace(t, rank, lora_splits(t, k, rank, adapters, tile)).bytes : 0;
       if (b > bytes) bytes = b;
     }
   return bytes;
@@ -747,12 +752,13 @@ template <int TILE, bool EXACT>
 static int lora_launch_down(const b200q_lora_args& a, const LoraPlan& p, int64_t tiles, cudaStream_t st) {
   static std::atomic<int> done[kMaxDevices];
   if (int rc = lora_ready(reinterpret_cast<const void*>(lora_down_kernel<TILE, EXACT>), done, kLoraShared)) return rc;
-  const LoraDownShape d((int)a.rank, TILE, kLoraShared - 1024);
+  const int ctas = lora_down_ctas(a.rank, TILE);
+  const LoraDownShape d((int)a.rank, TILE, (ctas == 2 ? kLoraShared : 220 * 1024 / ctas - 4096) - 1024);
   CUtensorMap map_a, map_x, map_run;
   if (int rc = lora_map(&map_a, a.a, a.k, a.rank, a.adapters, a.a_row_stride, a.a_stride, d.rows, 3)) return rc;
   if (int rc = lora_map(&map_x, a.x, a.k, a.tokens, 1, a.x_stride, 0, 1, 2)) return rc;
   if (int rc = lora_map(&map_run, a.x, a.k, a.tokens, 1, a.x_stride, 0, TILE, 2)) return rc;
-  const int64_t items = tiles * p.splits * ((a.rank + 127) / 128), most = 2 * kNumSMs;
+  const int64_t items = tiles * p.splits * ((a.rank + 127) / 128), most = ctas * kNumSMs;
   // (the rows behind a block's ranks, which the product reads too and whose results nobody looks at, are within the allocation)
   launch_dependent(lora_down_kernel<TILE, EXACT>, dim3((unsigned)(items < most ? items : most)), dim3(32 * kLoraDownWarps), (size_t)d.stages * d.stage + 16384 + 1024, st, map_a, map_x,
                    map_run, a, p, d);
@@ -770,7 +776,7 @@ static int lora_launch_up(const b200q_lora_args& a, const LoraPlan& p, int64_t t
   d.chunks = (int)((a.rank + 63) / 64);
   d.terms_bytes = kTerms * d.chunks * TILE * 128;
   // as many stages as leave room for the SM's other CTAs, if that is two; else as many as there is room for
-  constexpr int kCtas = lora_up_ctas(sizeof(Y) == 4, TILE), kHere = 4 * lora_result_warps(TILE) * 16 * 36 + 1024;  // (static memory)
+  constexpr int kCtas = lora_up_ctas(sizeof(Y) == 4, TILE), kHere = 4 * lora_result_warps(TILE) * 16 * 36 + (int)sizeof(LoraFew) + 512;  // (static memory)
   constexpr int kOne = (226 * 1024 / kCtas - 1024 - kHere) / 1024 * 1024, kShare = kOne < kMost ? kOne : kMost;
   const int room = (d.terms_bytes + 2 * 16384 + 1024 <= kShare ? kShare : kMost) - 1024 - d.terms_bytes;
   d.stages = room / 16384 < kLoraMostStages ? room / 16384 : kLoraMostStages;
@@ -792,7 +798,7 @@ static int lora_launch_up_tile(const b200q_lora_args& a, const LoraPlan& p, int6
 
 static int lora_chunk_fast(const b200q_lora_args& a, cudaStream_t st) {
   const int tile = lora_tile_tokens(a.tokens, a.rank, a.adapters, a.y_dtype == B200Q_F32);
-  const int64_t splits = lora_splits(a.tokens, a.k, a.adapters, tile), tiles = lora_most_tiles(a.tokens, a.adapters, tile);
+  const int64_t splits = lora_splits(a.tokens, a.k, a.rank, a.adapters, tile), tiles = lora_most_tiles(a.tokens, a.adapters, tile);
   const LoraSpace space(a.tokens, a.rank, splits);
   uint8_t* w = static_cast<uint8_t*>(a.workspace);
   LoraPlan p;
