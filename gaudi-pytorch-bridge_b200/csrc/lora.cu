@@ -53,8 +53,8 @@ __global__ void __launch_bounds__(kLoraPlainThreads) lora_plain_up_kernel(const 
 // the adapter's matrix has the 128 rows of tcgen05.mma (ranks, or columns of y) and the tile's tokens are its columns, so that a warp's results are
 // neighbours in memory: a x is bf16 times bf16, both by TMA (tokens by gathered rows); b (a x) has a x in bf16 terms that follow one another along K.
 //
-// us: 4096 tokens of 4096 -> 14336, rank 64, 8 adapters in runs of 512 tokens 92 (floor, y twice and x once, 38: the sorting 5, a x 20, the rest b (a x)); 64 tokens of 8192 -> 8192 with
-// some 40 of 64 adapters of rank 32 23 (floor 9.4: the steps of two kernels one behind the other); one token of 4096 -> 4096, rank 16, 9.3 (8.2 on the device), two kernels' latency.
+// us: 4096 tokens of 4096 -> 14336, rank 64, 8 adapters in runs of 512 tokens 81 to 89 (floor, y twice and x once, 38: the sorting 5, a x 18, the rest b (a x)); 64 tokens of 8192 -> 8192 with
+// some 40 of 64 adapters of rank 32 23 (floor 9.4: the steps of two kernels one behind the other); one token of 4096 -> 4096, rank 16, 9.3 (7.2 on the device), two kernels' latency.
 // With mma.sync and the tokens as rows these were 162, 32 and 6.2.
 constexpr int kLoraSortThreads = 1024;
 constexpr int kLoraFew = 128;  // tokens up to which each CTA sorts for itself
@@ -68,7 +68,8 @@ struct LoraPlan {
   LoraTile* tiles;
   int* sorted;
   float* low;  // [splits][tokens][rank]: a x, in parts over k
-  int splits, steps, part_steps;  // parts of k; steps of 64 values of k, and of a part
+  int splits, slots;  // parts of k at most; CTAs that share a x
+  int steps;          // of 64 values of k
   int tile;                       // tokens of a tile at most
   int* status;
 };
@@ -92,13 +93,15 @@ static int lora_tile_tokens(int64_t tokens, int64_t rank, int64_t adapters, bool
 // CTAs of an SM that share a x: more where ranks are few, because an item is a chain of steps
 // (64 tokens of 40 adapters of rank 32, 8192 values each: 24.3 us with two, 22.6 with four)
 static int lora_down_ctas(int64_t rank, int tile) { return tile == 16 && rank <= 64 ? 4 : 2; }
-// tiles that the tokens may need at most, and parts of k such that no CTA has a second item (a second round costs as much as the first)
+// tiles that the tokens may need at most, and parts of k at most.  The kernels, which know how many tiles there are, take as many parts as leave no CTA a second item (a second
+// round costs as much as the first); the workspace has room for as many as that can be, which is little where tokens are few, and where they are many for what the most tiles leave.
 static int64_t lora_most_tiles(int64_t tokens, int64_t adapters, int tile) {
   const int64_t t = tokens < kLoraChunk ? tokens : kLoraChunk, shared = adapters + t / tile;
   return t < shared ? t : shared;
 }
 static int64_t lora_splits(int64_t tokens, int64_t k, int64_t rank, int64_t adapters, int tile) {
-  const int64_t most = (k + 255) / 256, tiles = lora_most_tiles(tokens, adapters, tile), wanted = lora_down_ctas(rank, tile) * kNumSMs / tiles;
+  const int64_t most = (k + 255) / 256, items = lora_most_tiles(tokens, adapters, tile) * ((rank + 127) / 128);
+  const int64_t wanted = tokens <= kLoraFew ? 16 : lora_down_ctas(rank, tile) * kNumSMs / items;
   const int64_t splits = wanted < most ? wanted : most;
   return splits < 1 ? 1 : splits < 16 ? splits : 16;
 }
@@ -190,6 +193,7 @@ struct LoraView {
   }
   __device__ __forceinline__ int token(int i) const { return made ? __ldcg(sorted + i) : sorted[i]; }
 };
+__device__ __forceinline__ int lora_parts(const LoraPlan& p, int items) { return max(1, min(p.splits, p.slots / max(items, 1))); }
 template <int TILE>
 __device__ __forceinline__ LoraView lora_view(const b200q_lora_args& a, const LoraPlan& p, LoraFew& few) {
   if (TILE > 16 || p.tiles_used) return {__ldcg(p.tiles_used), true, p.tiles, p.sorted};
@@ -300,7 +304,8 @@ __global__ void __launch_bounds__(32 * kLoraDownWarps, TILE == 16 ? 4 : 2)
   const uint32_t tmem = s_tmem;
   pdl_enter();
   const LoraView view = lora_view<TILE>(a, p, s_few);
-  const int blocks = ((int)a.rank + 127) / 128, items = view.tiles_used * p.splits * blocks;
+  const int blocks = ((int)a.rank + 127) / 128, splits = lora_parts(p, view.tiles_used * blocks), part_steps = (p.steps + splits - 1) / splits;
+  const int items = view.tiles_used * splits * blocks;
   bool ok = true;
   // item: block of ranks, part of k, tile
   struct Item {
@@ -311,10 +316,10 @@ __global__ void __launch_bounds__(32 * kLoraDownWarps, TILE == 16 ? 4 : 2)
     Item it;
     it.block = blocks == 1 ? 0 : i & 1;  // (at most two)
     const int rest = blocks == 1 ? i : i >> 1;
-    const int tile = rest / p.splits;
-    it.part = rest - tile * p.splits;
-    it.k0 = it.part * p.part_steps;
-    it.k1 = min(it.k0 + p.part_steps, p.steps);
+    const int tile = rest / splits;
+    it.part = rest - tile * splits;
+    it.k0 = it.part * part_steps;
+    it.k1 = min(it.k0 + part_steps, p.steps);
     it.tile = view.tile(tile);
     return it;
   };
@@ -447,7 +452,7 @@ constexpr int lora_result_warps(int tile) { return tile == 16 ? 4 : 8; }
 constexpr int lora_up_threads(int tile) { return 64 + 32 * lora_result_warps(tile); }  // copies, MMAs, results
 constexpr int lora_up_ctas(int wide, int tile) { return tile == 16 ? (wide ? 3 : 4) : wide ? 1 : 2; }  // of an SM, as many as the registers are enough for
 struct LoraUpShape {
-  int chunks, terms_bytes, stages, parts;  // chunks of 64 ranks; bytes of the terms; parts of n: every `parts`-th block of 128 columns
+  int chunks, terms_bytes, stages;  // chunks of 64 ranks; bytes of the terms
 };
 
 // 16 bytes of a row, at once or (rows between boundaries) value by value; PAST: past L1, which the kernels before may have left older than y
@@ -531,14 +536,16 @@ __global__ void __launch_bounds__(lora_up_threads(TILE), lora_up_ctas(sizeof(Y) 
   constexpr bool kEarly = TILE == 16;
   if (!kEarly) pdl_enter();
   const LoraView view = lora_view<TILE>(a, p, s_few);
-  const int items = view.tiles_used * d.parts, n_blocks = (int)((a.n + 127) / 128);
+  // parts of n (every `parts`-th block of 128 columns): as many as leave no CTA a second item.  (Found by the host from the most tiles that there may be, they left every fourth
+  // CTA without one where 8 adapters have 512 tokens each: 91 us, now 81 to 89.)
+  const int n_blocks = (int)((a.n + 127) / 128), parts = max(1, min(n_blocks, (int)gridDim.x / max(view.tiles_used, 1))), items = view.tiles_used * parts;
   bool ok = true;
   if (warp == 0) {
     uint32_t stage = 0, phase = 0;
     int made = 0;
     for (int i = blockIdx.x; i < items && ok; i += gridDim.x) {
-      const int tile = i / d.parts, part = i - tile * d.parts, adapter = view.tile(tile).adapter;
-      for (int n = part; n < n_blocks && ok; n += d.parts)
+      const int tile = i / parts, part = i - tile * parts, adapter = view.tile(tile).adapter;
+      for (int n = part; n < n_blocks && ok; n += parts)
         for (int c = 0; c < d.chunks; ++c) {
           ok = ptx::mbar_wait_uniform(bar_empty + 8 * stage, phase ^ 1, &s_abort, p.status, kLoraErrCopy);
           if (!ok) break;
@@ -560,10 +567,10 @@ __global__ void __launch_bounds__(lora_up_threads(TILE), lora_up_ctas(sizeof(Y) 
     int done = 0, item = 0;
     const uint64_t a0 = ptx::smem_desc_k_sw128(ring), b0 = ptx::smem_desc_k_sw128(terms);
     for (int i = blockIdx.x; i < items && ok; i += gridDim.x, ++item) {
-      const int tile = i / d.parts, part = i - tile * d.parts;
+      const int tile = i / parts, part = i - tile * parts;
       const uint32_t idesc = ptx::umma_idesc(1, 1, 128, lora_columns(view.tile(tile).count));
       ok = ptx::mbar_wait_uniform(bar_terms, item & 1, &s_abort, p.status, kLoraErrMma);
-      for (int n = part; n < n_blocks && ok; n += d.parts, ++done) {
+      for (int n = part; n < n_blocks && ok; n += parts, ++done) {
         const uint32_t acc = done & 1, out = tmem + acc * TILE;
         ok = ptx::mbar_wait_uniform(bar_free + 8 * acc, ((done >> 1) & 1) ^ 1, &s_abort, p.status, kLoraErrMma);
         if (!ok) break;
@@ -593,7 +600,7 @@ __global__ void __launch_bounds__(lora_up_threads(TILE), lora_up_ctas(sizeof(Y) 
     const int wt = tid - 64, quarter = warp & 3, half = (warp - 2) >> 2, my_row = lane / kLanes, my_column = 32 * quarter + lane % kLanes * kPer;
     float* const turn = s_turn[warp - 2];
     for (int i = blockIdx.x; i < items; i += gridDim.x, ++item) {  // (all its warps come to each item's barrier, whatever became of their waits)
-      const int index = i / d.parts, part = i - index * d.parts;
+      const int index = i / parts, part = i - index * parts;
       const LoraTile tile = view.tile(index);
       const int first = tile.first + kHalf * half, count = min(tile.count - kHalf * half, kHalf);  // of this half
       int token[kPieces];  // of a lane's pieces; -1 behind the last one
@@ -610,19 +617,20 @@ __global__ void __launch_bounds__(lora_up_threads(TILE), lora_up_ctas(sizeof(Y) 
       ok = ok && ptx::mbar_wait_uniform(bar_used, (item & 1) ^ 1, &s_abort, p.status, kLoraErrResults);  // (the products with the terms before are done)
       const float scale = a.scales ? a.scales[tile.adapter] : 1.f;
       const int pieces = 8 * d.chunks;  // of eight ranks
+      const int splits = lora_parts(p, view.tiles_used * ((d.chunks + 1) / 2));
       for (int q = wt; ok && q < tile.count * pieces; q += 32 * kWarps) {
         const int j = q / pieces, r = 8 * (q - j * pieces);
         float v[8] = {};
         if (r < a.rank) {
           const float4* low = reinterpret_cast<const float4*>(p.low + (int64_t)view.sorted[tile.first + j] * a.rank + r);
           const int64_t step = a.tokens * a.rank / 4;
-          constexpr int kTogether = sizeof(Y) == 4 ? 2 : 4;  // parts of k on their way (with more, an fp32 y's kernel spills)
-          for (int s0 = 0; s0 < p.splits; s0 += kTogether) {
+          constexpr int kTogether = TILE == 16 && sizeof(Y) == 2 ? 4 : 2;  // parts of k on their way: few tokens have many (one token 7.2 us, with two 7.7); else registers
+          for (int s0 = 0; s0 < splits; s0 += kTogether) {
             float4 x[kTogether][2];
 #pragma unroll
             for (int s = 0; s < kTogether; ++s)
 #pragma unroll
-              for (int h = 0; h < 2; ++h) x[s][h] = s0 + s < p.splits ? __ldcg(low + (s0 + s) * step + h) : make_float4(0.f, 0.f, 0.f, 0.f);
+              for (int h = 0; h < 2; ++h) x[s][h] = s0 + s < splits ? __ldcg(low + (s0 + s) * step + h) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int s = 0; s < kTogether; ++s) {
               v[0] += x[s][0].x; v[1] += x[s][0].y; v[2] += x[s][0].z; v[3] += x[s][0].w;
@@ -648,7 +656,7 @@ __global__ void __launch_bounds__(lora_up_threads(TILE), lora_up_ctas(sizeof(Y) 
       ok = layer_bar_and(1, 32 * kWarps, ok);
       if (!ok) break;
       if (lane == 0) ptx::mbar_arrive(bar_terms);
-      for (int n = part; n < n_blocks && ok; n += d.parts, ++done) {
+      for (int n = part; n < n_blocks && ok; n += parts, ++done) {
         const uint32_t acc = done & 1, in = tmem + acc * TILE + kHalf * half + ((uint32_t)(32 * quarter) << 16);
         ok = ptx::mbar_wait_uniform(bar_done + 8 * acc, (done >> 1) & 1, &s_abort, p.status, kLoraErrResults);
         if (!ok) break;
@@ -686,7 +694,7 @@ __global__ void __launch_bounds__(lora_up_threads(TILE), lora_up_ctas(sizeof(Y) 
               w.w = pack_bf16x2(__uint_as_float(old[c].w << 16) + z.z, __uint_as_float(old[c].w & 0xFFFF0000u) + z.w);
             }
             if (there && token[c] >= 0) lora_store16<WHOLE>(columns + token[c] * a.y_stride + 128 * n, w);
-            ask(c, n + d.parts);
+            ask(c, n + parts);
           }
         }
         ptx::tc_fence_before();
@@ -758,7 +766,7 @@ static int lora_launch_down(const b200q_lora_args& a, const LoraPlan& p, int64_t
   if (int rc = lora_map(&map_a, a.a, a.k, a.rank, a.adapters, a.a_row_stride, a.a_stride, d.rows, 3)) return rc;
   if (int rc = lora_map(&map_x, a.x, a.k, a.tokens, 1, a.x_stride, 0, 1, 2)) return rc;
   if (int rc = lora_map(&map_run, a.x, a.k, a.tokens, 1, a.x_stride, 0, TILE, 2)) return rc;
-  const int64_t items = tiles * p.splits * ((a.rank + 127) / 128), most = ctas * kNumSMs;
+  const int64_t items = tiles * p.splits * ((a.rank + 127) / 128), most = p.slots;
   // (the rows behind a block's ranks, which the product reads too and whose results nobody looks at, are within the allocation)
   launch_dependent(lora_down_kernel<TILE, EXACT>, dim3((unsigned)(items < most ? items : most)), dim3(32 * kLoraDownWarps), (size_t)d.stages * d.stage + 16384 + 1024, st, map_a, map_x,
                    map_run, a, p, d);
@@ -780,9 +788,7 @@ static int lora_launch_up(const b200q_lora_args& a, const LoraPlan& p, int64_t t
   constexpr int kOne = (226 * 1024 / kCtas - 1024 - kHere) / 1024 * 1024, kShare = kOne < kMost ? kOne : kMost;
   const int room = (d.terms_bytes + 2 * 16384 + 1024 <= kShare ? kShare : kMost) - 1024 - d.terms_bytes;
   d.stages = room / 16384 < kLoraMostStages ? room / 16384 : kLoraMostStages;
-  const int64_t blocks = (a.n + 127) / 128, wanted = kCtas * kNumSMs / tiles;  // (one round, as above)
-  d.parts = (int)(wanted < 1 ? 1 : wanted < blocks ? wanted : blocks);
-  const int64_t items = tiles * d.parts, most = kCtas * kNumSMs;
+  const int64_t items = tiles * ((a.n + 127) / 128), most = kCtas * kNumSMs;
   launch_dependent(lora_up_kernel<Y, TILE, WHOLE>, dim3((unsigned)(items < most ? items : most)), dim3(lora_up_threads(TILE)), (size_t)d.terms_bytes + d.stages * 16384 + 1024, st, map_b, a, p,
                    d);
   B200Q_LAUNCH_CHECK();
@@ -808,7 +814,7 @@ static int lora_chunk_fast(const b200q_lora_args& a, cudaStream_t st) {
   p.low = reinterpret_cast<float*>(w + space.low);
   p.splits = (int)splits;
   p.steps = (int)((a.k + 63) / 64);
-  p.part_steps = (int)((p.steps + splits - 1) / splits);
+  p.slots = lora_down_ctas(a.rank, tile) * kNumSMs;
   p.tile = tile;
   p.status = device_status_ptr();
   if (!p.status) return B200Q_ERR_CUDA;
