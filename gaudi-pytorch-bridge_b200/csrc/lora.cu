@@ -611,46 +611,63 @@ __global__ void __launch_bounds__(lora_up_threads(TILE), lora_up_ctas(sizeof(Y) 
       };
 #pragma unroll
       for (int c = 0; c < kPieces; ++c) token[c] = c * kRows + my_row < count ? view.token(first + c * kRows + my_row) : -1;
+      if constexpr (kEarly) {
 #pragma unroll
-      for (int c = 0; c < kPieces; ++c) ask(c, part);
-      if (kEarly && item == 0) pdl_enter();
+        for (int c = 0; c < kPieces; ++c) ask(c, part);
+        if (item == 0) pdl_enter();
+      }
       ok = ok && ptx::mbar_wait_uniform(bar_used, (item & 1) ^ 1, &s_abort, p.status, kLoraErrResults);  // (the products with the terms before are done)
       const float scale = a.scales ? a.scales[tile.adapter] : 1.f;
-      const int pieces = 8 * d.chunks;  // of eight ranks
+      // The terms: a thread has four ranks of a token or two at a time, eight parts of k at once.  (Eight ranks of a token, two parts at once: twice the sectors, 89 us for
+      // 4096 tokens where this is 86; what spills, four tokens and two parts for instance, 110.)
+      const int pieces = 16 * d.chunks, total = tile.count * pieces;  // of four ranks
       const int splits = lora_parts(p, view.tiles_used * ((d.chunks + 1) / 2));
-      for (int q = wt; ok && q < tile.count * pieces; q += 32 * kWarps) {
-        const int j = q / pieces, r = 8 * (q - j * pieces);
-        float v[8] = {};
-        if (r < a.rank) {
-          const float4* low = reinterpret_cast<const float4*>(p.low + (int64_t)view.sorted[tile.first + j] * a.rank + r);
-          const int64_t step = a.tokens * a.rank / 4;
-          constexpr int kTogether = TILE == 16 && sizeof(Y) == 2 ? 4 : 2;  // parts of k on their way: few tokens have many (one token 7.2 us, with two 7.7); else registers
-          for (int s0 = 0; s0 < splits; s0 += kTogether) {
-            float4 x[kTogether][2];
+      constexpr int kSets = TILE == 16 ? 1 : 2, kTogether = 8;
+      for (int q0 = wt; ok && q0 < total; q0 += 32 * kWarps * kSets) {
+        const float* low[kSets];
+        float v[kSets][4] = {};
 #pragma unroll
-            for (int s = 0; s < kTogether; ++s)
+        for (int e = 0; e < kSets; ++e) {
+          const int q = q0 + 32 * kWarps * e, j = q / pieces, r = 4 * (q - j * pieces);
+          low[e] = q < total && r < a.rank ? p.low + (int64_t)view.sorted[tile.first + j] * a.rank + r : nullptr;
+        }
+        const int64_t step = a.tokens * a.rank;
+        for (int s0 = 0; s0 < splits; s0 += kTogether) {
+          float4 x[kSets][kTogether];
 #pragma unroll
-              for (int h = 0; h < 2; ++h) x[s][h] = s0 + s < splits ? __ldcg(low + (s0 + s) * step + h) : make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int s = 0; s < kTogether; ++s)
 #pragma unroll
-            for (int s = 0; s < kTogether; ++s) {
-              v[0] += x[s][0].x; v[1] += x[s][0].y; v[2] += x[s][0].z; v[3] += x[s][0].w;
-              v[4] += x[s][1].x; v[5] += x[s][1].y; v[6] += x[s][1].z; v[7] += x[s][1].w;
+            for (int e = 0; e < kSets; ++e)
+              x[e][s] = low[e] && s0 + s < splits ? __ldcg(reinterpret_cast<const float4*>(low[e] + (s0 + s) * step)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int s = 0; s < kTogether; ++s)
+#pragma unroll
+            for (int e = 0; e < kSets; ++e) {
+              v[e][0] += x[e][s].x; v[e][1] += x[e][s].y; v[e][2] += x[e][s].z; v[e][3] += x[e][s].w;
             }
-          }
         }
 #pragma unroll
-        for (int c = 0; c < 8; ++c) v[c] *= scale;
+        for (int e = 0; e < kSets; ++e) {
+          const int q = q0 + 32 * kWarps * e, j = q / pieces, r = 4 * (q - j * pieces);
+          if (q >= total) break;
 #pragma unroll
-        for (int e = 0; e < kTerms; ++e) {
-          uint32_t w[4];
+          for (int c = 0; c < 4; ++c) v[e][c] *= scale;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            w[c] = pack_bf16x2(v[2 * c], v[2 * c + 1]);
-            v[2 * c] -= __uint_as_float(w[c] << 16);
-            v[2 * c + 1] -= __uint_as_float(w[c] & 0xFFFF0000u);
+          for (int t = 0; t < kTerms; ++t) {
+            uint32_t w[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              w[c] = pack_bf16x2(v[e][2 * c], v[e][2 * c + 1]);
+              v[e][2 * c] -= __uint_as_float(w[c] << 16);
+              v[e][2 * c + 1] -= __uint_as_float(w[c] & 0xFFFF0000u);
+            }
+            *reinterpret_cast<uint2*>(s_terms + ((t * d.chunks + r / 64) * TILE + j) * 128 + (((r / 8 & 7) ^ (j & 7)) << 4) + 2 * (r & 4)) = make_uint2(w[0], w[1]);
           }
-          *reinterpret_cast<uint4*>(s_terms + ((e * d.chunks + r / 64) * TILE + j) * 128 + (((r / 8 & 7) ^ (j & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
+      }
+      if constexpr (!kEarly) {  // (here, because the registers are wanted for the terms before)
+#pragma unroll
+        for (int c = 0; c < kPieces; ++c) ask(c, part);
       }
       ptx::fence_proxy_async_smem();
       ok = layer_bar_and(1, 32 * kWarps, ok);
