@@ -53,8 +53,8 @@ __global__ void __launch_bounds__(kLoraPlainThreads) lora_plain_up_kernel(const 
 // the adapter's matrix has the 128 rows of tcgen05.mma (ranks, or columns of y) and the tile's tokens are its columns, so that a warp's results are
 // neighbours in memory: a x is bf16 times bf16, both by TMA (tokens by gathered rows); b (a x) has a x in bf16 terms that follow one another along K.
 //
-// us: 4096 tokens of 4096 -> 14336, rank 64, 8 adapters in runs of 512 tokens 81 to 89 (floor, y twice and x once, 38: the sorting 5, a x 18, the rest b (a x)); 64 tokens of 8192 -> 8192 with
-// some 40 of 64 adapters of rank 32 23 (floor 9.4: the steps of two kernels one behind the other); one token of 4096 -> 4096, rank 16, 9.3 (7.2 on the device), two kernels' latency.
+// us: 4096 tokens of 4096 -> 14336, rank 64, 8 adapters in runs of 512 tokens 78 to 86 (floor, y twice and x once, 38: the sorting 5, a x 18, the rest b (a x)); 64 tokens of 8192 -> 8192 with
+// some 40 of 64 adapters of rank 32 22 (floor 9.4: the steps of two kernels one behind the other); one token of 4096 -> 4096, rank 16, 8.6 (7.2 on the device), two kernels' latency.
 // With mma.sync and the tokens as rows these were 162, 32 and 6.2.
 constexpr int kLoraSortThreads = 1024;
 constexpr int kLoraFew = 128;  // tokens up to which each CTA sorts for itself
@@ -401,6 +401,10 @@ __global__ void __launch_bounds__(32 * kLoraDownWarps, TILE == 16 ? 4 : 2)
     for (int i = blockIdx.x; i < items && ok; i += gridDim.x) {
       const Item it = item_of(i);
       const int r = 128 * it.block + 32 * quarter + lane;
+      constexpr int kHeld = (TILE + 31) / 32;
+      int held[kHeld];  // a lane has each 32nd token, fetched while the products run
+#pragma unroll
+      for (int h = 0; h < kHeld; ++h) held[h] = 32 * h + lane < it.tile.count ? view.sorted[it.tile.first + 32 * h + lane] : 0;
       // (a part behind the end of k: zeros)
       for (int k = it.k0; k == it.k0 || (EXACT && k < it.k1); k += kLoraSub) {
         const bool none = it.k0 >= it.k1;
@@ -411,26 +415,28 @@ __global__ void __launch_bounds__(32 * kLoraDownWarps, TILE == 16 ? 4 : 2)
           ++n;
           ptx::tc_fence_after();
         }
-        for (int j0 = 0; j0 < it.tile.count; j0 += 8) {
-          float v[8] = {};
-          if (!none) {
-            layer_tmem_ld8(in + j0, v);
-            ptx::tmem_ld_wait();
+#pragma unroll
+        for (int h = 0; h < kHeld; ++h)
+          for (int j0 = 32 * h; j0 < min(it.tile.count, 32 * h + 32); j0 += 8) {
+            float v[8] = {};
+            if (!none) {
+              layer_tmem_ld8(in + j0, v);
+              ptx::tmem_ld_wait();
+            }
+            float* to[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) to[j] = p.low + ((int64_t)it.part * a.tokens + __shfl_sync(0xFFFFFFFFu, held[h], j0 + j - 32 * h)) * a.rank + r;
+            if (EXACT && k > it.k0) {  // (a thread's own sums)
+              float before[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) before[j] = r < a.rank && j0 + j < it.tile.count ? *to[j] : 0.f;
+#pragma unroll
+              for (int j = 0; j < 8; ++j) v[j] += before[j];
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (j0 + j < it.tile.count && r < a.rank) *to[j] = v[j];
           }
-          float* to[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) to[j] = p.low + ((int64_t)it.part * a.tokens + view.sorted[it.tile.first + min(j0 + j, it.tile.count - 1)]) * a.rank + r;
-          if (EXACT && k > it.k0) {  // (a thread's own sums)
-            float before[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) before[j] = r < a.rank ? *to[j] : 0.f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] += before[j];
-          }
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (j0 + j < it.tile.count && r < a.rank) *to[j] = v[j];
-        }
         if (!none) {
           ptx::tc_fence_before();
           __syncwarp();
