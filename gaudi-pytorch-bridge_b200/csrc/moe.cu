@@ -326,8 +326,8 @@ __global__ void __launch_bounds__(kMoeThreads) moe_sum_kernel(const b200q_moe_ar
 // registers first.
 //
 // One persistent CTA per SM; the units of the work are (group of an expert's tokens, tile of weight rows), which the CTAs take from a counter: in equal
-// runs of one list the SMs that get at the memory fastest were done after 203 us and the last ones after 272 (29 tokens, 108 experts of 4096 x 1792).  The last
-// tile and a quarter per CTA are cut into parts of a few steps of 128 bytes of a row, so that all end together, and few experts load every SM; a cut
+// runs of one list the SMs that get at the memory fastest were done after 203 us and the last ones after 272 (29 tokens, 108 experts of 4096 x 1792).  Long
+// tiles are cut into parts of a few steps of 128 bytes of a row where they do not come out even, so that all end together, and few experts load every SM; a cut
 // tile is summed, in the parts' order, by a CTA that its number gives.  (By the one whose part comes last, a CTA that falls behind gets the sums too.)
 // Both products are one stream of units without a barrier between: the second one of a group waits for the group's first.
 //
@@ -400,8 +400,10 @@ __device__ __forceinline__ void moe_fence_async() { asm volatile("fence.proxy.as
 __device__ __forceinline__ int moe_divide(int x, float inverse) { return (int)(((float)x + 0.5f) * inverse); }
 
 // The units of a product: `whole` tiles, then the parts of the others.  Fewer than 2^22 of them: at most 640 groups, of 512 tiles each.
-// Cut are the tiles that do not come out even, and a quarter of a round of all CTAs at least; but none where a tile is short, because a sum of parts takes as long as
-// some eight steps, and none where so many CTAs have one whole tile that they draw all that the memory gives.
+// Cut are the tiles that do not come out even, and a quarter of a round of all CTAs at least; but none of up to 32 steps (4096 bytes of a row), because fewer CTAs draw more each and
+// the sums come on top, and none where so many CTAs have one whole tile that they draw all that the memory gives.  us with cuts above 8 steps, above 32, and none at all: 64 tokens
+// of 32 experts 2048 x 688 66, 60, 60; 16 tokens of 64 experts 2048 x 1408 94, 86, 86; 29 tokens of 128 experts 4096 x 1792 383, 378, 377; 5 tokens of 8 experts 4096 x 4096 in
+// bf16 (64 steps) 116, 116, 120.
 struct MoeUnits {
   int tiles, steps, whole, cut, parts, units;  // tiles of a group, steps of a tile
   float per_group, per_tile;
@@ -410,7 +412,7 @@ struct MoeUnits {
     steps = steps_;
     const int total = groups * tiles, rounds = max(0, moe_divide(total - ctas / 4, __frcp_rn((float)ctas)));
     cut = total - rounds * ctas;
-    if (steps <= 8 || (total <= ctas && 10 * total >= 7 * ctas)) cut = 0;
+    if (steps <= 32 || (total <= ctas && 10 * total >= 7 * ctas)) cut = 0;
     const int length = max(3, min((int)((float)(cut * steps) * __frcp_rn((float)(3 * ctas))), 8));
     parts = min(moe_divide(steps + length - 1, __frcp_rn((float)length)), kMoeMostParts);
     whole = total - cut;
@@ -729,8 +731,9 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
       for (int i = 0, u = cta; ok; ++i) {
         publish(u < list.units ? u : -1);
         if (!ok || u >= list.units) break;
-        int next = u + ctas;
-        if (i + 1 >= dealt && lane == 0) next = dealt * ctas + (int)atomicAdd(&w.control->next[product], 1u);
+        const bool ask = i + 1 >= dealt && dealt * ctas < list.units;
+        uint32_t taken = 0;  // (nothing is computed from it before the copies are on their way: that would wait for the answer)
+        if (ask && lane == 0) asm volatile("atom.global.add.u32 %0, [%1], 1;" : "=r"(taken) : "l"(&w.control->next[product]) : "memory");
         const MoeUnit unit(list, u);
         const int e = s_group_expert[unit.group];
         for (int k = unit.k0; k < unit.k1; ++k) {
@@ -753,7 +756,8 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
             phase ^= 1;
           }
         }
-        u = __shfl_sync(0xFFFFFFFFu, next, 0);
+        taken = __shfl_sync(0xFFFFFFFFu, taken, 0);
+        u = ask ? dealt * ctas + (int)taken : u + ctas;
       }
     };
     stream(std::integral_constant<int, 0>());

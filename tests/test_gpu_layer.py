@@ -534,6 +534,14 @@ def test_moe_cut_tiles(tokens, hidden, inner, experts, top_k, weights):
     _check_moe(_run_moe(case, top_k), case, top_k)
 
 
+@pytest.mark.parametrize("tokens,hidden,inner,experts,top_k,weights", [(100, 4352, 160, 4, 2, E4M3), (70, 160, 4400, 3, 1, E4M3), (4, 4480, 144, 80, 16, E4M3), (9, 5120, 4224, 2, 1, E4M3),
+                                                                     (100, 2176, 144, 4, 2, BF16), (24, 2304, 320, 60, 8, BF16), (2, 2112, 2120, 5, 3, BF16)])
+def test_moe_cut_long_rows(tokens, hidden, inner, experts, top_k, weights):
+    """Rows of more than 4096 bytes, whose tiles are cut where they do not come out even: few tiles, more than the SMs, several groups of an expert, both products."""
+    case = _moe_case(tokens, hidden, inner, experts, weights)
+    _check_moe(_run_moe(case, top_k), case, top_k)
+
+
 def test_moe_of_nothing():
     z = lambda *s: torch.zeros(*s, dtype=BF16).cuda()  # noqa: E731
     out, weights, ids = torch.ops.b200q.moe_layer(z(0, 64), z(4, 64), z(4, 64, 64), z(4, 64, 32), None, None, 2)
