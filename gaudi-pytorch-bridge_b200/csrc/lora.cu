@@ -54,7 +54,7 @@ __global__ void __launch_bounds__(kLoraPlainThreads) lora_plain_up_kernel(const 
 // neighbours in memory: a x is bf16 times bf16, both by TMA (tokens by gathered rows); b (a x) has a x in bf16 terms that follow one another along K.
 //
 // us: 4096 tokens of 4096 -> 14336, rank 64, 8 adapters in runs of 512 tokens 78 to 86 (floor, y twice and x once, 38: the sorting 5, a x 18, the rest b (a x)); 64 tokens of 8192 -> 8192 with
-// some 40 of 64 adapters of rank 32 22 (floor 9.4: the steps of two kernels one behind the other); one token of 4096 -> 4096, rank 16, 8.6 (7.2 on the device), two kernels' latency.
+// 56 of 64 adapters of rank 32 22 (floor 9.4: the steps of two kernels one behind the other); one token of 4096 -> 4096, rank 16, 8.6 (7.2 on the device), two kernels' latency.
 // With mma.sync and the tokens as rows these were 162, 32 and 6.2.
 constexpr int kLoraSortThreads = 1024;
 constexpr int kLoraFew = 128;  // tokens up to which each CTA sorts for itself
@@ -91,7 +91,7 @@ static int lora_tile_tokens(int64_t tokens, int64_t rank, int64_t adapters, bool
   return t >= 24 * adapters && t > kLoraFew && blocks <= 6 ? 128 : 16;
 }
 // CTAs of an SM that share a x: more where ranks are few, because an item is a chain of steps
-// (64 tokens of 40 adapters of rank 32, 8192 values each: 24.3 us with two, 22.6 with four)
+// (64 tokens of 56 adapters of rank 32, 8192 values each: 24.3 us with two, 22.6 with four)
 static int lora_down_ctas(int64_t rank, int tile) { return tile == 16 && rank <= 64 ? 4 : 2; }
 // tiles that the tokens may need at most, and parts of k at most.  The kernels, which know how many tiles there are, take as many parts as leave no CTA a second item (a second
 // round costs as much as the first); the workspace has room for as many as that can be, which is little where tokens are few, and where they are many for what the most tiles leave.

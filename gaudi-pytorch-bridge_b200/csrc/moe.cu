@@ -339,7 +339,7 @@ constexpr int kMoeErrWeights = 821, kMoeErrTokens = 822, kMoeErrMma = 823, kMoeE
 constexpr int kMoeGroupTokens = 32;     // of an expert, at a time
 constexpr int kMoeSubBytes = 128 * 128;  // a weight tile: 128 rows of 128 bytes; a step has two (gate and up, or 256 outputs)
 constexpr int kMoeMostDim = 65536;
-constexpr uint32_t kMoeGridPolls = 1u << 23;
+constexpr uint32_t kMoeGridPolls = 1u << 21;  // some two seconds
 
 constexpr int kMoeCutTiles = kNumSMs * 5 / 4 + 1, kMoeMostParts = 8, kMoeSumTokens = 4;
 constexpr int kMoeMostGroups = kMoeMaxExperts + (int)kMoeChunk * kMoeMaxTopK / kMoeGroupTokens;
