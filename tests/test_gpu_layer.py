@@ -658,6 +658,45 @@ def test_the_same_call_gives_the_same_bytes():
         assert all(torch.equal(a, b) for a, b in zip(first, got))
 
 
+@pytest.mark.parametrize("tokens,n,adapters", [(1, 4096, 2), (20, 1032, 7), (128, 2048, 60), (400, 512, 90), (1500, 256, 3)])
+def test_adapters_one_behind_the_other(tokens, n, adapters):
+    """Kernels begin before those in front of them are done, and fetch y early: a chain of calls on one y, between kernels that change y and x, has the bytes of calls that are waited for."""
+    y, x, a, b, which, scales = (t.cuda() for t in _lora_case(tokens, 256, n, 16, adapters, BF16))
+
+    def chain(y, x, wait):
+        for i in range(12):
+            torch.ops.b200q.lora_add_(y, x, a, b, which, scales)
+            wait()
+            if i % 3 == 1:
+                y.mul_(0.75)
+                wait()
+            if i % 4 == 2:
+                x.neg_()
+                wait()
+            which.copy_(which.roll(1))
+            wait()
+        return y
+
+    first = which.clone()
+    want = chain(y.clone(), x.clone(), torch.cuda.synchronize)
+    for _ in range(5):
+        which.copy_(first)
+        assert torch.equal(chain(y.clone(), x.clone(), lambda: None), want)
+    ys, xs = y.clone(), x.clone()
+    which.copy_(first)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        chain(ys, xs, lambda: None)
+    for _ in range(3):
+        which.copy_(first)
+        ys.copy_(y)
+        xs.copy_(x)
+        graph.replay()
+        assert torch.equal(ys, want)
+    graph.reset()
+
+
 def test_two_streams_at_once():
     x, residual, w = _step_inputs(19, 256)
     d = {k: v.cuda() for k, v in w.items()}
