@@ -630,7 +630,7 @@ size_t b200q_moe_workspace_bytes(int64_t tokens, int64_t hidden, int64_t inner, 
   return moe_workspace_bytes_impl(tokens, hidden, inner, experts, top_k);
 }
 
-int b200q_moe_layer(const b200q_moe_args* a) {
+static int check_moe(const b200q_moe_args* a) {
   if (!a) return B200Q_ERR_BAD_ARGUMENT;
   if (a->tokens < 0 || a->hidden < 0 || a->inner < 0 || a->experts < 1 || a->top_k < 1 || a->top_k > a->experts) return B200Q_ERR_BAD_ARGUMENT;
   if (!is_wide(a->router_dtype) || !is_wide(a->out_dtype) || !(a->weight_dtype == B200Q_BF16 || a->weight_dtype == B200Q_E4M3)) return B200Q_ERR_BAD_ARGUMENT;
@@ -643,7 +643,19 @@ int b200q_moe_layer(const b200q_moe_args* a) {
       !on_elements(a->down, a->weight_dtype, 1) || !on_elements(a->out, a->out_dtype, 1) ||
       !on_bytes(4, {a->gate_up_scale, a->down_scale, a->num_tokens, a->weights, a->ids}))
     return B200Q_ERR_UNSUPPORTED;
+  return B200Q_OK;
+}
+
+int b200q_moe_layer(const b200q_moe_args* a) {
+  const int rc = check_moe(a);
+  if (rc || a->tokens == 0) return rc;
   return moe_layer_impl(*a, static_cast<cudaStream_t>(a->stream));
+}
+
+int b200q_selftest_moe_wait_timeout(const b200q_moe_args* a, int lost) {
+  if (int rc = check_moe(a)) return rc;
+  if (a->tokens == 0) return B200Q_ERR_BAD_ARGUMENT;
+  return moe_selftest_impl(*a, lost, static_cast<cudaStream_t>(a->stream));
 }
 
 }  // extern "C"

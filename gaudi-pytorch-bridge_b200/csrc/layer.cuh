@@ -15,6 +15,7 @@ size_t lora_workspace_bytes_impl(int64_t tokens, int64_t k, int64_t n, int64_t r
 int lora_add_impl(const b200q_lora_args& a, cudaStream_t st);
 size_t moe_workspace_bytes_impl(int64_t tokens, int64_t hidden, int64_t inner, int experts, int top_k);
 int moe_layer_impl(const b200q_moe_args& a, cudaStream_t st);
+int moe_selftest_impl(const b200q_moe_args& a, int lost, cudaStream_t st);
 
 // A named barrier that tells whether all its threads say yes.  Warps that share a barrier must all come to it, also where the waits of some have run out.
 __device__ __forceinline__ bool layer_bar_and(int id, int threads, bool yes) {

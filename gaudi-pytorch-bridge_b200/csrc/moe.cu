@@ -340,6 +340,7 @@ constexpr int kMoeGroupTokens = 32;     // of an expert, at a time
 constexpr int kMoeSubBytes = 128 * 128;  // a weight tile: 128 rows of 128 bytes; a step has two (gate and up, or 256 outputs)
 constexpr int kMoeMostDim = 65536;
 constexpr uint32_t kMoeGridPolls = 1u << 21;  // some two seconds
+constexpr uint32_t kMoeTestPolls = 1u << 14;  // of the self-test: some ten milliseconds
 
 constexpr int kMoeCutTiles = kNumSMs * 5 / 4 + 1, kMoeMostParts = 8, kMoeSumTokens = 4;
 constexpr int kMoeMostGroups = kMoeMaxExperts + (int)kMoeChunk * kMoeMaxTopK / kMoeGroupTokens;
@@ -374,7 +375,10 @@ struct MoeFused {
   MoeControl* control;
   int* status;
   int up_tiles, up_steps, down_tiles, down_steps;
+  int lost;  // self-test: what never comes (MoeLost)
 };
+// What a self-test waits for in vain: a CTA's choices, a CTA's results, the weights of a step, the tokens of a step (the last two in CTA 0).
+enum MoeLost { kMoeLostChoice, kMoeLostResults, kMoeLostWeights, kMoeLostTokens, kMoeLostCount };
 
 __device__ __forceinline__ uint32_t moe_ld_acquire(const uint32_t* p) {
   uint32_t v;
@@ -383,8 +387,8 @@ __device__ __forceinline__ uint32_t moe_ld_acquire(const uint32_t* p) {
 }
 __device__ __forceinline__ void moe_add_release(uint32_t* p, int n = 1) { asm volatile("red.release.gpu.global.add.u32 [%0], %1;" ::"l"(p), "r"(n) : "memory"); }
 // until all CTAs have arrived (one warp); false when they do not
-__device__ __forceinline__ bool moe_grid_wait(const uint32_t* p, uint32_t want, volatile int* abort_flag, int* status) {
-  for (uint32_t i = 0; i < kMoeGridPolls; ++i) {
+__device__ __forceinline__ bool moe_grid_wait(const uint32_t* p, uint32_t want, volatile int* abort_flag, int* status, uint32_t polls) {
+  for (uint32_t i = 0; i < polls; ++i) {
     if (__all_sync(0xFFFFFFFFu, moe_ld_acquire(p) >= want)) return true;
     if ((i & 63u) == 63u && __any_sync(0xFFFFFFFFu, *abort_flag)) return false;
     if (i > 64u) __nanosleep(64);
@@ -441,12 +445,13 @@ struct MoeUnit {
   }
 };
 
-template <bool FP8, int MAXN>
+template <bool FP8, int MAXN, bool TEST>  // TEST: short waits, one of them in vain
 __global__ void __launch_bounds__(32 * kMoeWarps, 1)
     moe_fused_kernel(const __grid_constant__ CUtensorMap map_up, const __grid_constant__ CUtensorMap map_down, const __grid_constant__ CUtensorMap map_x,
                      const __grid_constant__ CUtensorMap map_h, const b200q_moe_args a, int64_t first, const MoeFused w) {
   using Tile = MoeTile<FP8, MAXN>;
   constexpr int kStages = Tile::kStages, kSteps = Tile::kStep;
+  constexpr uint32_t kLimit = TEST ? kMoeTestPolls : ptx::kWaitLimit, kPolls = TEST ? kMoeTestPolls : kMoeGridPolls;
   constexpr int kMostSlots = MAXN == 8 ? 8 * kMoeMaxTopK : (int)kMoeChunk * kMoeMaxTopK;
   constexpr int kMostGroups = MAXN == 8 ? 8 * kMoeMaxTopK : kMoeMaxExperts + kMostSlots / kMoeGroupTokens;
   constexpr int kMaskWords = MAXN == 8 ? 1 : (int)kMoeChunk / 32;
@@ -519,7 +524,7 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
     __threadfence();
     __syncthreads();
     if (tid == 0) moe_add_release(&w.control->chosen);
-    ok = moe_grid_wait(&w.control->chosen, (uint32_t)ctas, &s_abort, w.status);
+    ok = moe_grid_wait(&w.control->chosen, (uint32_t)ctas + (TEST && w.lost == kMoeLostChoice), &s_abort, w.status, kPolls);
     for (int i = tid; i < slots; i += 32 * kMoeWarps) s_ids[i] = (int16_t)__ldcg(a.ids + i);
     ok = __syncthreads_and(ok);
   }
@@ -594,7 +599,7 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
   uint32_t turn = 0, turn_phase = 0;
   auto next_unit = [&](int code) {
     int unit = -1;
-    ok = ptx::mbar_wait_uniform(bar_unit + 8 * turn, turn_phase, &s_abort, w.status, code);
+    ok = ptx::mbar_wait_uniform(bar_unit + 8 * turn, turn_phase, &s_abort, w.status, code, kLimit);
     if (!ok) return unit;
     unit = *(volatile int*)&s_unit[turn];
     __syncwarp();
@@ -625,7 +630,7 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
       if (s_group_slot[mid] <= slot) group = mid;
       else hi = mid - 1;
     }
-    ok = moe_grid_wait(&w.control->up[group], 4 * (uint32_t)(w.up_tiles * blocks_of(group)), &s_abort, w.status);
+    ok = moe_grid_wait(&w.control->up[group], 4 * (uint32_t)(w.up_tiles * blocks_of(group)), &s_abort, w.status, kPolls);
     if (!ok) return;
     const float factor = moe_up_factor(__ldcg(w.h_top + slot));
     for (int64_t i = 8 * (tid - 96); i < a.inner; i += 8 * 128) {
@@ -711,7 +716,7 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
     // ------------------------------------------------------------ weights
     uint32_t stage = 0, phase = 0;
     auto publish = [&](int u) {
-      ok = ok && ptx::mbar_wait_uniform(bar_taken + 8 * turn, turn_phase ^ 1, &s_abort, w.status, kMoeErrWeights);
+      ok = ok && ptx::mbar_wait_uniform(bar_taken + 8 * turn, turn_phase ^ 1, &s_abort, w.status, kMoeErrWeights, kLimit);
       if (!ok) return;
       if (lane == 0) {
         *(volatile int*)&s_unit[turn] = u;
@@ -737,12 +742,14 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
         const MoeUnit unit(list, u);
         const int e = s_group_expert[unit.group];
         for (int k = unit.k0; k < unit.k1; ++k) {
-          ok = ptx::mbar_wait_uniform(bar_empty + 8 * stage, phase ^ 1, &s_abort, w.status, kMoeErrWeights);
+          ok = ptx::mbar_wait_uniform(bar_empty + 8 * stage, phase ^ 1, &s_abort, w.status, kMoeErrWeights, kLimit);
           if (!ok) break;
           if (ptx::elect_one()) {
             const uint32_t bar = bar_weights + 8 * stage, dst = ring + stage * Tile::kStage;
             ptx::mbar_arrive_expect_tx(bar, 2 * kMoeSubBytes);
-            if (product == 0) {
+            if (TEST && w.lost == kMoeLostWeights && cta == 0 && made == 0) {
+              // (never copied)
+            } else if (product == 0) {
               ptx::tma_load_3d(dst, &map_up, bar, k * kSteps, unit.row * 128, 2 * e);
               ptx::tma_load_3d(dst + kMoeSubBytes, &map_up, bar, k * kSteps, unit.row * 128, 2 * e + 1);
             } else {
@@ -778,11 +785,11 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
         const int cols = ((s_group_tokens[unit.group] + 7) / 8 * 8 * terms + 15) / 16 * 16;
         const uint32_t idesc = FP8 ? ptx::umma_idesc(0, 0, 128, cols) : ptx::umma_idesc(1, 1, 128, cols);
         const uint32_t acc = pieces & 1, d = tmem + acc * 2 * Tile::kCols;
-        ok = ptx::mbar_wait_uniform(bar_free + 8 * acc, ((pieces >> 1) & 1) ^ 1, &s_abort, w.status, kMoeErrMma);
+        ok = ptx::mbar_wait_uniform(bar_free + 8 * acc, ((pieces >> 1) & 1) ^ 1, &s_abort, w.status, kMoeErrMma, kLimit);
         if (!ok) break;
         ptx::tc_fence_after();
         for (int k = unit.k0; k < unit.k1; ++k) {
-          ok = ptx::mbar_wait2_uniform(bar_weights + 8 * stage, phase, bar_tokens + 8 * stage, phase, &s_abort, w.status, kMoeErrMma);
+          ok = ptx::mbar_wait2_uniform(bar_weights + 8 * stage, phase, bar_tokens + 8 * stage, phase, &s_abort, w.status, kMoeErrMma, kLimit);
           if (!ok) break;
           ptx::tc_fence_after();
           const uint64_t off = stage * (uint32_t)(Tile::kStage >> 4);
@@ -816,8 +823,8 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
         const MoeUnit unit(list, u);
         const int slot = s_group_slot[unit.group], n = s_group_tokens[unit.group], blocks = (n + 7) / 8;
         if (product == 1 && unit.group != there) {
-          ok = FP8 ? moe_grid_wait(&w.control->terms[unit.group], 4 * (uint32_t)n, &s_abort, w.status)
-                   : moe_grid_wait(&w.control->up[unit.group], 4 * (uint32_t)(w.up_tiles * blocks_of(unit.group)), &s_abort, w.status);
+          ok = FP8 ? moe_grid_wait(&w.control->terms[unit.group], 4 * (uint32_t)n, &s_abort, w.status, kPolls)
+                   : moe_grid_wait(&w.control->up[unit.group], 4 * (uint32_t)(w.up_tiles * blocks_of(unit.group)), &s_abort, w.status, kPolls);
           if (!ok) break;
           moe_fence_async();
           there = unit.group;
@@ -830,7 +837,7 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
           for (int i = 0; i < 4; ++i) rows[i] = term * tokens + s_token_of[slot + min(8 * block + 4 * four + i, n - 1)];
         }
         for (int k = unit.k0; k < unit.k1; ++k) {
-          ok = ptx::mbar_wait_uniform(bar_empty + 8 * stage, phase ^ 1, &s_abort, w.status, kMoeErrTokens);
+          ok = ptx::mbar_wait_uniform(bar_empty + 8 * stage, phase ^ 1, &s_abort, w.status, kMoeErrTokens, kLimit);
           if (!ok) break;
           if (ptx::elect_one()) {
             const uint32_t bar = bar_tokens + 8 * stage, dst = ring + stage * Tile::kStage + 2 * kMoeSubBytes;
@@ -839,7 +846,7 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
               for (int g = 0; g < blocks; ++g) ptx::tma_load_3d(dst + g * terms * 1024, &map_h, bar, k * kSteps, slot + 8 * g, 0);
           }
           __syncwarp();
-          if (product == 0 && block < blocks)
+          if (product == 0 && block < blocks && !(TEST && w.lost == kMoeLostTokens && cta == 0 && made == 0))
             layer_gather4(ring + stage * Tile::kStage + 2 * kMoeSubBytes + (lane >> 1) * 1024 + four * 512, &map_x, bar_tokens + 8 * stage, k * kSteps, rows);
           __syncwarp();
           ++made;
@@ -867,7 +874,7 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
         const MoeUnit unit(list, list.whole + c * list.parts);
         const int n = s_group_tokens[unit.group];
         if (j0 >= n) continue;
-        ok = moe_grid_wait(&w.control->parts[product][c], 4 * (uint32_t)list.parts, &s_abort, w.status);
+        ok = moe_grid_wait(&w.control->parts[product][c], 4 * (uint32_t)list.parts, &s_abort, w.status, kPolls);
         if (!ok) break;
         float scale[2];
         scales_of(which, unit, row, scale);
@@ -924,7 +931,7 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
           if (product == 0) backs = backs_of(which, unit);
         }
         float* part = w.parts + (((int64_t)product * kMoeCutTiles + unit.cut) * kMoeMostParts + unit.part) * Tile::kPart + row;
-        ok = ptx::mbar_wait_uniform(bar_full + 8 * acc, (pieces >> 1) & 1, &s_abort, w.status, kMoeErrResults);
+        ok = ptx::mbar_wait_uniform(bar_full + 8 * acc, (pieces >> 1) & 1, &s_abort, w.status, kMoeErrResults, kLimit);
         if (!ok) break;
         ptx::tc_fence_after();
         if (whole && product == 1) backs = backs_of(which, unit);  // (h's largest value is known now that it has been multiplied)
@@ -966,15 +973,15 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
     if (ok) results_of(std::integral_constant<int, 0>());
     if (ok) results_of(std::integral_constant<int, 1>());
     finished_all();
-    // ---- the weighted sums
-    if (ok) ok = moe_grid_wait(&w.control->done, (uint32_t)ctas, &s_abort, w.status);
+    // ---- the weighted sums.  Where a wait has run out nothing is read: the list may have been made of choices that were never written, and a token's slots with it.
+    if (ok) ok = moe_grid_wait(&w.control->done, (uint32_t)ctas + (TEST && w.lost == kMoeLostResults), &s_abort, w.status, kPolls);
     const int et = tid - 224;
     const int64_t quads = (a.hidden + 3) / 4;
     for (int64_t i = (int64_t)cta * 128 + et; i < tokens * quads; i += (int64_t)ctas * 128) {
       const int t = (int)(i / quads);
       const int64_t c = (i - t * quads) * 4;
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (t < live)
+      if (ok && t < live)
         for (int j = 0; j < top_k; ++j) {
           const float p = __ldcg(a.weights + t * top_k + j);
           const float4 y = __ldcg(reinterpret_cast<const float4*>(w.outputs + (int64_t)s_slot_of[t * top_k + j] * a.hidden + c));
@@ -1035,10 +1042,10 @@ static int moe_map(CUtensorMap* map, const void* base, bool fp8, int64_t depth, 
   return r == CUDA_SUCCESS ? B200Q_OK : B200Q_ERR_UNSUPPORTED;
 }
 
-template <bool FP8, int MAXN>
-static int moe_launch_fused(const b200q_moe_args& a, int64_t first, const MoeSpace& space, cudaStream_t st) {
+template <bool FP8, int MAXN, bool TEST = false>
+static int moe_launch_fused(const b200q_moe_args& a, int64_t first, const MoeSpace& space, cudaStream_t st, int lost = 0) {
   using Tile = MoeTile<FP8, MAXN>;
-  auto kernel = moe_fused_kernel<FP8, MAXN>;
+  auto kernel = moe_fused_kernel<FP8, MAXN, TEST>;
   constexpr int kSmem = Tile::kStages * Tile::kStage + 1024;
   static std::atomic<int> grid_of[kMaxDevices];  // CTAs that are resident together
   const int dev = current_device_index();
@@ -1058,6 +1065,7 @@ static int moe_launch_fused(const b200q_moe_args& a, int64_t first, const MoeSpa
   if (int rc = moe_map(&map_down, a.down, FP8, a.inner, a.hidden, a.experts)) return rc;
   uint8_t* p = static_cast<uint8_t*>(a.workspace);
   MoeFused w;
+  w.lost = lost;
   w.slots = (int)a.tokens * a.top_k;
   w.h_terms = p + space.h_terms;
   CUtensorMap map_x, map_h;
@@ -1151,10 +1159,12 @@ static int moe_chunk(const b200q_moe_args& a, int64_t first, cudaStream_t st) {
   return B200Q_OK;
 }
 
+static bool moe_has_workspace(const b200q_moe_args& a) {
+  return a.workspace && a.workspace_bytes >= moe_workspace_bytes_impl(a.tokens, a.hidden, a.inner, a.experts, a.top_k) && reinterpret_cast<uintptr_t>(a.workspace) % 16 == 0;
+}
+
 int moe_layer_impl(const b200q_moe_args& a, cudaStream_t st) {
-  if (!a.workspace || a.workspace_bytes < moe_workspace_bytes_impl(a.tokens, a.hidden, a.inner, a.experts, a.top_k) ||
-      reinterpret_cast<uintptr_t>(a.workspace) % 16)
-    return B200Q_ERR_BAD_ARGUMENT;
+  if (!moe_has_workspace(a)) return B200Q_ERR_BAD_ARGUMENT;
   for (int64_t t = 0; t < a.tokens; t += kMoeChunk) {
     b200q_moe_args c = a;
     c.tokens = a.tokens - t < kMoeChunk ? a.tokens - t : kMoeChunk;
@@ -1165,6 +1175,16 @@ int moe_layer_impl(const b200q_moe_args& a, cudaStream_t st) {
     if (int rc = moe_chunk(c, t, st)) return rc;
   }
   return B200Q_OK;
+}
+
+// The kernel for 8-bit weights and more tokens than a CTA chooses for by itself, with a wait that is in vain.
+int moe_selftest_impl(const b200q_moe_args& a, int lost, cudaStream_t st) {
+  if (lost < 0 || lost >= kMoeLostCount || !moe_has_workspace(a)) return B200Q_ERR_BAD_ARGUMENT;
+  if (!moe_fits_tensor_cores(a) || a.weight_dtype != B200Q_E4M3 || a.router_dtype != B200Q_BF16 || a.tokens <= 4 * kMoeWarps || a.tokens > kMoeChunk)
+    return B200Q_ERR_UNSUPPORTED;
+  const MoeSpace space(a.tokens, a.hidden, a.inner, a.experts, a.top_k);
+  if (int rc = moe_launch_router<__nv_bfloat16>(a, 0, space, st)) return rc;
+  return moe_launch_fused<true, kMoeGroupTokens, true>(a, 0, space, st, lost);
 }
 
 }  // namespace b200q

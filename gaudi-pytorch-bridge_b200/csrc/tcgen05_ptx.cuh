@@ -85,7 +85,7 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 // The same for two barriers at once: the two polls are in flight together (a poll of a completed phase takes
 // about a hundred cycles).
 [[nodiscard]] __device__ __forceinline__ bool mbar_wait2_uniform(uint32_t bar0, uint32_t parity0, uint32_t bar1, uint32_t parity1,
-                                                                 volatile int* abort_flag, int* status, int code) {
+                                                                 volatile int* abort_flag, int* status, int code, uint32_t limit = kWaitLimit) {
   uint32_t ok;
   asm volatile(
       "{\n"
@@ -99,7 +99,7 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
       : "r"(bar0), "r"(parity0), "r"(bar1), "r"(parity1)
       : "memory");
   if (__all_sync(0xFFFFFFFFu, ok)) return true;
-  return mbar_wait_uniform(bar0, parity0, abort_flag, status, code) && mbar_wait_uniform(bar1, parity1, abort_flag, status, code);
+  return mbar_wait_uniform(bar0, parity0, abort_flag, status, code, limit) && mbar_wait_uniform(bar1, parity1, abort_flag, status, code, limit);
 }
 // The index of the calling warp, known to be the same in all its lanes.
 __device__ __forceinline__ int uniform_warp_index() { return __shfl_sync(0xFFFFFFFFu, (int)(threadIdx.x >> 5), 0); }

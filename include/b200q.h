@@ -726,6 +726,10 @@ typedef struct b200q_moe_args {
 
 size_t b200q_moe_workspace_bytes(int64_t tokens, int64_t hidden, int64_t inner, int experts, int top_k);
 int b200q_moe_layer(const b200q_moe_args* args);
+/* Self-test of its bounded waits: the same call (45 to 256 tokens, e4m3 weights, a bf16 router, sizes of the tensor-core kernel, else B200Q_ERR_UNSUPPORTED) with short waits, in which
+ * one thing never comes: 0 a block's choices, 1 a block's results, 2 the weights of block 0's first step, 3 its tokens.  The kernel ends by itself, out is NaN
+ * and the status one of 821 to 825; the GPU does not fault. */
+int b200q_selftest_moe_wait_timeout(const b200q_moe_args* args, int lost);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,28 @@
+"""The norm, the adapters and the experts, without a GPU: what their self-tests refuse before any CUDA call."""
+import ctypes
+
+import pytest
+
+from b200_hpu_ops import abi
+from test_cpu_layer import AT, BAD, UNSUPPORTED, _call
+
+SOME = 1 << 40  # bytes of a workspace that nothing reads
+
+
+def _moe_selftest(lost=0, **kw):
+    a = abi.MoeArgs()
+    a.x, a.router, a.gate_up, a.down, a.out, a.weights, a.ids, a.workspace = (AT,) * 8
+    a.router_dtype, a.weight_dtype, a.out_dtype = abi.BF16, abi.E4M3, abi.BF16
+    a.tokens, a.hidden, a.inner, a.experts, a.top_k, a.x_stride, a.workspace_bytes = 45, 64, 32, 8, 2, 64, SOME
+    return _call(lambda p: abi.lib.b200q_selftest_moe_wait_timeout(p, lost), a, kw)
+
+
+@pytest.mark.parametrize("kw,rc", [(dict(lost=-1), BAD), (dict(lost=4), BAD), (dict(workspace=None), BAD), (dict(workspace_bytes=100), BAD), (dict(tokens=-1), BAD), (dict(tokens=0), BAD),
+                                   (dict(tokens=44), UNSUPPORTED), (dict(tokens=257), UNSUPPORTED), (dict(weight_dtype=abi.BF16), UNSUPPORTED), (dict(router_dtype=abi.F32), UNSUPPORTED),
+                                   (dict(force_plain=1), UNSUPPORTED), (dict(hidden=40), UNSUPPORTED)])
+def test_moe_selftest_refuses(kw, rc):
+    assert _moe_selftest(**kw) == rc
+
+
+def test_selftests_refuse_nothing():
+    assert abi.lib.b200q_selftest_moe_wait_timeout(ctypes.POINTER(abi.MoeArgs)(), 0) == BAD
