@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
   __shared__ uint16_t s_group_expert[kMostGroups], s_group_slot[kMostGroups];
   __shared__ uint8_t s_group_tokens[kMostGroups];
   constexpr int kQueue = 4;  // units that the producer is ahead of the others at most
-  __shared__ __align__(8) uint64_t s_bars[3 * kStages + 4 + 2 * kQueue];
+  __shared__ __align__(8) uint64_t s_bars[3 * kStages + 4 + 2 * kQueue + 1];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort, s_groups, s_slots, s_scan[2][kMoeWarps], s_unit[kQueue];
   __shared__ uint16_t s_expert_slot[kMoeMaxExperts];  // an expert's first slot
@@ -473,7 +473,7 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
   const int cta = blockIdx.x, ctas = gridDim.x;
   const uint32_t bar_weights = ptx::smem_u32(s_bars), bar_tokens = bar_weights + 8 * kStages, bar_empty = bar_tokens + 8 * kStages;
   const uint32_t bar_full = bar_empty + 8 * kStages, bar_free = bar_full + 16;  // of the two accumulators
-  const uint32_t bar_unit = bar_free + 16, bar_taken = bar_unit + 8 * kQueue;
+  const uint32_t bar_unit = bar_free + 16, bar_taken = bar_unit + 8 * kQueue, bar_last = bar_taken + 8 * kQueue;
   const uint32_t ring = ptx::smem_u32(s_ring);
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
@@ -489,6 +489,7 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
       ptx::mbar_init(bar_unit + 8 * i, 1);
       ptx::mbar_init(bar_taken + 8 * i, 6);  // (MMAs, terms, four of the results)
     }
+    ptx::mbar_init(bar_last, 1);
     s_abort = 0;
     ptx::fence_barrier_init();
     ptx::tma_prefetch_desc(&map_up);
@@ -611,7 +612,7 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
     return unit;
   };
 
-  // where a wait has run out: the copies in flight are waited for, as far as they come
+  // Before a CTA ends its copies in flight are waited for, as far as they come.  (Where no wait has run out they have been multiplied, or will be next.)
   int made = 0;
   auto drain = [&](uint32_t bars, uint32_t stage, uint32_t phase) {
     for (int i = 0; i < min(made, kStages); ++i) {
@@ -769,7 +770,7 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
     };
     stream(std::integral_constant<int, 0>());
     if (ok) stream(std::integral_constant<int, 1>());
-    if (!ok) drain(bar_weights, stage, phase);
+    drain(bar_weights, stage, phase);
   } else if (warp == 1) {
     // ------------------------------------------------------------ products
     uint32_t stage = 0, phase = 0;
@@ -810,6 +811,10 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
         }
       }
     }
+    // nor do products outlive the tensor memory and the ring
+    if (ptx::elect_one()) ptx::umma_commit(bar_last);
+    __syncwarp();
+    for (int k = 0; k < 4096 && !ptx::mbar_try_wait(bar_last, 0); ++k) __nanosleep(64);
   } else if (warp == 2) {
     // ------------------------------------------------------------ terms
     uint32_t stage = 0, phase = 0;
@@ -859,7 +864,7 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
     };
     stream(std::integral_constant<int, 0>());
     if (ok) stream(std::integral_constant<int, 1>());
-    if (!ok) drain(bar_tokens, stage, phase);
+    drain(bar_tokens, stage, phase);
   } else if (warp < 7) {
     // ------------------------------------------------------------ sums of cut tiles, terms of h
     const int row = tid - 96;
