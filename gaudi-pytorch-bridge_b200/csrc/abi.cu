@@ -614,15 +614,28 @@ size_t b200q_lora_workspace_bytes(int64_t tokens, int64_t k, int64_t n, int64_t 
   return lora_workspace_bytes_impl(tokens, k, n, rank, adapters);
 }
 
-int b200q_lora_add(const b200q_lora_args* a) {
+static bool lora_adds_nothing(const b200q_lora_args* a) { return a->tokens == 0 || a->n == 0 || a->rank == 0 || a->adapters == 0 || a->k == 0; }
+static int check_lora(const b200q_lora_args* a) {
   if (!a) return B200Q_ERR_BAD_ARGUMENT;
   if (a->tokens < 0 || a->k < 0 || a->n < 0 || a->rank < 0 || a->adapters < 0 || !is_wide(a->y_dtype)) return B200Q_ERR_BAD_ARGUMENT;
   if (a->tokens > 1 && a->y_stride < a->n) return B200Q_ERR_BAD_ARGUMENT;
   if (a->rank > kLoraMaxRank || a->adapters > kLoraMaxAdapters || a->tokens > INT32_MAX || a->k > INT32_MAX || a->n > INT32_MAX) return B200Q_ERR_TOO_LARGE;
-  if (a->tokens == 0 || a->n == 0 || a->rank == 0 || a->adapters == 0 || a->k == 0) return B200Q_OK;  // (nothing is added)
+  if (lora_adds_nothing(a)) return B200Q_OK;
   if (!a->x || !a->y || !a->a || !a->b || !a->adapter) return B200Q_ERR_BAD_ARGUMENT;
   if (!on_bytes(2, {a->x, a->a, a->b}) || !on_elements(a->y, a->y_dtype, 1) || !on_bytes(4, {a->adapter, a->scales})) return B200Q_ERR_UNSUPPORTED;
+  return B200Q_OK;
+}
+
+int b200q_lora_add(const b200q_lora_args* a) {
+  const int rc = check_lora(a);
+  if (rc || lora_adds_nothing(a)) return rc;
   return lora_add_impl(*a, static_cast<cudaStream_t>(a->stream));
+}
+
+int b200q_selftest_lora_wait_timeout(const b200q_lora_args* a, int lost) {
+  if (int rc = check_lora(a)) return rc;
+  if (lora_adds_nothing(a)) return B200Q_ERR_BAD_ARGUMENT;
+  return lora_selftest_impl(*a, lost, static_cast<cudaStream_t>(a->stream));
 }
 
 size_t b200q_moe_workspace_bytes(int64_t tokens, int64_t hidden, int64_t inner, int experts, int top_k) {

@@ -59,6 +59,7 @@ __global__ void __launch_bounds__(kLoraPlainThreads) lora_plain_up_kernel(const 
 constexpr int kLoraSortThreads = 1024;
 constexpr int kLoraFew = 128;  // tokens up to which each CTA sorts for itself
 constexpr int kLoraErrCopy = 831, kLoraErrMma = 832, kLoraErrResults = 833;  // status codes: a wait ran out
+constexpr uint32_t kLoraTestPolls = 1u << 14;  // of the self-test: some ten milliseconds
 
 struct __align__(16) LoraTile {
   int adapter, first, count, unused;  // tokens sorted[first] ...
@@ -266,7 +267,8 @@ struct LoraDownShape {
   }
 };
 
-template <int TILE, bool EXACT>  // EXACT: no more than kLoraSub steps are added inside the tensor core
+// EXACT: no more than kLoraSub steps are added inside the tensor core.  TEST: short waits, and the first copy of block 0 is never made.
+template <int TILE, bool EXACT, bool TEST>
 __global__ void __launch_bounds__(32 * kLoraDownWarps, TILE == 16 ? 4 : 2)
     lora_down_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_run, const b200q_lora_args a, const LoraPlan p, const LoraDownShape d) {
   extern __shared__ uint8_t s_raw[];
@@ -276,6 +278,7 @@ __global__ void __launch_bounds__(32 * kLoraDownWarps, TILE == 16 ? 4 : 2)
   __shared__ int s_abort;
   __shared__ __align__(16) LoraFew s_few;
   constexpr int kTmem = 2 * TILE < 32 ? 32 : 2 * TILE;
+  constexpr uint32_t kLimit = TEST ? kLoraTestPolls : ptx::kWaitLimit;
   const int tid = threadIdx.x, lane = tid & 31, warp = ptx::uniform_warp_index();
   const uint32_t ring = ptx::smem_u32(s_ring), bar_full = ptx::smem_u32(s_bars), bar_empty = bar_full + 8 * kLoraMostStages;
   const uint32_t bar_done = bar_empty + 8 * kLoraMostStages, bar_free = bar_done + 16;
@@ -341,12 +344,12 @@ __global__ void __launch_bounds__(32 * kLoraDownWarps, TILE == 16 ? 4 : 2)
       for (int r = 0; r < 4; ++r) run = run && (4 * lane + r >= it.tile.count || rows[r] == first + 4 * lane + r);
       run = __all_sync(0xFFFFFFFFu, run);
       for (int k = it.k0; k < it.k1; ++k) {
-        ok = ptx::mbar_wait_uniform(bar_empty + 8 * stage, phase ^ 1, &s_abort, p.status, kLoraErrCopy);
+        ok = ptx::mbar_wait_uniform(bar_empty + 8 * stage, phase ^ 1, &s_abort, p.status, kLoraErrCopy, kLimit);
         if (!ok) break;
         const uint32_t bar = bar_full + 8 * stage, dst = ring + stage * d.stage;
         if (ptx::elect_one()) {
           ptx::mbar_arrive_expect_tx(bar, d.row_bytes + (run ? TILE * 128 : eights * 1024));
-          ptx::tma_load_3d(dst, &map_a, bar, 64 * k, 128 * it.block, it.tile.adapter);
+          if (!(TEST && blockIdx.x == 0 && made == 0)) ptx::tma_load_3d(dst, &map_a, bar, 64 * k, 128 * it.block, it.tile.adapter);
           if (run) ptx::tma_load_2d(dst + d.row_bytes, &map_run, bar, 64 * k, first);  // (rows behind the tile's are columns that nobody looks at)
         }
         __syncwarp();
@@ -373,12 +376,12 @@ __global__ void __launch_bounds__(32 * kLoraDownWarps, TILE == 16 ? 4 : 2)
         if (sub == 0) {
           acc = n & 1;
           out = tmem + acc * TILE;
-          ok = ptx::mbar_wait_uniform(bar_free + 8 * acc, ((n >> 1) & 1) ^ 1, &s_abort, p.status, kLoraErrMma);
+          ok = ptx::mbar_wait_uniform(bar_free + 8 * acc, ((n >> 1) & 1) ^ 1, &s_abort, p.status, kLoraErrMma, kLimit);
           if (!ok) break;
           ++n;
           ptx::tc_fence_after();
         }
-        ok = ptx::mbar_wait_uniform(bar_full + 8 * stage, phase, &s_abort, p.status, kLoraErrMma);
+        ok = ptx::mbar_wait_uniform(bar_full + 8 * stage, phase, &s_abort, p.status, kLoraErrMma, kLimit);
         if (!ok) break;
         ptx::tc_fence_after();
         if (ptx::elect_one()) {
@@ -396,9 +399,10 @@ __global__ void __launch_bounds__(32 * kLoraDownWarps, TILE == 16 ? 4 : 2)
       }
     }
   } else {
+    // Where a wait has run out, what should be there is NaN: the other kernel would make finite values of whatever lay there.
     int n = 0;
     const int quarter = warp & 3;
-    for (int i = blockIdx.x; i < items && ok; i += gridDim.x) {
+    for (int i = blockIdx.x; i < items; i += gridDim.x) {
       const Item it = item_of(i);
       const int r = 128 * it.block + 32 * quarter + lane;
       constexpr int kHeld = (TILE + 31) / 32;
@@ -407,18 +411,19 @@ __global__ void __launch_bounds__(32 * kLoraDownWarps, TILE == 16 ? 4 : 2)
       for (int h = 0; h < kHeld; ++h) held[h] = 32 * h + lane < it.tile.count ? view.sorted[it.tile.first + 32 * h + lane] : 0;
       // (a part behind the end of k: zeros)
       for (int k = it.k0; k == it.k0 || (EXACT && k < it.k1); k += kLoraSub) {
-        const bool none = it.k0 >= it.k1;
+        bool none = it.k0 >= it.k1;
         const uint32_t acc = n & 1, in = tmem + acc * TILE + ((uint32_t)(32 * quarter) << 16);
         if (!none) {
-          ok = ptx::mbar_wait_uniform(bar_done + 8 * acc, (n >> 1) & 1, &s_abort, p.status, kLoraErrResults);
-          if (!ok) break;
+          ok = ok && ptx::mbar_wait_uniform(bar_done + 8 * acc, (n >> 1) & 1, &s_abort, p.status, kLoraErrResults, kLimit);
+          none = !ok;
           ++n;
           ptx::tc_fence_after();
         }
+        const float nothing = ok ? 0.f : __int_as_float(0x7FC00000);
 #pragma unroll
         for (int h = 0; h < kHeld; ++h)
           for (int j0 = 32 * h; j0 < min(it.tile.count, 32 * h + 32); j0 += 8) {
-            float v[8] = {};
+            float v[8] = {nothing, nothing, nothing, nothing, nothing, nothing, nothing, nothing};
             if (!none) {
               layer_tmem_ld8(in + j0, v);
               ptx::tmem_ld_wait();
@@ -497,7 +502,7 @@ __device__ __forceinline__ void lora_store16(Y* p, const uint4& w) {
   }
 }
 
-template <typename Y, int TILE, bool WHOLE>
+template <typename Y, int TILE, bool WHOLE, bool TEST>  // TEST: short waits, and the first copy of block 0 is never made
 __global__ void __launch_bounds__(lora_up_threads(TILE), lora_up_ctas(sizeof(Y) == 4, TILE)) lora_up_kernel(const __grid_constant__ CUtensorMap map_b, const b200q_lora_args a, const LoraPlan p, const LoraUpShape d) {
   constexpr int kTerms = sizeof(Y) == 4 ? 3 : 2, kStage = 128 * 128, kWarps = lora_result_warps(TILE), kHalf = TILE / (kWarps / 4);
   constexpr int kPer = 16 / sizeof(Y), kLanes = 32 / kPer, kRows = 32 / kLanes, kPieces = kHalf / kRows;  // values of a lane's piece of a row; lanes of a row
@@ -510,6 +515,7 @@ __global__ void __launch_bounds__(lora_up_threads(TILE), lora_up_ctas(sizeof(Y) 
   __shared__ int s_abort;
   __shared__ __align__(16) LoraFew s_few;
   constexpr int kTmem = 2 * TILE < 32 ? 32 : 2 * TILE;
+  constexpr uint32_t kLimit = TEST ? kLoraTestPolls : ptx::kWaitLimit;
   const int tid = threadIdx.x, lane = tid & 31, warp = ptx::uniform_warp_index();
   const uint32_t terms = ptx::smem_u32(s_terms), ring = terms + d.terms_bytes;
   const uint32_t bar_full = ptx::smem_u32(s_bars), bar_empty = bar_full + 8 * kLoraMostStages, bar_done = bar_empty + 8 * kLoraMostStages, bar_free = bar_done + 16;
@@ -553,11 +559,11 @@ __global__ void __launch_bounds__(lora_up_threads(TILE), lora_up_ctas(sizeof(Y) 
       const int tile = i / parts, part = i - tile * parts, adapter = view.tile(tile).adapter;
       for (int n = part; n < n_blocks && ok; n += parts)
         for (int c = 0; c < d.chunks; ++c) {
-          ok = ptx::mbar_wait_uniform(bar_empty + 8 * stage, phase ^ 1, &s_abort, p.status, kLoraErrCopy);
+          ok = ptx::mbar_wait_uniform(bar_empty + 8 * stage, phase ^ 1, &s_abort, p.status, kLoraErrCopy, kLimit);
           if (!ok) break;
           if (ptx::elect_one()) {
             ptx::mbar_arrive_expect_tx(bar_full + 8 * stage, kStage);
-            ptx::tma_load_3d(ring + stage * kStage, &map_b, bar_full + 8 * stage, 64 * c, 128 * n, adapter);
+            if (!(TEST && blockIdx.x == 0 && made == 0)) ptx::tma_load_3d(ring + stage * kStage, &map_b, bar_full + 8 * stage, 64 * c, 128 * n, adapter);
           }
           __syncwarp();
           ++made;
@@ -575,14 +581,14 @@ __global__ void __launch_bounds__(lora_up_threads(TILE), lora_up_ctas(sizeof(Y) 
     for (int i = blockIdx.x; i < items && ok; i += gridDim.x, ++item) {
       const int tile = i / parts, part = i - tile * parts;
       const uint32_t idesc = ptx::umma_idesc(1, 1, 128, lora_columns(view.tile(tile).count));
-      ok = ptx::mbar_wait_uniform(bar_terms, item & 1, &s_abort, p.status, kLoraErrMma);
+      ok = ptx::mbar_wait_uniform(bar_terms, item & 1, &s_abort, p.status, kLoraErrMma, kLimit);
       for (int n = part; n < n_blocks && ok; n += parts, ++done) {
         const uint32_t acc = done & 1, out = tmem + acc * TILE;
-        ok = ptx::mbar_wait_uniform(bar_free + 8 * acc, ((done >> 1) & 1) ^ 1, &s_abort, p.status, kLoraErrMma);
+        ok = ptx::mbar_wait_uniform(bar_free + 8 * acc, ((done >> 1) & 1) ^ 1, &s_abort, p.status, kLoraErrMma, kLimit);
         if (!ok) break;
         ptx::tc_fence_after();
         for (int c = 0; c < d.chunks; ++c) {
-          ok = ptx::mbar_wait_uniform(bar_full + 8 * stage, phase, &s_abort, p.status, kLoraErrMma);
+          ok = ptx::mbar_wait_uniform(bar_full + 8 * stage, phase, &s_abort, p.status, kLoraErrMma, kLimit);
           if (!ok) break;
           ptx::tc_fence_after();
           if (ptx::elect_one()) {
@@ -622,7 +628,7 @@ __global__ void __launch_bounds__(lora_up_threads(TILE), lora_up_ctas(sizeof(Y) 
         for (int c = 0; c < kPieces; ++c) ask(c, part);
         if (item == 0) pdl_enter();
       }
-      ok = ok && ptx::mbar_wait_uniform(bar_used, (item & 1) ^ 1, &s_abort, p.status, kLoraErrResults);  // (the products with the terms before are done)
+      ok = ok && ptx::mbar_wait_uniform(bar_used, (item & 1) ^ 1, &s_abort, p.status, kLoraErrResults, kLimit);  // (the products with the terms before are done)
       const float scale = a.scales ? a.scales[tile.adapter] : 1.f;
       // The terms: a thread has four ranks of a token or two at a time, eight parts of k at once.  (Eight ranks of a token, two parts at once: twice the sectors, 89 us for
       // 4096 tokens where this is 86; what spills, four tokens and two parts for instance, 110.)
@@ -681,7 +687,7 @@ __global__ void __launch_bounds__(lora_up_threads(TILE), lora_up_ctas(sizeof(Y) 
       if (lane == 0) ptx::mbar_arrive(bar_terms);
       for (int n = part; n < n_blocks && ok; n += parts, ++done) {
         const uint32_t acc = done & 1, in = tmem + acc * TILE + kHalf * half + ((uint32_t)(32 * quarter) << 16);
-        ok = ptx::mbar_wait_uniform(bar_done + 8 * acc, (done >> 1) & 1, &s_abort, p.status, kLoraErrResults);
+        ok = ptx::mbar_wait_uniform(bar_done + 8 * acc, (done >> 1) & 1, &s_abort, p.status, kLoraErrResults, kLimit);
         if (!ok) break;
         ptx::tc_fence_after();
         const bool there = 128 * n + my_column < a.n;
@@ -779,10 +785,10 @@ static int lora_ready(const void* kernel, std::atomic<int> (&done)[kMaxDevices],
 
 constexpr int kLoraShared = 100 * 1024;  // of a CTA where two share an SM, beside what its kernel has of its own
 
-template <int TILE, bool EXACT>
+template <int TILE, bool EXACT, bool TEST = false>
 static int lora_launch_down(const b200q_lora_args& a, const LoraPlan& p, int64_t tiles, cudaStream_t st) {
   static std::atomic<int> done[kMaxDevices];
-  if (int rc = lora_ready(reinterpret_cast<const void*>(lora_down_kernel<TILE, EXACT>), done, kLoraShared)) return rc;
+  if (int rc = lora_ready(reinterpret_cast<const void*>(lora_down_kernel<TILE, EXACT, TEST>), done, kLoraShared)) return rc;
   const int ctas = lora_down_ctas(a.rank, TILE);
   const LoraDownShape d((int)a.rank, TILE, (ctas == 2 ? kLoraShared : 220 * 1024 / ctas - 4096) - 1024);
   CUtensorMap map_a, map_x, map_run;
@@ -791,16 +797,16 @@ static int lora_launch_down(const b200q_lora_args& a, const LoraPlan& p, int64_t
   if (int rc = lora_map(&map_run, a.x, a.k, a.tokens, 1, a.x_stride, 0, TILE, 2)) return rc;
   const int64_t items = tiles * p.splits * ((a.rank + 127) / 128), most = p.slots;
   // (the rows behind a block's ranks, which the product reads too and whose results nobody looks at, are within the allocation)
-  launch_dependent(lora_down_kernel<TILE, EXACT>, dim3((unsigned)(items < most ? items : most)), dim3(32 * kLoraDownWarps), (size_t)d.stages * d.stage + 16384 + 1024, st, map_a, map_x,
+  launch_dependent(lora_down_kernel<TILE, EXACT, TEST>, dim3((unsigned)(items < most ? items : most)), dim3(32 * kLoraDownWarps), (size_t)d.stages * d.stage + 16384 + 1024, st, map_a, map_x,
                    map_run, a, p, d);
   B200Q_LAUNCH_CHECK();
   return B200Q_OK;
 }
-template <typename Y, int TILE, bool WHOLE>
+template <typename Y, int TILE, bool WHOLE, bool TEST = false>
 static int lora_launch_up(const b200q_lora_args& a, const LoraPlan& p, int64_t tiles, cudaStream_t st) {
   constexpr int kTerms = sizeof(Y) == 4 ? 3 : 2, kMost = 200 * 1024;
   static std::atomic<int> done[kMaxDevices];
-  if (int rc = lora_ready(reinterpret_cast<const void*>(lora_up_kernel<Y, TILE, WHOLE>), done, kMost)) return rc;
+  if (int rc = lora_ready(reinterpret_cast<const void*>(lora_up_kernel<Y, TILE, WHOLE, TEST>), done, kMost)) return rc;
   CUtensorMap map_b;
   if (int rc = lora_map(&map_b, a.b, a.rank, a.n, a.adapters, a.b_row_stride, a.b_stride, 128, 3)) return rc;
   LoraUpShape d;
@@ -812,20 +818,25 @@ static int lora_launch_up(const b200q_lora_args& a, const LoraPlan& p, int64_t t
   const int room = (d.terms_bytes + 2 * 16384 + 1024 <= kShare ? kShare : kMost) - 1024 - d.terms_bytes;
   d.stages = room / 16384 < kLoraMostStages ? room / 16384 : kLoraMostStages;
   const int64_t items = tiles * ((a.n + 127) / 128), most = kCtas * kNumSMs;
-  launch_dependent(lora_up_kernel<Y, TILE, WHOLE>, dim3((unsigned)(items < most ? items : most)), dim3(lora_up_threads(TILE)), (size_t)d.terms_bytes + d.stages * 16384 + 1024, st, map_b, a, p,
+  launch_dependent(lora_up_kernel<Y, TILE, WHOLE, TEST>, dim3((unsigned)(items < most ? items : most)), dim3(lora_up_threads(TILE)), (size_t)d.terms_bytes + d.stages * 16384 + 1024, st, map_b, a, p,
                    d);
   B200Q_LAUNCH_CHECK();
   return B200Q_OK;
 }
 
+static bool lora_y_whole(const b200q_lora_args& a) {  // rows of y on boundaries of 16 bytes
+  return reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && (a.tokens == 1 || a.y_stride * (a.y_dtype == B200Q_F32 ? 4 : 2) % 16 == 0);
+}
 template <typename Y>
 static int lora_launch_up_tile(const b200q_lora_args& a, const LoraPlan& p, int64_t tiles, cudaStream_t st) {
-  const bool whole = reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && (a.tokens == 1 || a.y_stride * sizeof(Y) % 16 == 0);
+  const bool whole = lora_y_whole(a);
   if (p.tile == 16) return whole ? lora_launch_up<Y, 16, true>(a, p, tiles, st) : lora_launch_up<Y, 16, false>(a, p, tiles, st);
   return whole ? lora_launch_up<Y, 128, true>(a, p, tiles, st) : lora_launch_up<Y, 128, false>(a, p, tiles, st);
 }
 
-static int lora_chunk_fast(const b200q_lora_args& a, cudaStream_t st) {
+enum LoraLost { kLoraLostNothing = -1, kLoraLostA, kLoraLostB, kLoraLostCount };  // what a self-test waits for in vain: the first copy of a, or of b, of block 0
+
+static int lora_chunk_fast(const b200q_lora_args& a, cudaStream_t st, int lost = kLoraLostNothing) {
   const int tile = lora_tile_tokens(a.tokens, a.rank, a.adapters, a.y_dtype == B200Q_F32);
   const int64_t splits = lora_splits(a.tokens, a.k, a.rank, a.adapters, tile), tiles = lora_most_tiles(a.tokens, a.adapters, tile);
   const LoraSpace space(a.tokens, a.rank, splits);
@@ -850,6 +861,10 @@ static int lora_chunk_fast(const b200q_lora_args& a, cudaStream_t st) {
     launch_dependent(lora_sort_kernel, dim3(1), dim3(kLoraSortThreads), sizeof(uint16_t) * (kLoraSortThreads / 32 + 1) * (size_t)a.adapters, st, a, p);
     B200Q_LAUNCH_CHECK();
   }
+  if (lost != kLoraLostNothing) {  // (tiles of 16 tokens, y in bf16 and on boundaries of 16 bytes)
+    if (int rc = lost == kLoraLostA ? lora_launch_down<16, false, true>(a, p, tiles, st) : lora_launch_down<16, false>(a, p, tiles, st)) return rc;
+    return lost == kLoraLostB ? lora_launch_up<__nv_bfloat16, 16, true, true>(a, p, tiles, st) : lora_launch_up<__nv_bfloat16, 16, true>(a, p, tiles, st);
+  }
   int rc;
   if (a.y_dtype == B200Q_F32) rc = tile == 16 ? lora_launch_down<16, true>(a, p, tiles, st) : lora_launch_down<128, true>(a, p, tiles, st);
   else rc = tile == 16 ? lora_launch_down<16, false>(a, p, tiles, st) : lora_launch_down<128, false>(a, p, tiles, st);
@@ -869,10 +884,12 @@ static int lora_chunk_plain(const b200q_lora_args& a, cudaStream_t st) {
   return B200Q_OK;
 }
 
+static bool lora_has_workspace(const b200q_lora_args& a) {
+  return a.workspace && a.workspace_bytes >= lora_workspace_bytes_impl(a.tokens, a.k, a.n, a.rank, a.adapters) && reinterpret_cast<uintptr_t>(a.workspace) % 16 == 0;
+}
+
 int lora_add_impl(const b200q_lora_args& a, cudaStream_t st) {
-  if (!a.workspace || a.workspace_bytes < lora_workspace_bytes_impl(a.tokens, a.k, a.n, a.rank, a.adapters) ||
-      reinterpret_cast<uintptr_t>(a.workspace) % 16)
-    return B200Q_ERR_BAD_ARGUMENT;
+  if (!lora_has_workspace(a)) return B200Q_ERR_BAD_ARGUMENT;
   for (int64_t t = 0; t < a.tokens; t += kLoraChunk) {
     b200q_lora_args c = a;
     c.tokens = a.tokens - t < kLoraChunk ? a.tokens - t : kLoraChunk;
@@ -884,6 +901,13 @@ int lora_add_impl(const b200q_lora_args& a, cudaStream_t st) {
     if (rc) return rc;
   }
   return B200Q_OK;
+}
+
+int lora_selftest_impl(const b200q_lora_args& a, int lost, cudaStream_t st) {
+  if (lost < 0 || lost >= kLoraLostCount || !lora_has_workspace(a)) return B200Q_ERR_BAD_ARGUMENT;
+  if (!lora_fits_tensor_cores(a) || a.y_dtype != B200Q_BF16 || !lora_y_whole(a) || a.tokens > kLoraChunk || lora_tile_tokens(a.tokens, a.rank, a.adapters, false) != 16)
+    return B200Q_ERR_UNSUPPORTED;
+  return lora_chunk_fast(a, st, lost);
 }
 
 }  // namespace b200q

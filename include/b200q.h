@@ -661,7 +661,8 @@ int b200q_add_rms_norm_cast(const b200q_norm_args* args);
  * rank <= 256, adapters <= 2048
  * workspace     b200q_lora_workspace_bytes(...) bytes, 16-byte aligned, not shared by calls that may overlap
  * rank, k and n of multiples of 8 with rows of x, a and b apart and on 16-byte boundaries run tensor-core kernels (y may lie anywhere), anything else (or
- * force_plain = 1) plain ones.  y must not overlap the inputs.  The same call gives the same bytes.  Status 831 to 833: a wait ran out (some of y is as it was).
+ * force_plain = 1) plain ones.  y must not overlap the inputs.  The same call gives the same bytes.  Status 831 to 833: a wait ran out (of y, what was
+ * to come behind it is as it was, or NaN).
  */
 typedef struct b200q_lora_args {
   const void* x;
@@ -682,6 +683,9 @@ typedef struct b200q_lora_args {
 
 size_t b200q_lora_workspace_bytes(int64_t tokens, int64_t k, int64_t n, int64_t rank, int64_t adapters);
 int b200q_lora_add(const b200q_lora_args* args);
+/* Self-test of its bounded waits: the same call (up to 8192 tokens, so many adapters or so few tokens that tiles have 16, bf16 y on boundaries of 16 bytes, sizes of the tensor-core kernels,
+ * else B200Q_ERR_UNSUPPORTED) with short waits, in which one copy never comes: block 0's first of a (lost = 0), or of b (1).  The kernels end by themselves; the GPU does not fault. */
+int b200q_selftest_lora_wait_timeout(const b200q_lora_args* args, int lost);
 
 /*
  * moe_layer: a whole mixture-of-experts layer (router, choice, gated experts, sum) for a few tokens.  Per token x

@@ -26,3 +26,23 @@ def test_moe_selftest_refuses(kw, rc):
 
 def test_selftests_refuse_nothing():
     assert abi.lib.b200q_selftest_moe_wait_timeout(ctypes.POINTER(abi.MoeArgs)(), 0) == BAD
+
+
+def _lora_selftest(lost=0, **kw):
+    a = abi.LoraArgs()
+    a.x, a.y, a.a, a.b, a.adapter, a.workspace = AT, AT << 4, AT << 5, AT << 6, AT, AT
+    a.y_dtype = abi.BF16
+    a.tokens, a.k, a.n, a.rank, a.adapters = 3, 64, 32, 16, 2
+    a.x_stride, a.y_stride, a.a_stride, a.a_row_stride, a.b_stride, a.b_row_stride, a.workspace_bytes = 64, 32, 1024, 64, 512, 16, SOME
+    return _call(lambda p: abi.lib.b200q_selftest_lora_wait_timeout(p, lost), a, kw)
+
+
+@pytest.mark.parametrize("kw,rc", [(dict(lost=-1), BAD), (dict(lost=2), BAD), (dict(workspace=None), BAD), (dict(workspace_bytes=100), BAD), (dict(tokens=-1), BAD), (dict(tokens=0), BAD),
+                                   (dict(rank=0), BAD), (dict(tokens=200), UNSUPPORTED), (dict(tokens=8193), UNSUPPORTED), (dict(y_dtype=abi.F32), UNSUPPORTED),
+                                   (dict(y=(AT << 4) + 2), UNSUPPORTED), (dict(force_plain=1), UNSUPPORTED), (dict(rank=12), UNSUPPORTED)])
+def test_lora_selftest_refuses(kw, rc):
+    assert _lora_selftest(**kw) == rc
+
+
+def test_lora_selftest_refuses_nothing():
+    assert abi.lib.b200q_selftest_lora_wait_timeout(ctypes.POINTER(abi.LoraArgs)(), 0) == BAD

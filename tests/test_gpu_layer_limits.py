@@ -49,3 +49,41 @@ def test_moe_that_waits_in_vain(tokens, hidden, inner, experts, top_k, lost):
         for got, w in zip(_run_moe(case, top_k), want):
             assert torch.equal(got.cpu(), w)
     assert b200_hpu_ops.device_status() == 0
+
+
+def _lora_args(y, x, a, b, which, scales, plain=0):
+    from b200_hpu_ops import abi
+    d = [_cu(t) for t in (y.clone(), x, a, b, which, scales)]
+    (tokens, n), k, adapters, rank = y.shape, x.shape[1], a.shape[0], a.shape[1]
+    size = abi.lib.b200q_lora_workspace_bytes(tokens, k, n, rank, adapters)
+    ws = torch.full((size,), 0x3F, dtype=torch.uint8, device="cuda")  # (as fp32: finite)
+    args = abi.LoraArgs(x=d[1].data_ptr(), x_stride=k, y=d[0].data_ptr(), y_dtype=abi.DTYPE[y.dtype], y_stride=n, a=d[2].data_ptr(), b=d[3].data_ptr(), a_stride=rank * k, a_row_stride=k,
+                        b_stride=n * rank, b_row_stride=rank, adapter=d[4].data_ptr(), scales=None if scales is None else d[5].data_ptr(), tokens=tokens, k=k, n=n, rank=rank,
+                        adapters=adapters, workspace=ws.data_ptr(), workspace_bytes=size, force_plain=plain, stream=abi.stream_ptr())
+    return args, d[0], (d, ws)
+
+
+@pytest.mark.parametrize("lost", [0, 1])
+@pytest.mark.parametrize("tokens,k,n,rank,adapters", [(1, 256, 128, 16, 1), (40, 4104, 520, 32, 5), (300, 520, 264, 16, 40), (6000, 264, 136, 16, 1900)])
+def test_lora_that_waits_in_vain(tokens, k, n, rank, adapters, lost):
+    """A copy never comes: the wait runs out (no GPU fault), the status says so, a value of y that missed something is NaN or as it was, the others have an undisturbed
+    call's bytes, and the next call is as it should be."""
+    import b200_hpu_ops
+    from b200_hpu_ops import abi
+    c = _lora_case(tokens, k, n, rank, adapters, BF16, which=torch.arange(tokens) % (adapters + 1))
+    y, which = c[0], c[4]
+    want = _run_lora(*c).cpu()
+    _check_lora(want, *c)
+    for _ in range(2):
+        a, got, held = _lora_args(*c)
+        abi.check(abi.lib.b200q_selftest_lora_wait_timeout(C.byref(a), lost))
+        assert 831 <= b200_hpu_ops.device_status() <= 833
+        got = got.cpu()
+        missed = got.isnan() if lost == 0 else (got != want) & (got == y)
+        assert torch.equal(got[~missed], want[~missed])
+        rows = missed.any(-1)
+        assert bool(rows.any()) and bool((which[rows] < adapters).all()) and (tokens == 1 or not bool(rows[which < adapters].all()))
+        if lost == 0:
+            assert torch.equal(missed.all(-1), rows)
+        assert torch.equal(_run_lora(*c).cpu(), want)
+    assert b200_hpu_ops.device_status() == 0
