@@ -240,13 +240,19 @@ __device__ __forceinline__ LoraView lora_view(const b200q_lora_args& a, const Lo
   return {used, false, few.tiles, few.sorted};
 }
 
-// where a wait has run out: the last copies are waited for, as far as they come
+// Before a CTA ends its last copies are waited for, as far as they come.  (Where no wait has run out they have been multiplied, or will be next.)
 __device__ __forceinline__ void lora_drain(uint32_t bars, int stages, int made, uint32_t stage, uint32_t phase) {
   for (int i = 0; i < min(made, stages); ++i) {
     phase ^= stage == 0;
     stage = stage == 0 ? stages - 1 : stage - 1;
     for (int k = 0; k < 4096 && !ptx::mbar_try_wait(bars + 8 * stage, phase); ++k) __nanosleep(64);
   }
+}
+// nor do products outlive the tensor memory and the ring (the warp that issued them; `bar` is for this alone)
+__device__ __forceinline__ void lora_drain_products(uint32_t bar) {
+  if (ptx::elect_one()) ptx::umma_commit(bar);
+  __syncwarp();
+  for (int k = 0; k < 4096 && !ptx::mbar_try_wait(bar, 0); ++k) __nanosleep(64);
 }
 __host__ __device__ constexpr int lora_columns(int tokens) { return (tokens + 15) / 16 * 16; }
 
@@ -273,7 +279,7 @@ __global__ void __launch_bounds__(32 * kLoraDownWarps, TILE == 16 ? 4 : 2)
     lora_down_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_run, const b200q_lora_args a, const LoraPlan p, const LoraDownShape d) {
   extern __shared__ uint8_t s_raw[];
   uint8_t* const s_ring = s_raw + (0u - ptx::smem_u32(s_raw) & 1023u);
-  __shared__ __align__(8) uint64_t s_bars[2 * kLoraMostStages + 4];
+  __shared__ __align__(8) uint64_t s_bars[2 * kLoraMostStages + 5];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   __shared__ __align__(16) LoraFew s_few;
@@ -281,7 +287,7 @@ __global__ void __launch_bounds__(32 * kLoraDownWarps, TILE == 16 ? 4 : 2)
   constexpr uint32_t kLimit = TEST ? kLoraTestPolls : ptx::kWaitLimit;
   const int tid = threadIdx.x, lane = tid & 31, warp = ptx::uniform_warp_index();
   const uint32_t ring = ptx::smem_u32(s_ring), bar_full = ptx::smem_u32(s_bars), bar_empty = bar_full + 8 * kLoraMostStages;
-  const uint32_t bar_done = bar_empty + 8 * kLoraMostStages, bar_free = bar_done + 16;
+  const uint32_t bar_done = bar_empty + 8 * kLoraMostStages, bar_free = bar_done + 16, bar_last = bar_free + 16;
   if (tid == 0) {
     for (int i = 0; i < d.stages; ++i) {
       ptx::mbar_init(bar_full + 8 * i, 1);
@@ -291,6 +297,7 @@ __global__ void __launch_bounds__(32 * kLoraDownWarps, TILE == 16 ? 4 : 2)
       ptx::mbar_init(bar_done + 8 * i, 1);
       ptx::mbar_init(bar_free + 8 * i, 4);
     }
+    ptx::mbar_init(bar_last, 1);
     s_abort = 0;
     ptx::fence_barrier_init();
     ptx::tma_prefetch_desc(&map_a);
@@ -362,7 +369,7 @@ __global__ void __launch_bounds__(32 * kLoraDownWarps, TILE == 16 ? 4 : 2)
         }
       }
     }
-    if (!ok) lora_drain(bar_full, d.stages, made, stage, phase);
+    lora_drain(bar_full, d.stages, made, stage, phase);
   } else if (warp == 1) {
     uint32_t stage = 0, phase = 0;
     int n = 0;
@@ -398,6 +405,7 @@ __global__ void __launch_bounds__(32 * kLoraDownWarps, TILE == 16 ? 4 : 2)
         }
       }
     }
+    lora_drain_products(bar_last);
   } else {
     // Where a wait has run out, what should be there is NaN: the other kernel would make finite values of whatever lay there.
     int n = 0;
@@ -509,7 +517,7 @@ __global__ void __launch_bounds__(lora_up_threads(TILE), lora_up_ctas(sizeof(Y) 
   constexpr int kBatch = kHalf < 16 ? kHalf : 16, kPitch = 36;  // tokens turned around together; floats of a token's 32 results
   extern __shared__ uint8_t s_raw[];
   uint8_t* const s_terms = s_raw + (0u - ptx::smem_u32(s_raw) & 1023u);  // [terms][chunks][tokens][128 bytes], then the ring
-  __shared__ __align__(8) uint64_t s_bars[2 * kLoraMostStages + 6];
+  __shared__ __align__(8) uint64_t s_bars[2 * kLoraMostStages + 7];
   __shared__ uint32_t s_tmem;
   __shared__ __align__(16) float s_turn[kWarps][kBatch * kPitch];
   __shared__ int s_abort;
@@ -519,7 +527,7 @@ __global__ void __launch_bounds__(lora_up_threads(TILE), lora_up_ctas(sizeof(Y) 
   const int tid = threadIdx.x, lane = tid & 31, warp = ptx::uniform_warp_index();
   const uint32_t terms = ptx::smem_u32(s_terms), ring = terms + d.terms_bytes;
   const uint32_t bar_full = ptx::smem_u32(s_bars), bar_empty = bar_full + 8 * kLoraMostStages, bar_done = bar_empty + 8 * kLoraMostStages, bar_free = bar_done + 16;
-  const uint32_t bar_terms = bar_free + 16, bar_used = bar_terms + 8;
+  const uint32_t bar_terms = bar_free + 16, bar_used = bar_terms + 8, bar_last = bar_used + 8;
   if (tid == 0) {
     for (int i = 0; i < d.stages; ++i) {
       ptx::mbar_init(bar_full + 8 * i, 1);
@@ -531,6 +539,7 @@ __global__ void __launch_bounds__(lora_up_threads(TILE), lora_up_ctas(sizeof(Y) 
     }
     ptx::mbar_init(bar_terms, kWarps);
     ptx::mbar_init(bar_used, 1);
+    ptx::mbar_init(bar_last, 1);
     s_abort = 0;
     ptx::fence_barrier_init();
     ptx::tma_prefetch_desc(&map_b);
@@ -573,7 +582,7 @@ __global__ void __launch_bounds__(lora_up_threads(TILE), lora_up_ctas(sizeof(Y) 
           }
         }
     }
-    if (!ok) lora_drain(bar_full, d.stages, made, stage, phase);
+    lora_drain(bar_full, d.stages, made, stage, phase);
   } else if (warp == 1) {
     uint32_t stage = 0, phase = 0;
     int done = 0, item = 0;
@@ -607,6 +616,7 @@ __global__ void __launch_bounds__(lora_up_threads(TILE), lora_up_ctas(sizeof(Y) 
       if (ok && ptx::elect_one()) ptx::umma_commit(bar_used);
       __syncwarp();
     }
+    lora_drain_products(bar_last);
   } else {
     int done = 0, item = 0;
     const int wt = tid - 64, quarter = warp & 3, half = (warp - 2) >> 2, my_row = lane / kLanes, my_column = 32 * quarter + lane % kLanes * kPer;
