@@ -25,7 +25,7 @@ EXPORTS = [
     "b200q_paged_plan", "b200q_qk_norm_rope_append", "b200q_paged_attention_workspace_bytes", "b200q_paged_attention",
     "b200q_selftest_paged_wait_timeout",
     "b200q_add_rms_norm_cast", "b200q_lora_workspace_bytes", "b200q_lora_add", "b200q_moe_workspace_bytes", "b200q_moe_layer",
-    "b200q_selftest_moe_wait_timeout", "b200q_selftest_lora_wait_timeout",
+    "b200q_selftest_moe_wait_timeout", "b200q_selftest_lora_wait_timeout", "b200q_selftest_norm_wait_timeout",
 ]
 
 DTYPE = {torch.float32: F32, torch.bfloat16: BF16, torch.float8_e4m3fn: E4M3, torch.float8_e5m2: E5M2}
@@ -191,6 +191,7 @@ def _bind():
     lib.b200q_moe_workspace_bytes.restype = C.c_size_t
     lib.b200q_moe_workspace_bytes.argtypes = [C.c_int64, C.c_int64, C.c_int64, C.c_int, C.c_int]
     lib.b200q_moe_layer.argtypes = [C.POINTER(MoeArgs)]
+    lib.b200q_selftest_norm_wait_timeout.argtypes = [C.POINTER(NormArgs)]
     lib.b200q_selftest_lora_wait_timeout.argtypes = [C.POINTER(LoraArgs), C.c_int]
     lib.b200q_selftest_moe_wait_timeout.argtypes = [C.POINTER(MoeArgs), C.c_int]
     return lib

@@ -592,7 +592,8 @@ int b200q_w4a16_gemm_noalloc(const void* x, int64_t ldx, const int32_t* qweight,
                                  static_cast<cudaStream_t>(stream));
 }
 
-int b200q_add_rms_norm_cast(const b200q_norm_args* a) {
+static bool norm_writes_nothing(const b200q_norm_args* a) { return a->tokens == 0 || (a->dim == 0 && !a->scale_inv); }
+static int check_norm(const b200q_norm_args* a) {
   if (!a) return B200Q_ERR_BAD_ARGUMENT;
   if (a->tokens < 0 || a->dim < 0 || !is_wide(a->x_dtype) || !(a->out_dtype == B200Q_BF16 || is_fp8(a->out_dtype))) return B200Q_ERR_BAD_ARGUMENT;
   if (a->weight && !is_wide(a->weight_dtype)) return B200Q_ERR_BAD_ARGUMENT;
@@ -606,7 +607,19 @@ int b200q_add_rms_norm_cast(const b200q_norm_args* a) {
     return B200Q_ERR_UNSUPPORTED;
   if (a->dim == 0 && !a->scale_inv) return B200Q_OK;
   if (a->residual && !rows_apart(a->residual, a->residual_stride, a->x, a->x_stride, a->x_dtype, a->tokens, a->dim)) return B200Q_ERR_BAD_ARGUMENT;
+  return B200Q_OK;
+}
+
+int b200q_add_rms_norm_cast(const b200q_norm_args* a) {
+  const int rc = check_norm(a);
+  if (rc || norm_writes_nothing(a)) return rc;
   return add_rms_norm_cast_impl(*a, static_cast<cudaStream_t>(a->stream));
+}
+
+int b200q_selftest_norm_wait_timeout(const b200q_norm_args* a) {
+  if (int rc = check_norm(a)) return rc;
+  if (norm_writes_nothing(a)) return B200Q_ERR_BAD_ARGUMENT;
+  return norm_selftest_impl(*a, static_cast<cudaStream_t>(a->stream));
 }
 
 size_t b200q_lora_workspace_bytes(int64_t tokens, int64_t k, int64_t n, int64_t rank, int64_t adapters) {

@@ -11,6 +11,7 @@ constexpr int64_t kLoraMaxRank = 256, kLoraMaxAdapters = 2048;
 constexpr int kMoeMaxExperts = 512, kMoeMaxTopK = 16;
 
 int add_rms_norm_cast_impl(const b200q_norm_args& a, cudaStream_t st);
+int norm_selftest_impl(const b200q_norm_args& a, cudaStream_t st);
 size_t lora_workspace_bytes_impl(int64_t tokens, int64_t k, int64_t n, int64_t rank, int64_t adapters);
 int lora_add_impl(const b200q_lora_args& a, cudaStream_t st);
 int lora_selftest_impl(const b200q_lora_args& a, int lost, cudaStream_t st);

@@ -367,6 +367,7 @@ static int norm_launch(const b200q_norm_args& a, float inv_dim, cudaStream_t st)
 // behind it; what that brings of its neighbours is masked out, and behind the last row nothing is fetched: its end is read value by value.  8000 x 8189: 180 us, bound by
 // instructions (masks, and weights that have to be moved into place), where value by value it was 288; 4096 x 13433: 114 us.
 constexpr int kNormErrCopy = 811;  // status code: a copy of a row did not arrive
+constexpr uint32_t kNormTestPolls = 1u << 14;  // of the self-test: some ten milliseconds
 constexpr int kNormRingBytes = 216 * 1024;  // of an SM
 
 __device__ __forceinline__ void norm_bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
@@ -378,7 +379,7 @@ __host__ __device__ constexpr int64_t norm_slot_row(int64_t dim, int form) {  //
   return (dim + (form == kNormShifted ? 7 : 0) + 7) / 8 * 8 * (int64_t)sizeof(T);  // (all vectors that begin in the row end in its place)
 }
 
-template <typename T, int FORM, int THREADS, int VECS, int BLOCKS>
+template <typename T, int FORM, int THREADS, int VECS, int BLOCKS, bool TEST>  // TEST: short waits, and block 0's first row is never copied
 __global__ void __launch_bounds__(THREADS, BLOCKS) norm_ring_kernel(const b200q_norm_args a, float inv_dim, int depth, int* status) {
   constexpr int kWarps = THREADS / 32, kMostDepth = 8;
   extern __shared__ __align__(128) uint8_t s_ring[];  // [depth] rows of x, with that of residual behind it
@@ -406,6 +407,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) norm_ring_kernel(const b200q_
     const uint32_t bytes = bytes_of(t);
     const int64_t back = shift_of(t);
     ptx::mbar_arrive_expect_tx(bars + 8 * slot, a.residual ? 2 * bytes : bytes);
+    if (TEST && t == 0) return;
     norm_bulk_copy(ring + slot * slot_bytes, static_cast<const T*>(a.x) + (t * a.x_stride - back), bytes, bars + 8 * slot);
     if (a.residual)
       norm_bulk_copy(ring + slot * slot_bytes + row, static_cast<const T*>(a.residual) + (t * a.residual_stride - back), bytes, bars + 8 * slot);
@@ -415,7 +417,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) norm_ring_kernel(const b200q_
   int slot = 0, turn = 0;
   uint32_t phase = 0;
   for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x, turn ^= 1) {
-    const bool here = ptx::mbar_wait(bars + 8 * slot, phase, &s_abort, status, kNormErrCopy);
+    const bool here = ptx::mbar_wait(bars + 8 * slot, phase, &s_abort, status, kNormErrCopy, 0, TEST ? kNormTestPolls : ptx::kWaitLimit);
     const T* x = reinterpret_cast<const T*>(s_ring + slot * slot_bytes);
     T* residual = static_cast<T*>(a.residual) + t * a.residual_stride;
     const int shift = shift_of(t);
@@ -470,7 +472,9 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) norm_ring_kernel(const b200q_
     for (int o = 16; o > 0; o >>= 1) s = norm_join(s, {__shfl_xor_sync(0xFFFFFFFFu, s.squares, o), __shfl_xor_sync(0xFFFFFFFFu, s.top, o)});
     if ((tid & 31) == 0) s_warp[turn][tid >> 5] = s;
     __syncthreads();  // (and the slot has been read by all)
-    if (s_abort) {  // a copy is missing: nothing more is written, and the copies in flight are waited for, as far as they come
+    // A copy is missing: nothing more is written, and the copies in flight are waited for, as far as they come.  (All threads see the same: one that waits for the next row in vain
+    // says so long after the others have looked.  A flag for each of two rows, or a barrier that carries it, cost registers: rows of odd lengths 180 -> 191 to 194 us.)
+    if (s_abort) {
       if (tid == 0)
         for (int i = 0; i < depth && t + (int64_t)i * gridDim.x < a.tokens; ++i) {
           const int at = slot + i < depth ? slot + i : slot + i - depth;
@@ -511,9 +515,9 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) norm_ring_kernel(const b200q_
   }
 }
 
-template <typename T, int FORM, int THREADS, int VECS, int BLOCKS>
+template <typename T, int FORM, int THREADS, int VECS, int BLOCKS, bool TEST = false>
 static int norm_launch_ring(const b200q_norm_args& a, float inv_dim, cudaStream_t st) {
-  auto kernel = norm_ring_kernel<T, FORM, THREADS, VECS, BLOCKS>;
+  auto kernel = norm_ring_kernel<T, FORM, THREADS, VECS, BLOCKS, TEST>;
   constexpr int kMost = kNormRingBytes / BLOCKS / 1024 * 1024;
   static std::atomic<int> ready[kMaxDevices];
   const int dev = current_device_index();
@@ -572,6 +576,17 @@ static int norm_launch_form(const b200q_norm_args& a, float inv_dim, cudaStream_
   return a.tokens <= kNumSMs ? norm_launch_few<T, FORM>(a, inv_dim, st) : norm_launch_many<T, FORM>(a, inv_dim, st);
 }
 
+static NormForm norm_form(const b200q_norm_args& a) {
+  bool aligned = true;
+  for (const void* p : {a.x, static_cast<const void*>(a.residual), a.weight, static_cast<const void*>(a.out), static_cast<const void*>(a.kept)})
+    aligned = aligned && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+  const int64_t strides[2] = {a.x_stride, a.residual ? a.residual_stride : a.x_stride};
+  const bool one = a.tokens == 1;  // (no stride is used)
+  if (aligned && a.dim % 8 == 0 && (one || (strides[0] % 8 == 0 && strides[1] % 8 == 0))) return kNormEven;
+  if (aligned && (one || ((strides[0] - a.dim) % 8 == 0 && (strides[1] - a.dim) % 8 == 0))) return kNormShifted;
+  return kNormLoose;
+}
+
 template <typename T>
 static int norm_launch_type(const b200q_norm_args& a, float inv_dim, cudaStream_t st) {
   if (a.dim > 32768 || (a.dim > 32760 && a.dim % 8)) {
@@ -580,19 +595,21 @@ static int norm_launch_type(const b200q_norm_args& a, float inv_dim, cudaStream_
     B200Q_LAUNCH_CHECK();
     return B200Q_OK;
   }
-  bool aligned = true;
-  for (const void* p : {a.x, static_cast<const void*>(a.residual), a.weight, static_cast<const void*>(a.out), static_cast<const void*>(a.kept)})
-    aligned = aligned && reinterpret_cast<uintptr_t>(p) % 16 == 0;
-  const int64_t strides[2] = {a.x_stride, a.residual ? a.residual_stride : a.x_stride};
-  const bool one = a.tokens == 1;  // (no stride is used)
-  if (aligned && a.dim % 8 == 0 && (one || (strides[0] % 8 == 0 && strides[1] % 8 == 0))) return norm_launch_form<T, kNormEven>(a, inv_dim, st);
-  if (aligned && (one || ((strides[0] - a.dim) % 8 == 0 && (strides[1] - a.dim) % 8 == 0))) return norm_launch_form<T, kNormShifted>(a, inv_dim, st);
-  return norm_launch_form<T, kNormLoose>(a, inv_dim, st);
+  switch (norm_form(a)) {
+    case kNormEven: return norm_launch_form<T, kNormEven>(a, inv_dim, st);
+    case kNormShifted: return norm_launch_form<T, kNormShifted>(a, inv_dim, st);
+    default: return norm_launch_form<T, kNormLoose>(a, inv_dim, st);
+  }
 }
 
 int add_rms_norm_cast_impl(const b200q_norm_args& a, cudaStream_t st) {
   const float inv_dim = a.dim ? 1.f / (float)a.dim : 0.f;
   return a.x_dtype == B200Q_BF16 ? norm_launch_type<__nv_bfloat16>(a, inv_dim, st) : norm_launch_type<float>(a, inv_dim, st);
+}
+
+int norm_selftest_impl(const b200q_norm_args& a, cudaStream_t st) {
+  if (a.x_dtype != B200Q_BF16 || a.dim <= 4096 || a.dim > 8192 || a.tokens <= kNumSMs || norm_form(a) != kNormEven) return B200Q_ERR_UNSUPPORTED;
+  return norm_launch_ring<__nv_bfloat16, kNormEven, 512, 2, 2, true>(a, 1.f / (float)a.dim, st);
 }
 
 }  // namespace b200q

@@ -648,6 +648,9 @@ typedef struct b200q_norm_args {
 } b200q_norm_args;
 
 int b200q_add_rms_norm_cast(const b200q_norm_args* args);
+/* Self-test of that: the same call (more than 148 tokens of 4104 to 8192 bf16 values, rows on boundaries of eight, else B200Q_ERR_UNSUPPORTED) with short waits, in which the copy of the
+ * first row never comes.  The kernel ends by itself; the GPU does not fault. */
+int b200q_selftest_norm_wait_timeout(const b200q_norm_args* args);
 
 /*
  * lora_add: low-rank adapters of many requests beside a product that they share.  Per token t with i = adapter[t] in [0, adapters)

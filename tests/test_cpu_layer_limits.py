@@ -46,3 +46,21 @@ def test_lora_selftest_refuses(kw, rc):
 
 def test_lora_selftest_refuses_nothing():
     assert abi.lib.b200q_selftest_lora_wait_timeout(ctypes.POINTER(abi.LoraArgs)(), 0) == BAD
+
+
+def _norm_selftest(**kw):
+    a = abi.NormArgs()
+    a.x, a.weight, a.out = AT, AT, AT
+    a.x_dtype, a.weight_dtype, a.out_dtype = abi.BF16, abi.BF16, abi.E4M3
+    a.tokens, a.dim, a.x_stride, a.residual_stride = 149, 8192, 8192, 8192
+    return _call(abi.lib.b200q_selftest_norm_wait_timeout, a, kw)
+
+
+@pytest.mark.parametrize("kw,rc", [(dict(tokens=-1), BAD), (dict(tokens=0), BAD), (dict(dim=0), BAD), (dict(x=None), BAD), (dict(tokens=148), UNSUPPORTED), (dict(dim=4096), UNSUPPORTED),
+                                   (dict(dim=8200, x_stride=8200), UNSUPPORTED), (dict(dim=8191, x_stride=8191), UNSUPPORTED), (dict(x_dtype=abi.F32), UNSUPPORTED), (dict(x=AT + 8), UNSUPPORTED)])
+def test_norm_selftest_refuses(kw, rc):
+    assert _norm_selftest(**kw) == rc
+
+
+def test_norm_selftest_refuses_nothing():
+    assert abi.lib.b200q_selftest_norm_wait_timeout(ctypes.POINTER(abi.NormArgs)()) == BAD

@@ -87,3 +87,31 @@ def test_lora_that_waits_in_vain(tokens, k, n, rank, adapters, lost):
             assert torch.equal(missed.all(-1), rows)
         assert torch.equal(_run_lora(*c).cpu(), want)
     assert b200_hpu_ops.device_status() == 0
+
+
+@pytest.mark.parametrize("tokens,dim,residual", [(149, 4104, True), (1300, 8192, True), (1300, 5000, False)])
+def test_norm_that_waits_in_vain(tokens, dim, residual):
+    """The first row never comes: the wait runs out (no GPU fault), the status says so, that row and those behind it of its block are not written, the others have an
+    undisturbed call's bytes, and the next call is as it should be."""
+    import b200_hpu_ops
+    from b200_hpu_ops import abi
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    x, r = (torch.randn(tokens, dim, generator=g, device="cuda").to(BF16) for _ in range(2))
+    run = lambda res: torch.ops.b200q.add_rms_norm_cast(x, res if residual else None, None, EPS, E4M3, None, True)  # noqa: E731
+    after = r.clone()
+    want = [*run(after), after]
+    mine = torch.zeros(tokens, dtype=torch.bool, device="cuda")
+    mine[::2 * 148] = True  # block 0's rows
+    for _ in range(2):
+        got = [torch.full((tokens, dim), 2.0, device="cuda").to(E4M3), torch.full((tokens, 1), 2.0, device="cuda"), torch.full((tokens, dim), 2.0, device="cuda", dtype=BF16), r.clone()]
+        before = [t.clone() for t in got]
+        a = abi.NormArgs(x=x.data_ptr(), x_dtype=abi.BF16, tokens=tokens, dim=dim, x_stride=dim, residual=got[3].data_ptr() if residual else None, residual_stride=dim, eps=EPS,
+                         out=got[0].data_ptr(), out_dtype=abi.E4M3, scale_inv=got[1].data_ptr(), kept=got[2].data_ptr(), stream=abi.stream_ptr())
+        abi.check(abi.lib.b200q_selftest_norm_wait_timeout(C.byref(a)))
+        assert b200_hpu_ops.device_status() == 811
+        for t, b, w in zip(got, before, want):
+            t, b, w = t.float(), b.float(), w.float()
+            assert torch.equal(t[mine], b[mine]) and torch.equal(t[~mine], w[~mine])
+        after = r.clone()
+        assert all(torch.equal(t.float(), w.float()) for t, w in zip([*run(after), after], want))
+    assert b200_hpu_ops.device_status() == 0
