@@ -612,9 +612,11 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
     return unit;
   };
 
-  // Before a CTA ends its copies in flight are waited for, as far as they come.  (Where no wait has run out they have been multiplied, or will be next.)
+  // a role's place in the ring, and its copies so far
+  uint32_t stage = 0, phase = 0;
   int made = 0;
-  auto drain = [&](uint32_t bars, uint32_t stage, uint32_t phase) {
+  // where a wait has run out: the copies in flight are waited for, as far as they come
+  auto drain = [&](uint32_t bars) {
     for (int i = 0; i < min(made, kStages); ++i) {
       phase ^= stage == 0;
       stage = stage == 0 ? kStages - 1 : stage - 1;
@@ -715,7 +717,6 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
     // (a CTA did not come: nothing is in flight, and nobody goes on)
   } else if (warp == 0) {
     // ------------------------------------------------------------ weights
-    uint32_t stage = 0, phase = 0;
     auto publish = [&](int u) {
       ok = ok && ptx::mbar_wait_uniform(bar_taken + 8 * turn, turn_phase ^ 1, &s_abort, w.status, kMoeErrWeights, kLimit);
       if (!ok) return;
@@ -770,10 +771,8 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
     };
     stream(std::integral_constant<int, 0>());
     if (ok) stream(std::integral_constant<int, 1>());
-    drain(bar_weights, stage, phase);
   } else if (warp == 1) {
     // ------------------------------------------------------------ products
-    uint32_t stage = 0, phase = 0;
     int pieces = 0;
     const uint64_t a0 = ptx::smem_desc_k_sw128(ring), b0 = ptx::smem_desc_k_sw128(ring + 2 * kMoeSubBytes);
     for (int product = 0; product < 2 && ok; ++product) {
@@ -811,13 +810,8 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
         }
       }
     }
-    // nor do products outlive the tensor memory and the ring
-    if (ptx::elect_one()) ptx::umma_commit(bar_last);
-    __syncwarp();
-    for (int k = 0; k < 4096 && !ptx::mbar_try_wait(bar_last, 0); ++k) __nanosleep(64);
   } else if (warp == 2) {
     // ------------------------------------------------------------ terms
-    uint32_t stage = 0, phase = 0;
     auto stream = [&](auto which) {
       constexpr int product = decltype(which)::value, terms = product ? Tile::kDownTerms : Tile::kUpTerms;
       const MoeUnits list = units_of(product);
@@ -864,7 +858,6 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
     };
     stream(std::integral_constant<int, 0>());
     if (ok) stream(std::integral_constant<int, 1>());
-    drain(bar_tokens, stage, phase);
   } else if (warp < 7) {
     // ------------------------------------------------------------ sums of cut tiles, terms of h
     const int row = tid - 96;
@@ -1000,6 +993,15 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
   __syncwarp();
   ptx::tc_fence_before();
   __syncthreads();
+  if (s_abort) {  // (a role may have been done before another's wait ran out)
+    if (warp == 0) drain(bar_weights);
+    if (warp == 2) drain(bar_tokens);
+    if (warp == 1) {  // nor do products outlive the tensor memory and the ring
+      if (ptx::elect_one()) ptx::umma_commit(bar_last);
+      __syncwarp();
+      for (int k = 0; k < 4096 && !ptx::mbar_try_wait(bar_last, 0); ++k) __nanosleep(64);
+    }
+  }
   if (warp == 1) ptx::tmem_dealloc(tmem, Tile::kTmem);
 }
 
