@@ -510,6 +510,9 @@ __device__ __forceinline__ void lora_store16(Y* p, const uint4& w) {
   }
 }
 
+// All terms but the last stay finite, so that the rest of an infinity is that infinity (and of a NaN a NaN), not inf - inf, and what lies between the ends of bf16 and fp32 has a rest.
+__device__ __forceinline__ float lora_within_bf16(float v) { return fminf(fmaxf(v, -3.3895313892515355e38f), 3.3895313892515355e38f); }
+
 template <typename Y, int TILE, bool WHOLE, bool TEST>  // TEST: short waits, and the first copy of block 0 is never made
 __global__ void __launch_bounds__(lora_up_threads(TILE), lora_up_ctas(sizeof(Y) == 4, TILE)) lora_up_kernel(const __grid_constant__ CUtensorMap map_b, const b200q_lora_args a, const LoraPlan p, const LoraUpShape d) {
   constexpr int kTerms = sizeof(Y) == 4 ? 3 : 2, kStage = 128 * 128, kWarps = lora_result_warps(TILE), kHalf = TILE / (kWarps / 4);
@@ -679,7 +682,7 @@ __global__ void __launch_bounds__(lora_up_threads(TILE), lora_up_ctas(sizeof(Y) 
             uint32_t w[2];
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              w[c] = pack_bf16x2(v[e][2 * c], v[e][2 * c + 1]);
+              w[c] = t + 1 < kTerms ? pack_bf16x2(lora_within_bf16(v[e][2 * c]), lora_within_bf16(v[e][2 * c + 1])) : pack_bf16x2(v[e][2 * c], v[e][2 * c + 1]);
               v[e][2 * c] -= __uint_as_float(w[c] << 16);
               v[e][2 * c + 1] -= __uint_as_float(w[c] & 0xFFFF0000u);
             }

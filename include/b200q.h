@@ -656,7 +656,8 @@ int b200q_selftest_norm_wait_timeout(const b200q_norm_args* args);
  * lora_add: low-rank adapters of many requests beside a product that they share.  Per token t with i = adapter[t] in [0, adapters)
  *   y[t] = T(y[t] + scales[i] * b[i] (a[i] x[t]))
  * and nothing for the others, whose rows of y are neither read nor written.  a x is summed in fp32 and meets b as three bf16 terms (24 bits) where y
- * is fp32 and as two (16 bits) where it is bf16; that product is summed in fp32, and rounded once with y.  A scaled a x beyond the end of bf16 makes the token's y NaN.
+ * is fp32 and as two (16 bits) where it is bf16; that product is summed in fp32, and rounded once with y.  An infinity or a NaN in x or a gives what these products and sums make of it; an infinity in b makes its column of the
+ * adapter's tokens infinite or NaN.
  *
  * x             bf16 [tokens][k];  y: F32 / BF16 [tokens][n], row stride >= n; row strides in elements, values contiguous
  * a             bf16 [adapters][rank][k];  b: bf16 [adapters][n][rank]; strides of adapter and row in elements, values contiguous

@@ -115,3 +115,28 @@ def test_norm_that_waits_in_vain(tokens, dim, residual):
         after = r.clone()
         assert all(torch.equal(t.float(), w.float()) for t, w in zip([*run(after), after], want))
     assert b200_hpu_ops.device_status() == 0
+
+
+# ----------------------------------------------------------------------------- infinities
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("tokens,k,n,rank", [(9, 64, 72, 16), (200, 264, 136, 72), (9, 60, 71, 12), (200, 61, 72, 3)])
+def test_lora_infinities(tokens, k, n, rank, dtype):
+    """Infinities of x and a, by tensor-core kernels (the first two sizes) and plain ones: what products and sums make of them, in either; and a x behind the end of bf16, but not of fp32."""
+    y, x, a, b, which, scales = _lora_case(tokens, k, n, rank, 3, dtype, which=torch.arange(tokens) % 3)
+    a, b = a.abs() + 2.0 ** -10, b.abs() + 2.0 ** -10  # (no zeros)
+    a[2, 1, 5] = math.inf   # one rank of an adapter
+    b[0, 7] = 0             # a column that an infinity meets with zeros
+    x[:, 5] = x[:, 5].abs() + 1
+    x[0, 3], x[3, k - 1], x[4, 3], x[6, 3], x[6, 4] = math.inf, -math.inf, math.inf, math.inf, -math.inf
+    x[7] = 0
+    x[7, 0] = 3.3e38
+    a[1, :, 0], b[1, :, :] = 1.0234375, 2.0 ** -12  # 3.377e38, and with the scale below as much as fp32 holds
+    scales[1] = 1.0058
+    want, size, live = O.lora_add(y, x, a, b, which, scales)
+    assert bool(want[0, :7].isposinf().all()) and bool(want[0, 7].isnan()) and bool(want[3, 0].isneginf()) and bool(want[4].isposinf().all()) and bool(want[6].isnan().all())
+    assert bool(want[2].isposinf().all()) and 3.3895313892515355e38 < float((a[1].double() @ x[7].double() * scales[1]).max()) < 3.4e38 and bool(want[7].isfinite().all())
+    got = _run_lora(y, x, a, b, which, scales).cpu().float()
+    finite = want.isfinite()
+    assert torch.equal(got[~finite].nan_to_num(nan=7.0), want[~finite].float().nan_to_num(nan=7.0))
+    tol = (HALF_STEP[dtype] * (1 + 2.0 ** -10)) * want.abs() + size * (((k + rank) / 16 + 32) * 2.0 ** -23 + 2.0 ** -16) + FLOOR[dtype]
+    _close(torch.where(finite, got, 0.0), torch.where(finite, want, 0.0), torch.where(finite, tol, 0.0))
