@@ -28,6 +28,8 @@ __device__ __forceinline__ float moe_x(const b200q_moe_args& a, int64_t t, int64
   return __bfloat162float(static_cast<const __nv_bfloat16*>(a.x)[t * a.x_stride + i]);
 }
 __device__ __forceinline__ float moe_silu(float g) { return g / (1.f + expf(-g)); }
+// An infinite value of h has no terms (e4m3 has no infinity, and inf - inf is no rest): NaN in all kernels, so that layouts do not differ.
+__device__ __forceinline__ float moe_finite(float h) { return fabsf(h) <= 3.402823466e38f ? h : __int_as_float(0x7FC00000); }
 
 // ---------------------------------------------------------------------------- router
 // Sums in fp64: neighbours in the order of the experts may be closer than the rounding of a sum in fp32, and another expert is another answer.
@@ -289,7 +291,7 @@ __global__ void __launch_bounds__(kMoeThreads) moe_plain_up_kernel(const b200q_m
     g *= a.gate_up_scale[gate];
     u *= a.gate_up_scale[up];
   }
-  if (lane == 0) hidden[at] = moe_silu(g) * u;
+  if (lane == 0) hidden[at] = moe_finite(moe_silu(g) * u);
 }
 __global__ void __launch_bounds__(kMoeThreads) moe_plain_down_kernel(const b200q_moe_args a, const float* hidden, float* outputs) {
   pdl_enter();
@@ -642,8 +644,7 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
       float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
-        v[c] *= factor;
-        if (!(fabsf(v[c]) <= 3.4e38f)) v[c] = __int_as_float(0x7FC00000);  // (e4m3 has no infinity, and would make it 448)
+        v[c] = moe_finite(v[c] * factor);
       }
       uint2 term[3];
       moe_terms_fp8<3>(v, term);
@@ -675,9 +676,11 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
         if (lane == 0) atomicMax(w.h_top + slot, top);
       } else if (r < a.inner) {
         __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(w.h_terms) + (int64_t)slot * a.inner + r;
-        const __nv_bfloat16 hi = __float2bfloat16_rn(h);
+        // (the first term stays within bf16, so that what lies between the ends of bf16 and fp32 has a rest)
+        const float v = moe_finite(h);
+        const __nv_bfloat16 hi = __float2bfloat16_rn(fminf(fmaxf(v, -3.3895313892515355e38f), 3.3895313892515355e38f));
         to[0] = hi;
-        to[(int64_t)w.slots * a.inner] = __float2bfloat16_rn(h - __bfloat162float(hi));
+        to[(int64_t)w.slots * a.inner] = __float2bfloat16_rn(v - __bfloat162float(hi));
       }
     } else {
       const int64_t r = unit.row * 256 + row;

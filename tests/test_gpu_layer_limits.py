@@ -140,3 +140,25 @@ def test_lora_infinities(tokens, k, n, rank, dtype):
     assert torch.equal(got[~finite].nan_to_num(nan=7.0), want[~finite].float().nan_to_num(nan=7.0))
     tol = (HALF_STEP[dtype] * (1 + 2.0 ** -10)) * want.abs() + size * (((k + rank) / 16 + 32) * 2.0 ** -23 + 2.0 ** -16) + FLOOR[dtype]
     _close(torch.where(finite, got, 0.0), torch.where(finite, want, 0.0), torch.where(finite, tol, 0.0))
+
+
+@pytest.mark.parametrize("weights", [E4M3, BF16])
+@pytest.mark.parametrize("hidden,inner", [(64, 32), (272, 160), (60, 33)])
+@pytest.mark.parametrize("tokens", [6, 12])
+def test_moe_h_at_the_end_of_fp32(tokens, hidden, inner, weights):
+    """An h of 3.397e38, which bf16 has no finite value for, and one beyond fp32: that makes its token NaN, by tensor-core kernels (the first two sizes) and plain ones alike."""
+    x, r, gu, down, s1, s2 = _moe_case(tokens, hidden, inner, 2, weights)
+    gu, down = torch.zeros(gu.shape), torch.full(down.shape, 2.0 ** -6).to(weights)
+    gu[:, 1, 0] = gu[:, inner + 1, 0] = 1.0  # of unit 1 alone: g = 8 x[0], u = 31.95 x[0]
+    s1, s2 = torch.ones_like(s1), torch.full_like(s2, 2.0 ** -13)
+    s1[:, 1], s1[:, inner + 1] = 8.0, 31.95
+    x[:, 0] = x[:, 0].abs() + 1
+    x[2, 0], x[4, 0] = 2.0 ** 60, 2.0 ** 64
+    assert 3.3895313892515355e38 < 2.0 ** 123 * float(s1[0, inner + 1]) < 3.402e38
+    case = (x, r, gu.to(weights), down, s1, s2)
+    w, i = O.moe_route(x, r, 1, True)
+    want, bound = O.moe_experts(x, w, i, *case[2:], rel_sum=40 * 2.0 ** -23, rel_hidden=2.0 ** -12, abs_hidden=2.0 ** -26)
+    want[4], bound[4] = math.nan, 0
+    out, weights_of, ids = _run_moe(case, 1)
+    assert torch.equal(ids.cpu(), i) and bool((weights_of == 1).all())
+    _close(out.float(), want, HALF_STEP[BF16] * (1 + 2.0 ** -10) * want.abs() + bound + FLOOR[BF16])
