@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(kMoeThreads) moe_sum_kernel(const b200q_moe_ar
 // ---------------------------------------------------------------------------- tensor cores
 // Bound by the weights of the chosen experts, each read once: a product of a weight tile with the few tokens of an expert has the weights as the
 // 128 rows of tcgen05.mma and the tokens as its columns.  What 8-bit weights meet has to be 8 bits too, so that a value becomes several e4m3
-// terms, a column each, scaled by powers of two: bf16 values of a token two terms (8 bits, which is all they have), h three (12 bits).  The
+// terms, a column each, scaled by powers of two: bf16 values of a token two terms (8 bits, which is all they have), h three (12 bits; for an fp32 output six, 24 bits).  The
 // weights then go from global memory to the tensor core as they are, by TMA alone; f16 operands would want every weight converted in
 // registers first.
 //
@@ -339,13 +339,14 @@ __global__ void __launch_bounds__(kMoeThreads) moe_sum_kernel(const b200q_moe_ar
 constexpr int kMoeWarps = 11;
 constexpr int kMoeErrWeights = 821, kMoeErrTokens = 822, kMoeErrMma = 823, kMoeErrResults = 824, kMoeErrGrid = 825;  // status codes: a wait ran out
 constexpr int kMoeGroupTokens = 32;     // of an expert, at a time
+constexpr int kMoeFineTokens = 16;      // the same for an fp32 output of 8-bit weights, whose six terms are that many columns more
 constexpr int kMoeSubBytes = 128 * 128;  // a weight tile: 128 rows of 128 bytes; a step has two (gate and up, or 256 outputs)
 constexpr int kMoeMostDim = 65536;
 constexpr uint32_t kMoeGridPolls = 1u << 21;  // some two seconds
 constexpr uint32_t kMoeTestPolls = 1u << 14;  // of the self-test: some ten milliseconds
 
 constexpr int kMoeCutTiles = kNumSMs * 5 / 4 + 1, kMoeMostParts = 8, kMoeSumTokens = 4;
-constexpr int kMoeMostGroups = kMoeMaxExperts + (int)kMoeChunk * kMoeMaxTopK / kMoeGroupTokens;
+constexpr int kMoeMostGroups = kMoeMaxExperts + (int)kMoeChunk * kMoeMaxTopK / kMoeFineTokens;
 struct MoeControl {  // cleared by the router's kernel
   uint32_t chosen, done, next[2];
   uint32_t parts[2][kMoeCutTiles];  // of a cut tile that are there, four warps each
@@ -353,17 +354,21 @@ struct MoeControl {  // cleared by the router's kernel
   uint32_t terms[kMoeMostGroups];   // slots of a group whose terms are there, four warps each
 };
 
-template <bool FP8, int MAXN>
+// FINE: the output is fp32.  Then h has as many terms as hold its 24 bits, and no more than 256 products are added inside the tensor core, whose additions drop what does not fit 24
+// bits of the sum so far (lora.cu has the figures): the results' warps add those sums in fp32.  Otherwise both would be far below the output's rounding to bf16.
+template <bool FP8, int MAXN, bool FINE>
 struct MoeTile {
-  static constexpr int kUpTerms = FP8 ? 2 : 1, kDownTerms = FP8 ? 3 : 2;
+  static constexpr int kUpTerms = FP8 ? 2 : 1, kDownTerms = FINE ? (FP8 ? 6 : 3) : FP8 ? 3 : 2;
   static constexpr int kCols = (kDownTerms * MAXN + 15) / 16 * 16;  // columns of an accumulator
   static constexpr int kTokenBytes = kCols * 128;
   static constexpr int kStage = 2 * kMoeSubBytes + kTokenBytes;
   static constexpr int kStages = 200 * 1024 / kStage < 5 ? 200 * 1024 / kStage : 5;
   static constexpr int kTmem = 4 * kCols <= 64 ? 64 : 4 * kCols <= 128 ? 128 : 4 * kCols <= 256 ? 256 : 512;  // two accumulators of two tiles
   static constexpr int kStep = FP8 ? 128 : 64;  // values of K in a step
+  static constexpr int kSub = 256 / kStep;      // steps that are added inside the tensor core where FINE
   static constexpr int kPart = 2 * MAXN * 128;  // floats of a partial result: [tile][token][row]
   static_assert(kTokenBytes % 1024 == 0, "tiles lie on boundaries of the swizzle");
+  static_assert(4 * kCols <= 512, "two accumulators of two tiles are in tensor memory");
 };
 
 struct MoeFused {
@@ -371,7 +376,7 @@ struct MoeFused {
   const uint32_t* x_top;   // bits of max |x| per token
   uint32_t* h_top;         // bits of max |h| per slot
   float *hidden, *outputs;  // [slots][inner] (8-bit weights), [slots][hidden]: slots in the order of experts
-  uint8_t* h_terms;        // [terms][slots][inner]
+  uint8_t* h_terms;        // [terms][slots][inner], of a byte or two
   int slots;               // of that
   float* parts;            // [products][cut tiles][parts][kPart]
   MoeControl* control;
@@ -405,7 +410,7 @@ __device__ __forceinline__ void moe_fence_async() { asm volatile("fence.proxy.as
 // integers is a hundred cycles, and some ten of them stood before the first copy.)
 __device__ __forceinline__ int moe_divide(int x, float inverse) { return (int)(((float)x + 0.5f) * inverse); }
 
-// The units of a product: `whole` tiles, then the parts of the others.  Fewer than 2^22 of them: at most 640 groups, of 512 tiles each.
+// The units of a product: `whole` tiles, then the parts of the others.  Fewer than 2^22 of them: at most 768 groups, of 512 tiles each.
 // Cut are the tiles that do not come out even, and a quarter of a round of all CTAs at least; but none of up to 32 steps (4096 bytes of a row), because fewer CTAs draw more each and
 // the sums come on top, and none where so many CTAs have one whole tile that they draw all that the memory gives.  us with cuts above 8 steps, above 32, and none at all: 64 tokens
 // of 32 experts 2048 x 688 66, 60, 60; 16 tokens of 64 experts 2048 x 1408 94, 86, 86; 29 tokens of 128 experts 4096 x 1792 383, 378, 377; 5 tokens of 8 experts 4096 x 4096 in
@@ -447,15 +452,15 @@ struct MoeUnit {
   }
 };
 
-template <bool FP8, int MAXN, bool TEST>  // TEST: short waits, one of them in vain
+template <bool FP8, int MAXN, bool FINE, bool TEST>  // TEST: short waits, one of them in vain
 __global__ void __launch_bounds__(32 * kMoeWarps, 1)
     moe_fused_kernel(const __grid_constant__ CUtensorMap map_up, const __grid_constant__ CUtensorMap map_down, const __grid_constant__ CUtensorMap map_x,
                      const __grid_constant__ CUtensorMap map_h, const b200q_moe_args a, int64_t first, const MoeFused w) {
-  using Tile = MoeTile<FP8, MAXN>;
+  using Tile = MoeTile<FP8, MAXN, FINE>;
   constexpr int kStages = Tile::kStages, kSteps = Tile::kStep;
   constexpr uint32_t kLimit = TEST ? kMoeTestPolls : ptx::kWaitLimit, kPolls = TEST ? kMoeTestPolls : kMoeGridPolls;
   constexpr int kMostSlots = MAXN == 8 ? 8 * kMoeMaxTopK : (int)kMoeChunk * kMoeMaxTopK;
-  constexpr int kMostGroups = MAXN == 8 ? 8 * kMoeMaxTopK : kMoeMaxExperts + kMostSlots / kMoeGroupTokens;
+  constexpr int kMostGroups = MAXN == 8 ? 8 * kMoeMaxTopK : kMoeMaxExperts + kMostSlots / MAXN;
   constexpr int kMaskWords = MAXN == 8 ? 1 : (int)kMoeChunk / 32;
   extern __shared__ __align__(1024) uint8_t s_raw[];
   uint8_t* const s_ring = s_raw + (0u - ptx::smem_u32(s_raw) & 1023u);
@@ -646,10 +651,10 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
       for (int c = 0; c < 8; ++c) {
         v[c] = moe_finite(v[c] * factor);
       }
-      uint2 term[3];
-      moe_terms_fp8<3>(v, term);
+      uint2 term[Tile::kDownTerms];
+      moe_terms_fp8<Tile::kDownTerms>(v, term);
 #pragma unroll
-      for (int c = 0; c < 3; ++c) *reinterpret_cast<uint2*>(w.h_terms + ((int64_t)c * w.slots + slot) * a.inner + i) = term[c];
+      for (int c = 0; c < Tile::kDownTerms; ++c) *reinterpret_cast<uint2*>(w.h_terms + ((int64_t)c * w.slots + slot) * a.inner + i) = term[c];
     }
     moe_fence_async();
     __syncwarp();
@@ -676,11 +681,14 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
         if (lane == 0) atomicMax(w.h_top + slot, top);
       } else if (r < a.inner) {
         __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(w.h_terms) + (int64_t)slot * a.inner + r;
-        // (the first term stays within bf16, so that what lies between the ends of bf16 and fp32 has a rest)
-        const float v = moe_finite(h);
-        const __nv_bfloat16 hi = __float2bfloat16_rn(fminf(fmaxf(v, -3.3895313892515355e38f), 3.3895313892515355e38f));
-        to[0] = hi;
-        to[(int64_t)w.slots * a.inner] = __float2bfloat16_rn(v - __bfloat162float(hi));
+        // (all terms but the last stay within bf16, so that what lies between the ends of bf16 and fp32 has a rest)
+        float v = moe_finite(h);
+#pragma unroll
+        for (int t = 0; t < Tile::kDownTerms; ++t) {
+          const __nv_bfloat16 term = __float2bfloat16_rn(t + 1 < Tile::kDownTerms ? fminf(fmaxf(v, -3.3895313892515355e38f), 3.3895313892515355e38f) : v);
+          to[t * (int64_t)w.slots * a.inner] = term;
+          v -= __bfloat162float(term);
+        }
       }
     } else {
       const int64_t r = unit.row * 256 + row;
@@ -781,17 +789,22 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
     for (int product = 0; product < 2 && ok; ++product) {
       const int terms = product ? Tile::kDownTerms : Tile::kUpTerms;
       const MoeUnits list = units_of(product);
-      for (; ok; ++pieces) {
+      while (ok) {
         const int u = next_unit(kMoeErrMma);
         if (u < 0) break;
         const MoeUnit unit(list, u);
         const int cols = ((s_group_tokens[unit.group] + 7) / 8 * 8 * terms + 15) / 16 * 16;
         const uint32_t idesc = FP8 ? ptx::umma_idesc(0, 0, 128, cols) : ptx::umma_idesc(1, 1, 128, cols);
-        const uint32_t acc = pieces & 1, d = tmem + acc * 2 * Tile::kCols;
-        ok = ptx::mbar_wait_uniform(bar_free + 8 * acc, ((pieces >> 1) & 1) ^ 1, &s_abort, w.status, kMoeErrMma, kLimit);
-        if (!ok) break;
-        ptx::tc_fence_after();
-        for (int k = unit.k0; k < unit.k1; ++k) {
+        uint32_t acc = 0, d = 0;
+        for (int k = unit.k0, sub_step = 0; k < unit.k1; ++k) {
+          if (sub_step == 0) {
+            acc = pieces & 1;
+            d = tmem + acc * 2 * Tile::kCols;
+            ok = ptx::mbar_wait_uniform(bar_free + 8 * acc, ((pieces >> 1) & 1) ^ 1, &s_abort, w.status, kMoeErrMma, kLimit);
+            if (!ok) break;
+            ++pieces;
+            ptx::tc_fence_after();
+          }
           ok = ptx::mbar_wait2_uniform(bar_weights + 8 * stage, phase, bar_tokens + 8 * stage, phase, &s_abort, w.status, kMoeErrMma, kLimit);
           if (!ok) break;
           ptx::tc_fence_after();
@@ -799,13 +812,14 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
           if (ptx::elect_one()) {
 #pragma unroll
             for (int sub = 0; sub < 2; ++sub) {
-              if (FP8) ptx::umma_f8_x4(d + sub * Tile::kCols, a0 + off + sub * (kMoeSubBytes >> 4), b0 + off, idesc, k != unit.k0, 2, 2);
-              else ptx::umma_f16_x4(d + sub * Tile::kCols, a0 + off + sub * (kMoeSubBytes >> 4), b0 + off, idesc, k != unit.k0, 2, 2);
+              if (FP8) ptx::umma_f8_x4(d + sub * Tile::kCols, a0 + off + sub * (kMoeSubBytes >> 4), b0 + off, idesc, sub_step != 0, 2, 2);
+              else ptx::umma_f16_x4(d + sub * Tile::kCols, a0 + off + sub * (kMoeSubBytes >> 4), b0 + off, idesc, sub_step != 0, 2, 2);
             }
             ptx::umma_commit(bar_empty + 8 * stage);
-            if (k + 1 == unit.k1) ptx::umma_commit(bar_full + 8 * acc);
+            if (k + 1 == unit.k1 || (FINE && sub_step + 1 == Tile::kSub)) ptx::umma_commit(bar_full + 8 * acc);
           }
           __syncwarp();
+          if (++sub_step == Tile::kSub && FINE) sub_step = 0;
           if (++stage == kStages) {
             stage = 0;
             phase ^= 1;
@@ -919,25 +933,30 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
     auto results_of = [&](auto which) {
       constexpr int product = decltype(which)::value, terms = product ? Tile::kDownTerms : Tile::kUpTerms;
       const MoeUnits list = units_of(product);
-      for (;; ++pieces) {
+      for (;;) {
         const int u = next_unit(kMoeErrResults);
         if (u < 0) break;
         const MoeUnit unit(list, u);
         const bool whole = unit.part < 0;
         const int n = s_group_tokens[unit.group];
-        const uint32_t acc = pieces & 1, d = tmem + acc * 2 * Tile::kCols + lane_base;
         float scale[2], backs = 1.f;
         if (whole) {
           scales_of(which, unit, row, scale);
           if (product == 0) backs = backs_of(which, unit);
         }
         float* part = w.parts + (((int64_t)product * kMoeCutTiles + unit.cut) * kMoeMostParts + unit.part) * Tile::kPart + row;
-        ok = ptx::mbar_wait_uniform(bar_full + 8 * acc, (pieces >> 1) & 1, &s_abort, w.status, kMoeErrResults, kLimit);
-        if (!ok) break;
-        ptx::tc_fence_after();
-        if (whole && product == 1) backs = backs_of(which, unit);  // (h's largest value is known now that it has been multiplied)
-        for (int j0 = 0; j0 < n; j0 += 8) {
-          float v[2][8];
+        // the next sums that are there, in tensor memory at d
+        uint32_t acc, d;
+        auto wait = [&] {
+          acc = pieces & 1;
+          d = tmem + acc * 2 * Tile::kCols + lane_base;
+          ok = ptx::mbar_wait_uniform(bar_full + 8 * acc, (pieces >> 1) & 1, &s_abort, w.status, kMoeErrResults, kLimit);
+          if (!ok) return;
+          ++pieces;
+          ptx::tc_fence_after();
+        };
+        // eight tokens' of them, their terms put together
+        auto get = [&](int j0, float (&v)[2][8]) {
 #pragma unroll
           for (int sub = 0; sub < 2; ++sub) {
             float term[terms][8];
@@ -951,24 +970,66 @@ __global__ void __launch_bounds__(32 * kMoeWarps, 1)
               for (int t = terms - 2; t >= 0; --t) v[sub][i] = term[t][i] + (FP8 ? 1.f / 32.f : 1.f) * v[sub][i];
             }
           }
+        };
+        auto put = [&](int j, float v0, float v1) {
+          if (whole) {
+            finish(which, unit, row, j, v0, v1, scale, backs);
+          } else {
+            __stcg(part + j * 128, v0);
+            __stcg(part + (MAXN + j) * 128, v1);
+          }
+        };
+        auto release = [&] {
+          ptx::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(bar_free + 8 * acc);
+        };
+        if constexpr (FINE) {
+          float sums[MAXN][2] = {};
+          for (int k = unit.k0; k < unit.k1; k += Tile::kSub) {
+            wait();
+            if (!ok) break;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            if (j0 + i >= n) break;
-            if (whole) {
-              finish(which, unit, row, j0 + i, v[0][i], v[1][i], scale, backs);
-            } else {
-              __stcg(part + (j0 + i) * 128, v[0][i]);
-              __stcg(part + (MAXN + j0 + i) * 128, v[1][i]);
+            for (int j0 = 0; j0 < MAXN; j0 += 8) {
+              if (j0 >= n) break;
+              float v[2][8];
+              get(j0, v);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                sums[j0 + i][0] += v[0][i];
+                sums[j0 + i][1] += v[1][i];
+              }
+            }
+            release();
+          }
+          if (!ok) break;
+          if (whole && product == 1) backs = backs_of(which, unit);  // (h's largest value is known now that it has been multiplied)
+#pragma unroll
+          for (int j = 0; j < MAXN; ++j) {
+            if (j >= n) break;
+            put(j, sums[j][0], sums[j][1]);
+          }
+        } else {
+          wait();
+          if (!ok) break;
+          if (whole && product == 1) backs = backs_of(which, unit);  // (as above)
+          for (int j0 = 0; j0 < n; j0 += 8) {
+            float v[2][8];
+            get(j0, v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              if (j0 + i >= n) break;
+              put(j0 + i, v[0][i], v[1][i]);
             }
           }
+          release();
         }
-        ptx::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          ptx::mbar_arrive(bar_free + 8 * acc);
-          if (!whole) moe_add_release(&w.control->parts[product][unit.cut]);
+        if (!whole) {
+          __syncwarp();
+          if (lane == 0) moe_add_release(&w.control->parts[product][unit.cut]);
+        } else if (product == 0) {
+          finished_up(unit.group, blocks_of(unit.group));
         }
-        if (whole && product == 0) finished_up(unit.group, blocks_of(unit.group));
       }
     };
     if (ok) results_of(std::integral_constant<int, 0>());
@@ -1019,8 +1080,8 @@ MoeSpace::MoeSpace(int64_t tokens, int64_t h, int64_t f, int experts, int top_k)
   hidden = moe_align(h_top + sizeof(uint32_t) * slots);
   outputs = moe_align(hidden + sizeof(float) * slots * (size_t)f);
   x_terms = moe_align(outputs + sizeof(float) * slots * (size_t)h);  // [2][tokens][h]
-  h_terms = moe_align(x_terms + 2 * t * (size_t)h);                    // three of a byte, or two of two
-  parts = moe_align(h_terms + 4 * slots * (size_t)f);
+  h_terms = moe_align(x_terms + 2 * t * (size_t)h);                    // three of a byte or two of two; for an fp32 output six or three
+  parts = moe_align(h_terms + 6 * slots * (size_t)f);
   const size_t group = t <= 8 ? 8 : kMoeGroupTokens;
   bytes = moe_align(parts + sizeof(float) * 2 * kMoeCutTiles * kMoeMostParts * 2 * group * 128);
 }
@@ -1052,10 +1113,10 @@ static int moe_map(CUtensorMap* map, const void* base, bool fp8, int64_t depth, 
   return r == CUDA_SUCCESS ? B200Q_OK : B200Q_ERR_UNSUPPORTED;
 }
 
-template <bool FP8, int MAXN, bool TEST = false>
+template <bool FP8, int MAXN, bool FINE, bool TEST = false>
 static int moe_launch_fused(const b200q_moe_args& a, int64_t first, const MoeSpace& space, cudaStream_t st, int lost = 0) {
-  using Tile = MoeTile<FP8, MAXN>;
-  auto kernel = moe_fused_kernel<FP8, MAXN, TEST>;
+  using Tile = MoeTile<FP8, MAXN, FINE>;
+  auto kernel = moe_fused_kernel<FP8, MAXN, FINE, TEST>;
   constexpr int kSmem = Tile::kStages * Tile::kStage + 1024;
   static std::atomic<int> grid_of[kMaxDevices];  // CTAs that are resident together
   const int dev = current_device_index();
@@ -1143,9 +1204,15 @@ static int moe_chunk(const b200q_moe_args& a, int64_t first, cudaStream_t st) {
   const MoeSpace space(a.tokens, a.hidden, a.inner, a.experts, a.top_k);
   if (int rc = a.router_dtype == B200Q_BF16 ? moe_launch_router<__nv_bfloat16>(a, first, space, st) : moe_launch_router<float>(a, first, space, st)) return rc;
   if (moe_fits_tensor_cores(a)) {
+    const bool few = a.tokens <= 8, fine = a.out_dtype == B200Q_F32;
     int rc;
-    if (a.weight_dtype == B200Q_E4M3) rc = a.tokens <= 8 ? moe_launch_fused<true, 8>(a, first, space, st) : moe_launch_fused<true, kMoeGroupTokens>(a, first, space, st);
-    else rc = a.tokens <= 8 ? moe_launch_fused<false, 8>(a, first, space, st) : moe_launch_fused<false, kMoeGroupTokens>(a, first, space, st);
+    if (a.weight_dtype == B200Q_E4M3) {
+      if (fine) rc = few ? moe_launch_fused<true, 8, true>(a, first, space, st) : moe_launch_fused<true, kMoeFineTokens, true>(a, first, space, st);
+      else rc = few ? moe_launch_fused<true, 8, false>(a, first, space, st) : moe_launch_fused<true, kMoeGroupTokens, false>(a, first, space, st);
+    } else {
+      if (fine) rc = few ? moe_launch_fused<false, 8, true>(a, first, space, st) : moe_launch_fused<false, kMoeGroupTokens, true>(a, first, space, st);
+      else rc = few ? moe_launch_fused<false, 8, false>(a, first, space, st) : moe_launch_fused<false, kMoeGroupTokens, false>(a, first, space, st);
+    }
     if (rc != B200Q_ERR_UNSUPPORTED) return rc;  // (a layout that has no tensor map takes the plain kernels)
   }
   uint8_t* p = static_cast<uint8_t*>(a.workspace);
@@ -1190,11 +1257,11 @@ int moe_layer_impl(const b200q_moe_args& a, cudaStream_t st) {
 // The kernel for 8-bit weights and more tokens than a CTA chooses for by itself, with a wait that is in vain.
 int moe_selftest_impl(const b200q_moe_args& a, int lost, cudaStream_t st) {
   if (lost < 0 || lost >= kMoeLostCount || !moe_has_workspace(a)) return B200Q_ERR_BAD_ARGUMENT;
-  if (!moe_fits_tensor_cores(a) || a.weight_dtype != B200Q_E4M3 || a.router_dtype != B200Q_BF16 || a.tokens <= 4 * kMoeWarps || a.tokens > kMoeChunk)
+  if (!moe_fits_tensor_cores(a) || a.weight_dtype != B200Q_E4M3 || a.out_dtype != B200Q_BF16 || a.router_dtype != B200Q_BF16 || a.tokens <= 4 * kMoeWarps || a.tokens > kMoeChunk)
     return B200Q_ERR_UNSUPPORTED;
   const MoeSpace space(a.tokens, a.hidden, a.inner, a.experts, a.top_k);
   if (int rc = moe_launch_router<__nv_bfloat16>(a, 0, space, st)) return rc;
-  return moe_launch_fused<true, kMoeGroupTokens, true>(a, 0, space, st, lost);
+  return moe_launch_fused<true, kMoeGroupTokens, false, true>(a, 0, space, st, lost);
 }
 
 }  // namespace b200q

@@ -697,7 +697,8 @@ int b200q_selftest_lora_wait_timeout(const b200q_lora_args* args, int lost);
  *   weights = softmax(logits)[ids], over all experts, or over the chosen ones (renormalize != 0)
  *   h_j = silu(g) * u with [g; u] = gate_up_scale * (gate_up[ids_j] x),   out = T(sum_j weights_j * down_scale * (down[ids_j] h_j))
  * in fp32 with one rounding to T.  Before its product an 8-bit weight meets x as two e4m3 terms (exact down to 2^-22 of the token's largest value)
- * and h as three (12 bits, down to 2^-26 of the largest of the token and expert); a bf16 weight meets x as it is and h as two bf16 terms (16 bits).
+ * and h, where out is bf16, as three (12 bits, down to 2^-26 of the largest of the token and expert); a bf16 weight meets x as it is and h as two bf16 terms (16 bits).  Where out is
+ * F32, h has six terms of e4m3 (24 bits, down to 2^-43 of that largest), or three of bf16 (24 bits), and no more than 256 products are summed inside the tensor core.
  * Tokens from *num_tokens on (NULL: none) are not routed: out and weights 0, ids -1, and no expert is read for them.
  *
  * x             bf16 [tokens][hidden], row stride in elements;  router: F32 / BF16 [experts][hidden]
@@ -708,7 +709,7 @@ int b200q_selftest_lora_wait_timeout(const b200q_lora_args* args, int lost);
  * workspace     b200q_moe_workspace_bytes(...) bytes, 16-byte aligned, not shared by calls that may overlap
  * hidden and inner of at most 65536 and multiples of 16 bytes (of weights), with weights, out and the rows of x apart and on 16-byte boundaries, run the tensor-core
  * kernel, anything else (or force_plain = 1) plain ones.  It is launched cooperatively, one block on each SM.
- * Weights of the chosen experts are read once for up to 32 tokens each, and batches of more than 256 tokens are taken 256 at a time: for a few tokens.
+ * Weights of the chosen experts are read once for up to 32 tokens each (16 where they are E4M3 and out is F32), and batches of more than 256 tokens are taken 256 at a time: for a few tokens.
  * An h beyond the end of fp32 makes its token's out NaN.  The same call gives the same bytes.  Status 821 to 825: a wait ran out (out is NaN where a sum is missing).
  */
 typedef struct b200q_moe_args {

@@ -162,3 +162,50 @@ def test_moe_h_at_the_end_of_fp32(tokens, hidden, inner, weights):
     out, weights_of, ids = _run_moe(case, 1)
     assert torch.equal(ids.cpu(), i) and bool((weights_of == 1).all())
     _close(out.float(), want, HALF_STEP[BF16] * (1 + 2.0 ** -10) * want.abs() + bound + FLOOR[BF16])
+
+
+# ----------------------------------------------------------------------------- fp32 outputs of the experts
+@pytest.mark.parametrize("weights", [E4M3, BF16])
+@pytest.mark.parametrize("tokens,inner", [(8, 1792), (30, 1792), (70, 4352), (5, 4352)])
+def test_moe_fp32_h(tokens, inner, weights):
+    """h is the same in all units of a token, so that what its terms drop adds up.  h itself: g and u one rounding each, 2^-24, expf, addition, division and two products, below
+    2^-21 where g is positive; its terms 2^-24.  The second sum is of one sign: 256 products at a time inside the tensor core, 9.5 * 2^-23 (as test_lora_fp32_sums has it), a tenth
+    more for the terms behind the first, inner / 256 additions of 2^-24, and three products: below 25 * 2^-23 for 4352 units, all together below 2^-18."""
+    hidden = 256
+    x, r, gu, down, s1, s2 = _moe_case(tokens, hidden, inner, 1, weights)
+    x[:, 1:], x[:, 0] = 0, x[:, 0].abs() + 0.5
+    gu, down = torch.ones(gu.shape).to(weights), torch.ones(down.shape).to(weights)
+    s1, s2 = torch.full_like(s1, 1 / 3), torch.full_like(s2, 1 / 7)
+    case = (x, r, gu, down, s1, s2)
+    want, _ = O.moe_experts(x, torch.ones(tokens, 1), torch.zeros(tokens, 1, dtype=torch.int32), gu, down, s1, s2)
+    out, _, _ = _run_moe(case, 1, dtype=F32)
+    _close(out, want, 2.0 ** -18 * want)
+
+
+@pytest.mark.parametrize("weights", [E4M3, BF16])
+@pytest.mark.parametrize("tokens,hidden", [(8, 8192), (40, 8192), (20, 2176)])
+def test_moe_fp32_sums(tokens, hidden, weights):
+    """Sums of one sign over hidden.  g and u are off by (9.5 + 1) * 2^-23 + hidden / 256 * 2^-24, below 28 * 2^-23, and with what follows as above: silu makes at most 1.3 of
+    it, that is 2.3 * 28 * 2^-23 in h, and 2^-19 behind: below 2^-16."""
+    x, r, gu, down, s1, s2 = _moe_case(tokens, hidden, 64, 2, weights)
+    x, gu, down = x.abs(), gu.float().abs().to(weights), down.float().abs().to(weights)
+    s1 = s1 * (3 * hidden ** -0.5)
+    case = (x, r, gu, down, s1, s2)
+    w, i = O.moe_route(x, r, 1, True)
+    want, _ = O.moe_experts(x, w, i, gu, down, s1, s2)
+    out, _, ids = _run_moe(case, 1, dtype=F32)
+    assert torch.equal(ids.cpu(), i)
+    _close(out, want, 2.0 ** -16 * want)
+
+
+@pytest.mark.parametrize("weights", [E4M3, BF16])
+@pytest.mark.parametrize("tokens,hidden,inner,experts,top_k", [(7, 512, 272, 16, 8), (45, 4352, 160, 6, 2), (256, 128, 96, 20, 4), (256, 64, 32, 129, 16), (20, 160, 4400, 40, 8), (300, 272, 144, 512, 16)])
+def test_moe_fp32(tokens, hidden, inner, experts, top_k, weights):
+    """Against the oracle with h to 2^-23 of itself and 2^-40 of the largest of its token and expert, where outputs in bf16 have 2^-12 and 2^-26."""
+    case = _moe_case(tokens, hidden, inner, experts, weights)
+    out, weights_of, ids = _run_moe(case, top_k, dtype=F32)
+    w, i = O.moe_route(case[0], case[1], top_k, True)
+    assert torch.equal(ids.cpu(), i)
+    n = max(hidden, inner)
+    want, bound = O.moe_experts(case[0], w, i, *case[2:], rel_sum=(min(n, 256) / 16 + n / 256 + 16) * 2.0 ** -23, rel_hidden=2.0 ** -23, abs_hidden=2.0 ** -40)
+    _close(out, want, 2.0 ** -22 * want.abs() + bound + FLOOR[F32])
