@@ -1592,9 +1592,14 @@ at::Tensor layer_aligned_rows(const at::Tensor& t) {
   return c.is_same(r) ? r.clone() : c;
 }
 int64_t layer_row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(-1); }
-// Whether a written matrix [rows][values] lies apart in itself, and from one that is read.
+// Where the values of a tensor of up to three dimensions lie (those of the last one are contiguous): whether a written matrix lies apart from what is read.
 b200q::CacheLayout layer_layout(const at::Tensor& t) {
-  return b200q::CacheLayout(t.const_data_ptr(), (int64_t)t.element_size(), t.size(1), {t.size(0), 1, 1}, {t.size(0) > 1 ? t.stride(0) : 0, 0, 0});
+  int64_t sizes[3] = {t.numel() ? 1 : 0, 1, 1}, strides[3] = {};
+  for (int64_t i = 0; i + 1 < t.dim() && t.numel(); ++i) {
+    sizes[i] = t.size(i);
+    strides[i] = t.stride(i);
+  }
+  return b200q::CacheLayout(t.const_data_ptr(), (int64_t)t.element_size(), t.dim() ? t.size(-1) : 1, sizes, strides);
 }
 void layer_check_written(const at::Tensor& out, const char* op, const char* name) {
   TORCH_CHECK(out.size(1) <= 1 || out.stride(1) == 1, op, ": the values of a row of ", name, " must be contiguous");
@@ -1671,10 +1676,8 @@ at::Tensor& lora_add_(at::Tensor& y, const at::Tensor& x, const at::Tensor& a_w,
   layer_check_written(y, op, "y");
   at::Tensor xr = layer_aligned_rows(x), ar = layer_rows(a_w), br = layer_rows(b_w), which = adapter.contiguous();
   if (scales.defined()) scales = scales.contiguous();
-  for (const at::Tensor* t : {&xr, &ar, &br}) {
-    if (t->numel() == 0 || y.numel() == 0 || !t->is_alias_of(y)) continue;
-    TORCH_CHECK(t == &xr && y.scalar_type() == at::kBFloat16 && layer_layout(y).apart_from(layer_layout(xr)), op, ": y must not overlap x, a or b");
-  }
+  for (const at::Tensor* t : {&xr, &ar, &br, &which, &scales})
+    TORCH_CHECK(!t->defined() || layer_layout(y).apart_from(layer_layout(*t)), op, ": y must not overlap x, a, b, adapter or scales");
   b200q_lora_args a{};
   a.x = xr.const_data_ptr(); a.x_stride = layer_row_stride(xr);
   a.y = y.data_ptr(); a.y_dtype = to_b200q_dtype(y.scalar_type()); a.y_stride = layer_row_stride(y);

@@ -209,3 +209,35 @@ def test_moe_fp32(tokens, hidden, inner, experts, top_k, weights):
     n = max(hidden, inner)
     want, bound = O.moe_experts(case[0], w, i, *case[2:], rel_sum=(min(n, 256) / 16 + n / 256 + 16) * 2.0 ** -23, rel_hidden=2.0 ** -23, abs_hidden=2.0 ** -40)
     _close(out, want, 2.0 ** -22 * want.abs() + bound + FLOOR[F32])
+
+
+# ----------------------------------------------------------------------------- memory that is shared
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_lora_in_one_allocation(dtype):
+    """All of a call's tensors as parts of one allocation, as a program that divides up its memory itself has them."""
+    y, x, a, b, which, scales = c = _lora_case(40, 64, 72, 16, 3, dtype)
+    pool, at = torch.zeros(1 << 20, dtype=torch.uint8, device="cuda"), 0
+
+    def place(t):
+        nonlocal at
+        part = pool[at:at + t.numel() * t.element_size()].view(t.dtype).view(t.shape)
+        at += -(-part.numel() * part.element_size() // 256) * 256
+        return part.copy_(t)
+
+    ad, sd, xd, yd, bd, wd = (place(t) for t in (a, scales, x, y, b, which))
+    torch.ops.b200q.lora_add_(yd, xd, ad, bd, wd, sd)
+    _check_lora(yd, *c)
+    wide = torch.zeros(40, 512, dtype=torch.uint8, device="cuda")  # y beside x in the rows of one buffer
+    ys, xs = wide[:, :72 * y.element_size()].view(dtype), wide[:, 384:512].view(BF16)
+    ys.copy_(y)
+    xs.copy_(x)
+    torch.ops.b200q.lora_add_(ys, xs, ad, bd, wd, sd)
+    _check_lora(ys, *c)
+
+
+def test_lora_refuses_to_write_its_inputs():
+    y, x, a, b, which, scales = (t.cuda() for t in _lora_case(4, 64, 32, 8, 2, F32))
+    op = torch.ops.b200q.lora_add_
+    for args in [(y, x, a, b, y.view(torch.int32)[1, 3:7]), (y, x, a, b, which, y[3, 30:]), (a.view(-1).view(F32)[:128].view(4, 32), x, a, b, which), (b.view(-1).view(F32)[128:256].view(4, 32), x, a, b, which)]:
+        with pytest.raises(RuntimeError, match="must not overlap"):
+            op(*args)
