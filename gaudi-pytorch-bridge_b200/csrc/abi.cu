@@ -139,11 +139,16 @@ static bool on_bytes(size_t bytes, std::initializer_list<const void*> pointers) 
     if (reinterpret_cast<uintptr_t>(p) % bytes) return false;
   return true;
 }
-// whether no byte belongs to both of two matrices of one type and shape (the first one's rows lie apart)
-static bool rows_apart(const void* p, int64_t p_stride, const void* q, int64_t q_stride, int dtype, int64_t rows, int64_t cols) {
-  const int64_t sizes[3] = {rows, 1, 1}, elt = dtype == B200Q_F32 ? 4 : 2;
-  const CacheLayout first(p, elt, cols, sizes, {p_stride, 0, 0}), second(q, elt, cols, sizes, {q_stride, 0, 0});
-  return first.apart() && first.apart_from(second);
+// where the values of a matrix of a 16-bit or 32-bit type lie, or of a row
+static CacheLayout matrix_at(const void* p, int dtype, int64_t rows, int64_t cols, int64_t stride) {
+  return CacheLayout(p, dtype == B200Q_F32 ? 4 : 2, cols, {rows, 1, 1}, {stride, 0, 0});
+}
+// whether a matrix that is written lies apart in itself and from all that is read
+static bool written_apart(const CacheLayout& out, std::initializer_list<CacheLayout> in) {
+  if (!out.apart()) return false;
+  for (const CacheLayout& c : in)
+    if (!out.apart_from(c)) return false;
+  return true;
 }
 static bool scale_args_ok(const float* dev, int mode) {
   if (mode < B200Q_BCAST_NONE || mode > B200Q_BCAST_FULL) return false;
@@ -606,7 +611,10 @@ static int check_norm(const b200q_norm_args* a) {
       !on_elements(a->out, a->out_dtype, 1) || !on_bytes(2, {a->kept}) || !on_bytes(4, {a->scale, a->scale_inv}))
     return B200Q_ERR_UNSUPPORTED;
   if (a->dim == 0 && !a->scale_inv) return B200Q_OK;
-  if (a->residual && !rows_apart(a->residual, a->residual_stride, a->x, a->x_stride, a->x_dtype, a->tokens, a->dim)) return B200Q_ERR_BAD_ARGUMENT;
+  if (a->residual && !written_apart(matrix_at(a->residual, a->x_dtype, a->tokens, a->dim, a->residual_stride),
+                                    {matrix_at(a->x, a->x_dtype, a->tokens, a->dim, a->x_stride), matrix_at(a->weight, a->weight_dtype, a->weight != nullptr, a->dim, 0),
+                                     matrix_at(a->scale, B200Q_F32, a->scale != nullptr, 1, 0)}))
+    return B200Q_ERR_BAD_ARGUMENT;
   return B200Q_OK;
 }
 
@@ -636,6 +644,12 @@ static int check_lora(const b200q_lora_args* a) {
   if (lora_adds_nothing(a)) return B200Q_OK;
   if (!a->x || !a->y || !a->a || !a->b || !a->adapter) return B200Q_ERR_BAD_ARGUMENT;
   if (!on_bytes(2, {a->x, a->a, a->b}) || !on_elements(a->y, a->y_dtype, 1) || !on_bytes(4, {a->adapter, a->scales})) return B200Q_ERR_UNSUPPORTED;
+  const int64_t planes[3] = {a->adapters, a->rank, 1}, columns[3] = {a->adapters, a->n, 1};
+  if (!written_apart(matrix_at(a->y, a->y_dtype, a->tokens, a->n, a->y_stride),
+                     {matrix_at(a->x, B200Q_BF16, a->tokens, a->k, a->x_stride), CacheLayout(a->a, 2, a->k, planes, {a->a_stride, a->a_row_stride, 0}),
+                      CacheLayout(a->b, 2, a->rank, columns, {a->b_stride, a->b_row_stride, 0}), matrix_at(a->adapter, B200Q_F32, 1, a->tokens, 0),
+                      matrix_at(a->scales, B200Q_F32, a->scales != nullptr, a->adapters, 0)}))
+    return B200Q_ERR_BAD_ARGUMENT;
   return B200Q_OK;
 }
 

@@ -1630,6 +1630,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rms_norm_cast(const at::Tenso
                 ": weight must be a float or bfloat16 tensor of ", dim, " values");
     weight = weight.contiguous();
   }
+  if (residual.defined())
+    for (const at::Tensor* t : {&weight, &scale}) TORCH_CHECK(!t->defined() || layer_layout(residual).apart_from(layer_layout(*t)), op, ": residual must not overlap weight or scale");
   const bool dynamic = is_fp8(dtype) && !scale.defined();
   at::Tensor out = new_tensor({tokens, dim}, dtype, dev);
   at::Tensor scale_inv = dynamic ? new_tensor({tokens, 1}, at::kFloat, dev) : new_tensor({0}, at::kFloat, dev);

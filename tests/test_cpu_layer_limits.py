@@ -1,12 +1,14 @@
-"""The norm, the adapters and the experts, without a GPU: what their self-tests refuse before any CUDA call."""
+"""The norm, the adapters and the experts, without a GPU: what their self-tests, and they themselves, refuse before any CUDA call."""
 import ctypes
 
 import pytest
+import torch
 
 from b200_hpu_ops import abi
-from test_cpu_layer import AT, BAD, UNSUPPORTED, _call
+from test_cpu_layer import AT, BAD, UNSUPPORTED, _call, _lora, _norm
 
 SOME = 1 << 40  # bytes of a workspace that nothing reads
+pytestmark = pytest.mark.skipif(torch.cuda.is_available(), reason="a call that is not refused would reach the GPU")
 
 
 def _moe_selftest(lost=0, **kw):
@@ -64,3 +66,15 @@ def test_norm_selftest_refuses(kw, rc):
 
 def test_norm_selftest_refuses_nothing():
     assert abi.lib.b200q_selftest_norm_wait_timeout(ctypes.POINTER(abi.NormArgs)()) == BAD
+
+
+@pytest.mark.parametrize("kw", [dict(residual=AT + 64, weight=AT, x=AT << 6), dict(residual=(AT << 4), weight=(AT << 4) + 3 * 128 - 2), dict(residual=AT << 4, scale=(AT << 4) + 256, out_dtype=abi.BF16),
+                                dict(residual=AT << 4, weight=(AT << 4) + 380, weight_dtype=abi.F32)])
+def test_norm_refuses_to_write_its_inputs(kw):
+    assert _norm(**kw) == BAD
+
+
+@pytest.mark.parametrize("kw", [dict(x=(AT << 4) + 190), dict(a=(AT << 4) - 2 * 2 * 16 * 64 + 2), dict(b=(AT << 4) + 64), dict(adapter=(AT << 4) + 188), dict(scales=(AT << 4) + 100),
+                                dict(y_stride=40, scales=(AT << 4) + 72), dict(x=(AT << 4) - 32 * 2, x_stride=0), dict(x=(AT << 4) + 64, x_stride=32)])
+def test_lora_refuses_to_write_its_inputs(kw):
+    assert _lora(workspace=AT, workspace_bytes=SOME, force_plain=1, **kw) == BAD

@@ -241,3 +241,14 @@ def test_lora_refuses_to_write_its_inputs():
     for args in [(y, x, a, b, y.view(torch.int32)[1, 3:7]), (y, x, a, b, which, y[3, 30:]), (a.view(-1).view(F32)[:128].view(4, 32), x, a, b, which), (b.view(-1).view(F32)[128:256].view(4, 32), x, a, b, which)]:
         with pytest.raises(RuntimeError, match="must not overlap"):
             op(*args)
+
+
+def test_norm_refuses_to_write_its_inputs():
+    x, r = torch.ones(4, 64, dtype=BF16, device="cuda"), torch.ones(4, 64, dtype=BF16, device="cuda")
+    op = torch.ops.b200q.add_rms_norm_cast
+    for weight, scale in [(r[1], None), (r.view(F32).view(-1)[10:74], None), (None, r.view(F32)[3, 5])]:
+        with pytest.raises(RuntimeError, match="must not overlap weight or scale"):
+            op(x, r, weight, EPS, BF16, scale)
+    both = torch.ones(6, 64, dtype=BF16, device="cuda")  # one allocation
+    op(x, both[:4], both[4], EPS, BF16, both[5].view(F32)[7])
+    assert bool((both[:4] == 2).all()) and bool((both[4:] == 1).all())
