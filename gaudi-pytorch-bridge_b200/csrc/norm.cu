@@ -583,7 +583,8 @@ static NormForm norm_form(const b200q_norm_args& a) {
   const int64_t strides[2] = {a.x_stride, a.residual ? a.residual_stride : a.x_stride};
   const bool one = a.tokens == 1;  // (no stride is used)
   if (aligned && a.dim % 8 == 0 && (one || (strides[0] % 8 == 0 && strides[1] % 8 == 0))) return kNormEven;
-  if (aligned && (one || ((strides[0] - a.dim) % 8 == 0 && (strides[1] - a.dim) % 8 == 0))) return kNormShifted;
+  // (rows that overlap: what is fetched beyond a row could lie behind the last one)
+  if (aligned && (one || ((strides[0] - a.dim) % 8 == 0 && (strides[1] - a.dim) % 8 == 0 && strides[0] >= a.dim))) return kNormShifted;
   return kNormLoose;
 }
 

@@ -623,7 +623,7 @@ int b200q_selftest_paged_wait_timeout(const b200q_paged_attention_args* args, in
  * fp8: to nearest even, saturating; NaN -> 0x7F.  A NaN anywhere in y makes the token's scale_inv NaN, and its fp8 values with it.
  * A quotient max(U) / max|y| that passes the end of fp32 (all of y below 1e-36) is cut to it.
  *
- * x             F32 / BF16 [tokens][dim], row stride in elements, values contiguous
+ * x             F32 / BF16 [tokens][dim], row stride in elements (rows may overlap, or be one), values contiguous
  * residual      type and shape of x, row stride >= dim, or NULL.  No byte may belong to an input as well
  * weight        F32 / BF16 [dim], or NULL: 1
  * out           BF16 / E4M3 / E5M2 [tokens][dim] contiguous;  kept: bf16 alike, or NULL;  scale_inv: fp32 [tokens], or NULL; apart from all inputs

@@ -252,3 +252,17 @@ def test_norm_refuses_to_write_its_inputs():
     both = torch.ones(6, 64, dtype=BF16, device="cuda")  # one allocation
     op(x, both[:4], both[4], EPS, BF16, both[5].view(F32)[7])
     assert bool((both[:4] == 2).all()) and bool((both[4:] == 1).all())
+
+
+@pytest.mark.parametrize("dim,step", [(525, 5), (521, 1), (1000, 8), (8189, 5), (261, 5)])
+def test_norm_rows_that_overlap(dim, step):
+    """Windows of one long row, up to its end."""
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    x = torch.randn(400 * step + dim, generator=g, device="cuda").to(BF16).as_strided((401, dim), (step, 1))
+    _, y = O.add_rms_norm(x, None, None, EPS)
+    out, inv, kept = torch.ops.b200q.add_rms_norm_cast(x, None, None, EPS, E4M3, None, True)
+    top = y.abs().amax(-1, keepdim=True)
+    v = y * (448.0 / top)
+    _close(inv, (top / 448.0).cpu(), 2.0 ** -16 * (top / 448.0).cpu())
+    _close(out.float(), v.cpu(), ((HALF_STEP[E4M3] + 2.0 ** -16) * v.abs() + FLOOR[E4M3]).cpu())
+    _close(kept.float(), y.cpu(), ((HALF_STEP[BF16] + 2.0 ** -17) * y.abs() + FLOOR[BF16]).cpu())
