@@ -411,10 +411,15 @@ __device__ __forceinline__ void moe_fence_async() { asm volatile("fence.proxy.as
 __device__ __forceinline__ int moe_divide(int x, float inverse) { return (int)(((float)x + 0.5f) * inverse); }
 
 // The units of a product: `whole` tiles, then the parts of the others.  Fewer than 2^22 of them: at most 768 groups, of 512 tiles each.
-// Cut are the tiles that do not come out even, and a quarter of a round of all CTAs at least; but none of up to 32 steps (4096 bytes of a row), because fewer CTAs draw more each and
-// the sums come on top, and none where so many CTAs have one whole tile that they draw all that the memory gives.  us with cuts above 8 steps, above 32, and none at all: 64 tokens
-// of 32 experts 2048 x 688 66, 60, 60; 16 tokens of 64 experts 2048 x 1408 94, 86, 86; 29 tokens of 128 experts 4096 x 1792 383, 378, 377; 5 tokens of 8 experts 4096 x 4096 in
-// bf16 (64 steps) 116, 116, 120.
+// Cut are the tiles that do not come out even, and a quarter of a round of all CTAs at least; but not
+// * tiles of up to 8 steps;
+// * tiles of up to 32 steps (4096 bytes of a row) where there is one for each third CTA or more: fewer CTAs draw more each, and the sums come on top.  us with cuts above 8 steps, above
+//   32 and none at all: 64 tokens of 32 experts 2048 x 688 (192 tiles) 66, 60, 60; 16 tokens of 64 experts 2048 x 1408 94, 86, 86; 29 tokens of 128 experts 4096 x 1792 383, 378, 377.
+//   One token, with and without: 14 tiles of 32 steps 26.6, 34.2; 28 28.7, 35.4; 32 28.8, 34.2; 32 of 16 steps 25.7, 27.2; 64 of 32 42.8, 39.4; 64 of 16 32.8, 29.3; 64 and 32 of 32 as now 42.0,
+//   uncut 45.2; bf16 weights, 8 and 8 of 32 and 16 steps 21.1, 31.5;
+// * any where a product has less than a round of the CTAs, but 70 % of one: those draw all that the memory gives.  One token of a bf16 expert of 4096 x 128 n, n tiles of 64 steps, us with
+//   and without: n = 40 42.2, -; 75 57.5, 58.6; 90 64.2, 64.8; 100 69.3, 68.6; 105 72.2, 70.3; 112 76.1, 73.8; 120 79.0, 74.7; 148 91.3, 88.1; in e4m3 (8192 x 128 n) 90 76.3, 75.0; 105 83.7,
+//   80.8; 140 102.9, 98.3.
 struct MoeUnits {
   int tiles, steps, whole, cut, parts, units;  // tiles of a group, steps of a tile
   float per_group, per_tile;
@@ -423,7 +428,7 @@ struct MoeUnits {
     steps = steps_;
     const int total = groups * tiles, rounds = max(0, moe_divide(total - ctas / 4, __frcp_rn((float)ctas)));
     cut = total - rounds * ctas;
-    if (steps <= 32 || (total <= ctas && 10 * total >= 7 * ctas)) cut = 0;
+    if (steps <= 8 || (steps <= 32 && 3 * total > ctas) || (total <= ctas && 10 * total >= 7 * ctas)) cut = 0;
     const int length = max(3, min((int)((float)(cut * steps) * __frcp_rn((float)(3 * ctas))), 8));
     parts = min(moe_divide(steps + length - 1, __frcp_rn((float)length)), kMoeMostParts);
     whole = total - cut;

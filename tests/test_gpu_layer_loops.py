@@ -104,3 +104,12 @@ def test_moe_several_units_to_a_block(tokens, hidden, inner, experts, top_k, wei
     """More tiles than three times the SMs: units from the counter, accumulators and rings that turn many times."""
     case = _moe_case(tokens, hidden, inner, experts, weights)
     _check_moe(_run_moe(case, top_k), case, top_k)
+
+
+@pytest.mark.parametrize("weights", [E4M3, BF16])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("tokens,hidden,inner,experts,top_k", [(1, 2048, 640, 4, 1), (3, 1280, 1536, 3, 2), (12, 2048, 160, 5, 2), (100, 1408, 128, 2, 2), (1, 4096, 2048, 2, 1)])
+def test_moe_cut_short_rows(tokens, hidden, inner, experts, top_k, dtype, weights):
+    """Rows of 9 to 32 steps, whose tiles are cut where they are fewer than a third of the SMs."""
+    case = _moe_case(tokens, hidden, inner, experts, weights)
+    _check_moe(_run_moe(case, top_k, dtype=dtype), case, top_k, dtype=dtype)
