@@ -85,11 +85,20 @@ struct LoraSpace {
   }
 };
 
-// Tiles of 128 tokens where an adapter has many on average and their terms leave room for the copies, else of 16: those take less shared memory, and so more copies
-// are on their way.
-static int lora_tile_tokens(int64_t tokens, int64_t rank, int64_t adapters, bool wide) {
+// Tiles of 128 tokens read the adapters' matrices less often, and tiles of 16 are more, take less shared memory and so have more copies on their way.  us with 16 and with 128, bf16, k = n =
+// 4096 and 8 adapters where nothing else is said:
+// * tokens: rank 16 to 64: 1024 22, 31 to 34; 2600 35, 40; 3500 45, 42; 5000 72, 48; 8192 82, 67 to 87, 67; fp32, rank 64: 2600 45, 53; 3500 68, 59.  A rank of 129 and more is two blocks of rows
+//   that fetch the tokens twice, rank 192: 1024 57, 89; 2048 81, 75 (n = 14336 159, 98); 4096 131, 85 (285, 132);
+// * tokens times k + n, 2^20: k = n = 1024 (4096 to 8192 tokens, 8 to 16) 22, 26 and 32, 33; k = 4096, n = 1024 (20) 29, 32; k = 1024, n = 4096 (20) 39, 38; (27) as above; rank 128, whose terms leave room
+//   for one CTA: 3500 tokens (27) 62, 71; 4096 (32) 65, 74; 5000 (39) 99, 75; n = 14336 (72) 138, 122; in fp32 (32) 98, 76;
+// * adapters: 8192 tokens of 128 adapters 79, 89 (k = 14336 133, 190), because their tiles and those that there might be leave a x whole; 4096 tokens of 64 53, 47, of 128 53, 60; 8192 of 84 90, 76.
+// What counts is the table's adapters, which the host knows, not those that are used: 4096 tokens of one of 256 60, 55.
+static int lora_tile_tokens(int64_t tokens, int64_t k, int64_t n, int64_t rank, int64_t adapters, bool wide) {
   const int64_t t = tokens < kLoraChunk ? tokens : kLoraChunk, blocks = (wide ? 3 : 2) * ((rank + 63) / 64);
-  return t >= 24 * adapters && t > kLoraFew && blocks <= 6 ? 128 : 16;
+  if (blocks > 6 || adapters + t / 128 > kNumSMs) return 16;  // (more terms leave no room for the copies)
+  if (rank > 128) return t >= 2048 ? 128 : 16;
+  const int64_t least = rank > 64 && !wide ? 36 : 24;
+  return t >= 3200 && t * (k + n) >= least << 20 ? 128 : 16;
 }
 // CTAs of an SM that share a x: more where ranks are few, because an item is a chain of steps
 // (64 tokens of 56 adapters of rank 32, 8192 values each: 24.3 us with two, 22.6 with four)
@@ -850,7 +859,7 @@ static int lora_launch_up_tile(const b200q_lora_args& a, const LoraPlan& p, int6
 enum LoraLost { kLoraLostNothing = -1, kLoraLostA, kLoraLostB, kLoraLostCount };  // what a self-test waits for in vain: the first copy of a, or of b, of block 0
 
 static int lora_chunk_fast(const b200q_lora_args& a, cudaStream_t st, int lost = kLoraLostNothing) {
-  const int tile = lora_tile_tokens(a.tokens, a.rank, a.adapters, a.y_dtype == B200Q_F32);
+  const int tile = lora_tile_tokens(a.tokens, a.k, a.n, a.rank, a.adapters, a.y_dtype == B200Q_F32);
   const int64_t splits = lora_splits(a.tokens, a.k, a.rank, a.adapters, tile), tiles = lora_most_tiles(a.tokens, a.adapters, tile);
   const LoraSpace space(a.tokens, a.rank, splits);
   uint8_t* w = static_cast<uint8_t*>(a.workspace);
@@ -918,7 +927,7 @@ int lora_add_impl(const b200q_lora_args& a, cudaStream_t st) {
 
 int lora_selftest_impl(const b200q_lora_args& a, int lost, cudaStream_t st) {
   if (lost < 0 || lost >= kLoraLostCount || !lora_has_workspace(a)) return B200Q_ERR_BAD_ARGUMENT;
-  if (!lora_fits_tensor_cores(a) || a.y_dtype != B200Q_BF16 || !lora_y_whole(a) || a.tokens > kLoraChunk || lora_tile_tokens(a.tokens, a.rank, a.adapters, false) != 16)
+  if (!lora_fits_tensor_cores(a) || a.y_dtype != B200Q_BF16 || !lora_y_whole(a) || a.tokens > kLoraChunk || lora_tile_tokens(a.tokens, a.k, a.n, a.rank, a.adapters, false) != 16)
     return B200Q_ERR_UNSUPPORTED;
   return lora_chunk_fast(a, st, lost);
 }

@@ -687,7 +687,7 @@ typedef struct b200q_lora_args {
 
 size_t b200q_lora_workspace_bytes(int64_t tokens, int64_t k, int64_t n, int64_t rank, int64_t adapters);
 int b200q_lora_add(const b200q_lora_args* args);
-/* Self-test of its bounded waits: the same call (up to 8192 tokens, so many adapters or so few tokens that tiles have 16, bf16 y on boundaries of 16 bytes, sizes of the tensor-core kernels,
+/* Self-test of its bounded waits: the same call (up to 8192 tokens, and so few that tiles have 16 of them: 2047 always are, bf16 y on boundaries of 16 bytes, sizes of the tensor-core kernels,
  * else B200Q_ERR_UNSUPPORTED) with short waits, in which one copy never comes: block 0's first of a (lost = 0), or of b (1).  The kernels end by themselves; the GPU does not fault. */
 int b200q_selftest_lora_wait_timeout(const b200q_lora_args* args, int lost);
 

@@ -40,7 +40,7 @@ def _lora_selftest(lost=0, **kw):
 
 
 @pytest.mark.parametrize("kw,rc", [(dict(lost=-1), BAD), (dict(lost=2), BAD), (dict(workspace=None), BAD), (dict(workspace_bytes=100), BAD), (dict(tokens=-1), BAD), (dict(tokens=0), BAD),
-                                   (dict(rank=0), BAD), (dict(tokens=200), UNSUPPORTED), (dict(tokens=8193), UNSUPPORTED), (dict(y_dtype=abi.F32), UNSUPPORTED),
+                                   (dict(rank=0), BAD), (dict(tokens=2048, rank=136, a_stride=136 * 64, b_row_stride=136, b_stride=136 * 32), UNSUPPORTED), (dict(tokens=8193), UNSUPPORTED), (dict(y_dtype=abi.F32), UNSUPPORTED),
                                    (dict(y=(AT << 4) + 2), UNSUPPORTED), (dict(force_plain=1), UNSUPPORTED), (dict(rank=12), UNSUPPORTED)])
 def test_lora_selftest_refuses(kw, rc):
     assert _lora_selftest(**kw) == rc

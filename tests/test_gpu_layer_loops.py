@@ -70,7 +70,7 @@ def test_norm_rows_of_wider_matrices_several_to_a_block(dim, step, tokens):
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("tokens,k,n,rank,adapters", [(6000, 72, 264, 16, 2048), (4000, 320, 136, 72, 1500), (2000, 136, 72, 256, 700), (8192, 72, 264, 16, 340), (8192, 200, 136, 64, 330)])
 def test_lora_more_tiles_than_blocks(tokens, k, n, rank, adapters, dtype):
-    """Tiles of 16 tokens and (the last two) of 128, some two to four to each block of both kernels, so that the terms, the accumulators and their barriers turn."""
+    """Tiles of 16 tokens, some two to four to each block of both kernels, so that the terms, the accumulators and their barriers turn."""
     c = _lora_case(tokens, k, n, rank, adapters, dtype)
     _check_lora(_run_lora(*c), *c)
 
@@ -79,7 +79,7 @@ def test_lora_more_tiles_than_blocks(tokens, k, n, rank, adapters, dtype):
 @pytest.mark.parametrize("order", ["runs", "scattered"])
 @pytest.mark.parametrize("tokens,k,n,rank,adapters", [(400, 2056, 136, 16, 2), (300, 4104, 72, 128, 1), (1024, 4104, 136, 64, 8), (2048, 8192, 64, 24, 16)])
 def test_lora_long_rows_of_many_tokens(tokens, k, n, rank, adapters, order, dtype):
-    """Tiles of 128 tokens with rows of k that are cut into parts, of more than four steps of 64 values each."""
+    """Rows of k that are cut into parts, of more than four steps of 64 values each."""
     which = torch.arange(tokens) * adapters // tokens
     if order == "scattered":
         which = which[torch.randperm(tokens, generator=torch.Generator().manual_seed(tokens))]
@@ -113,3 +113,81 @@ def test_moe_cut_short_rows(tokens, hidden, inner, experts, top_k, dtype, weight
     """Rows of 9 to 32 steps, whose tiles are cut where they are fewer than a third of the SMs."""
     case = _moe_case(tokens, hidden, inner, experts, weights)
     _check_moe(_run_moe(case, top_k, dtype=dtype), case, top_k, dtype=dtype)
+
+
+# ----------------------------------------------------------------------------- adapters: tiles of 128 tokens, which only long batches have
+def _order(order, tokens, adapters):
+    if order == "runs":
+        return torch.arange(tokens) * adapters // tokens
+    if order == "scattered":
+        return torch.randint(-1, adapters + 1, (tokens,), generator=torch.Generator().manual_seed(tokens))
+    lens = [1, 255, 1, 16, 64, 127, 128, 129, 700, 3]  # prompts beside single tokens
+    which = torch.repeat_interleave(torch.arange(len(lens)) * 7 % (adapters + 1), torch.tensor(lens))
+    return which.repeat(-(-tokens // len(which)))[:tokens]
+
+
+LARGE = [(3200, 4104, 4104, 16, 8), (8192, 2056, 1416, 64, 84), (4000, 6400, 264, 40, 3), (6001, 200, 4304, 8, 20), (2048, 264, 136, 192, 3), (3000, 72, 1032, 136, 100), (6400, 4104, 2056, 128, 5)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("order", ["runs", "scattered", "mixed"])
+@pytest.mark.parametrize("tokens,k,n,rank,adapters", LARGE)
+def test_lora_long_batches(tokens, k, n, rank, adapters, order, dtype):
+    c = _lora_case(tokens, k, n, rank, adapters, dtype, which=_order(order, tokens, adapters))
+    _check_lora(_run_lora(*c), *c)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("at", [3, 8])
+def test_lora_long_batches_between_boundaries(at, dtype):
+    """y from a column of a wider matrix on, x of another."""
+    y, x, a, b, which, scales = c = _lora_case(4000, 6400, 264, 16, 6, dtype, which=_order("mixed", 4000, 6))
+    wide, xs = torch.zeros(4000, 264 + 13, dtype=dtype).cuda(), torch.zeros(4000, 6416, dtype=BF16).cuda()
+    wide[:, at:at + 264], xs[:, 8:6408] = y.cuda(), x.cuda()
+    torch.ops.b200q.lora_add_(wide[:, at:at + 264], xs[:, 8:6408], a.cuda(), b.cuda(), which.cuda(), scales.cuda())
+    _check_lora(wide[:, at:at + 264], *c)
+    assert bool((wide[:, :at] == 0).all()) and bool((wide[:, at + 264:] == 0).all())
+
+
+def test_lora_long_batches_fp32_sums():
+    """As test_lora_fp32_sums_of_many_tokens."""
+    y, x, a, b, which, scales = _lora_case(3300, 8192, 64, 8, 4, F32, which=torch.arange(3300) % 4)
+    x, a, b, y = x.abs(), a.abs(), b.abs(), torch.zeros_like(y)
+    want, size, _ = O.lora_add(y, x, a, b, which, scales)
+    _close(_run_lora(y, x, a, b, which, scales), want, 2.0 ** -17 * size)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_lora_long_batches_one_behind_the_other(dtype):
+    """A chain of calls on one y, between kernels that change y and x, has the bytes of calls that are waited for."""
+    y, x, a, b, which, scales = (t.cuda() for t in _lora_case(4096, 4096, 2056, 16, 8, dtype, which=_order("mixed", 4096, 8)))
+
+    def chain(wait):
+        ys, xs, ws = y.clone(), x.clone(), which.clone()
+        for i in range(6):
+            torch.ops.b200q.lora_add_(ys, xs, a, b, ws, scales)
+            wait()
+            ys.mul_(0.75)
+            wait()
+            xs.neg_()
+            wait()
+            ws.copy_(ws.roll(1))
+            wait()
+        return ys
+
+    want = chain(torch.cuda.synchronize)
+    for _ in range(3):
+        assert torch.equal(chain(lambda: None), want)
+
+
+def test_lora_long_batches_infinities():
+    import math
+    y, x, a, b, which, scales = _lora_case(4000, 6400, 264, 16, 3, BF16, which=torch.arange(4000) % 3)
+    a, b = a.abs() + 2.0 ** -10, b.abs() + 2.0 ** -10
+    x[[0, 1, 300], 3] = math.inf
+    x[7, 5], x[8, 6399], x[9, 0] = -math.inf, math.nan, math.inf
+    want, _, _ = O.lora_add(y, x, a, b, which, scales)
+    got = _run_lora(y, x, a, b, which, scales).cpu().float()
+    bad = ~want.isfinite()
+    assert int(bad.any(-1).sum()) == 6 and torch.equal(got[bad].nan_to_num(nan=7.0), want[bad].float().nan_to_num(nan=7.0))
+    assert bool(got[~bad].isfinite().all())
