@@ -558,7 +558,10 @@ static int norm_launch_many(const b200q_norm_args& a, float inv_dim, cudaStream_
     int rc = B200Q_ERR_UNSUPPORTED;
     if (dim <= 1024) rc = norm_launch_ring<T, FORM, 64, 2, 12>(a, inv_dim, st);
     else if (dim <= 2048) rc = norm_launch_ring<T, FORM, 128, 2, 6>(a, inv_dim, st);
-    else if (dim <= 2560) rc = norm_launch_ring<T, FORM, 128, 4, 6>(a, inv_dim, st);
+    // (us with six blocks of 128 threads an SM and with four of 256, 60e6 values, bf16 with residual / without / fp32 with, half as many / without: 2624 88, 93 / 64, 78 / 67, 72 / 71, 78; 2816 76,
+    // 87 / 61, 73 / 68, 70 / 61, 73; 3008 75, 83 / 58, 70 / 70, 69 / 60, 69; 3200 86, 81 / 63, 68 / 69, 66 / 61, 67; 3584 79, 75 / 54, 62 / 69, 66 / 60, 62; 4096 75, 71 / 49, 56 / 68, 67 / 55, 57.
+    // Rows of odd lengths, bf16 with residual: 2817 143, 175; 3001 136, 139; 3201 180, 135; 4001 120, 114)
+    else if (dim <= 3008 || (dim <= 4096 && !a.residual && FORM == kNormEven)) rc = norm_launch_ring<T, FORM, 128, 4, 6>(a, inv_dim, st);
     else if (dim <= 4096) rc = norm_launch_ring<T, FORM, 256, 2, 4>(a, inv_dim, st);
     else if (dim <= 8192) rc = norm_launch_ring<T, FORM, 512, 2, 2>(a, inv_dim, st);
     else if (dim <= 16384) rc = norm_launch_ring<T, FORM, 512, 4, 2>(a, inv_dim, st);

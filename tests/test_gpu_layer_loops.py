@@ -19,7 +19,7 @@ def _off(got, want, tol, what):
 
 # Rows of each instance of the ring (12, 6, 6, 4, 2, 2 and 1 blocks of an SM) and of the kernel that has a row in a warp or block, so many that each block has the
 # ring's places twice and some have a row more: (dim, tokens).
-ROWS = [(200, 12001), (400, 9000), (600, 16005), (1500, 6301), (2300, 4447), (4000, 3001), (8192, 1301), (12000, 1201), (20000, 601), (32768, 303)]
+ROWS = [(200, 12001), (400, 9000), (600, 16005), (1500, 6301), (2300, 4447), (3000, 4501), (4000, 5003), (8192, 1301), (12000, 1201), (20000, 601), (32768, 303)]
 
 
 @pytest.mark.parametrize("odd", [0, 1, 3])
