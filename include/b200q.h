@@ -76,7 +76,7 @@ int b200q_selftest_wait_timeout(int code, void* stream);
 /* Number of kernels this library has launched in this process (all threads). */
 uint64_t b200q_launch_count(void);
 /* sizeof of an argument struct as this library was built: which = 0 b200q_gemm_args, 1 b200q_sdpa_args,
- * 2 b200q_append_args, 3 b200q_paged_attention_args; 0 for any other value.  A binding that mirrors the structs (ctypes, cgo, JNI) checks its own layout against it. */
+ * 2 b200q_append_args, 3 b200q_paged_attention_args, 4 b200q_norm_args, 5 b200q_lora_args, 6 b200q_moe_args; 0 for any other value.  A binding that mirrors the structs (ctypes, cgo, JNI) checks its own layout against it. */
 size_t b200q_sizeof_args(int which);
 
 /*
@@ -615,11 +615,11 @@ int b200q_selftest_paged_wait_timeout(const b200q_paged_attention_args* args, in
  *
  * add_rms_norm_cast: the step between two products, in one pass.  Per token
  *   z = T(residual + x) (stored to residual; the sum is formed in fp32 and rounded once), or x where residual is NULL
- *   y = z * rsqrt(mean(z^2) + eps) * weight                           in fp32
+ *   y = (z * weight) * rsqrt(mean(z^2) + eps)                         in fp32
  *   kept = bf16(y)                                                    where kept is not NULL
  *   out  = U(y * scale)                                               scale one fp32 on the device, or NULL: 1
  *   or, where scale_inv is not NULL (fp8 outputs; scale must be NULL):
- *   scale_inv = max|y| / max(U),  out = U(y * (max(U) / max|y|));     a token of zeros gets scale_inv 1 and zeros
+ *   scale_inv = max|y| / max(U),  out = U(y * (max(U) / max|y|));     a token of zeros (and eps > 0) gets scale_inv 1 and zeros
  * fp8: to nearest even, saturating; NaN -> 0x7F.  A NaN anywhere in y makes the token's scale_inv NaN, and its fp8 values with it.
  * A quotient max(U) / max|y| that passes the end of fp32 (all of y below 1e-36) is cut to it.
  *
