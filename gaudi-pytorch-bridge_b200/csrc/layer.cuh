@@ -22,6 +22,7 @@ int moe_selftest_impl(const b200q_moe_args& a, int lost, cudaStream_t st);
 // A named barrier that tells whether all its threads say yes.  Warps that share a barrier must all come to it, also where the waits of some have run out.
 __device__ __forceinline__ bool layer_bar_and(int id, int threads, bool yes) {
   uint32_t all;
+  __syncwarp();  // (an aligned barrier wants a warp's threads together, and they may come from a loop that each left when it was done)
   asm volatile(
       "{\n"
       ".reg .pred p, q;\n"
