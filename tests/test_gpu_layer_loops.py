@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from oracle import hpu_oracle as O
-from test_gpu_layer import (BF16, E4M3, E5M2, EPS, F32, FLOOR, HALF_STEP, LIMIT, NORM, _check_lora, _check_moe, _close, _lora_case, _moe_case, _run_lora, _run_moe,  # noqa: F401
+from test_gpu_layer import (BF16, E4M3, E5M2, EPS, F32, FLOOR, HALF_STEP, LIMIT, NORM, _check_lora, _check_moe, _close, _lora_case, _lora_tol, _moe_case, _run_lora, _run_moe,  # noqa: F401
                             _status)
 
 pytestmark = pytest.mark.gpu
@@ -126,6 +126,19 @@ def _order(order, tokens, adapters):
     return which.repeat(-(-tokens // len(which)))[:tokens]
 
 
+def _check_long(got, y, x, a, b, which, scales):
+    """_check_lora with the oracle's sums adapter by adapter, which for thousands of tokens is quicker than token by token."""
+    want, size = y.double().clone(), torch.zeros(y.shape, dtype=torch.float64)
+    live = (which >= 0) & (which < a.shape[0])
+    for i in which[live].unique().tolist():
+        rows, s = (which == i).nonzero()[:, 0], float(scales[i])
+        u, v, t = a[i].double(), b[i].double(), x[rows].double()
+        want[rows] += s * (t @ u.T @ v.T)
+        size[rows] = abs(s) * (t.abs() @ u.abs().T @ v.abs().T)
+    assert torch.equal(got.cpu()[~live], y[~live])
+    _close(got.float(), want, _lora_tol(want, size, x.shape[1], a.shape[1], y.dtype))
+
+
 LARGE = [(3200, 4104, 4104, 16, 8), (8192, 2056, 1416, 64, 84), (4000, 6400, 264, 40, 3), (6001, 200, 4304, 8, 20), (2048, 264, 136, 192, 3), (3000, 72, 1032, 136, 100), (6400, 4104, 2056, 128, 5)]
 
 
@@ -134,7 +147,7 @@ LARGE = [(3200, 4104, 4104, 16, 8), (8192, 2056, 1416, 64, 84), (4000, 6400, 264
 @pytest.mark.parametrize("tokens,k,n,rank,adapters", LARGE)
 def test_lora_long_batches(tokens, k, n, rank, adapters, order, dtype):
     c = _lora_case(tokens, k, n, rank, adapters, dtype, which=_order(order, tokens, adapters))
-    _check_lora(_run_lora(*c), *c)
+    _check_long(_run_lora(*c), *c)
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
@@ -145,7 +158,7 @@ def test_lora_long_batches_between_boundaries(at, dtype):
     wide, xs = torch.zeros(4000, 264 + 13, dtype=dtype).cuda(), torch.zeros(4000, 6416, dtype=BF16).cuda()
     wide[:, at:at + 264], xs[:, 8:6408] = y.cuda(), x.cuda()
     torch.ops.b200q.lora_add_(wide[:, at:at + 264], xs[:, 8:6408], a.cuda(), b.cuda(), which.cuda(), scales.cuda())
-    _check_lora(wide[:, at:at + 264], *c)
+    _check_long(wide[:, at:at + 264], *c)
     assert bool((wide[:, :at] == 0).all()) and bool((wide[:, at + 264:] == 0).all())
 
 
